@@ -315,6 +315,92 @@ INTP_API intp_status intp_device_info(int32_t* sm_major, int32_t* sm_minor, int3
 INTP_API int32_t intp_abi_version(void);
 INTP_API const char* intp_status_string(intp_status status);
 
+/* ---- operators that read an encoder's states --------------------------------
+ * Cross attention (forward, backward, few query rows), the 8-bit state cache and
+ * attention over a prefix that a whole batch shares.
+ *
+ * A call that needs scratch memory takes it from the caller: the *_workspace
+ * functions (host only, no launch) say how many bytes.  A workspace belongs to
+ * one call in flight at a time.
+ *
+ * Shapes: q, out, grad_out, grad_q (B, H, M, D); k, v, grad_k, grad_v (B, G, N, D)
+ * with H a multiple of G (query head h reads key head h / (H / G)); D a multiple
+ * of 8 up to 128 (of 16 for the 8-bit cache).  Every tensor has unit stride along
+ * D, 16-byte aligned rows, and outer strides that are positive multiples of 16
+ * bytes (a dimension of one element may have any stride).  dtype is INTP_F16 or
+ * INTP_BF16.  lengths[b] (int32, may be null = N) is the number of states that
+ * sequence b has; it is clamped to [0, N].  States at or past it take no part
+ * whatever they hold.  A row without states gives zeros (lse -inf), and its
+ * gradients are zero.
+ */
+/* Kernel selection (xattn_args.kernel). */
+#define XATTN_KERNEL_AUTO  0  /* few rows per key head: ROWS, else TILES            */
+#define XATTN_KERNEL_ROWS  1  /* 16-row tiles over warp-private key slices          */
+#define XATTN_KERNEL_TILES 2  /* 128-row tiles on tcgen05                           */
+
+typedef struct xattn_args {
+  int64_t batch, heads, groups, queries, states, head_dim;
+  float   scale;                 /* > 0 and finite                                   */
+  int32_t dtype;                 /* of q, out and (without exponents) k, v           */
+  const void* q; int64_t q_stride[4];
+  const void* k; int64_t k_stride[4];
+  const void* v; int64_t v_stride[4];
+  /* 8-bit states: one exponent byte per (sequence, head, state), unit stride along
+   * states; k and v then hold e4m3 codes and stand for code * 2^(byte - 127).
+   * Null for 16-bit states. */
+  const uint8_t* k_exponents; const uint8_t* v_exponents; int64_t exponent_stride[2];
+  /* States that every sequence shares, (G, P, D), read before the sequence's own
+   * (xattn_shared_prefix_*; null otherwise). */
+  const void* prefix_k; int64_t prefix_k_stride[3];
+  const void* prefix_v; int64_t prefix_v_stride[3];
+  int64_t prefix;
+  const int32_t* lengths;
+  void* out; int64_t out_stride[4];
+  float* lse;                    /* (B, H, M) natural log, may be null               */
+  void* workspace; int64_t workspace_bytes;
+  int32_t* status;               /* device status word (see sla_read_status)         */
+  int32_t kernel;
+} xattn_args;
+
+typedef struct xattn_backward_args {
+  xattn_args fwd;                /* out = the forward's result, lse = its row sums   */
+  const void* grad_out; int64_t grad_out_stride[4];
+  void* grad_q;                  /* (B, H, M, D) contiguous, may be null             */
+  void* grad_k; void* grad_v;    /* (B, G, N, D) contiguous, may be null             */
+} xattn_backward_args;
+
+/* Bytes of workspace that the call with these arguments needs (pointers may be null). */
+INTP_API intp_status xattn_forward_workspace(const xattn_args* a, int64_t* bytes);
+INTP_API intp_status xattn_backward_workspace(const xattn_backward_args* a, int64_t* bytes);
+
+/* out (and lse) of softmax(scale q k^T) v over each sequence's states; with
+ * exponents over 8-bit states; with a prefix over the prefix and then its own. */
+INTP_API intp_status xattn_forward(const xattn_args* a, void* stream);
+
+/* Gradients from the forward's out and lse (16-bit states, no prefix). */
+INTP_API intp_status xattn_backward(const xattn_backward_args* a, void* stream);
+
+/* The 8-bit cache: codes (B, G, C, D) e4m3 contiguous, exponents (B, G, C)
+ * contiguous.  Each state's row stands for code * 2^(byte - 127) with the
+ * smallest power of two whose 448-fold reaches the row's largest finite value. */
+typedef struct state_cache_args {
+  int64_t batch, groups, capacity, count, head_dim;
+  int32_t dtype;                                  /* of the 16-bit states             */
+  void* k; int64_t k_stride[4];                   /* (B, G, count, D)                 */
+  void* v; int64_t v_stride[4];
+  const int32_t* start;                           /* (B) first cache row, null = 0    */
+  const int32_t* counts;                          /* (B) rows of each sequence, null = count */
+  uint8_t* k_codes; uint8_t* k_exponents;
+  uint8_t* v_codes; uint8_t* v_exponents;
+} state_cache_args;
+
+/* Row i < counts[b] of k, v goes to cache row start[b] + i; rows outside the cache
+ * are skipped, every other cache row is left as it was. */
+INTP_API intp_status state_cache_write(const state_cache_args* a, void* stream);
+/* k, v rows i < counts[b] from cache rows start[b] + i; rows past counts[b] or
+ * outside the cache read as zero. */
+INTP_API intp_status state_cache_read(const state_cache_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

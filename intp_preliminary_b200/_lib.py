@@ -42,6 +42,12 @@ EXPORTED_SYMBOLS = (
     "sla_forward_noalloc",
     "dlg_forward",
     "dlg_backward",
+    "xattn_forward_workspace",
+    "xattn_backward_workspace",
+    "xattn_forward",
+    "xattn_backward",
+    "state_cache_write",
+    "state_cache_read",
     "intp_set_wait_budget_ns",
     "intp_device_info",
     "intp_abi_version",
@@ -58,6 +64,8 @@ SHARE_VIT_SYMBOLS = (
     "svit_linear_bias",
     "svit_linear_residual_layernorm",
 )
+
+XATTN_KERNEL_AUTO, XATTN_KERNEL_ROWS, XATTN_KERNEL_TILES = 0, 1, 2
 
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -162,6 +170,53 @@ class SvitGatherPlan(ctypes.Structure):
     ]
 
 
+class XattnArgs(ctypes.Structure):
+    """Mirror of ``xattn_args`` (include/intp_b200.h)."""
+
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("groups", _i64), ("queries", _i64), ("states", _i64), ("head_dim", _i64),
+        ("scale", ctypes.c_float),
+        ("dtype", _i32),
+        ("q", _vp), ("q_stride", _Stride),
+        ("k", _vp), ("k_stride", _Stride),
+        ("v", _vp), ("v_stride", _Stride),
+        ("k_exponents", _vp), ("v_exponents", _vp), ("exponent_stride", _i64 * 2),
+        ("prefix_k", _vp), ("prefix_k_stride", _i64 * 3),
+        ("prefix_v", _vp), ("prefix_v_stride", _i64 * 3),
+        ("prefix", _i64),
+        ("lengths", _vp),
+        ("out", _vp), ("out_stride", _Stride),
+        ("lse", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+        ("status", _vp),
+        ("kernel", _i32),
+    ]
+
+
+class XattnBackwardArgs(ctypes.Structure):
+    """Mirror of ``xattn_backward_args`` (include/intp_b200.h)."""
+
+    _fields_ = [
+        ("fwd", XattnArgs),
+        ("grad_out", _vp), ("grad_out_stride", _Stride),
+        ("grad_q", _vp), ("grad_k", _vp), ("grad_v", _vp),
+    ]
+
+
+class StateCacheArgs(ctypes.Structure):
+    """Mirror of ``state_cache_args`` (include/intp_b200.h)."""
+
+    _fields_ = [
+        ("batch", _i64), ("groups", _i64), ("capacity", _i64), ("count", _i64), ("head_dim", _i64),
+        ("dtype", _i32),
+        ("k", _vp), ("k_stride", _Stride),
+        ("v", _vp), ("v_stride", _Stride),
+        ("start", _vp), ("counts", _vp),
+        ("k_codes", _vp), ("k_exponents", _vp),
+        ("v_codes", _vp), ("v_exponents", _vp),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -228,6 +283,12 @@ def load() -> ctypes.CDLL:
         lib.svit_linear_residual_layernorm.argtypes = [_vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _vp,
                                                        ctypes.c_float, _vp, _i64, _vp, _vp]
         lib.svit_linear_residual_layernorm.restype = _i32
+        for name in ("xattn_forward", "xattn_backward", "state_cache_write", "state_cache_read"):
+            getattr(lib, name).argtypes = [_vp, _vp]
+            getattr(lib, name).restype = _i32
+        for name in ("xattn_forward_workspace", "xattn_backward_workspace"):
+            getattr(lib, name).argtypes = [_vp, ctypes.POINTER(_i64)]
+            getattr(lib, name).restype = _i32
         lib.intp_abi_version.argtypes = []
         lib.intp_abi_version.restype = _i32
         lib.intp_status_string.argtypes = [_i32]

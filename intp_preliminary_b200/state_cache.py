@@ -1,0 +1,154 @@
+"""The 8-bit cache of an encoder's key / value states, and attention over it.
+
+A state's row of D values (one sequence, one key head) is held as e4m3 codes
+and one exponent byte and stands for ``code * 2^(byte - 127)``; the power of
+two is the smallest whose 448-fold (e4m3's largest value) reaches the row's
+largest finite value, no smaller than 2^-126.  So a value that is normal in
+e4m3 is off by at most 2^-4 of itself, and a row costs D + 1 bytes instead of
+2 D.  Infinities and NaN become NaN.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .cross_attention import (_base_args, _call, _check_counts, _check_query, _check_scale, _laid_out, _output, _refuse_grad,
+                              _run_forward)
+from .look_attention import _DTYPE_CODE
+
+
+class StateCache:
+    """Codes ``keys``, ``values`` ``(B, G, C, D)`` float8_e4m3fn and exponent bytes
+    ``key_exponents``, ``value_exponents`` ``(B, G, C)`` uint8, all contiguous, of
+    C states per sequence and key head; D a multiple of 16 up to 128.
+
+    The cache does not know how many of its states are filled: a program keeps
+    its sequences' lengths and passes them (``start`` of a write, ``lengths`` of
+    the attention)."""
+
+    def __init__(self, keys, key_exponents, values, value_exponents) -> None:
+        tensors = (keys, values, key_exponents, value_exponents)
+        if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in tensors):
+            raise ValueError("a state cache requires CUDA tensors")
+        if keys.ndim != 4 or keys.shape != values.shape:
+            raise ValueError("keys and values must share shape (B, G, C, D)")
+        if key_exponents.shape != keys.shape[:3] or value_exponents.shape != keys.shape[:3]:
+            raise ValueError("the exponents must have shape (B, G, C)")
+        if keys.dtype != torch.float8_e4m3fn or values.dtype != torch.float8_e4m3fn:
+            raise ValueError("keys and values must be float8_e4m3fn")
+        if key_exponents.dtype != torch.uint8 or value_exponents.dtype != torch.uint8:
+            raise ValueError("the exponents must be uint8")
+        if keys.shape[3] % 16 or not 16 <= keys.shape[3] <= 128:
+            raise ValueError("head_dim must be a multiple of 16 up to 128")
+        if not all(t.is_contiguous() for t in tensors) or keys.data_ptr() % 16 or values.data_ptr() % 16:
+            raise ValueError("the cache's tensors must be contiguous, codes 16-byte aligned")
+        if len({t.device for t in tensors}) != 1:
+            raise ValueError("all tensors must be on the same CUDA device")
+        self.keys, self.values = keys, values
+        self.key_exponents, self.value_exponents = key_exponents, value_exponents
+
+    @classmethod
+    def empty(cls, batch: int, groups: int, capacity: int, head_dim: int, *, device) -> "StateCache":
+        """A cache of zeros."""
+        shape = (batch, groups, capacity, head_dim)
+        codes = [torch.zeros(shape, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)]
+        exponents = [torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(codes[0], exponents[0], codes[1], exponents[1])
+
+    @property
+    def device(self) -> torch.device:
+        return self.keys.device
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return tuple(self.keys.shape)
+
+    def _args(self, k, v, start, counts) -> _lib.StateCacheArgs:
+        args = _lib.StateCacheArgs()
+        args.batch, args.groups, args.capacity, args.head_dim = self.keys.shape
+        args.count = k.shape[2]
+        args.dtype = _DTYPE_CODE[k.dtype]
+        args.k, args.k_stride = k.data_ptr(), k.stride()
+        args.v, args.v_stride = v.data_ptr(), v.stride()
+        if start is not None:
+            args.start = start.data_ptr()
+        if counts is not None:
+            args.counts = counts.data_ptr()
+        args.k_codes, args.k_exponents = self.keys.data_ptr(), self.key_exponents.data_ptr()
+        args.v_codes, args.v_exponents = self.values.data_ptr(), self.value_exponents.data_ptr()
+        return args
+
+    def write(self, k, v, *, start=None, counts=None) -> None:
+        """Quantise ``k``, ``v`` ``(B, G, n, D)`` (bf16 or f16) into the cache: row i of
+        sequence b goes to state ``start[b] + i`` (``start`` ``(B,)``, zero without
+        it) for ``i < counts[b]`` (all n without it).  Rows that fall outside the
+        cache are skipped; every other state is left as it was."""
+        batch, groups, _, head_dim = self.keys.shape
+        for t in (k, v):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise ValueError("a state cache requires CUDA tensors")
+            if t.ndim != 4 or t.shape != k.shape or (t.shape[0], t.shape[1], t.shape[3]) != (batch, groups, head_dim):
+                raise ValueError("k and v must share shape (B, G, n, D) with the cache's B, G and D")
+            if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != k.dtype:
+                raise ValueError("k and v must be bfloat16 or float16 and share a dtype")
+            if t.device != self.device:
+                raise ValueError("all tensors must be on the same CUDA device")
+        _refuse_grad("a state cache", k, v)
+        start = _check_counts(start, batch, self.device, "start")
+        counts = _check_counts(counts, batch, self.device, "counts")
+        k, v = _laid_out(k), _laid_out(v)
+        args = self._args(k, v, start, counts)
+        _lib.check(_call(_lib.load().state_cache_write, args, self.device), "state cache write")
+
+    def read(self, count: int | None = None, *, start=None, counts=None, dtype=torch.bfloat16):
+        """The values of ``count`` states per sequence (all C without it) from state
+        ``start[b]`` on, as ``(k, v)`` ``(B, G, count, D)``: exact, but for what lies
+        past the dtype's range (its largest value instead) or below it.  States past
+        ``counts[b]`` or outside the cache read as zero."""
+        batch, groups, capacity, head_dim = self.keys.shape
+        count = capacity if count is None else int(count)
+        if count < 0:
+            raise ValueError("count must not be negative")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("dtype must be bfloat16 or float16")
+        start = _check_counts(start, batch, self.device, "start")
+        counts = _check_counts(counts, batch, self.device, "counts")
+        k, v = (torch.empty(batch, groups, count, head_dim, dtype=dtype, device=self.device) for _ in range(2))
+        args = self._args(k, v, start, counts)
+        _lib.check(_call(_lib.load().state_cache_read, args, self.device), "state cache read")
+        return k, v
+
+    def _set_states(self, args) -> None:
+        _, args.groups, args.states, _ = self.keys.shape
+        args.k, args.k_stride = self.keys.data_ptr(), self.keys.stride()
+        args.v, args.v_stride = self.values.data_ptr(), self.values.stride()
+        args.k_exponents, args.v_exponents = self.key_exponents.data_ptr(), self.value_exponents.data_ptr()
+        strides = self.key_exponents.stride()
+        args.exponent_stride[0], args.exponent_stride[1] = strides[0], strides[1]
+
+
+def cached_cross_attention(q, cache, *, scale, lengths=None, out=None):
+    """``cross_attention`` of ``q`` ``(B, H, M, D)`` over a :class:`StateCache`, whose
+    codes are widened inside the kernel: a state is read once for every 16 rows of
+    its key head.  Made for new tokens (few rows); inference only.  ``lengths``
+    counts each sequence's filled states (the whole capacity without it)."""
+    what = "cached cross attention"
+    if not isinstance(cache, StateCache):
+        raise ValueError("cache must be a StateCache")
+    _refuse_grad(what, q)
+    _check_query(q, cache.keys.shape[1], cache.keys.shape[3], what, 16)
+    if q.device != cache.device:
+        raise ValueError("all tensors must be on the same CUDA device")
+    if q.shape[0] != cache.keys.shape[0]:
+        raise ValueError("q and the cache must share the batch size")
+    if cache.keys.shape[2] < 1:
+        raise ValueError("the cache must hold at least one state")
+    lengths = _check_counts(lengths, q.shape[0], q.device, "lengths")
+    scale = _check_scale(scale)
+    out = _output(q, out)
+    q = _laid_out(q)
+    args = _base_args(q, scale, lengths, out, None, "auto")
+    cache._set_states(args)
+    _run_forward(args, q.device, what)
+    return out

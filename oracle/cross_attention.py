@@ -1,0 +1,131 @@
+"""float64 restatement of cross attention to encoder states, its gradients, the
+8-bit state cache's rounding, and elementwise error bounds for 16-bit kernels.
+
+The bounds follow from where a kernel may round, with u the unit roundoff of a
+16-bit type (half its eps) and fp32 sums:
+  out:  each probability is rounded once (u), its exponential is within 1e-4 of
+        itself (a 7.5e-5 polynomial, fp32 scores, two of them in a split), and the
+        result is rounded once: (u_p + EXP) sum_j p_j |v_j| + u |out|.
+  P, dS of the backward: the same EXP, plus the row sum's own (it is an fp32 log
+        within 2e-4), one rounding each; delta carries the rounding of out.
+f16 operands below 2^-14 lose bits: at most 2^-25 each.
+"""
+
+from __future__ import annotations
+
+import torch
+
+EXP = 2.5e-4
+LSE = 2e-4
+
+
+def _u(dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+def _lengths(lengths, batch, n):
+    return [n] * batch if lengths is None else [min(max(int(x), 0), n) for x in lengths]
+
+
+def cross_attention(q, k, v, *, scale, lengths=None, prefix=None, out_dtype=None, p_dtype=None, key_weight=None):
+    """``(out, lse, bound)`` in float64 on the CPU; ``prefix`` = (k, v) of shape (G, P, D).
+
+    ``key_weight`` (B, G, N): the size of a unit of each value row (8-bit states), for
+    the loss of small f16 probabilities."""
+    out_dtype = out_dtype or q.dtype
+    p_dtype = p_dtype or q.dtype
+    q, k, v = (t.detach().cpu().double() for t in (q, k, v))
+    batch, heads, queries, dim = q.shape
+    groups, n = k.shape[1], k.shape[2]
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.full((batch, heads, queries), -float("inf"), dtype=torch.float64)
+    u_p, u_o = _u(p_dtype), _u(out_dtype)
+    for b, length in enumerate(_lengths(lengths, batch, n)):
+        for h in range(heads):
+            g = h // (heads // groups)
+            kk, vv = k[b, g, :length], v[b, g, :length]
+            if prefix is not None:
+                kk = torch.cat([prefix[0][g].detach().cpu().double(), kk])
+                vv = torch.cat([prefix[1][g].detach().cpu().double(), vv])
+            if kk.shape[0] == 0:
+                continue
+            s = scale * (q[b, h] @ kk.T)
+            lse[b, h] = torch.logsumexp(s, -1)
+            p = torch.exp(s - lse[b, h][:, None])
+            out[b, h] = p @ vv
+            bound[b, h] = (u_p + EXP) * (p @ vv.abs()) + u_o * out[b, h].abs()
+            if p_dtype == torch.float16:
+                if key_weight is None:
+                    # the running reference is at most 2^8 below the row's maximum
+                    bound[b, h] += 2.0 ** -25 * p.amax(-1, keepdim=True) * vv.abs().sum(0) * 2.0
+                else:
+                    w = key_weight[b, g, :length].detach().cpu().double()
+                    bound[b, h] += 2.0 ** -25 * (p * w).amax(-1, keepdim=True) * (vv.abs() / w[:, None]).sum(0) * 2.0
+            bound[b, h] += 1e-7
+    return out, lse, bound
+
+
+def cross_attention_gradients(q, k, v, grad, *, scale, lengths=None):
+    """``((dq, dk, dv), (their bounds))`` in float64 on the CPU."""
+    dtype = q.dtype
+    u = _u(dtype)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    _, _, out_bound = cross_attention(q, k, v, scale=scale, lengths=lengths)
+    q, k, v, grad = (t.detach().cpu().double() for t in (q, k, v, grad))
+    batch, heads = q.shape[:2]
+    groups, n = k.shape[1], k.shape[2]
+    d = [torch.zeros_like(t) for t in (q, k, v)]
+    e = [torch.zeros_like(t) for t in (q, k, v)]
+    rel = u + EXP + 2 * LSE
+    for b, length in enumerate(_lengths(lengths, batch, n)):
+        if length == 0:
+            continue
+        for h in range(heads):
+            g = h // (heads // groups)
+            kk, vv, go = k[b, g, :length], v[b, g, :length], grad[b, h]
+            p = torch.softmax(scale * (q[b, h] @ kk.T), -1)
+            dp = go @ vv.T
+            ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+            delta_bound = (go.abs() * out_bound[b, h]).sum(-1, keepdim=True)
+            ds_bound = rel * ds.abs() + p * (delta_bound + 1e-5 * (go.abs() @ vv.abs().T)) + tiny
+            p_bound = rel * p + tiny
+            d[0][b, h] = scale * (ds @ kk)
+            d[1][b, g, :length] += scale * (ds.T @ q[b, h])
+            d[2][b, g, :length] += p.T @ go
+            e[0][b, h] = scale * (ds_bound @ kk.abs())
+            e[1][b, g, :length] += scale * (ds_bound.T @ q[b, h].abs())
+            e[2][b, g, :length] += p_bound.T @ go.abs()
+    return tuple(d), tuple(x + u * t.abs() + 1e-7 for x, t in zip(e, d))
+
+
+def e4m3_values() -> torch.Tensor:
+    """The non-negative finite e4m3 values in order (index = code)."""
+    values = []
+    for code in range(127):
+        exponent, mantissa = code >> 3, code & 7
+        values.append((mantissa / 8) * 2.0 ** -6 if exponent == 0 else (1 + mantissa / 8) * 2.0 ** (exponent - 7))
+    return torch.tensor(values, dtype=torch.float64)
+
+
+def quantise_rows(x):
+    """``(values, exponents)``: each row of x as e4m3 codes times a power of two, in float64."""
+    x = x.detach().cpu().double()
+    finite = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x))
+    amax = finite.amax(-1)
+    exponents = torch.zeros_like(amax)
+    flat, flat_e = amax.reshape(-1), exponents.reshape(-1)
+    for i, a in enumerate(flat.tolist()):
+        if a > 0:
+            e = -126
+            while a > 448 * 2.0 ** e:
+                e += 1
+            flat_e[i] = e
+    unit = torch.exp2(exponents)[..., None]
+    table = e4m3_values()
+    y = (finite / unit).contiguous()
+    hi = torch.searchsorted(table, y).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    below, above = y - table[lo], table[hi] - y
+    code = torch.where((below < above) | ((below == above) & (lo % 2 == 0)), lo, hi)
+    values = table[code] * unit * torch.sign(x)
+    return torch.where(torch.isfinite(x), values, torch.full_like(x, float("nan"))), exponents.long()

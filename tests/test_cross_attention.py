@@ -1,0 +1,172 @@
+"""Cross attention, the state cache and shared prefixes without a GPU: the C ABI's
+structs, refusals and workspace sizes, CPU tensors, and the oracle itself."""
+
+import ctypes
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+from intp_preliminary_b200 import (StateCache, _lib, cached_cross_attention, cross_attention,
+                                   cross_attention_backward, cross_attention_forward, shared_prefix_attention)
+from oracle import cross_attention as oracle
+
+HEADER = Path(__file__).resolve().parent.parent / "include" / "intp_b200.h"
+FAKE = 1 << 20  # never dereferenced: every call below is refused before a launch
+
+
+@pytest.mark.parametrize("name,mirror", [("xattn_args", _lib.XattnArgs), ("xattn_backward_args", _lib.XattnBackwardArgs),
+                                         ("state_cache_args", _lib.StateCacheArgs)])
+def test_struct_layout_matches_header_field_order(name, mirror):
+    text = HEADER.read_text()
+    body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    assert re.findall(r"(\w+)(?:\[\d\])?\s*[;,]", body) == [f[0] for f in mirror._fields_]
+
+
+def _args(**over):
+    a = _lib.XattnArgs()
+    a.batch, a.heads, a.groups, a.queries, a.states, a.head_dim = 2, 4, 2, 3, 100, 64
+    a.scale, a.dtype = 0.125, _lib.INTP_BF16
+    a.q = a.k = a.v = a.out = a.status = FAKE
+    a.q_stride = a.out_stride = _lib._Stride(768, 192, 64, 1)
+    a.k_stride = a.v_stride = _lib._Stride(12800, 6400, 64, 1)
+    for key, value in over.items():
+        setattr(a, key, value)
+    return a
+
+
+@pytest.mark.parametrize("over,status", [
+    ({"heads": 3}, _lib.INTP_ERR_SHAPE),                       # not a multiple of the key heads
+    ({"head_dim": 60}, _lib.INTP_ERR_SHAPE),
+    ({"head_dim": 136}, _lib.INTP_ERR_SHAPE),
+    ({"batch": -1}, _lib.INTP_ERR_SHAPE),
+    ({"batch": 1 << 29, "queries": 1 << 29}, _lib.INTP_ERR_SHAPE),
+    ({"states": 0}, _lib.INTP_ERR_SHAPE),                      # nothing to attend to, and no prefix
+    ({"dtype": _lib.INTP_F32}, _lib.INTP_ERR_DTYPE),
+    ({"scale": 0.0}, _lib.INTP_ERR_ARGUMENT),
+    ({"scale": float("inf")}, _lib.INTP_ERR_ARGUMENT),
+    ({"scale": float("nan")}, _lib.INTP_ERR_ARGUMENT),
+    ({"kernel": 7}, _lib.INTP_ERR_ARGUMENT),
+    ({"q": None}, _lib.INTP_ERR_ARGUMENT),
+    ({"status": None}, _lib.INTP_ERR_ARGUMENT),
+    ({"k_exponents": FAKE}, _lib.INTP_ERR_ARGUMENT),           # one of the two
+    ({"k_exponents": FAKE, "v_exponents": FAKE, "kernel": _lib.XATTN_KERNEL_TILES}, _lib.INTP_ERR_UNSUPPORTED),
+    ({"k_exponents": FAKE, "v_exponents": FAKE, "head_dim": 40}, _lib.INTP_ERR_SHAPE),
+    ({"prefix": 5}, _lib.INTP_ERR_ARGUMENT),                   # no prefix tensors
+    ({"q": FAKE + 8}, _lib.INTP_ERR_LAYOUT),
+    ({"k_stride": _lib._Stride(12800, 6400, 68, 1)}, _lib.INTP_ERR_LAYOUT),
+    ({"v_stride": _lib._Stride(12800, 6400, 64, 2)}, _lib.INTP_ERR_LAYOUT),
+    ({"k_stride": _lib._Stride(0, 6400, 64, 1)}, _lib.INTP_ERR_LAYOUT),
+    ({"states": 100_000, "k_stride": _lib._Stride(12_800_000, 6_400_000, 64, 1),
+      "v_stride": _lib._Stride(12_800_000, 6_400_000, 64, 1)}, _lib.INTP_ERR_ARGUMENT),  # no workspace
+])
+def test_forward_refuses_before_a_launch(over, status):
+    args = _args(**over)
+    assert _lib.load().xattn_forward(ctypes.addressof(args), None) == status
+
+
+def test_backward_refuses_before_a_launch():
+    lib = _lib.load()
+    assert lib.xattn_backward(None, None) == lib.xattn_forward(None, None) == _lib.INTP_ERR_ARGUMENT
+    b = _lib.XattnBackwardArgs()
+    b.fwd = _args()
+    b.grad_q = FAKE
+    assert lib.xattn_backward(ctypes.addressof(b), None) == _lib.INTP_ERR_ARGUMENT  # no row sums
+    b.fwd.lse, b.grad_out = FAKE, FAKE
+    assert lib.xattn_backward(ctypes.addressof(b), None) == _lib.INTP_ERR_LAYOUT    # strides of grad_out
+    b.grad_out_stride = b.fwd.q_stride
+    assert lib.xattn_backward(ctypes.addressof(b), None) == _lib.INTP_ERR_ARGUMENT  # no workspace
+    b.fwd.prefix, b.fwd.prefix_k, b.fwd.prefix_v = 4, FAKE, FAKE
+    assert lib.xattn_backward(ctypes.addressof(b), None) == _lib.INTP_ERR_UNSUPPORTED
+
+
+def test_cache_refuses_before_a_launch():
+    lib = _lib.load()
+    a = _lib.StateCacheArgs()
+    a.batch, a.groups, a.capacity, a.count, a.head_dim, a.dtype = 1, 2, 16, 4, 64, _lib.INTP_F16
+    assert lib.state_cache_write(ctypes.addressof(a), None) == _lib.INTP_ERR_ARGUMENT
+    for name in ("k", "v", "k_codes", "v_codes", "k_exponents", "v_exponents"):
+        setattr(a, name, FAKE)
+    assert lib.state_cache_write(ctypes.addressof(a), None) == _lib.INTP_ERR_LAYOUT
+    a.head_dim = 40
+    assert lib.state_cache_read(ctypes.addressof(a), None) == _lib.INTP_ERR_SHAPE
+    a.head_dim, a.dtype = 64, _lib.INTP_F32
+    assert lib.state_cache_read(ctypes.addressof(a), None) == _lib.INTP_ERR_DTYPE
+    a.dtype, a.count = _lib.INTP_F16, 0
+    assert lib.state_cache_read(ctypes.addressof(a), None) == _lib.INTP_OK  # nothing to do
+    assert lib.state_cache_write(None, None) == _lib.INTP_ERR_ARGUMENT
+
+
+@pytest.mark.parametrize("batch,heads,groups,queries,states,prefix", [
+    (1, 3, 3, 1, 196, 0), (64, 32, 8, 1, 4096, 0), (1, 1, 1, 1, 1 << 20, 0), (4, 3, 3, 1, 33, 196),
+    (1, 8, 8, 2048, 512, 0), (2, 8, 2, 100, 5000, 0), (64, 32, 8, 1, 0, 16384)])
+def test_workspace_holds_every_part(batch, heads, groups, queries, states, prefix):
+    """The parts of a split pass, their row sums, and nothing for a pass in one piece."""
+    a = _args(batch=batch, heads=heads, groups=groups, queries=queries, states=states, prefix=prefix)
+    size = ctypes.c_int64(-1)
+    assert _lib.load().xattn_forward_workspace(ctypes.addressof(a), ctypes.byref(size)) == _lib.INTP_OK
+    part = batch * heads * queries * (64 + 1) * 4
+    assert size.value == 0 or size.value >= 2 * part
+    if states and prefix:
+        assert size.value >= 2 * part
+    b = _lib.XattnBackwardArgs()
+    b.fwd = a
+    assert _lib.load().xattn_backward_workspace(ctypes.addressof(b), ctypes.byref(size)) == _lib.INTP_OK
+    assert size.value >= (batch * heads * queries * 2 * 4 if states else 0)
+
+
+def test_operators_refuse_cpu_tensors():
+    q = torch.randn(1, 2, 3, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        cross_attention(q, q, q, scale=0.25)
+    with pytest.raises(ValueError, match="CUDA"):
+        cross_attention(q.requires_grad_(), q, q, scale=0.25)
+    q = q.detach()
+    with pytest.raises(ValueError, match="CUDA"):
+        cross_attention_forward(q, q, q, scale=0.25)
+    with pytest.raises(ValueError, match="CUDA"):
+        cross_attention_backward(q, q, q, q, q[..., 0].float(), q, scale=0.25)
+    with pytest.raises(ValueError, match="CUDA"):
+        shared_prefix_attention(q, q[0], q[0], q, q, scale=0.25)
+    with pytest.raises(ValueError, match="CUDA"):
+        StateCache.empty(1, 2, 8, 16, device="cpu")
+    with pytest.raises(ValueError, match="StateCache"):
+        cached_cross_attention(q, q, scale=0.25)
+
+
+def test_oracle_gradients_match_differences():
+    """The gradient formulas against central differences of the forward, in float64."""
+    g = torch.Generator().manual_seed(5)
+    q, k, v, grad = (torch.randn(s, generator=g, dtype=torch.float64).half()
+                     for s in ((2, 4, 3, 8), (2, 2, 5, 8), (2, 2, 5, 8), (2, 4, 3, 8)))
+    lengths = [5, 3]
+    grads, _ = oracle.cross_attention_gradients(q, k, v, grad, scale=0.3, lengths=lengths)
+
+    def loss(tensors):
+        out, _, _ = oracle.cross_attention(*tensors, scale=0.3, lengths=lengths, out_dtype=torch.float16,
+                                           p_dtype=torch.float16)
+        return float((out * grad.double()).sum())
+
+    step = 1e-5
+    for which in range(3):
+        base = [t.double() for t in (q, k, v)]
+        flat = grads[which].reshape(-1)
+        for i in range(0, flat.numel(), 7):
+            moved = []
+            for sign in (1, -1):
+                t = base[which].clone()
+                t.view(-1)[i] += sign * step
+                moved.append(loss([t if j == which else base[j] for j in range(3)]))
+            # central differences: O(step^2) truncation and 1e-15 / step cancellation
+            assert abs((moved[0] - moved[1]) / (2 * step) - float(flat[i])) < 1e-7
+
+
+def test_oracle_e4m3_table_matches_torch():
+    codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    assert torch.equal(codes, oracle.e4m3_values())
+    x = torch.randn(7, 33, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    values, exponents = oracle.quantise_rows(x)
+    again = (x.double() / torch.exp2(exponents.double())[:, None]).to(torch.float8_e4m3fn).double()
+    assert torch.equal(values, again * torch.exp2(exponents.double())[:, None])

@@ -1,0 +1,396 @@
+"""Cross attention on the GPU against the float64 oracle, elementwise within the
+oracle's error bounds (derived there from where the kernels round)."""
+
+import ctypes
+
+import pytest
+import torch
+
+from intp_preliminary_b200 import (_lib, check_device_status, cross_attention, cross_attention_backward,
+                                   cross_attention_forward, shared_prefix_attention)
+from oracle import cross_attention as oracle
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def _device_status(cuda_device):
+    yield
+    check_device_status(cuda_device)
+
+
+def _normal(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def _inputs(batch, heads, groups, queries, states, dim, dtype, seed=0):
+    return (_normal((batch, heads, queries, dim), dtype, seed + 1), _normal((batch, groups, states, dim), dtype, seed + 2),
+            _normal((batch, groups, states, dim), dtype, seed + 3))
+
+
+def _assert_within(got, want, bound):
+    off = (got.detach().cpu().double() - want).abs()
+    assert torch.isfinite(off).all()
+    worst = (off / bound).max()
+    assert (off <= bound).all(), f"error {float(worst):.2f} times the bound"
+
+
+def _check_forward(q, k, v, lengths, device, kernel, scale=None):
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    want, lse, bound = oracle.cross_attention(q, k, v, scale=scale, lengths=lengths)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device)
+    out, got_lse = cross_attention_forward(q.to(device), k.to(device), v.to(device), scale=scale, lengths=lens,
+                                           want_lse=True, kernel=kernel)
+    _assert_within(out, want, bound)
+    got_lse = got_lse.cpu().double()
+    empty = torch.isinf(lse)
+    assert torch.equal(torch.isinf(got_lse), empty)
+    assert (got_lse - lse)[~empty].abs().max() <= oracle.LSE if (~empty).any() else True
+
+
+SHAPES = [
+    # batch, heads, groups, queries, states, dim, lengths
+    (1, 1, 1, 1, 1, 8, None),
+    (2, 3, 3, 5, 17, 64, None),
+    (1, 4, 2, 3, 127, 40, None),
+    (2, 2, 1, 64, 128, 64, [128, 77]),
+    (3, 2, 2, 33, 129, 72, [0, 1, 129]),
+    (2, 4, 4, 130, 300, 80, [299, 128]),
+    (1, 6, 2, 100, 513, 128, [511]),
+    (2, 2, 2, 257, 64, 96, None),
+    (1, 8, 1, 70, 1000, 128, [999]),
+    (4, 3, 3, 1, 196, 64, [196, 0, 63, 64]),
+    (2, 8, 2, 1, 2500, 128, [2500, 1300]),
+    (1, 16, 2, 2, 3001, 64, None),
+]
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles", "auto"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_matches_oracle(cuda_device, shape, dtype, kernel):
+    *sizes, lengths = shape
+    q, k, v = _inputs(*sizes, dtype)
+    _check_forward(q, k, v, lengths, cuda_device, kernel)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), "lowest"])
+def test_padded_states_never_show(cuda_device, kernel, poison):
+    """Whatever sits past a length: NaN, infinities, the type's lowest value."""
+    q, k, v = _inputs(3, 4, 2, 9, 700, 64, BF16, seed=9)
+    lengths = [0, 333, 640]
+    value = torch.finfo(BF16).min if poison == "lowest" else poison
+    clean = [t.clone() for t in (k, v)]
+    for b, n in enumerate(lengths):
+        k[b, :, n:] = value
+        v[b, :, n:] = value
+        for t in clean:
+            t[b, :, n:] = 0
+    lens = torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    a, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, lengths=lens, want_lse=True,
+                                     kernel=kernel)
+    b, lse0 = cross_attention_forward(q.to(cuda_device), *(t.to(cuda_device) for t in clean), scale=0.125, lengths=lens,
+                                      want_lse=True, kernel=kernel)
+    assert torch.equal(a, b) and torch.equal(lse, lse0)
+    assert a[0].abs().max() == 0 and torch.isinf(lse[0]).all()
+    grad = torch.randn_like(a)
+    got = cross_attention_backward(*(t.to(cuda_device) for t in (q, k, v)), a, lse, grad, scale=0.125, lengths=lens)
+    ref = cross_attention_backward(q.to(cuda_device), *(t.to(cuda_device) for t in clean), a, lse, grad, scale=0.125,
+                                   lengths=lens)
+    for x, y in zip(got, ref):
+        assert torch.equal(x, y)
+    for x in got[1:]:
+        for i, n in enumerate(lengths):
+            assert x[i, :, n:].abs().sum() == 0
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+def test_lengths_outside_the_range_are_clamped(cuda_device, kernel):
+    q, k, v = (t.to(cuda_device) for t in _inputs(3, 2, 2, 4, 150, 64, BF16, seed=3))
+    wild = torch.tensor([-5, 1000, 2 ** 40], device=cuda_device)
+    got, _ = cross_attention_forward(q, k, v, scale=0.125, lengths=wild, kernel=kernel)
+    tame = torch.tensor([0, 150, 150], dtype=torch.int32, device=cuda_device)
+    assert torch.equal(got, cross_attention_forward(q, k, v, scale=0.125, lengths=tame, kernel=kernel)[0])
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+def test_values_that_are_not_finite_spread_as_in_a_softmax(cuda_device, kernel):
+    """A NaN score makes its row NaN; a key with -inf scores drops out; a row of them gives zeros."""
+    q, k, v = _inputs(1, 1, 1, 6, 300, 64, BF16, seed=4)
+    q = q.abs() + 0.1
+    k[0, 0, 290] = -float("inf")
+    got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, want_lse=True, kernel=kernel)
+    keep = [i for i in range(300) if i != 290]
+    want, _, bound = oracle.cross_attention(q, k[:, :, keep], v[:, :, keep], scale=0.125)
+    _assert_within(got, want, bound)
+    k[:] = -float("inf")
+    got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, want_lse=True, kernel=kernel)
+    assert got.abs().max() == 0 and torch.isinf(lse).all()
+    q, k, v = _inputs(1, 1, 1, 6, 300, 64, BF16, seed=4)
+    for at in (0, 150, 299):
+        for e in range(8):
+            broken = k.clone()
+            broken[0, 0, (at + e) % 300, 3] = float("nan")
+            got, _ = cross_attention_forward(*(t.to(cuda_device) for t in (q, broken, v)), scale=0.125, kernel=kernel)
+            assert torch.isnan(got).all()
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+def test_scores_of_any_size(cuda_device, kernel):
+    """Peaked rows: the running maximum moves by hundreds from tile to tile."""
+    q, k, v = _inputs(1, 2, 1, 40, 900, 64, BF16, seed=6)
+    ramp = torch.linspace(0.1, 12.0, 900)[None, None, :, None]
+    _check_forward(q, (k.float() * ramp).to(BF16), v, None, cuda_device, kernel, scale=0.5)
+    _check_forward(q, (k.float() * ramp.flip(2)).to(BF16), v, None, cuda_device, kernel, scale=0.5)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+def test_strided_inputs(cuda_device, kernel):
+    """(B, M, H, D) projections seen as (B, H, M, D), slices of a wider tensor, broadcast states, odd rows."""
+    q = _normal((2, 37, 4, 64), BF16, 1).to(cuda_device).transpose(1, 2)
+    kv = _normal((2, 210, 2, 2, 64), BF16, 2).to(cuda_device)
+    k, v = kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+    want, _ = cross_attention_forward(q.contiguous(), k.contiguous(), v.contiguous(), scale=0.125, kernel=kernel)
+    got, _ = cross_attention_forward(q, k, v, scale=0.125, kernel=kernel)
+    assert torch.equal(got, want)
+    wide = torch.empty(2, 4, 37, 72, dtype=BF16, device=cuda_device)[..., 8:]
+    got, _ = cross_attention_forward(q, k, v, scale=0.125, kernel=kernel, out=wide)
+    assert got.data_ptr() == wide.data_ptr() and torch.equal(wide, want)
+    odd = torch.empty(2, 4, 37, 67, dtype=BF16, device=cuda_device)[..., 1:65].copy_(q)  # not 16-byte aligned
+    assert torch.equal(cross_attention_forward(odd, k, v, scale=0.125, kernel=kernel)[0], want)
+    with pytest.raises(ValueError, match="16-byte"):
+        cross_attention_forward(q, k, v, scale=0.125, out=odd)
+    one = k[:1].expand(2, -1, -1, -1)
+    got, _ = cross_attention_forward(q, one, v, scale=0.125, kernel=kernel)
+    assert torch.equal(got, cross_attention_forward(q, one.contiguous(), v, scale=0.125, kernel=kernel)[0])
+
+
+GRAD_SHAPES = [
+    (1, 1, 1, 1, 16, 8, None),
+    (2, 3, 3, 65, 64, 64, None),
+    (2, 4, 2, 63, 130, 64, [129, 64]),
+    (3, 4, 1, 40, 200, 80, [0, 200, 77]),
+    (1, 2, 2, 129, 257, 128, [193]),
+    (1, 2, 1, 300, 20, 96, None),
+    (1, 1, 1, 20, 2000, 128, None),
+    (1, 2, 1, 2000, 40, 64, [33]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", GRAD_SHAPES)
+def test_gradients_match_oracle(cuda_device, shape, dtype):
+    *sizes, lengths = shape
+    q, k, v = _inputs(*sizes, dtype, seed=20)
+    grad = _normal(q.shape, dtype, 31)
+    scale = q.shape[-1] ** -0.5
+    want, bounds = oracle.cross_attention_gradients(q, k, v, grad, scale=scale, lengths=lengths)
+    leaves = [t.to(cuda_device).requires_grad_() for t in (q, k, v)]
+    lens = None if lengths is None else torch.tensor(lengths, device=cuda_device)
+    out = cross_attention(*leaves, scale=scale, lengths=lens)
+    got = torch.autograd.grad(out, leaves, grad.to(cuda_device))
+    for g, w, b, leaf in zip(got, want, bounds, leaves):
+        assert g.shape == leaf.shape and g.dtype == dtype
+        _assert_within(g, w, b)
+
+
+def test_gradients_of_broadcast_and_strided_inputs(cuda_device):
+    """Leaves that are expanded or transposed on their way in get their own shape's gradient."""
+    q = _normal((2, 30, 4, 64), BF16, 1).to(cuda_device).requires_grad_()
+    k = _normal((1, 2, 90, 64), BF16, 2).to(cuda_device).requires_grad_()
+    v = _normal((2, 2, 90, 64), BF16, 3).to(cuda_device).requires_grad_()
+    out = cross_attention(q.transpose(1, 2), k.expand(2, -1, -1, -1), v, scale=0.125)
+    grad = torch.ones(1, dtype=BF16, device=cuda_device).expand(out.shape)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), grad)
+    full = [t.detach().clone().requires_grad_() for t in (q.transpose(1, 2).contiguous(),
+                                                          k.expand(2, -1, -1, -1).contiguous(), v)]
+    ref = torch.autograd.grad(cross_attention(*full, scale=0.125), full, torch.ones_like(out))
+    assert torch.equal(dq, ref[0].transpose(1, 2)) and torch.equal(dv, ref[2])
+    assert dk.shape == k.shape and torch.equal(dk, ref[1].sum(0, keepdim=True))
+
+
+def test_only_what_needs_a_gradient(cuda_device):
+    q, k, v = (t.to(cuda_device) for t in _inputs(1, 2, 2, 20, 90, 64, BF16))
+    out, lse = cross_attention_forward(q, k, v, scale=0.125, want_lse=True)
+    grad = torch.randn_like(out)
+    full = cross_attention_backward(q, k, v, out, lse, grad, scale=0.125)
+    for i in range(3):
+        needs = [j == i for j in range(3)]
+        part = cross_attention_backward(q, k, v, out, lse, grad, scale=0.125, needs=needs)
+        assert torch.equal(part[i], full[i]) and all(part[j] is None for j in range(3) if j != i)
+    k.requires_grad_()
+    (dk,) = torch.autograd.grad(cross_attention(q, k, v, scale=0.125), k, grad)
+    assert torch.equal(dk, full[1])
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        twice = torch.autograd.grad(cross_attention(q, k, v, scale=0.125), k, grad.requires_grad_(), create_graph=True)
+        twice[0].sum().backward()
+
+
+def test_results_repeat_bit_for_bit(cuda_device):
+    q, k, v = (t.to(cuda_device).requires_grad_() for t in _inputs(2, 4, 2, 300, 1000, 128, BF16))
+    grad = torch.randn(q.shape, device=cuda_device).to(BF16)
+    first = None
+    for _ in range(5):
+        out = cross_attention(q, k, v, scale=0.1)
+        got = (out, *torch.autograd.grad(out, (q, k, v), grad))
+        token = cross_attention_forward(q.detach()[:, :, :1], k.detach(), v.detach(), scale=0.1)[0]
+        got = (*got, token)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("queries", [1, 3, 40])
+@pytest.mark.parametrize("prefix,states,lengths", [(1, 5, None), (196, 33, [33, 0, 17, 1]), (1500, 700, [700, 650, 3, 0]),
+                                                   (300, 0, None)])
+@pytest.mark.parametrize("heads,groups,dim,dtype", [(3, 3, 64, BF16), (8, 2, 128, BF16), (4, 1, 40, F16)])
+def test_shared_prefix_matches_oracle(cuda_device, heads, groups, dim, dtype, prefix, states, lengths, queries):
+    q, k, v = _inputs(4, heads, groups, queries, states, dim, dtype, seed=50)
+    pk, pv = _normal((groups, prefix, dim), dtype, 61), _normal((groups, prefix, dim), dtype, 62)
+    want, _, bound = oracle.cross_attention(q, k, v, scale=0.2, lengths=lengths, prefix=(pk, pv))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    got = shared_prefix_attention(*(t.to(cuda_device) for t in (q, pk, pv, k, v)), scale=0.2, lengths=lens)
+    _assert_within(got, want, bound)
+
+
+def test_shared_prefix_equals_cross_attention_of_the_joined_states(cuda_device):
+    q, k, v = (t.to(cuda_device) for t in _inputs(40, 8, 2, 1, 100, 64, BF16, seed=70))
+    pk, pv = (_normal((2, 400, 64), BF16, s).to(cuda_device) for s in (71, 72))
+    got = shared_prefix_attention(q, pk, pv, k, v, scale=0.125)
+    joined = [torch.cat([p.expand(40, -1, -1, -1), t], 2) for p, t in ((pk, k), (pv, v))]
+    want, _, bound = oracle.cross_attention(q, *joined, scale=0.125)
+    _assert_within(got, want, bound)
+    _assert_within(cross_attention(q, *joined, scale=0.125), want, bound)
+
+
+def test_long_states_past_32_bit_offsets(cuda_device):
+    """The last sequence's states start past 2^31 elements."""
+    batch, states, dim = 9, 2_000_000, 128
+    base = torch.zeros(batch, 1, states, dim, dtype=BF16, device=cuda_device)
+    k, v = _normal((1, 1, 333, dim), BF16, 1), _normal((1, 1, 333, dim), BF16, 2)
+    q = _normal((batch, 2, 1, dim), BF16, 3)
+    base[-1, :, -333:] = k.to(cuda_device)[0]
+    vals = torch.zeros_like(base)
+    vals[-1, :, -333:] = v.to(cuda_device)[0]
+    tail = [t[:, :, states - 333:] for t in (base, vals)]
+    want, _, bound = oracle.cross_attention(q[-1:], k, v, scale=0.1)
+    for kernel in ("rows", "tiles"):
+        got, _ = cross_attention_forward(q.to(cuda_device), *tail, scale=0.1, kernel=kernel)
+        _assert_within(got[-1:], want, bound)
+
+
+def test_captured_and_replayed(cuda_device):
+    """A training step and a token step in one graph each, replayed on new inputs."""
+    q, k, v = (t.to(cuda_device) for t in _inputs(2, 4, 2, 50, 600, 64, BF16))
+    grad = torch.randn_like(q)
+    pk, pv = k[0, :, :100].contiguous(), v[0, :, :100].contiguous()
+
+    def step():
+        out, lse = cross_attention_forward(q, k, v, scale=0.125, want_lse=True)
+        grads = cross_attention_backward(q, k, v, out, lse, grad, scale=0.125)
+        return (out, *grads)
+
+    def token():
+        return (shared_prefix_attention(q[:, :, :1], pk, pv, k, v, scale=0.125),
+                cross_attention(q[:, :, :1], k, v, scale=0.125))
+
+    step(), token()
+    torch.cuda.synchronize()
+    graphs = []
+    for fn in (step, token):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = fn()
+        graphs.append((graph, results, fn))
+    for seed in (100, 200):
+        for t, s in ((q, 1), (k, 2), (v, 3), (grad, 4)):
+            t.copy_(_normal(t.shape, BF16, seed + s))
+        for graph, results, fn in graphs:
+            graph.replay()
+            for a, b in zip(results, fn()):
+                assert torch.equal(a, b)
+
+
+def test_other_streams(cuda_device):
+    """Two streams at once, each with its own inputs and workspace."""
+    sets = [[t.to(cuda_device) for t in _inputs(1, 4, 4, 8, 5000, 64, BF16, seed=s)] for s in (1, 2)]
+    want = [cross_attention(*s, scale=0.125) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(20):
+        for i, (s, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(cross_attention(*s, scale=0.125))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
+
+
+def test_refusals(cuda_device):
+    q, k, v = (t.to(cuda_device) for t in _inputs(2, 4, 2, 3, 50, 64, BF16))
+    ok = dict(scale=0.125)
+    for args, kw, text in [
+        ((q.float(), k.float(), v.float()), ok, "bfloat16 or float16"),
+        ((q, k.half(), v), ok, "share a dtype"),
+        ((q, k, v[:, :, :49]), ok, "share shape"),
+        ((q[0], k, v), ok, "shape"),
+        ((q[..., :60], k[..., :60], v[..., :60]), ok, "multiple of 8"),
+        ((q, k[..., :32], v[..., :32]), ok, "head_dim"),
+        ((q[:, :3], k, v), ok, "multiple of the key heads"),
+        ((q[:1], k, v), ok, "batch"),
+        ((q, k[:, :, :0], v[:, :, :0]), ok, "at least one state"),
+        ((q, k, v), dict(scale=0.0), "scale"),
+        ((q, k, v), dict(scale=float("nan")), "scale"),
+        ((q, k, v.cpu()), ok, "CUDA"),
+        ((q, k, v), dict(scale=0.125, lengths=torch.ones(3, dtype=torch.int32, device=cuda_device)), "lengths"),
+        ((q, k, v), dict(scale=0.125, lengths=torch.ones(2, device=cuda_device)), "lengths"),
+        ((q, k, v), dict(scale=0.125, lengths=torch.ones(2, dtype=torch.int32)), "lengths"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            cross_attention(*args, **kw)
+    with pytest.raises(ValueError, match="kernel"):
+        cross_attention_forward(q, k, v, scale=0.125, kernel="simt")
+    with pytest.raises(ValueError, match="out must match"):
+        cross_attention_forward(q, k, v, scale=0.125, out=q[:, :, :2])
+    with pytest.raises(ValueError, match="row sums"):
+        cross_attention_backward(q, k, v, q, q[..., 0], q, scale=0.125)
+    for args, text in [((q, k[0], v[0][:, :9], k, v), "share shape"), ((q, k[0][:, :0], v[0][:, :0], k, v), "prefix"),
+                       ((q, k[0], v[0], k[:, :1], v[:, :1]), "own states"), ((q, k[0], v[0], k[:1], v[:1]), "own states")]:
+        with pytest.raises(ValueError, match=text):
+            shared_prefix_attention(*args, scale=0.125)
+    with pytest.raises(ValueError, match="no backward"):
+        shared_prefix_attention(q.requires_grad_(), k[0], v[0], k, v, scale=0.125)
+
+
+def test_empty_batches_and_queries(cuda_device):
+    k, v = (_normal((2, 2, 50, 64), BF16, s).to(cuda_device).requires_grad_() for s in (1, 2))
+    q = torch.empty(2, 4, 0, 64, dtype=BF16, device=cuda_device, requires_grad=True)
+    out = cross_attention(q, k, v, scale=0.125)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.empty_like(out))
+    assert out.shape == q.shape == dq.shape and dk.abs().sum() == 0 and dv.abs().sum() == 0
+    none = cross_attention(q.detach()[:0].new_empty(0, 4, 3, 64), k.detach()[:0], v.detach()[:0], scale=0.125)
+    assert none.shape == (0, 4, 3, 64)
+
+
+def test_wait_budget_reports_and_the_next_call_is_clean(cuda_device):
+    """Every wait of the tensor-core kernels is bounded: a 300 ns budget runs out, the
+    status word says so, and the next call with the usual budget is right."""
+    lib = _lib.load()
+    q, k, v = _inputs(4, 4, 4, 200, 700, 64, BF16, seed=80)
+    dev = [t.to(cuda_device) for t in (q, k, v)]
+    out, lse = cross_attention_forward(*dev, scale=0.125, want_lse=True, kernel="tiles")
+    calls = [lambda: cross_attention_forward(*dev, scale=0.125, kernel="tiles"),
+             lambda: cross_attention_backward(*dev, out, lse, dev[0], scale=0.125)]
+    check_device_status(cuda_device)
+    for call in calls:
+        assert lib.intp_set_wait_budget_ns(ctypes.c_uint64(300)) == _lib.INTP_OK
+        try:
+            call()
+            with pytest.raises(RuntimeError, match="device wait failed: code 0x10"):
+                check_device_status(cuda_device)
+        finally:
+            assert lib.intp_set_wait_budget_ns(ctypes.c_uint64(1_000_000_000)) == _lib.INTP_OK
+    _check_forward(q, k, v, None, cuda_device, "tiles", scale=0.125)

@@ -24,11 +24,9 @@
 // order that changes results, or a key-length workspace).
 // P and dS are rounded to 16 bits as the tensor core's operands; all sums are fp32.
 #include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"
-#include "sm100_ptx.cuh"
+#include "xattn_common.cuh"
 #include "xattn_internal.h"
 
 namespace intp {
@@ -70,7 +68,7 @@ struct alignas(8) Bars {
 struct Args {
   XaBwdParams p;
   MapOrder of0, of1, or0, or1;
-  float* stats;                            // [B * H][m_pad / 64][lse 64 | delta 64]
+  float* stats;                            // [B * H][m_pad / 64][-lse 64 | -delta 64], lse in log2 units
   int32_t m_tiles64;                       // 64-row tiles of a head's queries
   int32_t n_row_tiles, n_split, split_tiles;
   int32_t k_steps;
@@ -83,21 +81,6 @@ struct Work {
   int32_t t0, n_t;           // streamed tiles [t0, t0 + n_t)
   int32_t length, split;
 };
-
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatile int32_t* abort, int32_t* status,
-                                          int32_t code, uint64_t budget) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort, status, code, budget));
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
-}
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
 
 // ============================================================================ row statistics
 // 8 lanes per query row.  Rows past M, and rows without states, get lse = +inf: their P is zero.
@@ -134,8 +117,8 @@ xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
   for (int s = 4; s > 0; s >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, s);
   if (sub == 0 && bh < static_cast<int64_t>(p.batch) * p.heads) {
     float* dst = stats + (bh * m_tiles64 + m / kCols) * (2 * kCols) + m % kCols;
-    dst[0] = lse;
-    dst[kCols] = delta;
+    dst[0] = -lse;
+    dst[kCols] = -delta;
   }
 }
 
@@ -239,60 +222,66 @@ __device__ __forceinline__ void mma_role(const Args& a, const Work& wk, Bars* ba
   using L = Shape<DP>;
   const XaParams& p = a.p.f;
   volatile int32_t* abort_flag = &bars->abort;
+  const uint32_t leader = elect_one();
   auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
-    return mbar_wait(bar, phase & 1, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
+    return warp_wait(bar, phase, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
   };
   const uint32_t idesc_s = idesc_f16(BF16, false, kRows, kCols);
   const uint32_t idesc_acc = idesc_f16(BF16, true, kRows, a.k_steps * 16);
   const uint64_t f0 = smem_desc_sw128(smem_u32(smem + L::fixed0), 16, 1024);
   const uint64_t f1 = smem_desc_sw128(smem_u32(smem + L::fixed1), 16, 1024);
+  // Streamed operands: K-major for the scores; MN-major for the sums (depth = the tile's
+  // 64 rows, N = head_dim in 64-column blocks).
+  const uint64_t r_score = smem_desc_sw128(smem_u32(smem + L::ring), 16, 1024);
+  const uint64_t r_acc = smem_desc_sw128(smem_u32(smem + L::ring), L::kRingBlock, 1024);
   bool issued = false;
   auto acc = [&](int32_t i) -> bool {
-    const int st = i & 1, s = i % kStages;
+    const uint32_t st = i & 1, s = i % kStages;
     if (!wait(&bars->ready[st], i >> 1)) return false;
     tc_fence_after();
-    const uint32_t r0_a = smem_u32(smem + L::ring + s * 2 * L::kRing);
-    // MN-major B: depth = the tile's 64 rows, N = head_dim in 64-column blocks
-    const uint64_t r0 = smem_desc_sw128(r0_a, L::kRingBlock, 1024);
-    const uint64_t r1 = smem_desc_sw128(r0_a + L::kRing, L::kRingBlock, 1024);
+    const uint64_t r0 = r_acc + ((s * 2 * L::kRing) >> 4), r1 = r0 + (L::kRing >> 4);
     const uint32_t x = tmem + st * 128, y = x + 64;
 #pragma unroll
     for (int kk = 0; kk < kCols / 16; ++kk)
-      mma_ts(tmem + kColAcc + (KV ? DP : 0), x + kk * kW, (KV ? r1 : r0) + ((kk * 2048) >> 4), idesc_acc,
-             (i > 0 || kk > 0) ? 1u : 0u);
+      mma_ts_warp(leader, tmem + kColAcc + (KV ? DP : 0), x + kk * kW, (KV ? r1 : r0) + ((kk * 2048) >> 4), idesc_acc,
+                  (i > 0 || kk > 0) ? 1u : 0u);
     if (KV) {
 #pragma unroll
       for (int kk = 0; kk < kCols / 16; ++kk)
-        mma_ts(tmem + kColAcc, y + kk * kW, r0 + ((kk * 2048) >> 4), idesc_acc, (i > 0 || kk > 0) ? 1u : 0u);
+        mma_ts_warp(leader, tmem + kColAcc, y + kk * kW, r0 + ((kk * 2048) >> 4), idesc_acc,
+                    (i > 0 || kk > 0) ? 1u : 0u);
     }
-    mma_commit(&bars->buf_free[st]);
-    mma_commit(&bars->ring_empty[s]);
+    mma_commit_warp(leader, &bars->buf_free[st]);
+    mma_commit_warp(leader, &bars->ring_empty[s]);
     return true;
   };
   bool ok = wait(&bars->fixed_full, 0);
   for (int32_t i = 0; i < wk.n_t && ok; ++i) {
-    const int st = i & 1, s = i % kStages;
+    const uint32_t st = i & 1, s = i % kStages;
     ok = wait(&bars->ring_full[s], i / kStages);
     if (ok && !KV && wk.length - (wk.t0 + i) * kCols < kCols && wk.length < p.states) ok = wait(&bars->clean, 0);
     if (ok && i >= 2) ok = wait(&bars->buf_free[st], (i - 2) >> 1);
     if (!ok) break;
     tc_fence_after();
-    const uint32_t r0_a = smem_u32(smem + L::ring + s * 2 * L::kRing);
-    const uint64_t r0 = smem_desc_sw128(r0_a, 16, 1024), r1 = smem_desc_sw128(r0_a + L::kRing, 16, 1024);
-    for (int kk = 0; kk < a.k_steps; ++kk)
-      mma_ss(tmem + st * 128, f0 + (((kk >> 2) * L::kFixedBlock + (kk & 3) * 32) >> 4),
-             r0 + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-    for (int kk = 0; kk < a.k_steps; ++kk)
-      mma_ss(tmem + st * 128 + 64, f1 + (((kk >> 2) * L::kFixedBlock + (kk & 3) * 32) >> 4),
-             r1 + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-    mma_commit(&bars->s_full[st]);
+    const uint64_t r0 = r_score + ((s * 2 * L::kRing) >> 4), r1 = r0 + (L::kRing >> 4);
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      if (kk < a.k_steps)
+        mma_ss_warp(leader, tmem + st * 128, f0 + (((kk >> 2) * L::kFixedBlock + (kk & 3) * 32) >> 4),
+                    r0 + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      if (kk < a.k_steps)
+        mma_ss_warp(leader, tmem + st * 128 + 64, f1 + (((kk >> 2) * L::kFixedBlock + (kk & 3) * 32) >> 4),
+                    r1 + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+    mma_commit_warp(leader, &bars->s_full[st]);
     issued = true;
     if (i >= 1) ok = acc(i - 1);
   }
-  if (ok && acc(wk.n_t - 1)) mma_commit(&bars->acc_full);
+  if (ok && acc(wk.n_t - 1)) mma_commit_warp(leader, &bars->acc_full);
   if (issued) {
     volatile int32_t no_abort = 0;
-    mma_commit(&bars->drain);
+    mma_commit_warp(leader, &bars->drain);
     mbar_wait(&bars->drain, 0, &no_abort, p.status, kDevTimeoutDrain);
   }
 }
@@ -360,7 +349,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Bars* bars = reinterpret_cast<Bars*>(smem + L::bars);
   const XaParams& p = a.p.f;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // read from lane 0: the compiler then knows the roles' values to be uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
 
   Work wk;
@@ -394,24 +384,25 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
 
   if (warp == kLoadWarp) {
     load_role<DP, false>(&tm_q, &tm_do, &tm_k, &tm_v, a, wk, bars, smem, lane);
   } else if (warp == kMmaWarp) {
-    if (lane == 0) mma_role<DP, BF16, false>(a, wk, bars, smem, tmem);
-    __syncwarp();
+    mma_role<DP, BF16, false>(a, wk, bars, smem, tmem);
   } else {
     const int row = threadIdx.x & (kRows - 1), wg = threadIdx.x >> 7;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float scale_log2 = p.scale * kLog2e;
-    float lse = INFINITY, delta = 0.f;
+    float nlse = -INFINITY, ndelta = 0.f;
     if (row < own) {
       const int32_t m = wk.row0 + row;
       const float* st = a.stats + (static_cast<int64_t>(bh) * a.m_tiles64 + m / kCols) * (2 * kCols) + m % kCols;
-      lse = __ldg(st);
-      delta = __ldg(st + kCols);
+      nlse = __ldg(st);
+      ndelta = __ldg(st + kCols);
     }
+    const float2 scale2 = make_float2(scale_log2, scale_log2), nlse2 = make_float2(nlse, nlse),
+                 ndelta2 = make_float2(ndelta, ndelta);
     auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
       return warp_wait(bar, phase, abort_flag, p.status, kDevTimeoutSoftmax, p.wait_ns);
     };
@@ -429,14 +420,12 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int32_t left = wk.length - (wk.t0 + i) * kCols - wg * kW;  // of this thread's columns
 #pragma unroll
       for (int e = 0; e < kW; e += 2) {
-        float d[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float pr = fast_exp2(fmaf(__uint_as_float(xr[e + u]), scale_log2, -lse));
-          d[u] = pr * (__uint_as_float(yr[e + u]) - delta);
-          if (e + u >= left) d[u] = 0.f;
-        }
-        dw[e / 2] = pack2<BF16>(d[0], d[1]);
+        const float2 t = fma2(make_float2(__uint_as_float(xr[e]), __uint_as_float(xr[e + 1])), scale2, nlse2);
+        float2 d = add2(make_float2(__uint_as_float(yr[e]), __uint_as_float(yr[e + 1])), ndelta2);
+        d = mul2(make_float2(fast_exp2(t.x), fast_exp2(t.y)), d);
+        if (e >= left) d.x = 0.f;
+        if (e + 1 >= left) d.y = 0.f;
+        dw[e / 2] = pack2<BF16>(d.x, d.y);
       }
       tmem_st8(x, dw);
       tmem_wait_st();
@@ -470,7 +459,8 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Bars* bars = reinterpret_cast<Bars*>(smem + L::bars);
   const XaParams& p = a.p.f;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // read from lane 0: the compiler then knows the roles' values to be uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
 
   Work wk;
@@ -508,17 +498,16 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
 
   if (warp == kLoadWarp) {
     load_role<DP, true>(&tm_k, &tm_v, &tm_q, &tm_do, a, wk, bars, smem, lane);
   } else if (warp == kMmaWarp) {
-    if (lane == 0) mma_role<DP, BF16, true>(a, wk, bars, smem, tmem);
-    __syncwarp();
+    mma_role<DP, BF16, true>(a, wk, bars, smem, tmem);
   } else {
     const int row = threadIdx.x & (kRows - 1), wg = threadIdx.x >> 7;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const float scale_log2 = p.scale * kLog2e;
+    const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
     auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
       return warp_wait(bar, phase, abort_flag, p.status, kDevTimeoutSoftmax, p.wait_ns);
     };
@@ -539,17 +528,18 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
       for (int e = 0; e < kW; e += 4) {
         const float4 l = lse4[e / 4], d = delta4[e / 4];
-        const float lv[4] = {l.x, l.y, l.z, l.w}, dl[4] = {d.x, d.y, d.z, d.w};
-        float pr[4], g[4];
+        // the statistics come negated
+        const float2 nl[2] = {make_float2(l.x, l.y), make_float2(l.z, l.w)};
+        const float2 nd[2] = {make_float2(d.x, d.y), make_float2(d.z, d.w)};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          pr[u] = fast_exp2(fmaf(__uint_as_float(xr[e + u]), scale_log2, -lv[u]));
-          g[u] = pr[u] * (__uint_as_float(yr[e + u]) - dl[u]);
+        for (int u = 0; u < 2; ++u) {
+          const int c = e + 2 * u;
+          const float2 t = fma2(make_float2(__uint_as_float(xr[c]), __uint_as_float(xr[c + 1])), scale2, nl[u]);
+          const float2 pr = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+          const float2 g = mul2(pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
+          pw[c / 2] = pack2<BF16>(pr.x, pr.y);
+          dw[c / 2] = pack2<BF16>(g.x, g.y);
         }
-        pw[e / 2] = pack2<BF16>(pr[0], pr[1]);
-        pw[e / 2 + 1] = pack2<BF16>(pr[2], pr[3]);
-        dw[e / 2] = pack2<BF16>(g[0], g[1]);
-        dw[e / 2 + 1] = pack2<BF16>(g[2], g[3]);
       }
       tmem_st8(x, pw);
       tmem_st8(x + 64, dw);

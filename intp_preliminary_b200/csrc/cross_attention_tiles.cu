@@ -28,7 +28,7 @@
 #include <cuda.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"
-#include "sm100_ptx.cuh"
+#include "xattn_common.cuh"
 #include "xattn_internal.h"
 
 namespace intp {
@@ -96,12 +96,6 @@ __device__ __forceinline__ Item decode_item(const Args& a, int32_t item) {
   return it;
 }
 
-// mbar_wait of a whole warp: every lane gets the same answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int32_t* abort, int32_t* status,
-                                          int32_t code, uint64_t budget) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, code, budget));
-}
-
 // Three-input maximum that keeps NaN (a NaN score makes its row NaN).
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
@@ -119,11 +113,6 @@ __device__ __forceinline__ float row_max(const uint32_t (&s)[BN]) {
       m[i] = c + 8 + i < BN ? max3_nan(m[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]))
                             : max3_nan(m[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + i]));
   return max3_nan(max3_nan(m[0], m[1], m[2]), max3_nan(m[3], m[4], m[5]), max3_nan(m[6], m[7], m[7]));
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
 
 template <int N>
@@ -147,7 +136,8 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* ring_s = smem + L::ring;
   Bars<KS>* bars = reinterpret_cast<Bars<KS>*>(smem + L::bars);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // read from lane 0: the compiler then knows the roles' values to be uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const XaParams& p = a.p;
   volatile int32_t* abort_flag = &bars->abort;
 
@@ -174,7 +164,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
 
   if (warp >= kGroups * 4) {
   regs_dec<kOtherRegs>();
@@ -240,77 +230,82 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
   } else if (warp == kMmaWarp) {
     // -------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      const uint32_t idesc_s = idesc_f16(BF16, false, BM, BN);
-      const uint32_t idesc_o = idesc_f16(BF16, true, BM, a.k_steps * 16);
-      uint32_t n_used = 0;                    // ring tiles consumed
-      uint32_t clean_phase = 0;               // bit s: parity of stage s's next cleaned tile
-      uint32_t gen[kGroups] = {0, 0};         // key tiles started per warpgroup
-      uint32_t q_gen[kGroups] = {0, 0};
-      bool ok = true, issued = false;
-      auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
-        return mbar_wait(bar, phase & 1, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
-      };
-      // S_w = q_w k^T from ring stage s into the columns P_w(previous) leaves.
-      auto issue_s = [&](int w, uint32_t s) -> bool {
-        if (gen[w] > 0 && !wait(&bars->o_done[w], gen[w] - 1)) return false;
-        tc_fence_after();
-        const uint64_t qd = smem_desc_sw128(smem_u32(smem + w * L::kTileBytes), 16, 1024);
-        const uint64_t kd = smem_desc_sw128(smem_u32(ring_s + s * L::kTileBytes), 16, 1024);
-        for (int kk = 0; kk < a.k_steps; ++kk) {
-          const uint32_t off = ((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
-          mma_ss(tmem + w * BN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
-        }
-        mma_commit(&bars->s_full[w]);
-        ++gen[w];
-        issued = true;
-        return true;
-      };
-      for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
-        const Item it = decode_item(a, item);
-        if (it.n_tiles == 0) continue;
-        if (!wait(&bars->full[n_used % KS], n_used / KS)) break;
-        for (int w = 0; w < it.active && ok; ++w) {
-          ok = wait(&bars->q_full[w], q_gen[w]);
-          ++q_gen[w];
-          ok = ok && issue_s(w, n_used % KS);
-        }
-        if (!ok) break;
-        mma_commit(&bars->empty[n_used % KS]);
-        for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
-          const uint32_t sv = (n_used + 1) % KS, sk = (n_used + 2) % KS;
-          const bool more = j + 1 < it.n_tiles;
-          ok = wait(&bars->full[sv], (n_used + 1) / KS);
-          if (ok && it.n_keys - j * BN < BN && it.length < p.states) {
-            ok = wait(&bars->clean[sv], clean_phase >> sv);
-            clean_phase ^= 1u << sv;
-          }
-          for (int w = 0; w < it.active && ok; ++w) {
-            ok = wait(&bars->p_full[w], gen[w] - 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t vd = smem_desc_sw128(smem_u32(ring_s + sv * L::kTileBytes), kBlockBytes, 1024);
+    const uint32_t leader = elect_one();
+    const uint32_t idesc_s = idesc_f16(BF16, false, BM, BN);
+    const uint32_t idesc_o = idesc_f16(BF16, true, BM, a.k_steps * 16);
+    const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t k_desc = smem_desc_sw128(smem_u32(ring_s), 16, 1024);
+    const uint64_t v_desc = smem_desc_sw128(smem_u32(ring_s), kBlockBytes, 1024);
+    uint32_t n_used = 0;                    // ring tiles consumed
+    uint32_t clean_phase = 0;               // bit s: parity of stage s's next cleaned tile
+    uint32_t gen[kGroups] = {0, 0};         // key tiles started per warpgroup
+    uint32_t q_gen[kGroups] = {0, 0};
+    bool ok = true, issued = false;
+    auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
+      return warp_wait(bar, phase & 1, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
+    };
+    // S_w = q_w k^T from ring stage s into the columns P_w(previous) leaves.
+    auto issue_s = [&](int w, uint32_t s) -> bool {
+      if (gen[w] > 0 && !wait(&bars->o_done[w], gen[w] - 1)) return false;
+      tc_fence_after();
+      const uint64_t qd = q_desc + ((w * L::kTileBytes) >> 4), kd = k_desc + ((s * L::kTileBytes) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              mma_ts(tmem + L::kColO + w * DP, tmem + w * BN + kk * 8, vd + ((kk * 2048) >> 4), idesc_o,
-                     (j > 0 || kk > 0) ? 1u : 0u);
-            mma_commit(&bars->o_done[w]);
-            if (w == it.active - 1) mma_commit(&bars->empty[sv]);
-            if (more) {
-              ok = (w > 0 || wait(&bars->full[sk], (n_used + 2) / KS)) && issue_s(w, sk);
-              if (ok && w == it.active - 1) mma_commit(&bars->empty[sk]);
-            }
-          }
-          n_used += 2;
-        }
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
+        if (kk < a.k_steps) mma_ss_warp(leader, tmem + w * BN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
       }
-      if (issued) {
-        mma_commit(&bars->drain);
-        volatile int32_t no_abort = 0;
-        mbar_wait(&bars->drain, 0, &no_abort, p.status, kDevTimeoutDrain);
+      mma_commit_warp(leader, &bars->s_full[w]);
+      ++gen[w];
+      issued = true;
+      return true;
+    };
+    for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
+      const Item it = decode_item(a, item);
+      if (it.n_tiles == 0) continue;
+      if (!wait(&bars->full[n_used % KS], n_used / KS)) break;
+#pragma unroll
+      for (int w = 0; w < kGroups; ++w) {
+        if (w >= it.active || !ok) continue;
+        ok = wait(&bars->q_full[w], q_gen[w]);
+        ++q_gen[w];
+        ok = ok && issue_s(w, n_used % KS);
+      }
+      if (!ok) break;
+      mma_commit_warp(leader, &bars->empty[n_used % KS]);
+      for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
+        const uint32_t sv = (n_used + 1) % KS, sk = (n_used + 2) % KS;
+        const bool more = j + 1 < it.n_tiles;
+        ok = wait(&bars->full[sv], (n_used + 1) / KS);
+        if (ok && it.n_keys - j * BN < BN && it.length < p.states) {
+          ok = wait(&bars->clean[sv], clean_phase >> sv);
+          clean_phase ^= 1u << sv;
+        }
+#pragma unroll
+        for (int w = 0; w < kGroups; ++w) {
+          if (w >= it.active || !ok) continue;
+          ok = wait(&bars->p_full[w], gen[w] - 1);
+          if (!ok) continue;
+          tc_fence_after();
+          const uint64_t vd = v_desc + ((sv * L::kTileBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            mma_ts_warp(leader, tmem + L::kColO + w * DP, tmem + w * BN + kk * 8, vd + ((kk * 2048) >> 4), idesc_o,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+          mma_commit_warp(leader, &bars->o_done[w]);
+          if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sv]);
+          if (more) {
+            ok = (w > 0 || wait(&bars->full[sk], (n_used + 2) / KS)) && issue_s(w, sk);
+            if (ok && w == it.active - 1) mma_commit_warp(leader, &bars->empty[sk]);
+          }
+        }
+        n_used += 2;
       }
     }
-    __syncwarp();
+    if (issued) {
+      mma_commit_warp(leader, &bars->drain);
+      volatile int32_t no_abort = 0;
+      mbar_wait(&bars->drain, 0, &no_abort, p.status, kDevTimeoutDrain);
+    }
   }
   } else {
     // -------------------------------------------------------------- softmax warpgroups

@@ -376,7 +376,7 @@ def test_empty_batches_and_queries(cuda_device):
 
 
 def test_wait_budget_reports_and_the_next_call_is_clean(cuda_device):
-    """Every wait of the tensor-core kernels is bounded: a 300 ns budget runs out, the
+    """Every wait of the tensor-core kernels is bounded: a 1 ns budget runs out at the first wait, the
     status word says so, and the next call with the usual budget is right."""
     lib = _lib.load()
     q, k, v = _inputs(4, 4, 4, 200, 700, 64, BF16, seed=80)
@@ -386,7 +386,7 @@ def test_wait_budget_reports_and_the_next_call_is_clean(cuda_device):
              lambda: cross_attention_backward(*dev, out, lse, dev[0], scale=0.125)]
     check_device_status(cuda_device)
     for call in calls:
-        assert lib.intp_set_wait_budget_ns(ctypes.c_uint64(300)) == _lib.INTP_OK
+        assert lib.intp_set_wait_budget_ns(ctypes.c_uint64(1)) == _lib.INTP_OK
         try:
             call()
             with pytest.raises(RuntimeError, match="device wait failed: code 0x10"):

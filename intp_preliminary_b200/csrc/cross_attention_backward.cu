@@ -59,7 +59,7 @@ struct alignas(8) Bars {
   uint64_t fixed_full;
   uint64_t ring_full[kStages], ring_empty[kStages];
   uint64_t clean;                          // padded key rows of a K tile zeroed (dq)
-  uint64_t s_full[2], ready[2], buf_free[2];
+  uint64_t s_full[2], ready[2];
   uint64_t acc_full, drain;
   uint32_t tmem_base;
   int32_t abort;
@@ -133,7 +133,6 @@ __device__ __forceinline__ void init_bars(Bars* bars) {
   for (int s = 0; s < 2; ++s) {
     mbar_init(&bars->s_full[s], 1);
     mbar_init(&bars->ready[s], kRowWarps);
-    mbar_init(&bars->buf_free[s], 1);
   }
   mbar_init(&bars->acc_full, 1);
   mbar_init(&bars->drain, 1);
@@ -251,7 +250,6 @@ __device__ __forceinline__ void mma_role(const Args& a, const Work& wk, Bars* ba
         mma_ts_warp(leader, tmem + kColAcc, y + kk * kW, r0 + ((kk * 2048) >> 4), idesc_acc,
                     (i > 0 || kk > 0) ? 1u : 0u);
     }
-    mma_commit_warp(leader, &bars->buf_free[st]);
     mma_commit_warp(leader, &bars->ring_empty[s]);
     return true;
   };
@@ -260,8 +258,8 @@ __device__ __forceinline__ void mma_role(const Args& a, const Work& wk, Bars* ba
     const uint32_t st = i & 1, s = i % kStages;
     ok = wait(&bars->ring_full[s], i / kStages);
     if (ok && !KV && wk.length - (wk.t0 + i) * kCols < kCols && wk.length < p.states) ok = wait(&bars->clean, 0);
-    if (ok && i >= 2) ok = wait(&bars->buf_free[st], (i - 2) >> 1);
     if (!ok) break;
+    // Buffer st was read by tile i - 2's sums, issued before: products execute in issue order.
     tc_fence_after();
     const uint64_t r0 = r_score + ((s * 2 * L::kRing) >> 4), r1 = r0 + (L::kRing >> 4);
 #pragma unroll

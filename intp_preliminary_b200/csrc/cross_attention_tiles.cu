@@ -20,7 +20,6 @@
 //                   a padded state would reach the output through the product.
 //   warp 9          issues S = q k^T and O += P v for both warpgroups in turn,
 //                   so one's products run under the other's softmax.
-// TMEM: S0 / P0 [0, 128), S1 / P1 [128, 256), O0 and O1 of DP columns after that.
 //
 // P is rounded to 16 bits because the tensor core takes no wider operand of this
 // rate; S, the softmax statistics and O stay in fp32.  Every mbarrier wait is
@@ -52,7 +51,13 @@ struct Shape {
   static constexpr int kBlocks = DP / 64;
   static constexpr uint32_t kTileBytes = kBlocks * kBlockBytes;  // a Q, K or V tile
   static constexpr int kStages = DP == 128 ? 4 : 8;
+  // TMEM: S0, S1, then O0, O1.  At head_dim <= 64 P has columns of its own, so the next S is
+  // formed while the exponentials of this one are taken; at 128 the columns are all in use
+  // and P lies over the S it came from.
+  static constexpr bool kOwnP = DP == 64;
   static constexpr uint32_t kColO = kGroups * BN;
+  static constexpr uint32_t kColP = kOwnP ? kColO + kGroups * DP : 0;
+  static constexpr uint32_t kStrideP = kOwnP ? BN / 2 : BN;
   static constexpr uint32_t ring = kGroups * kTileBytes;
   static constexpr uint32_t bars = ring + kStages * kTileBytes;
 };
@@ -62,7 +67,8 @@ struct alignas(8) Bars {
   uint64_t full[KS], empty[KS];      // ring of K and V tiles
   uint64_t clean[KS];                // padded rows of the V tile in a stage zeroed
   uint64_t q_full[kGroups];          // query rows staged (4 warps)
-  uint64_t s_full[kGroups], p_full[kGroups], o_done[kGroups];
+  uint64_t s_full[kGroups], p_half[kGroups], p_full[kGroups], o_done[kGroups];
+  uint64_t s_free[kGroups];          // S is in registers (P in columns of its own)
   uint64_t drain;
   uint32_t tmem_base;
   int32_t abort;
@@ -124,8 +130,9 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Key pairs of each 16 whose exponentials run on the FMA pipe (the rest on the MUFU).
-constexpr int kFmaPairs = 4;
+// Of each four key pairs, those whose exponentials run on the FMA pipe (the rest on the MUFU).
+// One measured best: 239 us (none: 249, two: 242) at B4 H16 M2048 N4096 D128.
+constexpr int kFmaPairs = 1;
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -150,7 +157,9 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (int w = 0; w < kGroups; ++w) {
       mbar_init(&bars->q_full[w], 4);
       mbar_init(&bars->s_full[w], 1);
+      mbar_init(&bars->p_half[w], 4);
       mbar_init(&bars->p_full[w], 4);
+      mbar_init(&bars->s_free[w], 4);
       mbar_init(&bars->o_done[w], 1);
     }
     mbar_init(&bars->drain, 1);
@@ -244,10 +253,9 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
       return warp_wait(bar, phase & 1, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
     };
-    // S_w = q_w k^T from ring stage s into the columns P_w(previous) leaves.
-    auto issue_s = [&](int w, uint32_t s) -> bool {
-      if (gen[w] > 0 && !wait(&bars->o_done[w], gen[w] - 1)) return false;
-      tc_fence_after();
+    // S_w = q_w k^T from ring stage s into the columns of the previous P_w.  The product that
+    // reads that P was issued before by this warp, and products execute in issue order.
+    auto issue_s = [&](int w, uint32_t s) {
       const uint64_t qd = q_desc + ((w * L::kTileBytes) >> 4), kd = k_desc + ((s * L::kTileBytes) >> 4);
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
@@ -257,7 +265,6 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       mma_commit_warp(leader, &bars->s_full[w]);
       ++gen[w];
       issued = true;
-      return true;
     };
     for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
       const Item it = decode_item(a, item);
@@ -268,35 +275,52 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         if (w >= it.active || !ok) continue;
         ok = wait(&bars->q_full[w], q_gen[w]);
         ++q_gen[w];
-        ok = ok && issue_s(w, n_used % KS);
+        if (ok) issue_s(w, n_used % KS);
       }
       if (!ok) break;
       mma_commit_warp(leader, &bars->empty[n_used % KS]);
       for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
         const uint32_t sv = (n_used + 1) % KS, sk = (n_used + 2) % KS;
         const bool more = j + 1 < it.n_tiles;
-        ok = wait(&bars->full[sv], (n_used + 1) / KS);
-        if (ok && it.n_keys - j * BN < BN && it.length < p.states) {
-          ok = wait(&bars->clean[sv], clean_phase >> sv);
-          clean_phase ^= 1u << sv;
-        }
+        const uint64_t vd = v_desc + ((sv * L::kTileBytes) >> 4);
+        // S of the next tile for warpgroup w.
+        auto next_s = [&](int w) {
+          if (!more || w >= it.active || !ok) return;
+          if (w == 0) ok = wait(&bars->full[sk], (n_used + 2) / KS);
+          if (ok && L::kOwnP) ok = wait(&bars->s_free[w], gen[w] - 1);
+          if (!ok) return;
+          tc_fence_after();
+          issue_s(w, sk);
+          if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sk]);
+        };
 #pragma unroll
         for (int w = 0; w < kGroups; ++w) {
           if (w >= it.active || !ok) continue;
-          ok = wait(&bars->p_full[w], gen[w] - 1);
-          if (!ok) continue;
-          tc_fence_after();
-          const uint64_t vd = v_desc + ((sv * L::kTileBytes) >> 4);
+          if (L::kOwnP) next_s(w);
+          if (w == 0 && ok) {
+            ok = wait(&bars->full[sv], (n_used + 1) / KS);
+            if (ok && it.n_keys - j * BN < BN && it.length < p.states) {
+              ok = wait(&bars->clean[sv], clean_phase >> sv);
+              clean_phase ^= 1u << sv;
+            }
+          }
+          const uint32_t tile = gen[w] - (L::kOwnP && more ? 2 : 1);  // of this warpgroup, whose P comes next
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            mma_ts_warp(leader, tmem + L::kColO + w * DP, tmem + w * BN + kk * 8, vd + ((kk * 2048) >> 4), idesc_o,
-                        (j > 0 || kk > 0) ? 1u : 0u);
+          // Over S, P's first half is multiplied while the second half's exponentials are taken.
+          for (int half = 0; half < 2; ++half) {
+            if (ok && (half == 0 || !L::kOwnP))
+              ok = wait(half == 0 && !L::kOwnP ? &bars->p_half[w] : &bars->p_full[w], tile);
+            if (!ok) continue;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = half * (BN / 32); kk < (half + 1) * (BN / 32); ++kk)
+              mma_ts_warp(leader, tmem + L::kColO + w * DP, tmem + L::kColP + w * L::kStrideP + kk * 8,
+                          vd + ((kk * 2048) >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          }
+          if (!ok) continue;
           mma_commit_warp(leader, &bars->o_done[w]);
           if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sv]);
-          if (more) {
-            ok = (w > 0 || wait(&bars->full[sk], (n_used + 2) / KS)) && issue_s(w, sk);
-            if (ok && w == it.active - 1) mma_commit_warp(leader, &bars->empty[sk]);
-          }
+          if (!L::kOwnP) next_s(w);
         }
         n_used += 2;
       }
@@ -314,6 +338,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int row = threadIdx.x & 127;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_addr = lane_base + w * BN, o_addr = lane_base + L::kColO + w * DP;
+    const uint32_t p_addr = lane_base + L::kColP + w * L::kStrideP;
     const float scale_log2 = p.scale * kLog2e;  // > 0 (checked on the host)
     uint8_t* q_s = smem + w * L::kTileBytes;
     uint32_t gen = 0;
@@ -367,6 +392,11 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < BN / 16; ++c) reg_fence16(*reinterpret_cast<uint32_t(*)[16]>(s + 16 * c));
+        if (L::kOwnP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->s_free[w]);
+        }
         const int32_t valid = it.n_keys - j * BN;
         if (valid < BN) {
 #pragma unroll
@@ -374,12 +404,21 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (c >= valid) s[c] = 0xff800000u;  // -inf, whatever a padded state gave
         }
         const float mx = row_max(s) * scale_log2;
+        // With P apart the last O += P v need not be done when S is: P's columns and O wait for it.
+        if (L::kOwnP && j > 0) {
+          if (!wait(&bars->o_done[w], gen - 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
         if (j == 0) {
           m = mx;
         } else {
           const bool need = !(mx <= m + kRescaleThreshold);
           if (__any_sync(0xffffffffu, need)) {
-            // S of this tile is issued after the previous O += P v has completed: O is at rest.
+            // O is at rest: without columns for P, S of this tile was issued after the previous
+            // O += P v and its barrier covers both.
             const float f = need ? fast_exp2(m - mx) : 1.f;
             for (int c = 0; c < a.k_steps; ++c) {
               uint32_t r[16];
@@ -390,8 +429,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
               tmem_st16(o_addr + c * 16, r);
             }
-            sum.x *= f;
-            sum.y *= f;
+            sum = mul2(sum, make_float2(f, f));
             if (need) m = mx;
           }
         }
@@ -405,12 +443,18 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           for (int e = 0; e < 16; ++e) {
             const float2 sv = make_float2(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1]));
             const float2 x = fma2(sv, c2, nm2);
-            const float2 e2 = (e & 3) == 3 && (e >> 2) < kFmaPairs ? exp2_fma(x)
+            const float2 e2 = (e & 3) < kFmaPairs ? exp2_fma(x)
                                                                    : make_float2(fast_exp2(x.x), fast_exp2(x.y));
             sum = add2(sum, e2);
             pk[e] = pack2<BF16>(e2.x, e2.y);
           }
-          tmem_st16(s_addr + c * 16, pk);
+          tmem_st16(p_addr + c * 16, pk);
+          if (!L::kOwnP && c == BN / 64 - 1) {  // half of P: its product may start
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->p_half[w]);
+          }
         }
         tmem_wait_st();
         tc_fence_before();

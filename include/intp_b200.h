@@ -339,34 +339,35 @@ INTP_API const char* intp_status_string(intp_status status);
 #define XATTN_KERNEL_TILES 2  /* 128-row tiles on tcgen05                           */
 
 typedef struct xattn_args {
-  int64_t batch, heads, groups, queries, states, head_dim;
-  float   scale;                 /* > 0 and finite                                   */
-  int32_t dtype;                 /* of q, out and (without exponents) k, v           */
-  const void* q; int64_t q_stride[4];
-  const void* k; int64_t k_stride[4];
-  const void* v; int64_t v_stride[4];
+  const void* q; const void* k; const void* v;
   /* 8-bit states: one exponent byte per (sequence, head, state), unit stride along
    * states; k and v then hold e4m3 codes and stand for code * 2^(byte - 127).
    * Null for 16-bit states. */
-  const uint8_t* k_exponents; const uint8_t* v_exponents; int64_t exponent_stride[2];
-  /* States that every sequence shares, (G, P, D), read before the sequence's own
-   * (xattn_shared_prefix_*; null otherwise). */
-  const void* prefix_k; int64_t prefix_k_stride[3];
-  const void* prefix_v; int64_t prefix_v_stride[3];
-  int64_t prefix;
+  const uint8_t* k_exponents; const uint8_t* v_exponents;
+  /* States that every sequence shares, (G, P, D), read before the sequence's own; null without. */
+  const void* prefix_k; const void* prefix_v;
   const int32_t* lengths;
-  void* out; int64_t out_stride[4];
+  void* out;
   float* lse;                    /* (B, H, M) natural log, may be null               */
-  void* workspace; int64_t workspace_bytes;
+  void* workspace;
   int32_t* status;               /* device status word (see sla_read_status)         */
+  int64_t workspace_bytes;
+  int64_t batch, heads, groups, queries, states, head_dim, prefix;
+  int64_t q_stride[4]; int64_t k_stride[4]; int64_t v_stride[4]; int64_t out_stride[4];
+  int64_t exponent_stride[2];    /* sequence, head                                   */
+  int64_t prefix_k_stride[3]; int64_t prefix_v_stride[3];
+  float   scale;                 /* > 0 and finite                                   */
+  int32_t dtype;                 /* of q, out and (without exponents) k, v           */
+  int32_t eight_bit;             /* 1: k_exponents and v_exponents are given         */
   int32_t kernel;
 } xattn_args;
 
 typedef struct xattn_backward_args {
   xattn_args fwd;                /* out = the forward's result, lse = its row sums   */
-  const void* grad_out; int64_t grad_out_stride[4];
+  const void* grad_out;
   void* grad_q;                  /* (B, H, M, D) contiguous, may be null             */
   void* grad_k; void* grad_v;    /* (B, G, N, D) contiguous, may be null             */
+  int64_t grad_out_stride[4];
 } xattn_backward_args;
 
 /* Bytes of workspace that the call with these arguments needs (pointers may be null). */
@@ -384,14 +385,14 @@ INTP_API intp_status xattn_backward(const xattn_backward_args* a, void* stream);
  * contiguous.  Each state's row stands for code * 2^(byte - 127) with the
  * smallest power of two whose 448-fold reaches the row's largest finite value. */
 typedef struct state_cache_args {
-  int64_t batch, groups, capacity, count, head_dim;
-  int32_t dtype;                                  /* of the 16-bit states             */
-  void* k; int64_t k_stride[4];                   /* (B, G, count, D)                 */
-  void* v; int64_t v_stride[4];
+  void* k; void* v;                               /* (B, G, count, D)                 */
   const int32_t* start;                           /* (B) first cache row, null = 0    */
   const int32_t* counts;                          /* (B) rows of each sequence, null = count */
   uint8_t* k_codes; uint8_t* k_exponents;
   uint8_t* v_codes; uint8_t* v_exponents;
+  int64_t batch, groups, capacity, count, head_dim;
+  int64_t k_stride[4]; int64_t v_stride[4];
+  int32_t dtype;                                  /* of the 16-bit states             */
 } state_cache_args;
 
 /* Row i < counts[b] of k, v goes to cache row start[b] + i; rows outside the cache

@@ -174,21 +174,23 @@ class XattnArgs(ctypes.Structure):
     """Mirror of ``xattn_args`` (include/intp_b200.h)."""
 
     _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp),
+        ("k_exponents", _vp), ("v_exponents", _vp),
+        ("prefix_k", _vp), ("prefix_v", _vp),
+        ("lengths", _vp),
+        ("out", _vp),
+        ("lse", _vp),
+        ("workspace", _vp),
+        ("status", _vp),
+        ("workspace_bytes", _i64),
         ("batch", _i64), ("heads", _i64), ("groups", _i64), ("queries", _i64), ("states", _i64), ("head_dim", _i64),
+        ("prefix", _i64),
+        ("q_stride", _Stride), ("k_stride", _Stride), ("v_stride", _Stride), ("out_stride", _Stride),
+        ("exponent_stride", _i64 * 2),
+        ("prefix_k_stride", _i64 * 3), ("prefix_v_stride", _i64 * 3),
         ("scale", ctypes.c_float),
         ("dtype", _i32),
-        ("q", _vp), ("q_stride", _Stride),
-        ("k", _vp), ("k_stride", _Stride),
-        ("v", _vp), ("v_stride", _Stride),
-        ("k_exponents", _vp), ("v_exponents", _vp), ("exponent_stride", _i64 * 2),
-        ("prefix_k", _vp), ("prefix_k_stride", _i64 * 3),
-        ("prefix_v", _vp), ("prefix_v_stride", _i64 * 3),
-        ("prefix", _i64),
-        ("lengths", _vp),
-        ("out", _vp), ("out_stride", _Stride),
-        ("lse", _vp),
-        ("workspace", _vp), ("workspace_bytes", _i64),
-        ("status", _vp),
+        ("eight_bit", _i32),
         ("kernel", _i32),
     ]
 
@@ -198,8 +200,9 @@ class XattnBackwardArgs(ctypes.Structure):
 
     _fields_ = [
         ("fwd", XattnArgs),
-        ("grad_out", _vp), ("grad_out_stride", _Stride),
+        ("grad_out", _vp),
         ("grad_q", _vp), ("grad_k", _vp), ("grad_v", _vp),
+        ("grad_out_stride", _Stride),
     ]
 
 
@@ -207,13 +210,13 @@ class StateCacheArgs(ctypes.Structure):
     """Mirror of ``state_cache_args`` (include/intp_b200.h)."""
 
     _fields_ = [
-        ("batch", _i64), ("groups", _i64), ("capacity", _i64), ("count", _i64), ("head_dim", _i64),
-        ("dtype", _i32),
-        ("k", _vp), ("k_stride", _Stride),
-        ("v", _vp), ("v_stride", _Stride),
+        ("k", _vp), ("v", _vp),
         ("start", _vp), ("counts", _vp),
         ("k_codes", _vp), ("k_exponents", _vp),
         ("v_codes", _vp), ("v_exponents", _vp),
+        ("batch", _i64), ("groups", _i64), ("capacity", _i64), ("count", _i64), ("head_dim", _i64),
+        ("k_stride", _Stride), ("v_stride", _Stride),
+        ("dtype", _i32),
     ]
 
 

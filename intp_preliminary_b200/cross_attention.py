@@ -34,6 +34,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -111,8 +112,7 @@ def _check_counts(t, batch: int, device, name: str):
     return t.contiguous()
 
 
-def _check_states(q, k, v, lengths):
-    """The checks of ``cross_attention``; returns the lengths as the kernels take them."""
+def _check_states(q, k, v) -> None:
     what = "cross attention"
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
@@ -122,7 +122,6 @@ def _check_states(q, k, v, lengths):
         raise ValueError("q, k and v must share the batch size")
     if k.shape[2] < 1:
         raise ValueError("k and v must hold at least one state (use lengths for empty sequences)")
-    return _check_counts(lengths, q.shape[0], q.device, "lengths")
 
 
 def _status(device) -> torch.Tensor:
@@ -135,59 +134,90 @@ def _status(device) -> torch.Tensor:
     return word
 
 
-def _call(fn, args, device) -> int:
-    """One library call on the device's current stream."""
-    index = device.index
-    if torch.cuda.current_device() == index:
-        return fn(ctypes.addressof(args), torch.cuda.current_stream(index).cuda_stream)
-    with torch.cuda.device(index):
-        return fn(ctypes.addressof(args), torch.cuda.current_stream(index).cuda_stream)
+# What a call's sizes, strides and types decide, kept by those alone: its checks have
+# passed, the library's argument block is filled but for the pointers, its scratch size known.
+_POINTERS = struct.Struct("13Q")   # xattn_args up to workspace_bytes
+_BACKWARD_POINTERS = struct.Struct("4Q")
+_POINTER_BYTES = _POINTERS.size
+_FORWARD_BYTES = ctypes.sizeof(_lib.XattnArgs)
+_MAX_PLANS = 1024
 
 
-def _base_args(q, scale: float, lengths, out, lse, kernel: str) -> _lib.XattnArgs:
-    batch, heads, queries, head_dim = q.shape
-    args = _lib.XattnArgs()
-    args.batch, args.heads, args.queries, args.head_dim = batch, heads, queries, head_dim
-    args.scale = scale
-    args.dtype = _DTYPE_CODE[q.dtype]
-    args.q, args.q_stride = q.data_ptr(), q.stride()
-    args.out, args.out_stride = out.data_ptr(), out.stride()
-    if lengths is not None:
-        args.lengths = lengths.data_ptr()
-    if lse is not None:
-        args.lse = lse.data_ptr()
+class _Plan:
+    __slots__ = ("tail", "scratch", "status", "index", "batch", "device", "empty", "backward_tail")
+
+
+_plans: dict = {}
+
+
+def _keep(key, plan):
+    if len(_plans) >= _MAX_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _base_args(q, scale: float, out_stride, kernel: str) -> _lib.XattnArgs:
     if kernel not in _KERNELS:
         raise ValueError(f"kernel must be one of {sorted(_KERNELS)}")
+    args = _lib.XattnArgs()
+    args.batch, args.heads, args.queries, args.head_dim = q.shape
+    args.scale = scale
+    args.dtype = _DTYPE_CODE[q.dtype]
+    args.q_stride, args.out_stride = q.stride(), out_stride
     args.kernel = _KERNELS[kernel]
-    args.status = _status(q.device).data_ptr()
     return args
 
 
-def _set_states(args, k, v) -> None:
+def _set_pair(args, k, v) -> None:
     args.groups, args.states = k.shape[1], k.shape[2]
-    args.k, args.k_stride = k.data_ptr(), k.stride()
-    args.v, args.v_stride = v.data_ptr(), v.stride()
+    args.k_stride, args.v_stride = k.stride(), v.stride()
 
 
-def _workspace(fn, args, fwd_args, device, what: str):
-    """Scratch memory for one call, from the current stream's allocator."""
-    size = ctypes.c_int64()
-    _lib.check(fn(ctypes.addressof(args), ctypes.byref(size)), what)
-    if size.value == 0:
-        return None
-    space = torch.empty(size.value, dtype=torch.uint8, device=device)
-    fwd_args.workspace, fwd_args.workspace_bytes = space.data_ptr(), size.value
-    return space
-
-
-def _run_forward(args, device, what: str) -> None:
+def _finish_plan(args, q, what: str, backward=None) -> _Plan:
+    """Scratch size and argument block of a filled ``XattnArgs`` (or of a backward's around it)."""
     lib = _lib.load()
-    space = _workspace(lib.xattn_forward_workspace, args, args, device, what)
-    status = _call(lib.xattn_forward, args, device)
-    del space
+    size = ctypes.c_int64()
+    if backward is None:
+        status = lib.xattn_forward_workspace(ctypes.addressof(args), ctypes.byref(size))
+    else:
+        backward.fwd = args
+        status = lib.xattn_backward_workspace(ctypes.addressof(backward), ctypes.byref(size))
     if status == _lib.INTP_ERR_UNSUPPORTED:
         raise ValueError(f"{what}: the selected kernel does not take these inputs")
     _lib.check(status, what)
+    plan = _Plan()
+    plan.scratch = size.value
+    plan.device, plan.index, plan.batch = q.device, q.device.index, q.shape[0]
+    plan.status = _status(q.device).data_ptr()
+    plan.empty = q.numel() == 0
+    plan.tail = bytes(args)[_POINTER_BYTES:]
+    if backward is not None:
+        plan.backward_tail = bytes(backward)[_FORWARD_BYTES + _BACKWARD_POINTERS.size:]
+    return plan
+
+
+def _call(fn, block, index: int, what: str) -> None:
+    """One library call on the device's current stream."""
+    if torch.cuda.current_device() == index:
+        status = fn(block, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(block, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, what)
+
+
+def _launch(plan: _Plan, what: str, q, k, v, k_exponents, v_exponents, prefix_k, prefix_v, lengths, out, lse) -> None:
+    if plan.empty:
+        return
+    space = 0
+    if plan.scratch:
+        scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=plan.device)  # from the current stream's pool
+        space = scratch.data_ptr()
+    block = _POINTERS.pack(q, k, v, k_exponents, v_exponents, prefix_k, prefix_v, lengths, out, lse, space, plan.status,
+                           plan.scratch) + plan.tail
+    _call(_lib.load().xattn_forward, block, plan.index, what)
 
 
 def _output(q, out):
@@ -200,28 +230,79 @@ def _output(q, out):
     return out
 
 
+def _lengths_pointer(lengths, plan: _Plan, name: str):
+    """``(tensor to keep, its address)`` of a per-sequence count."""
+    if lengths is None:
+        return None, 0
+    lengths = _check_counts(lengths, plan.batch, plan.device, name)
+    return lengths, lengths.data_ptr()
+
+
+def _forward_plan(q, k, v, scale, out_stride, kernel):
+    """The plan for these tensors, or None when one has to be laid out first."""
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.device,
+           k.device, v.device, scale, out_stride, kernel)
+    plan = _plans.get(key)
+    if plan is None:
+        _check_states(q, k, v)
+        args = _base_args(q, _check_scale(scale), out_stride, kernel)
+        if not (_ready(q) and _ready(k) and _ready(v)):
+            return None
+        _set_pair(args, k, v)
+        plan = _keep(key, _finish_plan(args, q, "cross attention"))
+    return plan
+
+
 def cross_attention_forward(q, k, v, *, scale, lengths=None, want_lse: bool = False, kernel: str = "auto", out=None):
     """Forward only.  Returns ``(out, lse_or_None)``; ``lse`` ``(B, H, M)`` float32 is
     the natural log of the row sums (-inf for a row without states).
 
     ``kernel``: ``"auto"`` chooses by the number of rows that share a key head
     (``M * H / G``), ``"rows"`` and ``"tiles"`` force one of the two kernels."""
-    lengths = _check_states(q, k, v, lengths)
-    scale = _check_scale(scale)
-    out = _output(q, out)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
-    args = _base_args(q, scale, lengths, out, lse, kernel)
-    _set_states(args, k, v)
-    _run_forward(args, q.device, "cross attention")
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise ValueError("cross attention requires CUDA tensors")
+    scale = float(scale)
+    out_stride = None
+    if out is not None:
+        out_stride = _output(q, out).stride()
+    elif q.ndim == 4:
+        _, h, m, d = q.shape
+        out_stride = (h * m * d, m * d, d, 1)
+    plan = _forward_plan(q, k, v, scale, out_stride, kernel)
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if plan is None or (qp | kp | vp) & 15:
+        q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
+        plan = _forward_plan(q, k, v, scale, out_stride, kernel)
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=plan.device)
+    lse, lse_p = None, 0
+    if want_lse:
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=plan.device)
+        lse_p = lse.data_ptr()
+    _launch(plan, "cross attention", qp, kp, vp, 0, 0, 0, 0, lengths_p, out.data_ptr(), lse_p)
     return out, lse
+
+
+def _backward_plan(q, k, v, out, grad_out, scale):
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.device,
+           k.device, v.device, scale, out.stride(), grad_out.stride())
+    plan = _plans.get(key)
+    if plan is None:
+        args = _base_args(q, scale, out.stride(), "auto")
+        _set_pair(args, k, v)
+        backward = _lib.XattnBackwardArgs()
+        backward.grad_out_stride = grad_out.stride()
+        plan = _keep(key, _finish_plan(args, q, "cross attention backward", backward))
+    return plan
 
 
 def cross_attention_backward(q, k, v, out, lse, grad_out, *, scale, lengths=None, needs=(True, True, True)):
     """Gradients ``(dq, dk, dv)`` of ``cross_attention_forward`` from its ``out`` and
     ``lse``, contiguous and in the inputs' dtype; None where ``needs`` is False.
     States past a sequence's length get zeros."""
-    lengths = _check_states(q, k, v, lengths)
+    _check_states(q, k, v)
     scale = _check_scale(scale)
     for name, t in (("out", out), ("grad_out", grad_out)):
         if not isinstance(t, torch.Tensor) or t.shape != q.shape or t.device != q.device:
@@ -239,21 +320,17 @@ def cross_attention_backward(q, k, v, out, lse, grad_out, *, scale, lengths=None
     dv = make(v.shape, dtype=q.dtype, device=device) if needs[2] else None
     if empty or not any(needs):
         return dq, dk, dv
+    if grad_out.dtype != q.dtype:
+        grad_out = grad_out.to(q.dtype)
     q, k, v, out, lse = _laid_out(q), _laid_out(k), _laid_out(v), _laid_out(out), lse.contiguous()
-    grad_out = _laid_out(grad_out.to(q.dtype))
-    args = _lib.XattnBackwardArgs()
-    args.fwd = _base_args(q, scale, lengths, out, lse, "auto")
-    _set_states(args.fwd, k, v)
-    args.grad_out, args.grad_out_stride = grad_out.data_ptr(), grad_out.stride()
-    for name, t in (("grad_q", dq), ("grad_k", dk), ("grad_v", dv)):
-        if t is not None:
-            setattr(args, name, t.data_ptr())
-    lib = _lib.load()
-    what = "cross attention backward"
-    space = _workspace(lib.xattn_backward_workspace, args, args.fwd, device, what)
-    status = _call(lib.xattn_backward, args, device)
-    del space
-    _lib.check(status, what)
+    grad_out = _laid_out(grad_out)
+    plan = _backward_plan(q, k, v, out, grad_out, scale)
+    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=device)
+    block = _POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, lengths_p, out.data_ptr(),
+                           lse.data_ptr(), scratch.data_ptr(), plan.status, plan.scratch) + plan.tail
+    block += _BACKWARD_POINTERS.pack(grad_out.data_ptr(), *(0 if t is None else t.data_ptr() for t in (dq, dk, dv)))
+    _call(_lib.load().xattn_backward, block + plan.backward_tail, plan.index, "cross attention backward")
     return dq, dk, dv
 
 
@@ -288,6 +365,45 @@ def _refuse_grad(what: str, *tensors) -> None:
         raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
+def _prefix_plan(q, prefix_k, prefix_v, k, v, cache, scale, out_stride):
+    """The plan of a shared-prefix call, or None when a tensor has to be laid out first."""
+    own = cache.layout if cache is not None else (k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype, k.device,
+                                                  v.device)
+    key = (q.shape, q.stride(), q.dtype, q.device, prefix_k.shape, prefix_k.stride(), prefix_v.shape,
+           prefix_v.stride(), prefix_k.dtype, prefix_v.dtype, prefix_k.device, prefix_v.device, own, scale, out_stride)
+    plan = _plans.get(key)
+    if plan is not None:
+        return plan
+    what = "shared-prefix attention"
+    if not q.is_cuda:
+        raise ValueError(f"{what} requires CUDA tensors")
+    _check_pair(q, prefix_k, prefix_v, "(G, P, D)", what)
+    groups, prefix, head_dim = prefix_k.shape
+    if prefix < 1:
+        raise ValueError("the prefix must hold at least one state")
+    scale = _check_scale(scale)
+    _check_query(q, groups, head_dim, what, 8 if cache is None else 16)
+    if cache is not None:
+        own_shape = cache.keys.shape
+        if cache.device != q.device:
+            raise ValueError("all tensors must be on the same CUDA device")
+    else:
+        _check_pair(q, k, v, "(B, G, N, D)", what)
+        own_shape = k.shape
+    if own_shape[0] != q.shape[0] or own_shape[1] != groups or own_shape[3] != head_dim:
+        raise ValueError("the sequences' own states must have shape (B, G, N, D) like q and the prefix")
+    if not all(_ready(t) for t in (q, prefix_k, prefix_v) + (() if cache is not None else (k, v))):
+        return None
+    args = _base_args(q, scale, out_stride, "auto")
+    if cache is not None:
+        cache._set_states(args)
+    else:
+        _set_pair(args, k, v)
+    args.prefix = prefix
+    args.prefix_k_stride, args.prefix_v_stride = prefix_k.stride(), prefix_v.stride()
+    return _keep(key, _finish_plan(args, q, what))
+
+
 def shared_prefix_attention(q, prefix_k, prefix_v, k, v=None, *, scale, lengths=None, out=None):
     """Attention of every sequence's ``q`` ``(B, H, M, D)`` to the prefix ``prefix_k``,
     ``prefix_v`` ``(G, P, D)`` and then to its own states: ``k``, ``v`` ``(B, G, N, D)``
@@ -296,38 +412,33 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k, v=None, *, scale, lengths=
     from .state_cache import StateCache
 
     what = "shared-prefix attention"
-    _refuse_grad(what, q, prefix_k, prefix_v, k, v)
-    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+    cache = k if isinstance(k, StateCache) else None
+    if cache is not None and v is not None:
+        raise ValueError("a StateCache holds both keys and values: leave v out")
+    if not all(isinstance(t, torch.Tensor) for t in (q, prefix_k, prefix_v) + (() if cache is not None else (k, v))):
         raise ValueError(f"{what} requires CUDA tensors")
-    _check_pair(q, prefix_k, prefix_v, "(G, P, D)", what)
-    groups, prefix, head_dim = prefix_k.shape
-    if prefix < 1:
-        raise ValueError("the prefix must hold at least one state")
-    scale = _check_scale(scale)
-    cached = isinstance(k, StateCache)
-    _check_query(q, groups, head_dim, what, 16 if cached else 8)
-    if cached:
-        if v is not None:
-            raise ValueError("a StateCache holds both keys and values: leave v out")
-        own_shape = k.keys.shape
-        if k.device != q.device:
-            raise ValueError("all tensors must be on the same CUDA device")
-    else:
-        _check_pair(q, k, v, "(B, G, N, D)", what)
-        own_shape = k.shape
-    if own_shape[0] != q.shape[0] or own_shape[1] != groups or own_shape[3] != head_dim:
-        raise ValueError("the sequences' own states must have shape (B, G, N, D) like q and the prefix")
-    lengths = _check_counts(lengths, q.shape[0], q.device, "lengths")
-    out = _output(q, out)
-    q, prefix_k, prefix_v = _laid_out(q), _laid_out(prefix_k), _laid_out(prefix_v)
-    args = _base_args(q, scale, lengths, out, None, "auto")
-    if cached:
-        k._set_states(args)
-    else:
-        k, v = _laid_out(k), _laid_out(v)
-        _set_states(args, k, v)
-    args.prefix = prefix
-    args.prefix_k, args.prefix_k_stride = prefix_k.data_ptr(), prefix_k.stride()
-    args.prefix_v, args.prefix_v_stride = prefix_v.data_ptr(), prefix_v.stride()
-    _run_forward(args, q.device, what)
+    _refuse_grad(what, q, prefix_k, prefix_v, k, v)
+    scale = float(scale)
+    out_stride = None
+    if out is not None:
+        out_stride = _output(q, out).stride()
+    elif q.ndim == 4:
+        _, h, m, d = q.shape
+        out_stride = (h * m * d, m * d, d, 1)
+    plan = _prefix_plan(q, prefix_k, prefix_v, k, v, cache, scale, out_stride)
+    own = (cache.keys, cache.values) if cache is not None else (k, v)
+    if plan is None or (q.data_ptr() | prefix_k.data_ptr() | prefix_v.data_ptr() | own[0].data_ptr()
+                        | own[1].data_ptr()) & 15:
+        q, prefix_k, prefix_v = _laid_out(q), _laid_out(prefix_k), _laid_out(prefix_v)
+        if cache is None:
+            k, v = own = _laid_out(k), _laid_out(v)
+        plan = _prefix_plan(q, prefix_k, prefix_v, k, v, cache, scale, out_stride)
+    exponents = (0, 0)
+    if cache is not None and cache.keys.shape[2] > 0:
+        exponents = (cache.key_exponents.data_ptr(), cache.value_exponents.data_ptr())
+    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=plan.device)
+    _launch(plan, what, q.data_ptr(), own[0].data_ptr(), own[1].data_ptr(), *exponents, prefix_k.data_ptr(),
+            prefix_v.data_ptr(), lengths_p, out.data_ptr(), 0)
     return out

@@ -630,7 +630,8 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream) {
     const int64_t grid = static_cast<int64_t>(p.batch) * p.heads * a.n_row_tiles * a.n_split;
     if (grid > INT32_MAX) return 8;
     auto kernel = xattn_dq_kernel<DP, BF16>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 6;
+    static std::atomic<uint64_t> done{0};
+    if (!allow_smem(kernel, smem, done)) return 6;
     kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(f0, f1, r0, r1, a);
     if (cudaGetLastError() != cudaSuccess) return 6;
     if (bp.dq_part != nullptr) {
@@ -648,7 +649,8 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream) {
     const int64_t grid = static_cast<int64_t>(p.batch) * p.groups * a.n_row_tiles * a.n_split;
     if (grid > INT32_MAX) return 8;
     auto kernel = xattn_dkv_kernel<DP, BF16>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 6;
+    static std::atomic<uint64_t> done{0};
+    if (!allow_smem(kernel, smem, done)) return 6;
     kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(f0, f1, r0, r1, a);
     if (cudaGetLastError() != cudaSuccess) return 6;
     const int64_t n = static_cast<int64_t>(p.batch) * p.groups * p.states * p.head_dim;

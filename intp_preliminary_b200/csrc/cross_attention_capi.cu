@@ -4,6 +4,7 @@
 // device memory.
 #include <cuda_runtime.h>
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -40,13 +41,13 @@ intp_status check_shape(const xattn_args* a) {
   for (int64_t n : {a->batch, a->heads, a->groups, a->queries, a->states, a->prefix})
     if (n < 0 || n > (int64_t(1) << 30)) return INTP_ERR_SHAPE;
   if (a->heads < 1 || a->groups < 1 || a->heads % a->groups) return INTP_ERR_SHAPE;
-  const int64_t unit = a->k_exponents ? 16 : 8;
+  const int64_t unit = a->eight_bit ? 16 : 8;
   if (a->head_dim < unit || a->head_dim > 128 || a->head_dim % unit) return INTP_ERR_SHAPE;
   if (a->dtype != INTP_F16 && a->dtype != INTP_BF16) return INTP_ERR_DTYPE;
   if (!std::isfinite(a->scale) || !(a->scale > 0.f)) return INTP_ERR_ARGUMENT;
   if (a->kernel < XATTN_KERNEL_AUTO || a->kernel > XATTN_KERNEL_TILES) return INTP_ERR_ARGUMENT;
-  if ((a->k_exponents == nullptr) != (a->v_exponents == nullptr)) return INTP_ERR_ARGUMENT;
-  if (a->k_exponents && a->kernel == XATTN_KERNEL_TILES) return INTP_ERR_UNSUPPORTED;
+  if (a->eight_bit != 0 && a->eight_bit != 1) return INTP_ERR_ARGUMENT;
+  if (a->eight_bit && a->kernel == XATTN_KERNEL_TILES) return INTP_ERR_UNSUPPORTED;
   // rows of an instance, instances and their tiles are 32-bit numbers in the kernels
   if (a->batch * a->heads > kMaxInt / std::max<int64_t>(a->queries, 1)) return INTP_ERR_SHAPE;
   return INTP_OK;
@@ -64,7 +65,7 @@ constexpr int64_t kRowsMax = 32;
 
 Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t states) {
   Pass s;
-  s.tiles = a->kernel == XATTN_KERNEL_TILES || (a->kernel == XATTN_KERNEL_AUTO && !a->k_exponents && rows > kRowsMax);
+  s.tiles = a->kernel == XATTN_KERNEL_TILES || (a->kernel == XATTN_KERNEL_AUTO && !a->eight_bit && rows > kRowsMax);
   if (s.tiles) {
     // One CTA per SM: the key axis is split until every SM has work, two tiles a part at least.
     const int64_t items = instances * ceil_div(rows, intp::kXaTileRows), tiles = ceil_div(states, intp::kXaTileKeys);
@@ -75,7 +76,7 @@ Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t sta
     // second kernel that joins parts costs more than it gains.
     const int64_t items = instances * ceil_div(rows, intp::kXaRowsTile);
     int64_t split = states <= 512 ? 1 : std::min(ceil_div(kPlanSms * 8, items), ceil_div(states, 256));
-    if (a->k_exponents) split = std::max(split, ceil_div(states, 2048));  // exponents of a part sit in shared memory
+    if (a->eight_bit) split = std::max(split, ceil_div(states, intp::kXaRowsKeys8));
     s.split_keys = ceil_div(ceil_div(states, split), 64) * 64;
   }
   s.n_split = ceil_div(states, s.split_keys);
@@ -113,21 +114,32 @@ Plan plan_forward(const xattn_args* a) {
 struct DeviceFacts {
   int sms;
 };
+// The current device's, asked for once.
 intp_status device_facts(DeviceFacts* f) {
+  static std::atomic<int> known[64];   // 0: not asked; else SMs + 1, negative if not sm_100
   int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&f->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return INTP_ERR_LAUNCH;
-  return major == 10 ? INTP_OK : INTP_ERR_ARCH;
+  if (cudaGetDevice(&dev) != cudaSuccess) return INTP_ERR_LAUNCH;
+  int v = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&f->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return INTP_ERR_LAUNCH;
+    v = major == 10 ? f->sms + 1 : -1;
+    if (dev < 64) known[dev].store(v, std::memory_order_relaxed);
+  }
+  f->sms = v - 1;
+  return v > 0 ? INTP_OK : INTP_ERR_ARCH;
 }
 
 // Checks pointers and layouts and fills the parameters that every pass shares.
 intp_status to_params(const xattn_args* a, XaParams* p) {
-  const int64_t elem = a->k_exponents ? 1 : 2;
+  const int64_t elem = a->eight_bit ? 1 : 2;
   const int64_t eq[3] = {a->batch, a->heads, a->queries}, ek[3] = {a->batch, a->groups, a->states};
   const int64_t ep[2] = {a->groups, a->prefix};
   if (!a->q || !a->out || !a->status) return INTP_ERR_ARGUMENT;
+  if ((a->k_exponents != nullptr) != (a->eight_bit == 1 && a->states > 0) ||
+      (a->v_exponents != nullptr) != (a->eight_bit == 1 && a->states > 0))
+    return INTP_ERR_ARGUMENT;
   if (!layout_ok(a->q, a->q_stride, eq, 3, 2) || !layout_ok(a->out, a->out_stride, eq, 3, 2)) return INTP_ERR_LAYOUT;
   if (a->states > 0) {
     if (!a->k || !a->v) return INTP_ERR_ARGUMENT;
@@ -289,7 +301,7 @@ intp_status xattn_backward(const xattn_backward_args* b, void* stream) {
   const xattn_args* a = &b->fwd;
   intp_status st = check_shape(a);
   if (st != INTP_OK) return st;
-  if (a->k_exponents || a->prefix > 0) return INTP_ERR_UNSUPPORTED;
+  if (a->eight_bit || a->prefix > 0) return INTP_ERR_UNSUPPORTED;
   if (a->batch == 0 || a->queries == 0) return INTP_OK;
   if (a->states == 0) return INTP_ERR_SHAPE;
   if (!b->grad_q && !b->grad_k && !b->grad_v) return INTP_OK;

@@ -462,8 +462,10 @@ int32_t launch(const RowsArgs& a, int64_t grid, cudaStream_t stream) {
   using L = RowsShape<DP, FP8>;
   auto kernel = xattn_rows_kernel<DP, BF16, FP8>;
   const int smem = L::kData + (FP8 ? 2 * a.p.split_keys : 0);
-  if (smem > 200 * 1024) return 8;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 6;
+  constexpr int most = L::kData + (FP8 ? 2 * kXaRowsKeys8 : 0);
+  static std::atomic<uint64_t> done{0};
+  if (smem > most) return 8;
+  if (!allow_smem(kernel, most, done)) return 6;
   kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 6;
 }

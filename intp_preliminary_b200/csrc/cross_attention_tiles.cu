@@ -542,7 +542,8 @@ int32_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int6
   auto kernel = xattn_tiles_kernel<DP, BF16>;
   constexpr int smem = Shape<DP>::bars + sizeof(Bars<Shape<DP>::kStages>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 6;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem(kernel, smem, done)) return 6;
   kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(mk, mv, a);
   return cudaGetLastError() == cudaSuccess ? 0 : 6;
 }

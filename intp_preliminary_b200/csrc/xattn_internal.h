@@ -1,6 +1,7 @@
 // xattn_internal.h - kernel-side parameters shared by the cross-attention
 // kernels and their C-ABI dispatcher (cross_attention_capi.cu).
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 #include "sla_internal.h"
@@ -47,9 +48,22 @@ struct XaBwdParams {
   float* dk_part; float* dv_part; int32_t kv_split, kv_split_tiles;
 };
 
+// Raises a kernel's dynamic shared memory limit, once per device (`done` is the kernel's own).
+template <class K>
+inline bool allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
 constexpr int kXaTileRows = 256;   // rows of a tcgen05 work item (two warpgroups of 128)
 constexpr int kXaTileKeys = 128;
 constexpr int kXaRowsTile = 16;    // rows of a few-rows work item
+constexpr int kXaRowsKeys8 = 2048; // keys of an 8-bit part at most: their exponents sit in shared memory
 
 int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count);
 int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream);

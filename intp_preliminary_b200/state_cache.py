@@ -10,12 +10,37 @@ e4m3 is off by at most 2^-4 of itself, and a row costs D + 1 bytes instead of
 
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
-from .cross_attention import (_base_args, _call, _check_counts, _check_query, _check_scale, _laid_out, _output, _refuse_grad,
-                              _run_forward)
+from .cross_attention import (_base_args, _call, _check_counts, _check_query, _check_scale, _finish_plan, _keep,
+                              _laid_out, _launch, _lengths_pointer, _output, _plans, _ready, _refuse_grad)
 from .look_attention import _DTYPE_CODE
+
+_POINTERS = struct.Struct("8Q")  # state_cache_args up to the sizes
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _check_tensors(keys, key_exponents, values, value_exponents) -> None:
+    tensors = (keys, values, key_exponents, value_exponents)
+    if not all(t.is_cuda for t in tensors):
+        raise ValueError("a state cache requires CUDA tensors")
+    if keys.ndim != 4 or keys.shape != values.shape:
+        raise ValueError("keys and values must share shape (B, G, C, D)")
+    if key_exponents.shape != keys.shape[:3] or value_exponents.shape != keys.shape[:3]:
+        raise ValueError("the exponents must have shape (B, G, C)")
+    if keys.dtype != torch.float8_e4m3fn or values.dtype != torch.float8_e4m3fn:
+        raise ValueError("keys and values must be float8_e4m3fn")
+    if key_exponents.dtype != torch.uint8 or value_exponents.dtype != torch.uint8:
+        raise ValueError("the exponents must be uint8")
+    if keys.shape[3] % 16 or not 16 <= keys.shape[3] <= 128:
+        raise ValueError("head_dim must be a multiple of 16 up to 128")
+    if not all(t.is_contiguous() for t in tensors):
+        raise ValueError("the cache's tensors must be contiguous, codes 16-byte aligned")
+    if len({t.device for t in tensors}) != 1:
+        raise ValueError("all tensors must be on the same CUDA device")
 
 
 class StateCache:
@@ -28,23 +53,15 @@ class StateCache:
     the attention)."""
 
     def __init__(self, keys, key_exponents, values, value_exponents) -> None:
-        tensors = (keys, values, key_exponents, value_exponents)
-        if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in tensors):
+        tensors = (keys, key_exponents, values, value_exponents)
+        if not all(isinstance(t, torch.Tensor) for t in tensors):
             raise ValueError("a state cache requires CUDA tensors")
-        if keys.ndim != 4 or keys.shape != values.shape:
-            raise ValueError("keys and values must share shape (B, G, C, D)")
-        if key_exponents.shape != keys.shape[:3] or value_exponents.shape != keys.shape[:3]:
-            raise ValueError("the exponents must have shape (B, G, C)")
-        if keys.dtype != torch.float8_e4m3fn or values.dtype != torch.float8_e4m3fn:
-            raise ValueError("keys and values must be float8_e4m3fn")
-        if key_exponents.dtype != torch.uint8 or value_exponents.dtype != torch.uint8:
-            raise ValueError("the exponents must be uint8")
-        if keys.shape[3] % 16 or not 16 <= keys.shape[3] <= 128:
-            raise ValueError("head_dim must be a multiple of 16 up to 128")
-        if not all(t.is_contiguous() for t in tensors) or keys.data_ptr() % 16 or values.data_ptr() % 16:
+        self.layout = ("state cache",) + tuple((t.shape, t.stride(), t.dtype, t.device) for t in tensors)
+        if self.layout not in _plans:
+            _check_tensors(*tensors)
+            _keep(self.layout, None)
+        if (keys.data_ptr() | values.data_ptr()) & 15:
             raise ValueError("the cache's tensors must be contiguous, codes 16-byte aligned")
-        if len({t.device for t in tensors}) != 1:
-            raise ValueError("all tensors must be on the same CUDA device")
         self.keys, self.values = keys, values
         self.key_exponents, self.value_exponents = key_exponents, value_exponents
 
@@ -64,20 +81,27 @@ class StateCache:
     def shape(self) -> tuple[int, ...]:
         return tuple(self.keys.shape)
 
-    def _args(self, k, v, start, counts) -> _lib.StateCacheArgs:
-        args = _lib.StateCacheArgs()
-        args.batch, args.groups, args.capacity, args.head_dim = self.keys.shape
-        args.count = k.shape[2]
-        args.dtype = _DTYPE_CODE[k.dtype]
-        args.k, args.k_stride = k.data_ptr(), k.stride()
-        args.v, args.v_stride = v.data_ptr(), v.stride()
-        if start is not None:
-            args.start = start.data_ptr()
-        if counts is not None:
-            args.counts = counts.data_ptr()
-        args.k_codes, args.k_exponents = self.keys.data_ptr(), self.key_exponents.data_ptr()
-        args.v_codes, args.v_exponents = self.values.data_ptr(), self.value_exponents.data_ptr()
-        return args
+    def _tail(self, k, v) -> bytes:
+        """The argument block of a copy between ``k``, ``v`` and this cache, behind its pointers."""
+        key = (self.layout, k.shape, k.stride(), v.stride(), k.dtype)
+        tail = _plans.get(key)
+        if tail is None:
+            args = _lib.StateCacheArgs()
+            args.batch, args.groups, args.capacity, args.head_dim = self.keys.shape
+            args.count = k.shape[2]
+            args.dtype = _DTYPE_CODE[k.dtype]
+            args.k_stride, args.v_stride = k.stride(), v.stride()
+            tail = _keep(key, bytes(args)[_POINTERS.size:])
+        return tail
+
+    def _copy(self, fn, k, v, start, counts, what: str) -> None:
+        batch, device = self.keys.shape[0], self.keys.device
+        start = _check_counts(start, batch, device, "start")
+        counts = _check_counts(counts, batch, device, "counts")
+        block = _POINTERS.pack(k.data_ptr(), v.data_ptr(), 0 if start is None else start.data_ptr(),
+                               0 if counts is None else counts.data_ptr(), self.keys.data_ptr(),
+                               self.key_exponents.data_ptr(), self.values.data_ptr(), self.value_exponents.data_ptr())
+        _call(fn, block + self._tail(k, v), device.index, what)
 
     def write(self, k, v, *, start=None, counts=None) -> None:
         """Quantise ``k``, ``v`` ``(B, G, n, D)`` (bf16 or f16) into the cache: row i of
@@ -90,16 +114,12 @@ class StateCache:
                 raise ValueError("a state cache requires CUDA tensors")
             if t.ndim != 4 or t.shape != k.shape or (t.shape[0], t.shape[1], t.shape[3]) != (batch, groups, head_dim):
                 raise ValueError("k and v must share shape (B, G, n, D) with the cache's B, G and D")
-            if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != k.dtype:
+            if t.dtype not in _HALF or t.dtype != k.dtype:
                 raise ValueError("k and v must be bfloat16 or float16 and share a dtype")
-            if t.device != self.device:
+            if t.device != self.keys.device:
                 raise ValueError("all tensors must be on the same CUDA device")
         _refuse_grad("a state cache", k, v)
-        start = _check_counts(start, batch, self.device, "start")
-        counts = _check_counts(counts, batch, self.device, "counts")
-        k, v = _laid_out(k), _laid_out(v)
-        args = self._args(k, v, start, counts)
-        _lib.check(_call(_lib.load().state_cache_write, args, self.device), "state cache write")
+        self._copy(_lib.load().state_cache_write, _laid_out(k), _laid_out(v), start, counts, "state cache write")
 
     def read(self, count: int | None = None, *, start=None, counts=None, dtype=torch.bfloat16):
         """The values of ``count`` states per sequence (all C without it) from state
@@ -110,22 +130,38 @@ class StateCache:
         count = capacity if count is None else int(count)
         if count < 0:
             raise ValueError("count must not be negative")
-        if dtype not in (torch.bfloat16, torch.float16):
+        if dtype not in _HALF:
             raise ValueError("dtype must be bfloat16 or float16")
-        start = _check_counts(start, batch, self.device, "start")
-        counts = _check_counts(counts, batch, self.device, "counts")
-        k, v = (torch.empty(batch, groups, count, head_dim, dtype=dtype, device=self.device) for _ in range(2))
-        args = self._args(k, v, start, counts)
-        _lib.check(_call(_lib.load().state_cache_read, args, self.device), "state cache read")
+        k, v = (torch.empty(batch, groups, count, head_dim, dtype=dtype, device=self.keys.device) for _ in range(2))
+        self._copy(_lib.load().state_cache_read, k, v, start, counts, "state cache read")
         return k, v
 
     def _set_states(self, args) -> None:
         _, args.groups, args.states, _ = self.keys.shape
-        args.k, args.k_stride = self.keys.data_ptr(), self.keys.stride()
-        args.v, args.v_stride = self.values.data_ptr(), self.values.stride()
-        args.k_exponents, args.v_exponents = self.key_exponents.data_ptr(), self.value_exponents.data_ptr()
+        args.k_stride, args.v_stride = self.keys.stride(), self.values.stride()
+        args.eight_bit = 1
         strides = self.key_exponents.stride()
         args.exponent_stride[0], args.exponent_stride[1] = strides[0], strides[1]
+
+
+def _cached_plan(q, cache: StateCache, scale, out_stride):
+    key = (cache.layout, q.shape, q.stride(), q.dtype, q.device, scale, out_stride)
+    plan = _plans.get(key)
+    if plan is None:
+        _check_query(q, cache.keys.shape[1], cache.keys.shape[3], "cached cross attention", 16)
+        if q.device != cache.device:
+            raise ValueError("all tensors must be on the same CUDA device")
+        if q.shape[0] != cache.keys.shape[0]:
+            raise ValueError("q and the cache must share the batch size")
+        if cache.keys.shape[2] < 1:
+            raise ValueError("the cache must hold at least one state")
+        scale = _check_scale(scale)
+        if not _ready(q):
+            return None
+        args = _base_args(q, scale, out_stride, "auto")
+        cache._set_states(args)
+        plan = _keep(key, _finish_plan(args, q, "cached cross attention"))
+    return plan
 
 
 def cached_cross_attention(q, cache, *, scale, lengths=None, out=None):
@@ -136,19 +172,23 @@ def cached_cross_attention(q, cache, *, scale, lengths=None, out=None):
     what = "cached cross attention"
     if not isinstance(cache, StateCache):
         raise ValueError("cache must be a StateCache")
+    if not isinstance(q, torch.Tensor):
+        raise ValueError(f"{what} requires CUDA tensors")
     _refuse_grad(what, q)
-    _check_query(q, cache.keys.shape[1], cache.keys.shape[3], what, 16)
-    if q.device != cache.device:
-        raise ValueError("all tensors must be on the same CUDA device")
-    if q.shape[0] != cache.keys.shape[0]:
-        raise ValueError("q and the cache must share the batch size")
-    if cache.keys.shape[2] < 1:
-        raise ValueError("the cache must hold at least one state")
-    lengths = _check_counts(lengths, q.shape[0], q.device, "lengths")
-    scale = _check_scale(scale)
-    out = _output(q, out)
-    q = _laid_out(q)
-    args = _base_args(q, scale, lengths, out, None, "auto")
-    cache._set_states(args)
-    _run_forward(args, q.device, what)
+    scale = float(scale)
+    out_stride = None
+    if out is not None:
+        out_stride = _output(q, out).stride()
+    elif q.ndim == 4:
+        _, h, m, d = q.shape
+        out_stride = (h * m * d, m * d, d, 1)
+    plan = _cached_plan(q, cache, scale, out_stride)
+    if plan is None or q.data_ptr() & 15:
+        q = _laid_out(q)
+        plan = _cached_plan(q, cache, scale, out_stride)
+    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=plan.device)
+    _launch(plan, what, q.data_ptr(), cache.keys.data_ptr(), cache.values.data_ptr(), cache.key_exponents.data_ptr(),
+            cache.value_exponents.data_ptr(), 0, 0, lengths_p, out.data_ptr(), 0)
     return out

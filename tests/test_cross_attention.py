@@ -51,9 +51,11 @@ def _args(**over):
     ({"kernel": 7}, _lib.INTP_ERR_ARGUMENT),
     ({"q": None}, _lib.INTP_ERR_ARGUMENT),
     ({"status": None}, _lib.INTP_ERR_ARGUMENT),
-    ({"k_exponents": FAKE}, _lib.INTP_ERR_ARGUMENT),           # one of the two
-    ({"k_exponents": FAKE, "v_exponents": FAKE, "kernel": _lib.XATTN_KERNEL_TILES}, _lib.INTP_ERR_UNSUPPORTED),
-    ({"k_exponents": FAKE, "v_exponents": FAKE, "head_dim": 40}, _lib.INTP_ERR_SHAPE),
+    ({"eight_bit": 1, "k_exponents": FAKE}, _lib.INTP_ERR_ARGUMENT),  # one of the two
+    ({"k_exponents": FAKE, "v_exponents": FAKE}, _lib.INTP_ERR_ARGUMENT),  # of 16-bit states
+    ({"eight_bit": 1, "kernel": _lib.XATTN_KERNEL_TILES}, _lib.INTP_ERR_UNSUPPORTED),
+    ({"eight_bit": 1, "head_dim": 40}, _lib.INTP_ERR_SHAPE),
+    ({"eight_bit": 2}, _lib.INTP_ERR_ARGUMENT),
     ({"prefix": 5}, _lib.INTP_ERR_ARGUMENT),                   # no prefix tensors
     ({"q": FAKE + 8}, _lib.INTP_ERR_LAYOUT),
     ({"k_stride": _lib._Stride(12800, 6400, 68, 1)}, _lib.INTP_ERR_LAYOUT),

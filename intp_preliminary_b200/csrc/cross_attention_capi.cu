@@ -77,7 +77,7 @@ Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t sta
     const int64_t items = instances * ceil_div(rows, intp::kXaRowsTile);
     int64_t split = states <= 512 ? 1 : std::min(ceil_div(kPlanSms * 8, items), ceil_div(states, 256));
     if (a->eight_bit) split = std::max(split, ceil_div(states, intp::kXaRowsKeys8));
-    s.split_keys = ceil_div(ceil_div(states, split), 64) * 64;
+    s.split_keys = ceil_div(ceil_div(states, split), 128) * 128;
   }
   s.n_split = ceil_div(states, s.split_keys);
   return s;

@@ -5,23 +5,26 @@
 //
 // Reading the states bounds this: 16 rows or fewer share each key, so a 16-bit
 // state of 4 D bytes carries at most 64 D multiply-adds, far below the tensor
-// cores' ratio.  What counts is bytes in flight.  A CTA of 4 warps takes 16 rows
-// and a range of keys; each warp streams its own 16-key slices through a private
-// cp.async ring (no CTA barrier in the loop), forms S = q k^T and O += P v with
-// 16 x 8 x 16 matrix instructions (16 rows is their natural height; a 128-row
-// tcgen05 tile would idle on 112 of them), and keeps its own running maximum and
-// sum.  The warps join through shared memory at the end; ranges of keys join
-// through a workspace (combine kernel) in a fixed order, so results repeat.
+// cores' ratio.  What counts is bytes in flight and few instructions per byte.
+// A CTA of 4 warps takes 8 or 16 rows and a range of keys; each warp streams its
+// own slices of keys through a private cp.async ring (no CTA barrier in the
+// loop) and keeps its own running maximum and sum.  The products are 16 x 8 x 16
+// matrix instructions with the states as the 16-high operand,
+//   S^T = k q^T (16 keys x 8 rows),   O^T += v^T P^T (16 columns x 8 rows),
+// so 8 rows fill them (a 128-row tcgen05 tile would idle on 112 rows or more).
+// P^T goes from the first product's layout to the second's by an 8 x 8 transpose
+// in registers.  The reference of the exponentials moves only when a score
+// passes it by 2^8, so a step needs one vote and no shuffles.
+// The warps join through shared memory at the end; ranges of keys join through a
+// workspace (combine kernel) in a fixed order, so results repeat.
 //
 // 8-bit states are widened to f16 (exact) as they leave shared memory.  The
 // key's power of two multiplies the score; the value's joins the exponent of the
-// probability, whose own running maximum (of score + value exponent) keeps the
-// f16 product operand in (0, 1] whatever the exponents are.  A bf16 query row is
+// probability, whose own reference (score + value exponent) keeps the f16
+// product operand below 2^8 whatever the exponents are.  A bf16 query row is
 // first scaled by a power of two into the f16 range.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cstdint>
-#include "sm100_ptx.cuh"
+#include "xattn_common.cuh"
 #include "xattn_internal.h"
 
 namespace intp {
@@ -29,20 +32,18 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStep = 16;                  // keys of a warp's slice
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kRescale = 8.f;            // log2 units a score may pass its reference by
 
 template <int DP, bool FP8>
 struct RowsShape {
   static constexpr int kElem = FP8 ? 1 : 2;                // bytes of a state's value
+  static constexpr int kStep = FP8 ? 32 : 16;              // keys of a warp's slice
   static constexpr int kChunks = DP * kElem / 16;          // 16-byte chunks of a state
   static constexpr int kPerChunk = 16 / kElem;             // values of a chunk
   static constexpr int kSliceBytes = kStep * DP * kElem;   // K or V of a slice
-  static constexpr int kStages = DP * kElem == 256 ? 3 : (DP * kElem == 128 ? 6 : 8);
+  static constexpr int kStages = DP == 128 ? 3 : 6;
   static constexpr int kRing = kWarps * kStages * 2 * kSliceBytes;
-  static constexpr int kJoinStride = DP + 8;               // floats; rows land on different banks
-  static constexpr int kJoin = kWarps * kXaRowsTile * kJoinStride * 4;
-  static constexpr int kData = kRing > kJoin ? kRing : kJoin;
 };
 
 template <int CH>
@@ -53,6 +54,9 @@ __device__ __forceinline__ uint32_t chunk_offset(int row, int c) {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -72,63 +76,70 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4])
                : "r"(addr)
                : "memory");
 }
+// Transpose of the 8 x 8 16-bit matrix whose row g this lane quad holds.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
 // C += A B for 16 rows, 8 columns and a depth of 16.
 template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
   if (BF16)
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two e4m3 codes (low byte first) to two f16 values, exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(d) : "r"(codes & 0xffffu));
-  return d;
+// Four e4m3 codes (low byte first) to two pairs of f16 values, exact.
+__device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// Over the four lanes that hold a row's columns.
-__device__ __forceinline__ float quad_max(float v) {
-  v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return max_nan(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// Over the eight lanes that hold a query row's keys.
+__device__ __forceinline__ float keys_max(float v) {
+#pragma unroll
+  for (int s = 4; s < 32; s <<= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, s));
+  return v;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
-}
-__device__ __forceinline__ float2 bf16x2_to_float2(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+__device__ __forceinline__ float keys_sum(float v) {
+#pragma unroll
+  for (int s = 4; s < 32; s <<= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+  return v;
 }
 
 struct RowsArgs {
   XaParams p;
   int32_t n_rt;
+  int32_t smem_scales;   // bytes from the dynamic shared memory's start to the exponents' values
 };
 
-template <int DP, bool BF16, bool FP8>
+// NT: tiles of 8 query rows.
+template <int DP, bool BF16, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads)
 xattn_rows_kernel(const RowsArgs a) {
   using L = RowsShape<DP, FP8>;
-  constexpr int CH = L::kChunks, NS = L::kStages;
+  constexpr int CH = L::kChunks, NS = L::kStages, KT = L::kStep / 16;  // KT: 16-key tiles of a slice
   constexpr bool MMA_BF16 = BF16 && !FP8;   // element type of the products
+  constexpr int kTile = 8 * NT;             // rows of a CTA
+  constexpr int kJoinStride = DP + 4;       // floats
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float m_s[kWarps][kXaRowsTile], l_s[kWarps][kXaRowsTile], w_s[kWarps][kXaRowsTile];
+  __shared__ float m_s[kWarps][kTile], l_s[kWarps][kTile], w_s[kWarps][kTile];
   const XaParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;    // fragment row and column pair
@@ -140,59 +151,77 @@ xattn_rows_kernel(const RowsArgs a) {
   const int32_t key0 = split * p.split_keys;
   const int32_t left = length - key0;
   const int32_t n_keys = left < 0 ? 0 : (left < p.split_keys ? left : p.split_keys);
-  const int32_t row0 = rt * kXaRowsTile;
-  const int32_t n_rows = p.rows - row0 < kXaRowsTile ? p.rows - row0 : kXaRowsTile;
+  const int32_t row0 = rt * kTile;
+  const int32_t n_rows = p.rows - row0 < kTile ? p.rows - row0 : kTile;
   const int32_t D = p.head_dim;
 
-  const uint8_t* k_src = static_cast<const uint8_t*>(p.k) +
-                         (b * p.ks[0] + grp * p.ks[1] + static_cast<int64_t>(key0) * p.ks[2]) * L::kElem;
-  const uint8_t* v_src = static_cast<const uint8_t*>(p.v) +
-                         (b * p.vs[0] + grp * p.vs[1] + static_cast<int64_t>(key0) * p.vs[2]) * L::kElem;
   const int64_t k_row = p.ks[2] * L::kElem, v_row = p.vs[2] * L::kElem;
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  const int32_t n_slices = (n_keys + kStep - 1) / kStep;
+  const int32_t n_slices = (n_keys + L::kStep - 1) / L::kStep;
   const int32_t mine = n_slices > warp ? (n_slices - warp + kWarps - 1) / kWarps : 0;
-  const int32_t d_read = (D + 15) & ~15;    // columns the products read
 
-  // Slice i of this warp (keys 16 (warp + 4 i) ..) into its ring; keys past the end and columns past D are zero.
-  auto issue = [&](int32_t i) {
-    if (i < mine) {
-      const int32_t k0 = (i * kWarps + warp) * kStep;
-      const uint32_t dst = ring + (i % NS) * 2 * L::kSliceBytes;
+  // This lane copies chunk `cc` of states `cr`, cr + 32 / CH, ... of each slice.
+  const int cr = lane / CH, cc = lane % CH;
+  const bool chunk_read = cc * L::kPerChunk < D;
+  const bool chunk_used = cc * L::kPerChunk < ((D + 15) & ~15);  // columns past D that the products read are zero
+  const uint8_t* k_src = static_cast<const uint8_t*>(p.k) +
+                         (b * p.ks[0] + grp * p.ks[1] + (static_cast<int64_t>(key0) + warp * L::kStep) * p.ks[2]) * L::kElem;
+  const uint8_t* v_src = static_cast<const uint8_t*>(p.v) +
+                         (b * p.vs[0] + grp * p.vs[1] + (static_cast<int64_t>(key0) + warp * L::kStep) * p.vs[2]) * L::kElem;
+  if (chunk_read) {
+    k_src += cr * k_row + cc * 16;
+    v_src += cr * v_row + cc * 16;
+  }
+  const int64_t k_next = (32 / CH) * k_row, v_next = (32 / CH) * v_row;
+  int32_t issued = 0;
+  // The next slice of this warp (keys 32 or 16 times (warp + 4 i) ..) into its ring; keys past the end are zero.
+  auto issue = [&]() {
+    if (issued < mine) {
+      const int32_t k0 = (issued * kWarps + warp) * L::kStep;
+      const uint32_t dst = ring + (issued % NS) * 2 * L::kSliceBytes;
+      const uint8_t *ks = k_src, *vs = v_src;
+      if (k0 + L::kStep <= n_keys && chunk_read) {
 #pragma unroll
-      for (int u = 0; u < kStep * CH / 32; ++u) {
-        const int idx = lane + 32 * u, row = idx / CH, c = idx % CH;
-        if (c * L::kPerChunk < d_read) {
-          const bool read = k0 + row < n_keys && c * L::kPerChunk < D;
-          const int64_t at = read ? k0 + row : 0;
-          const int col = read ? c * 16 : 0;
-          cp_async16(dst + chunk_offset<CH>(row, c), k_src + at * k_row + col, read);
-          cp_async16(dst + L::kSliceBytes + chunk_offset<CH>(row, c), v_src + at * v_row + col, read);
+        for (int u = 0; u < L::kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
+          const uint32_t to = dst + chunk_offset<CH>(cr + u * (32 / CH), cc);
+          cp_async16(to, ks);
+          cp_async16(to + L::kSliceBytes, vs);
+        }
+      } else if (chunk_used) {
+#pragma unroll
+        for (int u = 0; u < L::kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
+          const int row = cr + u * (32 / CH);
+          const bool read = k0 + row < n_keys && chunk_read;
+          const uint32_t to = dst + chunk_offset<CH>(row, cc);
+          cp_async16(to, read ? ks : static_cast<const uint8_t*>(p.k), read);
+          cp_async16(to + L::kSliceBytes, read ? vs : static_cast<const uint8_t*>(p.v), read);
         }
       }
+      k_src += kWarps * L::kStep * k_row;
+      v_src += kWarps * L::kStep * v_row;
     }
+    ++issued;
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) issue(i);
+  for (int i = 0; i < NS - 1; ++i) issue();
 
-  // Exponent bytes of the range (8-bit states), keys' then values'.
-  uint8_t* exp_s = smem + L::kData;
+  // 8-bit states: each key's power of two, and its value's exponent.
+  float2* scale_s = reinterpret_cast<float2*>(smem + a.smem_scales);
   if (FP8) {
     const int64_t base = b * p.es[0] + grp * p.es[1] + key0;
-    for (int i = threadIdx.x; i < n_keys; i += kThreads) {
-      exp_s[i] = p.k_exp[base + i];
-      exp_s[p.split_keys + i] = p.v_exp[base + i];
-    }
+    for (int i = threadIdx.x; i < n_keys; i += kThreads)
+      scale_s[i] = make_float2(__uint_as_float(static_cast<uint32_t>(p.k_exp[base + i]) << 23),
+                               static_cast<float>(p.v_exp[base + i]) - 127.f);
   }
 
-  // Query fragments: rows g and g + 8; the depth order follows the K fragments
+  // Query fragments (rows 8 n + g as columns of q^T); the depth order follows the K fragments
   // (16-bit: columns 2t, 2t+1 and 2t+8, 2t+9 of each 16; 8-bit: 4t .. 4t+3).
-  uint32_t qa[DP / 16][4];
-  float row_scale[2] = {p.scale * kLog2e, p.scale * kLog2e};
+  uint32_t qb[NT][DP / 16][2];
+  float row_scale[NT][2];                   // of rows 8 n + 2 t, + 1 (the score fragment's columns)
 #pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
-    const int32_t r = row0 + g + 8 * hf;
+  for (int n = 0; n < NT; ++n) {
+    const int32_t r = row0 + 8 * n + g;
     const uint16_t* src = nullptr;
     if (r < p.rows) {
       const XaRow x = xa_row(p, inst, r);
@@ -201,9 +230,10 @@ xattn_rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
       const int d0 = kk * 16 + (FP8 ? 4 * t : 2 * t), d1 = d0 + (FP8 ? 2 : 8);
-      qa[kk][hf] = src != nullptr && d0 < D ? *reinterpret_cast<const uint32_t*>(src + d0) : 0u;
-      qa[kk][2 + hf] = src != nullptr && d1 < D ? *reinterpret_cast<const uint32_t*>(src + d1) : 0u;
+      qb[n][kk][0] = src != nullptr && d0 < D ? *reinterpret_cast<const uint32_t*>(src + d0) : 0u;
+      qb[n][kk][1] = src != nullptr && d1 < D ? *reinterpret_cast<const uint32_t*>(src + d1) : 0u;
     }
+    float up = p.scale * kLog2e;
     if (FP8 && BF16) {
       // Largest magnitude to [2^14, 2^15): every value within 2^-28 of it is exact in f16.
       float top = 0.f;
@@ -211,167 +241,218 @@ xattn_rows_kernel(const RowsArgs a) {
       for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float2 f = bf16x2_to_float2(qa[kk][2 * e + hf]);
+          const float2 f = unpack2<true>(qb[n][kk][e]);
           top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
-      top = quad_max(top);
-      const int e = top >= 1.17549435e-38f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14 : 0;
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - (e < -126 ? -126 : e)) << 23);
-      row_scale[hf] *= __uint_as_float(static_cast<uint32_t>(127 + (e < -126 ? -126 : e)) << 23);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int e = top >= 1.17549435e-38f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14 : 0;
+      e = e < -126 ? -126 : e;
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      up *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 f = bf16x2_to_float2(qa[kk][2 * i + hf]);
-          qa[kk][2 * i + hf] = pack_f16x2(f.x * down, f.y * down);
+          const float2 f = unpack2<true>(qb[n][kk][i]);
+          qb[n][kk][i] = pack_f16x2(f.x * down, f.y * down);
         }
     }
+    row_scale[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);       // the lanes of g = 2 t
+    row_scale[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
   }
-  if (FP8) __syncthreads();  // exponents are in
+  if (FP8) __syncthreads();  // the exponents are in
 
-  float o[DP / 8][4];
+  float o[NT][DP / 16][4];
+  // Per row (8 n + 2 t + h): running reference, that of score + value exponent, this lane's part of the sum.
+  float m[NT][2], mw[NT][2], l[NT][2];
 #pragma unroll
-  for (int n = 0; n < DP / 8; ++n)
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, mw[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][c][e] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[n][h] = mw[n][h] = -INFINITY;
+      l[n][h] = 0.f;
+    }
+  }
   const int mi = lane >> 3, mr = lane & 7;
 
   for (int32_t i = 0; i < mine; ++i) {
     cp_async_wait<NS - 2>();
     __syncwarp();
     const uint32_t k_s = ring + (i % NS) * 2 * L::kSliceBytes, v_s = k_s + L::kSliceBytes;
-    const int32_t k0 = (i * kWarps + warp) * kStep;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    if (FP8) {
+    const int32_t k0 = (i * kWarps + warp) * L::kStep;
+    float s[NT][KT][4];                     // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1) of each 16
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        if (c * 16 >= D) break;
-        uint32_t r[4];
-        ldmatrix4(k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), c + (mi >> 1)), r);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if ((c + u) * 16 >= D) break;
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-            mma16816<false>(s[n], qa[c + u], e4m3x2_to_f16x2(r[2 * u + n]), e4m3x2_to_f16x2(r[2 * u + n] >> 16));
-        }
-      }
-    } else {
+        for (int e = 0; e < 4; ++e) s[n][kt][e] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        if (kk * 16 >= D) break;
-        uint32_t r[4];
-        ldmatrix4(k_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), 2 * kk + (mi & 1)), r);
-        mma16816<MMA_BF16>(s[0], qa[kk], r[0], r[1]);
-        mma16816<MMA_BF16>(s[1], qa[kk], r[2], r[3]);
-      }
-    }
-    // Scores of rows g, g + 8 and keys 8 n + 2 t, + 1 in log2 units; padded keys -inf.
-    float tv[2][4];                         // with the value's exponent (8-bit states)
-    float mx[2] = {-INFINITY, -INFINITY}, mxw[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int32_t key = k0 + 8 * n + 2 * t + (e & 1);
-        const int hf = e >> 1;
-        float v = s[n][e] * row_scale[hf], w = 0.f;
-        if (FP8 && key < n_keys) {
-          v *= __uint_as_float(static_cast<uint32_t>(exp_s[key]) << 23);
-          w = static_cast<float>(exp_s[p.split_keys + key]) - 127.f;
-        }
-        v = key < n_keys ? v : -INFINITY;
-        s[n][e] = v;
-        mx[hf] = max_nan(mx[hf], v);
-        if (FP8) {
-          tv[n][e] = v + w;
-          mxw[hf] = max_nan(mxw[hf], tv[n][e]);
-        }
-      }
-    float ref[2], refw[2], fo[2];
-    bool grow = false;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const float top = max_nan(m[hf], quad_max(mx[hf]));
-      const float topw = FP8 ? max_nan(mw[hf], quad_max(mxw[hf])) : top;
-      grow = grow || !(top <= m[hf]) || (FP8 && !(topw <= mw[hf]));
-      // A row without a score above -inf keeps 0 as its reference.
-      ref[hf] = top == -INFINITY ? 0.f : top;
-      refw[hf] = topw == -INFINITY ? 0.f : topw;
-      l[hf] *= fast_exp2(m[hf] - ref[hf]);
-      fo[hf] = FP8 ? fast_exp2(mw[hf] - refw[hf]) : fast_exp2(m[hf] - ref[hf]);
-      m[hf] = top;
-      mw[hf] = topw;
-    }
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] *= fo[e >> 1];
-    }
-    uint32_t pa[4];                         // P as the A operand: keys 2t, 2t+1 | 2t+8, 2t+9
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float pr[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pr[e] = fast_exp2(s[n][e] - ref[e >> 1]);
-        l[e >> 1] += pr[e];
-        if (FP8) pr[e] = fast_exp2(tv[n][e] - refw[e >> 1]);
-      }
-      pa[2 * n] = pack2<MMA_BF16>(pr[0], pr[1]);
-      pa[2 * n + 1] = pack2<MMA_BF16>(pr[2], pr[3]);
-    }
-#pragma unroll
-    for (int c = 0; c < CH; c += 2) {
-      if (c * L::kPerChunk >= D) break;
-      uint32_t r[4];
-      ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi & 1) << 3), c + (mi >> 1)), r);
+    for (int kt = 0; kt < KT; ++kt) {
       if (FP8) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if ((c + u) * 16 >= D) break;
-          // r: keys 2t, 2t+1 of two columns each -> key pairs of the even, then of the odd column
-          const uint32_t lo = __byte_perm(r[2 * u], 0u, 0x3120), hi = __byte_perm(r[2 * u + 1], 0u, 0x3120);
-          mma16816<false>(o[2 * (c + u)], pa, e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(hi));
-          mma16816<false>(o[2 * (c + u) + 1], pa, e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi >> 16));
+        for (int c = 0; c < CH; c += 2) {
+          if (c * 16 >= D) break;
+          uint32_t r[4];                    // keys 0-7 and 8-15 of chunk c, then of c + 1
+          ldmatrix4(k_s + chunk_offset<CH>(kt * 16 + mr + ((mi & 1) << 3), c + (mi >> 1)), r);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if ((c + u) * 16 >= D) break;
+            uint32_t a0, a1, a2, a3;
+            widen4(r[2 * u], a0, a2);
+            widen4(r[2 * u + 1], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<false>(s[n][kt], a0, a1, a2, a3, qb[n][c + u][0], qb[n][c + u][1]);
+          }
         }
       } else {
-        mma16816<MMA_BF16>(o[c], pa, r[0], r[1]);
-        mma16816<MMA_BF16>(o[c + 1], pa, r[2], r[3]);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          if (kk * 16 >= D) break;
+          uint32_t r[4];                    // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
+          ldmatrix4(k_s + chunk_offset<CH>(kt * 16 + mr + ((mi & 1) << 3), 2 * kk + (mi >> 1)), r);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<MMA_BF16>(s[n][kt], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
+        }
+      }
+    }
+    // Scores in log2 units; padded keys -inf.
+    float w[KT][2];                         // value exponents
+    bool grow = false;
+    const bool padded = k0 + L::kStep > n_keys;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh) {
+        const int32_t key = k0 + kt * 16 + kh * 8 + g;
+        float2 f = make_float2(1.f, 0.f);
+        if (FP8) f = scale_s[!padded || key < n_keys ? key : 0];
+        w[kt][kh] = f.y;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& v = s[n][kt][2 * kh + h];
+            v *= row_scale[n][h];
+            if (FP8) v *= f.x;
+            if (padded && key >= n_keys) v = -INFINITY;
+            // a NaN score counts as growth: it has to reach the reference
+            grow = grow || !(v <= m[n][h] + kRescale) || (FP8 && !(v + f.y <= mw[n][h] + kRescale));
+          }
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float fo[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = m[n][h], topw = mw[n][h];
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+              top = max_nan(top, s[n][kt][2 * kh + h]);
+              if (FP8) topw = max_nan(topw, s[n][kt][2 * kh + h] + w[kt][kh]);
+            }
+          top = keys_max(top);
+          topw = FP8 ? keys_max(topw) : top;
+          l[n][h] *= top == -INFINITY ? 1.f : fast_exp2(m[n][h] - top);
+          fo[h] = topw == -INFINITY ? 1.f : fast_exp2((FP8 ? mw[n][h] : m[n][h]) - topw);
+          m[n][h] = top;
+          mw[n][h] = topw;
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][c][e] *= fo[e & 1];
+      }
+    }
+    uint32_t pb[NT][KT][2];                 // P^T as the 8-wide operand: keys 2t, 2t+1 of each 8, row g
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // A row without a score above -inf keeps 0 as its reference.
+      const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+      const float refw[2] = {mw[n][0] == -INFINITY ? 0.f : mw[n][0], mw[n][1] == -INFINITY ? 0.f : mw[n][1]};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          float pr[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float v = s[n][kt][2 * kh + h];
+            pr[h] = fast_exp2(v - ref[h]);
+            l[n][h] += pr[h];
+            if (FP8) pr[h] = fast_exp2(v + w[kt][kh] - refw[h]);
+          }
+          pb[n][kt][kh] = transpose8(pack2<MMA_BF16>(pr[0], pr[1]));
+        }
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int c = 0; c < CH; c += 2) {
+        if (c * L::kPerChunk >= D) break;
+        uint32_t r[4];
+        if (FP8) {
+          // keys 0-7 and 8-15 of chunk c, then of c + 1: two columns of two keys each
+          ldmatrix4_trans(v_s + chunk_offset<CH>(kt * 16 + mr + ((mi & 1) << 3), c + (mi >> 1)), r);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if ((c + u) * 16 >= D) break;
+            // -> key pairs of the even, then of the odd column
+            uint32_t a0, a1, a2, a3;
+            widen4(__byte_perm(r[2 * u], 0u, 0x3120), a0, a1);
+            widen4(__byte_perm(r[2 * u + 1], 0u, 0x3120), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<false>(o[n][c + u], a0, a1, a2, a3, pb[n][kt][0], pb[n][kt][1]);
+          }
+        } else {
+          // chunk c and c + 1 of keys 0-7, then of 8-15
+          ldmatrix4_trans(v_s + chunk_offset<CH>(kt * 16 + mr + ((mi >> 1) << 3), c + (mi & 1)), r);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][kt][0], pb[n][kt][1]);
+        }
       }
     }
     __syncwarp();
-    issue(i + NS - 1);
+    issue();
   }
   cp_async_wait<0>();
   __syncthreads();  // every ring is at rest: the space takes the warps' sums
 
   float* join = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
-    const int r = g + 8 * hf;
-    const float sum = quad_sum(l[hf]);
-    if (t == 0) {
-      m_s[warp][r] = m[hf];
-      l_s[warp][r] = sum;
-      w_s[warp][r] = FP8 ? mw[hf] : m[hf];
-    }
-    if (r < n_rows && mine > 0) {
-      float* dst = join + (warp * kXaRowsTile + r) * L::kJoinStride;
-      if (FP8) {
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-          *reinterpret_cast<float4*>(dst + c * 16 + 4 * t) =
-              make_float4(o[2 * c][2 * hf], o[2 * c + 1][2 * hf], o[2 * c][2 * hf + 1], o[2 * c + 1][2 * hf + 1]);
-      } else {
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * n + 2 * t + h;
+      const float sum = keys_sum(l[n][h]);
+      if (g == 0) {
+        m_s[warp][r] = m[n][h];
+        l_s[warp][r] = sum;
+        w_s[warp][r] = FP8 ? mw[n][h] : m[n][h];
+      }
+      if (r < n_rows && mine > 0) {
+        float* dst = join + (warp * kTile + r) * kJoinStride;
 #pragma unroll
-        for (int n = 0; n < DP / 8; ++n)
-          *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hf], o[n][2 * hf + 1]);
+        for (int c = 0; c < DP / 16; ++c) {
+          // fragment rows g, g + 8: columns 2 g, 2 g + 1 (8-bit) or g, g + 8 of each 16
+          if (FP8) {
+            *reinterpret_cast<float2*>(dst + c * 16 + 2 * g) = make_float2(o[n][c][h], o[n][c][2 + h]);
+          } else {
+            dst[c * 16 + g] = o[n][c][h];
+            dst[c * 16 + 8 + g] = o[n][c][2 + h];
+          }
+        }
       }
     }
-  }
   __syncthreads();
   const bool part = p.part_o != nullptr;
   for (int r = warp; r < n_rows; r += kWarps) {
@@ -396,7 +477,7 @@ xattn_rows_kernel(const RowsArgs a) {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
         if (f[w] != 0.f) {
-          const float4 v = *reinterpret_cast<const float4*>(join + (w * kXaRowsTile + r) * L::kJoinStride + d);
+          const float4 v = *reinterpret_cast<const float4*>(join + (w * kTile + r) * kJoinStride + d);
           acc.x = fmaf(v.x, f[w], acc.x);
           acc.y = fmaf(v.y, f[w], acc.y);
           acc.z = fmaf(v.z, f[w], acc.z);
@@ -457,22 +538,32 @@ xattn_combine_kernel(const XaParams p, int32_t n_slots) {
   if (lane == 0 && p.lse != nullptr) p.lse[lin] = none ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
-template <int DP, bool BF16, bool FP8>
-int32_t launch(const RowsArgs& a, int64_t grid, cudaStream_t stream) {
+template <int DP, bool BF16, bool FP8, int NT>
+int32_t launch(RowsArgs a, cudaStream_t stream) {
   using L = RowsShape<DP, FP8>;
-  auto kernel = xattn_rows_kernel<DP, BF16, FP8>;
-  const int smem = L::kData + (FP8 ? 2 * a.p.split_keys : 0);
-  constexpr int most = L::kData + (FP8 ? 2 * kXaRowsKeys8 : 0);
+  auto kernel = xattn_rows_kernel<DP, BF16, FP8, NT>;
+  constexpr int kJoin = kWarps * 8 * NT * (DP + 4) * 4;   // the warps' sums, in the rings' place
+  constexpr int kData = L::kRing > kJoin ? L::kRing : kJoin;
+  constexpr int kMost = kData + (FP8 ? 8 * kXaRowsKeys8 : 0);
+  static_assert(kMost <= 227 * 1024, "shared memory of a CTA");
+  a.smem_scales = kData;
+  const int smem = kData + (FP8 ? 8 * a.p.split_keys : 0);
   static std::atomic<uint64_t> done{0};
-  if (smem > most) return 8;
-  if (!allow_smem(kernel, most, done)) return 6;
+  if (smem > kMost) return 8;
+  if (!allow_smem(kernel, kMost, done)) return 6;
+  a.n_rt = (a.p.rows + 8 * NT - 1) / (8 * NT);
+  const int64_t grid = static_cast<int64_t>(a.n_rt) * a.p.instances * a.p.n_split;
+  if (grid > INT32_MAX) return 8;
   kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 6;
 }
 
 template <bool BF16, bool FP8>
-int32_t launch_dim(const RowsArgs& a, int64_t grid, cudaStream_t stream) {
-  return a.p.head_dim <= 64 ? launch<64, BF16, FP8>(a, grid, stream) : launch<128, BF16, FP8>(a, grid, stream);
+int32_t launch_dim(const RowsArgs& a, cudaStream_t stream) {
+  const bool narrow = a.p.rows <= 8;
+  if (a.p.head_dim <= 64)
+    return narrow ? launch<64, BF16, FP8, 1>(a, stream) : launch<64, BF16, FP8, 2>(a, stream);
+  return narrow ? launch<128, BF16, FP8, 1>(a, stream) : launch<128, BF16, FP8, 2>(a, stream);
 }
 
 }  // namespace
@@ -480,12 +571,9 @@ int32_t launch_dim(const RowsArgs& a, int64_t grid, cudaStream_t stream) {
 int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream) {
   RowsArgs a;
   a.p = p;
-  a.n_rt = (p.rows + kXaRowsTile - 1) / kXaRowsTile;
-  const int64_t grid = static_cast<int64_t>(a.n_rt) * p.instances * p.n_split;
-  if (grid > INT32_MAX) return 8;
   const bool fp8 = p.k_exp != nullptr, bf16 = p.dtype == 2;
-  if (fp8) return bf16 ? launch_dim<true, true>(a, grid, stream) : launch_dim<false, true>(a, grid, stream);
-  return bf16 ? launch_dim<true, false>(a, grid, stream) : launch_dim<false, false>(a, grid, stream);
+  if (fp8) return bf16 ? launch_dim<true, true>(a, stream) : launch_dim<false, true>(a, stream);
+  return bf16 ? launch_dim<true, false>(a, stream) : launch_dim<false, false>(a, stream);
 }
 
 int32_t launch_xattn_combine(const XaParams& p, int32_t n_slots, cudaStream_t stream) {

@@ -111,26 +111,6 @@ Plan plan_forward(const xattn_args* a) {
   return p;
 }
 
-struct DeviceFacts {
-  int sms;
-};
-// The current device's, asked for once.
-intp_status device_facts(DeviceFacts* f) {
-  static std::atomic<int> known[64];   // 0: not asked; else SMs + 1, negative if not sm_100
-  int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return INTP_ERR_LAUNCH;
-  int v = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
-  if (v == 0) {
-    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&f->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-      return INTP_ERR_LAUNCH;
-    v = major == 10 ? f->sms + 1 : -1;
-    if (dev < 64) known[dev].store(v, std::memory_order_relaxed);
-  }
-  f->sms = v - 1;
-  return v > 0 ? INTP_OK : INTP_ERR_ARCH;
-}
-
 // Checks pointers and layouts and fills the parameters that every pass shares.
 intp_status to_params(const xattn_args* a, XaParams* p) {
   const int64_t elem = a->eight_bit ? 1 : 2;
@@ -234,6 +214,24 @@ bool workspace_ok(const xattn_args* a, int64_t bytes) {
 
 }  // namespace
 
+namespace intp {
+int32_t current_device_facts(int* sms) {
+  static std::atomic<int> known[64];   // 0: not asked; else SMs + 1, negative if not sm_100
+  int dev = 0, major = 0, count = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return INTP_ERR_LAUNCH;
+  int v = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return INTP_ERR_LAUNCH;
+    v = major == 10 ? count + 1 : -1;
+    if (dev < 64) known[dev].store(v, std::memory_order_relaxed);
+  }
+  *sms = v - 1;
+  return v > 0 ? INTP_OK : INTP_ERR_ARCH;
+}
+}  // namespace intp
+
 extern "C" {
 
 intp_status xattn_forward_workspace(const xattn_args* a, int64_t* bytes) {
@@ -264,8 +262,8 @@ intp_status xattn_forward(const xattn_args* a, void* stream) {
   if (st != INTP_OK) return st;
   const Plan plan = plan_forward(a);
   if (!workspace_ok(a, plan.bytes)) return INTP_ERR_ARGUMENT;
-  DeviceFacts f;
-  st = device_facts(&f);
+  int sms = 0;
+  st = intp::current_device_facts(&sms);
   if (st != INTP_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.parts) {
@@ -285,11 +283,11 @@ intp_status xattn_forward(const xattn_args* a, void* stream) {
     x.ks[0] = x.vs[0] = 0;
     take_strides(x.ks + 1, a->prefix_k_stride, ep, 2, a->head_dim);
     take_strides(x.vs + 1, a->prefix_v_stride, ep, 2, a->head_dim);
-    st = launch_pass(x, plan.pre, 0, s, f.sms);
+    st = launch_pass(x, plan.pre, 0, s, sms);
     if (st != INTP_OK) return st;
   }
   if (a->states > 0) {
-    st = launch_pass(p, plan.own, plan.pre_slots, s, f.sms);
+    st = launch_pass(p, plan.own, plan.pre_slots, s, sms);
     if (st != INTP_OK) return st;
   }
   if (!plan.parts) return INTP_OK;
@@ -316,8 +314,8 @@ intp_status xattn_backward(const xattn_backward_args* b, void* stream) {
     if (reinterpret_cast<uintptr_t>(g) % 16) return INTP_ERR_LAYOUT;
   const BackwardPlan plan = plan_backward(b);
   if (!workspace_ok(a, plan.bytes)) return INTP_ERR_ARGUMENT;
-  DeviceFacts f;
-  st = device_facts(&f);
+  int sms = 0;
+  st = intp::current_device_facts(&sms);
   if (st != INTP_OK) return st;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.dout = b->grad_out;

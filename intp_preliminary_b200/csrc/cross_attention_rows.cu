@@ -32,16 +32,18 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kStep = 16;                  // keys of a warp's slice
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;            // log2 units a score may pass its reference by
 
 template <int DP, bool FP8>
 struct RowsShape {
   static constexpr int kElem = FP8 ? 1 : 2;                // bytes of a state's value
-  static constexpr int kStep = FP8 ? 32 : 16;              // keys of a warp's slice
   static constexpr int kChunks = DP * kElem / 16;          // 16-byte chunks of a state
   static constexpr int kPerChunk = 16 / kElem;             // values of a chunk
   static constexpr int kSliceBytes = kStep * DP * kElem;   // K or V of a slice
+  // 8-bit states cost more instructions a byte: less shared memory a CTA and twice the warps an
+  // SM (16-key slices, 48 KB: 142 us at B64 G8 H32 N8192 D128; 32-key slices, 96 KB: 178 us).
   static constexpr int kStages = DP == 128 ? 3 : 6;
   static constexpr int kRing = kWarps * kStages * 2 * kSliceBytes;
 };
@@ -134,7 +136,7 @@ template <int DP, bool BF16, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads)
 xattn_rows_kernel(const RowsArgs a) {
   using L = RowsShape<DP, FP8>;
-  constexpr int CH = L::kChunks, NS = L::kStages, KT = L::kStep / 16;  // KT: 16-key tiles of a slice
+  constexpr int CH = L::kChunks, NS = L::kStages;
   constexpr bool MMA_BF16 = BF16 && !FP8;   // element type of the products
   constexpr int kTile = 8 * NT;             // rows of a CTA
   constexpr int kJoinStride = DP + 4;       // floats
@@ -157,7 +159,7 @@ xattn_rows_kernel(const RowsArgs a) {
 
   const int64_t k_row = p.ks[2] * L::kElem, v_row = p.vs[2] * L::kElem;
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  const int32_t n_slices = (n_keys + L::kStep - 1) / L::kStep;
+  const int32_t n_slices = (n_keys + kStep - 1) / kStep;
   const int32_t mine = n_slices > warp ? (n_slices - warp + kWarps - 1) / kWarps : 0;
 
   // This lane copies chunk `cc` of states `cr`, cr + 32 / CH, ... of each slice.
@@ -165,31 +167,31 @@ xattn_rows_kernel(const RowsArgs a) {
   const bool chunk_read = cc * L::kPerChunk < D;
   const bool chunk_used = cc * L::kPerChunk < ((D + 15) & ~15);  // columns past D that the products read are zero
   const uint8_t* k_src = static_cast<const uint8_t*>(p.k) +
-                         (b * p.ks[0] + grp * p.ks[1] + (static_cast<int64_t>(key0) + warp * L::kStep) * p.ks[2]) * L::kElem;
+                         (b * p.ks[0] + grp * p.ks[1] + (static_cast<int64_t>(key0) + warp * kStep) * p.ks[2]) * L::kElem;
   const uint8_t* v_src = static_cast<const uint8_t*>(p.v) +
-                         (b * p.vs[0] + grp * p.vs[1] + (static_cast<int64_t>(key0) + warp * L::kStep) * p.vs[2]) * L::kElem;
+                         (b * p.vs[0] + grp * p.vs[1] + (static_cast<int64_t>(key0) + warp * kStep) * p.vs[2]) * L::kElem;
   if (chunk_read) {
     k_src += cr * k_row + cc * 16;
     v_src += cr * v_row + cc * 16;
   }
   const int64_t k_next = (32 / CH) * k_row, v_next = (32 / CH) * v_row;
   int32_t issued = 0;
-  // The next slice of this warp (keys 32 or 16 times (warp + 4 i) ..) into its ring; keys past the end are zero.
+  // The next slice of this warp (keys 16 (warp + 4 i) ..) into its ring; keys past the end are zero.
   auto issue = [&]() {
     if (issued < mine) {
-      const int32_t k0 = (issued * kWarps + warp) * L::kStep;
+      const int32_t k0 = (issued * kWarps + warp) * kStep;
       const uint32_t dst = ring + (issued % NS) * 2 * L::kSliceBytes;
       const uint8_t *ks = k_src, *vs = v_src;
-      if (k0 + L::kStep <= n_keys && chunk_read) {
+      if (k0 + kStep <= n_keys && chunk_read) {
 #pragma unroll
-        for (int u = 0; u < L::kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
+        for (int u = 0; u < kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
           const uint32_t to = dst + chunk_offset<CH>(cr + u * (32 / CH), cc);
           cp_async16(to, ks);
           cp_async16(to + L::kSliceBytes, vs);
         }
       } else if (chunk_used) {
 #pragma unroll
-        for (int u = 0; u < L::kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
+        for (int u = 0; u < kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
           const int row = cr + u * (32 / CH);
           const bool read = k0 + row < n_keys && chunk_read;
           const uint32_t to = dst + chunk_offset<CH>(row, cc);
@@ -197,8 +199,8 @@ xattn_rows_kernel(const RowsArgs a) {
           cp_async16(to + L::kSliceBytes, read ? vs : static_cast<const uint8_t*>(p.v), read);
         }
       }
-      k_src += kWarps * L::kStep * k_row;
-      v_src += kWarps * L::kStep * v_row;
+      k_src += kWarps * kStep * k_row;
+      v_src += kWarps * kStep * v_row;
     }
     ++issued;
     cp_async_commit();
@@ -206,13 +208,12 @@ xattn_rows_kernel(const RowsArgs a) {
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) issue();
 
-  // 8-bit states: each key's power of two, and its value's exponent.
-  float2* scale_s = reinterpret_cast<float2*>(smem + a.smem_scales);
+  // 8-bit states: each state's exponent bytes, the key's low and the value's high.
+  uint16_t* exp_s = reinterpret_cast<uint16_t*>(smem + a.smem_scales);
   if (FP8) {
     const int64_t base = b * p.es[0] + grp * p.es[1] + key0;
     for (int i = threadIdx.x; i < n_keys; i += kThreads)
-      scale_s[i] = make_float2(__uint_as_float(static_cast<uint32_t>(p.k_exp[base + i]) << 23),
-                               static_cast<float>(p.v_exp[base + i]) - 127.f);
+      exp_s[i] = static_cast<uint16_t>(p.k_exp[base + i] | (p.v_exp[base + i] << 8));
   }
 
   // Query fragments (rows 8 n + g as columns of q^T); the depth order follows the K fragments
@@ -284,67 +285,64 @@ xattn_rows_kernel(const RowsArgs a) {
     cp_async_wait<NS - 2>();
     __syncwarp();
     const uint32_t k_s = ring + (i % NS) * 2 * L::kSliceBytes, v_s = k_s + L::kSliceBytes;
-    const int32_t k0 = (i * kWarps + warp) * L::kStep;
-    float s[NT][KT][4];                     // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1) of each 16
+    const int32_t k0 = (i * kWarps + warp) * kStep;
+    float s[NT][4];                         // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+    if (FP8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][kt][e] = 0.f;
+      for (int c = 0; c < CH; c += 2) {
+        if (c * 16 >= D) break;
+        uint32_t r[4];                    // keys 0-7 and 8-15 of chunk c, then of c + 1
+        ldmatrix4(k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), c + (mi >> 1)), r);
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      if (FP8) {
+        for (int u = 0; u < 2; ++u) {
+          if ((c + u) * 16 >= D) break;
+          uint32_t a0, a1, a2, a3;
+          widen4(r[2 * u], a0, a2);
+          widen4(r[2 * u + 1], a1, a3);
 #pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-          if (c * 16 >= D) break;
-          uint32_t r[4];                    // keys 0-7 and 8-15 of chunk c, then of c + 1
-          ldmatrix4(k_s + chunk_offset<CH>(kt * 16 + mr + ((mi & 1) << 3), c + (mi >> 1)), r);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if ((c + u) * 16 >= D) break;
-            uint32_t a0, a1, a2, a3;
-            widen4(r[2 * u], a0, a2);
-            widen4(r[2 * u + 1], a1, a3);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<false>(s[n][kt], a0, a1, a2, a3, qb[n][c + u][0], qb[n][c + u][1]);
-          }
+          for (int n = 0; n < NT; ++n) mma16816<false>(s[n], a0, a1, a2, a3, qb[n][c + u][0], qb[n][c + u][1]);
         }
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          if (kk * 16 >= D) break;
-          uint32_t r[4];                    // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
-          ldmatrix4(k_s + chunk_offset<CH>(kt * 16 + mr + ((mi & 1) << 3), 2 * kk + (mi >> 1)), r);
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        if (kk * 16 >= D) break;
+        uint32_t r[4];                    // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
+        ldmatrix4(k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), 2 * kk + (mi >> 1)), r);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<MMA_BF16>(s[n][kt], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
-        }
+        for (int n = 0; n < NT; ++n) mma16816<MMA_BF16>(s[n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
       }
     }
     // Scores in log2 units; padded keys -inf.
-    float w[KT][2];                         // value exponents
+    float w[2];                             // value exponents
     bool grow = false;
-    const bool padded = k0 + L::kStep > n_keys;
+    const bool padded = k0 + kStep > n_keys;
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
-        const int32_t key = k0 + kt * 16 + kh * 8 + g;
-        float2 f = make_float2(1.f, 0.f);
-        if (FP8) f = scale_s[!padded || key < n_keys ? key : 0];
-        w[kt][kh] = f.y;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& v = s[n][kt][2 * kh + h];
-            v *= row_scale[n][h];
-            if (FP8) v *= f.x;
-            if (padded && key >= n_keys) v = -INFINITY;
-            // a NaN score counts as growth: it has to reach the reference
-            grow = grow || !(v <= m[n][h] + kRescale) || (FP8 && !(v + f.y <= mw[n][h] + kRescale));
-          }
+    for (int kh = 0; kh < 2; ++kh) {
+      const int32_t key = k0 + kh * 8 + g;
+      float2 f = make_float2(1.f, 0.f);   // the key's power of two, the value's exponent
+      if (FP8) {
+        const uint32_t e = exp_s[!padded || key < n_keys ? key : 0];
+        // a byte below 2^23's mantissa is that number above it
+        f = make_float2(__uint_as_float((e & 0xffu) << 23), __uint_as_float(0x4b000000u | (e >> 8)) - 8388735.f);
       }
+      w[kh] = f.y;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float& v = s[n][2 * kh + h];
+          v *= row_scale[n][h];
+          if (FP8) v *= f.x;
+          if (padded && key >= n_keys) v = -INFINITY;
+          // a NaN score counts as growth: it has to reach the reference
+          grow = grow || !(v <= m[n][h] + kRescale) || (FP8 && !(v + f.y <= mw[n][h] + kRescale));
+        }
+    }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -353,12 +351,10 @@ xattn_rows_kernel(const RowsArgs a) {
         for (int h = 0; h < 2; ++h) {
           float top = m[n][h], topw = mw[n][h];
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh) {
-              top = max_nan(top, s[n][kt][2 * kh + h]);
-              if (FP8) topw = max_nan(topw, s[n][kt][2 * kh + h] + w[kt][kh]);
-            }
+          for (int kh = 0; kh < 2; ++kh) {
+            top = max_nan(top, s[n][2 * kh + h]);
+            if (FP8) topw = max_nan(topw, s[n][2 * kh + h] + w[kh]);
+          }
           top = keys_max(top);
           topw = FP8 ? keys_max(topw) : top;
           l[n][h] *= top == -INFINITY ? 1.f : fast_exp2(m[n][h] - top);
@@ -372,53 +368,48 @@ xattn_rows_kernel(const RowsArgs a) {
           for (int e = 0; e < 4; ++e) o[n][c][e] *= fo[e & 1];
       }
     }
-    uint32_t pb[NT][KT][2];                 // P^T as the 8-wide operand: keys 2t, 2t+1 of each 8, row g
+    uint32_t pb[NT][2];                     // P^T as the 8-wide operand: keys 2t, 2t+1 of each 8, row g
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       // A row without a score above -inf keeps 0 as its reference.
       const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
       const float refw[2] = {mw[n][0] == -INFINITY ? 0.f : mw[n][0], mw[n][1] == -INFINITY ? 0.f : mw[n][1]};
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+      for (int kh = 0; kh < 2; ++kh) {
+        float pr[2];
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          float pr[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float v = s[n][kt][2 * kh + h];
-            pr[h] = fast_exp2(v - ref[h]);
-            l[n][h] += pr[h];
-            if (FP8) pr[h] = fast_exp2(v + w[kt][kh] - refw[h]);
-          }
-          pb[n][kt][kh] = transpose8(pack2<MMA_BF16>(pr[0], pr[1]));
+        for (int h = 0; h < 2; ++h) {
+          const float v = s[n][2 * kh + h];
+          pr[h] = fast_exp2(v - ref[h]);
+          l[n][h] += pr[h];
+          if (FP8) pr[h] = fast_exp2(v + w[kh] - refw[h]);
         }
+        pb[n][kh] = transpose8(pack2<MMA_BF16>(pr[0], pr[1]));
+      }
     }
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
+    for (int c = 0; c < CH; c += 2) {
+      if (c * L::kPerChunk >= D) break;
+      uint32_t r[4];
+      if (FP8) {
+        // keys 0-7 and 8-15 of chunk c, then of c + 1: two columns of two keys each
+        ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi & 1) << 3), c + (mi >> 1)), r);
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        if (c * L::kPerChunk >= D) break;
-        uint32_t r[4];
-        if (FP8) {
-          // keys 0-7 and 8-15 of chunk c, then of c + 1: two columns of two keys each
-          ldmatrix4_trans(v_s + chunk_offset<CH>(kt * 16 + mr + ((mi & 1) << 3), c + (mi >> 1)), r);
+        for (int u = 0; u < 2; ++u) {
+          if ((c + u) * 16 >= D) break;
+          // -> key pairs of the even, then of the odd column
+          uint32_t a0, a1, a2, a3;
+          widen4(__byte_perm(r[2 * u], 0u, 0x3120), a0, a1);
+          widen4(__byte_perm(r[2 * u + 1], 0u, 0x3120), a2, a3);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if ((c + u) * 16 >= D) break;
-            // -> key pairs of the even, then of the odd column
-            uint32_t a0, a1, a2, a3;
-            widen4(__byte_perm(r[2 * u], 0u, 0x3120), a0, a1);
-            widen4(__byte_perm(r[2 * u + 1], 0u, 0x3120), a2, a3);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<false>(o[n][c + u], a0, a1, a2, a3, pb[n][kt][0], pb[n][kt][1]);
-          }
-        } else {
-          // chunk c and c + 1 of keys 0-7, then of 8-15
-          ldmatrix4_trans(v_s + chunk_offset<CH>(kt * 16 + mr + ((mi >> 1) << 3), c + (mi & 1)), r);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][kt][0], pb[n][kt][1]);
+          for (int n = 0; n < NT; ++n) mma16816<false>(o[n][c + u], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
+      } else {
+        // chunk c and c + 1 of keys 0-7, then of 8-15
+        ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), c + (mi & 1)), r);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
       }
     }
     __syncwarp();
@@ -544,10 +535,10 @@ int32_t launch(RowsArgs a, cudaStream_t stream) {
   auto kernel = xattn_rows_kernel<DP, BF16, FP8, NT>;
   constexpr int kJoin = kWarps * 8 * NT * (DP + 4) * 4;   // the warps' sums, in the rings' place
   constexpr int kData = L::kRing > kJoin ? L::kRing : kJoin;
-  constexpr int kMost = kData + (FP8 ? 8 * kXaRowsKeys8 : 0);
+  constexpr int kMost = kData + (FP8 ? 2 * kXaRowsKeys8 : 0);
   static_assert(kMost <= 227 * 1024, "shared memory of a CTA");
   a.smem_scales = kData;
-  const int smem = kData + (FP8 ? 8 * a.p.split_keys : 0);
+  const int smem = kData + (FP8 ? 2 * a.p.split_keys : 0);
   static std::atomic<uint64_t> done{0};
   if (smem > kMost) return 8;
   if (!allow_smem(kernel, kMost, done)) return 6;

@@ -5,15 +5,15 @@
 // largest value).  A power of two loses nothing that e4m3 keeps: the codes' own three
 // mantissa bits bound the error (2^-4 relative for normal codes), and code * 2^e is exact
 // in bf16 and fp32.
-// Bound by memory: one pass, 16-byte loads, 8-byte code stores.  LPR = D / 8 lanes (rounded
-// to a power of two) hold a row, so its maximum is a few shuffles; each lane group takes
-// kUnroll rows at once to keep loads in flight.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+// Bound by memory: one pass, 32-byte loads and 16-byte code stores a lane.  A lane holds 16
+// values, LPR lanes (D / 16, rounded to a power of two) a row, so its maximum is a few shuffles
+// of 16-bit integers (magnitudes order like their bits); each lane group takes kUnroll rows at
+// once to keep loads in flight.
 #include <cstdint>
 #include <cstring>
 #include "../../include/intp_b200.h"
-#include "sm100_ptx.cuh"
+#include "xattn_common.cuh"
+#include "xattn_internal.h"
 
 namespace intp {
 namespace {
@@ -31,28 +31,25 @@ struct CacheArgs {
 };
 
 struct RowAt {
-  int32_t which, b, g, i;
+  uint16_t* x;                           // the row's 16-bit values
   int64_t cache;                         // cache row, or -1 outside it / past the sequence's count
+  int32_t which;
 };
 
 __device__ __forceinline__ RowAt row_at(const CacheArgs& a, int64_t row) {
   RowAt r;
   r.which = row >= a.n_rows ? 1 : 0;
-  uint32_t x = static_cast<uint32_t>(row - (r.which ? a.n_rows : 0));  // n_rows < 2^31 (checked on the host)
+  const uint32_t x = static_cast<uint32_t>(row - (r.which ? a.n_rows : 0));  // n_rows < 2^31 (checked on the host)
   const uint32_t bg = x / static_cast<uint32_t>(a.count);
-  r.i = static_cast<int32_t>(x - bg * a.count);
-  r.b = static_cast<int32_t>(bg / a.groups);
-  r.g = static_cast<int32_t>(bg - r.b * a.groups);
-  const int64_t at = (a.start == nullptr ? 0 : static_cast<int64_t>(a.start[r.b])) + r.i;
-  const bool in = at >= 0 && at < a.capacity && (a.counts == nullptr || r.i < a.counts[r.b]);
-  r.cache = in ? (static_cast<int64_t>(r.b) * a.groups + r.g) * a.capacity + at : -1;
+  const int32_t i = static_cast<int32_t>(x - bg * a.count);
+  const int32_t b = static_cast<int32_t>(bg / static_cast<uint32_t>(a.groups));
+  const int32_t g = static_cast<int32_t>(bg - b * a.groups);
+  const int64_t at = (a.start == nullptr ? 0 : static_cast<int64_t>(a.start[b])) + i;
+  const bool in = at >= 0 && at < a.capacity && (a.counts == nullptr || i < a.counts[b]);
+  r.cache = in ? static_cast<int64_t>(bg) * a.capacity + at : -1;
+  const int64_t* s = a.xs[r.which];
+  r.x = static_cast<uint16_t*>(a.x[r.which]) + b * s[0] + g * s[1] + i * s[2];
   return r;
-}
-
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
 // The smallest e >= -126 with amax <= 448 * 2^e (448 = 1.75 * 2^8), 0 for amax = 0.
@@ -70,115 +67,126 @@ template <int LPR, bool BF16>
 __global__ void __launch_bounds__(kThreads)
 cache_write_kernel(const CacheArgs a) {
   constexpr int kRowsPer = kThreads / LPR;
+  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;     // bits of infinity: magnitudes at or above are not finite
   const int sub = threadIdx.x % LPR;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * kUnroll) * kRowsPer + threadIdx.x / LPR;
-  const bool col = sub * 8 < a.head_dim;
+  const bool col = sub * 16 < a.head_dim;
   RowAt at[kUnroll];
-  uint4 v[kUnroll];
+  uint4 v[kUnroll][2];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const int64_t row = first + u * kRowsPer;
     at[u].cache = -1;
-    v[u] = make_uint4(0u, 0u, 0u, 0u);
+    v[u][0] = v[u][1] = make_uint4(0u, 0u, 0u, 0u);
     if (row < 2 * a.n_rows) {
       at[u] = row_at(a, row);
       if (col && at[u].cache >= 0) {
-        const int64_t* s = a.xs[at[u].which];
-        v[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x[at[u].which]) + at[u].b * s[0] +
-                                                    at[u].g * s[1] + at[u].i * s[2] + sub * 8));
+        const uint4* src = reinterpret_cast<const uint4*>(at[u].x + sub * 16);
+        v[u][0] = __ldcs(src);
+        v[u][1] = __ldcs(src + 1);
       }
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-    float f[8];
-    float amax = 0.f;
+    uint32_t w[8] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w, v[u][1].x, v[u][1].y, v[u][1].z, v[u][1].w};
+    uint32_t top = 0u;                   // two running maxima of magnitude bits
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 p = unpack2<BF16>(w[e]);
-      f[2 * e] = p.x;
-      f[2 * e + 1] = p.y;
+    for (int e = 0; e < 8; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+    if ((top & 0xffffu) >= kInf || (top >> 16) >= kInf) {
+      // Not finite: such values do not count and become NaN (e4m3 has no infinity).
+      top = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if ((w[e] & 0x7fffu) >= kInf) w[e] |= 0x7fffu;
+        else top = __vmaxu2(top, w[e] & 0x7fffu);
+        if (((w[e] >> 16) & 0x7fffu) >= kInf) w[e] |= 0x7fff0000u;
+        else top = __vmaxu2(top, w[e] & 0x7fff0000u);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float m = fabsf(f[e]);
-      if (m < INFINITY)
-        amax = fmaxf(amax, m);
-      else
-        f[e] = __uint_as_float(0x7fffffffu);  // e4m3 has no infinity: infinities and NaN are its NaN
-    }
-#pragma unroll
-    for (int s = LPR / 2; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
-    const int32_t e = row_exponent(amax);
+    for (int s = LPR / 2; s > 0; s >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float2 pair = unpack2<BF16>(top);
+    const int32_t e = row_exponent(fmaxf(pair.x, pair.y));
     const float down = power_of_two(-e);
-    uint32_t codes[2];
+    uint32_t codes[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 4; ++h) {
       uint32_t c[2];
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+      for (int q = 0; q < 2; ++q) {
+        const float2 f = mul2(unpack2<BF16>(w[2 * h + q]), make_float2(down, down));
         asm("{\n\t.reg .b16 h;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %1, %2;\n\tcvt.u32.u16 %0, h;\n\t}"
             : "=r"(c[q])
-            : "f"(f[4 * h + 2 * q + 1] * down), "f"(f[4 * h + 2 * q] * down));
-      codes[h] = c[0] | (c[1] << 16);
+            : "f"(f.y), "f"(f.x));
+      }
+      codes[h] = __byte_perm(c[0], c[1], 0x5410);
     }
     if (at[u].cache >= 0 && col) {
-      *reinterpret_cast<uint2*>(a.codes[at[u].which] + at[u].cache * a.head_dim + sub * 8) =
-          make_uint2(codes[0], codes[1]);
+      __stcs(reinterpret_cast<uint4*>(a.codes[at[u].which] + at[u].cache * a.head_dim + sub * 16),
+             make_uint4(codes[0], codes[1], codes[2], codes[3]));
       if (sub == 0) a.exps[at[u].which][at[u].cache] = static_cast<uint8_t>(e + 127);
     }
   }
 }
 
-// Two codes times 2^e, rounded to the output type; values past its range (a row's largest
-// may have been rounded up) become its largest finite value.
+// Four codes times 2^e, rounded to the output type.  With `clamp`, values past its range (a
+// row's largest may have been rounded up) become its largest finite value.
 template <bool BF16>
-__device__ __forceinline__ uint32_t decode2(uint32_t codes, float up) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(h) : "r"(codes & 0xffffu));
-  float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  f.x *= up;
-  f.y *= up;
-  const float top = BF16 ? __uint_as_float(0x7f7f0000u) : 65504.f;
-  if (f.x == f.x) f.x = fminf(fmaxf(f.x, -top), top);
-  if (f.y == f.y) f.y = fminf(fmaxf(f.y, -top), top);
-  return BF16 ? pack_bf16x2(f.x, f.y) : pack_f16x2(f.x, f.y);
+__device__ __forceinline__ uint2 decode4(uint32_t codes, float up, bool clamp) {
+  uint32_t h[2], r[2];
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(h[0]), "=r"(h[1])
+      : "r"(codes));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float2 f = mul2(unpack2<false>(h[i]), make_float2(up, up));
+    if (clamp) {
+      const float top = BF16 ? __uint_as_float(0x7f7f0000u) : 65504.f;
+      if (f.x == f.x) f.x = fminf(fmaxf(f.x, -top), top);
+      if (f.y == f.y) f.y = fminf(fmaxf(f.y, -top), top);
+    }
+    r[i] = pack2<BF16>(f.x, f.y);
+  }
+  return make_uint2(r[0], r[1]);
 }
 
 template <int LPR, bool BF16>
 __global__ void __launch_bounds__(kThreads)
 cache_read_kernel(const CacheArgs a) {
   constexpr int kRowsPer = kThreads / LPR;
+  constexpr int32_t kSafe = BF16 ? 119 : 7;   // 448 * 2^e is within the type
   const int sub = threadIdx.x % LPR;
-  if (sub * 8 >= a.head_dim) return;
+  if (sub * 16 >= a.head_dim) return;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * kUnroll) * kRowsPer + threadIdx.x / LPR;
   RowAt at[kUnroll];
-  uint2 c[kUnroll];
-  uint32_t e[kUnroll];
+  uint4 c[kUnroll];
+  int32_t e[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const int64_t row = first + u * kRowsPer;
     at[u].cache = -1;
-    c[u] = make_uint2(0u, 0u);
-    e[u] = 127u;
+    c[u] = make_uint4(0u, 0u, 0u, 0u);
+    e[u] = 0;
     if (row < 2 * a.n_rows) {
       at[u] = row_at(a, row);
       if (at[u].cache >= 0) {
-        c[u] = __ldg(reinterpret_cast<const uint2*>(a.codes[at[u].which] + at[u].cache * a.head_dim + sub * 8));
-        e[u] = __ldg(a.exps[at[u].which] + at[u].cache);
+        c[u] = __ldg(reinterpret_cast<const uint4*>(a.codes[at[u].which] + at[u].cache * a.head_dim + sub * 16));
+        e[u] = static_cast<int32_t>(__ldg(a.exps[at[u].which] + at[u].cache)) - 127;
       }
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     if (first + u * kRowsPer >= 2 * a.n_rows) continue;
-    const float up = power_of_two(static_cast<int32_t>(e[u]) - 127);
-    const int64_t* s = a.xs[at[u].which];
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.x[at[u].which]) + at[u].b * s[0] + at[u].g * s[1] +
-                              at[u].i * s[2] + sub * 8) =
-        make_uint4(decode2<BF16>(c[u].x, up), decode2<BF16>(c[u].x >> 16, up), decode2<BF16>(c[u].y, up),
-                   decode2<BF16>(c[u].y >> 16, up));
+    const float up = power_of_two(e[u]);
+    const bool clamp = e[u] > kSafe;
+    const uint2 r0 = decode4<BF16>(c[u].x, up, clamp), r1 = decode4<BF16>(c[u].y, up, clamp);
+    const uint2 r2 = decode4<BF16>(c[u].z, up, clamp), r3 = decode4<BF16>(c[u].w, up, clamp);
+    uint4* dst = reinterpret_cast<uint4*>(at[u].x + sub * 16);
+    __stcs(dst, make_uint4(r0.x, r0.y, r1.x, r1.y));
+    __stcs(dst + 1, make_uint4(r2.x, r2.y, r3.x, r3.y));
   }
 }
 
@@ -215,11 +223,9 @@ int32_t run(const state_cache_args* c, bool write, cudaStream_t stream) {
   if (!row_layout_ok(c->k, c->k_stride, extent) || !row_layout_ok(c->v, c->v_stride, extent)) return INTP_ERR_LAYOUT;
   if (reinterpret_cast<uintptr_t>(c->k_codes) % 16 || reinterpret_cast<uintptr_t>(c->v_codes) % 16)
     return INTP_ERR_LAYOUT;
-  int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-    return INTP_ERR_LAUNCH;
-  if (major != 10) return INTP_ERR_ARCH;
+  int sms = 0;
+  const int32_t device = current_device_facts(&sms);
+  if (device != INTP_OK) return device;
   CacheArgs a;
   a.batch = static_cast<int32_t>(c->batch);
   a.groups = static_cast<int32_t>(c->groups);
@@ -238,9 +244,9 @@ int32_t run(const state_cache_args* c, bool write, cudaStream_t stream) {
   a.start = c->start;
   a.counts = c->counts;
   const bool bf16 = c->dtype == INTP_BF16;
-  if (a.head_dim <= 32) return bf16 ? launch<4, true>(a, write, stream) : launch<4, false>(a, write, stream);
-  if (a.head_dim <= 64) return bf16 ? launch<8, true>(a, write, stream) : launch<8, false>(a, write, stream);
-  return bf16 ? launch<16, true>(a, write, stream) : launch<16, false>(a, write, stream);
+  if (a.head_dim <= 32) return bf16 ? launch<2, true>(a, write, stream) : launch<2, false>(a, write, stream);
+  if (a.head_dim <= 64) return bf16 ? launch<4, true>(a, write, stream) : launch<4, false>(a, write, stream);
+  return bf16 ? launch<8, true>(a, write, stream) : launch<8, false>(a, write, stream);
 }
 
 }  // namespace

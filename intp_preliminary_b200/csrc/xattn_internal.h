@@ -48,6 +48,9 @@ struct XaBwdParams {
   float* dk_part; float* dv_part; int32_t kv_split, kv_split_tiles;
 };
 
+// SMs of the current device, asked for once; an error status where it is not sm_100.
+int32_t current_device_facts(int* sms);
+
 // Raises a kernel's dynamic shared memory limit, once per device (`done` is the kernel's own).
 template <class K>
 inline bool allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {

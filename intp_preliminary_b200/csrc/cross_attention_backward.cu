@@ -6,10 +6,10 @@
 // Nothing of size M x N is written: two kernels recompute the score tiles.
 //   xattn_stats_kernel   lse in log2 units and delta of every query row, rows padded
 //                        to whole tiles so that a tile's values are one bulk copy.
-//   xattn_dq_kernel      a CTA owns 128 query rows of a head and streams 64-key tiles:
+//   dq kernel            an item owns 128 query rows of a head and streams 64-key tiles:
 //                        X = q k^T and Y = dO v^T into TMEM, dS (16-bit) back over X,
 //                        dq += dS k with dS read from TMEM.
-//   xattn_dkv_kernel     a CTA owns 128 keys of a key head and streams 64-query tiles of
+//   dk / dv kernel       an item owns 128 keys of a key head and streams 64-query tiles of
 //                        all its query heads: X = k q^T, Y = v dO^T, P^T over X and dS^T
 //                        over Y, dv += P^T dO and dk += dS^T q.  Grouped heads are summed
 //                        in the accumulators, in a fixed order.
@@ -17,11 +17,16 @@
 // parts are summed in order (xattn_sum_kernel).  Every output element has one writer
 // and no atomics are used, so results repeat bit for bit.
 //
-// A CTA: 16 row warps (thread t owns TMEM lane t % 128 and 16 of a tile's 64 columns),
-// a TMA warp and an MMA warp.  Score buffers are double: the products of tile t + 1 run
-// under the row threads' tile t.  Recomputing the scores in both kernels costs 7 matrix
-// products where 5 would do; in exchange dq needs no cross-CTA sum (fp32 atomics in an
-// order that changes results, or a key-length workspace).
+// A CTA (persistent over work items) has 16 row warps (thread t owns TMEM lane t % 128 and 16
+// of a tile's 64 columns), a TMA warp and an MMA warp.  Score buffers are double: the products
+// of tile t + 1 run under the row threads' tile t, and the next item's first score product runs
+// under this one's epilogue.  A 128 x 64 x 16 product reads 6 KB of shared memory where both
+// operands lie there (48 cycles) and 2 KB with the owned operand in TMEM (32 cycles, the
+// tensor core's own pace), so the owned rows go to TMEM where it has room: dq, and dk / dv at
+// head_dim <= 64 (two accumulators of 128 columns fill it otherwise).
+// Recomputing the scores in both kernels costs 7 matrix products where 5 would do; in exchange
+// dq needs no cross-CTA sum (fp32 atomics in an order that changes results, or a key-length
+// workspace).
 // P and dS are rounded to 16 bits as the tensor core's operands; all sums are fp32.
 #include <cuda.h>
 #include <cstdint>
@@ -43,22 +48,25 @@ constexpr int kStages = 4;
 constexpr uint32_t kTmemCols = 512, kColAcc = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int DP>
+// DP: head_dim rounded up to 64 or 128.  KV: the dk / dv kernel.
+template <int DP, bool KV>
 struct Shape {
+  static constexpr bool kOwnedInTmem = !KV || DP == 64;
   static constexpr int kBlocks = DP / 64;
-  static constexpr uint32_t kFixedBlock = kRows * 128, kRingBlock = kCols * 128;
-  static constexpr uint32_t kFixed = kBlocks * kFixedBlock;   // one resident operand
+  static constexpr uint32_t kOwnedBlock = kRows * 128, kRingBlock = kCols * 128;
+  static constexpr uint32_t kOwned = kBlocks * kOwnedBlock;   // one owned operand
   static constexpr uint32_t kRing = kBlocks * kRingBlock;     // one streamed operand
-  static constexpr uint32_t kStats = 2 * kCols * 4;           // lse, delta of 64 query rows
-  static constexpr uint32_t fixed0 = 0, fixed1 = kFixed, ring = 2 * kFixed;
+  static constexpr uint32_t kStats = 2 * kCols * 4;           // -lse, -delta of 64 query rows
+  static constexpr uint32_t ring = kOwnedInTmem ? 0 : 2 * kOwned;
   static constexpr uint32_t stats = ring + kStages * 2 * kRing;
   static constexpr uint32_t bars = stats + kStages * kStats;
+  static constexpr uint32_t kColOwned = kColAcc + (KV ? 2 : 1) * DP;   // TMEM: two operands of DP / 2 columns
 };
 
 struct alignas(8) Bars {
-  uint64_t fixed_full;
+  uint64_t owned_full, owned_empty;        // the item's own operands
   uint64_t ring_full[kStages], ring_empty[kStages];
-  uint64_t clean;                          // padded key rows of a K tile zeroed (dq)
+  uint64_t clean[kStages];                 // padded key rows of the K tile in a stage zeroed (dq)
   uint64_t s_full[2], ready[2];
   uint64_t acc_full, drain;
   uint32_t tmem_base;
@@ -70,17 +78,39 @@ struct Args {
   MapOrder of0, of1, or0, or1;
   float* stats;                            // [B * H][m_pad / 64][-lse 64 | -delta 64], lse in log2 units
   int32_t m_tiles64;                       // 64-row tiles of a head's queries
-  int32_t n_row_tiles, n_split, split_tiles;
+  int32_t n_row_tiles, n_split, split_tiles, n_items;
   int32_t k_steps;
 };
 
-// What a CTA streams and owns.
+// One work item: what it owns and what it streams.
 struct Work {
   int32_t b, g, h0;          // sequence, key head, first query head (dq: the head itself)
-  int32_t row0;              // first owned row
+  int32_t row0, own;         // first owned row, owned rows
   int32_t t0, n_t;           // streamed tiles [t0, t0 + n_t)
   int32_t length, split;
 };
+
+template <bool KV>
+__device__ __forceinline__ Work decode_work(const Args& a, int32_t item) {
+  const XaParams& p = a.p.f;
+  Work w;
+  const int32_t rest = item / a.n_row_tiles;
+  w.row0 = (item - rest * a.n_row_tiles) * kRows;
+  const int32_t outer = rest / a.n_split, heads = KV ? p.groups : p.heads;
+  w.split = rest - outer * a.n_split;
+  w.b = outer / heads;
+  const int32_t head = outer - w.b * heads;
+  w.g = KV ? head : head / p.per_group;
+  w.h0 = KV ? head * p.per_group : head;
+  w.length = xa_length(p, w.b);
+  w.t0 = w.split * a.split_tiles;
+  const int32_t extent = KV ? p.states : p.queries;
+  w.own = extent - w.row0 < kRows ? extent - w.row0 : kRows;
+  const int32_t total = KV ? (w.row0 < w.length ? p.per_group * a.m_tiles64 : 0) : (w.length + kCols - 1) / kCols;
+  const int32_t left = total - w.t0;
+  w.n_t = left < 0 ? 0 : (left < a.split_tiles ? left : a.split_tiles);
+  return w;
+}
 
 // ============================================================================ row statistics
 // 8 lanes per query row.  Rows past M, and rows without states, get lse = +inf: their P is zero.
@@ -122,14 +152,15 @@ xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
   }
 }
 
-// ============================================================================ shared roles
-__device__ __forceinline__ void init_bars(Bars* bars) {
-  mbar_init(&bars->fixed_full, 1);
+// ============================================================================ roles
+__device__ __forceinline__ void init_bars(Bars* bars, uint32_t owned_arrivals) {
+  mbar_init(&bars->owned_full, owned_arrivals);
+  mbar_init(&bars->owned_empty, 1);
   for (int s = 0; s < kStages; ++s) {
     mbar_init(&bars->ring_full[s], 1);
     mbar_init(&bars->ring_empty[s], 1);
+    mbar_init(&bars->clean[s], 1);
   }
-  mbar_init(&bars->clean, 1);
   for (int s = 0; s < 2; ++s) {
     mbar_init(&bars->s_full[s], 1);
     mbar_init(&bars->ready[s], kRowWarps);
@@ -146,79 +177,105 @@ __device__ __forceinline__ void tma_rows(uint8_t* dst, const CUtensorMap* tm, ui
               map_coord(o, 3, row, head, b));
 }
 
-// Streamed tile t of the CTA: key tile t (dq), or query tile t % m_tiles64 of query head h0 + t / m_tiles64.
+// dq: a padded key tile of a sequence (rows past the tensor's end arrive as zeros by themselves).
+__device__ __forceinline__ bool needs_cleaning(const XaParams& p, const Work& w, int32_t i) {
+  return w.length < p.states && w.length - (w.t0 + i) * kCols < kCols;
+}
+
+// Streamed tile t of an item: key tile t (dq), or query tile t % m_tiles64 of query head h0 + t / m_tiles64.
 template <int DP, bool KV>
 __device__ __forceinline__ void load_role(const CUtensorMap* f0, const CUtensorMap* f1, const CUtensorMap* r0,
-                                          const CUtensorMap* r1, const Args& a, const Work& wk, Bars* bars,
-                                          uint8_t* smem, int lane) {
-  using L = Shape<DP>;
+                                          const CUtensorMap* r1, const Args& a, Bars* bars, uint8_t* smem, int lane) {
+  using L = Shape<DP, KV>;
   const XaParams& p = a.p.f;
   volatile int32_t* abort_flag = &bars->abort;
-  const int32_t fixed_head = KV ? wk.g : wk.h0;
+  auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
+    return warp_wait(bar, phase, abort_flag, p.status, kDevTimeoutProducer, p.wait_ns);
+  };
   if (lane == 0) {
-    tma_prefetch_desc(f0);
-    tma_prefetch_desc(f1);
+    if (!L::kOwnedInTmem) {
+      tma_prefetch_desc(f0);
+      tma_prefetch_desc(f1);
+    }
     tma_prefetch_desc(r0);
     tma_prefetch_desc(r1);
-    mbar_arrive_expect_tx(&bars->fixed_full, 2 * L::kFixed);
-#pragma unroll
-    for (int blk = 0; blk < L::kBlocks; ++blk) {
-      tma_rows(smem + L::fixed0 + blk * L::kFixedBlock, f0, &bars->fixed_full, a.of0, blk * 64, wk.row0, fixed_head, wk.b);
-      tma_rows(smem + L::fixed1 + blk * L::kFixedBlock, f1, &bars->fixed_full, a.of1, blk * 64, wk.row0, fixed_head, wk.b);
-    }
   }
-  int32_t loaded = 0;
-  for (int32_t i = 0; i < wk.n_t; ++i) {
-    const int s = i % kStages;
-    if (i >= kStages && !warp_wait(&bars->ring_empty[s], i / kStages - 1, abort_flag, p.status, kDevTimeoutProducer,
-                                   p.wait_ns))
-      break;
-    uint8_t* r0_s = smem + L::ring + s * 2 * L::kRing;
-    uint8_t* r1_s = r0_s + L::kRing;
-    const int32_t t = wk.t0 + i;
-    const int32_t hq = KV ? t / a.m_tiles64 : 0;
-    const int32_t row = (KV ? t - hq * a.m_tiles64 : t) * kCols, head = KV ? wk.h0 + hq : wk.g;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&bars->ring_full[s], 2 * L::kRing + (KV ? L::kStats : 0));
+  uint32_t tile = 0, items = 0;            // loaded by this CTA
+  bool ok = true;
+  for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
+    const Work wk = decode_work<KV>(a, item);
+    if (wk.n_t == 0) continue;
+    if (!L::kOwnedInTmem) {
+      if (items > 0 && !wait(&bars->owned_empty, items - 1)) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars->owned_full, 2 * L::kOwned);
 #pragma unroll
-      for (int blk = 0; blk < L::kBlocks; ++blk) {
-        tma_rows(r0_s + blk * L::kRingBlock, r0, &bars->ring_full[s], a.or0, blk * 64, row, head, wk.b);
-        tma_rows(r1_s + blk * L::kRingBlock, r1, &bars->ring_full[s], a.or1, blk * 64, row, head, wk.b);
+        for (int blk = 0; blk < L::kBlocks; ++blk) {
+          tma_rows(smem + blk * L::kOwnedBlock, f0, &bars->owned_full, a.of0, blk * 64, wk.row0, wk.g, wk.b);
+          tma_rows(smem + L::kOwned + blk * L::kOwnedBlock, f1, &bars->owned_full, a.of1, blk * 64, wk.row0, wk.g, wk.b);
+        }
       }
-      if (KV)
-        bulk_load(smem + L::stats + s * L::kStats,
-                  a.stats + ((static_cast<int64_t>(wk.b) * p.heads + head) * a.m_tiles64 + row / kCols) * (2 * kCols),
-                  L::kStats, &bars->ring_full[s]);
-    }
-    __syncwarp();
-    ++loaded;
-    const int32_t valid = wk.length - row;
-    if (!KV && valid < kCols && wk.length < p.states) {
-      // dS is zero for padded keys, but 0 * NaN is not: their K rows become zeros.
-      if (!warp_wait(&bars->ring_full[s], i / kStages, abort_flag, p.status, kDevTimeoutProducer, p.wait_ns)) break;
-      for (int c = valid * 8 + lane; c < kCols * 8; c += 32)
-#pragma unroll
-        for (int blk = 0; blk < L::kBlocks; ++blk)
-          reinterpret_cast<uint4*>(r0_s + blk * L::kRingBlock)[c] = make_uint4(0u, 0u, 0u, 0u);
-      fence_proxy_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->clean);
+      ++items;
+    }
+    for (int32_t i = 0; i < wk.n_t; ++i) {
+      const uint32_t s = tile % kStages;
+      if (tile >= kStages && !wait(&bars->ring_empty[s], tile / kStages - 1)) {
+        ok = false;
+        break;
+      }
+      uint8_t* r0_s = smem + L::ring + s * 2 * L::kRing;
+      uint8_t* r1_s = r0_s + L::kRing;
+      const int32_t t = wk.t0 + i;
+      const int32_t hq = KV ? t / a.m_tiles64 : 0;
+      const int32_t row = (KV ? t - hq * a.m_tiles64 : t) * kCols, head = KV ? wk.h0 + hq : wk.g;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars->ring_full[s], 2 * L::kRing + (KV ? L::kStats : 0));
+#pragma unroll
+        for (int blk = 0; blk < L::kBlocks; ++blk) {
+          tma_rows(r0_s + blk * L::kRingBlock, r0, &bars->ring_full[s], a.or0, blk * 64, row, head, wk.b);
+          tma_rows(r1_s + blk * L::kRingBlock, r1, &bars->ring_full[s], a.or1, blk * 64, row, head, wk.b);
+        }
+        if (KV)
+          bulk_load(smem + L::stats + s * L::kStats,
+                    a.stats + ((static_cast<int64_t>(wk.b) * p.heads + head) * a.m_tiles64 + row / kCols) * (2 * kCols),
+                    L::kStats, &bars->ring_full[s]);
+      }
+      __syncwarp();
+      ++tile;
+      if (!KV && needs_cleaning(p, wk, i)) {
+        // dS is zero for padded keys, but 0 * NaN is not: their K rows become zeros.
+        if (!wait(&bars->ring_full[s], (tile - 1) / kStages)) {
+          ok = false;
+          break;
+        }
+        for (int c = (wk.length - row) * 8 + lane; c < kCols * 8; c += 32)
+#pragma unroll
+          for (int blk = 0; blk < L::kBlocks; ++blk)
+            reinterpret_cast<uint4*>(r0_s + blk * L::kRingBlock)[c] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->clean[s]);
+      }
     }
   }
   // Every issued copy has landed before the CTA exits.
   volatile int32_t no_abort = 0;
-  mbar_wait(&bars->fixed_full, 0, &no_abort, p.status, kDevTimeoutDrain);
-  for (int s = 0; s < kStages; ++s) {
-    const int32_t cnt = loaded > s ? (loaded - s + kStages - 1) / kStages : 0;
+  if (!L::kOwnedInTmem && items > 0)
+    mbar_wait(&bars->owned_full, (items - 1) & 1, &no_abort, p.status, kDevTimeoutDrain);
+  for (uint32_t s = 0; s < kStages; ++s) {
+    const uint32_t cnt = tile > s ? (tile - s + kStages - 1) / kStages : 0;
     if (cnt > 0) mbar_wait(&bars->ring_full[s], (cnt - 1) & 1, &no_abort, p.status, kDevTimeoutDrain);
   }
 }
 
-// Tile i: X = F0 R0^T, Y = F1 R1^T into buffer i & 1; then, once the row threads have
-// written tile i - 1's operands, dq: acc0 += X R0;  dk, dv: acc1 += X R1, acc0 += Y R0.
+// Tile i: X = F0 R0^T, Y = F1 R1^T (F0, F1 owned, R0, R1 streamed) into the buffer of its parity;
+// once the row threads have written a tile's operands, dq: acc0 += X R0;  dk, dv: acc1 += X R1,
+// acc0 += Y R0.  A buffer is overwritten by products that were issued after those that read it,
+// and products execute in issue order.
 template <int DP, bool BF16, bool KV>
-__device__ __forceinline__ void mma_role(const Args& a, const Work& wk, Bars* bars, uint8_t* smem, uint32_t tmem) {
-  using L = Shape<DP>;
+__device__ __forceinline__ void mma_role(const Args& a, Bars* bars, uint8_t* smem, uint32_t tmem) {
+  using L = Shape<DP, KV>;
   const XaParams& p = a.p.f;
   volatile int32_t* abort_flag = &bars->abort;
   const uint32_t leader = elect_one();
@@ -227,61 +284,117 @@ __device__ __forceinline__ void mma_role(const Args& a, const Work& wk, Bars* ba
   };
   const uint32_t idesc_s = idesc_f16(BF16, false, kRows, kCols);
   const uint32_t idesc_acc = idesc_f16(BF16, true, kRows, a.k_steps * 16);
-  const uint64_t f0 = smem_desc_sw128(smem_u32(smem + L::fixed0), 16, 1024);
-  const uint64_t f1 = smem_desc_sw128(smem_u32(smem + L::fixed1), 16, 1024);
+  const uint64_t f0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
+  const uint64_t f1 = smem_desc_sw128(smem_u32(smem + (L::kOwnedInTmem ? 0 : L::kOwned)), 16, 1024);
   // Streamed operands: K-major for the scores; MN-major for the sums (depth = the tile's
   // 64 rows, N = head_dim in 64-column blocks).
   const uint64_t r_score = smem_desc_sw128(smem_u32(smem + L::ring), 16, 1024);
   const uint64_t r_acc = smem_desc_sw128(smem_u32(smem + L::ring), L::kRingBlock, 1024);
-  bool issued = false;
-  auto acc = [&](int32_t i) -> bool {
-    const uint32_t st = i & 1, s = i % kStages;
-    if (!wait(&bars->ready[st], i >> 1)) return false;
-    tc_fence_after();
-    const uint64_t r0 = r_acc + ((s * 2 * L::kRing) >> 4), r1 = r0 + (L::kRing >> 4);
-    const uint32_t x = tmem + st * 128, y = x + 64;
-#pragma unroll
-    for (int kk = 0; kk < kCols / 16; ++kk)
-      mma_ts_warp(leader, tmem + kColAcc + (KV ? DP : 0), x + kk * kW, (KV ? r1 : r0) + ((kk * 2048) >> 4), idesc_acc,
-                  (i > 0 || kk > 0) ? 1u : 0u);
-    if (KV) {
-#pragma unroll
-      for (int kk = 0; kk < kCols / 16; ++kk)
-        mma_ts_warp(leader, tmem + kColAcc, y + kk * kW, r0 + ((kk * 2048) >> 4), idesc_acc,
-                    (i > 0 || kk > 0) ? 1u : 0u);
+  uint32_t tile = 0, items = 0;            // tiles summed, items begun
+  uint32_t clean_phase = 0;                // bit s: parity of stage s's next cleaned tile
+  bool ok = true, issued = false;
+  // The streamed tile `t` (the item's i-th) has arrived.
+  auto arrived = [&](const Work& wk, uint32_t t, int32_t i) {
+    const uint32_t s = t % kStages;
+    ok = wait(&bars->ring_full[s], t / kStages);
+    if (ok && !KV && needs_cleaning(p, wk, i)) {
+      ok = wait(&bars->clean[s], clean_phase >> s);
+      clean_phase ^= 1u << s;
     }
-    mma_commit_warp(leader, &bars->ring_empty[s]);
-    return true;
   };
-  bool ok = wait(&bars->fixed_full, 0);
-  for (int32_t i = 0; i < wk.n_t && ok; ++i) {
-    const uint32_t st = i & 1, s = i % kStages;
-    ok = wait(&bars->ring_full[s], i / kStages);
-    if (ok && !KV && wk.length - (wk.t0 + i) * kCols < kCols && wk.length < p.states) ok = wait(&bars->clean, 0);
-    if (!ok) break;
-    // Buffer st was read by tile i - 2's sums, issued before: products execute in issue order.
+  auto score = [&](uint32_t t) {
+    const uint32_t st = t & 1, s = t % kStages;
     tc_fence_after();
-    const uint64_t r0 = r_score + ((s * 2 * L::kRing) >> 4), r1 = r0 + (L::kRing >> 4);
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-      if (kk < a.k_steps)
-        mma_ss_warp(leader, tmem + st * 128, f0 + (((kk >> 2) * L::kFixedBlock + (kk & 3) * 32) >> 4),
-                    r0 + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+    for (int y = 0; y < 2; ++y) {
+      const uint64_t r = r_score + ((s * 2 * L::kRing + y * L::kRing) >> 4);
+      const uint32_t d = tmem + st * 128 + y * 64;
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-      if (kk < a.k_steps)
-        mma_ss_warp(leader, tmem + st * 128 + 64, f1 + (((kk >> 2) * L::kFixedBlock + (kk & 3) * 32) >> 4),
-                    r1 + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        if (kk >= a.k_steps) continue;
+        const uint64_t rb = r + (((kk >> 2) * L::kRingBlock + (kk & 3) * 32) >> 4);
+        if (L::kOwnedInTmem)
+          mma_ts_warp(leader, d, tmem + L::kColOwned + y * (DP / 2) + kk * 8, rb, idesc_s, kk > 0 ? 1u : 0u);
+        else
+          mma_ss_warp(leader, d, (y ? f1 : f0) + (((kk >> 2) * L::kOwnedBlock + (kk & 3) * 32) >> 4), rb, idesc_s,
+                      kk > 0 ? 1u : 0u);
+      }
+    }
     mma_commit_warp(leader, &bars->s_full[st]);
     issued = true;
-    if (i >= 1) ok = acc(i - 1);
+  };
+  for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
+    const Work wk = decode_work<KV>(a, item);
+    if (wk.n_t == 0) continue;
+    arrived(wk, tile, 0);
+    if (ok) ok = wait(&bars->owned_full, items);
+    if (!ok) break;
+    ++items;
+    score(tile);
+    if (wk.n_t > 1) arrived(wk, tile + 1, 1);
+    for (int32_t i = 0; i < wk.n_t && ok; ++i, ++tile) {
+      if (i + 1 < wk.n_t)
+        score(tile + 1);
+      else
+        mma_commit_warp(leader, &bars->owned_empty);
+      if (i + 2 < wk.n_t) arrived(wk, tile + 2, i + 2);   // while the products run
+      const uint32_t st = tile & 1, s = tile % kStages;
+      if (ok) ok = wait(&bars->ready[st], tile >> 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t r0 = r_acc + ((s * 2 * L::kRing) >> 4), r1 = r0 + (L::kRing >> 4);
+      const uint32_t x = tmem + st * 128, y = x + 64;
+#pragma unroll
+      for (int kk = 0; kk < kCols / 16; ++kk)
+        mma_ts_warp(leader, tmem + kColAcc + (KV ? DP : 0), x + kk * kW, (KV ? r1 : r0) + ((kk * 2048) >> 4), idesc_acc,
+                    (i > 0 || kk > 0) ? 1u : 0u);
+      if (KV) {
+#pragma unroll
+        for (int kk = 0; kk < kCols / 16; ++kk)
+          mma_ts_warp(leader, tmem + kColAcc, y + kk * kW, r0 + ((kk * 2048) >> 4), idesc_acc,
+                      (i > 0 || kk > 0) ? 1u : 0u);
+      }
+      mma_commit_warp(leader, &bars->ring_empty[s]);
+    }
+    if (ok) mma_commit_warp(leader, &bars->acc_full);
   }
-  if (ok && acc(wk.n_t - 1)) mma_commit_warp(leader, &bars->acc_full);
   if (issued) {
     volatile int32_t no_abort = 0;
     mma_commit_warp(leader, &bars->drain);
     mbar_wait(&bars->drain, 0, &no_abort, p.status, kDevTimeoutDrain);
   }
+}
+
+// The row threads' owned operands on their way to TMEM: this thread's quarter of its row of F0 and F1.
+template <int DP>
+struct OwnedRow {
+  uint4 f[2][DP / 32];
+};
+
+template <int DP>
+__device__ __forceinline__ void fetch_owned(OwnedRow<DP>& o, const uint16_t* f0, const uint16_t* f1, int c0, int32_t head_dim) {
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const uint16_t* src = y ? f1 : f0;
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+      o.f[y][c] = make_uint4(0u, 0u, 0u, 0u);
+      if (src != nullptr && c0 + c * 8 < head_dim) o.f[y][c] = __ldg(reinterpret_cast<const uint4*>(src + c0 + c * 8));
+    }
+  }
+}
+
+template <int DP>
+__device__ __forceinline__ void store_owned(const OwnedRow<DP>& o, uint32_t taddr) {
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    if (DP == 128)
+      tmem_st16(taddr + y * (DP / 2), *reinterpret_cast<const uint32_t(*)[16]>(o.f[y]));
+    else
+      tmem_st8(taddr + y * (DP / 2), *reinterpret_cast<const uint32_t(*)[8]>(o.f[y]));
+  }
+  tmem_wait_st();
+  tc_fence_before();
 }
 
 // This thread's 16 columns of X and Y.
@@ -324,10 +437,10 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int c0, float f, bool 
   }
 }
 
-// A CTA without streamed tiles: zeros for its rows.
+// An item without streamed tiles: zeros for its rows.
 __device__ __forceinline__ void store_zero_rows(int32_t rows, uint16_t* dst, float* part, int32_t head_dim) {
   const int64_t chunks = static_cast<int64_t>(rows) * head_dim / 8;
-  for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) {
+  for (int64_t i = threadIdx.x; i < chunks; i += kRowThreads) {
     if (part != nullptr) {
       reinterpret_cast<float4*>(part)[2 * i] = make_float4(0.f, 0.f, 0.f, 0.f);
       reinterpret_cast<float4*>(part)[2 * i + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -337,12 +450,13 @@ __device__ __forceinline__ void store_zero_rows(int32_t rows, uint16_t* dst, flo
   }
 }
 
-// ============================================================================ dq
-template <int DP, bool BF16>
+// The dq (KV false) and the dk / dv kernel.  Tensor maps f0, f1 of the owned operands (dk / dv
+// at head_dim > 64 only), r0, r1 of the streamed ones.
+template <int DP, bool BF16, bool KV>
 __global__ void __launch_bounds__(kThreads, 1)
-xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a) {
-  using L = Shape<DP>;
+xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_constant__ CUtensorMap tm_f1,
+                  const __grid_constant__ CUtensorMap tm_r0, const __grid_constant__ CUtensorMap tm_r1, const Args a) {
+  using L = Shape<DP, KV>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Bars* bars = reinterpret_cast<Bars*>(smem + L::bars);
@@ -351,30 +465,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int32_t* abort_flag = &bars->abort;
 
-  Work wk;
-  const int32_t rest = blockIdx.x / a.n_row_tiles;
-  wk.row0 = (blockIdx.x - rest * a.n_row_tiles) * kRows;
-  const int32_t bh = rest / a.n_split;
-  wk.split = rest - bh * a.n_split;
-  wk.b = bh / p.heads;
-  wk.h0 = bh - wk.b * p.heads;
-  wk.g = wk.h0 / p.per_group;
-  wk.length = xa_length(p, wk.b);
-  wk.t0 = wk.split * a.split_tiles;
-  const int32_t tiles = (wk.length + kCols - 1) / kCols - wk.t0;
-  wk.n_t = tiles < 0 ? 0 : (tiles < a.split_tiles ? tiles : a.split_tiles);
-
-  const int32_t own = p.queries - wk.row0 < kRows ? p.queries - wk.row0 : kRows;
-  const int64_t lin0 = static_cast<int64_t>(bh) * p.queries + wk.row0;
-  uint16_t* out = static_cast<uint16_t*>(a.p.dq) + lin0 * p.head_dim;
-  float* part = a.p.dq_part == nullptr ? nullptr
-                                       : a.p.dq_part + (wk.split * p.rows_total + lin0) * p.head_dim;
-  if (wk.n_t == 0) {
-    store_zero_rows(own, out, part, p.head_dim);
-    return;
-  }
-
-  if (threadIdx.x == 0) init_bars(bars);
+  if (threadIdx.x == 0) init_bars(bars, L::kOwnedInTmem ? kRowWarps : 1);
   if (warp == kMmaWarp) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
@@ -385,176 +476,147 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
 
   if (warp == kLoadWarp) {
-    load_role<DP, false>(&tm_q, &tm_do, &tm_k, &tm_v, a, wk, bars, smem, lane);
+    load_role<DP, KV>(&tm_f0, &tm_f1, &tm_r0, &tm_r1, a, bars, smem, lane);
   } else if (warp == kMmaWarp) {
-    mma_role<DP, BF16, false>(a, wk, bars, smem, tmem);
-  } else {
-    const int row = threadIdx.x & (kRows - 1), wg = threadIdx.x >> 7;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const float scale_log2 = p.scale * kLog2e;
-    float nlse = -INFINITY, ndelta = 0.f;
-    if (row < own) {
-      const int32_t m = wk.row0 + row;
-      const float* st = a.stats + (static_cast<int64_t>(bh) * a.m_tiles64 + m / kCols) * (2 * kCols) + m % kCols;
-      nlse = __ldg(st);
-      ndelta = __ldg(st + kCols);
-    }
-    const float2 scale2 = make_float2(scale_log2, scale_log2), nlse2 = make_float2(nlse, nlse),
-                 ndelta2 = make_float2(ndelta, ndelta);
-    auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
-      return warp_wait(bar, phase, abort_flag, p.status, kDevTimeoutSoftmax, p.wait_ns);
-    };
-    bool ok = true;
-    for (int32_t i = 0; i < wk.n_t; ++i) {
-      const int st = i & 1;
-      if (!wait(&bars->s_full[st], i >> 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      uint32_t xr[kW], yr[kW], dw[kW / 2];
-      const uint32_t x = lane_base + st * 128 + wg * kW;
-      load_scores(x, xr, yr);
-      const int32_t left = wk.length - (wk.t0 + i) * kCols - wg * kW;  // of this thread's columns
-#pragma unroll
-      for (int e = 0; e < kW; e += 2) {
-        const float2 t = fma2(make_float2(__uint_as_float(xr[e]), __uint_as_float(xr[e + 1])), scale2, nlse2);
-        float2 d = add2(make_float2(__uint_as_float(yr[e]), __uint_as_float(yr[e + 1])), ndelta2);
-        d = mul2(make_float2(fast_exp2(t.x), fast_exp2(t.y)), d);
-        if (e >= left) d.x = 0.f;
-        if (e + 1 >= left) d.y = 0.f;
-        dw[e / 2] = pack2<BF16>(d.x, d.y);
-      }
-      tmem_st8(x, dw);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ready[st]);
-    }
-    if (ok && wait(&bars->acc_full, 0)) {
-      tc_fence_after();
-      store_row<DP, BF16>(lane_base + kColAcc, wg * (DP / 4), p.scale, row < own, false,
-                          out + static_cast<int64_t>(row) * p.head_dim,
-                          part == nullptr ? nullptr : part + static_cast<int64_t>(row) * p.head_dim, p.head_dim);
-      tc_fence_before();
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == kMmaWarp) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
-  }
-}
-
-// ============================================================================ dk, dv
-template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
-xattn_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do, const Args a) {
-  using L = Shape<DP>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  Bars* bars = reinterpret_cast<Bars*>(smem + L::bars);
-  const XaParams& p = a.p.f;
-  // read from lane 0: the compiler then knows the roles' values to be uniform
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  volatile int32_t* abort_flag = &bars->abort;
-
-  Work wk;
-  const int32_t rest = blockIdx.x / a.n_row_tiles;
-  wk.row0 = (blockIdx.x - rest * a.n_row_tiles) * kRows;
-  const int32_t bg = rest / a.n_split;
-  wk.split = rest - bg * a.n_split;
-  wk.b = bg / p.groups;
-  wk.g = bg - wk.b * p.groups;
-  wk.h0 = wk.g * p.per_group;
-  wk.length = xa_length(p, wk.b);
-  wk.t0 = wk.split * a.split_tiles;
-  const int32_t tiles = p.per_group * a.m_tiles64 - wk.t0;
-  wk.n_t = tiles < 0 || wk.row0 >= wk.length ? 0 : (tiles < a.split_tiles ? tiles : a.split_tiles);
-
-  const int32_t own = p.states - wk.row0 < kRows ? p.states - wk.row0 : kRows;
-  const int64_t n_states = static_cast<int64_t>(p.batch) * p.groups * p.states;
-  const int64_t lin0 = static_cast<int64_t>(bg) * p.states + wk.row0;
-  uint16_t* dk = static_cast<uint16_t*>(a.p.dk) + lin0 * p.head_dim;
-  uint16_t* dv = static_cast<uint16_t*>(a.p.dv) + lin0 * p.head_dim;
-  const int64_t at = (wk.split * n_states + lin0) * p.head_dim;
-  float* dk_part = a.p.dk_part == nullptr ? nullptr : a.p.dk_part + at;
-  float* dv_part = a.p.dv_part == nullptr ? nullptr : a.p.dv_part + at;
-  if (wk.n_t == 0) {
-    if (a.p.dk != nullptr) store_zero_rows(own, dk, dk_part, p.head_dim);
-    if (a.p.dv != nullptr) store_zero_rows(own, dv, dv_part, p.head_dim);
-    return;
-  }
-
-  if (threadIdx.x == 0) init_bars(bars);
-  if (warp == kMmaWarp) {
-    tmem_alloc(&bars->tmem_base, kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
-
-  if (warp == kLoadWarp) {
-    load_role<DP, true>(&tm_k, &tm_v, &tm_q, &tm_do, a, wk, bars, smem, lane);
-  } else if (warp == kMmaWarp) {
-    mma_role<DP, BF16, true>(a, wk, bars, smem, tmem);
+    mma_role<DP, BF16, KV>(a, bars, smem, tmem);
   } else {
     const int row = threadIdx.x & (kRows - 1), wg = threadIdx.x >> 7;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
+    const int64_t n_states = static_cast<int64_t>(p.batch) * p.groups * p.states;
     auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
       return warp_wait(bar, phase, abort_flag, p.status, kDevTimeoutSoftmax, p.wait_ns);
     };
+    // The next item with tiles, its owned row and (dq) the row's statistics, fetched one item ahead.
+    OwnedRow<DP> owned;
+    float nlse = -INFINITY, ndelta = 0.f, next_nlse = -INFINITY, next_ndelta = 0.f;
+    auto fetch = [&](int32_t from) -> bool {
+      for (int32_t i = from; i < a.n_items; i += gridDim.x) {
+        const Work w = decode_work<KV>(a, i);
+        if (w.n_t == 0) continue;
+        if (L::kOwnedInTmem) {
+          const uint16_t *f0 = nullptr, *f1 = nullptr;
+          if (row < w.own) {
+            const int64_t r = w.row0 + row;
+            f0 = KV ? static_cast<const uint16_t*>(p.k) + w.b * p.ks[0] + w.g * p.ks[1] + r * p.ks[2]
+                    : static_cast<const uint16_t*>(p.q) + w.b * p.qs[0] + w.h0 * p.qs[1] + r * p.qs[2];
+            f1 = KV ? static_cast<const uint16_t*>(p.v) + w.b * p.vs[0] + w.g * p.vs[1] + r * p.vs[2]
+                    : static_cast<const uint16_t*>(a.p.dout) + w.b * a.p.ds[0] + w.h0 * a.p.ds[1] + r * a.p.ds[2];
+          }
+          fetch_owned<DP>(owned, f0, f1, wg * (DP / 4), p.head_dim);
+        }
+        if (!KV) {
+          next_nlse = -INFINITY;
+          next_ndelta = 0.f;
+          if (row < w.own) {
+            const int32_t m = w.row0 + row;
+            const float* st = a.stats + (static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 + m / kCols) * (2 * kCols) +
+                              m % kCols;
+            next_nlse = __ldg(st);
+            next_ndelta = __ldg(st + kCols);
+          }
+        }
+        return true;
+      }
+      return false;
+    };
+    auto hand_over = [&] {
+      if (L::kOwnedInTmem) {
+        store_owned<DP>(owned, lane_base + L::kColOwned + wg * (DP / 8));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->owned_full);
+      }
+      nlse = next_nlse;
+      ndelta = next_ndelta;
+    };
+    uint32_t tile = 0, items = 0;
     bool ok = true;
-    for (int32_t i = 0; i < wk.n_t; ++i) {
-      const int st = i & 1, s = i % kStages;
-      // The statistics came with the tile that the finished products have read.
-      if (!wait(&bars->ring_full[s], i / kStages) || !wait(&bars->s_full[st], i >> 1)) {
+    if (fetch(blockIdx.x)) hand_over();
+    for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
+      const Work wk = decode_work<KV>(a, item);
+      const int64_t outer = KV ? static_cast<int64_t>(wk.b) * p.groups + wk.g : static_cast<int64_t>(wk.b) * p.heads + wk.h0;
+      const int64_t lin0 = outer * (KV ? p.states : p.queries) + wk.row0;
+      const int64_t at = (wk.split * (KV ? n_states : p.rows_total) + lin0) * p.head_dim;
+      void* const dst[2] = {KV ? a.p.dk : a.p.dq, KV ? a.p.dv : nullptr};
+      float* const parts[2] = {KV ? a.p.dk_part : a.p.dq_part, KV ? a.p.dv_part : nullptr};
+      if (wk.n_t == 0) {
+#pragma unroll
+        for (int y = 0; y < (KV ? 2 : 1); ++y)
+          if (dst[y] != nullptr)
+            store_zero_rows(wk.own, static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim,
+                            parts[y] == nullptr ? nullptr : parts[y] + at, p.head_dim);
+        continue;
+      }
+      const bool more = fetch(item + gridDim.x);
+      const float2 nlse2 = make_float2(nlse, nlse), ndelta2 = make_float2(ndelta, ndelta);
+      for (int32_t i = 0; i < wk.n_t; ++i, ++tile) {
+        const uint32_t st = tile & 1, s = tile % kStages;
+        // The statistics came with the tile that the finished products have read.
+        if ((KV && !wait(&bars->ring_full[s], tile / kStages)) || !wait(&bars->s_full[st], tile >> 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t xr[kW], yr[kW], pw[kW / 2], dw[kW / 2];
+        const uint32_t x = lane_base + st * 128 + wg * kW;
+        load_scores(x, xr, yr);
+        const float4* lse4 = reinterpret_cast<const float4*>(smem + L::stats + s * L::kStats) + wg * (kW / 4);
+        const float4* delta4 = lse4 + kCols / 4;
+#pragma unroll
+        for (int e = 0; e < kW; e += 4) {
+          // dk, dv: a query's statistics are a column's; dq: the thread's own row's
+          float2 nl[2] = {nlse2, nlse2}, nd[2] = {ndelta2, ndelta2};
+          if (KV) {
+            const float4 l = lse4[e / 4], d = delta4[e / 4];
+            nl[0] = make_float2(l.x, l.y);
+            nl[1] = make_float2(l.z, l.w);
+            nd[0] = make_float2(d.x, d.y);
+            nd[1] = make_float2(d.z, d.w);
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int c = e + 2 * u;
+            const float2 t = fma2(make_float2(__uint_as_float(xr[c]), __uint_as_float(xr[c + 1])), scale2, nl[u]);
+            const float2 pr = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+            const float2 g = mul2(pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
+            if (KV) pw[c / 2] = pack2<BF16>(pr.x, pr.y);
+            dw[c / 2] = pack2<BF16>(g.x, g.y);
+          }
+        }
+        if (!KV) {
+          const int32_t left = wk.length - (wk.t0 + i) * kCols - wg * kW;  // of this thread's columns
+          if (left < kW) {
+#pragma unroll
+            for (int c = 0; c < kW / 2; ++c) {
+              if (2 * c >= left) dw[c] = 0u;
+              else if (2 * c + 1 >= left) dw[c] &= 0xffffu;
+            }
+          }
+        }
+        if (KV) tmem_st8(x, pw);               // P^T over the read X columns
+        tmem_st8(KV ? x + 64 : x, dw);         // dS (dk, dv: its transpose over Y)
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ready[st]);
+      }
+      if (!ok) break;
+      if (more) hand_over();                   // the item's last score product is done
+      if (!wait(&bars->acc_full, items)) {
         ok = false;
         break;
       }
+      ++items;
       tc_fence_after();
-      uint32_t xr[kW], yr[kW], pw[kW / 2], dw[kW / 2];
-      const uint32_t x = lane_base + st * 128 + wg * kW;
-      load_scores(x, xr, yr);
-      const float4* lse4 = reinterpret_cast<const float4*>(smem + L::stats + s * L::kStats) + wg * (kW / 4);
-      const float4* delta4 = lse4 + kCols / 4;
-#pragma unroll
-      for (int e = 0; e < kW; e += 4) {
-        const float4 l = lse4[e / 4], d = delta4[e / 4];
-        // the statistics come negated
-        const float2 nl[2] = {make_float2(l.x, l.y), make_float2(l.z, l.w)};
-        const float2 nd[2] = {make_float2(d.x, d.y), make_float2(d.z, d.w)};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int c = e + 2 * u;
-          const float2 t = fma2(make_float2(__uint_as_float(xr[c]), __uint_as_float(xr[c + 1])), scale2, nl[u]);
-          const float2 pr = make_float2(fast_exp2(t.x), fast_exp2(t.y));
-          const float2 g = mul2(pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
-          pw[c / 2] = pack2<BF16>(pr.x, pr.y);
-          dw[c / 2] = pack2<BF16>(g.x, g.y);
-        }
-      }
-      tmem_st8(x, pw);
-      tmem_st8(x + 64, dw);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ready[st]);
-    }
-    if (ok && wait(&bars->acc_full, 0)) {
-      tc_fence_after();
-      // A padded key's row of the accumulators holds whatever its states gave.
-      const bool zero = wk.row0 + row >= wk.length;
+      // A padded key's rows of the accumulators hold whatever its states gave.
+      const bool zero = KV && wk.row0 + row >= wk.length;
       const int64_t off = static_cast<int64_t>(row) * p.head_dim;
-      store_row<DP, BF16>(lane_base + kColAcc, wg * (DP / 4), p.scale, row < own && a.p.dk != nullptr, zero, dk + off,
-                          dk_part == nullptr ? nullptr : dk_part + off, p.head_dim);
-      store_row<DP, BF16>(lane_base + kColAcc + DP, wg * (DP / 4), 1.f, row < own && a.p.dv != nullptr, zero, dv + off,
-                          dv_part == nullptr ? nullptr : dv_part + off, p.head_dim);
+#pragma unroll
+      for (int y = 0; y < (KV ? 2 : 1); ++y)
+        store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / 4), y == 0 ? p.scale : 1.f,
+                            row < wk.own && dst[y] != nullptr, zero,
+                            static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim + off,
+                            parts[y] == nullptr ? nullptr : parts[y] + at + off, p.head_dim);
       tc_fence_before();
     }
   }
@@ -593,12 +655,32 @@ int32_t launch_sum(const float* part, void* dst, int64_t n, int32_t n_split, cud
   return cudaGetLastError() == cudaSuccess ? 0 : 6;
 }
 
-template <int DP, bool BF16>
-int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream) {
-  using L = Shape<DP>;
-  const XaParams& p = bp.f;
-  constexpr int smem = L::bars + sizeof(Bars) + 1024;
+template <int DP, bool BF16, bool KV>
+int32_t launch_grad(const CUtensorMap& f0, const CUtensorMap& f1, const CUtensorMap& r0, const CUtensorMap& r1, Args a,
+                    int sm_count, cudaStream_t stream) {
+  constexpr int smem = Shape<DP, KV>::bars + sizeof(Bars) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+  static_assert(Shape<DP, KV>::kColOwned + (Shape<DP, KV>::kOwnedInTmem ? DP : 0) <= kTmemCols, "tensor memory");
+  const XaParams& p = a.p.f;
+  const int64_t outer = static_cast<int64_t>(p.batch) * (KV ? p.groups : p.heads);
+  a.n_row_tiles = ((KV ? p.states : p.queries) + kRows - 1) / kRows;
+  a.n_split = KV ? a.p.kv_split : a.p.dq_split;
+  a.split_tiles = KV ? a.p.kv_split_tiles : a.p.dq_split_tiles;
+  const int64_t items = outer * a.n_row_tiles * a.n_split;
+  if (items > (1 << 30)) return 8;
+  a.n_items = static_cast<int32_t>(items);
+  auto kernel = xattn_grad_kernel<DP, BF16, KV>;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem(kernel, smem, done)) return 6;
+  // one CTA per SM: it holds all of the SM's tensor memory
+  const unsigned grid = static_cast<unsigned>(items < sm_count ? items : sm_count);
+  kernel<<<grid, kThreads, smem, stream>>>(f0, f1, r0, r1, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : 6;
+}
+
+template <int DP, bool BF16>
+int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
+  const XaParams& p = bp.f;
   Args a;
   a.p = bp;
   a.stats = bp.delta;
@@ -606,6 +688,7 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream) {
   a.k_steps = (p.head_dim + 15) / 16;
 
   const int64_t stat_rows = static_cast<int64_t>(p.batch) * p.heads * a.m_tiles64 * kCols;
+  if (stat_rows / 32 > INT32_MAX) return 8;
   xattn_stats_kernel<BF16><<<static_cast<unsigned>(stat_rows / 32), 256, 0, stream>>>(bp, bp.delta, a.m_tiles64);
   if (cudaGetLastError() != cudaSuccess) return 6;
 
@@ -619,59 +702,38 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream) {
   tk.seq = p.states;
   const int64_t qs[4] = {p.qs[0], p.qs[1], p.qs[2], 1}, ds[4] = {bp.ds[0], bp.ds[1], bp.ds[2], 1};
   const int64_t ks[4] = {p.ks[0], p.ks[1], p.ks[2], 1}, vs[4] = {p.vs[0], p.vs[1], p.vs[2], 1};
-  CUtensorMap f0, f1, r0, r1;
   if (bp.dq != nullptr) {
-    if (!make_map(&f0, &a.of0, p.q, qs, tq, kRows) || !make_map(&f1, &a.of1, bp.dout, ds, tq, kRows) ||
-        !make_map(&r0, &a.or0, p.k, ks, tk, kCols) || !make_map(&r1, &a.or1, p.v, vs, tk, kCols))
-      return 4;
-    a.n_row_tiles = (p.queries + kRows - 1) / kRows;
-    a.n_split = bp.dq_split;
-    a.split_tiles = bp.dq_split_tiles;
-    const int64_t grid = static_cast<int64_t>(p.batch) * p.heads * a.n_row_tiles * a.n_split;
-    if (grid > INT32_MAX) return 8;
-    auto kernel = xattn_dq_kernel<DP, BF16>;
-    static std::atomic<uint64_t> done{0};
-    if (!allow_smem(kernel, smem, done)) return 6;
-    kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(f0, f1, r0, r1, a);
-    if (cudaGetLastError() != cudaSuccess) return 6;
-    if (bp.dq_part != nullptr) {
-      const int32_t st = launch_sum<BF16>(bp.dq_part, bp.dq, p.rows_total * p.head_dim, a.n_split, stream);
-      if (st) return st;
-    }
+    CUtensorMap r0, r1;
+    if (!make_map(&r0, &a.or0, p.k, ks, tk, kCols) || !make_map(&r1, &a.or1, p.v, vs, tk, kCols)) return 4;
+    static_assert(Shape<DP, false>::kOwnedInTmem, "no maps of q and dO");
+    int32_t st = launch_grad<DP, BF16, false>(r0, r1, r0, r1, a, sm_count, stream);
+    if (st == 0 && bp.dq_part != nullptr)
+      st = launch_sum<BF16>(bp.dq_part, bp.dq, p.rows_total * p.head_dim, bp.dq_split, stream);
+    if (st) return st;
   }
   if (bp.dk != nullptr || bp.dv != nullptr) {
-    if (!make_map(&f0, &a.of0, p.k, ks, tk, kRows) || !make_map(&f1, &a.of1, p.v, vs, tk, kRows) ||
-        !make_map(&r0, &a.or0, p.q, qs, tq, kCols) || !make_map(&r1, &a.or1, bp.dout, ds, tq, kCols))
+    CUtensorMap f0, f1, r0, r1;
+    if (!make_map(&r0, &a.or0, p.q, qs, tq, kCols) || !make_map(&r1, &a.or1, bp.dout, ds, tq, kCols)) return 4;
+    f0 = r0;
+    f1 = r1;
+    if (!Shape<DP, true>::kOwnedInTmem &&
+        (!make_map(&f0, &a.of0, p.k, ks, tk, kRows) || !make_map(&f1, &a.of1, p.v, vs, tk, kRows)))
       return 4;
-    a.n_row_tiles = (p.states + kRows - 1) / kRows;
-    a.n_split = bp.kv_split;
-    a.split_tiles = bp.kv_split_tiles;
-    const int64_t grid = static_cast<int64_t>(p.batch) * p.groups * a.n_row_tiles * a.n_split;
-    if (grid > INT32_MAX) return 8;
-    auto kernel = xattn_dkv_kernel<DP, BF16>;
-    static std::atomic<uint64_t> done{0};
-    if (!allow_smem(kernel, smem, done)) return 6;
-    kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(f0, f1, r0, r1, a);
-    if (cudaGetLastError() != cudaSuccess) return 6;
+    int32_t st = launch_grad<DP, BF16, true>(f0, f1, r0, r1, a, sm_count, stream);
     const int64_t n = static_cast<int64_t>(p.batch) * p.groups * p.states * p.head_dim;
-    if (bp.dk_part != nullptr && bp.dk != nullptr) {
-      const int32_t st = launch_sum<BF16>(bp.dk_part, bp.dk, n, a.n_split, stream);
-      if (st) return st;
-    }
-    if (bp.dv_part != nullptr && bp.dv != nullptr) {
-      const int32_t st = launch_sum<BF16>(bp.dv_part, bp.dv, n, a.n_split, stream);
-      if (st) return st;
-    }
+    if (st == 0 && bp.dk_part != nullptr && bp.dk != nullptr) st = launch_sum<BF16>(bp.dk_part, bp.dk, n, bp.kv_split, stream);
+    if (st == 0 && bp.dv_part != nullptr && bp.dv != nullptr) st = launch_sum<BF16>(bp.dv_part, bp.dv, n, bp.kv_split, stream);
+    if (st) return st;
   }
   return 0;
 }
 
 }  // namespace
 
-int32_t launch_xattn_backward(const XaBwdParams& bp, cudaStream_t stream) {
+int32_t launch_xattn_backward(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
   if (bp.f.head_dim <= 64)
-    return bp.f.dtype == 2 ? launch_typed<64, true>(bp, stream) : launch_typed<64, false>(bp, stream);
-  return bp.f.dtype == 2 ? launch_typed<128, true>(bp, stream) : launch_typed<128, false>(bp, stream);
+    return bp.f.dtype == 2 ? launch_typed<64, true>(bp, stream, sm_count) : launch_typed<64, false>(bp, stream, sm_count);
+  return bp.f.dtype == 2 ? launch_typed<128, true>(bp, stream, sm_count) : launch_typed<128, false>(bp, stream, sm_count);
 }
 
 }  // namespace intp

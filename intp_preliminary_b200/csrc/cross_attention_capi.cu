@@ -177,9 +177,10 @@ struct BackwardPlan {
   int32_t dq_split, dq_tiles, kv_split, kv_tiles;
 };
 
-// The streamed axis is split until about two CTAs wait for each SM, four 64-wide tiles a part at least.
-void plan_split(int64_t ctas, int64_t tiles, int32_t* split, int32_t* split_tiles) {
-  const int64_t want = ctas >= kPlanSms ? 1 : std::min(2 * kPlanSms / std::max<int64_t>(ctas, 1), std::max<int64_t>(tiles / 4, 1));
+// The streamed axis is split until every SM has an item, four 64-wide tiles a part at least.
+void plan_split(int64_t items, int64_t tiles, int32_t* split, int32_t* split_tiles) {
+  const int64_t want =
+      items >= kPlanSms ? 1 : std::min(kPlanSms / std::max<int64_t>(items, 1), std::max<int64_t>(tiles / 4, 1));
   *split_tiles = static_cast<int32_t>(std::max<int64_t>(ceil_div(tiles, want), 1));
   *split = static_cast<int32_t>(std::max<int64_t>(ceil_div(tiles, *split_tiles), 1));
 }
@@ -331,7 +332,7 @@ intp_status xattn_backward(const xattn_backward_args* b, void* stream) {
   p.dq_split_tiles = plan.dq_tiles;
   p.kv_split = plan.kv_split;
   p.kv_split_tiles = plan.kv_tiles;
-  return intp::launch_xattn_backward(p, static_cast<cudaStream_t>(stream));
+  return intp::launch_xattn_backward(p, static_cast<cudaStream_t>(stream), sms);
 }
 
 }  // extern "C"

@@ -72,7 +72,7 @@ int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count)
 int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream);
 // Joins n slots of part_o / part_lse into out / lse.
 int32_t launch_xattn_combine(const XaParams& p, int32_t n_slots, cudaStream_t stream);
-int32_t launch_xattn_backward(const XaBwdParams& p, cudaStream_t stream);
+int32_t launch_xattn_backward(const XaBwdParams& p, cudaStream_t stream, int sm_count);
 
 // Row r of instance `inst`: sequence, head and query.
 struct XaRow {

@@ -17,8 +17,8 @@
 // parts are summed in order (xattn_sum_kernel).  Every output element has one writer
 // and no atomics are used, so results repeat bit for bit.
 //
-// A CTA (persistent over work items) has 16 row warps (thread t owns TMEM lane t % 128 and 16
-// of a tile's 64 columns), a TMA warp and an MMA warp.  Score buffers are double: the products
+// A CTA (persistent over work items) has an MMA warp, a TMA warp and 16 row warps (row thread t
+// owns TMEM lane t % 128 and 16 of a tile's 64 columns).  Score buffers are double: the products
 // of tile t + 1 run under the row threads' tile t, and the next item's first score product runs
 // under this one's epilogue.  A 128 x 64 x 16 product reads 6 KB of shared memory where both
 // operands lie there (48 cycles) and 2 KB with the owned operand in TMEM (32 cycles, the
@@ -42,8 +42,9 @@ constexpr int kCols = 64;                  // streamed tile: keys (dq) / query r
 constexpr int kW = 16;                     // columns of a tile per row thread
 constexpr int kRowThreads = kRows * kCols / kW;  // 512
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kLoadWarp = kRowWarps, kMmaWarp = kRowWarps + 1;
-constexpr int kThreads = kRowThreads + 64;
+// The MMA and TMA warps come first, with two idle ones, so that row warp w reaches TMEM lanes 32 (w % 4) ..
+constexpr int kMmaWarp = 0, kLoadWarp = 1, kFirstRowWarp = 4;
+constexpr int kThreads = kFirstRowWarp * 32 + kRowThreads;
 constexpr int kStages = 4;
 constexpr uint32_t kTmemCols = 512, kColAcc = 256;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -337,8 +338,10 @@ __device__ __forceinline__ void mma_role(const Args& a, Bars* bars, uint8_t* sme
         score(tile + 1);
       else
         mma_commit_warp(leader, &bars->owned_empty);
-      if (i + 2 < wk.n_t) arrived(wk, tile + 2, i + 2);   // while the products run
       const uint32_t st = tile & 1, s = tile % kStages;
+      // A wait that is already over costs 60 cycles and more.  The next tile's goes under the
+      // sums, or, where those are short, before the row threads are waited for.
+      if (DP == 64 && i + 2 < wk.n_t) arrived(wk, tile + 2, i + 2);
       if (ok) ok = wait(&bars->ready[st], tile >> 1);
       if (!ok) break;
       tc_fence_after();
@@ -355,6 +358,7 @@ __device__ __forceinline__ void mma_role(const Args& a, Bars* bars, uint8_t* sme
                       (i > 0 || kk > 0) ? 1u : 0u);
       }
       mma_commit_warp(leader, &bars->ring_empty[s]);
+      if (DP != 64 && i + 2 < wk.n_t) arrived(wk, tile + 2, i + 2);
     }
     if (ok) mma_commit_warp(leader, &bars->acc_full);
   }
@@ -438,9 +442,9 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int c0, float f, bool 
 }
 
 // An item without streamed tiles: zeros for its rows.
-__device__ __forceinline__ void store_zero_rows(int32_t rows, uint16_t* dst, float* part, int32_t head_dim) {
+__device__ __forceinline__ void store_zero_rows(int tid, int32_t rows, uint16_t* dst, float* part, int32_t head_dim) {
   const int64_t chunks = static_cast<int64_t>(rows) * head_dim / 8;
-  for (int64_t i = threadIdx.x; i < chunks; i += kRowThreads) {
+  for (int64_t i = tid; i < chunks; i += kRowThreads) {
     if (part != nullptr) {
       reinterpret_cast<float4*>(part)[2 * i] = make_float4(0.f, 0.f, 0.f, 0.f);
       reinterpret_cast<float4*>(part)[2 * i + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -479,8 +483,8 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     load_role<DP, KV>(&tm_f0, &tm_f1, &tm_r0, &tm_r1, a, bars, smem, lane);
   } else if (warp == kMmaWarp) {
     mma_role<DP, BF16, KV>(a, bars, smem, tmem);
-  } else {
-    const int row = threadIdx.x & (kRows - 1), wg = threadIdx.x >> 7;
+  } else if (warp >= kFirstRowWarp) {
+    const int tid = threadIdx.x - kFirstRowWarp * 32, row = tid & (kRows - 1), wg = tid >> 7;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float2 scale2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
     const int64_t n_states = static_cast<int64_t>(p.batch) * p.groups * p.states;
@@ -543,7 +547,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
 #pragma unroll
         for (int y = 0; y < (KV ? 2 : 1); ++y)
           if (dst[y] != nullptr)
-            store_zero_rows(wk.own, static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim,
+            store_zero_rows(tid, wk.own, static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim,
                             parts[y] == nullptr ? nullptr : parts[y] + at, p.head_dim);
         continue;
       }

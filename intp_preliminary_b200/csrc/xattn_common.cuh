@@ -13,9 +13,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatil
   const uint32_t parity = phase & 1;
   if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   const uint64_t start = global_ns();
-  const uint32_t hint = budget_ns < 200000ull ? static_cast<uint32_t>(budget_ns) : 200000u;
+  const bool spin = budget_ns < 2000ull;
   while (true) {
-    const bool done = hint < 2000u ? mbar_test_wait(bar, parity) : mbar_try_wait_sleep(bar, parity, hint);
+    const bool done = spin ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity);
     if (__all_sync(0xffffffffu, done)) return true;
     if (__any_sync(0xffffffffu, *abort != 0)) return false;
     if (__any_sync(0xffffffffu, global_ns() - start > budget_ns)) {

@@ -144,7 +144,9 @@ _MAX_PLANS = 1024
 
 
 class _Plan:
-    __slots__ = ("tail", "scratch", "status", "index", "batch", "device", "empty", "backward_tail")
+    # backward: by the output gradient's strides, (the argument block's end, scratch bytes)
+    __slots__ = ("tail", "scratch", "status", "index", "batch", "device", "empty", "out_shape", "lse_shape", "dtype",
+                 "args", "backward")
 
 
 _plans: dict = {}
@@ -174,26 +176,25 @@ def _set_pair(args, k, v) -> None:
     args.k_stride, args.v_stride = k.stride(), v.stride()
 
 
-def _finish_plan(args, q, what: str, backward=None) -> _Plan:
-    """Scratch size and argument block of a filled ``XattnArgs`` (or of a backward's around it)."""
-    lib = _lib.load()
+def _scratch_bytes(fn, args, what: str) -> int:
     size = ctypes.c_int64()
-    if backward is None:
-        status = lib.xattn_forward_workspace(ctypes.addressof(args), ctypes.byref(size))
-    else:
-        backward.fwd = args
-        status = lib.xattn_backward_workspace(ctypes.addressof(backward), ctypes.byref(size))
+    status = fn(ctypes.addressof(args), ctypes.byref(size))
     if status == _lib.INTP_ERR_UNSUPPORTED:
         raise ValueError(f"{what}: the selected kernel does not take these inputs")
     _lib.check(status, what)
+    return size.value
+
+
+def _finish_plan(args, q, what: str) -> _Plan:
+    """Scratch size and argument block of a filled ``XattnArgs``."""
     plan = _Plan()
-    plan.scratch = size.value
-    plan.device, plan.index, plan.batch = q.device, q.device.index, q.shape[0]
+    plan.scratch = _scratch_bytes(_lib.load().xattn_forward_workspace, args, what)
+    plan.device, plan.index, plan.batch, plan.dtype = q.device, q.device.index, q.shape[0], q.dtype
+    plan.out_shape, plan.lse_shape = q.shape, q.shape[:3]
     plan.status = _status(q.device).data_ptr()
     plan.empty = q.numel() == 0
     plan.tail = bytes(args)[_POINTER_BYTES:]
-    if backward is not None:
-        plan.backward_tail = bytes(backward)[_FORWARD_BYTES + _BACKWARD_POINTERS.size:]
+    plan.args, plan.backward = args, {}
     return plan
 
 
@@ -253,12 +254,8 @@ def _forward_plan(q, k, v, scale, out_stride, kernel):
     return plan
 
 
-def cross_attention_forward(q, k, v, *, scale, lengths=None, want_lse: bool = False, kernel: str = "auto", out=None):
-    """Forward only.  Returns ``(out, lse_or_None)``; ``lse`` ``(B, H, M)`` float32 is
-    the natural log of the row sums (-inf for a row without states).
-
-    ``kernel``: ``"auto"`` chooses by the number of rows that share a key head
-    (``M * H / G``), ``"rows"`` and ``"tiles"`` force one of the two kernels."""
+def _forward(q, k, v, scale, lengths, want_lse: bool, kernel: str, out):
+    """``(out, lse, plan, q, k, v, lengths)``, the last four as the kernels took them."""
     if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
         raise ValueError("cross attention requires CUDA tensors")
     scale = float(scale)
@@ -274,28 +271,54 @@ def cross_attention_forward(q, k, v, *, scale, lengths=None, want_lse: bool = Fa
         q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
         plan = _forward_plan(q, k, v, scale, out_stride, kernel)
         qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    lengths, lengths_p = _lengths_pointer(lengths, plan, "lengths")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=plan.device)
+        out = torch.empty(plan.out_shape, dtype=plan.dtype, device=plan.device)
     lse, lse_p = None, 0
     if want_lse:
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=plan.device)
+        lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=plan.device)
         lse_p = lse.data_ptr()
     _launch(plan, "cross attention", qp, kp, vp, 0, 0, 0, 0, lengths_p, out.data_ptr(), lse_p)
-    return out, lse
+    return out, lse, plan, q, k, v, lengths
 
 
-def _backward_plan(q, k, v, out, grad_out, scale):
-    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.device,
-           k.device, v.device, scale, out.stride(), grad_out.stride())
-    plan = _plans.get(key)
-    if plan is None:
-        args = _base_args(q, scale, out.stride(), "auto")
-        _set_pair(args, k, v)
-        backward = _lib.XattnBackwardArgs()
-        backward.grad_out_stride = grad_out.stride()
-        plan = _keep(key, _finish_plan(args, q, "cross attention backward", backward))
-    return plan
+def cross_attention_forward(q, k, v, *, scale, lengths=None, want_lse: bool = False, kernel: str = "auto", out=None):
+    """Forward only.  Returns ``(out, lse_or_None)``; ``lse`` ``(B, H, M)`` float32 is
+    the natural log of the row sums (-inf for a row without states).
+
+    ``kernel``: ``"auto"`` chooses by the number of rows that share a key head
+    (``M * H / G``), ``"rows"`` and ``"tiles"`` force one of the two kernels."""
+    return _forward(q, k, v, scale, lengths, want_lse, kernel, out)[:2]
+
+
+def _backward(plan: _Plan, q, k, v, lengths, out, lse, grad_out, needs):
+    """The gradients; every tensor but ``grad_out`` as ``_forward`` took or made it."""
+    if plan.empty or not any(needs):
+        return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) if n else None
+                     for t, n in zip((q, k, v), needs))
+    if grad_out.dtype != plan.dtype:
+        grad_out = grad_out.to(plan.dtype)
+    grad_stride = grad_out.stride()
+    known = plan.backward.get(grad_stride)
+    if known is None or grad_out.data_ptr() & 15:
+        grad_out = _laid_out(grad_out)
+        grad_stride = grad_out.stride()
+        args = _lib.XattnBackwardArgs()
+        args.fwd = plan.args
+        args.grad_out_stride = grad_stride
+        scratch = _scratch_bytes(_lib.load().xattn_backward_workspace, args, "cross attention backward")
+        known = plan.backward[grad_stride] = (bytes(args)[_FORWARD_BYTES + _BACKWARD_POINTERS.size:], scratch)
+    end, scratch_bytes = known
+    dq, dk, dv = (torch.empty(t.shape, dtype=plan.dtype, device=plan.device) if n else None
+                  for t, n in zip((q, k, v), needs))
+    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=plan.device)
+    block = _POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, 0,
+                           0 if lengths is None else lengths.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                           scratch.data_ptr(), plan.status, scratch_bytes) + plan.tail
+    block += _BACKWARD_POINTERS.pack(grad_out.data_ptr(), 0 if dq is None else dq.data_ptr(),
+                                     0 if dk is None else dk.data_ptr(), 0 if dv is None else dv.data_ptr()) + end
+    _call(_lib.load().xattn_backward, block, plan.index, "cross attention backward")
+    return dq, dk, dv
 
 
 def cross_attention_backward(q, k, v, out, lse, grad_out, *, scale, lengths=None, needs=(True, True, True)):
@@ -312,26 +335,10 @@ def cross_attention_backward(q, k, v, out, lse, grad_out, *, scale, lengths=None
     if (not isinstance(lse, torch.Tensor) or lse.shape != q.shape[:3] or lse.dtype != torch.float32
             or lse.device != q.device):
         raise ValueError("lse must be the forward's (B, H, M) float32 row sums")
-    device = q.device
-    empty = q.numel() == 0
-    make = torch.zeros if empty else torch.empty
-    dq = make(q.shape, dtype=q.dtype, device=device) if needs[0] else None
-    dk = make(k.shape, dtype=q.dtype, device=device) if needs[1] else None
-    dv = make(v.shape, dtype=q.dtype, device=device) if needs[2] else None
-    if empty or not any(needs):
-        return dq, dk, dv
-    if grad_out.dtype != q.dtype:
-        grad_out = grad_out.to(q.dtype)
     q, k, v, out, lse = _laid_out(q), _laid_out(k), _laid_out(v), _laid_out(out), lse.contiguous()
-    grad_out = _laid_out(grad_out)
-    plan = _backward_plan(q, k, v, out, grad_out, scale)
-    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
-    scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=device)
-    block = _POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, lengths_p, out.data_ptr(),
-                           lse.data_ptr(), scratch.data_ptr(), plan.status, plan.scratch) + plan.tail
-    block += _BACKWARD_POINTERS.pack(grad_out.data_ptr(), *(0 if t is None else t.data_ptr() for t in (dq, dk, dv)))
-    _call(_lib.load().xattn_backward, block + plan.backward_tail, plan.index, "cross attention backward")
-    return dq, dk, dv
+    plan = _forward_plan(q, k, v, scale, out.stride(), "auto")
+    lengths, _ = _lengths_pointer(lengths, plan, "lengths")
+    return _backward(plan, q, k, v, lengths, out, lse, grad_out, needs)
 
 
 class _CrossAttention(torch.autograd.Function):
@@ -339,25 +346,29 @@ class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, scale):
-        out, lse = cross_attention_forward(q, k, v, scale=scale, lengths=lengths, want_lse=True)
-        ctx.scale = scale
+        out, lse, ctx.plan, q, k, v, lengths = _forward(q, k, v, scale, lengths, True, "auto", None)
         ctx.save_for_backward(q, k, v, lengths, out, lse)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
+        if torch.is_grad_enabled():  # create_graph: refuse a second derivative in so many words
+            return _CrossAttention._once(ctx, grad_out)
+        return _CrossAttention._first(ctx, grad_out)
+
+    @staticmethod
+    def _first(ctx, grad_out):
         q, k, v, lengths, out, lse = ctx.saved_tensors
-        dq, dk, dv = cross_attention_backward(q, k, v, out, lse, grad_out, scale=ctx.scale, lengths=lengths,
-                                              needs=ctx.needs_input_grad[:3])
-        return dq, dk, dv, None, None
+        return (*_backward(ctx.plan, q, k, v, lengths, out, lse, grad_out, ctx.needs_input_grad[:3]), None, None)
+
+    _once = staticmethod(once_differentiable(_first))
 
 
 def cross_attention(q, k, v, *, scale, lengths=None):
     """Attention of ``q`` to the states ``k``, ``v`` (see the module's text)."""
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
         return _CrossAttention.apply(q, k, v, lengths, _check_scale(scale))
-    return cross_attention_forward(q, k, v, scale=scale, lengths=lengths)[0]
+    return _forward(q, k, v, scale, lengths, False, "auto", None)[0]
 
 
 def _refuse_grad(what: str, *tensors) -> None:
@@ -436,9 +447,9 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k, v=None, *, scale, lengths=
     exponents = (0, 0)
     if cache is not None and cache.keys.shape[2] > 0:
         exponents = (cache.key_exponents.data_ptr(), cache.value_exponents.data_ptr())
-    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    lengths, lengths_p = _lengths_pointer(lengths, plan, "lengths")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=plan.device)
+        out = torch.empty(plan.out_shape, dtype=plan.dtype, device=plan.device)
     _launch(plan, what, q.data_ptr(), own[0].data_ptr(), own[1].data_ptr(), *exponents, prefix_k.data_ptr(),
             prefix_v.data_ptr(), lengths_p, out.data_ptr(), 0)
     return out

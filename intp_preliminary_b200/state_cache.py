@@ -186,7 +186,7 @@ def cached_cross_attention(q, cache, *, scale, lengths=None, out=None):
     if plan is None or q.data_ptr() & 15:
         q = _laid_out(q)
         plan = _cached_plan(q, cache, scale, out_stride)
-    kept, lengths_p = _lengths_pointer(lengths, plan, "lengths")
+    lengths, lengths_p = _lengths_pointer(lengths, plan, "lengths")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=plan.device)
     _launch(plan, what, q.data_ptr(), cache.keys.data_ptr(), cache.values.data_ptr(), cache.key_exponents.data_ptr(),

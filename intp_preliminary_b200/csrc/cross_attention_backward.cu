@@ -13,8 +13,8 @@
 //                        all its query heads: X = k q^T, Y = v dO^T, P^T over X and dS^T
 //                        over Y, dv += P^T dO and dk += dS^T q.  Grouped heads are summed
 //                        in the accumulators, in a fixed order.
-// Where one side has too few tiles for the GPU, the streamed axis is split and fp32
-// parts are summed in order (xattn_sum_kernel).  Every output element has one writer
+// Where one side has too few tiles for the GPU, the streamed axis is split and fp32 parts
+// are summed in order (xattn_sum_kernel).  Every output element has one writer
 // and no atomics are used, so results repeat bit for bit.
 //
 // A CTA (persistent over work items) has an MMA warp, a TMA warp and 16 row warps (row thread t
@@ -114,42 +114,43 @@ __device__ __forceinline__ Work decode_work(const Args& a, int32_t item) {
 }
 
 // ============================================================================ row statistics
-// 8 lanes per query row.  Rows past M, and rows without states, get lse = +inf: their P is zero.
-template <bool BF16>
+// A block takes 64 rows of one head, D / 8 lanes (rounded to a power of two) a row, every
+// lane's loads in flight at once.  Rows past M, and rows without states, get -lse = -inf:
+// their P is zero.
+template <int LPR, bool BF16>
 __global__ void __launch_bounds__(256)
 xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
+  constexpr int kPerPass = 256 / LPR, kPasses = kCols / kPerPass;
   const XaParams& p = bp.f;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
-  const int sub = threadIdx.x & 7;
-  const int64_t m_pad = static_cast<int64_t>(m_tiles64) * kCols;
-  const int64_t bh = row / m_pad;
-  const int32_t m = static_cast<int32_t>(row - bh * m_pad);
-  float delta = 0.f, lse = INFINITY;
-  if (bh < static_cast<int64_t>(p.batch) * p.heads && m < p.queries) {
-    const int32_t b = static_cast<int32_t>(bh / p.heads), h = static_cast<int32_t>(bh - static_cast<int64_t>(b) * p.heads);
-    const uint4* o = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.out) + b * p.os[0] + h * p.os[1] +
-                                                    m * p.os[2]);
-    const uint4* d = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(bp.dout) + b * bp.ds[0] +
-                                                    h * bp.ds[1] + m * bp.ds[2]);
-    for (int c = sub; c * 8 < p.head_dim; c += 8) {
-      const uint4 x = __ldg(o + c), y = __ldg(d + c);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  const int32_t bh = blockIdx.x / m_tiles64, m0 = (blockIdx.x - bh * m_tiles64) * kCols;
+  const int32_t b = bh / p.heads, h = bh - b * p.heads;
+  const int sub = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
+  const uint16_t* o = static_cast<const uint16_t*>(p.out) + b * p.os[0] + h * p.os[1] + sub * 8;
+  const uint16_t* d = static_cast<const uint16_t*>(bp.dout) + b * bp.ds[0] + h * bp.ds[1] + sub * 8;
+  uint4 x[kPasses], y[kPasses];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 u = unpack2<BF16>(xs[e]), v = unpack2<BF16>(ys[e]);
-        delta = fmaf(u.x, v.x, delta);
-        delta = fmaf(u.y, v.y, delta);
-      }
-    }
-    const float l = p.lse[bh * p.queries + m];
-    lse = l == -INFINITY ? INFINITY : l * kLog2e;
+  for (int i = 0; i < kPasses; ++i) {
+    const int32_t m = m0 + r0 + i * kPerPass;
+    const bool in = m < p.queries && sub * 8 < p.head_dim;
+    x[i] = in ? __ldg(reinterpret_cast<const uint4*>(o + m * p.os[2])) : make_uint4(0u, 0u, 0u, 0u);
+    y[i] = in ? __ldg(reinterpret_cast<const uint4*>(d + m * bp.ds[2])) : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
-  for (int s = 4; s > 0; s >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, s);
-  if (sub == 0 && bh < static_cast<int64_t>(p.batch) * p.heads) {
-    float* dst = stats + (bh * m_tiles64 + m / kCols) * (2 * kCols) + m % kCols;
-    dst[0] = -lse;
-    dst[kCols] = -delta;
+  for (int i = 0; i < kPasses; ++i) {
+    const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = fma2(unpack2<BF16>(xs[e]), unpack2<BF16>(ys[e]), sum);
+    float delta = sum.x + sum.y;
+#pragma unroll
+    for (int s = LPR / 2; s > 0; s >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, s);
+    if (sub == 0) {
+      const int32_t r = r0 + i * kPerPass, m = m0 + r;
+      const float l = m < p.queries ? p.lse[static_cast<int64_t>(bh) * p.queries + m] : -INFINITY;
+      float* dst = stats + static_cast<int64_t>(blockIdx.x) * (2 * kCols) + r;
+      dst[0] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+      dst[kCols] = -delta;
+    }
   }
 }
 
@@ -633,29 +634,31 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
 }
 
 // ============================================================================ split sums
-// dst = round(sum_s part[s]), parts in order; 8 values per thread.
+// dst = round(sum_s part[s]), parts in order; 4 values per thread, up to two sums (blockIdx.y).
 template <bool BF16>
-__global__ void __launch_bounds__(256)
-xattn_sum_kernel(const float* part, uint16_t* dst, int64_t n, int32_t n_split) {
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+__global__ void __launch_bounds__(128)
+xattn_sum_kernel(const float* part0, uint16_t* dst0, const float* part1, uint16_t* dst1, int64_t n, int32_t n_split) {
+  const float* part = blockIdx.y ? part1 : part0;
+  uint16_t* dst = blockIdx.y ? dst1 : dst0;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x) * 4;
   if (i >= n) return;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-#pragma unroll 4
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
   for (int s = 0; s < n_split; ++s) {
-    const float4 x = *reinterpret_cast<const float4*>(part + s * n + i);
-    const float4 y = *reinterpret_cast<const float4*>(part + s * n + i + 4);
+    const float4 x = __ldcs(reinterpret_cast<const float4*>(part + s * n + i));
     a = make_float4(a.x + x.x, a.y + x.y, a.z + x.z, a.w + x.w);
-    b = make_float4(b.x + y.x, b.y + y.y, b.z + y.z, b.w + y.w);
   }
-  *reinterpret_cast<uint4*>(dst + i) =
-      make_uint4(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w), pack2<BF16>(b.x, b.y), pack2<BF16>(b.z, b.w));
+  *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w));
 }
 
+// One sum, or two of equal size (the second null without).
 template <bool BF16>
-int32_t launch_sum(const float* part, void* dst, int64_t n, int32_t n_split, cudaStream_t stream) {
-  const int64_t grid = (n / 8 + 255) / 256;
+int32_t launch_sum(const float* part0, void* dst0, const float* part1, void* dst1, int64_t n, int32_t n_split,
+                   cudaStream_t stream) {
+  const int64_t grid = (n / 4 + 127) / 128;
   if (grid > INT32_MAX) return 8;
-  xattn_sum_kernel<BF16><<<static_cast<unsigned>(grid), 256, 0, stream>>>(part, static_cast<uint16_t*>(dst), n, n_split);
+  xattn_sum_kernel<BF16><<<dim3(static_cast<unsigned>(grid), dst1 != nullptr ? 2 : 1), 128, 0, stream>>>(
+      part0, static_cast<uint16_t*>(dst0), part1, static_cast<uint16_t*>(dst1), n, n_split);
   return cudaGetLastError() == cudaSuccess ? 0 : 6;
 }
 
@@ -691,9 +694,9 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
   a.m_tiles64 = (p.queries + kCols - 1) / kCols;
   a.k_steps = (p.head_dim + 15) / 16;
 
-  const int64_t stat_rows = static_cast<int64_t>(p.batch) * p.heads * a.m_tiles64 * kCols;
-  if (stat_rows / 32 > INT32_MAX) return 8;
-  xattn_stats_kernel<BF16><<<static_cast<unsigned>(stat_rows / 32), 256, 0, stream>>>(bp, bp.delta, a.m_tiles64);
+  const int64_t stat_blocks = static_cast<int64_t>(p.batch) * p.heads * a.m_tiles64;
+  if (stat_blocks > INT32_MAX) return 8;
+  xattn_stats_kernel<DP / 8, BF16><<<static_cast<unsigned>(stat_blocks), 256, 0, stream>>>(bp, bp.delta, a.m_tiles64);
   if (cudaGetLastError() != cudaSuccess) return 6;
 
   SlaParams tq{}, tk{};
@@ -712,7 +715,7 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
     static_assert(Shape<DP, false>::kOwnedInTmem, "no maps of q and dO");
     int32_t st = launch_grad<DP, BF16, false>(r0, r1, r0, r1, a, sm_count, stream);
     if (st == 0 && bp.dq_part != nullptr)
-      st = launch_sum<BF16>(bp.dq_part, bp.dq, p.rows_total * p.head_dim, bp.dq_split, stream);
+      st = launch_sum<BF16>(bp.dq_part, bp.dq, nullptr, nullptr, p.rows_total * p.head_dim, bp.dq_split, stream);
     if (st) return st;
   }
   if (bp.dk != nullptr || bp.dv != nullptr) {
@@ -725,8 +728,12 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
       return 4;
     int32_t st = launch_grad<DP, BF16, true>(f0, f1, r0, r1, a, sm_count, stream);
     const int64_t n = static_cast<int64_t>(p.batch) * p.groups * p.states * p.head_dim;
-    if (st == 0 && bp.dk_part != nullptr && bp.dk != nullptr) st = launch_sum<BF16>(bp.dk_part, bp.dk, n, bp.kv_split, stream);
-    if (st == 0 && bp.dv_part != nullptr && bp.dv != nullptr) st = launch_sum<BF16>(bp.dv_part, bp.dv, n, bp.kv_split, stream);
+    if (st == 0 && bp.dk_part != nullptr) {
+      if (bp.dk != nullptr)
+        st = launch_sum<BF16>(bp.dk_part, bp.dk, bp.dv_part, bp.dv, n, bp.kv_split, stream);
+      else
+        st = launch_sum<BF16>(bp.dv_part, bp.dv, nullptr, nullptr, n, bp.kv_split, stream);
+    }
     if (st) return st;
   }
   return 0;

@@ -492,6 +492,7 @@ xattn_rows_kernel(const RowsArgs a) {
 }
 
 // out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max), one warp per row, parts in order.
+// Lane s holds part s's weight, so the parts' values are loaded without waiting for one another.
 template <bool BF16>
 __global__ void __launch_bounds__(128)
 xattn_combine_kernel(const XaParams p, int32_t n_slots) {
@@ -506,17 +507,25 @@ xattn_combine_kernel(const XaParams p, int32_t n_slots) {
   const int d = lane * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < n_slots; ++s) {
-    const float e = p.part_lse[s * p.rows_total + lin];
-    const float w = e == -INFINITY ? 0.f : fast_exp2(e - top);
-    total += w;
-    if (w != 0.f && d < p.head_dim) {  // an empty part's values were never written
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * p.rows_total + lin) * p.head_dim + d);
-      acc.x = fmaf(v.x, w, acc.x);
-      acc.y = fmaf(v.y, w, acc.y);
-      acc.z = fmaf(v.z, w, acc.z);
-      acc.w = fmaf(v.w, w, acc.w);
+  for (int s0 = 0; s0 < n_slots; s0 += 32) {
+    float mine = 0.f;
+    if (s0 + lane < n_slots) {
+      const float e = p.part_lse[(s0 + lane) * p.rows_total + lin];
+      mine = e == -INFINITY ? 0.f : fast_exp2(e - top);
+    }
+    const int n = n_slots - s0 < 32 ? n_slots - s0 : 32;
+    const float* src = p.part_o + (s0 * p.rows_total + lin) * p.head_dim + d;
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float w = __shfl_sync(0xffffffffu, mine, s);
+      total += w;
+      if (w != 0.f && d < p.head_dim) {  // an empty part's values were never written
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(src + s * p.rows_total * p.head_dim));
+        acc.x = fmaf(v.x, w, acc.x);
+        acc.y = fmaf(v.y, w, acc.y);
+        acc.z = fmaf(v.z, w, acc.z);
+        acc.w = fmaf(v.w, w, acc.w);
+      }
     }
   }
   const float inv = none ? 0.f : 1.f / total;

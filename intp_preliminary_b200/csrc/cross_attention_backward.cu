@@ -81,6 +81,7 @@ struct Args {
   int32_t m_tiles64;                       // 64-row tiles of a head's queries
   int32_t n_row_tiles, n_split, split_tiles, n_items;
   int32_t k_steps;
+  bool wide;                               // gradient rows are 32-byte aligned
 };
 
 // One work item: what it owns and what it streams.
@@ -414,7 +415,7 @@ __device__ __forceinline__ void load_scores(uint32_t x, uint32_t (&xr)[kW], uint
 // Columns [c0, c0 + DP / 4) of an accumulator row, scaled, to a 16-bit or (split) fp32 row.
 template <int DP, bool BF16>
 __device__ __forceinline__ void store_row(uint32_t taddr, int c0, float f, bool write, bool zero, uint16_t* dst,
-                                          float* part, int32_t head_dim) {
+                                          float* part, bool wide, int32_t head_dim) {
 #pragma unroll
   for (int c = 0; c < DP / 4; c += 16) {
     uint32_t r[16];
@@ -424,20 +425,7 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int c0, float f, bool 
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = zero ? 0.f : __uint_as_float(r[e]) * f;
-    if (write) {
-#pragma unroll
-      for (int e = 0; e < 16; e += 8) {
-        if (c0 + c + e >= head_dim) break;
-        if (part != nullptr) {
-          reinterpret_cast<float4*>(part + c0 + c + e)[0] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          reinterpret_cast<float4*>(part + c0 + c + e)[1] = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
-        } else {
-          *reinterpret_cast<uint4*>(dst + c0 + c + e) =
-              make_uint4(pack2<BF16>(v[e], v[e + 1]), pack2<BF16>(v[e + 2], v[e + 3]), pack2<BF16>(v[e + 4], v[e + 5]),
-                         pack2<BF16>(v[e + 6], v[e + 7]));
-        }
-      }
-    }
+    if (write) store16<BF16>(v, dst, part, wide, c0 + c, head_dim);
     __syncwarp();
   }
 }
@@ -621,7 +609,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
         store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / 4), y == 0 ? p.scale : 1.f,
                             row < wk.own && dst[y] != nullptr, zero,
                             static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim + off,
-                            parts[y] == nullptr ? nullptr : parts[y] + at + off, p.head_dim);
+                            parts[y] == nullptr ? nullptr : parts[y] + at + off, a.wide, p.head_dim);
       tc_fence_before();
     }
   }
@@ -693,6 +681,8 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
   a.stats = bp.delta;
   a.m_tiles64 = (p.queries + kCols - 1) / kCols;
   a.k_steps = (p.head_dim + 15) / 16;
+  a.wide = p.head_dim % 16 == 0;
+  for (const void* g : {bp.dq, bp.dk, bp.dv}) a.wide = a.wide && reinterpret_cast<uintptr_t>(g) % 32 == 0;
 
   const int64_t stat_blocks = static_cast<int64_t>(p.batch) * p.heads * a.m_tiles64;
   if (stat_blocks > INT32_MAX) return 8;

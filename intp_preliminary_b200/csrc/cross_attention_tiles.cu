@@ -80,6 +80,7 @@ struct Args {
   int32_t n_rt;          // row tiles of an instance
   int32_t n_items;
   int32_t k_steps;       // 16-wide steps that cover head_dim
+  bool wide;             // rows of out are 32-byte aligned
 };
 
 struct Item {
@@ -500,22 +501,9 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(o[e]) * inv;
-        if (r >= p.rows) {
-          // a lane past the instance's rows only takes part in the TMEM loads
-        } else if (split) {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + slot * p.head_dim + c * 16);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c * 16 + 4 * e < p.head_dim) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + x.b * p.os[0] + x.h * p.os[1] +
-                                                x.m * p.os[2] + c * 16);
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (c * 16 + 8 * e < p.head_dim)
-              dst[e] = make_uint4(pack2<BF16>(v[8 * e], v[8 * e + 1]), pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
-                                  pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
-        }
+        if (r < p.rows)  // a lane past the instance's rows only takes part in the TMEM loads
+          store16<BF16>(v, static_cast<uint16_t*>(p.out) + x.b * p.os[0] + x.h * p.os[1] + x.m * p.os[2],
+                        split ? p.part_o + slot * p.head_dim : nullptr, a.wide, c * 16, p.head_dim);
         __syncwarp();
       }
       tc_fence_before();
@@ -558,6 +546,8 @@ int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count)
   if (items > (1 << 30)) return 8;
   a.n_items = static_cast<int32_t>(items);
   a.k_steps = (p.head_dim + 15) / 16;
+  a.wide = p.head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.os[0] % 16 == 0 &&
+           p.os[1] % 16 == 0 && p.os[2] % 16 == 0;
   SlaParams t{};
   t.batch = p.shared ? 1 : p.batch;
   t.heads = p.groups;

@@ -36,4 +36,37 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+// 32 bytes of one thread, a whole memory sector (dst 32-byte aligned).
+__device__ __forceinline__ void store32(void* dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
+                                        uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(a), "r"(b), "r"(c), "r"(d),
+               "r"(e), "r"(f), "r"(g), "r"(h)
+               : "memory");
+}
+// 16 columns [c0, c0 + 16) of a row-per-thread result: fp32 to `part` if it is not null, else
+// rounded to 16 bits to `dst`; `wide` says that 16-bit rows are 32-byte aligned.  Rows differ
+// by thread, so a store is worth a sector each or it is worth less.
+template <bool BF16>
+__device__ __forceinline__ void store16(const float (&v)[16], uint16_t* dst, float* part, bool wide, int32_t c0,
+                                        int32_t head_dim) {
+  if (part != nullptr) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 8)
+      if (c0 + e < head_dim)
+        store32(part + c0 + e, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]),
+                __float_as_uint(v[e + 3]), __float_as_uint(v[e + 4]), __float_as_uint(v[e + 5]), __float_as_uint(v[e + 6]),
+                __float_as_uint(v[e + 7]));
+    return;
+  }
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(v[2 * e], v[2 * e + 1]);
+  if (wide) {
+    if (c0 < head_dim) store32(dst + c0, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+    return;
+  }
+  if (c0 < head_dim) *reinterpret_cast<uint4*>(dst + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (c0 + 8 < head_dim) *reinterpret_cast<uint4*>(dst + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
 }  // namespace intp

@@ -231,6 +231,8 @@ class NativeLibraryError(RuntimeError):
 def load() -> ctypes.CDLL:
     """Load the library once; raise NativeLibraryError when it is unavailable."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -44,7 +44,13 @@ from .look_attention import _DTYPE_CODE, _status_word, _status_words
 
 _KERNELS = {"auto": _lib.XATTN_KERNEL_AUTO, "rows": _lib.XATTN_KERNEL_ROWS, "tiles": _lib.XATTN_KERNEL_TILES}
 _HALF = (torch.bfloat16, torch.float16)
+_INTEGERS = (torch.int32, torch.int64)
 _MAX_STRIDE = 1 << 39  # elements: 2^40 bytes
+
+
+# torch's own accessors, without the lazy initialisation that a CUDA tensor's existence has done.
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _ready(t: torch.Tensor) -> bool:
@@ -103,13 +109,13 @@ def _check_counts(t, batch: int, device, name: str):
     """A per-sequence int32 vector (int64 is converted), or None."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.shape != (batch,) or t.dtype not in (torch.int32, torch.int64):
+    if not isinstance(t, torch.Tensor) or t.shape != (batch,) or t.dtype not in _INTEGERS:
         raise ValueError(f"{name} must be an int32 or int64 tensor of shape (B,)")
     if t.device != device:
         raise ValueError(f"{name} must be on the same CUDA device as q")
     if t.dtype == torch.int64:
         t = t.clamp(-2147483648, 2147483647).to(torch.int32)
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_states(q, k, v) -> None:
@@ -200,11 +206,11 @@ def _finish_plan(args, q, what: str) -> _Plan:
 
 def _call(fn, block, index: int, what: str) -> None:
     """One library call on the device's current stream."""
-    if torch.cuda.current_device() == index:
-        status = fn(block, torch._C._cuda_getCurrentRawStream(index))
+    if _current_device() == index:
+        status = fn(block, _current_stream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(block, torch._C._cuda_getCurrentRawStream(index))
+            status = fn(block, _current_stream(index))
     if status:
         _lib.check(status, what)
 
@@ -366,13 +372,13 @@ class _CrossAttention(torch.autograd.Function):
 
 def cross_attention(q, k, v, *, scale, lengths=None):
     """Attention of ``q`` to the states ``k``, ``v`` (see the module's text)."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
+    if torch.is_grad_enabled() and any([isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)]):
         return _CrossAttention.apply(q, k, v, lengths, _check_scale(scale))
     return _forward(q, k, v, scale, lengths, False, "auto", None)[0]
 
 
 def _refuse_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any([isinstance(t, torch.Tensor) and t.requires_grad for t in tensors]):
         raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 

@@ -53,12 +53,16 @@ class StateCache:
     the attention)."""
 
     def __init__(self, keys, key_exponents, values, value_exponents) -> None:
-        tensors = (keys, key_exponents, values, value_exponents)
-        if not all(isinstance(t, torch.Tensor) for t in tensors):
-            raise ValueError("a state cache requires CUDA tensors")
-        self.layout = ("state cache",) + tuple((t.shape, t.stride(), t.dtype, t.device) for t in tensors)
+        for t in (keys, key_exponents, values, value_exponents):
+            if not isinstance(t, torch.Tensor):
+                raise ValueError("a state cache requires CUDA tensors")
+        # what the tensors' layout decides is checked once and known by it
+        self.layout = (keys.shape, keys.stride(), keys.dtype, keys.device, values.shape, values.stride(), values.dtype,
+                       values.device, key_exponents.shape, key_exponents.stride(), key_exponents.dtype,
+                       key_exponents.device, value_exponents.shape, value_exponents.stride(), value_exponents.dtype,
+                       value_exponents.device)
         if self.layout not in _plans:
-            _check_tensors(*tensors)
+            _check_tensors(keys, key_exponents, values, value_exponents)
             _keep(self.layout, None)
         if (keys.data_ptr() | values.data_ptr()) & 15:
             raise ValueError("the cache's tensors must be contiguous, codes 16-byte aligned")
@@ -81,33 +85,30 @@ class StateCache:
     def shape(self) -> tuple[int, ...]:
         return tuple(self.keys.shape)
 
-    def _tail(self, k, v) -> bytes:
+    def _tail(self, k, v, key) -> bytes:
         """The argument block of a copy between ``k``, ``v`` and this cache, behind its pointers."""
-        key = (self.layout, k.shape, k.stride(), v.stride(), k.dtype)
-        tail = _plans.get(key)
-        if tail is None:
-            args = _lib.StateCacheArgs()
-            args.batch, args.groups, args.capacity, args.head_dim = self.keys.shape
-            args.count = k.shape[2]
-            args.dtype = _DTYPE_CODE[k.dtype]
-            args.k_stride, args.v_stride = k.stride(), v.stride()
-            tail = _keep(key, bytes(args)[_POINTERS.size:])
-        return tail
+        args = _lib.StateCacheArgs()
+        args.batch, args.groups, args.capacity, args.head_dim = self.keys.shape
+        args.count = k.shape[2]
+        args.dtype = _DTYPE_CODE[k.dtype]
+        args.k_stride, args.v_stride = k.stride(), v.stride()
+        return _keep(key, bytes(args)[_POINTERS.size:])
 
-    def _copy(self, fn, k, v, start, counts, what: str) -> None:
-        batch, device = self.keys.shape[0], self.keys.device
-        start = _check_counts(start, batch, device, "start")
-        counts = _check_counts(counts, batch, device, "counts")
-        block = _POINTERS.pack(k.data_ptr(), v.data_ptr(), 0 if start is None else start.data_ptr(),
-                               0 if counts is None else counts.data_ptr(), self.keys.data_ptr(),
+    def _copy(self, fn, tail: bytes, k, v, start, counts, what: str) -> None:
+        keys = self.keys
+        device = keys.device
+        start_p = counts_p = 0
+        if start is not None:
+            start = _check_counts(start, keys.shape[0], device, "start")
+            start_p = start.data_ptr()
+        if counts is not None:
+            counts = _check_counts(counts, keys.shape[0], device, "counts")
+            counts_p = counts.data_ptr()
+        block = _POINTERS.pack(k.data_ptr(), v.data_ptr(), start_p, counts_p, keys.data_ptr(),
                                self.key_exponents.data_ptr(), self.values.data_ptr(), self.value_exponents.data_ptr())
-        _call(fn, block + self._tail(k, v), device.index, what)
+        _call(fn, block + tail, device.index, what)
 
-    def write(self, k, v, *, start=None, counts=None) -> None:
-        """Quantise ``k``, ``v`` ``(B, G, n, D)`` (bf16 or f16) into the cache: row i of
-        sequence b goes to state ``start[b] + i`` (``start`` ``(B,)``, zero without
-        it) for ``i < counts[b]`` (all n without it).  Rows that fall outside the
-        cache are skipped; every other state is left as it was."""
+    def _check_pair(self, k, v) -> None:
         batch, groups, _, head_dim = self.keys.shape
         for t in (k, v):
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -118,8 +119,23 @@ class StateCache:
                 raise ValueError("k and v must be bfloat16 or float16 and share a dtype")
             if t.device != self.keys.device:
                 raise ValueError("all tensors must be on the same CUDA device")
+
+    def write(self, k, v, *, start=None, counts=None) -> None:
+        """Quantise ``k``, ``v`` ``(B, G, n, D)`` (bf16 or f16) into the cache: row i of
+        sequence b goes to state ``start[b] + i`` (``start`` ``(B,)``, zero without
+        it) for ``i < counts[b]`` (all n without it).  Rows that fall outside the
+        cache are skipped; every other state is left as it was."""
+        if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+            raise ValueError("a state cache requires CUDA tensors")
         _refuse_grad("a state cache", k, v)
-        self._copy(_lib.load().state_cache_write, _laid_out(k), _laid_out(v), start, counts, "state cache write")
+        key = (self.layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device)
+        tail = _plans.get(key)
+        if tail is None or (k.data_ptr() | v.data_ptr()) & 15:
+            self._check_pair(k, v)
+            k, v = _laid_out(k), _laid_out(v)
+            key = (self.layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device)
+            tail = _plans.get(key) or self._tail(k, v, key)
+        self._copy(_lib.load().state_cache_write, tail, k, v, start, counts, "state cache write")
 
     def read(self, count: int | None = None, *, start=None, counts=None, dtype=torch.bfloat16):
         """The values of ``count`` states per sequence (all C without it) from state
@@ -132,8 +148,12 @@ class StateCache:
             raise ValueError("count must not be negative")
         if dtype not in _HALF:
             raise ValueError("dtype must be bfloat16 or float16")
-        k, v = (torch.empty(batch, groups, count, head_dim, dtype=dtype, device=self.keys.device) for _ in range(2))
-        self._copy(_lib.load().state_cache_read, k, v, start, counts, "state cache read")
+        shape, device = (batch, groups, count, head_dim), self.keys.device
+        k = torch.empty(shape, dtype=dtype, device=device)
+        v = torch.empty(shape, dtype=dtype, device=device)
+        key = (self.layout, count, dtype)
+        tail = _plans.get(key) or self._tail(k, v, key)
+        self._copy(_lib.load().state_cache_read, tail, k, v, start, counts, "state cache read")
         return k, v
 
     def _set_states(self, args) -> None:

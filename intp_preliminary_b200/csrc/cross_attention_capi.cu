@@ -83,7 +83,22 @@ Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t sta
   return s;
 }
 
+// Whether a shared prefix is better read by each sequence before its own states, in one pass and
+// one launch, than once for all rows with its part joined by a third kernel: few rows and few
+// states.  Measured, one pass against three (prefix + own states, re-read bytes): 196 + 33
+// 4.9 / 10.0 us (B4 G3 D64, 0.6 MB) and 13.6 / 24.4 us (B64 G8 D128, 51 MB), 512 + 256 13.1 / 17.9
+// us (8 MB), 512 + 64 22.3 / 24.6 us (134 MB), 1024 + 256 19.3 / 18.9 us (17 MB), 1024 + 64
+// 36.4 / 25.6 us (268 MB), 2048 + 256 31.8 / 19.0 us (34 MB).
+constexpr int64_t kJoinedStates = 1024, kJoinedBytes = 128 << 20;
+
+bool joined_prefix(const xattn_args* a) {
+  const int64_t per_group = a->heads / a->groups;
+  return a->prefix > 0 && a->kernel != XATTN_KERNEL_TILES && !a->eight_bit && per_group * a->queries <= kRowsMax &&
+         a->prefix + a->states <= kJoinedStates && a->batch * a->groups * a->prefix * a->head_dim * 4 <= kJoinedBytes;
+}
+
 struct Plan {
+  bool joined;
   Pass own, pre;
   int64_t own_slots, pre_slots;      // parts written to the workspace
   int64_t rows_total, o_bytes, bytes;
@@ -94,6 +109,13 @@ Plan plan_forward(const xattn_args* a) {
   Plan p{};
   const int64_t per_group = a->heads / a->groups;
   p.rows_total = a->batch * a->heads * a->queries;
+  p.joined = joined_prefix(a);
+  if (p.joined) {
+    p.own.n_split = 1;
+    p.own.split_keys = std::max<int64_t>(a->states, 1);
+    p.own_slots = 1;
+    return p;
+  }
   if (a->states > 0) {
     p.own = plan_pass(a, per_group * a->queries, a->batch * a->groups, a->states);
     p.own_slots = p.own.n_split;
@@ -271,9 +293,17 @@ intp_status xattn_forward(const xattn_args* a, void* stream) {
     p.part_o = static_cast<float*>(a->workspace);
     p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + plan.o_bytes);
   }
+  const int64_t ep[2] = {a->groups, a->prefix};
+  if (plan.joined) {
+    p.pre_k = a->prefix_k;
+    p.pre_v = a->prefix_v;
+    take_strides(p.pre_ks, a->prefix_k_stride, ep, 2, a->head_dim);
+    take_strides(p.pre_vs, a->prefix_v_stride, ep, 2, a->head_dim);
+    p.prefix = static_cast<int32_t>(a->prefix);
+    return launch_pass(p, plan.own, 0, s, sms);
+  }
   if (a->prefix > 0) {
     XaParams x = p;
-    const int64_t ep[2] = {a->groups, a->prefix};
     x.shared = 1;
     x.states = static_cast<int32_t>(a->prefix);
     x.rows = static_cast<int32_t>(a->batch * x.per_group * a->queries);

@@ -157,32 +157,48 @@ xattn_rows_kernel(const RowsArgs a) {
   const int32_t n_rows = p.rows - row0 < kTile ? p.rows - row0 : kTile;
   const int32_t D = p.head_dim;
 
-  const int64_t k_row = p.ks[2] * L::kElem, v_row = p.vs[2] * L::kElem;
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  const int32_t n_slices = (n_keys + kStep - 1) / kStep;
+  // Slices: those of a prefix that is read in the same pass (16-bit states), then the range's own.
+  const int32_t n_prefix = FP8 ? 0 : p.prefix;
+  const int32_t pre_slices = (n_prefix + kStep - 1) / kStep;
+  const int32_t n_slices = pre_slices + (n_keys + kStep - 1) / kStep;
   const int32_t mine = n_slices > warp ? (n_slices - warp + kWarps - 1) / kWarps : 0;
 
   // This lane copies chunk `cc` of states `cr`, cr + 32 / CH, ... of each slice.
   const int cr = lane / CH, cc = lane % CH;
   const bool chunk_read = cc * L::kPerChunk < D;
   const bool chunk_used = cc * L::kPerChunk < ((D + 15) & ~15);  // columns past D that the products read are zero
-  const uint8_t* k_src = static_cast<const uint8_t*>(p.k) +
-                         (b * p.ks[0] + grp * p.ks[1] + (static_cast<int64_t>(key0) + warp * kStep) * p.ks[2]) * L::kElem;
-  const uint8_t* v_src = static_cast<const uint8_t*>(p.v) +
-                         (b * p.vs[0] + grp * p.vs[1] + (static_cast<int64_t>(key0) + warp * kStep) * p.vs[2]) * L::kElem;
-  if (chunk_read) {
-    k_src += cr * k_row + cc * 16;
-    v_src += cr * v_row + cc * 16;
-  }
-  const int64_t k_next = (32 / CH) * k_row, v_next = (32 / CH) * v_row;
+  const int32_t lane_byte = chunk_read ? cc * 16 : 0;
+  int64_t k_row = 0, v_row = 0;
+  const uint8_t *k_src = nullptr, *v_src = nullptr;
+  // Points this lane at its first state of slice `first` of a segment's states.
+  auto enter = [&](const void* k, const void* v, int64_t k_base, int64_t v_base, int64_t k_stride, int64_t v_stride,
+                   int32_t first) {
+    k_row = k_stride * L::kElem;
+    v_row = v_stride * L::kElem;
+    const int64_t state = static_cast<int64_t>(first) * kStep + cr;
+    k_src = static_cast<const uint8_t*>(k) + k_base * L::kElem + state * k_row + lane_byte;
+    v_src = static_cast<const uint8_t*>(v) + v_base * L::kElem + state * v_row + lane_byte;
+  };
+  auto enter_own = [&](int32_t first) {
+    enter(p.k, p.v, b * p.ks[0] + grp * p.ks[1] + key0 * p.ks[2], b * p.vs[0] + grp * p.vs[1] + key0 * p.vs[2], p.ks[2],
+          p.vs[2], first);
+  };
+  if (!FP8 && warp < pre_slices)
+    enter(p.pre_k, p.pre_v, grp * p.pre_ks[0], grp * p.pre_vs[0], p.pre_ks[1], p.pre_vs[1], warp);
+  else
+    enter_own(warp - pre_slices);
   int32_t issued = 0;
-  // The next slice of this warp (keys 16 (warp + 4 i) ..) into its ring; keys past the end are zero.
+  // The next slice of this warp (warp, warp + 4, ...) into its ring; keys past the end are zero.
   auto issue = [&]() {
     if (issued < mine) {
-      const int32_t k0 = (issued * kWarps + warp) * kStep;
+      const int32_t slice = issued * kWarps + warp;
+      const bool pre = !FP8 && slice < pre_slices;
+      const int32_t left = pre ? n_prefix - slice * kStep : n_keys - (slice - pre_slices) * kStep;
       const uint32_t dst = ring + (issued % NS) * 2 * L::kSliceBytes;
+      const int64_t k_next = (32 / CH) * k_row, v_next = (32 / CH) * v_row;
       const uint8_t *ks = k_src, *vs = v_src;
-      if (k0 + kStep <= n_keys && chunk_read) {
+      if (left >= kStep && chunk_read) {
 #pragma unroll
         for (int u = 0; u < kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
           const uint32_t to = dst + chunk_offset<CH>(cr + u * (32 / CH), cc);
@@ -193,14 +209,18 @@ xattn_rows_kernel(const RowsArgs a) {
 #pragma unroll
         for (int u = 0; u < kStep * CH / 32; ++u, ks += k_next, vs += v_next) {
           const int row = cr + u * (32 / CH);
-          const bool read = k0 + row < n_keys && chunk_read;
+          const bool read = row < left && chunk_read;
           const uint32_t to = dst + chunk_offset<CH>(row, cc);
-          cp_async16(to, read ? ks : static_cast<const uint8_t*>(p.k), read);
-          cp_async16(to + L::kSliceBytes, read ? vs : static_cast<const uint8_t*>(p.v), read);
+          cp_async16(to, read ? ks : static_cast<const uint8_t*>(p.q), read);
+          cp_async16(to + L::kSliceBytes, read ? vs : static_cast<const uint8_t*>(p.q), read);
         }
       }
-      k_src += kWarps * kStep * k_row;
-      v_src += kWarps * kStep * v_row;
+      if (pre && slice + kWarps >= pre_slices) {
+        enter_own(slice + kWarps - pre_slices);
+      } else {
+        k_src += kWarps * kStep * k_row;
+        v_src += kWarps * kStep * v_row;
+      }
     }
     ++issued;
     cp_async_commit();
@@ -285,7 +305,10 @@ xattn_rows_kernel(const RowsArgs a) {
     cp_async_wait<NS - 2>();
     __syncwarp();
     const uint32_t k_s = ring + (i % NS) * 2 * L::kSliceBytes, v_s = k_s + L::kSliceBytes;
-    const int32_t k0 = (i * kWarps + warp) * kStep;
+    // First key of the slice, and the segment's end, in the segment's own count.
+    const int32_t slice = i * kWarps + warp;
+    const bool pre = !FP8 && slice < pre_slices;
+    const int32_t k0 = (pre ? slice : slice - pre_slices) * kStep, end = pre ? n_prefix : n_keys;
     float s[NT][4];                         // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -320,13 +343,13 @@ xattn_rows_kernel(const RowsArgs a) {
     // Scores in log2 units; padded keys -inf.
     float w[2];                             // value exponents
     bool grow = false;
-    const bool padded = k0 + kStep > n_keys;
+    const bool padded = k0 + kStep > end;
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
       const int32_t key = k0 + kh * 8 + g;
       float2 f = make_float2(1.f, 0.f);   // the key's power of two, the value's exponent
       if (FP8) {
-        const uint32_t e = exp_s[!padded || key < n_keys ? key : 0];
+        const uint32_t e = exp_s[!padded || key < end ? key : 0];
         // a byte below 2^23's mantissa is that number above it
         f = make_float2(__uint_as_float((e & 0xffu) << 23), __uint_as_float(0x4b000000u | (e >> 8)) - 8388735.f);
       }
@@ -338,7 +361,7 @@ xattn_rows_kernel(const RowsArgs a) {
           float& v = s[n][2 * kh + h];
           v *= row_scale[n][h];
           if (FP8) v *= f.x;
-          if (padded && key >= n_keys) v = -INFINITY;
+          if (padded && key >= end) v = -INFINITY;
           // a NaN score counts as growth: it has to reach the reference
           grow = grow || !(v <= m[n][h] + kRescale) || (FP8 && !(v + f.y <= mw[n][h] + kRescale));
         }

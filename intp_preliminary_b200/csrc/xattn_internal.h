@@ -25,6 +25,10 @@ struct XaParams {
   const void* k; int64_t ks[3];  // batch, group, state
   const void* v; int64_t vs[3];
   const uint8_t* k_exp; const uint8_t* v_exp; int64_t es[2];
+  // Few-rows kernel only: states that every sequence reads before its own (group and state
+  // strides as in ks, vs), in one unsplit pass.
+  const void* pre_k; const void* pre_v; int64_t pre_ks[2], pre_vs[2];
+  int32_t prefix;
   const int32_t* lengths;
   void* out; int64_t os[3];
   float* lse;

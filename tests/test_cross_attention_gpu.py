@@ -394,3 +394,27 @@ def test_wait_budget_reports_and_the_next_call_is_clean(cuda_device):
         finally:
             assert lib.intp_set_wait_budget_ns(ctypes.c_uint64(1_000_000_000)) == _lib.INTP_OK
     _check_forward(q, k, v, None, cuda_device, "tiles", scale=0.125)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F16), (40, BF16)])
+@pytest.mark.parametrize("queries", [1, 3, 8])
+@pytest.mark.parametrize("prefix,states,lengths", [(15, 1, None), (16, 16, [16, 0, 7]), (63, 65, [65, 64, 1]),
+                                                   (257, 300, [0, 299, 128]), (900, 100, [100, 3, 99]), (1000, 40, None)])
+def test_short_prefix_in_one_pass_and_in_three(cuda_device, prefix, states, lengths, queries, dim, dtype):
+    """Around the border where a prefix is read by each sequence in one pass: slices of both
+    segments end anywhere, and padded own states may hold NaN."""
+    q, k, v = _inputs(3, 4, 2, queries, states, dim, dtype, seed=90)
+    pk, pv = _normal((2, prefix, dim), dtype, 91), _normal((2, prefix, dim), dtype, 92)
+    want, _, bound = oracle.cross_attention(q, k, v, scale=0.15, lengths=lengths, prefix=(pk, pv))
+    if lengths is not None:
+        for b, n in enumerate(lengths):
+            k[b, :, n:] = float("nan")
+            v[b, :, n:] = float("nan")
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    got = shared_prefix_attention(*(t.to(cuda_device) for t in (q, pk, pv, k, v)), scale=0.15, lengths=lens)
+    _assert_within(got, want, bound)
+    wide = torch.empty(2, prefix, 2 * dim, dtype=dtype, device=cuda_device)
+    wide[..., :dim], wide[..., dim:] = pk.to(cuda_device), pv.to(cuda_device)
+    again = shared_prefix_attention(q.to(cuda_device), wide[..., :dim], wide[..., dim:], k.to(cuda_device),
+                                    v.to(cuda_device), scale=0.15, lengths=lens)
+    assert torch.equal(got, again)

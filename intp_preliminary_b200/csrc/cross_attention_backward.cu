@@ -17,8 +17,8 @@
 // are summed in order (xattn_sum_kernel).  Every output element has one writer
 // and no atomics are used, so results repeat bit for bit.
 //
-// A CTA (persistent over work items) has an MMA warp, a TMA warp and 16 row warps (row thread t
-// owns TMEM lane t % 128 and 16 of a tile's 64 columns).  Score buffers are double: the products
+// A CTA (persistent over work items) has an MMA warp, a TMA warp and 8 row warps (row thread t
+// owns TMEM lane t % 128 and 32 of a tile's 64 columns).  Score buffers are double: the products
 // of tile t + 1 run under the row threads' tile t, and the next item's first score product runs
 // under this one's epilogue.  A 128 x 64 x 16 product reads 6 KB of shared memory where both
 // operands lie there (48 cycles) and 2 KB with the owned operand in TMEM (32 cycles, the
@@ -39,8 +39,11 @@ namespace {
 
 constexpr int kRows = 128;                 // TMEM lanes: query rows (dq) / keys (dk, dv)
 constexpr int kCols = 64;                  // streamed tile: keys (dq) / query rows (dk, dv)
-constexpr int kW = 16;                     // columns of a tile per row thread
-constexpr int kRowThreads = kRows * kCols / kW;  // 512
+// Columns of a tile per row thread.  8 warps of 32 columns: 716 us for the backward of B4 H16
+// M2048 N4096 D128; 16 warps of 16 columns execute a third more instructions: 735 us.
+constexpr int kW = 32;
+constexpr int kParts = kCols / kW;         // row threads of a row
+constexpr int kRowThreads = kRows * kParts;
 constexpr int kRowWarps = kRowThreads / 32;
 // The MMA and TMA warps come first, with two idle ones, so that row warp w reaches TMEM lanes 32 (w % 4) ..
 constexpr int kMmaWarp = 0, kLoadWarp = 1, kFirstRowWarp = 4;
@@ -178,6 +181,12 @@ __device__ __forceinline__ void tma_rows(uint8_t* dst, const CUtensorMap* tm, ui
                                          int32_t row, int32_t head, int32_t b) {
   tma_load_4d(dst, tm, bar, x, map_coord(o, 1, row, head, b), map_coord(o, 2, row, head, b),
               map_coord(o, 3, row, head, b));
+}
+
+// TMEM column of the 16-bit operand of depth step kk: each row thread packs its kW columns into
+// the first half of them.
+__device__ __forceinline__ constexpr uint32_t operand_col(int kk) {
+  return static_cast<uint32_t>(kk * 16 / kW * kW + kk * 16 % kW / 2);
 }
 
 // dq: a padded key tile of a sequence (rows past the tensor's end arrive as zeros by themselves).
@@ -351,12 +360,12 @@ __device__ __forceinline__ void mma_role(const Args& a, Bars* bars, uint8_t* sme
       const uint32_t x = tmem + st * 128, y = x + 64;
 #pragma unroll
       for (int kk = 0; kk < kCols / 16; ++kk)
-        mma_ts_warp(leader, tmem + kColAcc + (KV ? DP : 0), x + kk * kW, (KV ? r1 : r0) + ((kk * 2048) >> 4), idesc_acc,
+        mma_ts_warp(leader, tmem + kColAcc + (KV ? DP : 0), x + operand_col(kk), (KV ? r1 : r0) + ((kk * 2048) >> 4), idesc_acc,
                     (i > 0 || kk > 0) ? 1u : 0u);
       if (KV) {
 #pragma unroll
         for (int kk = 0; kk < kCols / 16; ++kk)
-          mma_ts_warp(leader, tmem + kColAcc, y + kk * kW, r0 + ((kk * 2048) >> 4), idesc_acc,
+          mma_ts_warp(leader, tmem + kColAcc, y + operand_col(kk), r0 + ((kk * 2048) >> 4), idesc_acc,
                       (i > 0 || kk > 0) ? 1u : 0u);
       }
       mma_commit_warp(leader, &bars->ring_empty[s]);
@@ -374,7 +383,7 @@ __device__ __forceinline__ void mma_role(const Args& a, Bars* bars, uint8_t* sme
 // The row threads' owned operands on their way to TMEM: this thread's quarter of its row of F0 and F1.
 template <int DP>
 struct OwnedRow {
-  uint4 f[2][DP / 32];
+  uint4 f[2][DP / (8 * kParts)];
 };
 
 template <int DP>
@@ -383,7 +392,7 @@ __device__ __forceinline__ void fetch_owned(OwnedRow<DP>& o, const uint16_t* f0,
   for (int y = 0; y < 2; ++y) {
     const uint16_t* src = y ? f1 : f0;
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) {
+    for (int c = 0; c < DP / (8 * kParts); ++c) {
       o.f[y][c] = make_uint4(0u, 0u, 0u, 0u);
       if (src != nullptr && c0 + c * 8 < head_dim) o.f[y][c] = __ldg(reinterpret_cast<const uint4*>(src + c0 + c * 8));
     }
@@ -392,32 +401,50 @@ __device__ __forceinline__ void fetch_owned(OwnedRow<DP>& o, const uint16_t* f0,
 
 template <int DP>
 __device__ __forceinline__ void store_owned(const OwnedRow<DP>& o, uint32_t taddr) {
+  constexpr int kWords = DP / (2 * kParts);   // 8, 16 or 32
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
-    if (DP == 128)
-      tmem_st16(taddr + y * (DP / 2), *reinterpret_cast<const uint32_t(*)[16]>(o.f[y]));
-    else
-      tmem_st8(taddr + y * (DP / 2), *reinterpret_cast<const uint32_t(*)[8]>(o.f[y]));
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(o.f[y]);
+    if (kWords == 8) {
+      tmem_st8(taddr + y * (DP / 2), *reinterpret_cast<const uint32_t(*)[8]>(w));
+    } else {
+#pragma unroll
+      for (int c = 0; c < kWords; c += 16)
+        tmem_st16(taddr + y * (DP / 2) + c, *reinterpret_cast<const uint32_t(*)[16]>(w + c));
+    }
   }
   tmem_wait_st();
   tc_fence_before();
 }
 
-// This thread's 16 columns of X and Y.
+// This thread's columns of X and Y.
 __device__ __forceinline__ void load_scores(uint32_t x, uint32_t (&xr)[kW], uint32_t (&yr)[kW]) {
-  tmem_ld16(x, xr);
-  tmem_ld16(x + 64, yr);
+#pragma unroll
+  for (int c = 0; c < kW; c += 16) {
+    tmem_ld16(x + c, *reinterpret_cast<uint32_t(*)[16]>(xr + c));
+    tmem_ld16(x + 64 + c, *reinterpret_cast<uint32_t(*)[16]>(yr + c));
+  }
   tmem_wait_ld();
-  reg_fence16(xr);
-  reg_fence16(yr);
+#pragma unroll
+  for (int c = 0; c < kW; c += 16) {
+    reg_fence16(*reinterpret_cast<uint32_t(*)[16]>(xr + c));
+    reg_fence16(*reinterpret_cast<uint32_t(*)[16]>(yr + c));
+  }
 }
 
-// Columns [c0, c0 + DP / 4) of an accumulator row, scaled, to a 16-bit or (split) fp32 row.
+__device__ __forceinline__ void store_operand(uint32_t taddr, const uint32_t (&w)[kW / 2]) {
+  if (kW == 16)
+    tmem_st8(taddr, *reinterpret_cast<const uint32_t(*)[8]>(w));
+  else
+    tmem_st16(taddr, *reinterpret_cast<const uint32_t(*)[16]>(w));
+}
+
+// Columns [c0, c0 + DP / kParts) of an accumulator row, scaled, to a 16-bit or (split) fp32 row.
 template <int DP, bool BF16>
 __device__ __forceinline__ void store_row(uint32_t taddr, int c0, float f, bool write, bool zero, uint16_t* dst,
                                           float* part, bool wide, int32_t head_dim) {
 #pragma unroll
-  for (int c = 0; c < DP / 4; c += 16) {
+  for (int c = 0; c < DP / kParts; c += 16) {
     uint32_t r[16];
     tmem_ld16(taddr + c0 + c, r);
     tmem_wait_ld();
@@ -496,7 +523,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             f1 = KV ? static_cast<const uint16_t*>(p.v) + w.b * p.vs[0] + w.g * p.vs[1] + r * p.vs[2]
                     : static_cast<const uint16_t*>(a.p.dout) + w.b * a.p.ds[0] + w.h0 * a.p.ds[1] + r * a.p.ds[2];
           }
-          fetch_owned<DP>(owned, f0, f1, wg * (DP / 4), p.head_dim);
+          fetch_owned<DP>(owned, f0, f1, wg * (DP / kParts), p.head_dim);
         }
         if (!KV) {
           next_nlse = -INFINITY;
@@ -515,7 +542,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     };
     auto hand_over = [&] {
       if (L::kOwnedInTmem) {
-        store_owned<DP>(owned, lane_base + L::kColOwned + wg * (DP / 8));
+        store_owned<DP>(owned, lane_base + L::kColOwned + wg * (DP / (2 * kParts)));
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->owned_full);
       }
@@ -586,8 +613,8 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             }
           }
         }
-        if (KV) tmem_st8(x, pw);               // P^T over the read X columns
-        tmem_st8(KV ? x + 64 : x, dw);         // dS (dk, dv: its transpose over Y)
+        if (KV) store_operand(x, pw);          // P^T over the read X columns
+        store_operand(KV ? x + 64 : x, dw);    // dS (dk, dv: its transpose over Y)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -606,7 +633,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       const int64_t off = static_cast<int64_t>(row) * p.head_dim;
 #pragma unroll
       for (int y = 0; y < (KV ? 2 : 1); ++y)
-        store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / 4), y == 0 ? p.scale : 1.f,
+        store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / kParts), y == 0 ? p.scale : 1.f,
                             row < wk.own && dst[y] != nullptr, zero,
                             static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim + off,
                             parts[y] == nullptr ? nullptr : parts[y] + at + off, a.wide, p.head_dim);

@@ -418,3 +418,70 @@ def test_short_prefix_in_one_pass_and_in_three(cuda_device, prefix, states, leng
     again = shared_prefix_attention(q.to(cuda_device), wide[..., :dim], wide[..., dim:], k.to(cuda_device),
                                     v.to(cuda_device), scale=0.15, lengths=lens)
     assert torch.equal(got, again)
+
+
+def test_autograd_step_in_a_graph(cuda_device):
+    """Forward and autograd's backward captured together (fresh leaves), replayed on new values."""
+    data = [t.to(cuda_device) for t in _inputs(2, 4, 2, 40, 300, 64, BF16, seed=120)]
+    grad = torch.randn_like(data[0])
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in data]
+        out = cross_attention(*leaves, scale=0.125)
+        return (out.detach(), *torch.autograd.grad(out, leaves, grad))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step()
+    for t in data:
+        t.mul_(-0.5)
+    graph.replay()
+    for a, b in zip(results, step()):
+        assert torch.equal(a, b)
+
+
+def test_calls_from_two_threads(cuda_device):
+    """Calls of different sizes at once from two host threads, each on its own stream."""
+    import threading
+
+    sets = [[t.to(cuda_device) for t in _inputs(2, 4, 4, m, n, 64, BF16, seed=m)] for m, n in ((1, 3000), (200, 500))]
+    want = [cross_attention(*s, scale=0.125) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                out = cross_attention(*sets[i], scale=0.125)
+                if not torch.equal(out, want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_largest_and_smallest_magnitudes(cuda_device):
+    """f16 at the ends of its range: outputs near its largest value, subnormal values."""
+    q, k, v = _inputs(1, 2, 1, 33, 200, 64, F16, seed=130)
+    for factor in (2.0 ** 13, 2.0 ** -20):
+        for kernel in ("rows", "tiles"):
+            _check_forward(q, k, (v.float() * factor).to(F16), [150], cuda_device, kernel)
+
+
+def test_kernels_agree_on_which_rows_share_a_head(cuda_device):
+    """H = 6 over G = 2 and 3: each query head reads the key head of its group."""
+    for groups in (1, 2, 3, 6):
+        q, k, v = _inputs(2, 6, groups, 5, 70, 64, BF16, seed=140)
+        v = torch.arange(groups).view(1, groups, 1, 1).expand(2, groups, 70, 64).to(BF16).contiguous()
+        for kernel in ("rows", "tiles"):
+            out, _ = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, kernel=kernel)
+            want = torch.arange(6) // (6 // groups)
+            assert (out.cpu().float().round() == want.view(1, 6, 1, 1)).all()

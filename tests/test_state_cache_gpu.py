@@ -259,3 +259,42 @@ def test_refusals(cuda_device):
             cached_cross_attention(*bad, scale=0.125)
     with pytest.raises(ValueError, match="leave v out"):
         shared_prefix_attention(q, x[0], x[0], cache, x, scale=0.125)
+
+
+def test_long_cache_past_32_bit_offsets(cuda_device):
+    """The last sequence's codes start past 2^31 bytes: written, read and attended to there."""
+    batch, capacity, dim = 9, 2_000_000, 128
+    cache = StateCache.empty(batch, 1, capacity, dim, device=cuda_device)
+    k, v = _normal((batch, 1, 50, dim), BF16, 1), _normal((batch, 1, 50, dim), BF16, 2)
+    start = torch.full((batch,), capacity - 50, dtype=torch.int32, device=cuda_device)
+    cache.write(k.to(cuda_device) * 0.05, v.to(cuda_device), start=start)
+    rk, rv = cache.read(50, start=start)
+    want_k, _ = oracle.quantise_rows((k.to(cuda_device) * 0.05)[-1:])
+    assert torch.equal(rk[-1:].cpu().double(), want_k)
+    q = _normal((batch, 2, 1, dim), BF16, 3).to(cuda_device)
+    tail = StateCache(cache.keys[:, :, -50:].contiguous(), cache.key_exponents[:, :, -50:].contiguous(),
+                      cache.values[:, :, -50:].contiguous(), cache.value_exponents[:, :, -50:].contiguous())
+    # zero keys score 0 and zero values add nothing: the sums over the tail and over all states
+    # differ by the number of zero states alone
+    part, full = (cached_cross_attention(q, c, scale=0.05).cpu().double() for c in (tail, cache))
+    kd, vd = _values(tail.keys, tail.key_exponents), _values(tail.values, tail.value_exponents)
+    want, lse, bound = oracle.cross_attention(q, kd, vd, scale=0.05, p_dtype=F16, out_dtype=BF16,
+                                              key_weight=torch.exp2(tail.value_exponents.double() - 127))
+    assert ((part - want).abs() <= bound).all()
+    share = torch.sigmoid(lse - torch.log(torch.tensor(float(capacity - 50))))[..., None]
+    # fp32 sums of two million equal terms over parts of 2048 keys or fewer: within 1e-4 of the count
+    assert ((full - want * share).abs() <= share * bound + 2e-4 * (want * share).abs() + 1e-7).all()
+
+
+def test_write_follows_strides(cuda_device):
+    """(B, n, G, 2, D) projections seen as keys and values."""
+    kv = _normal((2, 37, 3, 2, 64), BF16, 1).to(cuda_device)
+    k, v = kv[:, :, :, 0].transpose(1, 2), kv[:, :, :, 1].transpose(1, 2)
+    a, b = (StateCache.empty(2, 3, 40, 64, device=cuda_device) for _ in range(2))
+    a.write(k, v)
+    b.write(k.contiguous(), v.contiguous())
+    assert torch.equal(a.keys.view(torch.uint8), b.keys.view(torch.uint8))
+    assert torch.equal(a.values.view(torch.uint8), b.values.view(torch.uint8))
+    odd = torch.empty(2, 3, 37, 65, dtype=BF16, device=cuda_device)[..., 1:].copy_(k)  # not 16-byte aligned
+    a.write(odd, v)
+    assert torch.equal(a.keys.view(torch.uint8), b.keys.view(torch.uint8))

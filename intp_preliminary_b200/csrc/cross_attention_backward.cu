@@ -85,6 +85,7 @@ struct Args {
   int32_t n_row_tiles, n_split, split_tiles, n_items;
   int32_t k_steps;
   bool wide;                               // gradient rows are 32-byte aligned
+  bool after_stats;                        // the kernel before this one writes the statistics
 };
 
 // One work item: what it owns and what it streams.
@@ -125,6 +126,7 @@ template <int LPR, bool BF16>
 __global__ void __launch_bounds__(256)
 xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
   constexpr int kPerPass = 256 / LPR, kPasses = kCols / kPerPass;
+  allow_next_kernel();
   const XaParams& p = bp.f;
   const int32_t bh = blockIdx.x / m_tiles64, m0 = (blockIdx.x - bh * m_tiles64) * kCols;
   const int32_t b = bh / p.heads, h = bh - b * p.heads;
@@ -214,6 +216,7 @@ __device__ __forceinline__ void load_role(const CUtensorMap* f0, const CUtensorM
   }
   uint32_t tile = 0, items = 0;            // loaded by this CTA
   bool ok = true;
+  if (KV && a.after_stats) wait_previous_kernel();
   for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
     const Work wk = decode_work<KV>(a, item);
     if (wk.n_t == 0) continue;
@@ -551,6 +554,9 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     };
     uint32_t tile = 0, items = 0;
     bool ok = true;
+    if (!KV) wait_previous_kernel();           // for the statistics
+    // The dk / dv kernel after dq needs the statistics too, and nothing of dq's.
+    allow_next_kernel();
     if (fetch(blockIdx.x)) hand_over();
     for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
       const Work wk = decode_work<KV>(a, item);
@@ -640,6 +646,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       tc_fence_before();
     }
   }
+  wait_previous_kernel();
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -653,6 +660,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
 template <bool BF16>
 __global__ void __launch_bounds__(128)
 xattn_sum_kernel(const float* part0, uint16_t* dst0, const float* part1, uint16_t* dst1, int64_t n, int32_t n_split) {
+  wait_previous_kernel();
   const float* part = blockIdx.y ? part1 : part0;
   uint16_t* dst = blockIdx.y ? dst1 : dst0;
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x) * 4;
@@ -672,9 +680,10 @@ int32_t launch_sum(const float* part0, void* dst0, const float* part1, void* dst
                    cudaStream_t stream) {
   const int64_t grid = (n / 4 + 127) / 128;
   if (grid > INT32_MAX) return 8;
-  xattn_sum_kernel<BF16><<<dim3(static_cast<unsigned>(grid), dst1 != nullptr ? 2 : 1), 128, 0, stream>>>(
-      part0, static_cast<uint16_t*>(dst0), part1, static_cast<uint16_t*>(dst1), n, n_split);
-  return cudaGetLastError() == cudaSuccess ? 0 : 6;
+  return launch_kernel(xattn_sum_kernel<BF16>, dim3(static_cast<unsigned>(grid), dst1 != nullptr ? 2 : 1), 128, 0, stream,
+                       true, part0, static_cast<uint16_t*>(dst0), part1, static_cast<uint16_t*>(dst1), n, n_split)
+             ? 0
+             : 6;
 }
 
 template <int DP, bool BF16, bool KV>
@@ -696,8 +705,7 @@ int32_t launch_grad(const CUtensorMap& f0, const CUtensorMap& f1, const CUtensor
   if (!allow_smem(kernel, smem, done)) return 6;
   // one CTA per SM: it holds all of the SM's tensor memory
   const unsigned grid = static_cast<unsigned>(items < sm_count ? items : sm_count);
-  kernel<<<grid, kThreads, smem, stream>>>(f0, f1, r0, r1, a);
-  return cudaGetLastError() == cudaSuccess ? 0 : 6;
+  return launch_kernel(kernel, dim3(grid), kThreads, smem, stream, true, f0, f1, r0, r1, a) ? 0 : 6;
 }
 
 template <int DP, bool BF16>
@@ -730,9 +738,8 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
     CUtensorMap r0, r1;
     if (!make_map(&r0, &a.or0, p.k, ks, tk, kCols) || !make_map(&r1, &a.or1, p.v, vs, tk, kCols)) return 4;
     static_assert(Shape<DP, false>::kOwnedInTmem, "no maps of q and dO");
-    int32_t st = launch_grad<DP, BF16, false>(r0, r1, r0, r1, a, sm_count, stream);
-    if (st == 0 && bp.dq_part != nullptr)
-      st = launch_sum<BF16>(bp.dq_part, bp.dq, nullptr, nullptr, p.rows_total * p.head_dim, bp.dq_split, stream);
+    a.after_stats = true;
+    const int32_t st = launch_grad<DP, BF16, false>(r0, r1, r0, r1, a, sm_count, stream);
     if (st) return st;
   }
   if (bp.dk != nullptr || bp.dv != nullptr) {
@@ -743,14 +750,19 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
     if (!Shape<DP, true>::kOwnedInTmem &&
         (!make_map(&f0, &a.of0, p.k, ks, tk, kRows) || !make_map(&f1, &a.of1, p.v, vs, tk, kRows)))
       return 4;
-    int32_t st = launch_grad<DP, BF16, true>(f0, f1, r0, r1, a, sm_count, stream);
+    a.after_stats = bp.dq == nullptr;
+    const int32_t st = launch_grad<DP, BF16, true>(f0, f1, r0, r1, a, sm_count, stream);
+    if (st) return st;
+  }
+  if (bp.dq != nullptr && bp.dq_part != nullptr) {
+    const int32_t st = launch_sum<BF16>(bp.dq_part, bp.dq, nullptr, nullptr, p.rows_total * p.head_dim, bp.dq_split, stream);
+    if (st) return st;
+  }
+  if ((bp.dk != nullptr || bp.dv != nullptr) && bp.dk_part != nullptr) {
     const int64_t n = static_cast<int64_t>(p.batch) * p.groups * p.states * p.head_dim;
-    if (st == 0 && bp.dk_part != nullptr) {
-      if (bp.dk != nullptr)
-        st = launch_sum<BF16>(bp.dk_part, bp.dk, bp.dv_part, bp.dv, n, bp.kv_split, stream);
-      else
-        st = launch_sum<BF16>(bp.dv_part, bp.dv, nullptr, nullptr, n, bp.kv_split, stream);
-    }
+    const int32_t st = bp.dk != nullptr
+                           ? launch_sum<BF16>(bp.dk_part, bp.dk, bp.dv_part, bp.dv, n, bp.kv_split, stream)
+                           : launch_sum<BF16>(bp.dv_part, bp.dv, nullptr, nullptr, n, bp.kv_split, stream);
     if (st) return st;
   }
   return 0;

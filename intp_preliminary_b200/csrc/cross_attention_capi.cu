@@ -187,11 +187,11 @@ intp_status to_params(const xattn_args* a, XaParams* p) {
   return INTP_OK;
 }
 
-int32_t launch_pass(XaParams p, const Pass& s, int64_t first, cudaStream_t stream, int sms) {
+int32_t launch_pass(XaParams p, const Pass& s, int64_t first, cudaStream_t stream, int sms, bool overlap) {
   p.n_split = static_cast<int32_t>(s.n_split);
   p.split_keys = static_cast<int32_t>(s.split_keys);
   p.part_first = static_cast<int32_t>(first);
-  return s.tiles ? intp::launch_xattn_tiles(p, stream, sms) : intp::launch_xattn_rows(p, stream);
+  return s.tiles ? intp::launch_xattn_tiles(p, stream, sms, overlap) : intp::launch_xattn_rows(p, stream, overlap);
 }
 
 struct BackwardPlan {
@@ -300,9 +300,14 @@ intp_status xattn_forward(const xattn_args* a, void* stream) {
     take_strides(p.pre_ks, a->prefix_k_stride, ep, 2, a->head_dim);
     take_strides(p.pre_vs, a->prefix_v_stride, ep, 2, a->head_dim);
     p.prefix = static_cast<int32_t>(a->prefix);
-    return launch_pass(p, plan.own, 0, s, sms);
+    return launch_pass(p, plan.own, 0, s, sms, false);
+  }
+  if (a->states > 0) {
+    st = launch_pass(p, plan.own, 0, s, sms, false);
+    if (st != INTP_OK) return st;
   }
   if (a->prefix > 0) {
+    // After the own states' pass, which ends in a partly filled GPU: this one moves in.
     XaParams x = p;
     x.shared = 1;
     x.states = static_cast<int32_t>(a->prefix);
@@ -314,11 +319,7 @@ intp_status xattn_forward(const xattn_args* a, void* stream) {
     x.ks[0] = x.vs[0] = 0;
     take_strides(x.ks + 1, a->prefix_k_stride, ep, 2, a->head_dim);
     take_strides(x.vs + 1, a->prefix_v_stride, ep, 2, a->head_dim);
-    st = launch_pass(x, plan.pre, 0, s, sms);
-    if (st != INTP_OK) return st;
-  }
-  if (a->states > 0) {
-    st = launch_pass(p, plan.own, plan.pre_slots, s, sms);
+    st = launch_pass(x, plan.pre, plan.own_slots, s, sms, a->states > 0);
     if (st != INTP_OK) return st;
   }
   if (!plan.parts) return INTP_OK;

@@ -142,6 +142,7 @@ xattn_rows_kernel(const RowsArgs a) {
   constexpr int kJoinStride = DP + 4;       // floats
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float m_s[kWarps][kTile], l_s[kWarps][kTile], w_s[kWarps][kTile];
+  allow_next_kernel();
   const XaParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;    // fragment row and column pair
@@ -512,6 +513,7 @@ xattn_rows_kernel(const RowsArgs a) {
         p.lse[lin] = lse2 * kLn2;
     }
   }
+  wait_previous_kernel();
 }
 
 // out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max), one warp per row, parts in order.
@@ -519,6 +521,7 @@ xattn_rows_kernel(const RowsArgs a) {
 template <bool BF16>
 __global__ void __launch_bounds__(128)
 xattn_combine_kernel(const XaParams p, int32_t n_slots) {
+  wait_previous_kernel();
   const int lane = threadIdx.x & 31;
   const int64_t lin = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (lin >= p.rows_total) return;
@@ -562,7 +565,7 @@ xattn_combine_kernel(const XaParams p, int32_t n_slots) {
 }
 
 template <int DP, bool BF16, bool FP8, int NT>
-int32_t launch(RowsArgs a, cudaStream_t stream) {
+int32_t launch(RowsArgs a, cudaStream_t stream, bool overlap) {
   using L = RowsShape<DP, FP8>;
   auto kernel = xattn_rows_kernel<DP, BF16, FP8, NT>;
   constexpr int kJoin = kWarps * 8 * NT * (DP + 4) * 4;   // the warps' sums, in the rings' place
@@ -577,36 +580,32 @@ int32_t launch(RowsArgs a, cudaStream_t stream) {
   a.n_rt = (a.p.rows + 8 * NT - 1) / (8 * NT);
   const int64_t grid = static_cast<int64_t>(a.n_rt) * a.p.instances * a.p.n_split;
   if (grid > INT32_MAX) return 8;
-  kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? 0 : 6;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, stream, overlap, a) ? 0 : 6;
 }
 
 template <bool BF16, bool FP8>
-int32_t launch_dim(const RowsArgs& a, cudaStream_t stream) {
+int32_t launch_dim(const RowsArgs& a, cudaStream_t stream, bool overlap) {
   const bool narrow = a.p.rows <= 8;
   if (a.p.head_dim <= 64)
-    return narrow ? launch<64, BF16, FP8, 1>(a, stream) : launch<64, BF16, FP8, 2>(a, stream);
-  return narrow ? launch<128, BF16, FP8, 1>(a, stream) : launch<128, BF16, FP8, 2>(a, stream);
+    return narrow ? launch<64, BF16, FP8, 1>(a, stream, overlap) : launch<64, BF16, FP8, 2>(a, stream, overlap);
+  return narrow ? launch<128, BF16, FP8, 1>(a, stream, overlap) : launch<128, BF16, FP8, 2>(a, stream, overlap);
 }
 
 }  // namespace
 
-int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream) {
+int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream, bool overlap) {
   RowsArgs a;
   a.p = p;
   const bool fp8 = p.k_exp != nullptr, bf16 = p.dtype == 2;
-  if (fp8) return bf16 ? launch_dim<true, true>(a, stream) : launch_dim<false, true>(a, stream);
-  return bf16 ? launch_dim<true, false>(a, stream) : launch_dim<false, false>(a, stream);
+  if (fp8) return bf16 ? launch_dim<true, true>(a, stream, overlap) : launch_dim<false, true>(a, stream, overlap);
+  return bf16 ? launch_dim<true, false>(a, stream, overlap) : launch_dim<false, false>(a, stream, overlap);
 }
 
 int32_t launch_xattn_combine(const XaParams& p, int32_t n_slots, cudaStream_t stream) {
   const int64_t grid = (p.rows_total + 3) / 4;
   if (grid > INT32_MAX) return 8;
-  if (p.dtype == 2)
-    xattn_combine_kernel<true><<<static_cast<unsigned>(grid), 128, 0, stream>>>(p, n_slots);
-  else
-    xattn_combine_kernel<false><<<static_cast<unsigned>(grid), 128, 0, stream>>>(p, n_slots);
-  return cudaGetLastError() == cudaSuccess ? 0 : 6;
+  auto kernel = p.dtype == 2 ? xattn_combine_kernel<true> : xattn_combine_kernel<false>;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), 128, 0, stream, true, p, n_slots) ? 0 : 6;
 }
 
 }  // namespace intp

@@ -149,6 +149,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const XaParams& p = a.p;
   volatile int32_t* abort_flag = &bars->abort;
 
+  allow_next_kernel();
   if (threadIdx.x == 0) {
     for (int s = 0; s < KS; ++s) {
       mbar_init(&bars->full[s], 1);
@@ -517,6 +518,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
   }
 
+  wait_previous_kernel();
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -526,19 +528,19 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 }
 
 template <int DP, bool BF16>
-int32_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int64_t grid, cudaStream_t stream) {
+int32_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int64_t grid, cudaStream_t stream,
+               bool overlap) {
   auto kernel = xattn_tiles_kernel<DP, BF16>;
   constexpr int smem = Shape<DP>::bars + sizeof(Bars<Shape<DP>::kStages>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
   if (!allow_smem(kernel, smem, done)) return 6;
-  kernel<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(mk, mv, a);
-  return cudaGetLastError() == cudaSuccess ? 0 : 6;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, stream, overlap, mk, mv, a) ? 0 : 6;
 }
 
 }  // namespace
 
-int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count) {
+int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count, bool overlap) {
   Args a;
   a.p = p;
   a.n_rt = (p.rows + kXaTileRows - 1) / kXaTileRows;
@@ -559,8 +561,10 @@ int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count)
   if (!make_map(&mk, &a.ok, p.k, ks, t, BN) || !make_map(&mv, &a.ov, p.v, vs, t, BN)) return 4;
   const int64_t grid = items < sm_count ? items : sm_count;
   if (p.head_dim <= 64)
-    return p.dtype == 2 ? launch<64, true>(mk, mv, a, grid, stream) : launch<64, false>(mk, mv, a, grid, stream);
-  return p.dtype == 2 ? launch<128, true>(mk, mv, a, grid, stream) : launch<128, false>(mk, mv, a, grid, stream);
+    return p.dtype == 2 ? launch<64, true>(mk, mv, a, grid, stream, overlap)
+                        : launch<64, false>(mk, mv, a, grid, stream, overlap);
+  return p.dtype == 2 ? launch<128, true>(mk, mv, a, grid, stream, overlap)
+                      : launch<128, false>(mk, mv, a, grid, stream, overlap);
 }
 
 }  // namespace intp

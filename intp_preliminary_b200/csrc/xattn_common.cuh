@@ -26,6 +26,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatil
   }
 }
 
+// Programmatic dependent launch within one call: the next kernel may start once every CTA of
+// this one has said so (or left); it waits where it needs this one's results, and at the latest
+// before its own end, so that a kernel's end always means its predecessors' too.  Both are
+// no-ops in a kernel that was launched plainly.
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);

@@ -67,13 +67,31 @@ inline bool allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return true;
 }
 
+// Launches a kernel that may overlap the end of the one before it on the stream (`overlap`), or plainly.
+template <class... P, class... A>
+inline bool launch_kernel(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, bool overlap,
+                          A&&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess;
+}
+
 constexpr int kXaTileRows = 256;   // rows of a tcgen05 work item (two warpgroups of 128)
 constexpr int kXaTileKeys = 128;
 constexpr int kXaRowsTile = 16;    // rows of a few-rows work item
 constexpr int kXaRowsKeys8 = 2048; // keys of an 8-bit part at most: their exponents sit in shared memory
 
-int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count);
-int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream);
+// `overlap`: the call's second pass; it does not read what the first one writes.
+int32_t launch_xattn_tiles(const XaParams& p, cudaStream_t stream, int sm_count, bool overlap);
+int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream, bool overlap);
 // Joins n slots of part_o / part_lse into out / lse.
 int32_t launch_xattn_combine(const XaParams& p, int32_t n_slots, cudaStream_t stream);
 int32_t launch_xattn_backward(const XaBwdParams& p, cudaStream_t stream, int sm_count);

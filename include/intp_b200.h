@@ -341,7 +341,7 @@ INTP_API const char* intp_status_string(intp_status status);
 typedef struct xattn_args {
   const void* q; const void* k; const void* v;
   /* 8-bit states: one exponent byte per (sequence, head, state), unit stride along
-   * states; k and v then hold e4m3 codes and stand for code * 2^(byte - 127).
+   * states; k and v then hold e4m3 codes and stand for code * 2^(byte - 127), byte 1 to 254.
    * Null for 16-bit states. */
   const uint8_t* k_exponents; const uint8_t* v_exponents;
   /* States that every sequence shares, (G, P, D), read before the sequence's own; null without. */

@@ -18,38 +18,46 @@
 namespace intp {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kUnroll = 4;
 
 struct CacheArgs {
   int32_t batch, groups, capacity, count, head_dim;
-  int64_t n_rows;                        // of k (as many again of v)
+  int32_t blocks;                        // of one sequence and key head
   void* x[2]; int64_t xs[2][3];          // k, v: batch, group, state strides
   uint8_t* codes[2];
   uint8_t* exps[2];
   const int32_t* start; const int32_t* counts;
 };
 
-struct RowAt {
-  uint16_t* x;                           // the row's 16-bit values
-  int64_t cache;                         // cache row, or -1 outside it / past the sequence's count
-  int32_t which;
+// The rows of one block: consecutive states of one sequence and key head, of k or of v, so what
+// a row's place takes of arithmetic is a block's.
+struct Rows {
+  uint16_t* x; int64_t stride;           // the 16-bit rows
+  uint8_t* codes; uint8_t* exps;         // the cache's, of the sequence and head
+  int64_t start;                         // cache row of state 0
+  int32_t first, counted;                // this thread's first state; states that are copied
 };
 
-__device__ __forceinline__ RowAt row_at(const CacheArgs& a, int64_t row) {
-  RowAt r;
-  r.which = row >= a.n_rows ? 1 : 0;
-  const uint32_t x = static_cast<uint32_t>(row - (r.which ? a.n_rows : 0));  // n_rows < 2^31 (checked on the host)
-  const uint32_t bg = x / static_cast<uint32_t>(a.count);
-  const int32_t i = static_cast<int32_t>(x - bg * a.count);
-  const int32_t b = static_cast<int32_t>(bg / static_cast<uint32_t>(a.groups));
-  const int32_t g = static_cast<int32_t>(bg - b * a.groups);
-  const int64_t at = (a.start == nullptr ? 0 : static_cast<int64_t>(a.start[b])) + i;
-  const bool in = at >= 0 && at < a.capacity && (a.counts == nullptr || i < a.counts[b]);
-  r.cache = in ? static_cast<int64_t>(bg) * a.capacity + at : -1;
-  const int64_t* s = a.xs[r.which];
-  r.x = static_cast<uint16_t*>(a.x[r.which]) + b * s[0] + g * s[1] + i * s[2];
+template <int LPR>
+__device__ __forceinline__ Rows block_rows(const CacheArgs& a) {
+  const int32_t outer = blockIdx.x / a.blocks, bg = outer >> 1, which = outer & 1;
+  const int32_t b = bg / a.groups, g = bg - b * a.groups;
+  const int64_t* s = a.xs[which];
+  Rows r;
+  r.x = static_cast<uint16_t*>(a.x[which]) + b * s[0] + g * s[1];
+  r.stride = s[2];
+  r.codes = a.codes[which] + static_cast<int64_t>(bg) * a.capacity * a.head_dim;
+  r.exps = a.exps[which] + static_cast<int64_t>(bg) * a.capacity;
+  r.start = a.start == nullptr ? 0 : a.start[b];
+  r.counted = a.counts == nullptr || a.counts[b] > a.count ? a.count : a.counts[b];
+  r.first = (blockIdx.x - outer * a.blocks) * (kThreads / LPR * kUnroll) + threadIdx.x / LPR;
   return r;
+}
+// Cache row of state i, or -1 outside the cache or past the sequence's count.
+__device__ __forceinline__ int64_t cache_row(const CacheArgs& a, const Rows& r, int32_t i) {
+  const int64_t at = r.start + i;
+  return i < r.counted && at >= 0 && at < a.capacity ? at : -1;
 }
 
 // The smallest e >= -126 with amax <= 448 * 2^e (448 = 1.75 * 2^8), 0 for amax = 0.
@@ -69,22 +77,19 @@ cache_write_kernel(const CacheArgs a) {
   constexpr int kRowsPer = kThreads / LPR;
   constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;     // bits of infinity: magnitudes at or above are not finite
   const int sub = threadIdx.x % LPR;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kUnroll) * kRowsPer + threadIdx.x / LPR;
+  const Rows rows = block_rows<LPR>(a);
   const bool col = sub * 16 < a.head_dim;
-  RowAt at[kUnroll];
+  int64_t at[kUnroll];
   uint4 v[kUnroll][2];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t row = first + u * kRowsPer;
-    at[u].cache = -1;
+    const int32_t i = rows.first + u * kRowsPer;
+    at[u] = cache_row(a, rows, i);
     v[u][0] = v[u][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < 2 * a.n_rows) {
-      at[u] = row_at(a, row);
-      if (col && at[u].cache >= 0) {
-        const uint4* src = reinterpret_cast<const uint4*>(at[u].x + sub * 16);
-        v[u][0] = __ldcs(src);
-        v[u][1] = __ldcs(src + 1);
-      }
+    if (col && at[u] >= 0) {
+      const uint4* src = reinterpret_cast<const uint4*>(rows.x + i * rows.stride + sub * 16);
+      v[u][0] = __ldcs(src);
+      v[u][1] = __ldcs(src + 1);
     }
   }
 #pragma unroll
@@ -122,10 +127,10 @@ cache_write_kernel(const CacheArgs a) {
       }
       codes[h] = __byte_perm(c[0], c[1], 0x5410);
     }
-    if (at[u].cache >= 0 && col) {
-      __stcs(reinterpret_cast<uint4*>(a.codes[at[u].which] + at[u].cache * a.head_dim + sub * 16),
+    if (at[u] >= 0 && col) {
+      __stcs(reinterpret_cast<uint4*>(rows.codes + at[u] * a.head_dim + sub * 16),
              make_uint4(codes[0], codes[1], codes[2], codes[3]));
-      if (sub == 0) a.exps[at[u].which][at[u].cache] = static_cast<uint8_t>(e + 127);
+      if (sub == 0) rows.exps[at[u]] = static_cast<uint8_t>(e + 127);
     }
   }
 }
@@ -159,41 +164,38 @@ cache_read_kernel(const CacheArgs a) {
   constexpr int32_t kSafe = BF16 ? 119 : 7;   // 448 * 2^e is within the type
   const int sub = threadIdx.x % LPR;
   if (sub * 16 >= a.head_dim) return;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kUnroll) * kRowsPer + threadIdx.x / LPR;
-  RowAt at[kUnroll];
+  const Rows rows = block_rows<LPR>(a);
   uint4 c[kUnroll];
   int32_t e[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t row = first + u * kRowsPer;
-    at[u].cache = -1;
+    const int64_t at = cache_row(a, rows, rows.first + u * kRowsPer);
     c[u] = make_uint4(0u, 0u, 0u, 0u);
     e[u] = 0;
-    if (row < 2 * a.n_rows) {
-      at[u] = row_at(a, row);
-      if (at[u].cache >= 0) {
-        c[u] = __ldg(reinterpret_cast<const uint4*>(a.codes[at[u].which] + at[u].cache * a.head_dim + sub * 16));
-        e[u] = static_cast<int32_t>(__ldg(a.exps[at[u].which] + at[u].cache)) - 127;
-      }
+    if (at >= 0) {
+      c[u] = __ldcs(reinterpret_cast<const uint4*>(rows.codes + at * a.head_dim + sub * 16));
+      e[u] = static_cast<int32_t>(__ldg(rows.exps + at)) - 127;
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    if (first + u * kRowsPer >= 2 * a.n_rows) continue;
+    const int32_t i = rows.first + u * kRowsPer;
+    if (i >= a.count) continue;
     const float up = power_of_two(e[u]);
     const bool clamp = e[u] > kSafe;
     const uint2 r0 = decode4<BF16>(c[u].x, up, clamp), r1 = decode4<BF16>(c[u].y, up, clamp);
     const uint2 r2 = decode4<BF16>(c[u].z, up, clamp), r3 = decode4<BF16>(c[u].w, up, clamp);
-    uint4* dst = reinterpret_cast<uint4*>(at[u].x + sub * 16);
+    uint4* dst = reinterpret_cast<uint4*>(rows.x + i * rows.stride + sub * 16);
     __stcs(dst, make_uint4(r0.x, r0.y, r1.x, r1.y));
     __stcs(dst + 1, make_uint4(r2.x, r2.y, r3.x, r3.y));
   }
 }
 
 template <int LPR, bool BF16>
-int32_t launch(const CacheArgs& a, bool write, cudaStream_t stream) {
-  const int64_t per = static_cast<int64_t>(kThreads / LPR) * kUnroll;
-  const int64_t grid = (2 * a.n_rows + per - 1) / per;
+int32_t launch(CacheArgs a, bool write, cudaStream_t stream) {
+  constexpr int32_t per = kThreads / LPR * kUnroll;
+  a.blocks = static_cast<int32_t>((static_cast<int64_t>(a.count) + per - 1) / per);
+  const int64_t grid = 2 * static_cast<int64_t>(a.batch) * a.groups * a.blocks;
   if (grid > INT32_MAX) return INTP_ERR_SHAPE;
   if (write)
     cache_write_kernel<LPR, BF16><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a);
@@ -216,8 +218,8 @@ int32_t run(const state_cache_args* c, bool write, cudaStream_t stream) {
   if (c->dtype != INTP_F16 && c->dtype != INTP_BF16) return INTP_ERR_DTYPE;
   if (c->batch == 0 || c->groups == 0 || c->count == 0) return INTP_OK;
   for (int64_t n : {c->batch, c->groups, c->capacity, c->count})
-    if (n > INT32_MAX) return INTP_ERR_SHAPE;
-  if (c->batch * c->groups > INT32_MAX / c->count) return INTP_ERR_SHAPE;
+    if (n > (int64_t(1) << 30)) return INTP_ERR_SHAPE;
+  if (c->batch * c->groups > INT32_MAX / 2) return INTP_ERR_SHAPE;
   if (!c->k || !c->v || !c->k_codes || !c->v_codes || !c->k_exponents || !c->v_exponents) return INTP_ERR_ARGUMENT;
   const int64_t extent[3] = {c->batch, c->groups, c->count};
   if (!row_layout_ok(c->k, c->k_stride, extent) || !row_layout_ok(c->v, c->v_stride, extent)) return INTP_ERR_LAYOUT;
@@ -232,7 +234,6 @@ int32_t run(const state_cache_args* c, bool write, cudaStream_t stream) {
   a.capacity = static_cast<int32_t>(c->capacity);
   a.count = static_cast<int32_t>(c->count);
   a.head_dim = static_cast<int32_t>(c->head_dim);
-  a.n_rows = c->batch * c->groups * c->count;
   a.x[0] = c->k;
   a.x[1] = c->v;
   std::memcpy(a.xs[0], c->k_stride, sizeof(a.xs[0]));

@@ -1,7 +1,7 @@
 """The 8-bit cache of an encoder's key / value states, and attention over it.
 
 A state's row of D values (one sequence, one key head) is held as e4m3 codes
-and one exponent byte and stands for ``code * 2^(byte - 127)``; the power of
+and one exponent byte (1 to 254) and stands for ``code * 2^(byte - 127)``; the power of
 two is the smallest whose 448-fold (e4m3's largest value) reaches the row's
 largest finite value, no smaller than 2^-126.  So a value that is normal in
 e4m3 is off by at most 2^-4 of itself, and a row costs D + 1 bytes instead of

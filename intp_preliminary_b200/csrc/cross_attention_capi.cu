@@ -56,12 +56,19 @@ intp_status check_shape(const xattn_args* a) {
 struct Pass {
   bool tiles;            // tcgen05 kernel, else the few-rows kernel
   int64_t n_split, split_keys;
+  int32_t warps;         // of a few-rows CTA
 };
 
 // Rows of an instance up to which the few-rows kernel is taken: a 128-row tcgen05 tile
 // costs the same for 1 row as for 128, the few-rows kernel reads the states once for
 // each 16 rows.
 constexpr int64_t kRowsMax = 32;
+
+// Few states and no more CTAs than SMs: one part, read by 8 warps, and no second launch that
+// joins parts.  Measured, one part against several (a pass among others, and on the GPU alone):
+// 600 states of D128 10.7 / 14.6 us (8.4 / 8.0), 1000 of D64 10.5 / 13.7 (9.0 / 6.9), 1000 of D128
+// 12.4 / 14.6 (11.0 / 7.5), 1500 of D128 16.5 / 14.7 (14.4 / 7.7).
+bool one_part(int64_t items, int64_t states) { return items <= kPlanSms && states <= 1024; }
 
 Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t states) {
   Pass s;
@@ -72,11 +79,21 @@ Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t sta
     int64_t split = items >= kPlanSms ? 1 : std::min(kPlanSms / items, std::max<int64_t>(tiles / 2, 1));
     s.split_keys = ceil_div(tiles, split) * intp::kXaTileKeys;
   } else {
-    // Several CTAs per SM, parts of 256 keys at least; one part up to 512 keys, where the
-    // second kernel that joins parts costs more than it gains.
     const int64_t items = instances * ceil_div(rows, intp::kXaRowsTile);
-    int64_t split = states <= 512 ? 1 : std::min(ceil_div(kPlanSms * 8, items), ceil_div(states, 256));
-    if (a->eight_bit) split = std::max(split, ceil_div(states, intp::kXaRowsKeys8));
+    int64_t split = 1;
+    if (one_part(items, states)) {
+      s.warps = 8;
+    } else {
+      // As many CTAs as the GPU holds at once: two an SM, four of 8-bit states.  At B32 G8 N1000
+      // D128 that is one part, 24.9 us (two: 30.4, five: 34.7); at B8 G8 N4000 of 8 bits nine
+      // parts, 17.7 us (four: 21.3).  Parts of 128 keys at least (B2 G2 N1000: 7.7 us, of 256
+      // 9.2), of 256 where there would be more than 16 (N16000: 18.5 us, of 128 29.1).
+      s.warps = 4;
+      const int64_t held = kPlanSms * (a->eight_bit ? 4 : 2);
+      split = std::min({std::max<int64_t>(held / items, 1), ceil_div(states, 128),
+                        std::max<int64_t>(ceil_div(states, 256), 16)});
+      if (a->eight_bit) split = std::max(split, ceil_div(states, intp::kXaRowsKeys8));
+    }
     s.split_keys = ceil_div(ceil_div(states, split), 128) * 128;
   }
   s.n_split = ceil_div(states, s.split_keys);
@@ -113,6 +130,7 @@ Plan plan_forward(const xattn_args* a) {
   if (p.joined) {
     p.own.n_split = 1;
     p.own.split_keys = std::max<int64_t>(a->states, 1);
+    p.own.warps = a->batch * a->groups * ceil_div(per_group * a->queries, intp::kXaRowsTile) <= kPlanSms ? 8 : 4;
     p.own_slots = 1;
     return p;
   }
@@ -191,6 +209,7 @@ int32_t launch_pass(XaParams p, const Pass& s, int64_t first, cudaStream_t strea
   p.n_split = static_cast<int32_t>(s.n_split);
   p.split_keys = static_cast<int32_t>(s.split_keys);
   p.part_first = static_cast<int32_t>(first);
+  p.warps = s.warps;
   return s.tiles ? intp::launch_xattn_tiles(p, stream, sms, overlap) : intp::launch_xattn_rows(p, stream, overlap);
 }
 

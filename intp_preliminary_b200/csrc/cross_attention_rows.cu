@@ -6,7 +6,7 @@
 // Reading the states bounds this: 16 rows or fewer share each key, so a 16-bit
 // state of 4 D bytes carries at most 64 D multiply-adds, far below the tensor
 // cores' ratio.  What counts is bytes in flight and few instructions per byte.
-// A CTA of 4 warps takes 8 or 16 rows and a range of keys; each warp streams its
+// A CTA of 4 (or 8) warps takes 8 or 16 rows and a range of keys; each warp streams its
 // own slices of keys through a private cp.async ring (no CTA barrier in the
 // loop) and keeps its own running maximum and sum.  The products are 16 x 8 x 16
 // matrix instructions with the states as the 16-high operand,
@@ -30,8 +30,6 @@
 namespace intp {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 16;                  // keys of a warp's slice
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;            // log2 units a score may pass its reference by
@@ -45,7 +43,7 @@ struct RowsShape {
   // 8-bit states cost more instructions a byte: less shared memory a CTA and twice the warps an
   // SM (16-key slices, 48 KB: 142 us at B64 G8 H32 N8192 D128; 32-key slices, 96 KB: 178 us).
   static constexpr int kStages = DP == 128 ? 3 : 6;
-  static constexpr int kRing = kWarps * kStages * 2 * kSliceBytes;
+  static constexpr int kWarpRing = kStages * 2 * kSliceBytes;
 };
 
 template <int CH>
@@ -131,9 +129,9 @@ struct RowsArgs {
   int32_t smem_scales;   // bytes from the dynamic shared memory's start to the exponents' values
 };
 
-// NT: tiles of 8 query rows.
-template <int DP, bool BF16, bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads)
+// NT: tiles of 8 query rows.  kWarps: 4, or 8 where a grid of one part leaves SMs empty.
+template <int DP, bool BF16, bool FP8, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32)
 xattn_rows_kernel(const RowsArgs a) {
   using L = RowsShape<DP, FP8>;
   constexpr int CH = L::kChunks, NS = L::kStages;
@@ -233,7 +231,7 @@ xattn_rows_kernel(const RowsArgs a) {
   uint16_t* exp_s = reinterpret_cast<uint16_t*>(smem + a.smem_scales);
   if (FP8) {
     const int64_t base = b * p.es[0] + grp * p.es[1] + key0;
-    for (int i = threadIdx.x; i < n_keys; i += kThreads)
+    for (int i = threadIdx.x; i < n_keys; i += kWarps * 32)
       exp_s[i] = static_cast<uint16_t>(p.k_exp[base + i] | (p.v_exp[base + i] << 8));
   }
 
@@ -516,14 +514,17 @@ xattn_rows_kernel(const RowsArgs a) {
   wait_previous_kernel();
 }
 
-// out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max), one warp per row, parts in order.
-// Lane s holds part s's weight, so the parts' values are loaded without waiting for one another.
-template <bool BF16>
+// out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max), WPR warps per row (warp i takes parts
+// i, i + WPR, .. in order, warps are joined in order).  Lane l holds the weight of its warp's l-th
+// part, so the parts' values are loaded without waiting for one another.
+template <bool BF16, int WPR>
 __global__ void __launch_bounds__(128)
 xattn_combine_kernel(const XaParams p, int32_t n_slots) {
+  __shared__ float4 acc_s[WPR > 1 ? WPR : 1][32];
+  __shared__ float total_s[WPR > 1 ? WPR : 1];
   wait_previous_kernel();
-  const int lane = threadIdx.x & 31;
-  const int64_t lin = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = WPR > 1 ? warp : 0;
+  const int64_t lin = WPR > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + warp;
   if (lin >= p.rows_total) return;
   float top = -INFINITY;
   for (int s = lane; s < n_slots; s += 32) top = max_nan(top, p.part_lse[s * p.rows_total + lin]);
@@ -533,25 +534,37 @@ xattn_combine_kernel(const XaParams p, int32_t n_slots) {
   const int d = lane * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.f;
-  for (int s0 = 0; s0 < n_slots; s0 += 32) {
+  for (int s0 = part; s0 < n_slots; s0 += 32 * WPR) {
     float mine = 0.f;
-    if (s0 + lane < n_slots) {
-      const float e = p.part_lse[(s0 + lane) * p.rows_total + lin];
+    if (s0 + lane * WPR < n_slots) {
+      const float e = p.part_lse[(s0 + lane * WPR) * p.rows_total + lin];
       mine = e == -INFINITY ? 0.f : fast_exp2(e - top);
     }
-    const int n = n_slots - s0 < 32 ? n_slots - s0 : 32;
+    const int left = (n_slots - s0 + WPR - 1) / WPR, n = left < 32 ? left : 32;
     const float* src = p.part_o + (s0 * p.rows_total + lin) * p.head_dim + d;
 #pragma unroll 8
     for (int s = 0; s < n; ++s) {
       const float w = __shfl_sync(0xffffffffu, mine, s);
       total += w;
       if (w != 0.f && d < p.head_dim) {  // an empty part's values were never written
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(src + s * p.rows_total * p.head_dim));
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(src + s * WPR * p.rows_total * p.head_dim));
         acc.x = fmaf(v.x, w, acc.x);
         acc.y = fmaf(v.y, w, acc.y);
         acc.z = fmaf(v.z, w, acc.z);
         acc.w = fmaf(v.w, w, acc.w);
       }
+    }
+  }
+  if (WPR > 1) {
+    acc_s[part][lane] = acc;
+    if (lane == 0) total_s[part] = total;
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int i = 1; i < WPR; ++i) {
+      const float4 v = acc_s[i][lane];
+      acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+      total += total_s[i];
     }
   }
   const float inv = none ? 0.f : 1.f / total;
@@ -564,14 +577,15 @@ xattn_combine_kernel(const XaParams p, int32_t n_slots) {
   if (lane == 0 && p.lse != nullptr) p.lse[lin] = none ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
-template <int DP, bool BF16, bool FP8, int NT>
+template <int DP, bool BF16, bool FP8, int NT, int W>
 int32_t launch(RowsArgs a, cudaStream_t stream, bool overlap) {
   using L = RowsShape<DP, FP8>;
-  auto kernel = xattn_rows_kernel<DP, BF16, FP8, NT>;
-  constexpr int kJoin = kWarps * 8 * NT * (DP + 4) * 4;   // the warps' sums, in the rings' place
-  constexpr int kData = L::kRing > kJoin ? L::kRing : kJoin;
+  auto kernel = xattn_rows_kernel<DP, BF16, FP8, NT, W>;
+  constexpr int kRing = W * L::kWarpRing;
+  constexpr int kJoin = W * 8 * NT * (DP + 4) * 4;   // the warps' sums, in the rings' place
+  constexpr int kData = kRing > kJoin ? kRing : kJoin;
   constexpr int kMost = kData + (FP8 ? 2 * kXaRowsKeys8 : 0);
-  static_assert(kMost <= 227 * 1024, "shared memory of a CTA");
+  static_assert(kMost <= 224 * 1024, "shared memory of a CTA");
   a.smem_scales = kData;
   const int smem = kData + (FP8 ? 2 * a.p.split_keys : 0);
   static std::atomic<uint64_t> done{0};
@@ -580,15 +594,21 @@ int32_t launch(RowsArgs a, cudaStream_t stream, bool overlap) {
   a.n_rt = (a.p.rows + 8 * NT - 1) / (8 * NT);
   const int64_t grid = static_cast<int64_t>(a.n_rt) * a.p.instances * a.p.n_split;
   if (grid > INT32_MAX) return 8;
-  return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, stream, overlap, a) ? 0 : 6;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), W * 32, smem, stream, overlap, a) ? 0 : 6;
+}
+
+template <int DP, bool BF16, bool FP8>
+int32_t launch_rows(const RowsArgs& a, cudaStream_t stream, bool overlap) {
+  const bool narrow = a.p.rows <= 8;
+  if (a.p.warps == 8)
+    return narrow ? launch<DP, BF16, FP8, 1, 8>(a, stream, overlap) : launch<DP, BF16, FP8, 2, 8>(a, stream, overlap);
+  return narrow ? launch<DP, BF16, FP8, 1, 4>(a, stream, overlap) : launch<DP, BF16, FP8, 2, 4>(a, stream, overlap);
 }
 
 template <bool BF16, bool FP8>
 int32_t launch_dim(const RowsArgs& a, cudaStream_t stream, bool overlap) {
-  const bool narrow = a.p.rows <= 8;
-  if (a.p.head_dim <= 64)
-    return narrow ? launch<64, BF16, FP8, 1>(a, stream, overlap) : launch<64, BF16, FP8, 2>(a, stream, overlap);
-  return narrow ? launch<128, BF16, FP8, 1>(a, stream, overlap) : launch<128, BF16, FP8, 2>(a, stream, overlap);
+  return a.p.head_dim <= 64 ? launch_rows<64, BF16, FP8>(a, stream, overlap)
+                            : launch_rows<128, BF16, FP8>(a, stream, overlap);
 }
 
 }  // namespace
@@ -602,9 +622,12 @@ int32_t launch_xattn_rows(const XaParams& p, cudaStream_t stream, bool overlap) 
 }
 
 int32_t launch_xattn_combine(const XaParams& p, int32_t n_slots, cudaStream_t stream) {
-  const int64_t grid = (p.rows_total + 3) / 4;
+  // Many parts: a CTA per row, whose four warps share them.
+  const bool many = n_slots >= 8;
+  const int64_t grid = many ? p.rows_total : (p.rows_total + 3) / 4;
   if (grid > INT32_MAX) return 8;
-  auto kernel = p.dtype == 2 ? xattn_combine_kernel<true> : xattn_combine_kernel<false>;
+  auto kernel = p.dtype == 2 ? (many ? xattn_combine_kernel<true, 4> : xattn_combine_kernel<true, 1>)
+                             : (many ? xattn_combine_kernel<false, 4> : xattn_combine_kernel<false, 1>);
   return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), 128, 0, stream, true, p, n_slots) ? 0 : 6;
 }
 

@@ -38,6 +38,7 @@ struct XaParams {
   float* part_o; float* part_lse;
   int64_t rows_total;
   int32_t n_split, split_keys, part_first;
+  int32_t warps;               // few-rows kernel: warps of a CTA (4 or 8)
   int32_t* status;
   uint64_t wait_ns;
 };

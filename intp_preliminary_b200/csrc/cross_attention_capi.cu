@@ -59,10 +59,18 @@ struct Pass {
   int32_t warps;         // of a few-rows CTA
 };
 
-// Rows of an instance up to which the few-rows kernel is taken: a 128-row tcgen05 tile
-// costs the same for 1 row as for 128, the few-rows kernel reads the states once for
-// each 16 rows.
-constexpr int64_t kRowsMax = 32;
+// Rows of an instance up to which the few-rows kernel is taken.  It reads the states once for each
+// 16 rows, a 128-row tcgen05 tile costs the same for 1 row as for 128: at B64 G8 N2000 D128 16 rows
+// take 91.6 us (tiles 104.4), 24 rows 159.3 (105.0).
+constexpr int64_t kRowsMax = 16;
+// While a few states and CTAs fill no more than the SMs, more rows cost it nothing: 64 rows at
+// B8 G4 N300 D64 7.2 us (tiles 9.0), at B1 G3 N196 6.5 (7.7).
+constexpr int64_t kRowsMaxSmall = 64, kSmallStates = 512;
+
+bool few_rows(int64_t rows, int64_t instances, int64_t states) {
+  return rows <= kRowsMax || (rows <= kRowsMaxSmall && states <= kSmallStates &&
+                              instances * ceil_div(rows, intp::kXaRowsTile) <= kPlanSms);
+}
 
 // Few states and no more CTAs than SMs: one part, read by 8 warps, and no second launch that
 // joins parts.  Measured, one part against several (a pass among others, and on the GPU alone):
@@ -72,7 +80,8 @@ bool one_part(int64_t items, int64_t states) { return items <= kPlanSms && state
 
 Pass plan_pass(const xattn_args* a, int64_t rows, int64_t instances, int64_t states) {
   Pass s;
-  s.tiles = a->kernel == XATTN_KERNEL_TILES || (a->kernel == XATTN_KERNEL_AUTO && !a->eight_bit && rows > kRowsMax);
+  s.tiles = a->kernel == XATTN_KERNEL_TILES ||
+            (a->kernel == XATTN_KERNEL_AUTO && !a->eight_bit && !few_rows(rows, instances, states));
   if (s.tiles) {
     // One CTA per SM: the key axis is split until every SM has work, two tiles a part at least.
     const int64_t items = instances * ceil_div(rows, intp::kXaTileRows), tiles = ceil_div(states, intp::kXaTileKeys);

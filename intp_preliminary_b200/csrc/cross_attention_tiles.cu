@@ -13,8 +13,8 @@
 //                   swizzled operand tile itself (rows of an instance have no
 //                   single stride that a tensor map could hold), reads S from
 //                   TMEM, keeps the running maximum and the fp32 row sum, and
-//                   writes P (16-bit) over the S columns.  O is rescaled in TMEM
-//                   only when the maximum grew by more than 2^8.
+//                   writes P (16-bit) to TMEM.  O is rescaled there only when the
+//                   maximum grew by more than 2^8.
 //   warp 8          TMA producer of K and V tiles through one ring; it zeroes the
 //                   V rows of a tile past the sequence's length, since 0 * NaN of
 //                   a padded state would reach the output through the product.
@@ -24,6 +24,12 @@
 // P is rounded to 16 bits because the tensor core takes no wider operand of this
 // rate; S, the softmax statistics and O stay in fp32.  Every mbarrier wait is
 // bounded (sm100_ptx.cuh); on expiry the CTA unwinds and reports.
+//
+// Bound by the chain scores -> exponentials -> product of each warpgroup, which the
+// other one's products fill: at B4 H16 M2048 N4096 D128 227 us, 1.21 PFLOP/s, the
+// tensor pipe busy 64 % of the time (32 % where one lane of a divergent branch issued
+// the products).  Two threads per row (16 softmax warps) measured 249 us: the
+// instructions of four warps a scheduler cost more than the shorter chain gives.
 #include <cuda.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"
@@ -178,161 +184,161 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
 
   if (warp >= kGroups * 4) {
-  regs_dec<kOtherRegs>();
-  if (warp == kLoadWarp) {
-    // -------------------------------------------------------------- producer
-    uint32_t n_loaded = 0;
-    bool ok = true;
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-    }
-    auto load = [&](const CUtensorMap* tm, const MapOrder& o, int32_t row, int32_t g, int32_t b) -> bool {
-      const uint32_t s = n_loaded % KS, n = n_loaded / KS;
-      if (n > 0 &&
-          !warp_wait(&bars->empty[s], (n - 1) & 1, abort_flag, p.status, kDevTimeoutProducer, p.wait_ns))
-        return false;
+    regs_dec<kOtherRegs>();
+    if (warp == kLoadWarp) {
+      // -------------------------------------------------------------- producer
+      uint32_t n_loaded = 0;
+      bool ok = true;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bars->full[s], L::kTileBytes);
-#pragma unroll
-        for (int blk = 0; blk < L::kBlocks; ++blk)
-          tma_load_4d(ring_s + s * L::kTileBytes + blk * kBlockBytes, tm, &bars->full[s], blk * 64,
-                      map_coord(o, 1, row, g, b), map_coord(o, 2, row, g, b), map_coord(o, 3, row, g, b));
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
       }
-      __syncwarp();
-      ++n_loaded;
-      return true;
-    };
-    for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
-      const Item it = decode_item(a, item);
-      const int32_t b = p.shared ? 0 : it.inst / p.groups;
-      const int32_t g = p.shared ? it.inst : it.inst - b * p.groups;
-      for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
-        const int32_t row = it.key0 + j * BN;
-        if (!load(&tm_k, a.ok, row, g, b) || !load(&tm_v, a.ov, row, g, b)) {
-          ok = false;
-          break;
+      auto load = [&](const CUtensorMap* tm, const MapOrder& o, int32_t row, int32_t g, int32_t b) -> bool {
+        const uint32_t s = n_loaded % KS, n = n_loaded / KS;
+        if (n > 0 &&
+            !warp_wait(&bars->empty[s], (n - 1) & 1, abort_flag, p.status, kDevTimeoutProducer, p.wait_ns))
+          return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->full[s], L::kTileBytes);
+#pragma unroll
+          for (int blk = 0; blk < L::kBlocks; ++blk)
+            tma_load_4d(ring_s + s * L::kTileBytes + blk * kBlockBytes, tm, &bars->full[s], blk * 64,
+                        map_coord(o, 1, row, g, b), map_coord(o, 2, row, g, b), map_coord(o, 3, row, g, b));
         }
-        const int32_t valid = it.key0 + it.n_keys - row;
-        if (valid < BN && it.length < p.states) {
-          // Padded states may hold anything (rows past the tensor's end arrive as zeros).
-          const uint32_t s = (n_loaded - 1) % KS;
-          if (!warp_wait(&bars->full[s], ((n_loaded - 1) / KS) & 1, abort_flag, p.status, kDevTimeoutProducer,
-                         p.wait_ns)) {
+        __syncwarp();
+        ++n_loaded;
+        return true;
+      };
+      for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
+        const Item it = decode_item(a, item);
+        const int32_t b = p.shared ? 0 : it.inst / p.groups;
+        const int32_t g = p.shared ? it.inst : it.inst - b * p.groups;
+        for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
+          const int32_t row = it.key0 + j * BN;
+          if (!load(&tm_k, a.ok, row, g, b) || !load(&tm_v, a.ov, row, g, b)) {
             ok = false;
             break;
           }
-          uint8_t* v_s = ring_s + s * L::kTileBytes;
-          for (int i = valid * 8 + lane; i < BN * 8; i += 32)
+          const int32_t valid = it.key0 + it.n_keys - row;
+          if (valid < BN && it.length < p.states) {
+            // Padded states may hold anything (rows past the tensor's end arrive as zeros).
+            const uint32_t s = (n_loaded - 1) % KS;
+            if (!warp_wait(&bars->full[s], ((n_loaded - 1) / KS) & 1, abort_flag, p.status, kDevTimeoutProducer,
+                           p.wait_ns)) {
+              ok = false;
+              break;
+            }
+            uint8_t* v_s = ring_s + s * L::kTileBytes;
+            for (int i = valid * 8 + lane; i < BN * 8; i += 32)
 #pragma unroll
-            for (int blk = 0; blk < L::kBlocks; ++blk)
-              reinterpret_cast<uint4*>(v_s + blk * kBlockBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->clean[s]);
+              for (int blk = 0; blk < L::kBlocks; ++blk)
+                reinterpret_cast<uint4*>(v_s + blk * kBlockBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->clean[s]);
+          }
         }
       }
-    }
-    // No copy may be in flight into the shared memory of an exiting CTA.
-    volatile int32_t no_abort = 0;
-    for (uint32_t s = 0; s < KS; ++s) {
-      const uint32_t cnt = n_loaded > s ? (n_loaded - s + KS - 1) / KS : 0;
-      if (cnt > 0) mbar_wait(&bars->full[s], (cnt - 1) & 1, &no_abort, p.status, kDevTimeoutDrain);
-    }
-  } else if (warp == kMmaWarp) {
-    // -------------------------------------------------------------- MMA issuer
-    const uint32_t leader = elect_one();
-    const uint32_t idesc_s = idesc_f16(BF16, false, BM, BN);
-    const uint32_t idesc_o = idesc_f16(BF16, true, BM, a.k_steps * 16);
-    const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
-    const uint64_t k_desc = smem_desc_sw128(smem_u32(ring_s), 16, 1024);
-    const uint64_t v_desc = smem_desc_sw128(smem_u32(ring_s), kBlockBytes, 1024);
-    uint32_t n_used = 0;                    // ring tiles consumed
-    uint32_t clean_phase = 0;               // bit s: parity of stage s's next cleaned tile
-    uint32_t gen[kGroups] = {0, 0};         // key tiles started per warpgroup
-    uint32_t q_gen[kGroups] = {0, 0};
-    bool ok = true, issued = false;
-    auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
-      return warp_wait(bar, phase & 1, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
-    };
-    // S_w = q_w k^T from ring stage s into the columns of the previous P_w.  The product that
-    // reads that P was issued before by this warp, and products execute in issue order.
-    auto issue_s = [&](int w, uint32_t s) {
-      const uint64_t qd = q_desc + ((w * L::kTileBytes) >> 4), kd = k_desc + ((s * L::kTileBytes) >> 4);
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t off = ((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
-        if (kk < a.k_steps) mma_ss_warp(leader, tmem + w * BN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+      // No copy may be in flight into the shared memory of an exiting CTA.
+      volatile int32_t no_abort = 0;
+      for (uint32_t s = 0; s < KS; ++s) {
+        const uint32_t cnt = n_loaded > s ? (n_loaded - s + KS - 1) / KS : 0;
+        if (cnt > 0) mbar_wait(&bars->full[s], (cnt - 1) & 1, &no_abort, p.status, kDevTimeoutDrain);
       }
-      mma_commit_warp(leader, &bars->s_full[w]);
-      ++gen[w];
-      issued = true;
-    };
-    for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
-      const Item it = decode_item(a, item);
-      if (it.n_tiles == 0) continue;
-      if (!wait(&bars->full[n_used % KS], n_used / KS)) break;
+    } else if (warp == kMmaWarp) {
+      // -------------------------------------------------------------- MMA issuer
+      const uint32_t leader = elect_one();
+      const uint32_t idesc_s = idesc_f16(BF16, false, BM, BN);
+      const uint32_t idesc_o = idesc_f16(BF16, true, BM, a.k_steps * 16);
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(ring_s), 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(smem_u32(ring_s), kBlockBytes, 1024);
+      uint32_t n_used = 0;                    // ring tiles consumed
+      uint32_t clean_phase = 0;               // bit s: parity of stage s's next cleaned tile
+      uint32_t gen[kGroups] = {0, 0};         // key tiles started per warpgroup
+      uint32_t q_gen[kGroups] = {0, 0};
+      bool ok = true, issued = false;
+      auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {
+        return warp_wait(bar, phase & 1, abort_flag, p.status, kDevTimeoutMma, p.wait_ns);
+      };
+      // S_w = q_w k^T from ring stage s into the columns of the previous P_w.  The product that
+      // reads that P was issued before by this warp, and products execute in issue order.
+      auto issue_s = [&](int w, uint32_t s) {
+        const uint64_t qd = q_desc + ((w * L::kTileBytes) >> 4), kd = k_desc + ((s * L::kTileBytes) >> 4);
 #pragma unroll
-      for (int w = 0; w < kGroups; ++w) {
-        if (w >= it.active || !ok) continue;
-        ok = wait(&bars->q_full[w], q_gen[w]);
-        ++q_gen[w];
-        if (ok) issue_s(w, n_used % KS);
-      }
-      if (!ok) break;
-      mma_commit_warp(leader, &bars->empty[n_used % KS]);
-      for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
-        const uint32_t sv = (n_used + 1) % KS, sk = (n_used + 2) % KS;
-        const bool more = j + 1 < it.n_tiles;
-        const uint64_t vd = v_desc + ((sv * L::kTileBytes) >> 4);
-        // S of the next tile for warpgroup w.
-        auto next_s = [&](int w) {
-          if (!more || w >= it.active || !ok) return;
-          if (w == 0) ok = wait(&bars->full[sk], (n_used + 2) / KS);
-          if (ok && L::kOwnP) ok = wait(&bars->s_free[w], gen[w] - 1);
-          if (!ok) return;
-          tc_fence_after();
-          issue_s(w, sk);
-          if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sk]);
-        };
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
+          if (kk < a.k_steps) mma_ss_warp(leader, tmem + w * BN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        mma_commit_warp(leader, &bars->s_full[w]);
+        ++gen[w];
+        issued = true;
+      };
+      for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
+        const Item it = decode_item(a, item);
+        if (it.n_tiles == 0) continue;
+        if (!wait(&bars->full[n_used % KS], n_used / KS)) break;
 #pragma unroll
         for (int w = 0; w < kGroups; ++w) {
           if (w >= it.active || !ok) continue;
-          if (L::kOwnP) next_s(w);
-          if (w == 0 && ok) {
-            ok = wait(&bars->full[sv], (n_used + 1) / KS);
-            if (ok && it.n_keys - j * BN < BN && it.length < p.states) {
-              ok = wait(&bars->clean[sv], clean_phase >> sv);
-              clean_phase ^= 1u << sv;
-            }
-          }
-          const uint32_t tile = gen[w] - (L::kOwnP && more ? 2 : 1);  // of this warpgroup, whose P comes next
-#pragma unroll
-          // Over S, P's first half is multiplied while the second half's exponentials are taken.
-          for (int half = 0; half < 2; ++half) {
-            if (ok && (half == 0 || !L::kOwnP))
-              ok = wait(half == 0 && !L::kOwnP ? &bars->p_half[w] : &bars->p_full[w], tile);
-            if (!ok) continue;
-            tc_fence_after();
-#pragma unroll
-            for (int kk = half * (BN / 32); kk < (half + 1) * (BN / 32); ++kk)
-              mma_ts_warp(leader, tmem + L::kColO + w * DP, tmem + L::kColP + w * L::kStrideP + kk * 8,
-                          vd + ((kk * 2048) >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-          }
-          if (!ok) continue;
-          mma_commit_warp(leader, &bars->o_done[w]);
-          if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sv]);
-          if (!L::kOwnP) next_s(w);
+          ok = wait(&bars->q_full[w], q_gen[w]);
+          ++q_gen[w];
+          if (ok) issue_s(w, n_used % KS);
         }
-        n_used += 2;
+        if (!ok) break;
+        mma_commit_warp(leader, &bars->empty[n_used % KS]);
+        for (int32_t j = 0; j < it.n_tiles && ok; ++j) {
+          const uint32_t sv = (n_used + 1) % KS, sk = (n_used + 2) % KS;
+          const bool more = j + 1 < it.n_tiles;
+          const uint64_t vd = v_desc + ((sv * L::kTileBytes) >> 4);
+          // S of the next tile for warpgroup w.
+          auto next_s = [&](int w) {
+            if (!more || w >= it.active || !ok) return;
+            if (w == 0) ok = wait(&bars->full[sk], (n_used + 2) / KS);
+            if (ok && L::kOwnP) ok = wait(&bars->s_free[w], gen[w] - 1);
+            if (!ok) return;
+            tc_fence_after();
+            issue_s(w, sk);
+            if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sk]);
+          };
+#pragma unroll
+          for (int w = 0; w < kGroups; ++w) {
+            if (w >= it.active || !ok) continue;
+            if (L::kOwnP) next_s(w);
+            if (w == 0 && ok) {
+              ok = wait(&bars->full[sv], (n_used + 1) / KS);
+              if (ok && it.n_keys - j * BN < BN && it.length < p.states) {
+                ok = wait(&bars->clean[sv], clean_phase >> sv);
+                clean_phase ^= 1u << sv;
+              }
+            }
+            const uint32_t tile = gen[w] - (L::kOwnP && more ? 2 : 1);  // of this warpgroup, whose P comes next
+            // Over S, P's first half is multiplied while the second half's exponentials are taken.
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (ok && (half == 0 || !L::kOwnP))
+                ok = wait(half == 0 && !L::kOwnP ? &bars->p_half[w] : &bars->p_full[w], tile);
+              if (!ok) continue;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = half * (BN / 32); kk < (half + 1) * (BN / 32); ++kk)
+                mma_ts_warp(leader, tmem + L::kColO + w * DP, tmem + L::kColP + w * L::kStrideP + kk * 8,
+                            vd + ((kk * 2048) >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) continue;
+            mma_commit_warp(leader, &bars->o_done[w]);
+            if (w == it.active - 1) mma_commit_warp(leader, &bars->empty[sv]);
+            if (!L::kOwnP) next_s(w);
+          }
+          n_used += 2;
+        }
+      }
+      if (issued) {
+        mma_commit_warp(leader, &bars->drain);
+        volatile int32_t no_abort = 0;
+        mbar_wait(&bars->drain, 0, &no_abort, p.status, kDevTimeoutDrain);
       }
     }
-    if (issued) {
-      mma_commit_warp(leader, &bars->drain);
-      volatile int32_t no_abort = 0;
-      mbar_wait(&bars->drain, 0, &no_abort, p.status, kDevTimeoutDrain);
-    }
-  }
   } else {
     // -------------------------------------------------------------- softmax warpgroups
     regs_inc<kSoftmaxRegs>();
@@ -445,8 +451,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           for (int e = 0; e < 16; ++e) {
             const float2 sv = make_float2(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1]));
             const float2 x = fma2(sv, c2, nm2);
-            const float2 e2 = (e & 3) < kFmaPairs ? exp2_fma(x)
-                                                                   : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            const float2 e2 = (e & 3) < kFmaPairs ? exp2_fma(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
             sum = add2(sum, e2);
             pk[e] = pack2<BF16>(e2.x, e2.y);
           }

@@ -14,7 +14,10 @@
 // so 8 rows fill them (a 128-row tcgen05 tile would idle on 112 rows or more).
 // P^T goes from the first product's layout to the second's by an 8 x 8 transpose
 // in registers.  The reference of the exponentials moves only when a score
-// passes it by 2^8, so a step needs one vote and no shuffles.
+// passes it by 2^8, so a step needs one vote and no shuffles.  Over 16-bit states the
+// probabilities go in as two 16-bit numbers each, the value and what it leaves out: the
+// second product is hidden under the reads, and only the result's own rounding remains
+// (one number each: 1.4 times the error of a 32-bit computation rounded once).
 // The warps join through shared memory at the end; ranges of keys join through a
 // workspace (combine kernel) in a fixed order, so results repeat.
 //
@@ -391,6 +394,7 @@ xattn_rows_kernel(const RowsArgs a) {
       }
     }
     uint32_t pb[NT][2];                     // P^T as the 8-wide operand: keys 2t, 2t+1 of each 8, row g
+    uint32_t pl[NT][2];                     // what its 16 bits leave out (16-bit states)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       // A row without a score above -inf keeps 0 as its reference.
@@ -406,7 +410,12 @@ xattn_rows_kernel(const RowsArgs a) {
           l[n][h] += pr[h];
           if (FP8) pr[h] = fast_exp2(v + w[kh] - refw[h]);
         }
-        pb[n][kh] = transpose8(pack2<MMA_BF16>(pr[0], pr[1]));
+        const uint32_t high = pack2<MMA_BF16>(pr[0], pr[1]);
+        pb[n][kh] = transpose8(high);
+        if (!FP8) {
+          const float2 h = unpack2<MMA_BF16>(high);
+          pl[n][kh] = transpose8(pack2<MMA_BF16>(pr[0] - h.x, pr[1] - h.y));
+        }
       }
     }
 #pragma unroll
@@ -430,8 +439,10 @@ xattn_rows_kernel(const RowsArgs a) {
         // chunk c and c + 1 of keys 0-7, then of 8-15
         ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), c + (mi & 1)), r);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
           mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+          mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
+        }
       }
     }
     __syncwarp();

@@ -439,10 +439,13 @@ xattn_rows_kernel(const RowsArgs a) {
         // chunk c and c + 1 of keys 0-7, then of 8-15
         ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), c + (mi & 1)), r);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
-          mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
-        }
+        for (int n = 0; n < NT; ++n) mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+        // the low parts may be zero or negative: against an infinite value they would turn the
+        // high parts' infinity into NaN, so they meet finite values
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = finite2<MMA_BF16>(r[e]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<MMA_BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
       }
     }
     __syncwarp();

@@ -1,5 +1,6 @@
 // xattn_common.cuh - device pieces that the tensor-core cross-attention kernels share.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "sm100_ptx.cuh"
 
@@ -41,6 +42,21 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// Both values with infinities (and NaN) at the type's largest finite value.
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  if (BF16) {
+    const uint32_t top = 0x7f7f7f7fu, bottom = 0xff7fff7fu;
+    __nv_bfloat162 r = *reinterpret_cast<const __nv_bfloat162*>(&v);
+    r = __hmax2(__hmin2(r, *reinterpret_cast<const __nv_bfloat162*>(&top)), *reinterpret_cast<const __nv_bfloat162*>(&bottom));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  const uint32_t top = 0x7bff7bffu, bottom = 0xfbfffbffu;
+  __half2 r = *reinterpret_cast<const __half2*>(&v);
+  r = __hmax2(__hmin2(r, *reinterpret_cast<const __half2*>(&top)), *reinterpret_cast<const __half2*>(&bottom));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // 32 bytes of one thread, a whole memory sector (dst 32-byte aligned).

@@ -117,6 +117,23 @@ def test_lengths_outside_the_range_are_clamped(cuda_device, kernel):
 
 
 @pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("states,queries,dim,flat", [(1, 1, 64, True), (300, 1, 64, True), (300, 6, 128, False),
+                                                     (2500, 1, 128, False), (37, 3, 72, False)])
+def test_an_infinite_value_makes_its_column_infinite(cuda_device, states, queries, dim, flat, dtype, kernel):
+    """Every weight is positive, so p * inf is inf of the value's sign; the other columns do not see it."""
+    q, k, v = _inputs(1, 2, 1, queries, states, dim, dtype, seed=states)
+    if flat:
+        q.zero_()
+    want, _, bound = oracle.cross_attention(q, k, v, scale=dim ** -0.5)
+    v[0, 0, states // 2, 3], v[0, 0, states - 1, dim - 1] = float("inf"), -float("inf")
+    got, _ = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=dim ** -0.5, kernel=kernel)
+    assert (got[..., 3] == float("inf")).all() and (got[..., dim - 1] == -float("inf")).all()
+    rest = [c for c in range(dim) if c not in (3, dim - 1)]
+    _assert_within(got[..., rest], want[..., rest], bound[..., rest])
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 def test_values_that_are_not_finite_spread_as_in_a_softmax(cuda_device, kernel):
     """A NaN score makes its row NaN; a key with -inf scores drops out; a row of them gives zeros."""
     q, k, v = _inputs(1, 1, 1, 6, 300, 64, BF16, seed=4)

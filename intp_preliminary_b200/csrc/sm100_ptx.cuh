@@ -208,7 +208,7 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 // (elect_one).  A role that a whole warp runs keeps its descriptors and addresses
 // in uniform registers, which the instruction wants; run by one lane of a
 // divergent branch each operand is moved there again for every instruction, and
-// issue, not the tensor core, sets the pace (cross_attention_tiles.cu: 180 against
+// issue, not the tensor core, sets the pace (cross_attention_tiles.cu, by clock probes: about 180 against
 // 64 cycles for a 128 x 128 x 16 product).
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t leader;

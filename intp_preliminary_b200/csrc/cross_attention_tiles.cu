@@ -482,7 +482,9 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         tc_fence_after();
       }
       const int32_t r = it.rt * kXaTileRows + w * BM + row;
-      const float l = sum.x + sum.y;
+      // A score of +inf makes its row NaN, as inf - inf does in a softmax.  The sum alone need not
+      // say so: exp2_fma's clamp takes a NaN for the least exponent.
+      const float l = m == INFINITY ? __int_as_float(0x7fffffff) : sum.x + sum.y;
       // No state, or every score -inf: zeros (exp2_fma leaves 2^-126 where a score is -inf).
       const bool none = m == -INFINITY;
       const float inv = none ? 0.f : 1.f / l;

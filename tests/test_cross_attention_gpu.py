@@ -502,3 +502,40 @@ def test_kernels_agree_on_which_rows_share_a_head(cuda_device):
             out, _ = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, kernel=kernel)
             want = torch.arange(6) // (6 // groups)
             assert (out.cpu().float().round() == want.view(1, 6, 1, 1)).all()
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("states,queries,dim", [(1, 2, 64), (16, 2, 64), (40, 2, 128), (300, 6, 64), (300, 2, 128),
+                                                (3000, 2, 64)])
+def test_a_score_of_plus_infinity_makes_its_row_nan(cuda_device, states, queries, dim, dtype, kernel):
+    """At every position of a group of 16 keys, in the first tile and in the last; a row to which
+    the same key scores -inf does not see it."""
+    batch = 32  # one position of the infinite key each
+    q, k, v = _inputs(batch, 1, 1, queries, states, dim, dtype, seed=states + dim)
+    q[..., 3] = 1.0
+    q[:, :, 1, 3] = -1.0
+    at = [(b if b < 16 else states - 1 - (b - 16)) % states for b in range(batch)]
+    for b, i in enumerate(at):
+        k[b, 0, i, 3] = float("inf")
+    got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=dim ** -0.5, want_lse=True,
+                                       kernel=kernel)
+    up = [m for m in range(queries) if m != 1]
+    assert torch.isnan(got[:, :, up]).all() and torch.isnan(lse[:, :, up]).all()
+    for b, i in enumerate(at):
+        keep = [j for j in range(states) if j != i]
+        want, _, bound = oracle.cross_attention(q[b:b + 1, :, 1:2], k[b:b + 1, :, keep], v[b:b + 1, :, keep],
+                                                scale=dim ** -0.5)
+        _assert_within(got[b:b + 1, :, 1:2], want, bound)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+def test_a_score_past_the_largest_number_makes_its_row_nan(cuda_device, kernel):
+    """Finite operands whose product is not: 2^100 * 2^100 at each of 16 keys."""
+    q, k, v = _inputs(16, 1, 1, 3, 40, 64, BF16, seed=5)
+    q[..., 3] = 2.0 ** 100
+    k[..., 3] = 0
+    for b in range(16):
+        k[b, 0, b, 3] = 2.0 ** 100
+    got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, want_lse=True, kernel=kernel)
+    assert torch.isnan(got).all() and torch.isnan(lse).all()

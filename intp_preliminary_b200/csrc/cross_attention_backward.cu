@@ -85,7 +85,12 @@ struct Args {
   int32_t n_row_tiles, n_split, split_tiles, n_items;
   int32_t k_steps;
   bool wide;                               // gradient rows are 32-byte aligned
-  bool after_stats;                        // the kernel before this one writes the statistics
+  // The kernel before this one writes the statistics.  False for dk / dv after dq, which then reads
+  // them without a wait of its own: it starts only once every dq CTA has called allow_next_kernel
+  // (or left), dq's threads call that after wait_previous_kernel and a fence, and that wait returns
+  // when the statistics' kernel has ended and its writes are in device memory.  The copies (bulk,
+  // through L2) see no cache line from before, and the kernel still waits for dq before its end.
+  bool after_stats;
 };
 
 // One work item: what it owns and what it streams.
@@ -535,8 +540,9 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             const int32_t m = w.row0 + row;
             const float* st = a.stats + (static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 + m / kCols) * (2 * kCols) +
                               m % kCols;
-            next_nlse = __ldg(st);
-            next_ndelta = __ldg(st + kCols);
+            // not __ldg: the kernel that writes them may still run when this one starts
+            next_nlse = __ldcg(st);
+            next_ndelta = __ldcg(st + kCols);
           }
         }
         return true;
@@ -554,7 +560,10 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     };
     uint32_t tile = 0, items = 0;
     bool ok = true;
-    if (!KV) wait_previous_kernel();           // for the statistics
+    if (!KV) {
+      wait_previous_kernel();                  // for the statistics
+      __threadfence();                         // and for whoever starts after this thread (after_stats)
+    }
     // The dk / dv kernel after dq needs the statistics too, and nothing of dq's.
     allow_next_kernel();
     if (fetch(blockIdx.x)) hand_over();

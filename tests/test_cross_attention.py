@@ -172,3 +172,17 @@ def test_oracle_e4m3_table_matches_torch():
     values, exponents = oracle.quantise_rows(x)
     again = (x.double() / torch.exp2(exponents.double())[:, None]).to(torch.float8_e4m3fn).double()
     assert torch.equal(values, again * torch.exp2(exponents.double())[:, None])
+
+
+def test_statistics_are_read_behind_their_writer():
+    """The gradient kernels start while the kernel that writes the row statistics may still run: a
+    read-only load could be moved before the wait or hit an old line, and dk / dv, which does not
+    wait itself, relies on dq's wait and fence standing before dq lets it start."""
+    text = (HEADER.parent.parent / "intp_preliminary_b200" / "csrc" / "cross_attention_backward.cu").read_text()
+    body = text[text.index("xattn_grad_kernel(const"):text.index("split sums")]
+    pointer = re.search(r"const float\* (\w+) = a\.stats", body).group(1)
+    loads = re.findall(rf"(\w+)\({pointer}\b", body)
+    assert loads and set(loads) == {"__ldcg"}
+    assert re.search(r"if \(!KV\) \{\s*wait_previous_kernel\(\);[^}]*__threadfence\(\);[^}]*\}", body)
+    assert body.index("wait_previous_kernel();") < body.index("__threadfence();") < body.index("allow_next_kernel();")
+    assert body.count("allow_next_kernel();") == 1 and "a.after_stats = bp.dq == nullptr;" in text

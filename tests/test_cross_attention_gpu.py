@@ -539,3 +539,26 @@ def test_a_score_past_the_largest_number_makes_its_row_nan(cuda_device, kernel):
         k[b, 0, b, 3] = 2.0 ** 100
     got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, want_lse=True, kernel=kernel)
     assert torch.isnan(got).all() and torch.isnan(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("needs", [(True, True, True), (True, False, False), (False, True, True), (False, False, True)])
+@pytest.mark.parametrize("sizes", [(2, 4, 2, 100, 196, 64), (1, 2, 2, 700, 300, 128), (1, 1, 1, 30, 2000, 64)])
+def test_backwards_in_a_row_use_their_own_statistics(cuda_device, sizes, needs, dtype):
+    """Calls that follow one another at once, on the same workspace memory with other values, give
+    what each gives alone."""
+    sets = []
+    for seed in (150, 250):
+        q, k, v = (t.to(cuda_device) for t in _inputs(*sizes, dtype, seed=seed))
+        grad = _normal(q.shape, dtype, seed + 9).to(cuda_device)
+        out, lse = cross_attention_forward(q, k, v, scale=0.125, want_lse=True)
+        sets.append((q, k, v, out, lse, grad))
+    torch.cuda.synchronize()
+    want = []
+    for s in sets:
+        want.append(cross_attention_backward(*s, scale=0.125, needs=needs))
+        torch.cuda.synchronize()
+    got = [cross_attention_backward(*sets[i % 2], scale=0.125, needs=needs) for i in range(40)]
+    for i, grads in enumerate(got):
+        for a, b in zip(grads, want[i % 2]):
+            assert a is b is None or torch.equal(a, b)

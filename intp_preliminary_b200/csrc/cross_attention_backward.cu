@@ -27,7 +27,12 @@
 // Recomputing the scores in both kernels costs 7 matrix products where 5 would do; in exchange
 // dq needs no cross-CTA sum (fp32 atomics in an order that changes results, or a key-length
 // workspace).
-// P and dS are rounded to 16 bits as the tensor core's operands; all sums are fp32.
+// P and dS are rounded to 16 bits as the tensor core's operands; all sums are fp32.  f16 has
+// full precision for 30 powers of two only, and P is about 1 / N, so there both are held times
+// an exact power of two that the accumulator's store takes out again: P times 2^12, dS times a
+// power that brings a bound of it to 2^12 (dS_i <= P (sum |dO_i| max |v| + |delta_i|)), one per query
+// row in dq (free: it joins the exponent of P), one per item in dk / dv (a multiplication a
+// pair).  The bound's parts come from the statistics kernel, which reads V once for it.
 #include <cuda.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"
@@ -51,6 +56,20 @@ constexpr int kThreads = kFirstRowWarp * 32 + kRowThreads;
 constexpr int kStages = 4;
 constexpr uint32_t kTmemCols = 512, kColAcc = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+// f16: P is held as 2^12 P.  P is at most 1, but for what the scores' own rounding between the
+// forward and here makes of it (a score of 2^24 is an even number): 2^16 P may not be reached.
+constexpr int32_t kPowP = 12;
+
+// f16: the power of two that brings a bound of |dS| / P to [2^11, 2^12), the same distance from
+// overflow; 0 for no bound (zero, or not finite: then the gradients are not either).
+__device__ __forceinline__ int32_t power_for(float bound) {
+  const int32_t e = static_cast<int32_t>(__float_as_uint(bound) >> 23) - 127;
+  return e == 128 || e == -127 ? 0 : kPowP - 1 - e;
+}
+__device__ __forceinline__ float two_to(int32_t e) { return __int_as_float((e + 127) << 23); }
+// Of numbers that are not negative; NaN counts as the largest.
+__device__ __forceinline__ float max_of(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
+__device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 
 // DP: head_dim rounded up to 64 or 128.  KV: the dk / dv kernel.
 template <int DP, bool KV>
@@ -126,13 +145,54 @@ __device__ __forceinline__ Work decode_work(const Args& a, int32_t item) {
 // ============================================================================ row statistics
 // A block takes 64 rows of one head, D / 8 lanes (rounded to a power of two) a row, every
 // lane's loads in flight at once.  Rows past M, and rows without states, get -lse = -inf:
-// their P is zero.
+// their P is zero.  In f16 it also takes what bounds dS: sum |dO| of each row, the largest of
+// it and of |delta| in the block, and, in blocks behind the rows', the largest |v| of 64 states.
+
+// The largest |v| of the visible ones of 64 states.
+template <int LPR>
+__device__ __forceinline__ void state_max(const XaBwdParams& bp, int32_t index) {
+  constexpr int kPerPass = 256 / LPR, kPasses = kCols / kPerPass;
+  __shared__ uint32_t warp_top[8];
+  const XaParams& p = bp.f;
+  const int32_t tiles = (p.states + kCols - 1) / kCols;
+  const int32_t bg = index / tiles, n0 = (index - bg * tiles) * kCols;
+  const int32_t b = bg / p.groups, g = bg - b * p.groups, length = xa_length(p, b);
+  const int sub = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
+  const uint16_t* v = static_cast<const uint16_t*>(p.v) + b * p.vs[0] + g * p.vs[1] + sub * 8;
+  uint4 x[kPasses];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int32_t n = n0 + r0 + i * kPerPass;
+    x[i] = n < length && sub * 8 < p.head_dim ? __ldg(reinterpret_cast<const uint4*>(v + n * p.vs[2]))
+                                              : make_uint4(0u, 0u, 0u, 0u);
+  }
+  uint32_t top = 0u;                       // magnitudes order like their bits
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const uint32_t m = 0x7fff7fffu;
+    top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & m, x[i].y & m), __vmaxu2(x[i].z & m, x[i].w & m)));
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+  if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) top = max(top, warp_top[i]);
+    bp.v_max[index] = unpack2<false>(top).x;
+  }
+}
+
 template <int LPR, bool BF16>
 __global__ void __launch_bounds__(256)
 xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
   constexpr int kPerPass = 256 / LPR, kPasses = kCols / kPerPass;
+  __shared__ float row_max[2][kCols];      // f16: sum |dO| and |delta| of the block's rows
   allow_next_kernel();
   const XaParams& p = bp.f;
+  const int32_t row_blocks = p.batch * p.heads * m_tiles64;
+  if (!BF16 && blockIdx.x >= row_blocks) {
+    state_max<LPR>(bp, blockIdx.x - row_blocks);
+    return;
+  }
   const int32_t bh = blockIdx.x / m_tiles64, m0 = (blockIdx.x - bh * m_tiles64) * kCols;
   const int32_t b = bh / p.heads, h = bh - b * p.heads;
   const int sub = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
@@ -149,18 +209,37 @@ xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
-    float2 sum = make_float2(0.f, 0.f);
+    float2 sum = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum = fma2(unpack2<BF16>(xs[e]), unpack2<BF16>(ys[e]), sum);
-    float delta = sum.x + sum.y;
+    for (int e = 0; e < 4; ++e) {
+      sum = fma2(unpack2<BF16>(xs[e]), unpack2<BF16>(ys[e]), sum);
+      if (!BF16) l1 = add2(l1, unpack2<BF16>(ys[e] & 0x7fff7fffu));
+    }
+    float delta = sum.x + sum.y, row_l1 = l1.x + l1.y;
 #pragma unroll
-    for (int s = LPR / 2; s > 0; s >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, s);
+    for (int s = LPR / 2; s > 0; s >>= 1) {
+      delta += __shfl_xor_sync(0xffffffffu, delta, s);
+      if (!BF16) row_l1 += __shfl_xor_sync(0xffffffffu, row_l1, s);
+    }
     if (sub == 0) {
       const int32_t r = r0 + i * kPerPass, m = m0 + r;
       const float l = m < p.queries ? p.lse[static_cast<int64_t>(bh) * p.queries + m] : -INFINITY;
       float* dst = stats + static_cast<int64_t>(blockIdx.x) * (2 * kCols) + r;
-      dst[0] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+      dst[0] = l == -INFINITY ? -INFINITY : BF16 ? -l * kLog2e : fmaf(-l, kLog2e, static_cast<float>(kPowP));
       dst[kCols] = -delta;
+      if (!BF16) {
+        bp.row_l1[static_cast<int64_t>(blockIdx.x) * kCols + r] = row_l1;
+        row_max[0][r] = row_l1;
+        row_max[1][r] = fabsf(delta);
+      }
+    }
+  }
+  if (!BF16) {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const int which = threadIdx.x >> 5, lane = threadIdx.x & 31;
+      const float top = warp_max(max_of(row_max[which][lane], row_max[which][lane + 32]));
+      if (lane == 0) bp.tile_max[static_cast<int64_t>(blockIdx.x) * 2 + which] = top;
     }
   }
 }
@@ -518,6 +597,17 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     // The next item with tiles, its owned row and (dq) the row's statistics, fetched one item ahead.
     OwnedRow<DP> owned;
     float nlse = -INFINITY, ndelta = 0.f, next_nlse = -INFINITY, next_ndelta = 0.f;
+    // f16: what the accumulators' store multiplies with, the powers of two that P and dS carry taken out.
+    float undo = p.scale, next_undo = p.scale;
+    int32_t v_of = -1;                         // dq: the sequence and key head of `v_top`
+    float v_top = 0.f;
+    // The largest |v| of 64-state tiles [t0, t1) of a sequence and key head, in every lane.
+    auto largest_value = [&](int32_t bg, int32_t t0, int32_t t1) -> float {
+      const float* src = a.p.v_max + static_cast<int64_t>(bg) * ((p.states + kCols - 1) / kCols);
+      float top = 0.f;
+      for (int32_t t = t0 + lane; t < t1; t += 32) top = max_of(top, __ldcg(src + t));
+      return warp_max(top);
+    };
     auto fetch = [&](int32_t from) -> bool {
       for (int32_t i = from; i < a.n_items; i += gridDim.x) {
         const Work w = decode_work<KV>(a, i);
@@ -544,6 +634,19 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             next_nlse = __ldcg(st);
             next_ndelta = __ldcg(st + kCols);
           }
+          if (!BF16) {
+            const int32_t bg = w.b * p.groups + w.g;
+            if (bg != v_of) v_top = largest_value(bg, 0, (w.length + kCols - 1) / kCols);
+            v_of = bg;
+            int32_t e = 0;
+            if (row < w.own) {
+              const int32_t m = w.row0 + row;
+              const float l1 = __ldcg(a.p.row_l1 + static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 * kCols + m);
+              e = power_for(fmaf(l1, v_top, fabsf(next_ndelta)));
+            }
+            next_nlse += static_cast<float>(e - kPowP);
+            next_undo = p.scale * two_to(-e);
+          }
         }
         return true;
       }
@@ -557,6 +660,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       }
       nlse = next_nlse;
       ndelta = next_ndelta;
+      if (!KV && !BF16) undo = next_undo;
     };
     uint32_t tile = 0, items = 0;
     bool ok = true;
@@ -566,6 +670,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     }
     // The dk / dv kernel after dq needs the statistics too, and nothing of dq's.
     allow_next_kernel();
+    if (KV && !BF16 && a.after_stats) wait_previous_kernel();  // these warps read the bound's parts
     if (fetch(blockIdx.x)) hand_over();
     for (int32_t item = blockIdx.x; item < a.n_items && ok; item += gridDim.x) {
       const Work wk = decode_work<KV>(a, item);
@@ -584,6 +689,22 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       }
       const bool more = fetch(item + gridDim.x);
       const float2 nlse2 = make_float2(nlse, nlse), ndelta2 = make_float2(ndelta, ndelta);
+      float2 lift = make_float2(1.f, 1.f);     // dk, dv in f16: from 2^12 P to the factor of dS
+      if (KV && !BF16) {
+        const float2* tops = reinterpret_cast<const float2*>(a.p.tile_max) +
+                             (static_cast<int64_t>(wk.b) * p.heads + wk.h0) * a.m_tiles64 + wk.t0;
+        float l1 = 0.f, delta = 0.f;
+        for (int32_t t = lane; t < wk.n_t; t += 32) {
+          const float2 top = __ldcg(tops + t);
+          l1 = max_of(l1, top.x);
+          delta = max_of(delta, top.y);
+        }
+        const int32_t t0 = wk.row0 / kCols, all = (wk.length + kCols - 1) / kCols;
+        const float v_most = largest_value(wk.b * p.groups + wk.g, t0, t0 + 2 < all ? t0 + 2 : all);
+        const int32_t e = power_for(fmaf(warp_max(l1), v_most, warp_max(delta)));
+        lift = make_float2(two_to(e - kPowP), two_to(e - kPowP));
+        undo = p.scale * two_to(-e);
+      }
       for (int32_t i = 0; i < wk.n_t; ++i, ++tile) {
         const uint32_t st = tile & 1, s = tile % kStages;
         // The statistics came with the tile that the finished products have read.
@@ -613,7 +734,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             const int c = e + 2 * u;
             const float2 t = fma2(make_float2(__uint_as_float(xr[c]), __uint_as_float(xr[c + 1])), scale2, nl[u]);
             const float2 pr = make_float2(fast_exp2(t.x), fast_exp2(t.y));
-            const float2 g = mul2(pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
+            const float2 g = mul2(KV && !BF16 ? mul2(pr, lift) : pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
             if (KV) pw[c / 2] = pack2<BF16>(pr.x, pr.y);
             dw[c / 2] = pack2<BF16>(g.x, g.y);
           }
@@ -648,7 +769,8 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       const int64_t off = static_cast<int64_t>(row) * p.head_dim;
 #pragma unroll
       for (int y = 0; y < (KV ? 2 : 1); ++y)
-        store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / kParts), y == 0 ? p.scale : 1.f,
+        store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / kParts),
+                            y == 0 ? (BF16 ? p.scale : undo) : (BF16 ? 1.f : two_to(-kPowP)),
                             row < wk.own && dst[y] != nullptr, zero,
                             static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim + off,
                             parts[y] == nullptr ? nullptr : parts[y] + at + off, a.wide, p.head_dim);
@@ -728,7 +850,8 @@ int32_t launch_typed(const XaBwdParams& bp, cudaStream_t stream, int sm_count) {
   a.wide = p.head_dim % 16 == 0;
   for (const void* g : {bp.dq, bp.dk, bp.dv}) a.wide = a.wide && reinterpret_cast<uintptr_t>(g) % 32 == 0;
 
-  const int64_t stat_blocks = static_cast<int64_t>(p.batch) * p.heads * a.m_tiles64;
+  const int64_t state_blocks = BF16 ? 0 : static_cast<int64_t>(p.batch) * p.groups * ((p.states + kCols - 1) / kCols);
+  const int64_t stat_blocks = static_cast<int64_t>(p.batch) * p.heads * a.m_tiles64 + state_blocks;
   if (stat_blocks > INT32_MAX) return 8;
   xattn_stats_kernel<DP / 8, BF16><<<static_cast<unsigned>(stat_blocks), 256, 0, stream>>>(bp, bp.delta, a.m_tiles64);
   if (cudaGetLastError() != cudaSuccess) return 6;

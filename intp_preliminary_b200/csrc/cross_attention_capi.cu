@@ -223,7 +223,8 @@ int32_t launch_pass(XaParams p, const Pass& s, int64_t first, cudaStream_t strea
 }
 
 struct BackwardPlan {
-  int64_t stats, dq_part, dk_part, dv_part, bytes;   // byte offsets; 0 = no part buffer
+  int64_t row_l1, tile_max, v_max;                   // byte offsets (f16); the statistics come first
+  int64_t dq_part, dk_part, dv_part, bytes;          // byte offsets; 0 = no part buffer
   int32_t dq_split, dq_tiles, kv_split, kv_tiles;
 };
 
@@ -241,7 +242,16 @@ BackwardPlan plan_backward(const xattn_backward_args* b) {
   const int64_t m64 = ceil_div(a->queries, 64), n64 = ceil_div(a->states, 64);
   plan_split(a->batch * a->heads * ceil_div(a->queries, 128), n64, &p.dq_split, &p.dq_tiles);
   plan_split(a->batch * a->groups * ceil_div(a->states, 128), m64 * (a->heads / a->groups), &p.kv_split, &p.kv_tiles);
-  int64_t at = align256(a->batch * a->heads * m64 * 128 * 4);
+  const int64_t row_tiles = a->batch * a->heads * m64;
+  int64_t at = align256(row_tiles * 128 * 4);
+  if (a->dtype == INTP_F16) {
+    p.row_l1 = at;
+    at += align256(row_tiles * 64 * 4);
+    p.tile_max = at;
+    at += align256(row_tiles * 2 * 4);
+    p.v_max = at;
+    at += align256(a->batch * a->groups * n64 * 4);
+  }
   const int64_t nq = a->batch * a->heads * a->queries * a->head_dim * 4;
   const int64_t nk = a->batch * a->groups * a->states * a->head_dim * 4;
   if (p.dq_split > 1) {
@@ -384,6 +394,11 @@ intp_status xattn_backward(const xattn_backward_args* b, void* stream) {
   p.dk = b->grad_k;
   p.dv = b->grad_v;
   p.delta = reinterpret_cast<float*>(ws);
+  if (a->dtype == INTP_F16) {
+    p.row_l1 = reinterpret_cast<float*>(ws + plan.row_l1);
+    p.tile_max = reinterpret_cast<float*>(ws + plan.tile_max);
+    p.v_max = reinterpret_cast<float*>(ws + plan.v_max);
+  }
   p.dq_part = plan.dq_part ? reinterpret_cast<float*>(ws + plan.dq_part) : nullptr;
   p.dk_part = plan.dk_part ? reinterpret_cast<float*>(ws + plan.dk_part) : nullptr;
   p.dv_part = plan.dv_part ? reinterpret_cast<float*>(ws + plan.dv_part) : nullptr;

@@ -47,7 +47,10 @@ struct XaBwdParams {
   XaParams f;
   const void* dout; int64_t ds[3];
   void* dq; void* dk; void* dv;      // 16-bit, contiguous; null when not wanted
-  float* delta;                      // (B, H, M) scratch
+  float* delta;                      // row statistics: [B * H][ceil(M / 64)][-lse 64 | -delta 64]
+  // f16 only, what bounds dS: sum |dO| of a query row, [B * H][ceil(M / 64)][64]; the largest of
+  // that and of |delta| in 64 rows, two numbers each; the largest |v| of 64 states, [B * G][ceil(N / 64)].
+  float* row_l1; float* tile_max; float* v_max;
   // Splits of the streamed axis: fp32 partial sums [split][elements], null when 1.
   float* dq_part; int32_t dq_split, dq_split_tiles;
   float* dk_part; float* dv_part; int32_t kv_split, kv_split_tiles;

@@ -65,11 +65,20 @@ def cross_attention(q, k, v, *, scale, lengths=None, prefix=None, out_dtype=None
     return out, lse, bound
 
 
-def cross_attention_gradients(q, k, v, grad, *, scale, lengths=None):
-    """``((dq, dk, dv), (their bounds))`` in float64 on the CPU."""
+def cross_attention_gradients(q, k, v, grad, *, scale, lengths=None, scaled=False):
+    """``((dq, dk, dv), (their bounds))`` in float64 on the CPU.
+
+    ``scaled``: for a kernel that brings P and dS into f16's range by powers of two, so that a
+    bound knows no absolute size but the result's own.  With r = sum |dO| max |v| + |delta| of a
+    query row, at least |dS|, it holds 2^e dS with 2^11 <= 2^e r: what f16 loses below 2^-14 is at
+    most 2^-25 of that unit, 2^-36 r (dk: the largest r of the streamed rows).  P is held as
+    2^12 P: 2^-37.  The result loses at most 2^-25 when it is rounded (f16's last step is 2^-24)."""
     dtype = q.dtype
     u = _u(dtype)
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    last = 1e-7
+    if scaled:
+        last = 2.0 ** -25 if dtype == torch.float16 else 0.0
     _, _, out_bound = cross_attention(q, k, v, scale=scale, lengths=lengths)
     q, k, v, grad = (t.detach().cpu().double() for t in (q, k, v, grad))
     batch, heads = q.shape[:2]
@@ -87,15 +96,23 @@ def cross_attention_gradients(q, k, v, grad, *, scale, lengths=None):
             dp = go @ vv.T
             ds = p * (dp - (p * dp).sum(-1, keepdim=True))
             delta_bound = (go.abs() * out_bound[b, h]).sum(-1, keepdim=True)
-            ds_bound = rel * ds.abs() + p * (delta_bound + 1e-5 * (go.abs() @ vv.abs().T)) + tiny
-            p_bound = rel * p + tiny
+            ds_bound = rel * ds.abs() + p * (delta_bound + 1e-5 * (go.abs() @ vv.abs().T))
+            ds_row, ds_all, p_tiny = tiny, tiny, tiny
+            if scaled:
+                delta = (p * dp).sum(-1, keepdim=True).abs()
+                ds_row = 2.0 ** -36 * (go.abs().sum(-1, keepdim=True) * vv.abs().max() + delta)
+                heads_of = range(g * (heads // groups), (g + 1) * (heads // groups))
+                most = max(float(grad[b, x].abs().sum(-1).max()) for x in heads_of)  # |delta| <= sum |dO| max |v|
+                ds_all = 2.0 ** -36 * 2 * most * float(vv.abs().max())
+                p_tiny = 2.0 ** -37
+            p_bound = rel * p + p_tiny
             d[0][b, h] = scale * (ds @ kk)
             d[1][b, g, :length] += scale * (ds.T @ q[b, h])
             d[2][b, g, :length] += p.T @ go
-            e[0][b, h] = scale * (ds_bound @ kk.abs())
-            e[1][b, g, :length] += scale * (ds_bound.T @ q[b, h].abs())
+            e[0][b, h] = scale * ((ds_bound + ds_row) @ kk.abs())
+            e[1][b, g, :length] += scale * ((ds_bound + ds_all).T @ q[b, h].abs())
             e[2][b, g, :length] += p_bound.T @ go.abs()
-    return tuple(d), tuple(x + u * t.abs() + 1e-7 for x, t in zip(e, d))
+    return tuple(d), tuple(x + u * t.abs() + last for x, t in zip(e, d))
 
 
 def e4m3_values() -> torch.Tensor:

@@ -562,3 +562,83 @@ def test_backwards_in_a_row_use_their_own_statistics(cuda_device, sizes, needs, 
     for i, grads in enumerate(got):
         for a, b in zip(grads, want[i % 2]):
             assert a is b is None or torch.equal(a, b)
+
+
+SCALED_GRADS = [
+    # sizes, lengths, sizes of q, k, v and grad as powers of two
+    ((1, 2, 1, 70, 4096, 64), None, (-8, 8, 0, -16)),        # dS far below f16's last step, dq is not
+    ((1, 2, 1, 70, 4096, 64), None, (8, -8, 0, -16)),        # the same for dk
+    ((2, 2, 2, 150, 1000, 128), [900, 77], (-8, 8, 0, -14)),
+    ((2, 2, 2, 150, 1000, 128), [900, 77], (8, -8, 0, -14)),
+    ((1, 4, 2, 33, 3000, 40), [2500], (-8, 8, -10, -4)),     # small values and small gradients
+    ((1, 1, 1, 700, 20, 64), None, (-6, -10, 8, 8)),         # dS past f16's largest number
+    ((1, 1, 1, 40, 20, 128), None, (-6, -10, 8, 8)),
+    ((1, 1, 1, 2, 131072, 16), None, (0, 0, 0, 6)),          # P near 2^-17
+    ((2, 3, 3, 65, 64, 64), None, (0, 0, 0, 0)),
+]
+
+
+def _powers(shape, dtype, seed, power):
+    return (_normal(shape, torch.float32, seed) * 2.0 ** power).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", SCALED_GRADS)
+def test_gradients_keep_their_bits_at_any_size(cuda_device, case, dtype):
+    """Bounds that know no absolute size but the result's own; values past the lengths are the
+    type's largest, infinite and NaN, and play no part in a scale either."""
+    (batch, heads, groups, queries, states, dim), lengths, powers = case
+    q = _powers((batch, heads, queries, dim), dtype, 161, powers[0])
+    k = _powers((batch, groups, states, dim), dtype, 162, powers[1])
+    v = _powers((batch, groups, states, dim), dtype, 163, powers[2])
+    grad = _powers((batch, heads, queries, dim), dtype, 164, powers[3])
+    scale = dim ** -0.5
+    want, bounds = oracle.cross_attention_gradients(q, k, v, grad, scale=scale, lengths=lengths, scaled=True)
+    for b, n in enumerate(lengths or []):
+        v[b, :, n:] = torch.finfo(dtype).max
+        v[b, :, n + 1:] = float("inf")
+        v[b, :, n + 2:] = float("nan")
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    dev = [t.to(cuda_device) for t in (q, k, v)]
+    out, lse = cross_attention_forward(*dev, scale=scale, lengths=lens, want_lse=True)
+    got = cross_attention_backward(*dev, out, lse, grad.to(cuda_device), scale=scale, lengths=lens)
+    for g, w, b in zip(got, want, bounds):
+        _assert_within(g, w, b)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_query_rows_with_gradients_of_any_size_together(cuda_device, dim):
+    """A row's dq keeps its bits beside rows whose gradients are 2^20 times as large, and zero."""
+    q, k = _powers((1, 2, 90, dim), F16, 171, -8), _powers((1, 1, 2000, dim), F16, 172, 8)
+    v = _powers((1, 1, 2000, dim), F16, 173, 0)
+    power = torch.tensor([-16.0, 4.0, -8.0])[torch.arange(90) % 3][None, None, :, None]
+    grad = _normal((1, 2, 90, dim), torch.float32, 174) * torch.exp2(power)
+    grad[:, :, 7] = 0
+    grad = grad.to(F16)
+    want, bounds = oracle.cross_attention_gradients(q, k, v, grad, scale=0.125, scaled=True)
+    dev = [t.to(cuda_device) for t in (q, k, v)]
+    out, lse = cross_attention_forward(*dev, scale=0.125, want_lse=True)
+    got = cross_attention_backward(*dev, out, lse, grad.to(cuda_device), scale=0.125)
+    for g, w, b in zip(got, want, bounds):
+        _assert_within(g, w, b)
+    assert got[0][:, :, 7].abs().max() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_gradients_that_are_not_finite_stay_in_their_rows(cuda_device, bad, dtype):
+    """A query row whose upstream gradient is not finite has no finite dq; the others keep theirs."""
+    q, k, v = (t.to(cuda_device) for t in _inputs(1, 2, 2, 100, 300, 64, dtype, seed=181))
+    grad = _normal(q.shape, dtype, 182).to(cuda_device)
+    out, lse = cross_attention_forward(q, k, v, scale=0.125, want_lse=True)
+    want = cross_attention_backward(q, k, v, out, lse, grad, scale=0.125)
+    grad[0, 0, 41, 5] = bad
+    got = cross_attention_backward(q, k, v, out, lse, grad, scale=0.125)
+    rest = [m for m in range(100) if m != 41]
+    assert not torch.isfinite(got[0][0, 0, 41]).any()
+    assert torch.equal(got[0][0, 0, rest], want[0][0, 0, rest])
+    for g, w in zip(got, want):
+        assert torch.equal(g[0, 1], w[0, 1])
+    assert not torch.isfinite(got[1][0, 0]).any() and not torch.isfinite(got[2][0, 0, :, 5]).any()
+    others = [c for c in range(64) if c != 5]
+    torch.testing.assert_close(got[2][0, 0][:, others], want[2][0, 0][:, others], rtol=0, atol=0)

@@ -378,7 +378,8 @@ INTP_API intp_status xattn_backward_workspace(const xattn_backward_args* a, int6
  * exponents over 8-bit states; with a prefix over the prefix and then its own. */
 INTP_API intp_status xattn_forward(const xattn_args* a, void* stream);
 
-/* Gradients from the forward's out and lse (16-bit states, no prefix). */
+/* Gradients from the forward's out and lse (16-bit states, no prefix).  Without
+ * queries (M = 0) grad_k and grad_v are zeros; no other pointer is needed then. */
 INTP_API intp_status xattn_backward(const xattn_backward_args* a, void* stream);
 
 /* The 8-bit cache: codes (B, G, C, D) e4m3 contiguous, exponents (B, G, C)

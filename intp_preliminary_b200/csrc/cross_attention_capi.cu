@@ -370,7 +370,15 @@ intp_status xattn_backward(const xattn_backward_args* b, void* stream) {
   intp_status st = check_shape(a);
   if (st != INTP_OK) return st;
   if (a->eight_bit || a->prefix > 0) return INTP_ERR_UNSUPPORTED;
-  if (a->batch == 0 || a->queries == 0) return INTP_OK;
+  if (a->batch == 0) return INTP_OK;
+  if (a->queries == 0) {
+    // No row reads the states: their gradients are there, and zero.
+    const size_t bytes = static_cast<size_t>(a->batch) * a->groups * a->states * a->head_dim * 2;
+    for (void* g : {b->grad_k, b->grad_v})
+      if (g != nullptr && bytes > 0 && cudaMemsetAsync(g, 0, bytes, static_cast<cudaStream_t>(stream)) != cudaSuccess)
+        return INTP_ERR_LAUNCH;
+    return INTP_OK;
+  }
   if (a->states == 0) return INTP_ERR_SHAPE;
   if (!b->grad_q && !b->grad_k && !b->grad_v) return INTP_OK;
   if (!a->lse || !b->grad_out) return INTP_ERR_ARGUMENT;

@@ -642,3 +642,32 @@ def test_gradients_that_are_not_finite_stay_in_their_rows(cuda_device, bad, dtyp
     assert not torch.isfinite(got[1][0, 0]).any() and not torch.isfinite(got[2][0, 0, :, 5]).any()
     others = [c for c in range(64) if c != 5]
     torch.testing.assert_close(got[2][0, 0][:, others], want[2][0, 0][:, others], rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("queries,batch", [(0, 2), (0, 0), (3, 2)])
+def test_the_library_writes_every_gradient(cuda_device, queries, batch):
+    """Through the C entry: without queries the states' gradients are zeros, not what the buffers held."""
+    q, k, v = (t.to(cuda_device) for t in _inputs(batch, 4, 2, queries, 70, 64, BF16, seed=190))
+    grads = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+    args = _lib.XattnBackwardArgs()
+    f = args.fwd
+    f.batch, f.heads, f.groups, f.queries, f.states, f.head_dim = batch, 4, 2, queries, 70, 64
+    f.scale, f.dtype = 0.125, _lib.INTP_BF16
+    if queries:
+        out, lse = cross_attention_forward(q, k, v, scale=0.125, want_lse=True)
+        status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+        f.q, f.k, f.v, f.out, f.lse, f.status = (t.data_ptr() for t in (q, k, v, out, lse, status))
+        args.grad_out = q.data_ptr()
+        f.q_stride = f.out_stride = args.grad_out_stride = _lib._Stride(*q.stride())
+        f.k_stride = f.v_stride = _lib._Stride(*k.stride())
+    args.grad_q, args.grad_k, args.grad_v = (t.data_ptr() or None for t in grads)
+    size = ctypes.c_int64()
+    lib = _lib.load()
+    assert lib.xattn_backward_workspace(ctypes.addressof(args), ctypes.byref(size)) == _lib.INTP_OK
+    space = torch.empty(size.value, dtype=torch.uint8, device=cuda_device)
+    f.workspace, f.workspace_bytes = space.data_ptr() or None, size.value
+    stream = torch.cuda.current_stream(cuda_device).cuda_stream
+    assert lib.xattn_backward(ctypes.addressof(args), stream) == _lib.INTP_OK
+    assert not any(torch.isnan(g).any() for g in grads)
+    if queries == 0:
+        assert all(g.abs().sum() == 0 for g in grads)

@@ -48,8 +48,9 @@ intp_status check_shape(const xattn_args* a) {
   if (a->kernel < XATTN_KERNEL_AUTO || a->kernel > XATTN_KERNEL_TILES) return INTP_ERR_ARGUMENT;
   if (a->eight_bit != 0 && a->eight_bit != 1) return INTP_ERR_ARGUMENT;
   if (a->eight_bit && a->kernel == XATTN_KERNEL_TILES) return INTP_ERR_UNSUPPORTED;
-  // rows of an instance, instances and their tiles are 32-bit numbers in the kernels
-  if (a->batch * a->heads > kMaxInt / std::max<int64_t>(a->queries, 1)) return INTP_ERR_SHAPE;
+  // Rows of an instance, instances and their tiles are 32-bit numbers in the kernels, the end of
+  // the last row tile among them.
+  if (a->batch * a->heads > (kMaxInt - intp::kXaTileRows) / std::max<int64_t>(a->queries, 1)) return INTP_ERR_SHAPE;
   return INTP_OK;
 }
 

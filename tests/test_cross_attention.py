@@ -186,3 +186,18 @@ def test_statistics_are_read_behind_their_writer():
     assert re.search(r"if \(!KV\) \{\s*wait_previous_kernel\(\);[^}]*__threadfence\(\);[^}]*\}", body)
     assert body.index("wait_previous_kernel();") < body.index("__threadfence();") < body.index("allow_next_kernel();")
     assert body.count("allow_next_kernel();") == 1 and "a.after_stats = bp.dq == nullptr;" in text
+
+
+@pytest.mark.parametrize("heads,queries,status", [
+    (2, (1 << 30) - 1, _lib.INTP_ERR_SHAPE),    # 2^31 - 2 rows of a key head: their last tile ends past 2^31
+    (2, (1 << 30) - 128, _lib.INTP_ERR_SHAPE),
+    (2, (1 << 30) - 129, _lib.INTP_OK),         # the last tile of 256 rows ends at 2^31 - 256
+    (1, 1 << 30, _lib.INTP_OK),
+])
+def test_rows_whose_last_tile_leaves_32_bits_are_refused(heads, queries, status):
+    a = _args(batch=1, heads=heads, groups=1, queries=queries, states=300)
+    size = ctypes.c_int64()
+    assert _lib.load().xattn_forward_workspace(ctypes.addressof(a), ctypes.byref(size)) == status
+    b = _lib.XattnBackwardArgs()
+    b.fwd = a
+    assert _lib.load().xattn_backward_workspace(ctypes.addressof(b), ctypes.byref(size)) == status

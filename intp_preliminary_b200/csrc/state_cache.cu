@@ -220,11 +220,13 @@ int32_t run(const state_cache_args* c, bool write, cudaStream_t stream) {
   for (int64_t n : {c->batch, c->groups, c->capacity, c->count})
     if (n > (int64_t(1) << 30)) return INTP_ERR_SHAPE;
   if (c->batch * c->groups > INT32_MAX / 2) return INTP_ERR_SHAPE;
-  if (!c->k || !c->v || !c->k_codes || !c->v_codes || !c->k_exponents || !c->v_exponents) return INTP_ERR_ARGUMENT;
+  if (!c->k || !c->v) return INTP_ERR_ARGUMENT;
+  if (c->capacity > 0 && (!c->k_codes || !c->v_codes || !c->k_exponents || !c->v_exponents)) return INTP_ERR_ARGUMENT;
   const int64_t extent[3] = {c->batch, c->groups, c->count};
   if (!row_layout_ok(c->k, c->k_stride, extent) || !row_layout_ok(c->v, c->v_stride, extent)) return INTP_ERR_LAYOUT;
   if (reinterpret_cast<uintptr_t>(c->k_codes) % 16 || reinterpret_cast<uintptr_t>(c->v_codes) % 16)
     return INTP_ERR_LAYOUT;
+  if (write && c->capacity == 0) return INTP_OK;  // every row falls outside; a read has zeros to write
   int sms = 0;
   const int32_t device = current_device_facts(&sms);
   if (device != INTP_OK) return device;

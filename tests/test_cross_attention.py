@@ -201,3 +201,14 @@ def test_rows_whose_last_tile_leaves_32_bits_are_refused(heads, queries, status)
     b = _lib.XattnBackwardArgs()
     b.fwd = a
     assert _lib.load().xattn_backward_workspace(ctypes.addressof(b), ctypes.byref(size)) == status
+
+
+def test_a_write_to_a_cache_without_room_has_nothing_to_do():
+    """Rows outside the cache are skipped, and all are; a cache of no states has no memory."""
+    a = _lib.StateCacheArgs()
+    a.batch, a.groups, a.capacity, a.count, a.head_dim, a.dtype = 1, 2, 0, 4, 64, _lib.INTP_F16
+    a.k = a.v = FAKE
+    a.k_stride = a.v_stride = _lib._Stride(512, 256, 64, 1)
+    assert _lib.load().state_cache_write(ctypes.addressof(a), None) == _lib.INTP_OK
+    a.capacity = 1
+    assert _lib.load().state_cache_write(ctypes.addressof(a), None) == _lib.INTP_ERR_ARGUMENT

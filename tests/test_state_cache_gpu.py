@@ -298,3 +298,22 @@ def test_write_follows_strides(cuda_device):
     odd = torch.empty(2, 3, 37, 65, dtype=BF16, device=cuda_device)[..., 1:].copy_(k)  # not 16-byte aligned
     a.write(odd, v)
     assert torch.equal(a.keys.view(torch.uint8), b.keys.view(torch.uint8))
+
+
+def test_a_cache_without_room(cuda_device):
+    """Capacity 0: writes are skipped, reads give zeros, a prefix alone is attended to."""
+    cache = StateCache.empty(2, 2, 0, 64, device=cuda_device)
+    k, v = (_normal((2, 2, 3, 64), BF16, s).to(cuda_device) for s in (1, 2))
+    cache.write(k, v)
+    cache.write(k, v, start=torch.tensor([0, 5], device=cuda_device))
+    rk, rv = cache.read(3)
+    assert rk.shape == rv.shape == (2, 2, 3, 64) and rk.abs().sum() == 0 and rv.abs().sum() == 0
+    assert cache.read()[0].shape == (2, 2, 0, 64)
+    q = _normal((2, 4, 1, 64), BF16, 3)
+    pk, pv = k[0, :, :3].contiguous(), v[0, :, :3].contiguous()
+    none = torch.zeros(2, 2, 0, 64)
+    want, _, bound = oracle.cross_attention(q, none, none, scale=0.125, prefix=(pk, pv))
+    got = shared_prefix_attention(q.to(cuda_device), pk, pv, cache, scale=0.125)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+    with pytest.raises(ValueError, match="at least one state"):
+        cached_cross_attention(q.to(cuda_device), cache, scale=0.125)

@@ -9,6 +9,15 @@ The bounds follow from where a kernel may round, with u the unit roundoff of a
   P, dS of the backward: the same EXP, plus the row sum's own (it is an fp32 log
         within 2e-4), one rounding each; delta carries the rounding of out.
 f16 operands below 2^-14 lose bits: at most 2^-25 each.
+
+``two_part`` bounds a kernel that multiplies each probability as two 16-bit numbers, so that
+hardly more than the result's own rounding remains.  Relative to p_j |v_j|, with D products in
+a score, n states and n / 16 matrix instructions in a sum:
+  the two parts leave out u_p^2 (f16 also 2^-25 of the largest);
+  ex2.approx 2^-22;  fp32 sums (n / 16 + 64) 2^-22, joins of warps and parts among them;
+  a score's own error, absolute in its exponent: a sum of D fp32 products, 2^-23 (D + 8)
+  scale sum |q k|, and four roundings of numbers of the largest score's size.
+The row sum carries the same once more.
 """
 
 from __future__ import annotations
@@ -27,11 +36,12 @@ def _lengths(lengths, batch, n):
     return [n] * batch if lengths is None else [min(max(int(x), 0), n) for x in lengths]
 
 
-def cross_attention(q, k, v, *, scale, lengths=None, prefix=None, out_dtype=None, p_dtype=None, key_weight=None):
+def cross_attention(q, k, v, *, scale, lengths=None, prefix=None, out_dtype=None, p_dtype=None, key_weight=None,
+                    two_part=False):
     """``(out, lse, bound)`` in float64 on the CPU; ``prefix`` = (k, v) of shape (G, P, D).
 
     ``key_weight`` (B, G, N): the size of a unit of each value row (8-bit states), for
-    the loss of small f16 probabilities."""
+    the loss of small f16 probabilities.  ``two_part``: see the module's text."""
     out_dtype = out_dtype or q.dtype
     p_dtype = p_dtype or q.dtype
     q, k, v = (t.detach().cpu().double() for t in (q, k, v))
@@ -53,6 +63,15 @@ def cross_attention(q, k, v, *, scale, lengths=None, prefix=None, out_dtype=None
             lse[b, h] = torch.logsumexp(s, -1)
             p = torch.exp(s - lse[b, h][:, None])
             out[b, h] = p @ vv
+            if two_part:
+                score = 2.0 ** -23 * ((dim + 8) * scale * (q[b, h].abs() @ kk.abs().T) + 4 * s.abs().amax(-1, keepdim=True))
+                rel = u_p ** 2 + 2.0 ** -22 * (1 + 64 + kk.shape[0] / 16)
+                mean = p @ vv.abs()
+                bound[b, h] = (p * (score + rel)) @ vv.abs() + (p * (score + rel)).sum(-1, keepdim=True) * mean
+                bound[b, h] += u_o * out[b, h].abs() + (2.0 ** -25 if out_dtype == torch.float16 else 0.0)
+                if p_dtype == torch.float16:
+                    bound[b, h] += 2.0 ** -25 * p.amax(-1, keepdim=True) * vv.abs().sum(0)
+                continue
             bound[b, h] = (u_p + EXP) * (p @ vv.abs()) + u_o * out[b, h].abs()
             if p_dtype == torch.float16:
                 if key_weight is None:

@@ -212,3 +212,20 @@ def test_a_write_to_a_cache_without_room_has_nothing_to_do():
     assert _lib.load().state_cache_write(ctypes.addressof(a), None) == _lib.INTP_OK
     a.capacity = 1
     assert _lib.load().state_cache_write(ctypes.addressof(a), None) == _lib.INTP_ERR_ARGUMENT
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("states,dim", [(5, 16), (17, 16), (60, 16), (17, 64)])
+def test_two_part_bound_tells_one_rounding_of_the_probabilities_from_two_parts(states, dim, dtype):
+    """The bound that the few-rows kernel is held to fails for probabilities rounded to 16 bits, and
+    for low parts that miss their place, and holds for two parts."""
+    g = torch.Generator().manual_seed(states)
+    q, k, v = (torch.randn(s, generator=g).to(dtype) for s in ((4, 4, 4, dim), (4, 4, states, dim), (4, 4, states, dim)))
+    want, _, bound = oracle.cross_attention(q, k, v, scale=dim ** -0.5, two_part=True)
+    s = (q.double() @ k.double().transpose(-1, -2)) * dim ** -0.5
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    high = p.to(dtype).double()
+    low = (p - high).to(dtype).double()
+    for operand, holds in ((high, False), (high + low, True), (high + low.flip(-1), False)):
+        got = ((operand @ v.double()) / p.sum(-1, keepdim=True)).to(dtype).double()
+        assert bool(((got - want).abs() <= bound).all()) == holds

@@ -671,3 +671,32 @@ def test_the_library_writes_every_gradient(cuda_device, queries, batch):
     assert not any(torch.isnan(g).any() for g in grads)
     if queries == 0:
         assert all(g.abs().sum() == 0 for g in grads)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", [
+    (4, 4, 4, 4, 5, 16, None), (4, 4, 4, 4, 17, 16, None), (4, 8, 2, 1, 60, 16, [60, 17, 0, 33]), (4, 4, 4, 4, 17, 64, None),
+    (2, 6, 2, 3, 129, 40, [129, 70]), (2, 8, 2, 4, 300, 128, [299, 128]), (1, 16, 4, 1, 3001, 64, None),
+    (3, 4, 2, 8, 196, 64, None)])
+def test_few_rows_carry_only_the_rounding_of_the_result(cuda_device, shape, dtype):
+    """The few-rows kernel multiplies two parts of each probability: held to the bound of that."""
+    *sizes, lengths = shape
+    q, k, v = _inputs(*sizes, dtype, seed=200)
+    scale = q.shape[-1] ** -0.5
+    want, _, bound = oracle.cross_attention(q, k, v, scale=scale, lengths=lengths, two_part=True)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    got, _ = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=scale, lengths=lens, kernel="rows")
+    _assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("prefix,states,lengths,dim", [(3, 4, None, 16), (16, 17, [17, 0, 9], 16), (100, 33, [33, 1, 0], 64),
+                                                       (600, 300, None, 64)])
+def test_a_prefix_read_in_one_pass_carries_only_the_rounding_of_the_result(cuda_device, prefix, states, lengths, dim, dtype):
+    q, k, v = _inputs(3, 8, 4, 2, states, dim, dtype, seed=210)
+    pk, pv = _normal((4, prefix, dim), dtype, 211), _normal((4, prefix, dim), dtype, 212)
+    scale = dim ** -0.5
+    want, _, bound = oracle.cross_attention(q, k, v, scale=scale, lengths=lengths, prefix=(pk, pv), two_part=True)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    got = shared_prefix_attention(*(t.to(cuda_device) for t in (q, pk, pv, k, v)), scale=scale, lengths=lens)
+    _assert_within(got, want, bound)

@@ -13,7 +13,9 @@ are clamped to 0..N); states past it take no part whatever they hold, NaN
 included, and a sequence without states gives zeros.  A row whose every score
 is -inf gives zeros too.  The operator is differentiable in q, k and v
 (``cross_attention_forward`` / ``cross_attention_backward`` are its two
-halves); results and gradients repeat bit for bit.
+halves); results and gradients repeat bit for bit.  Reverse mode, once: a second
+derivative, forward-mode tangents and ``torch.jit.trace`` are refused, and the
+operators over a cache or a prefix take no part in autograd at all.
 
 Many rows per key head run on 128-row tensor-core tiles, few (single tokens)
 on a kernel that streams the states once for every 16 rows; ``kernel`` selects.
@@ -40,7 +42,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .look_attention import _DTYPE_CODE, _status_word, _status_words
+from .look_attention import _DTYPE_CODE, _refuse_transforms, _status_word, _status_words
 
 _KERNELS = {"auto": _lib.XATTN_KERNEL_AUTO, "rows": _lib.XATTN_KERNEL_ROWS, "tiles": _lib.XATTN_KERNEL_TILES}
 _HALF = (torch.bfloat16, torch.float16)
@@ -294,6 +296,7 @@ def cross_attention_forward(q, k, v, *, scale, lengths=None, want_lse: bool = Fa
 
     ``kernel``: ``"auto"`` chooses by the number of rows that share a key head
     (``M * H / G``), ``"rows"`` and ``"tiles"`` force one of the two kernels."""
+    _refuse_transforms("cross attention", q, k, v)
     return _forward(q, k, v, scale, lengths, want_lse, kernel, out)[:2]
 
 
@@ -331,6 +334,7 @@ def cross_attention_backward(q, k, v, out, lse, grad_out, *, scale, lengths=None
     """Gradients ``(dq, dk, dv)`` of ``cross_attention_forward`` from its ``out`` and
     ``lse``, contiguous and in the inputs' dtype; None where ``needs`` is False.
     States past a sequence's length get zeros."""
+    _refuse_transforms("cross attention backward", q, k, v, out, lse, grad_out)
     _check_states(q, k, v)
     scale = _check_scale(scale)
     for name, t in (("out", out), ("grad_out", grad_out)):
@@ -372,12 +376,14 @@ class _CrossAttention(torch.autograd.Function):
 
 def cross_attention(q, k, v, *, scale, lengths=None):
     """Attention of ``q`` to the states ``k``, ``v`` (see the module's text)."""
+    _refuse_transforms("cross attention", q, k, v)
     if torch.is_grad_enabled() and any([isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)]):
         return _CrossAttention.apply(q, k, v, lengths, _check_scale(scale))
     return _forward(q, k, v, scale, lengths, False, "auto", None)[0]
 
 
 def _refuse_grad(what: str, *tensors) -> None:
+    _refuse_transforms(what, *tensors)
     if torch.is_grad_enabled() and any([isinstance(t, torch.Tensor) and t.requires_grad for t in tensors]):
         raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 

@@ -36,6 +36,7 @@ import threading
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -166,6 +167,17 @@ def check_device_status(device=None) -> None:
         status = _lib.load().sla_read_status(ctypes.c_void_p(word.data_ptr()), ctypes.byref(code), ctypes.c_void_p(stream))
     if status != _lib.INTP_OK:
         raise RuntimeError(f"device wait failed: code {code.value:#x} ({_lib.status_string(status)})")
+
+
+def _refuse_transforms(what: str, *tensors) -> None:
+    """Forward-mode derivatives and torch.jit.trace see nothing of a kernel call: a tangent would be
+    lost and a trace would return memory that nothing writes."""
+    if forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    ):
+        raise ValueError(f"{what} has no forward-mode derivative: call it on the primal values")
+    if torch._C._get_tracing_state() is not None:
+        raise ValueError(f"{what} cannot be traced by torch.jit.trace")
 
 
 def _stride4(t: torch.Tensor):

@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from .cross_attention import (_base_args, _call, _check_counts, _check_query, _check_scale, _finish_plan, _keep,
                               _laid_out, _launch, _lengths_pointer, _output, _plans, _ready, _refuse_grad)
-from .look_attention import _DTYPE_CODE
+from .look_attention import _DTYPE_CODE, _refuse_transforms
 
 _POINTERS = struct.Struct("8Q")  # state_cache_args up to the sizes
 _HALF = (torch.bfloat16, torch.float16)
@@ -142,6 +142,7 @@ class StateCache:
         ``start[b]`` on, as ``(k, v)`` ``(B, G, count, D)``: exact, but for what lies
         past the dtype's range (its largest value instead) or below it.  States past
         ``counts[b]`` or outside the cache read as zero."""
+        _refuse_transforms("a state cache")
         batch, groups, capacity, head_dim = self.keys.shape
         count = capacity if count is None else int(count)
         if count < 0:

@@ -229,3 +229,36 @@ def test_two_part_bound_tells_one_rounding_of_the_probabilities_from_two_parts(s
     for operand, holds in ((high, False), (high + low, True), (high + low.flip(-1), False)):
         got = ((operand @ v.double()) / p.sum(-1, keepdim=True)).to(dtype).double()
         assert bool(((got - want).abs() <= bound).all()) == holds
+
+
+def _operator_calls(make):
+    """Every operator's call on the tensors that ``make(shape)`` gives, one of them marked by it."""
+    plain = torch.zeros(1, 2, 3, 16, dtype=torch.bfloat16)
+    marked = make(plain)
+    lse = torch.zeros(1, 2, 3)
+    return [lambda: cross_attention(marked, plain, plain, scale=0.25),
+            lambda: cross_attention(plain, plain, marked, scale=0.25),
+            lambda: cross_attention(plain.clone().requires_grad_(), marked, plain, scale=0.25),
+            lambda: cross_attention_forward(plain, marked, plain, scale=0.25),
+            lambda: cross_attention_backward(plain, plain, plain, plain, lse, marked, scale=0.25),
+            lambda: shared_prefix_attention(plain, plain[0], marked[0], plain, plain, scale=0.25),
+            lambda: shared_prefix_attention(plain, plain[0], plain[0], marked, plain, scale=0.25)]
+
+
+def test_tangents_are_refused():
+    """A forward-mode tangent would be lost: the kernels know nothing of it."""
+    forward_ad = torch.autograd.forward_ad
+    with forward_ad.dual_level():
+        for call in _operator_calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        for call in _operator_calls(lambda t: t):  # the primal alone gets as far as before
+            with pytest.raises(ValueError, match="CUDA"):
+                call()
+
+
+def test_tracing_is_refused():
+    """A trace would hold the output's allocation and not the kernel that fills it."""
+    for call in _operator_calls(lambda t: t):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(lambda t: (call(), t)[1], torch.zeros(1), check_trace=False)

@@ -700,3 +700,26 @@ def test_a_prefix_read_in_one_pass_carries_only_the_rounding_of_the_result(cuda_
     lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
     got = shared_prefix_attention(*(t.to(cuda_device) for t in (q, pk, pv, k, v)), scale=scale, lengths=lens)
     _assert_within(got, want, bound)
+
+
+def test_transforms_that_the_kernels_do_not_see_are_refused(cuda_device):
+    """Forward-mode tangents, traces and functional transforms: an error each, not a lost derivative."""
+    forward_ad = torch.autograd.forward_ad
+    q, k, v = (t.to(cuda_device) for t in _inputs(2, 2, 2, 3, 20, 64, BF16, seed=220))
+
+    def call(t):
+        return cross_attention(t, k, v, scale=0.125)
+
+    want = call(q)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(forward_ad.make_dual(q, torch.ones_like(q)))
+        with pytest.raises(ValueError, match="forward-mode"):
+            shared_prefix_attention(q, k[0], v[0], k, forward_ad.make_dual(v, torch.ones_like(v)), scale=0.125)
+        assert torch.equal(call(q), want)
+    with pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(call, q)
+    for transform in (lambda: torch.func.jvp(call, (q,), (q,)), lambda: torch.func.vmap(call)(q[:, None]),
+                      lambda: torch.func.grad(lambda t: call(t).float().sum())(q)):
+        with pytest.raises((ValueError, RuntimeError)):
+            transform()

@@ -317,3 +317,19 @@ def test_a_cache_without_room(cuda_device):
     assert ((got.cpu().double() - want).abs() <= bound).all()
     with pytest.raises(ValueError, match="at least one state"):
         cached_cross_attention(q.to(cuda_device), cache, scale=0.125)
+
+
+def test_tangents_and_traces_are_refused(cuda_device):
+    forward_ad = torch.autograd.forward_ad
+    cache = StateCache.empty(2, 2, 16, 64, device=cuda_device)
+    x = torch.zeros(2, 2, 3, 64, dtype=BF16, device=cuda_device)
+    q = torch.zeros(2, 4, 1, 64, dtype=BF16, device=cuda_device)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="forward-mode"):
+            cache.write(x, forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(ValueError, match="forward-mode"):
+            cached_cross_attention(forward_ad.make_dual(q, torch.ones_like(q)), cache, scale=0.125)
+    for fn in (lambda t: cached_cross_attention(t, cache, scale=0.125), lambda t: (cache.read(), t)[1],
+               lambda t: (cache.write(x, x), t)[1]):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(fn, q, check_trace=False)

@@ -492,6 +492,7 @@ def structured_look_attention(q, k, v, pose, fields, *, scale, dense_bias=None):
 
     fields = compact_fields(fields)
     values = fields.values if isinstance(fields, LookSlotFields) else fields
+    _refuse_transforms("structured Look attention", q, k, v, pose, values, dense_bias)
     if not torch.is_grad_enabled() or not any(
         t.requires_grad for t in (q, k, v, pose, values, dense_bias) if isinstance(t, torch.Tensor)
     ):

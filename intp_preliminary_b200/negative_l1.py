@@ -15,6 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .look_attention import _refuse_transforms
 
 
 def _validate(x: torch.Tensor, prototype: torch.Tensor) -> None:
@@ -95,6 +96,7 @@ class _NegativeL1(torch.autograd.Function):
 
 def negative_l1_distance(x: torch.Tensor, prototype: torch.Tensor) -> torch.Tensor:
     """Return ``-||x-w||_1`` as [Q,H] without a broadcast difference tensor."""
+    _refuse_transforms("negative L1 distance", x, prototype)
     if torch.is_grad_enabled() and (x.requires_grad or prototype.requires_grad):
         return _NegativeL1.apply(x, prototype)
     return negative_l1_forward(x, prototype)

@@ -199,3 +199,23 @@ def test_slot_fields_mode_argument_checks():
     args.fields = 16
     args.slots = 0
     assert lib.sla_forward(ctypes.byref(args), None) == _lib.INTP_ERR_ARGUMENT  # no slots
+
+
+def test_differentiable_operators_refuse_tangents_and_traces():
+    """The kernels know nothing of a forward-mode tangent or of a trace: an error, not a lost derivative."""
+    from intp_preliminary_b200 import negative_l1_distance, structured_look_attention
+
+    forward_ad = torch.autograd.forward_ad
+    x = torch.randn(4, 8)
+    q, pose = torch.randn(1, 2, 5, 64), torch.randn(1, 4, 2, 3)
+    fields = torch.randn(2, 3, 4, 4)
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, q, pose)]
+        for call in (lambda: negative_l1_distance(dual[0], x), lambda: negative_l1_distance(x, dual[0]),
+                     lambda: structured_look_attention(dual[1], q, q, pose, fields, scale=0.1),
+                     lambda: structured_look_attention(q, q, q, dual[2], fields, scale=0.1)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+    for call in (lambda: negative_l1_distance(x, x), lambda: structured_look_attention(q, q, q, pose, fields, scale=0.1)):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(lambda t: (call(), t)[1], torch.zeros(1), check_trace=False)

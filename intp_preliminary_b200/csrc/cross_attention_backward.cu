@@ -597,16 +597,15 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     // The next item with tiles, its owned row and (dq) the row's statistics, fetched one item ahead.
     OwnedRow<DP> owned;
     float nlse = -INFINITY, ndelta = 0.f, next_nlse = -INFINITY, next_ndelta = 0.f;
-    // f16: what the accumulators' store multiplies with, the powers of two that P and dS carry taken out.
-    float undo = p.scale, next_undo = p.scale;
-    int32_t v_of = -1;                         // dq: the sequence and key head of `v_top`
-    float v_top = 0.f;
-    // The largest |v| of 64-state tiles [t0, t1) of a sequence and key head, in every lane.
-    auto largest_value = [&](int32_t bg, int32_t t0, int32_t t1) -> float {
-      const float* src = a.p.v_max + static_cast<int64_t>(bg) * ((p.states + kCols - 1) / kCols);
-      float top = 0.f;
-      for (int32_t t = t0 + lane; t < t1; t += 32) top = max_of(top, __ldcg(src + t));
-      return warp_max(top);
+    // f16: the bound of dS as fetched, this lane's part of it (dq: |dO| of the row itself), and what
+    // it gives at the hand-over: the factor that takes dS's power of two out of an accumulator again
+    // and (dk, dv) the one from 2^12 P to the factor of dS.
+    float l1_part = 0.f, delta_part = 0.f, v_part = 0.f, undo = p.scale, lift = 1.f;
+    // This lane's part of the largest |v| in 64-state tiles [t0, t1) of a sequence and key head.
+    auto fetch_values = [&](const Work& w, int32_t t0, int32_t t1) {
+      const float* src = a.p.v_max + static_cast<int64_t>(w.b * p.groups + w.g) * ((p.states + kCols - 1) / kCols);
+      v_part = t0 + lane < t1 ? __ldcg(src + t0 + lane) : 0.f;
+      for (int32_t t = t0 + lane + 32; t < t1; t += 32) v_part = max_of(v_part, __ldcg(src + t));
     };
     auto fetch = [&](int32_t from) -> bool {
       for (int32_t i = from; i < a.n_items; i += gridDim.x) {
@@ -635,18 +634,24 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             next_ndelta = __ldcg(st + kCols);
           }
           if (!BF16) {
-            const int32_t bg = w.b * p.groups + w.g;
-            if (bg != v_of) v_top = largest_value(bg, 0, (w.length + kCols - 1) / kCols);
-            v_of = bg;
-            int32_t e = 0;
-            if (row < w.own) {
-              const int32_t m = w.row0 + row;
-              const float l1 = __ldcg(a.p.row_l1 + static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 * kCols + m);
-              e = power_for(fmaf(l1, v_top, fabsf(next_ndelta)));
-            }
-            next_nlse += static_cast<float>(e - kPowP);
-            next_undo = p.scale * two_to(-e);
+            l1_part = row < w.own ? __ldcg(a.p.row_l1 + static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 * kCols +
+                                           w.row0 + row)
+                                  : 0.f;
+            fetch_values(w, 0, (w.length + kCols - 1) / kCols);
           }
+        } else if (!BF16) {
+          const float2* tops = reinterpret_cast<const float2*>(a.p.tile_max) +
+                               (static_cast<int64_t>(w.b) * p.heads + w.h0) * a.m_tiles64 + w.t0;
+          const float2 top = lane < w.n_t ? __ldcg(tops + lane) : make_float2(0.f, 0.f);
+          l1_part = top.x;
+          delta_part = top.y;
+          for (int32_t t = lane + 32; t < w.n_t; t += 32) {
+            const float2 more_top = __ldcg(tops + t);
+            l1_part = max_of(l1_part, more_top.x);
+            delta_part = max_of(delta_part, more_top.y);
+          }
+          const int32_t t0 = w.row0 / kCols, all = (w.length + kCols - 1) / kCols;
+          fetch_values(w, t0, t0 + kRows / kCols < all ? t0 + kRows / kCols : all);
         }
         return true;
       }
@@ -660,7 +665,16 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       }
       nlse = next_nlse;
       ndelta = next_ndelta;
-      if (!KV && !BF16) undo = next_undo;
+      if (!BF16) {
+        const float v_top = warp_max(v_part);
+        const float bound = KV ? fmaf(warp_max(l1_part), v_top, warp_max(delta_part)) : fmaf(l1_part, v_top, fabsf(ndelta));
+        const int32_t e = power_for(bound);
+        undo = p.scale * two_to(-e);
+        if (KV)
+          lift = two_to(e - kPowP);
+        else
+          nlse += static_cast<float>(e - kPowP);
+      }
     };
     uint32_t tile = 0, items = 0;
     bool ok = true;
@@ -689,22 +703,9 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       }
       const bool more = fetch(item + gridDim.x);
       const float2 nlse2 = make_float2(nlse, nlse), ndelta2 = make_float2(ndelta, ndelta);
-      float2 lift = make_float2(1.f, 1.f);     // dk, dv in f16: from 2^12 P to the factor of dS
-      if (KV && !BF16) {
-        const float2* tops = reinterpret_cast<const float2*>(a.p.tile_max) +
-                             (static_cast<int64_t>(wk.b) * p.heads + wk.h0) * a.m_tiles64 + wk.t0;
-        float l1 = 0.f, delta = 0.f;
-        for (int32_t t = lane; t < wk.n_t; t += 32) {
-          const float2 top = __ldcg(tops + t);
-          l1 = max_of(l1, top.x);
-          delta = max_of(delta, top.y);
-        }
-        const int32_t t0 = wk.row0 / kCols, all = (wk.length + kCols - 1) / kCols;
-        const float v_most = largest_value(wk.b * p.groups + wk.g, t0, t0 + 2 < all ? t0 + 2 : all);
-        const int32_t e = power_for(fmaf(warp_max(l1), v_most, warp_max(delta)));
-        lift = make_float2(two_to(e - kPowP), two_to(e - kPowP));
-        undo = p.scale * two_to(-e);
-      }
+      // the item's own: the hand-over of the next one comes before this one's store
+      const float2 lift2 = make_float2(lift, lift);
+      const float item_undo = undo;
       for (int32_t i = 0; i < wk.n_t; ++i, ++tile) {
         const uint32_t st = tile & 1, s = tile % kStages;
         // The statistics came with the tile that the finished products have read.
@@ -734,7 +735,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             const int c = e + 2 * u;
             const float2 t = fma2(make_float2(__uint_as_float(xr[c]), __uint_as_float(xr[c + 1])), scale2, nl[u]);
             const float2 pr = make_float2(fast_exp2(t.x), fast_exp2(t.y));
-            const float2 g = mul2(KV && !BF16 ? mul2(pr, lift) : pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
+            const float2 g = mul2(KV && !BF16 ? mul2(pr, lift2) : pr, add2(make_float2(__uint_as_float(yr[c]), __uint_as_float(yr[c + 1])), nd[u]));
             if (KV) pw[c / 2] = pack2<BF16>(pr.x, pr.y);
             dw[c / 2] = pack2<BF16>(g.x, g.y);
           }
@@ -770,7 +771,7 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
 #pragma unroll
       for (int y = 0; y < (KV ? 2 : 1); ++y)
         store_row<DP, BF16>(lane_base + kColAcc + y * DP, wg * (DP / kParts),
-                            y == 0 ? (BF16 ? p.scale : undo) : (BF16 ? 1.f : two_to(-kPowP)),
+                            y == 0 ? (BF16 ? p.scale : item_undo) : (BF16 ? 1.f : two_to(-kPowP)),
                             row < wk.own && dst[y] != nullptr, zero,
                             static_cast<uint16_t*>(dst[y]) + lin0 * p.head_dim + off,
                             parts[y] == nullptr ? nullptr : parts[y] + at + off, a.wide, p.head_dim);

@@ -723,3 +723,29 @@ def test_transforms_that_the_kernels_do_not_see_are_refused(cuda_device):
                       lambda: torch.func.grad(lambda t: call(t).float().sum())(q)):
         with pytest.raises((ValueError, RuntimeError)):
             transform()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("sizes,lengths", [((4, 12, 4, 1100, 77, 64), [77, 40, 0, 65]),      # 432 dq items
+                                           ((3, 8, 8, 800, 150, 128), [150, 129, 3]),       # 168 dq, 48 dk / dv
+                                           ((2, 64, 64, 60, 260, 64), [260, 200]),          # 384 dk / dv items
+                                           ((2, 40, 40, 60, 300, 128), None)])
+def test_gradients_of_more_items_than_ctas(cuda_device, sizes, lengths, dtype):
+    """A CTA runs several items, whose gradients differ in size by up to 2^16 from row to row and head
+    to head, and whose values do by 2^8: each item keeps its own scale."""
+    batch, heads, groups, queries, states, dim = sizes
+    q, k, v = _inputs(*sizes, dtype, seed=230)
+    g = torch.Generator().manual_seed(231)
+    rows = torch.randint(-8, 1, (batch, heads, queries, 1), generator=g) + torch.randint(-8, 1, (batch, heads, 1, 1), generator=g)
+    grad = (torch.randn(q.shape, generator=g) * torch.exp2(rows.float())).to(dtype)
+    v = (v.float() * torch.exp2(torch.randint(-8, 1, (batch, groups, 1, 1), generator=g).float())).to(dtype)
+    scale = dim ** -0.5
+    want, bounds = oracle.cross_attention_gradients(q, k, v, grad, scale=scale, lengths=lengths, scaled=True)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    dev = [t.to(cuda_device) for t in (q, k, v)]
+    out, lse = cross_attention_forward(*dev, scale=scale, lengths=lens, want_lse=True)
+    for needs in ((True, True, True), (False, True, True)):
+        got = cross_attention_backward(*dev, out, lse, grad.to(cuda_device), scale=scale, lengths=lens, needs=needs)
+        for g, w, b in zip(got, want, bounds):
+            if g is not None:
+                _assert_within(g, w, b)

@@ -333,3 +333,54 @@ def test_tangents_and_traces_are_refused(cuda_device):
                lambda t: (cache.write(x, x), t)[1]):
         with pytest.raises(ValueError, match="traced"):
             torch.jit.trace(fn, q, check_trace=False)
+
+
+def test_from_the_encoder_to_a_decoder(cuda_device):
+    """As a program uses them: the encoder's features, a step of training over their keys and values,
+    then the cache, a new state, and tokens over it and behind a prefix."""
+    from intp_preliminary_b200.share_vit import ShareViTHalf6d3r
+
+    batch, heads, groups, dim, capacity = 2, 4, 2, 64, 200
+    g = torch.Generator().manual_seed(7)
+    encoder = ShareViTHalf6d3r(precision="bf16").init_weights(seed=1, look_grid_std=0.02).to(cuda_device)
+    images = torch.randn(batch, 3, 224, 224, generator=g).to(cuda_device)
+    to_k, to_v = (torch.nn.Linear(192, groups * dim, bias=False).to(cuda_device, BF16) for _ in range(2))
+    with torch.no_grad():
+        states = encoder.forward_features(images).bfloat16()
+
+    def keys_and_values(states):
+        return [w(states).view(batch, -1, groups, dim).transpose(1, 2) for w in (to_k, to_v)]
+
+    k, v = keys_and_values(states)
+    q = torch.randn(batch, heads, 9, dim, generator=g).to(BF16).to(cuda_device).requires_grad_()
+    grad = torch.randn(batch, heads, 9, dim, generator=g).to(BF16).to(cuda_device)
+    scale = dim ** -0.5
+    out = cross_attention(q, k, v, scale=scale)
+    want, _, bound = oracle.cross_attention(q, k, v, scale=scale)
+    assert ((out.detach().cpu().double() - want).abs() <= bound).all()
+    wants, bounds = oracle.cross_attention_gradients(q, k, v, grad, scale=scale)
+    for got, want, bound in zip(torch.autograd.grad(out, (q, k, v), grad, retain_graph=True), wants, bounds):
+        assert ((got.cpu().double() - want).abs() <= bound).all()
+    out.backward(grad)
+    assert all(torch.isfinite(w.weight.grad).all() and w.weight.grad.abs().max() > 0 for w in (to_k, to_v))
+
+    cache = StateCache.empty(batch, groups, capacity, dim, device=cuda_device)
+    with pytest.raises(ValueError, match="no backward"):
+        cache.write(k, v)
+    filled = torch.full((batch,), k.shape[2], dtype=torch.int32, device=cuda_device)
+    with torch.no_grad():
+        k, v = keys_and_values(states)
+        cache.write(k, v)
+        cache.write(k[:, :, :1], v[:, :, 1:2], start=filled)
+        token = q[:, :, :1]
+        lengths = filled + 1
+        kd, vd = _values(cache.keys, cache.key_exponents), _values(cache.values, cache.value_exponents)
+        got = cached_cross_attention(token, cache, scale=scale, lengths=lengths)
+        want, _, bound = oracle.cross_attention(token, kd, vd, scale=scale, lengths=lengths.tolist(), p_dtype=F16,
+                                                out_dtype=BF16,
+                                                key_weight=torch.exp2(cache.value_exponents.double() - 127))
+        assert ((got.cpu().double() - want).abs() <= bound).all()
+        got = shared_prefix_attention(token, k[0], v[0], cache, scale=scale, lengths=lengths)
+        want, _, bound = oracle.cross_attention(token, kd, vd, scale=scale, lengths=lengths.tolist(),
+                                                prefix=(k[0], v[0]), p_dtype=BF16)
+        assert ((got.cpu().double() - want).abs() <= bound).all()

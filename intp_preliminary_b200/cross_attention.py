@@ -153,8 +153,9 @@ _MAX_PLANS = 1024
 
 class _Plan:
     # backward: by the output gradient's strides, (the argument block's end, scratch bytes)
+    # layout: of q, k, v and out (_layout), for the tensors that a backward gets back
     __slots__ = ("tail", "scratch", "status", "index", "batch", "device", "empty", "out_shape", "lse_shape", "dtype",
-                 "args", "backward")
+                 "args", "backward", "layout", "scale")
 
 
 _plans: dict = {}
@@ -247,6 +248,10 @@ def _lengths_pointer(lengths, plan: _Plan, name: str):
     return lengths, lengths.data_ptr()
 
 
+def _layout(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype
+
+
 def _forward_plan(q, k, v, scale, out_stride, kernel):
     """The plan for these tensors, or None when one has to be laid out first."""
     key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.device,
@@ -258,7 +263,10 @@ def _forward_plan(q, k, v, scale, out_stride, kernel):
         if not (_ready(q) and _ready(k) and _ready(v)):
             return None
         _set_pair(args, k, v)
-        plan = _keep(key, _finish_plan(args, q, "cross attention"))
+        plan = _finish_plan(args, q, "cross attention")
+        plan.layout = (_layout(q), _layout(k), _layout(v), (q.shape, out_stride, q.dtype))
+        plan.scale = scale
+        _keep(key, plan)
     return plan
 
 
@@ -369,7 +377,13 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def _first(ctx, grad_out):
         q, k, v, lengths, out, lse = ctx.saved_tensors
-        return (*_backward(ctx.plan, q, k, v, lengths, out, lse, grad_out, ctx.needs_input_grad[:3]), None, None)
+        plan, needs = ctx.plan, ctx.needs_input_grad[:3]
+        if ((_layout(q), _layout(k), _layout(v), _layout(out)) != plan.layout
+                or (q.data_ptr() | k.data_ptr() | v.data_ptr() | out.data_ptr()) & 15 or not lse.is_contiguous()):
+            # hooks on saved tensors (offloading, compression) return the values, not always the strides
+            return (*cross_attention_backward(q, k, v, out, lse, grad_out, scale=plan.scale, lengths=lengths,
+                                              needs=needs), None, None)
+        return (*_backward(plan, q, k, v, lengths, out, lse, grad_out, needs), None, None)
 
     _once = staticmethod(once_differentiable(_first))
 

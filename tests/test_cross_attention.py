@@ -3,6 +3,7 @@ structs, refusals and workspace sizes, CPU tensors, and the oracle itself."""
 
 import ctypes
 import re
+import sys
 from pathlib import Path
 
 import pytest
@@ -262,3 +263,57 @@ def test_tracing_is_refused():
     for call in _operator_calls(lambda t: t):
         with pytest.raises(ValueError, match="traced"):
             torch.jit.trace(lambda t: (call(), t)[1], torch.zeros(1), check_trace=False)
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """The operators on CPU tensors with every library call recorded instead of made: what a call's
+    argument block says can be compared with the tensors it points to."""
+    module = sys.modules["intp_preliminary_b200.cross_attention"]
+    blocks = []
+    monkeypatch.setattr(module, "_check_states", lambda q, k, v: None)
+    monkeypatch.setattr(module, "_status", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(module, "_plans", {})
+    monkeypatch.setattr(module, "_call", lambda fn, block, index, what: blocks.append(block))
+    return blocks
+
+
+def _strided_leaves():
+    q = torch.randn(2, 7, 4, 16).bfloat16().requires_grad_()
+    kv = torch.randn(2, 30, 2, 2, 16).bfloat16().requires_grad_()
+    return q.transpose(1, 2), kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+
+
+@pytest.mark.parametrize("form", ["same", "contiguous", "padded", "unaligned"])
+def test_backward_describes_the_tensors_that_hooks_return(recorded, form):
+    """Hooks on saved tensors (offloading, compression) may return other strides than were saved: the
+    backward's block must hold the strides and the 16-byte rows of what it points to."""
+    held = {}
+
+    def pack(t):
+        if form == "same" or t.dtype != torch.bfloat16:
+            kept = t
+        elif form == "contiguous":
+            kept = t.clone(memory_format=torch.contiguous_format)
+        else:
+            wide = torch.empty(*t.shape[:-1], t.shape[-1] + 8, dtype=t.dtype)
+            kept = wide[..., 8:] if form == "padded" else wide[..., 1:t.shape[-1] + 1]
+            kept.copy_(t)
+        held[kept.data_ptr()] = kept
+        return kept
+
+    q, k, v = _strided_leaves()
+    lengths = torch.tensor([30, 11], dtype=torch.int32)
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = cross_attention(q, k, v, scale=0.25, lengths=lengths)
+    torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    args = _lib.XattnBackwardArgs.from_buffer_copy(recorded[-1])
+    f = args.fwd
+    assert (f.batch, f.heads, f.groups, f.queries, f.states, f.head_dim) == (2, 4, 2, 7, 30, 16)
+    for pointer, stride in ((f.q, f.q_stride), (f.k, f.k_stride), (f.v, f.v_stride), (f.out, f.out_stride)):
+        assert pointer % 16 == 0
+        if form == "unaligned":
+            assert pointer not in held and list(stride[2:]) == [16, 1]
+        else:
+            assert tuple(stride) == held[pointer].stride()
+    assert f.lengths in held and f.lse in held

@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from intp_preliminary_b200 import (_lib, check_device_status, cross_attention, cross_attention_backward,
                                    cross_attention_forward, shared_prefix_attention)
@@ -749,3 +750,36 @@ def test_gradients_of_more_items_than_ctas(cuda_device, sizes, lengths, dtype):
         for g, w, b in zip(got, want, bounds):
             if g is not None:
                 _assert_within(g, w, b)
+
+
+@pytest.mark.parametrize("form", ["contiguous", "padded", "unaligned", "cpu", "checkpoint"])
+def test_gradients_through_hooks_on_saved_tensors(cuda_device, form):
+    """Offloaded, copied and recomputed tensors come back in other layouts: the same gradients."""
+    base = _normal((2, 37, 4, 64), BF16, 240).to(cuda_device)
+    both = _normal((2, 210, 2, 2, 64), BF16, 241).to(cuda_device)
+    grad = _normal((2, 4, 37, 64), BF16, 242).to(cuda_device)
+    lengths = torch.tensor([210, 77], dtype=torch.int32, device=cuda_device)
+
+    def pack(t):
+        if form == "cpu":
+            return t.cpu()
+        if t.dtype != BF16:
+            return t
+        if form == "contiguous":
+            return t.clone(memory_format=torch.contiguous_format)
+        wide = torch.empty(*t.shape[:-1], t.shape[-1] + 8, dtype=t.dtype, device=t.device)
+        return (wide[..., 8:] if form == "padded" else wide[..., 1:t.shape[-1] + 1]).copy_(t)
+
+    def attend(x, kv):
+        return cross_attention(x.transpose(1, 2), kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2), scale=0.125,
+                               lengths=lengths)
+
+    leaves = [base.clone().requires_grad_(), both.clone().requires_grad_()]
+    want = torch.autograd.grad(attend(*leaves), leaves, grad)
+    if form == "checkpoint":
+        out = torch.utils.checkpoint.checkpoint(attend, *leaves, use_reentrant=False)
+    else:
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(cuda_device)):
+            out = attend(*leaves)
+    for g, w in zip(torch.autograd.grad(out, leaves, grad), want):
+        assert torch.equal(g, w)

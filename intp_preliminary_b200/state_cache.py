@@ -50,24 +50,32 @@ class StateCache:
 
     The cache does not know how many of its states are filled: a program keeps
     its sequences' lengths and passes them (``start`` of a write, ``lengths`` of
-    the attention)."""
+    the attention).  Its tensors may be written to but not replaced: other tensors
+    are another ``StateCache``, which costs no copy."""
 
     def __init__(self, keys, key_exponents, values, value_exponents) -> None:
         for t in (keys, key_exponents, values, value_exponents):
             if not isinstance(t, torch.Tensor):
                 raise ValueError("a state cache requires CUDA tensors")
         # what the tensors' layout decides is checked once and known by it
-        self.layout = (keys.shape, keys.stride(), keys.dtype, keys.device, values.shape, values.stride(), values.dtype,
+        self._layout = (keys.shape, keys.stride(), keys.dtype, keys.device, values.shape, values.stride(), values.dtype,
                        values.device, key_exponents.shape, key_exponents.stride(), key_exponents.dtype,
                        key_exponents.device, value_exponents.shape, value_exponents.stride(), value_exponents.dtype,
                        value_exponents.device)
-        if self.layout not in _plans:
+        if self._layout not in _plans:
             _check_tensors(keys, key_exponents, values, value_exponents)
-            _keep(self.layout, None)
+            _keep(self._layout, None)
         if (keys.data_ptr() | values.data_ptr()) & 15:
             raise ValueError("the cache's tensors must be contiguous, codes 16-byte aligned")
-        self.keys, self.values = keys, values
-        self.key_exponents, self.value_exponents = key_exponents, value_exponents
+        self._keys, self._values = keys, values
+        self._key_exponents, self._value_exponents = key_exponents, value_exponents
+
+    # read only: a call takes the layout that was checked above
+    keys = property(lambda self: self._keys)
+    values = property(lambda self: self._values)
+    key_exponents = property(lambda self: self._key_exponents)
+    value_exponents = property(lambda self: self._value_exponents)
+    layout = property(lambda self: self._layout)
 
     @classmethod
     def empty(cls, batch: int, groups: int, capacity: int, head_dim: int, *, device) -> "StateCache":

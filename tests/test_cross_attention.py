@@ -317,3 +317,15 @@ def test_backward_describes_the_tensors_that_hooks_return(recorded, form):
         else:
             assert tuple(stride) == held[pointer].stride()
     assert f.lengths in held and f.lse in held
+
+
+def test_a_cache_keeps_its_tensors(monkeypatch):
+    """Calls take the layout that was checked when the cache was made: its tensors cannot be replaced."""
+    module = sys.modules["intp_preliminary_b200.state_cache"]
+    monkeypatch.setattr(module, "_check_tensors", lambda *tensors: None)
+    monkeypatch.setattr(module, "_keep", lambda key, plan: plan)
+    cache = StateCache.empty(2, 2, 8, 16, device="cpu")
+    for name in ("keys", "values", "key_exponents", "value_exponents", "layout"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name)[:1])
+    assert cache.shape == tuple(cache.keys.shape) == (2, 2, 8, 16)

@@ -508,7 +508,7 @@ xattn_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
         float v[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(o[e]) * inv;
+        for (int e = 0; e < 16; ++e) v[e] = none ? 0.f : __uint_as_float(o[e]) * inv;
         if (r < p.rows)  // a lane past the instance's rows only takes part in the TMEM loads
           store16<BF16>(v, static_cast<uint16_t*>(p.out) + x.b * p.os[0] + x.h * p.os[1] + x.m * p.os[2],
                         split ? p.part_o + slot * p.head_dim : nullptr, a.wide, c * 16, p.head_dim);

@@ -783,3 +783,17 @@ def test_gradients_through_hooks_on_saved_tensors(cuda_device, form):
             out = attend(*leaves)
     for g, w in zip(torch.autograd.grad(out, leaves, grad), want):
         assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan"), "largest"])
+@pytest.mark.parametrize("states", [1, 40, 300, 3000])
+def test_a_row_of_minus_infinite_scores_gives_zeros_whatever_the_values(cuda_device, states, value, kernel):
+    """Its output is zero, not a sum of values times zero; the row beside it sees them."""
+    q, k, v = _inputs(2, 2, 2, 2, states, 64, BF16, seed=250)
+    q[..., 3], k[..., 3] = 1.0, -float("inf")
+    q[:, :, 1, 3] = 0.0                    # 0 * -inf: a NaN row
+    v[:, :, ::3] = torch.finfo(BF16).max if value == "largest" else value
+    got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, want_lse=True, kernel=kernel)
+    assert (got[:, :, 0] == 0).all() and (lse[:, :, 0] == -float("inf")).all()
+    assert torch.isnan(got[:, :, 1]).all()

@@ -32,7 +32,10 @@
 // an exact power of two that the accumulator's store takes out again: P times 2^12, dS times a
 // power that brings a bound of it to 2^12 (dS_i <= P (sum |dO_i| max |v| + |delta_i|)), one per query
 // row in dq (free: it joins the exponent of P), one per item in dk / dv (a multiplication a
-// pair).  The bound's parts come from the statistics kernel, which reads V once for it.
+// pair).  The bound's parts come from the statistics kernel, which reads V once for it.  That and
+// the multiplication cost f16 5 to 7 % (B4 H16 M2048 N4096: D128 759 -> 793 to 808 us, D64 514 to 522
+// -> 557 to 564).  delta uses the rounded result, whose error is one rounding of dO out: the
+// unrounded one is not kept by a forward.
 #include <cuda.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"
@@ -45,7 +48,8 @@ namespace {
 constexpr int kRows = 128;                 // TMEM lanes: query rows (dq) / keys (dk, dv)
 constexpr int kCols = 64;                  // streamed tile: keys (dq) / query rows (dk, dv)
 // Columns of a tile per row thread.  8 warps of 32 columns: 716 us for the backward of B4 H16
-// M2048 N4096 D128; 16 warps of 16 columns execute a third more instructions: 735 us.
+// M2048 N4096 D128; 16 warps of 16 columns execute a third more instructions: 735 us (one box, in
+// turn; the backward takes 726 to 751 us on others).
 constexpr int kW = 32;
 constexpr int kParts = kCols / kW;         // row threads of a row
 constexpr int kRowThreads = kRows * kParts;

@@ -24,7 +24,8 @@
 // 8-bit states are widened to f16 (exact) as they leave shared memory.  The
 // key's power of two multiplies the score; the value's joins the exponent of the
 // probability, whose own reference (score + value exponent) keeps the f16
-// product operand below 2^8 whatever the exponents are.  A bf16 query row is
+// product operand below 2^8 whatever the exponents are.  It goes in as one f16 number: its 2^-11
+// is a hundredth of the codes' own 2^-4, and issue slots, not only memory, bound this form.  A bf16 query row is
 // first scaled by a power of two into the f16 range.
 #include <cstdint>
 #include "xattn_common.cuh"

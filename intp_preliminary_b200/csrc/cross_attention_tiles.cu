@@ -22,13 +22,15 @@
 //                   so one's products run under the other's softmax.
 //
 // P is rounded to 16 bits because the tensor core takes no wider operand of this
-// rate; S, the softmax statistics and O stay in fp32.  Every mbarrier wait is
+// rate (two parts of it, as the few-rows kernel multiplies, would be half as many products
+// again): 1.4 times the error of a 32-bit computation rounded once, 0.0024 for 0.0017 in
+// bf16.  S, the softmax statistics and O stay in fp32.  Every mbarrier wait is
 // bounded (sm100_ptx.cuh); on expiry the CTA unwinds and reports.
 //
 // Bound by the chain scores -> exponentials -> product of each warpgroup, which the
-// other one's products fill: at B4 H16 M2048 N4096 D128 227 us, 1.21 PFLOP/s, the
-// tensor pipe busy 64 % of the time (32 % where one lane of a divergent branch issued
-// the products).  Two threads per row (16 softmax warps) measured 249 us: the
+// other one's products fill: at B4 H16 M2048 N4096 D128 226 to 228 us in bf16, 1.21 PFLOP/s.
+// The tensor pipe is busy 64 % of the time at B1 (32 % where one lane of a divergent branch
+// issued the products).  Two threads per row (16 softmax warps) measured 249 us: the
 // instructions of four warps a scheduler cost more than the shorter chain gives.
 #include <cuda.h>
 #include <cstdint>
@@ -138,7 +140,8 @@ __device__ __forceinline__ void regs_dec() {
 }
 
 // Of each four key pairs, those whose exponentials run on the FMA pipe (the rest on the MUFU).
-// One measured best: 239 us (none: 249, two: 242) at B4 H16 M2048 N4096 D128.
+// One measured best: 239 us (none: 249, two: 242) at B4 H16 M2048 N4096 D128; the polynomial is
+// within 7.5e-5, a fiftieth of a bf16 rounding and a sixth of an f16 one.  Head_dim 64 was not swept.
 constexpr int kFmaPairs = 1;
 
 template <int DP, bool BF16>

@@ -30,12 +30,14 @@
 // P and dS are rounded to 16 bits as the tensor core's operands; all sums are fp32.  f16 has
 // full precision for 30 powers of two only, and P is about 1 / N, so there both are held times
 // an exact power of two that the accumulator's store takes out again: P times 2^12, dS times a
-// power that brings a bound of it to 2^12 (dS_i <= P (sum |dO_i| max |v| + |delta_i|)), one per query
-// row in dq (free: it joins the exponent of P), one per item in dk / dv (a multiplication a
-// pair).  The bound's parts come from the statistics kernel, which reads V once for it.  That and
-// the multiplication cost f16 5 to 7 % (B4 H16 M2048 N4096: D128 759 -> 793 to 808 us, D64 514 to 522
-// -> 557 to 564).  delta uses the rounded result, whose error is one rounding of dO out: the
-// unrounded one is not kept by a forward.
+// power that brings a bound of it to 2^15 (|dS_ij| <= P (|dO_i| |v_j| + |delta_i|), vectors'
+// lengths), one per query row in dq (free: it joins the exponent of P), one per key and item in
+// dk / dv (a multiplication a pair).  A state that is hardly read, with a value R times as long as
+// the others', takes log2(R) of those bits from dq's other states and none from dk's.  The bound's
+// parts come from the statistics kernel, which reads V once for it.  That and the multiplication
+// cost f16 5 to 7 % (B4 H16 M2048 N4096: D128 755 to 765 -> 793 to 815 us, D64 514 to 528 -> 543 to
+// 578).  delta uses the rounded result, whose error is one rounding of dO out: the unrounded one
+// is not kept by a forward.
 #include <cuda.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"
@@ -64,11 +66,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 // forward and here makes of it (a score of 2^24 is an even number): 2^16 P may not be reached.
 constexpr int32_t kPowP = 12;
 
-// f16: the power of two that brings a bound of |dS| / P to [2^11, 2^12), the same distance from
-// overflow; 0 for no bound (zero, or not finite: then the gradients are not either).
+// f16: the power of two that brings a bound of |dS| / P to [2^14, 2^15): P up to 2 does not
+// overflow, and where it is past 1 by rounding it is the row's only one, whose dP - delta is near
+// zero.  0 for no bound (zero, or not finite: then the gradients are not either).
 __device__ __forceinline__ int32_t power_for(float bound) {
   const int32_t e = static_cast<int32_t>(__float_as_uint(bound) >> 23) - 127;
-  return e == 128 || e == -127 ? 0 : kPowP - 1 - e;
+  return e == 128 || e == -127 ? 0 : 14 - e;
 }
 __device__ __forceinline__ float two_to(int32_t e) { return __int_as_float((e + 127) << 23); }
 // Of numbers that are not negative; NaN counts as the largest.
@@ -149,14 +152,14 @@ __device__ __forceinline__ Work decode_work(const Args& a, int32_t item) {
 // ============================================================================ row statistics
 // A block takes 64 rows of one head, D / 8 lanes (rounded to a power of two) a row, every
 // lane's loads in flight at once.  Rows past M, and rows without states, get -lse = -inf:
-// their P is zero.  In f16 it also takes what bounds dS: sum |dO| of each row, the largest of
-// it and of |delta| in the block, and, in blocks behind the rows', the largest |v| of 64 states.
+// their P is zero.  In f16 it also takes what bounds dS: |dO| of each row, the largest of it and
+// of |delta| in the block, and, in blocks behind the rows', |v| of each of 64 states and the largest.
 
-// The largest |v| of the visible ones of 64 states.
+// |v| of 64 states (zero for one that is not visible) and the largest of them.
 template <int LPR>
-__device__ __forceinline__ void state_max(const XaBwdParams& bp, int32_t index) {
+__device__ __forceinline__ void state_norms(const XaBwdParams& bp, int32_t index) {
   constexpr int kPerPass = 256 / LPR, kPasses = kCols / kPerPass;
-  __shared__ uint32_t warp_top[8];
+  __shared__ float warp_top[8];
   const XaParams& p = bp.f;
   const int32_t tiles = (p.states + kCols - 1) / kCols;
   const int32_t bg = index / tiles, n0 = (index - bg * tiles) * kCols;
@@ -170,18 +173,30 @@ __device__ __forceinline__ void state_max(const XaBwdParams& bp, int32_t index) 
     x[i] = n < length && sub * 8 < p.head_dim ? __ldg(reinterpret_cast<const uint4*>(v + n * p.vs[2]))
                                               : make_uint4(0u, 0u, 0u, 0u);
   }
-  uint32_t top = 0u;                       // magnitudes order like their bits
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
-    const uint32_t m = 0x7fff7fffu;
-    top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & m, x[i].y & m), __vmaxu2(x[i].z & m, x[i].w & m)));
+    const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack2<false>(xs[e]);
+      sum = fma2(f, f, sum);
+    }
+    float square = sum.x + sum.y;
+#pragma unroll
+    for (int s = LPR / 2; s > 0; s >>= 1) square += __shfl_xor_sync(0xffffffffu, square, s);
+    const float norm = sqrtf(square);
+    const int32_t n = n0 + r0 + i * kPerPass;
+    if (sub == 0 && n < p.states) bp.v_norm[static_cast<int64_t>(bg) * p.states + n] = norm;
+    top = max_of(top, norm);
   }
-  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+  top = warp_max(top);
   if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) top = max(top, warp_top[i]);
-    bp.v_max[index] = unpack2<false>(top).x;
+    for (int i = 1; i < 8; ++i) top = max_of(top, warp_top[i]);
+    bp.v_max[index] = top;
   }
 }
 
@@ -189,12 +204,12 @@ template <int LPR, bool BF16>
 __global__ void __launch_bounds__(256)
 xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
   constexpr int kPerPass = 256 / LPR, kPasses = kCols / kPerPass;
-  __shared__ float row_max[2][kCols];      // f16: sum |dO| and |delta| of the block's rows
+  __shared__ float row_max[2][kCols];      // f16: |dO| and |delta| of the block's rows
   allow_next_kernel();
   const XaParams& p = bp.f;
   const int32_t row_blocks = p.batch * p.heads * m_tiles64;
   if (!BF16 && blockIdx.x >= row_blocks) {
-    state_max<LPR>(bp, blockIdx.x - row_blocks);
+    state_norms<LPR>(bp, blockIdx.x - row_blocks);
     return;
   }
   const int32_t bh = blockIdx.x / m_tiles64, m0 = (blockIdx.x - bh * m_tiles64) * kCols;
@@ -213,17 +228,18 @@ xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
-    float2 sum = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
+    float2 sum = make_float2(0.f, 0.f), squares = make_float2(0.f, 0.f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      sum = fma2(unpack2<BF16>(xs[e]), unpack2<BF16>(ys[e]), sum);
-      if (!BF16) l1 = add2(l1, unpack2<BF16>(ys[e] & 0x7fff7fffu));
+      const float2 go = unpack2<BF16>(ys[e]);
+      sum = fma2(unpack2<BF16>(xs[e]), go, sum);
+      if (!BF16) squares = fma2(go, go, squares);
     }
-    float delta = sum.x + sum.y, row_l1 = l1.x + l1.y;
+    float delta = sum.x + sum.y, square = squares.x + squares.y;
 #pragma unroll
     for (int s = LPR / 2; s > 0; s >>= 1) {
       delta += __shfl_xor_sync(0xffffffffu, delta, s);
-      if (!BF16) row_l1 += __shfl_xor_sync(0xffffffffu, row_l1, s);
+      if (!BF16) square += __shfl_xor_sync(0xffffffffu, square, s);
     }
     if (sub == 0) {
       const int32_t r = r0 + i * kPerPass, m = m0 + r;
@@ -232,8 +248,9 @@ xattn_stats_kernel(const XaBwdParams bp, float* stats, int32_t m_tiles64) {
       dst[0] = l == -INFINITY ? -INFINITY : BF16 ? -l * kLog2e : fmaf(-l, kLog2e, static_cast<float>(kPowP));
       dst[kCols] = -delta;
       if (!BF16) {
-        bp.row_l1[static_cast<int64_t>(blockIdx.x) * kCols + r] = row_l1;
-        row_max[0][r] = row_l1;
+        const float norm = sqrtf(square);
+        bp.row_norm[static_cast<int64_t>(blockIdx.x) * kCols + r] = norm;
+        row_max[0][r] = norm;
         row_max[1][r] = fabsf(delta);
       }
     }
@@ -601,16 +618,11 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
     // The next item with tiles, its owned row and (dq) the row's statistics, fetched one item ahead.
     OwnedRow<DP> owned;
     float nlse = -INFINITY, ndelta = 0.f, next_nlse = -INFINITY, next_ndelta = 0.f;
-    // f16: the bound of dS as fetched, this lane's part of it (dq: |dO| of the row itself), and what
-    // it gives at the hand-over: the factor that takes dS's power of two out of an accumulator again
-    // and (dk, dv) the one from 2^12 P to the factor of dS.
-    float l1_part = 0.f, delta_part = 0.f, v_part = 0.f, undo = p.scale, lift = 1.f;
-    // This lane's part of the largest |v| in 64-state tiles [t0, t1) of a sequence and key head.
-    auto fetch_values = [&](const Work& w, int32_t t0, int32_t t1) {
-      const float* src = a.p.v_max + static_cast<int64_t>(w.b * p.groups + w.g) * ((p.states + kCols - 1) / kCols);
-      v_part = t0 + lane < t1 ? __ldcg(src + t0 + lane) : 0.f;
-      for (int32_t t = t0 + lane + 32; t < t1; t += 32) v_part = max_of(v_part, __ldcg(src + t));
-    };
+    // f16: the bound of dS as fetched (dq: |dO| of the row, this lane's part of the largest |v|;
+    // dk, dv: this lane's part of the largest |dO| and |delta|, |v| of the key), and what it gives at
+    // the hand-over: the factor that takes dS's power of two out of an accumulator again and (dk,
+    // dv) the one from 2^12 P to the factor of dS.
+    float go_part = 0.f, delta_part = 0.f, v_part = 0.f, undo = p.scale, lift = 1.f;
     auto fetch = [&](int32_t from) -> bool {
       for (int32_t i = from; i < a.n_items; i += gridDim.x) {
         const Work w = decode_work<KV>(a, i);
@@ -638,24 +650,27 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
             next_ndelta = __ldcg(st + kCols);
           }
           if (!BF16) {
-            l1_part = row < w.own ? __ldcg(a.p.row_l1 + static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 * kCols +
+            go_part = row < w.own ? __ldcg(a.p.row_norm + static_cast<int64_t>(w.b * p.heads + w.h0) * a.m_tiles64 * kCols +
                                            w.row0 + row)
                                   : 0.f;
-            fetch_values(w, 0, (w.length + kCols - 1) / kCols);
+            const int32_t t1 = (w.length + kCols - 1) / kCols;
+            const float* src = a.p.v_max + static_cast<int64_t>(w.b * p.groups + w.g) * ((p.states + kCols - 1) / kCols);
+            v_part = lane < t1 ? __ldcg(src + lane) : 0.f;
+            for (int32_t t = lane + 32; t < t1; t += 32) v_part = max_of(v_part, __ldcg(src + t));
           }
         } else if (!BF16) {
           const float2* tops = reinterpret_cast<const float2*>(a.p.tile_max) +
                                (static_cast<int64_t>(w.b) * p.heads + w.h0) * a.m_tiles64 + w.t0;
           const float2 top = lane < w.n_t ? __ldcg(tops + lane) : make_float2(0.f, 0.f);
-          l1_part = top.x;
+          go_part = top.x;
           delta_part = top.y;
           for (int32_t t = lane + 32; t < w.n_t; t += 32) {
             const float2 more_top = __ldcg(tops + t);
-            l1_part = max_of(l1_part, more_top.x);
+            go_part = max_of(go_part, more_top.x);
             delta_part = max_of(delta_part, more_top.y);
           }
-          const int32_t t0 = w.row0 / kCols, all = (w.length + kCols - 1) / kCols;
-          fetch_values(w, t0, t0 + kRows / kCols < all ? t0 + kRows / kCols : all);
+          v_part = row < w.own ? __ldcg(a.p.v_norm + static_cast<int64_t>(w.b * p.groups + w.g) * p.states + w.row0 + row)
+                               : 0.f;
         }
         return true;
       }
@@ -670,9 +685,8 @@ xattn_grad_kernel(const __grid_constant__ CUtensorMap tm_f0, const __grid_consta
       nlse = next_nlse;
       ndelta = next_ndelta;
       if (!BF16) {
-        const float v_top = warp_max(v_part);
-        const float bound = KV ? fmaf(warp_max(l1_part), v_top, warp_max(delta_part)) : fmaf(l1_part, v_top, fabsf(ndelta));
-        const int32_t e = power_for(bound);
+        const int32_t e = power_for(KV ? fmaf(warp_max(go_part), v_part, warp_max(delta_part))
+                                       : fmaf(go_part, warp_max(v_part), fabsf(ndelta)));
         undo = p.scale * two_to(-e);
         if (KV)
           lift = two_to(e - kPowP);

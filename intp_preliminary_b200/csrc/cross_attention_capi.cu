@@ -224,7 +224,7 @@ int32_t launch_pass(XaParams p, const Pass& s, int64_t first, cudaStream_t strea
 }
 
 struct BackwardPlan {
-  int64_t row_l1, tile_max, v_max;                   // byte offsets (f16); the statistics come first
+  int64_t row_norm, tile_max, v_norm, v_max;         // byte offsets (f16); the statistics come first
   int64_t dq_part, dk_part, dv_part, bytes;          // byte offsets; 0 = no part buffer
   int32_t dq_split, dq_tiles, kv_split, kv_tiles;
 };
@@ -246,10 +246,12 @@ BackwardPlan plan_backward(const xattn_backward_args* b) {
   const int64_t row_tiles = a->batch * a->heads * m64;
   int64_t at = align256(row_tiles * 128 * 4);
   if (a->dtype == INTP_F16) {
-    p.row_l1 = at;
+    p.row_norm = at;
     at += align256(row_tiles * 64 * 4);
     p.tile_max = at;
     at += align256(row_tiles * 2 * 4);
+    p.v_norm = at;
+    at += align256(a->batch * a->groups * a->states * 4);
     p.v_max = at;
     at += align256(a->batch * a->groups * n64 * 4);
   }
@@ -404,8 +406,9 @@ intp_status xattn_backward(const xattn_backward_args* b, void* stream) {
   p.dv = b->grad_v;
   p.delta = reinterpret_cast<float*>(ws);
   if (a->dtype == INTP_F16) {
-    p.row_l1 = reinterpret_cast<float*>(ws + plan.row_l1);
+    p.row_norm = reinterpret_cast<float*>(ws + plan.row_norm);
     p.tile_max = reinterpret_cast<float*>(ws + plan.tile_max);
+    p.v_norm = reinterpret_cast<float*>(ws + plan.v_norm);
     p.v_max = reinterpret_cast<float*>(ws + plan.v_max);
   }
   p.dq_part = plan.dq_part ? reinterpret_cast<float*>(ws + plan.dq_part) : nullptr;

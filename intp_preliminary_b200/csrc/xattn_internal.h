@@ -48,9 +48,10 @@ struct XaBwdParams {
   const void* dout; int64_t ds[3];
   void* dq; void* dk; void* dv;      // 16-bit, contiguous; null when not wanted
   float* delta;                      // row statistics: [B * H][ceil(M / 64)][-lse 64 | -delta 64]
-  // f16 only, what bounds dS: sum |dO| of a query row, [B * H][ceil(M / 64)][64]; the largest of
-  // that and of |delta| in 64 rows, two numbers each; the largest |v| of 64 states, [B * G][ceil(N / 64)].
-  float* row_l1; float* tile_max; float* v_max;
+  // f16 only, what bounds dS: the length |dO| of a query row, [B * H][ceil(M / 64)][64]; the largest of
+  // that and of |delta| in 64 rows, two numbers each; the length |v| of a state, [B * G][N], and the
+  // largest of 64 states, [B * G][ceil(N / 64)].
+  float* row_norm; float* tile_max; float* v_norm; float* v_max;
   // Splits of the streamed axis: fp32 partial sums [split][elements], null when 1.
   float* dq_part; int32_t dq_split, dq_split_tiles;
   float* dk_part; float* dv_part; int32_t kv_split, kv_split_tiles;

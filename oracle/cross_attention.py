@@ -88,20 +88,24 @@ def cross_attention_gradients(q, k, v, grad, *, scale, lengths=None, scaled=Fals
     """``((dq, dk, dv), (their bounds))`` in float64 on the CPU.
 
     ``scaled``: for a kernel that brings P and dS into f16's range by powers of two, so that a
-    bound knows no absolute size but the result's own.  With r = sum |dO| max |v| + |delta| of a
-    query row, at least |dS|, it holds 2^e dS with 2^11 <= 2^e r: what f16 loses below 2^-14 is at
-    most 2^-25 of that unit, 2^-36 r (dk: the largest r of the streamed rows).  P is held as
-    2^12 P: 2^-37.  The result loses at most 2^-25 when it is rounded (f16's last step is 2^-24)."""
+    bound knows no absolute size but the result's own.  With r = |dO| max |v_j| + |delta| of a query
+    row (lengths of vectors), at least |dS|, it holds 2^e dS with 2^14 <= 2^e r: what f16 loses below
+    2^-14 is at most 2^-25 of that unit, 2^-39 r (dk: of the key's own |v_j| and the largest |dO| and
+    |delta| of the rows that read it).  P is held as 2^12 P: 2^-37.  The result loses at most 2^-25 when it is rounded (f16's last step is 2^-24)."""
     dtype = q.dtype
     u = _u(dtype)
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     last = 1e-7
     if scaled:
         last = 2.0 ** -25 if dtype == torch.float16 else 0.0
-    _, _, out_bound = cross_attention(q, k, v, scale=scale, lengths=lengths)
+    out, _, out_bound = cross_attention(q, k, v, scale=scale, lengths=lengths)
     q, k, v, grad = (t.detach().cpu().double() for t in (q, k, v, grad))
     batch, heads = q.shape[:2]
     groups, n = k.shape[1], k.shape[2]
+
+    def delta_of(b, h):
+        return (grad[b, h] * out[b, h]).sum(-1, keepdim=True).abs()
+
     d = [torch.zeros_like(t) for t in (q, k, v)]
     e = [torch.zeros_like(t) for t in (q, k, v)]
     rel = u + EXP + 2 * LSE
@@ -118,11 +122,10 @@ def cross_attention_gradients(q, k, v, grad, *, scale, lengths=None, scaled=Fals
             ds_bound = rel * ds.abs() + p * (delta_bound + 1e-5 * (go.abs() @ vv.abs().T))
             ds_row, ds_all, p_tiny = tiny, tiny, tiny
             if scaled:
-                delta = (p * dp).sum(-1, keepdim=True).abs()
-                ds_row = 2.0 ** -36 * (go.abs().sum(-1, keepdim=True) * vv.abs().max() + delta)
-                heads_of = range(g * (heads // groups), (g + 1) * (heads // groups))
-                most = max(float(grad[b, x].abs().sum(-1).max()) for x in heads_of)  # |delta| <= sum |dO| max |v|
-                ds_all = 2.0 ** -36 * 2 * most * float(vv.abs().max())
+                ds_row = 2.0 ** -39 * (go.norm(dim=-1, keepdim=True) * vv.norm(dim=-1).max() + delta_of(b, h))
+                of_group = range(g * (heads // groups), (g + 1) * (heads // groups))
+                most = max(float(grad[b, x].norm(dim=-1).max()) for x in of_group)
+                ds_all = 2.0 ** -39 * (most * vv.norm(dim=-1) + max(float(delta_of(b, x).max()) for x in of_group))
                 p_tiny = 2.0 ** -37
             p_bound = rel * p + p_tiny
             d[0][b, h] = scale * (ds @ kk)

@@ -797,3 +797,29 @@ def test_a_row_of_minus_infinite_scores_gives_zeros_whatever_the_values(cuda_dev
     got, lse = cross_attention_forward(*(t.to(cuda_device) for t in (q, k, v)), scale=0.125, want_lse=True, kernel=kernel)
     assert (got[:, :, 0] == 0).all() and (lse[:, :, 0] == -float("inf")).all()
     assert torch.isnan(got[:, :, 1]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("far", [1e3, 6e4])
+@pytest.mark.parametrize("dim,states", [(64, 4096), (128, 1000)])
+def test_a_large_value_that_is_hardly_read_costs_the_others_nothing(cuda_device, dim, states, far, dtype):
+    """States with values far above the others' and probabilities near zero: dk of every other key
+    keeps its bits, and dq loses 2^-39 of |dO| |v| per state."""
+    q, k, v = _inputs(1, 2, 1, 100, states, dim, dtype, seed=260)
+    q[..., 3] = 4.0
+    hidden = list(range(5, states, 97))
+    k[:, :, hidden, 3] = -60.0             # scores of -30 and below: probabilities near 2^-55
+    v[:, :, hidden] = far
+    grad = _normal(q.shape, dtype, 261)
+    scale = dim ** -0.5
+    want, bounds = oracle.cross_attention_gradients(q, k, v, grad, scale=scale, scaled=True)
+    dev = [t.to(cuda_device) for t in (q, k, v)]
+    out, lse = cross_attention_forward(*dev, scale=scale, want_lse=True)
+    got = cross_attention_backward(*dev, out, lse, grad.to(cuda_device), scale=scale)
+    for g, w, b in zip(got, want, bounds):
+        _assert_within(g, w, b)
+    # As a whole, too: dS and the result are rounded (u each), P is within 6.5e-4 (1.4 u in f16).  dq adds
+    # 2^-39 |dO| |v| to each dS of about 2^-12 |dO|: 2^-27 |v|, 2^-14 for |v| = 8e3, ten times u for 5e5.
+    for g, w in list(zip(got, want))[1 if far > 1e4 else 0:2]:
+        off = (g.cpu().double() - w).norm() / w.norm()
+        assert off <= 4 * torch.finfo(dtype).eps / 2, float(off)

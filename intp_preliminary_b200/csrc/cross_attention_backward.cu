@@ -36,8 +36,8 @@
 // the others', takes log2(R) of those bits from dq's other states and none from dk's.  The bound's
 // parts come from the statistics kernel, which reads V once for it.  That and the multiplication
 // cost f16 5 to 7 % (B4 H16 M2048 N4096: D128 755 to 765 -> 793 to 815 us, D64 514 to 528 -> 543 to
-// 578).  delta uses the rounded result, whose error is one rounding of dO out: the unrounded one
-// is not kept by a forward.
+// 578).  delta uses the rounded result, the only one a forward gives: nothing beside the rounding
+// of dS over many states (dq 0.0024 for 0.0017 in bf16), a little over few (0.0025 at 50).
 #include <cuda.h>
 #include <cstdint>
 #include "sla_tc_common.cuh"

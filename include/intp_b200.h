@@ -403,6 +403,70 @@ INTP_API intp_status state_cache_write(const state_cache_args* a, void* stream);
  * outside the cache read as zero. */
 INTP_API intp_status state_cache_read(const state_cache_args* a, void* stream);
 
+/* ---- a decoder's own tokens --------------------------------------------------
+ * Queries and keys turned by their positions, a paged cache of keys and values,
+ * and attention of new tokens over it.
+ *
+ * q (B, H, n, D), k and v (B, G, n, D); D a multiple of 8 up to 128; dtype INTP_F16
+ * or INTP_BF16 (rotary_positions also INTP_F32).  Unit stride along D, 16-byte
+ * aligned rows, outer strides that are multiples of 16 bytes below 2^40: positive,
+ * or (inputs q, k, v of the two rotary calls) zero for a broadcast dimension.
+ *
+ * The cache: keys and values (pages, G, page_size, D), any such strides.  State p of
+ * sequence b is row p % page_size of page page_table[b][p / page_size]; the table
+ * holds table_width pages a sequence.  A page number outside 0 .. pages - 1 is no
+ * page: rows that belong there are not written, and states there take no part.
+ */
+typedef struct rotary_args {
+  const void* q; const void* k; const void* v;    /* absent ones null; v only to append */
+  void* q_out; void* k_out; void* v_out;          /* like the inputs; k_out, v_out of an append: the cache */
+  /* Pair i of the first rotary_dim columns turns by position[axis[i]] * turns[i] turns
+   * (radians / 2 pi), rotary_dim / 2 entries each, axis[i] < axes. */
+  const double* turns; const int32_t* axis;
+  const void* positions;                          /* (B, n, axes), position_stride in elements, any sign */
+  const int32_t* start;                           /* (B) position of row 0 in its sequence, null = 0     */
+  const int32_t* counts;                          /* (B) rows that are appended, null = n                */
+  const int32_t* page_table;                      /* (B, table_width), unit stride along the pages       */
+  int64_t batch, heads, groups, rows, head_dim, rotary_dim, axes;
+  int64_t pages, page_size, table_width;
+  int64_t q_stride[4]; int64_t k_stride[4]; int64_t v_stride[4];
+  int64_t q_out_stride[4]; int64_t k_out_stride[4]; int64_t v_out_stride[4]; /* cache: page, head, row  */
+  int64_t position_stride[3];
+  int64_t table_stride;
+  int32_t dtype;
+  int32_t position_type;  /* 0: the row's position in its sequence on every axis (append only);
+                             positions of 1: int32, 2: int64, 3: float                        */
+  int32_t interleaved;    /* 0: pair i is columns i and rotary_dim / 2 + i; 1: 2 i and 2 i + 1 */
+  int32_t inverse;        /* 1: by the negative angles (the gradient)                         */
+} rotary_args;
+
+/* q_out, k_out = q, k turned by their positions. */
+INTP_API intp_status rotary_positions(const rotary_args* a, void* stream);
+/* Row i < counts[b] of k, turned, and of v goes to state start[b] + i of sequence b;
+ * rows outside the table or without a page are skipped, every other row of the cache is
+ * left as it was.  q_out = q turned, every row.  rotary_dim 0 turns nothing. */
+INTP_API intp_status paged_cache_append(const rotary_args* a, void* stream);
+
+typedef struct paged_attention_args {
+  const void* q; const void* k; const void* v;    /* (B, H, M, D); the cache's keys and values */
+  void* out;
+  const int32_t* page_table;
+  const int32_t* start;                           /* (B) position of row 0 in its sequence     */
+  const int32_t* counts;                          /* (B) rows that are tokens, null = M        */
+  int64_t batch, heads, groups, queries, head_dim;
+  int64_t pages, page_size, table_width;
+  int64_t q_stride[4]; int64_t k_stride[4]; int64_t v_stride[4]; int64_t out_stride[4];
+  int64_t table_stride;
+  int64_t window, sinks;                          /* window 0: the whole sequence              */
+  float   scale;
+  int32_t dtype;
+} paged_attention_args;
+
+/* Row m of sequence b stands at position start[b] + m and sees the states up to it; with a
+ * window W only those at positions above start[b] + m - W, and the first `sinks`.  Rows from
+ * counts[b] on, and rows that see nothing, give zeros. */
+INTP_API intp_status paged_attention(const paged_attention_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,8 @@ Public operators:
   * ``dense_look_grid_sample`` / ``look_sampling_tables`` (dense_look_grid.py)
   * ``cross_attention`` / ``shared_prefix_attention`` (cross_attention.py)
   * ``StateCache`` / ``cached_cross_attention`` (state_cache.py)
+  * ``rotate_positions`` / ``RotaryAxes`` (rotary.py)
+  * ``PagedCache`` / ``paged_attention`` (paged_cache.py)
 The compute runs in ``_lib/libintp_b200.so`` (built by ``build.py``).
 """
 
@@ -18,6 +20,8 @@ from .dense_look_grid import (dense_look_grid_backward, dense_look_grid_forward,
 from .cross_attention import (cross_attention, cross_attention_backward, cross_attention_forward,
                               shared_prefix_attention)
 from .state_cache import StateCache, cached_cross_attention
+from .rotary import RotaryAxes, rotate_positions
+from .paged_cache import PagedCache, paged_attention
 
 __all__ = [
     "LookSlotFields",
@@ -40,4 +44,8 @@ __all__ = [
     "shared_prefix_attention",
     "StateCache",
     "cached_cross_attention",
+    "RotaryAxes",
+    "rotate_positions",
+    "PagedCache",
+    "paged_attention",
 ]

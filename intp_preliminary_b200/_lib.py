@@ -48,6 +48,9 @@ EXPORTED_SYMBOLS = (
     "xattn_backward",
     "state_cache_write",
     "state_cache_read",
+    "rotary_positions",
+    "paged_cache_append",
+    "paged_attention",
     "intp_set_wait_budget_ns",
     "intp_device_info",
     "intp_abi_version",
@@ -220,6 +223,49 @@ class StateCacheArgs(ctypes.Structure):
     ]
 
 
+ROTARY_ROW, ROTARY_INT32, ROTARY_INT64, ROTARY_FLOAT32 = 0, 1, 2, 3
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``rotary_args`` (include/intp_b200.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp),
+        ("q_out", _vp), ("k_out", _vp), ("v_out", _vp),
+        ("turns", _vp), ("axis", _vp),
+        ("positions", _vp),
+        ("start", _vp), ("counts", _vp), ("page_table", _vp),
+        ("batch", _i64), ("heads", _i64), ("groups", _i64), ("rows", _i64), ("head_dim", _i64), ("rotary_dim", _i64),
+        ("axes", _i64),
+        ("pages", _i64), ("page_size", _i64), ("table_width", _i64),
+        ("q_stride", _Stride), ("k_stride", _Stride), ("v_stride", _Stride),
+        ("q_out_stride", _Stride), ("k_out_stride", _Stride), ("v_out_stride", _Stride),
+        ("position_stride", _i64 * 3),
+        ("table_stride", _i64),
+        ("dtype", _i32),
+        ("position_type", _i32),
+        ("interleaved", _i32),
+        ("inverse", _i32),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """Mirror of ``paged_attention_args`` (include/intp_b200.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp),
+        ("out", _vp),
+        ("page_table", _vp), ("start", _vp), ("counts", _vp),
+        ("batch", _i64), ("heads", _i64), ("groups", _i64), ("queries", _i64), ("head_dim", _i64),
+        ("pages", _i64), ("page_size", _i64), ("table_width", _i64),
+        ("q_stride", _Stride), ("k_stride", _Stride), ("v_stride", _Stride), ("out_stride", _Stride),
+        ("table_stride", _i64),
+        ("window", _i64), ("sinks", _i64),
+        ("scale", ctypes.c_float),
+        ("dtype", _i32),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -288,7 +334,8 @@ def load() -> ctypes.CDLL:
         lib.svit_linear_residual_layernorm.argtypes = [_vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _vp,
                                                        ctypes.c_float, _vp, _i64, _vp, _vp]
         lib.svit_linear_residual_layernorm.restype = _i32
-        for name in ("xattn_forward", "xattn_backward", "state_cache_write", "state_cache_read"):
+        for name in ("xattn_forward", "xattn_backward", "state_cache_write", "state_cache_read", "rotary_positions",
+                     "paged_cache_append", "paged_attention"):
             getattr(lib, name).argtypes = [_vp, _vp]
             getattr(lib, name).restype = _i32
         for name in ("xattn_forward_workspace", "xattn_backward_workspace"):

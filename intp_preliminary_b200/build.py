@@ -26,7 +26,7 @@ LIB_PATH = LIB_DIR / "libintp_b200.so"
 SOURCES = ("capi.cu", "look_attention_simt.cu", "look_attention_tc.cu", "look_attention_short.cu", "negative_l1.cu",
            "noalloc.cu", "share_vit_ops.cu", "backward.cu", "backward_tc.cu", "backward_fused.cu", "gemm_epilogue.cu", "dense_look_grid.cu",
            "cross_attention_capi.cu", "cross_attention_tiles.cu", "cross_attention_rows.cu", "cross_attention_backward.cu",
-           "state_cache.cu")
+           "state_cache.cu", "rotary.cu", "paged_attention.cu")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 

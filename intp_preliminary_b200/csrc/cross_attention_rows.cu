@@ -28,6 +28,7 @@
 // is a hundredth of the codes' own 2^-4, and issue slots, not only memory, bound this form.  A bf16 query row is
 // first scaled by a power of two into the f16 range.
 #include <cstdint>
+#include "row_mma.cuh"
 #include "xattn_common.cuh"
 #include "xattn_internal.h"
 
@@ -50,59 +51,6 @@ struct RowsShape {
   static constexpr int kWarpRing = kStages * 2 * kSliceBytes;
 };
 
-template <int CH>
-__device__ __forceinline__ uint32_t chunk_offset(int row, int c) {
-  const int sw = CH == 4 ? (row >> 1) & 3 : row & 7;
-  return static_cast<uint32_t>(row * CH + (c ^ sw)) * 16;
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-// Transpose of the 8 x 8 16-bit matrix whose row g this lane quad holds.
-__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
-  uint32_t d;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
-  return d;
-}
-// C += A B for 16 rows, 8 columns and a depth of 16.
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  if (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // Four e4m3 codes (low byte first) to two pairs of f16 values, exact.
 __device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
@@ -110,23 +58,6 @@ __device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& h
       : "=r"(lo), "=r"(hi)
       : "r"(codes));
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-// Over the eight lanes that hold a query row's keys.
-__device__ __forceinline__ float keys_max(float v) {
-#pragma unroll
-  for (int s = 4; s < 32; s <<= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, s));
-  return v;
-}
-__device__ __forceinline__ float keys_sum(float v) {
-#pragma unroll
-  for (int s = 4; s < 32; s <<= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-  return v;
-}
-
 struct RowsArgs {
   XaParams p;
   int32_t n_rt;

@@ -59,6 +59,13 @@ __device__ __forceinline__ uint32_t finite2(uint32_t v) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Whether one of the two values is an infinity or NaN.
+template <bool BF16>
+__device__ __forceinline__ bool not_finite2(uint32_t v) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  return (v & kExp) == kExp || (v >> 16 & kExp) == kExp;
+}
+
 // 32 bytes of one thread, a whole memory sector (dst 32-byte aligned).
 __device__ __forceinline__ void store32(void* dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
                                         uint32_t g, uint32_t h) {

@@ -1,0 +1,254 @@
+"""A paged cache of a decoder's own keys and values, and attention over it.
+
+The cache is a pool of pages, each ``page_size`` states of every key head; a page
+table names each sequence's pages, so sequences grow without moving and may share
+pages.  State p of sequence b is row ``p % page_size`` of page
+``page_table[b, p // page_size]``.  Entries that are no page of the pool (-1 for
+instance) hold nothing: rows that belong there are not written and states there
+take no part in the attention.
+
+The cache does not know how many states a sequence has: a program keeps each
+sequence's length and passes it as ``start``, the position of the first new row.
+A step appends its keys and values there and attends from there:
+
+    q = cache.append(k, v, page_table=table, start=length, rotary=rotary, q=q)
+    out = paged_attention(q, cache, page_table=table, start=length, scale=scale)
+
+The operators take no part in autograd.  Every call runs one CUDA kernel of
+``libintp_b200.so`` on the current stream; CPU tensors raise ``ValueError``.
+"""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _lib
+from .cross_attention import (_HALF, _MAX_STRIDE, _call, _check_counts, _check_scale, _keep, _output, _plans, _ready,
+                              _refuse_grad)
+from .look_attention import _DTYPE_CODE
+from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _check_rotary, _rows_laid_out, _rows_ready,
+                     _set_rotary)
+
+_ATTENTION_POINTERS = struct.Struct("7Q")  # paged_attention_args up to the sizes
+_MAX_STATES = 1 << 30
+
+
+def _check_cache(keys, values) -> None:
+    for t in (keys, values):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError("a paged cache requires CUDA tensors")
+    if keys.ndim != 4 or keys.shape != values.shape:
+        raise ValueError("keys and values must share shape (pages, G, page_size, D)")
+    if keys.dtype not in _HALF or values.dtype != keys.dtype:
+        raise ValueError("keys and values must be bfloat16 or float16 and share a dtype")
+    if keys.device != values.device:
+        raise ValueError("all tensors must be on the same CUDA device")
+    if min(keys.shape[:3]) < 1:
+        raise ValueError("a paged cache needs a page, a key head and a state")
+    if keys.shape[3] % 8 or not 8 <= keys.shape[3] <= 128:
+        raise ValueError("head_dim must be a multiple of 8 up to 128")
+    if not (_ready(keys) and _ready(values)):
+        raise ValueError("the cache's tensors need unit stride on head_dim and 16-byte aligned rows")
+
+
+class PagedCache:
+    """``keys`` and ``values`` ``(pages, G, page_size, D)`` bf16 or f16 of the pool's
+    pages, any page size from one up, D a multiple of 8 up to 128.  Outer strides are free
+    (multiples of 16 bytes): a pool laid out ``(pages, page_size, G, D)`` is passed
+    transposed.  The tensors may be written to but not replaced."""
+
+    def __init__(self, keys, values) -> None:
+        _check_cache(keys, values)
+        self._keys, self._values = keys, values
+        # what calls know the pool by
+        self._layout = (keys.shape, keys.stride(), values.stride(), keys.dtype, keys.device)
+
+    # read only: a call takes the layout that was checked above
+    keys = property(lambda self: self._keys)
+    values = property(lambda self: self._values)
+    layout = property(lambda self: self._layout)
+
+    @classmethod
+    def empty(cls, pages: int, groups: int, page_size: int, head_dim: int, *, dtype=torch.bfloat16,
+              device) -> "PagedCache":
+        """A pool of zeros."""
+        return cls(*(torch.zeros(pages, groups, page_size, head_dim, dtype=dtype, device=device) for _ in range(2)))
+
+    @property
+    def device(self) -> torch.device:
+        return self._keys.device
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return tuple(self._keys.shape)
+
+    def _append_tail(self, q, k, v, q_out, page_table, rotary, positions) -> bytes:
+        """Checks an append and returns its argument block behind the pointers."""
+        what = "a paged cache"
+        pages, groups, page_size, head_dim = self._keys.shape
+        for name, t in (("k", k), ("v", v), ("q", q)):
+            if t is None:
+                continue
+            _check_heads(t, name, what, _HALF)
+            if t.dtype != self._keys.dtype or t.device != self._keys.device:
+                raise ValueError(f"{name} must have the cache's dtype and device")
+            if t.shape[0] != k.shape[0] or t.shape[2:] != (k.shape[2], head_dim) or (name != "q" and t.shape[1] != groups):
+                raise ValueError("k and v must have shape (B, G, n, D) and q (B, H, n, D) with the cache's G and D")
+        _check_table(page_table, k.shape[0], page_size, k.device)
+        args = _lib.RotaryArgs()
+        args.batch, args.groups, args.rows, args.head_dim = k.shape
+        args.k_stride, args.v_stride = k.stride(), v.stride()
+        args.k_out_stride, args.v_out_stride = self._keys.stride(), self._values.stride()
+        if q is not None:
+            args.heads = q.shape[1]
+            args.q_stride, args.q_out_stride = q.stride(), q_out.stride()
+        args.pages, args.page_size = pages, page_size
+        args.table_width, args.table_stride = page_table.shape[1], page_table.stride(0)
+        args.dtype = _DTYPE_CODE[k.dtype]
+        if rotary is not None:
+            _check_rotary(rotary, head_dim, k.device)
+            if positions is not None:
+                _check_positions(positions, k.shape[0], k.shape[2], max(rotary.axes) + 1, k.device)
+            _set_rotary(args, rotary, positions)
+        elif q is not None or positions is not None:
+            raise ValueError("q and positions are for a rotation: pass rotary too")
+        return bytes(args)[_POINTERS.size:]
+
+    def append(self, k, v, *, page_table, start, counts=None, rotary=None, positions=None, q=None):
+        """Row i of ``k``, ``v`` ``(B, G, n, D)`` to state ``start[b] + i`` of sequence b for
+        ``i < counts[b]`` (all n without it); rows outside the table or without a page are
+        skipped, and every other row of the pool is left as it was.
+
+        With ``rotary`` (a :class:`~intp_preliminary_b200.RotaryAxes`) the keys are turned
+        on the way, by ``positions`` ``(B, n, axes)`` or ``(n, axes)``, or without them by
+        the state's number on every axis; ``q`` ``(B, H, n, D)`` is turned likewise, every
+        row of it, and returned.  Two rows that go to the same row of the pool leave it
+        unspecified."""
+        for t in (k, v) + (() if q is None else (q,)):
+            if not isinstance(t, torch.Tensor):
+                raise ValueError("a paged cache requires CUDA tensors")
+        if rotary is not None and not isinstance(rotary, RotaryAxes):
+            raise ValueError("rotary must be a RotaryAxes")
+        if positions is not None and not isinstance(positions, torch.Tensor):
+            raise ValueError("positions must be a tensor")
+        _refuse_grad("a paged cache", k, v, q, positions)
+        page_table = _table(page_table)
+        k, v = _rows_laid_out(k), _rows_laid_out(v)
+        q_out = None
+        if q is not None:
+            q = _rows_laid_out(q)
+            q_out = torch.empty_like(q)
+        key = ("append", self._layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+               page_table.shape, page_table.stride(), page_table.device,
+               None if q is None else (q.shape, q.stride(), q.dtype, q.device),
+               None if rotary is None else rotary._layout,
+               None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device))
+        tail = _plans.get(key)
+        if tail is None:
+            tail = self._append_tail(q, k, v, q_out, page_table, rotary, positions)
+            _keep(key, tail)
+        device = self._keys.device
+        start = _check_counts(start, k.shape[0], device, "start")
+        if start is None:
+            raise ValueError("start must be an int32 or int64 tensor of shape (B,)")
+        counts = _check_counts(counts, k.shape[0], device, "counts")
+        block = _POINTERS.pack(0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                               0 if q is None else q_out.data_ptr(), self._keys.data_ptr(), self._values.data_ptr(),
+                               0 if rotary is None else rotary._turns.data_ptr(),
+                               0 if rotary is None else rotary._axis.data_ptr(),
+                               0 if positions is None else positions.data_ptr(), start.data_ptr(),
+                               0 if counts is None else counts.data_ptr(), page_table.data_ptr()) + tail
+        _call(_lib.load().paged_cache_append, block, device.index, "paged cache append")
+        return q_out
+
+
+def _table(page_table) -> torch.Tensor:
+    """The page table as the kernels take it: int32, unit stride along a sequence's pages."""
+    if not isinstance(page_table, torch.Tensor) or page_table.ndim != 2 or page_table.dtype not in (torch.int32, torch.int64):
+        raise ValueError("page_table must be an int32 or int64 tensor of shape (B, width)")
+    if page_table.dtype == torch.int64:
+        page_table = page_table.clamp(-1, 2147483647).to(torch.int32)
+    strides = page_table.stride()
+    if (strides[1] != 1 and page_table.shape[1] > 1) or not 0 <= strides[0] < _MAX_STRIDE:
+        page_table = page_table.contiguous()
+    return page_table
+
+
+def _check_table(page_table, batch: int, page_size: int, device) -> None:
+    if page_table.shape[0] != batch:
+        raise ValueError("page_table must have a row for each sequence")
+    if page_table.shape[1] < 1 or page_table.shape[1] * page_size > _MAX_STATES:
+        raise ValueError("page_table must name at least one page and at most 2^30 states a sequence")
+    if page_table.device != device:
+        raise ValueError("page_table must be on the same CUDA device as q")
+
+
+def _attention_tail(q, cache: PagedCache, page_table, scale, window, sinks, out_stride) -> bytes:
+    what = "paged attention"
+    _check_heads(q, "q", what, _HALF)
+    pages, groups, page_size, head_dim = cache._keys.shape
+    if q.dtype != cache._keys.dtype or q.device != cache._keys.device:
+        raise ValueError("q must have the cache's dtype and device")
+    if q.shape[3] != head_dim:
+        raise ValueError("q and the cache must share head_dim")
+    if q.shape[1] < 1 or q.shape[1] % groups:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    _check_table(page_table, q.shape[0], page_size, q.device)
+    if window is not None and not 1 <= window <= _MAX_STATES:
+        raise ValueError("window must be at least 1 (None: the whole sequence)")
+    if not 0 <= sinks <= _MAX_STATES:
+        raise ValueError("sinks must not be negative")
+    if sinks and window is None:
+        raise ValueError("sinks are the states that stay visible beside a window: pass window too")
+    args = _lib.PagedAttentionArgs()
+    args.batch, args.heads, args.queries, args.head_dim = q.shape
+    args.groups, args.pages, args.page_size = groups, pages, page_size
+    args.q_stride, args.out_stride = q.stride(), out_stride
+    args.k_stride, args.v_stride = cache._keys.stride(), cache._values.stride()
+    args.table_width, args.table_stride = page_table.shape[1], page_table.stride(0)
+    args.window, args.sinks = window or 0, sinks
+    args.scale = _check_scale(scale)
+    args.dtype = _DTYPE_CODE[q.dtype]
+    return bytes(args)[_ATTENTION_POINTERS.size:]
+
+
+def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=None, sinks: int = 0, out=None):
+    """Attention of the new tokens ``q`` ``(B, H, M, D)`` over a :class:`PagedCache`.
+
+    Row m of sequence b stands at position ``start[b] + m`` and sees the states up to
+    and with its own; with ``window`` only the last ``window`` of them, and the
+    sequence's first ``sinks`` states.  Query head h reads key head ``h // (H / G)``.
+    Rows from ``counts[b]`` on (all M count without it) and rows that see nothing give
+    zeros; states that a row does not see take no part whatever they hold.
+
+    Made for few rows: the states are read once for every 16 rows (tokens times
+    ``H / G``) of a key head.  fp32 sums and statistics; the result is rounded once."""
+    what = "paged attention"
+    if not isinstance(cache, PagedCache):
+        raise ValueError("cache must be a PagedCache")
+    if not isinstance(q, torch.Tensor):
+        raise ValueError(f"{what} requires CUDA tensors")
+    _refuse_grad(what, q)
+    page_table = _table(page_table)
+    scale, window, sinks = float(scale), None if window is None else int(window), int(sinks)
+    if not _ready(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = _output(q, out) if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, q.device, page_table.shape, page_table.stride(),
+           page_table.device, scale, window, sinks, out.stride())
+    tail = _plans.get(key)
+    if tail is None:
+        tail = _attention_tail(q, cache, page_table, scale, window, sinks, out.stride())
+        _keep(key, tail)
+    device = q.device
+    start = _check_counts(start, q.shape[0], device, "start")
+    if start is None:
+        raise ValueError("start must be an int32 or int64 tensor of shape (B,)")
+    counts = _check_counts(counts, q.shape[0], device, "counts")
+    block = _ATTENTION_POINTERS.pack(q.data_ptr(), cache._keys.data_ptr(), cache._values.data_ptr(), out.data_ptr(),
+                                     page_table.data_ptr(), start.data_ptr(),
+                                     0 if counts is None else counts.data_ptr()) + tail
+    _call(_lib.load().paged_attention, block, device.index, what)
+    return out

@@ -1,0 +1,98 @@
+"""float64 restatement of a decoder's own tokens: positions that turn pairs of columns, a paged
+cache, attention of new tokens over it, and elementwise error bounds for the kernels.
+
+Where a kernel may round, with u the unit roundoff of the output type (half its eps):
+  turned values: the angle is a 64-bit product (2 roundings of 2^-53 of it, one more here), its
+        reduced part is rounded to 32 bits (2^-24 of pi / 4 at most), sin and cos are within 2 units
+        in the last place (2^-24 each, below 1): 4 * 2^-24 + 3 * 2^-53 |t| of |x1| + |x2|.  Two fp32
+        products and a sum: 2 * 2^-24 more.  The result is rounded once: u |y| (f16: at most 2^-25
+        below its normal range).
+  attention: the bound of a kernel that multiplies each probability as two 16-bit numbers, as
+        oracle.cross_attention's ``two_part`` derives it.
+"""
+
+from __future__ import annotations
+
+import torch
+
+
+def _u(dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+def turn(x, positions, frequencies, axes, *, interleaved=False, inverse=False):
+    """``(y, bound)`` of x (B, heads, n, D) on the CPU; positions (B, n, axes) or (n, axes)."""
+    dtype = x.dtype
+    x = x.detach().cpu().double()
+    positions = positions.detach().cpu().double().expand(x.shape[0], x.shape[2], -1)
+    pairs = len(axes)
+    y, size, angles = x.clone(), x.abs(), torch.zeros_like(x)
+    for i, (f, a) in enumerate(zip(frequencies, axes)):
+        one, two = (2 * i, 2 * i + 1) if interleaved else (i, pairs + i)
+        t = (positions[:, None, :, a] * f) * (-1 if inverse else 1)
+        c, s = torch.cos(t), torch.sin(t)
+        y[..., one] = x[..., one] * c - x[..., two] * s
+        y[..., two] = x[..., two] * c + x[..., one] * s
+        size[..., one] = size[..., two] = x[..., one].abs() + x[..., two].abs()
+        angles[..., one] = angles[..., two] = t.abs()
+    bound = size * (6 * 2.0 ** -24 + 3 * 2.0 ** -53 * angles) + _u(dtype) * y.abs()
+    bound[..., 2 * pairs:] = 0
+    if dtype == torch.float16:
+        bound[..., :2 * pairs] += 2.0 ** -25
+    return y, bound
+
+
+def place(page_table, page_size, pages, sequence, state):
+    """(page, row) of a sequence's state, or None."""
+    if state < 0 or state // page_size >= page_table.shape[1]:
+        return None
+    page = int(page_table[sequence, state // page_size])
+    return (page, state % page_size) if 0 <= page < pages else None
+
+
+def append(keys, values, k, v, *, page_table, start, counts=None):
+    """Writes rows of k, v into (pages, G, S, D) tensors of any dtype, in place, on the CPU."""
+    for b in range(k.shape[0]):
+        for i in range(k.shape[2] if counts is None else min(max(int(counts[b]), 0), k.shape[2])):
+            at = place(page_table, keys.shape[2], keys.shape[0], b, int(start[b]) + i)
+            if at is not None:
+                keys[at[0], :, at[1]] = k[b, :, i].to(keys.dtype)
+                values[at[0], :, at[1]] = v[b, :, i].to(values.dtype)
+
+
+def attend(q, keys, values, *, page_table, start, scale, counts=None, window=None, sinks=0):
+    """``(out, bound)`` in float64 on the CPU."""
+    dtype = q.dtype
+    q, keys, values = (t.detach().cpu().double() for t in (q, keys, values))
+    page_table = page_table.cpu()
+    batch, heads, rows, dim = q.shape
+    groups = keys.shape[1]
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    u = _u(dtype)
+    for b in range(batch):
+        for m in range(rows if counts is None else min(max(int(counts[b]), 0), rows)):
+            at = int(start[b]) + m
+            last = min(at, page_table.shape[1] * keys.shape[2] - 1)
+            states = [j for j in range(last + 1) if window is None or j > at - window or j < sinks]
+            found = [place(page_table, keys.shape[2], keys.shape[0], b, j) for j in states]
+            found = [f for f in found if f is not None]
+            if not found:
+                continue
+            pages, slots = (torch.tensor(x) for x in zip(*found))
+            for h in range(heads):
+                g = h // (heads // groups)
+                kk, vv = keys[pages, g, slots], values[pages, g, slots]
+                s = scale * (kk @ q[b, h, m])
+                if not bool((s != -float("inf")).any()):
+                    continue
+                p = torch.softmax(s, -1)
+                out[b, h, m] = p @ vv
+                # a score of -inf is exact: its probability is zero
+                size = torch.where(s == -float("inf"), torch.zeros_like(s), scale * (kk.abs() @ q[b, h, m].abs()))
+                score = 2.0 ** -23 * ((dim + 8) * size + 4 * s[s != -float("inf")].abs().max())
+                rel = u ** 2 + 2.0 ** -22 * (1 + 64 + len(found) / 16)
+                w = p * (score + rel)
+                bound[b, h, m] = w @ vv.abs() + w.sum() * (p @ vv.abs()) + u * out[b, h, m].abs()
+                if dtype == torch.float16:
+                    bound[b, h, m] += 2.0 ** -25 * (1 + p.max() * vv.abs().sum(0))
+    return out, bound

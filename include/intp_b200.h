@@ -447,12 +447,20 @@ INTP_API intp_status rotary_positions(const rotary_args* a, void* stream);
  * left as it was.  q_out = q turned, every row.  rotary_dim 0 turns nothing. */
 INTP_API intp_status paged_cache_append(const rotary_args* a, void* stream);
 
+/* Kernel selection (paged_attention_args.kernel). */
+#define PAGED_KERNEL_AUTO   0
+#define PAGED_KERNEL_JOINED 1  /* one launch, a cluster of CTAs for each sequence and key head         */
+#define PAGED_KERNEL_PARTS  2  /* equal shares of the whole batch, joined by a second launch; at most
+                                  16 rows (M * H / G) and 1024 sequences                               */
+
 typedef struct paged_attention_args {
   const void* q; const void* k; const void* v;    /* (B, H, M, D); the cache's keys and values */
   void* out;
   const int32_t* page_table;
   const int32_t* start;                           /* (B) position of row 0 in its sequence     */
   const int32_t* counts;                          /* (B) rows that are tokens, null = M        */
+  void* workspace;                                /* 256-byte aligned                          */
+  int64_t workspace_bytes;
   int64_t batch, heads, groups, queries, head_dim;
   int64_t pages, page_size, table_width;
   int64_t q_stride[4]; int64_t k_stride[4]; int64_t v_stride[4]; int64_t out_stride[4];
@@ -460,7 +468,11 @@ typedef struct paged_attention_args {
   int64_t window, sinks;                          /* window 0: the whole sequence              */
   float   scale;
   int32_t dtype;
+  int32_t kernel;
 } paged_attention_args;
+
+/* Bytes of workspace that the call with these arguments needs (pointers may be null). */
+INTP_API intp_status paged_attention_workspace(const paged_attention_args* a, int64_t* bytes);
 
 /* Row m of sequence b stands at position start[b] + m and sees the states up to it; with a
  * window W only those at positions above start[b] + m - W, and the first `sinks`.  Rows from

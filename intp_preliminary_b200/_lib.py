@@ -50,6 +50,7 @@ EXPORTED_SYMBOLS = (
     "state_cache_read",
     "rotary_positions",
     "paged_cache_append",
+    "paged_attention_workspace",
     "paged_attention",
     "intp_set_wait_budget_ns",
     "intp_device_info",
@@ -223,6 +224,7 @@ class StateCacheArgs(ctypes.Structure):
     ]
 
 
+PAGED_KERNEL_AUTO, PAGED_KERNEL_JOINED, PAGED_KERNEL_PARTS = 0, 1, 2
 ROTARY_ROW, ROTARY_INT32, ROTARY_INT64, ROTARY_FLOAT32 = 0, 1, 2, 3
 
 
@@ -256,6 +258,8 @@ class PagedAttentionArgs(ctypes.Structure):
         ("q", _vp), ("k", _vp), ("v", _vp),
         ("out", _vp),
         ("page_table", _vp), ("start", _vp), ("counts", _vp),
+        ("workspace", _vp),
+        ("workspace_bytes", _i64),
         ("batch", _i64), ("heads", _i64), ("groups", _i64), ("queries", _i64), ("head_dim", _i64),
         ("pages", _i64), ("page_size", _i64), ("table_width", _i64),
         ("q_stride", _Stride), ("k_stride", _Stride), ("v_stride", _Stride), ("out_stride", _Stride),
@@ -263,6 +267,7 @@ class PagedAttentionArgs(ctypes.Structure):
         ("window", _i64), ("sinks", _i64),
         ("scale", ctypes.c_float),
         ("dtype", _i32),
+        ("kernel", _i32),
     ]
 
 
@@ -338,7 +343,7 @@ def load() -> ctypes.CDLL:
                      "paged_cache_append", "paged_attention"):
             getattr(lib, name).argtypes = [_vp, _vp]
             getattr(lib, name).restype = _i32
-        for name in ("xattn_forward_workspace", "xattn_backward_workspace"):
+        for name in ("xattn_forward_workspace", "xattn_backward_workspace", "paged_attention_workspace"):
             getattr(lib, name).argtypes = [_vp, ctypes.POINTER(_i64)]
             getattr(lib, name).restype = _i32
         lib.intp_abi_version.argtypes = []

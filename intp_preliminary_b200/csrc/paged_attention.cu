@@ -47,6 +47,19 @@ struct PagedParams {
   const int32_t* start; const int32_t* counts;
 };
 
+// A call in parts: every warp of the GPU takes the same number of slices of the batch, laid end to
+// end (sequence, key head, slice), whatever the sequences' lengths; a part is what one warp has of
+// one item (sequence and key head), in slot warp + item, which no two parts share.
+struct Parts {
+  float* o;                                // [slot][tile row][D], not normalised
+  float2* ml;                              // [slot][tile row]: reference (log2 units) and sum
+  int32_t* plan;                           // [batch + 1] slices of one key head before each sequence; then slices a warp
+};
+constexpr int kPartsCtas = 296, kPartsWarps = 4;          // two CTAs an SM
+constexpr int kPartsAll = kPartsCtas * kPartsWarps;
+constexpr int kPartsBatch = 1024;          // sequences whose prefix sums fit beside the rings
+constexpr int kPartsLeast = 2;             // slices of a part at least
+
 template <int DP>
 struct Shape {
   static constexpr int kChunks = DP * 2 / 16;
@@ -84,135 +97,122 @@ __device__ __forceinline__ View tile_view(const PagedParams& p, int32_t b, int32
   return x;
 }
 
-// NT: tiles of 8 query rows.  kWarps warps a CTA, a cluster of any size.
-template <int DP, bool BF16, int NT, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32)
-paged_attention_kernel(const PagedParams p) {
-  namespace cg = cooperative_groups;
+// The slices of one warp, `stride` slices apart within an item, copied into its ring in turn.
+template <int DP>
+struct Feed {
   using L = Shape<DP>;
-  constexpr int CH = L::kChunks, NS = L::kStages;
-  constexpr int kTile = 8 * NT;
-  constexpr int kJoinStride = DP + 4;       // floats
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float m_s[kWarps][kTile], l_s[kWarps][kTile];
-  __shared__ float top_s[kTile], total_s[kTile];
-  __shared__ uint32_t seen_s[kWarps][NS];   // which keys of a ring's slice are read
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int32_t n_ranks = static_cast<int32_t>(cluster.num_blocks()), rank = static_cast<int32_t>(cluster.block_rank());
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;    // fragment row and column pair
+  static constexpr int CH = L::kChunks, NS = L::kStages;
+  const PagedParams& p;
+  uint32_t ring;
+  uint32_t* seen_s;                         // [NS]: which keys of a ring's slice are read
+  int lane, cr, cc;                         // this lane copies chunk cc of rows cr, cr + 32 / CH, ...
+  bool chunk_read, chunk_used;
+  // The item: lanes 0-15 look up a slice's keys for K, 16-31 for V.
+  const int32_t* table;
+  const uint8_t* base;
+  int64_t page_bytes, row_bytes;
+  int32_t next_page, next_row;
+  int32_t issued;
 
-  const int32_t item = blockIdx.x / n_ranks;
-  const int32_t bg = item / p.n_rt, rt = item - bg * p.n_rt;
-  const int32_t b = bg / p.groups, grp = bg - b * p.groups;
-  const int32_t D = p.head_dim;
-  const View view = tile_view<kTile>(p, b, rt);
-  // This CTA's share of the slices; warps take them in turn.
-  const int32_t s0 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * rank / n_ranks);
-  const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * (rank + 1) / n_ranks);
-  const int32_t mine = s1 - s0 > warp ? (s1 - s0 - warp + kWarps - 1) / kWarps : 0;
-  const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-
-  // Lanes 0-15 look up the slice's keys for K, 16-31 for V.
-  const int32_t* table = p.table + b * p.table_stride;
-  const bool for_v = lane >= 16;
-  const uint8_t* base = static_cast<const uint8_t*>(for_v ? p.v : p.k) + grp * (for_v ? p.vs[1] : p.ks[1]) * 2;
-  const int64_t page_bytes = (for_v ? p.vs[0] : p.ks[0]) * 2, row_bytes = (for_v ? p.vs[2] : p.ks[2]) * 2;
-  int32_t looked = 0, next_page = -1, next_row = 0;
-  auto look_up = [&]() {                    // the next slice's pages: used a step later
+  __device__ __forceinline__ Feed(const PagedParams& params, uint32_t ring_at, uint32_t* seen) : p(params), ring(ring_at), seen_s(seen) {
+    lane = threadIdx.x & 31;
+    cr = lane / CH;
+    cc = lane % CH;
+    chunk_read = cc * 8 < p.head_dim;
+    chunk_used = cc * 8 < ((p.head_dim + 15) & ~15);  // columns past D that the products read are zero
+    page_bytes = (lane >= 16 ? p.vs[0] : p.ks[0]) * 2;
+    row_bytes = (lane >= 16 ? p.vs[2] : p.ks[2]) * 2;
     next_page = -1;
-    if (looked < mine) {
-      const int32_t key = view.slice(s0 + looked * kWarps + warp) * kStep + (lane & 15);
-      if (key < view.end && (key >= view.low || key < view.sink_end)) {
-        const uint32_t index = static_cast<uint32_t>(key) / static_cast<uint32_t>(p.page_size);
-        next_page = __ldg(table + index);
-        next_row = key - static_cast<int32_t>(index) * p.page_size;
-      }
+    next_row = 0;
+    issued = 0;
+  }
+  __device__ __forceinline__ void enter(int32_t b, int32_t grp) {
+    table = p.table + b * p.table_stride;
+    base = static_cast<const uint8_t*>(lane >= 16 ? p.v : p.k) + grp * (lane >= 16 ? p.vs[1] : p.ks[1]) * 2;
+  }
+  // A slice's pages: used a step later.
+  __device__ __forceinline__ void look_up(const View& view, int32_t slice) {
+    const int32_t key = view.slice(slice) * kStep + (lane & 15);
+    next_page = -1;
+    if (key < view.end && (key >= view.low || key < view.sink_end)) {
+      const uint32_t index = static_cast<uint32_t>(key) / static_cast<uint32_t>(p.page_size);
+      next_page = __ldg(table + index);
+      next_row = key - static_cast<int32_t>(index) * p.page_size;
     }
-    ++looked;
-  };
-  const int cr = lane / CH, cc = lane % CH; // this lane copies chunk cc of rows cr, cr + 32 / CH, ...
-  const bool chunk_read = cc * 8 < D;
-  const bool chunk_used = cc * 8 < ((D + 15) & ~15);  // columns past D that the products read are zero
-  int32_t issued = 0;
-  auto issue = [&]() {
-    if (issued < mine) {
-      const bool there = next_page >= 0 && next_page < p.pages;
-      const uint8_t* row = base + (there ? next_page * page_bytes + next_row * row_bytes : 0);
-      const uint32_t seen = __ballot_sync(0xffffffffu, there) & 0xffffu;
-      const int slot = issued % NS;
-      if (lane == 0) seen_s[warp][slot] = seen;
-      const uint32_t dst = ring + slot * 2 * L::kSliceBytes;
-      const uint64_t bits = reinterpret_cast<uint64_t>(row);
-      look_up();
+  }
+  // The rows that were looked up; returns this lane's row, before the next look-up may change the item.
+  __device__ __forceinline__ uint64_t found(uint32_t& seen) const {
+    const bool there = next_page >= 0 && next_page < p.pages;
+    seen = __ballot_sync(0xffffffffu, there) & 0xffffu;
+    return reinterpret_cast<uint64_t>(base + (there ? next_page * page_bytes + next_row * row_bytes : 0));
+  }
+  __device__ __forceinline__ void copy(uint64_t row, uint32_t seen) {
+    const int slot = issued % NS;
+    if (lane == 0) seen_s[slot] = seen;
+    const uint32_t dst = ring + slot * 2 * L::kSliceBytes;
 #pragma unroll
-      for (int u = 0; u < kStep * CH / 32; ++u) {
-        const int r = cr + u * (32 / CH);
-        const uint64_t ks = __shfl_sync(0xffffffffu, bits, r), vs = __shfl_sync(0xffffffffu, bits, 16 + r);
-        const bool read = chunk_read && (seen >> r & 1u);
-        const uint32_t to = dst + chunk_offset<CH>(r, cc);
-        if (chunk_used) {
-          cp_async16(to, read ? reinterpret_cast<const uint8_t*>(ks) + cc * 16 : static_cast<const uint8_t*>(p.q), read);
-          cp_async16(to + L::kSliceBytes, read ? reinterpret_cast<const uint8_t*>(vs) + cc * 16 : static_cast<const uint8_t*>(p.q),
-                     read);
-        }
+    for (int u = 0; u < kStep * CH / 32; ++u) {
+      const int r = cr + u * (32 / CH);
+      const uint64_t ks = __shfl_sync(0xffffffffu, row, r), vs = __shfl_sync(0xffffffffu, row, 16 + r);
+      const bool read = chunk_read && (seen >> r & 1u);
+      const uint32_t to = dst + chunk_offset<CH>(r, cc);
+      if (chunk_used) {
+        const uint8_t* none = static_cast<const uint8_t*>(p.q);
+        cp_async16(to, read ? reinterpret_cast<const uint8_t*>(ks) + cc * 16 : none, read);
+        cp_async16(to + L::kSliceBytes, read ? reinterpret_cast<const uint8_t*>(vs) + cc * 16 : none, read);
       }
     }
+  }
+  __device__ __forceinline__ void commit() {
     ++issued;
     cp_async_commit();
-  };
-  look_up();
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i) issue();
-
-  // Query fragments (rows 8 n + g as columns of q^T) and the positions of rows 8 n + 2 t, + 1.
-  const int32_t row0 = rt * kTile;
-  const int32_t n_rows = min(p.rows - row0, kTile);
-  uint32_t qb[NT][DP / 16][2];
-  int32_t pos[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int32_t r = row0 + 8 * n + g;
-    const uint16_t* src = nullptr;
-    if (r < p.rows) {
-      const int32_t m = r / p.per_group, h = grp * p.per_group + (r - m * p.per_group);
-      src = static_cast<const uint16_t*>(p.q) + b * p.qs[0] + h * p.qs[1] + m * p.qs[2];
-    }
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      const int d0 = kk * 16 + 2 * t, d1 = d0 + 8;
-      qb[n][kk][0] = src != nullptr && d0 < D ? *reinterpret_cast<const uint32_t*>(src + d0) : 0u;
-      qb[n][kk][1] = src != nullptr && d1 < D ? *reinterpret_cast<const uint32_t*>(src + d1) : 0u;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      pos[n][h] = view.first_pos + (row0 + 8 * n + 2 * t + h) / p.per_group - row0 / p.per_group;
   }
-  const float score_scale = p.scale * kLog2e;
+};
 
+// What a warp holds of a tile of rows: the queries, and the sums over the slices so far.
+template <int DP, bool BF16, int NT>
+struct Rows {
+  static constexpr int CH = Shape<DP>::kChunks;
+  uint32_t qb[NT][DP / 16][2];              // rows 8 n + g as columns of q^T
+  int32_t pos[NT][2];                       // positions of rows 8 n + 2 t, + 1
   float o[NT][DP / 16][4];
   float m[NT][2], l[NT][2];                 // rows 8 n + 2 t + h: running reference, this lane's part of the sum
+
+  __device__ __forceinline__ void enter(const PagedParams& p, const View& view, int32_t b, int32_t grp, int32_t row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
+      const int32_t r = row0 + 8 * n + g;
+      const uint16_t* src = nullptr;
+      if (r < p.rows) {
+        const int32_t tok = r / p.per_group, h = grp * p.per_group + (r - tok * p.per_group);
+        src = static_cast<const uint16_t*>(p.q) + b * p.qs[0] + h * p.qs[1] + tok * p.qs[2];
+      }
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const int d0 = kk * 16 + 2 * t, d1 = d0 + 8;
+        qb[n][kk][0] = src != nullptr && d0 < p.head_dim ? *reinterpret_cast<const uint32_t*>(src + d0) : 0u;
+        qb[n][kk][1] = src != nullptr && d1 < p.head_dim ? *reinterpret_cast<const uint32_t*>(src + d1) : 0u;
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][c][e] = 0.f;
+      for (int h = 0; h < 2; ++h) {
+        pos[n][h] = view.first_pos + (row0 + 8 * n + 2 * t + h) / p.per_group - row0 / p.per_group;
+        m[n][h] = -INFINITY;
+        l[n][h] = 0.f;
+      }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      m[n][h] = -INFINITY;
-      l[n][h] = 0.f;
+      for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][c][e] = 0.f;
     }
   }
-  const int mi = lane >> 3, mr = lane & 7;
-  const bool one_token = view.first_pos == view.last_pos;
 
-  for (int32_t i = 0; i < mine; ++i) {
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    const uint32_t k_s = ring + (i % NS) * 2 * L::kSliceBytes, v_s = k_s + L::kSliceBytes;
-    const uint32_t seen = seen_s[warp][i % NS];
-    const int32_t k0 = view.slice(s0 + i * kWarps + warp) * kStep;
+  // One slice, keys k0 .. k0 + 15, of which the bits of `seen` are there.
+  __device__ __forceinline__ void step(const PagedParams& p, const View& view, uint32_t k_s, int32_t k0, uint32_t seen) {
+    const uint32_t v_s = k_s + Shape<DP>::kSliceBytes;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mi = lane >> 3, mr = lane & 7;
+    const int D = p.head_dim;
+    const float score_scale = p.scale * kLog2e;
     float s[NT][4];                         // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -227,7 +227,7 @@ paged_attention_kernel(const PagedParams p) {
       for (int n = 0; n < NT; ++n) mma16816<BF16>(s[n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
     }
     // Whether rows of the tile differ in what they see of the slice.
-    const bool mixed = !one_token && (k0 + kStep - 1 > view.first_pos ||
+    const bool mixed = view.first_pos != view.last_pos && (k0 + kStep - 1 > view.first_pos ||
                                       (p.window > 0 && k0 <= view.last_pos - p.window && k0 + kStep > p.sinks));
     bool grow = false;
 #pragma unroll
@@ -348,6 +348,59 @@ paged_attention_kernel(const PagedParams p) {
         }
       }
     }
+  }
+};
+
+// NT: tiles of 8 query rows.  kWarps warps a CTA, the CTAs of an item a cluster of any size.
+template <int DP, bool BF16, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32)
+paged_joined_kernel(const PagedParams p) {
+  namespace cg = cooperative_groups;
+  using L = Shape<DP>;
+  constexpr int NS = L::kStages;
+  constexpr int kTile = 8 * NT;
+  constexpr int kJoinStride = DP + 4;       // floats
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float m_s[kWarps][kTile], l_s[kWarps][kTile];
+  __shared__ float top_s[kTile], total_s[kTile];
+  __shared__ uint32_t seen_s[kWarps][NS];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int32_t n_ranks = static_cast<int32_t>(cluster.num_blocks()), rank = static_cast<int32_t>(cluster.block_rank());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;    // fragment row and column pair
+
+  const int32_t item = blockIdx.x / n_ranks;
+  const int32_t bg = item / p.n_rt, rt = item - bg * p.n_rt;
+  const int32_t b = bg / p.groups, grp = bg - b * p.groups;
+  const int32_t D = p.head_dim;
+  const View view = tile_view<kTile>(p, b, rt);
+  // This CTA's share of the slices; warps take them in turn.
+  const int32_t s0 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * rank / n_ranks) + warp;
+  const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * (rank + 1) / n_ranks);
+  const int32_t mine = s1 > s0 ? (s1 - s0 + kWarps - 1) / kWarps : 0;
+  const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
+  Feed<DP> feed(p, ring, seen_s[warp]);
+  feed.enter(b, grp);
+  auto issue = [&]() {
+    if (feed.issued < mine) {
+      uint32_t seen;
+      const uint64_t row = feed.found(seen);
+      if (feed.issued + 1 < mine) feed.look_up(view, s0 + (feed.issued + 1) * kWarps);
+      feed.copy(row, seen);
+    }
+    feed.commit();
+  };
+  if (mine > 0) feed.look_up(view, s0);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) issue();
+  const int32_t row0 = rt * kTile;
+  const int32_t n_rows = min(p.rows - row0, kTile);
+  Rows<DP, BF16, NT> rows;
+  rows.enter(p, view, b, grp, row0);
+  for (int32_t i = 0; i < mine; ++i) {
+    cp_async_wait<NS - 2>();
+    __syncwarp();
+    rows.step(p, view, ring + (i % NS) * 2 * L::kSliceBytes, view.slice(s0 + i * kWarps) * kStep, seen_s[warp][i % NS]);
     __syncwarp();
     issue();
   }
@@ -360,17 +413,17 @@ paged_attention_kernel(const PagedParams p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = 8 * n + 2 * t + h;
-      const float sum = keys_sum(l[n][h]);
+      const float sum = keys_sum(rows.l[n][h]);
       if (g == 0) {
-        m_s[warp][r] = m[n][h];
+        m_s[warp][r] = rows.m[n][h];
         l_s[warp][r] = sum;
       }
       if (r < n_rows && mine > 0) {
         float* dst = join + (warp * kTile + r) * kJoinStride;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
-          dst[c * 16 + g] = o[n][c][h];
-          dst[c * 16 + 8 + g] = o[n][c][2 + h];
+          dst[c * 16 + g] = rows.o[n][c][h];
+          dst[c * 16 + 8 + g] = rows.o[n][c][2 + h];
         }
       }
     }
@@ -437,6 +490,205 @@ paged_attention_kernel(const PagedParams p) {
   cluster.sync();  // nobody leaves while others read its sums
 }
 
+// Every warp on its own: kWarps warps a CTA, one wave of CTAs.
+template <int DP, bool BF16, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32)
+paged_parts_kernel(const PagedParams p, const Parts parts) {
+  using L = Shape<DP>;
+  constexpr int NS = L::kStages, kTile = 8 * NT, kThreads = kWarps * 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t seen_s[kWarps][NS];
+  __shared__ int32_t sum_s[kWarps];
+  int32_t* before = reinterpret_cast<int32_t*>(smem + kWarps * L::kWarpRing);  // [batch + 1]
+  allow_next_kernel();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Prefix sums of the sequences' slices: a run of sequences a thread, the runs' sums across the CTA.
+  const int32_t run = (p.batch + kThreads - 1) / kThreads, first = threadIdx.x * run;
+  int32_t sum = 0;
+  for (int32_t b = first; b < min(first + run, p.batch); ++b) {
+    before[b] = sum;
+    sum += tile_view<kTile>(p, b, 0).n_slices;
+  }
+  int32_t scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int32_t x = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += x;
+  }
+  if (lane == 31) sum_s[warp] = scan;
+  __syncthreads();
+  int32_t base = scan - sum, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) base += sum_s[w];
+    all += sum_s[w];
+  }
+  for (int32_t b = first; b < min(first + run, p.batch); ++b) before[b] += base;
+  if (threadIdx.x == 0) before[p.batch] = all;
+  __syncthreads();
+  const int32_t total = all * p.groups;
+  const int32_t per = max((total + kPartsAll - 1) / kPartsAll, kPartsLeast);
+  if (blockIdx.x == 0) {
+    for (int32_t b = threadIdx.x; b <= p.batch; b += kThreads) parts.plan[b] = before[b];
+    if (threadIdx.x == 0) parts.plan[p.batch + 1] = per;
+  }
+  // Consecutive warps' parts on different SMs, so that few parts find many.
+  const int32_t me = warp * kPartsCtas + blockIdx.x;
+  if (static_cast<int64_t>(me) * per >= total) return;
+  const int32_t f0 = me * per, mine = min(per, total - f0);
+  int32_t lo = 0, hi = p.batch;             // the last sequence that starts at f0 or before
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (before[mid] * p.groups <= f0) lo = mid; else hi = mid;
+  }
+  struct Cursor {
+    int32_t b, grp, slice, n;
+  };
+  Cursor out;
+  out.b = lo;
+  out.n = before[lo + 1] - before[lo];
+  const int32_t rest = f0 - before[lo] * p.groups;
+  out.grp = rest / out.n;
+  out.slice = rest - out.grp * out.n;
+  Cursor in = out;
+  View view = tile_view<kTile>(p, in.b, 0), view_in = view;
+  // To the next slice; true where that is another item's.
+  auto advance = [&](Cursor& c, View& v) {
+    if (++c.slice < c.n) return false;
+    c.slice = 0;
+    if (++c.grp == p.groups) {
+      c.grp = 0;
+      do {
+        ++c.b;
+        c.n = before[c.b + 1] - before[c.b];
+      } while (c.n == 0);
+      v = tile_view<kTile>(p, c.b, 0);
+    }
+    return true;
+  };
+  const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
+  Feed<DP> feed(p, ring, seen_s[warp]);
+  feed.enter(in.b, in.grp);
+  auto issue = [&]() {
+    if (feed.issued < mine) {
+      uint32_t seen;
+      const uint64_t row = feed.found(seen);
+      if (feed.issued + 1 < mine) {
+        if (advance(in, view_in)) feed.enter(in.b, in.grp);
+        feed.look_up(view_in, in.slice);
+      }
+      feed.copy(row, seen);
+    }
+    feed.commit();
+  };
+  feed.look_up(view_in, in.slice);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) issue();
+  Rows<DP, BF16, NT> rows;
+  rows.enter(p, view, out.b, out.grp, 0);
+  const int g = lane >> 2, t = lane & 3;
+  for (int32_t i = 0; i < mine; ++i) {
+    cp_async_wait<NS - 2>();
+    __syncwarp();
+    rows.step(p, view, ring + (i % NS) * 2 * L::kSliceBytes, view.slice(out.slice) * kStep, seen_s[warp][i % NS]);
+    __syncwarp();
+    issue();
+    if (i + 1 < mine && out.slice + 1 < out.n) {
+      ++out.slice;
+      continue;
+    }
+    const int64_t slot = static_cast<int64_t>(me) + out.b * p.groups + out.grp;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 8 * n + 2 * t + h;
+        const float part = keys_sum(rows.l[n][h]);
+        if (r >= p.rows) continue;
+        if (g == 0) parts.ml[slot * kTile + r] = make_float2(rows.m[n][h], part);
+        float* dst = parts.o + (slot * kTile + r) * p.head_dim;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+          if (c * 16 + g < p.head_dim) dst[c * 16 + g] = rows.o[n][c][h];
+          if (c * 16 + 8 + g < p.head_dim) dst[c * 16 + 8 + g] = rows.o[n][c][2 + h];
+        }
+      }
+    if (i + 1 < mine) {
+      advance(out, view);
+      rows.enter(p, view, out.b, out.grp, 0);
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the parts of each row, WPR warps a row: warp i takes parts i, i + WPR, .. in order, the
+// warps are joined in order.  Lane l holds the weight of its warp's l-th part, so that the parts'
+// values are loaded without waiting for one another.
+template <bool BF16, int WPR>
+__global__ void __launch_bounds__(128)
+paged_combine_kernel(const PagedParams p, const Parts parts, int32_t tile) {
+  __shared__ float4 acc_s[WPR][32];
+  __shared__ float total_s[WPR];
+  wait_previous_kernel();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = WPR > 1 ? warp : 0;
+  const int64_t lin = WPR > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + warp;  // (sequence, head, token)
+  if (lin >= static_cast<int64_t>(p.batch) * p.heads * p.queries) return;
+  const int32_t tok = static_cast<int32_t>(lin % p.queries), bh = static_cast<int32_t>(lin / p.queries);
+  const int32_t b = bh / p.heads, h = bh - b * p.heads;
+  const int32_t grp = h / p.per_group, item = b * p.groups + grp, row = tok * p.per_group + h - grp * p.per_group;
+  const int32_t before = __ldcg(parts.plan + b), n = __ldcg(parts.plan + b + 1) - before, per = __ldcg(parts.plan + p.batch + 1);
+  const bool counts = n > 0 && (p.counts == nullptr || tok < p.counts[b]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+  const int d = lane * 4;
+  if (counts) {
+    const int32_t f0 = before * p.groups + grp * n, w0 = f0 / per, n_parts = (f0 + n - 1) / per - w0 + 1;
+    const int64_t first = (static_cast<int64_t>(w0) + item) * tile + row;
+    float top = -INFINITY;
+    for (int32_t s = lane; s < n_parts; s += 32) top = max_nan(top, __ldcg(&parts.ml[first + static_cast<int64_t>(s) * tile]).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int32_t s0 = mine; s0 < n_parts; s0 += 32 * WPR) {
+      float weight = 0.f, part = 0.f;
+      if (s0 + lane * WPR < n_parts) {
+        const float2 e = __ldcg(&parts.ml[first + static_cast<int64_t>(s0 + lane * WPR) * tile]);
+        weight = e.x == -INFINITY ? 0.f : fast_exp2(e.x - top);
+        part = e.x == -INFINITY ? 0.f : e.y * weight;
+      }
+      const int32_t left = (n_parts - s0 + WPR - 1) / WPR, m = left < 32 ? left : 32;
+      const float* src = parts.o + (first + static_cast<int64_t>(s0) * tile) * p.head_dim + d;
+#pragma unroll 8
+      for (int s = 0; s < m; ++s) {
+        const float w = __shfl_sync(0xffffffffu, weight, s);
+        total += __shfl_sync(0xffffffffu, part, s);
+        if (w != 0.f && d < p.head_dim) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * WPR * tile * p.head_dim));
+          acc.x = fmaf(v.x, w, acc.x);
+          acc.y = fmaf(v.y, w, acc.y);
+          acc.z = fmaf(v.z, w, acc.z);
+          acc.w = fmaf(v.w, w, acc.w);
+        }
+      }
+    }
+  }
+  if (WPR > 1) {
+    acc_s[mine][lane] = acc;
+    if (lane == 0) total_s[mine] = total;
+    __syncthreads();
+    if (mine > 0) return;
+#pragma unroll
+    for (int i = 1; i < WPR; ++i) {
+      const float4 v = acc_s[i][lane];
+      acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+      total += total_s[i];
+    }
+  }
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+  if (d < p.head_dim)
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + b * p.os[0] + h * p.os[1] + tok * p.os[2] + d) =
+        make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+}
+
 constexpr int64_t kPlanSms = 148;
 constexpr int64_t kMaxSize = int64_t(1) << 30;
 
@@ -451,10 +703,43 @@ void take(int64_t* dst, const int64_t* src, const int64_t* extent) {
   for (int d = 0; d < 3; ++d) dst[d] = extent[d] > 1 ? src[d] : 0;
 }
 
-template <int DP, bool BF16, int NT, int W>
-int32_t launch(PagedParams p, cudaStream_t stream) {
+// Rows of a tile: 8 where they hold all.
+int tile_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
+
+struct Plan {
+  bool parts;
+  int64_t o_bytes, ml_bytes, bytes;        // of the workspace
+};
+
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Largest number of states that a row can see, from what the host knows.
+int64_t most_states(const paged_attention_args* a) {
+  const int64_t capacity = a->table_width * a->page_size;
+  return a->window > 0 ? std::min(capacity, a->window + a->sinks + a->queries) : capacity;
+}
+
+Plan plan(const paged_attention_args* a) {
+  Plan x{};
+  const int64_t rows = a->heads / a->groups * a->queries, items = a->batch * a->groups;
+  const int64_t slices = most_states(a) / kStep + 3;
+  // One tile a key head, prefix sums that fit, 32-bit slice numbers.
+  const bool able = rows <= 16 && a->batch <= kPartsBatch && items * slices <= INT32_MAX - 2 * kPartsAll;
+  x.parts = able && (a->kernel == PAGED_KERNEL_PARTS || (a->kernel == PAGED_KERNEL_AUTO && items * slices >= kPartsAll * 2));
+  if (x.parts) {
+    const int64_t slots = (kPartsAll + items) * tile_rows(rows);
+    x.o_bytes = align256(slots * a->head_dim * 4);
+    x.ml_bytes = align256(slots * 8);
+    x.bytes = x.o_bytes + x.ml_bytes + align256((a->batch + 2) * 4);
+  }
+  return x;
+}
+
+template <int DP, bool BF16, int NT>
+int32_t launch_joined(PagedParams p, cudaStream_t stream) {
+  constexpr int W = 4;
   using L = Shape<DP>;
-  auto kernel = paged_attention_kernel<DP, BF16, NT, W>;
+  auto kernel = paged_joined_kernel<DP, BF16, NT, W>;
   constexpr int kRing = W * L::kWarpRing, kJoin = W * 8 * NT * (DP + 4) * 4;
   constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
   static_assert(kSmem <= 224 * 1024, "shared memory of a CTA");
@@ -479,13 +764,34 @@ int32_t launch(PagedParams p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? INTP_OK : INTP_ERR_LAUNCH;
 }
 
-template <int DP, bool BF16>
-int32_t launch_rows(const PagedParams& p, cudaStream_t stream) {
-  return p.rows <= 8 ? launch<DP, BF16, 1, 4>(p, stream) : launch<DP, BF16, 2, 4>(p, stream);
+template <int DP, bool BF16, int NT>
+int32_t launch_parts(PagedParams p, const Parts& parts, cudaStream_t stream) {
+  using L = Shape<DP>;
+  auto kernel = paged_parts_kernel<DP, BF16, NT, kPartsWarps>;
+  constexpr int kRing = kPartsWarps * L::kWarpRing, kMost = kRing + (kPartsBatch + 1) * 4;
+  static_assert(kMost <= 112 * 1024, "two CTAs an SM");
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem(kernel, kMost, done)) return INTP_ERR_LAUNCH;
+  p.n_rt = 1;
+  if (!launch_kernel(kernel, dim3(kPartsCtas), kPartsWarps * 32, kRing + (p.batch + 1) * 4, stream, false, p, parts))
+    return INTP_ERR_LAUNCH;
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.queries;
+  // Few items have many parts each: a CTA per row, whose four warps share them.
+  const bool many = static_cast<int64_t>(p.batch) * p.groups * 8 <= kPartsAll;
+  auto combine = many ? paged_combine_kernel<BF16, 4> : paged_combine_kernel<BF16, 1>;
+  const int64_t grid = many ? rows : (rows + 3) / 4;
+  return launch_kernel(combine, dim3(static_cast<unsigned>(grid)), 128, 0, stream, true, p, parts, 8 * NT) ? INTP_OK
+                                                                                                        : INTP_ERR_LAUNCH;
 }
 
-intp_status run(const paged_attention_args* a, cudaStream_t stream) {
-  if (!a) return INTP_ERR_ARGUMENT;
+template <int DP, bool BF16>
+int32_t launch_rows(const PagedParams& p, const Parts* parts, cudaStream_t stream) {
+  if (parts != nullptr)
+    return p.rows <= 8 ? launch_parts<DP, BF16, 1>(p, *parts, stream) : launch_parts<DP, BF16, 2>(p, *parts, stream);
+  return p.rows <= 8 ? launch_joined<DP, BF16, 1>(p, stream) : launch_joined<DP, BF16, 2>(p, stream);
+}
+
+intp_status check_shape(const paged_attention_args* a) {
   for (int64_t n : {a->batch, a->heads, a->groups, a->queries, a->pages, a->page_size, a->table_width})
     if (n < 0 || n > kMaxSize) return INTP_ERR_SHAPE;
   if (a->heads < 1 || a->groups < 1 || a->heads % a->groups) return INTP_ERR_SHAPE;
@@ -497,12 +803,25 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
   if (a->heads / a->groups * std::max<int64_t>(a->queries, 1) > kMaxSize || a->batch * a->groups > kMaxSize) return INTP_ERR_SHAPE;
   if (a->dtype != INTP_F16 && a->dtype != INTP_BF16) return INTP_ERR_DTYPE;
   if (!std::isfinite(a->scale) || !(a->scale > 0.f)) return INTP_ERR_ARGUMENT;
+  if (a->kernel < PAGED_KERNEL_AUTO || a->kernel > PAGED_KERNEL_PARTS) return INTP_ERR_ARGUMENT;
+  if (a->kernel == PAGED_KERNEL_PARTS && a->batch > 0 && a->queries > 0 && !plan(a).parts) return INTP_ERR_UNSUPPORTED;
+  return INTP_OK;
+}
+
+intp_status run(const paged_attention_args* a, cudaStream_t stream) {
+  if (!a) return INTP_ERR_ARGUMENT;
+  const intp_status st = check_shape(a);
+  if (st != INTP_OK) return st;
   if (a->batch == 0 || a->queries == 0) return INTP_OK;
   if (!a->q || !a->k || !a->v || !a->out || !a->page_table || !a->start) return INTP_ERR_ARGUMENT;
   const int64_t eq[3] = {a->batch, a->heads, a->queries}, ek[3] = {a->pages, a->groups, a->page_size};
   if (!rows_ok(a->q, a->q_stride, eq) || !rows_ok(a->out, a->out_stride, eq) || !rows_ok(a->k, a->k_stride, ek) ||
       !rows_ok(a->v, a->v_stride, ek))
     return INTP_ERR_LAYOUT;
+  const Plan how = plan(a);
+  if (how.bytes > 0 &&
+      (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < how.bytes))
+    return INTP_ERR_ARGUMENT;
   int sms = 0;
   const int32_t device = current_device_facts(&sms);
   if (device != INTP_OK) return device;
@@ -533,13 +852,33 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
   p.table_stride = a->table_stride;
   p.start = a->start;
   p.counts = a->counts;
-  if (a->dtype == INTP_BF16) return p.head_dim <= 64 ? launch_rows<64, true>(p, stream) : launch_rows<128, true>(p, stream);
-  return p.head_dim <= 64 ? launch_rows<64, false>(p, stream) : launch_rows<128, false>(p, stream);
+  Parts parts{};
+  if (how.parts) {
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    parts.o = reinterpret_cast<float*>(ws);
+    parts.ml = reinterpret_cast<float2*>(ws + how.o_bytes);
+    parts.plan = reinterpret_cast<int32_t*>(ws + how.o_bytes + how.ml_bytes);
+  }
+  const Parts* x = how.parts ? &parts : nullptr;
+  if (a->dtype == INTP_BF16) return p.head_dim <= 64 ? launch_rows<64, true>(p, x, stream) : launch_rows<128, true>(p, x, stream);
+  return p.head_dim <= 64 ? launch_rows<64, false>(p, x, stream) : launch_rows<128, false>(p, x, stream);
 }
 
 }  // namespace
 }  // namespace intp
 
-extern "C" intp_status paged_attention(const paged_attention_args* a, void* stream) {
+extern "C" {
+
+intp_status paged_attention_workspace(const paged_attention_args* a, int64_t* bytes) {
+  if (!a || !bytes) return INTP_ERR_ARGUMENT;
+  const intp_status st = intp::check_shape(a);
+  if (st != INTP_OK) return st;
+  *bytes = a->batch == 0 || a->queries == 0 ? 0 : intp::plan(a).bytes;
+  return INTP_OK;
+}
+
+intp_status paged_attention(const paged_attention_args* a, void* stream) {
   return intp::run(a, static_cast<cudaStream_t>(stream));
 }
+
+}  // extern "C"

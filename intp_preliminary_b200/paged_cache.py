@@ -26,13 +26,14 @@ import torch
 
 from . import _lib
 from .cross_attention import (_HALF, _MAX_STRIDE, _call, _check_counts, _check_scale, _keep, _output, _plans, _ready,
-                              _refuse_grad)
+                              _refuse_grad, _scratch_bytes)
 from .look_attention import _DTYPE_CODE
 from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _check_rotary, _rows_laid_out, _rows_ready,
                      _set_rotary)
 
-_ATTENTION_POINTERS = struct.Struct("7Q")  # paged_attention_args up to the sizes
+_ATTENTION_POINTERS = struct.Struct("9Q")  # paged_attention_args up to the sizes
 _MAX_STATES = 1 << 30
+_KERNELS = {"auto": _lib.PAGED_KERNEL_AUTO, "joined": _lib.PAGED_KERNEL_JOINED, "parts": _lib.PAGED_KERNEL_PARTS}
 
 
 def _check_cache(keys, values) -> None:
@@ -185,7 +186,8 @@ def _check_table(page_table, batch: int, page_size: int, device) -> None:
         raise ValueError("page_table must be on the same CUDA device as q")
 
 
-def _attention_tail(q, cache: PagedCache, page_table, scale, window, sinks, out_stride) -> bytes:
+def _attention_tail(q, cache: PagedCache, page_table, scale, window, sinks, out_stride, kernel):
+    """Checks a call; its argument block behind the pointers and its scratch bytes."""
     what = "paged attention"
     _check_heads(q, "q", what, _HALF)
     pages, groups, page_size, head_dim = cache._keys.shape
@@ -211,10 +213,15 @@ def _attention_tail(q, cache: PagedCache, page_table, scale, window, sinks, out_
     args.window, args.sinks = window or 0, sinks
     args.scale = _check_scale(scale)
     args.dtype = _DTYPE_CODE[q.dtype]
-    return bytes(args)[_ATTENTION_POINTERS.size:]
+    if kernel not in _KERNELS:
+        raise ValueError(f"kernel must be one of {sorted(_KERNELS)}")
+    args.kernel = _KERNELS[kernel]
+    scratch = _scratch_bytes(_lib.load().paged_attention_workspace, args, what)
+    return bytes(args)[_ATTENTION_POINTERS.size:], scratch
 
 
-def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=None, sinks: int = 0, out=None):
+def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=None, sinks: int = 0,
+                    kernel: str = "auto", out=None):
     """Attention of the new tokens ``q`` ``(B, H, M, D)`` over a :class:`PagedCache`.
 
     Row m of sequence b stands at position ``start[b] + m`` and sees the states up to
@@ -224,7 +231,10 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
     zeros; states that a row does not see take no part whatever they hold.
 
     Made for few rows: the states are read once for every 16 rows (tokens times
-    ``H / G``) of a key head.  fp32 sums and statistics; the result is rounded once."""
+    ``H / G``) of a key head.  fp32 sums and statistics; the result is rounded once.
+    ``kernel``: ``"auto"`` chooses; ``"joined"`` (a cluster of CTAs for each sequence and key
+    head, one launch) and ``"parts"`` (equal shares of the batch's states, joined by a second
+    launch; at most 16 rows) force one of the two."""
     what = "paged attention"
     if not isinstance(cache, PagedCache):
         raise ValueError("cache must be a PagedCache")
@@ -237,18 +247,22 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
         q = q.clone(memory_format=torch.contiguous_format)
     out = _output(q, out) if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, q.device, page_table.shape, page_table.stride(),
-           page_table.device, scale, window, sinks, out.stride())
-    tail = _plans.get(key)
-    if tail is None:
-        tail = _attention_tail(q, cache, page_table, scale, window, sinks, out.stride())
-        _keep(key, tail)
+           page_table.device, scale, window, sinks, out.stride(), kernel)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _attention_tail(q, cache, page_table, scale, window, sinks, out.stride(), kernel))
+    tail, scratch_bytes = plan
     device = q.device
     start = _check_counts(start, q.shape[0], device, "start")
     if start is None:
         raise ValueError("start must be an int32 or int64 tensor of shape (B,)")
     counts = _check_counts(counts, q.shape[0], device, "counts")
+    space = 0
+    if scratch_bytes:
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)  # from the current stream's pool
+        space = scratch.data_ptr()
     block = _ATTENTION_POINTERS.pack(q.data_ptr(), cache._keys.data_ptr(), cache._values.data_ptr(), out.data_ptr(),
-                                     page_table.data_ptr(), start.data_ptr(),
-                                     0 if counts is None else counts.data_ptr()) + tail
+                                     page_table.data_ptr(), start.data_ptr(), 0 if counts is None else counts.data_ptr(),
+                                     space, scratch_bytes) + tail
     _call(_lib.load().paged_attention, block, device.index, what)
     return out

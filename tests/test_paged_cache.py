@@ -115,6 +115,10 @@ def test_append_refuses_before_a_launch(over, status):
     ({"k_stride": _lib._Stride(2048, 1024, 68, 1)}, _lib.INTP_ERR_LAYOUT),
     ({"v_stride": _lib._Stride(2048, 0, 64, 1)}, _lib.INTP_ERR_LAYOUT),
     ({"out_stride": _lib._Stride(768, 192, 64, 2)}, _lib.INTP_ERR_LAYOUT),
+    ({"kernel": 3}, _lib.INTP_ERR_ARGUMENT),
+    ({"kernel": _lib.PAGED_KERNEL_PARTS}, _lib.INTP_ERR_ARGUMENT),              # no workspace
+    ({"kernel": _lib.PAGED_KERNEL_PARTS, "queries": 9}, _lib.INTP_ERR_UNSUPPORTED),
+    ({"kernel": _lib.PAGED_KERNEL_PARTS, "batch": 1025}, _lib.INTP_ERR_UNSUPPORTED),
     ({"batch": 0}, _lib.INTP_OK),
     ({"queries": 0}, _lib.INTP_OK),
 ])

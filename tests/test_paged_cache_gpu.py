@@ -9,6 +9,7 @@ from oracle import paged as oracle
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
+KERNELS = ["joined", "parts"]
 NAN, INF = float("nan"), float("inf")
 
 
@@ -46,8 +47,8 @@ def _attend(device, q, keys, values, table, start, **more):
                            **on)
 
 
-def _check(device, q, keys, values, table, start, **more):
-    got = _attend(device, q, keys, values, table, start, **more).cpu().double()
+def _check(device, q, keys, values, table, start, kernel="auto", **more):
+    got = _attend(device, q, keys, values, table, start, kernel=kernel, **more).cpu().double()
     want, bound = oracle.attend(q, keys, values, page_table=table, start=start, **more)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     wrong = ~(((got - want).abs() <= bound) | torch.isnan(want) | (got == want))
@@ -150,14 +151,16 @@ def test_append_follows_strides(cuda_device):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("heads,groups,dim", [(1, 1, 8), (3, 3, 64), (8, 2, 64), (8, 1, 128), (9, 1, 40), (32, 2, 72), (6, 2, 128)])
 @pytest.mark.parametrize("states,page_size", [(1, 1), (15, 16), (16, 3), (17, 16), (100, 5), (333, 32)])
-def test_token_matches_oracle(cuda_device, dtype, heads, groups, dim, states, page_size):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_token_matches_oracle(cuda_device, dtype, heads, groups, dim, states, page_size, kernel):
     keys, values, table = _filled(2, groups, states, dim, page_size, dtype, 10)
     q = _rand((2, heads, 1, dim), dtype, 20)
-    _check(cuda_device, q, keys, values, table, [states - 1, states // 2], scale=dim ** -0.5)
+    _check(cuda_device, q, keys, values, table, [states - 1, states // 2], kernel=kernel, scale=dim ** -0.5)
 
 
 @pytest.mark.parametrize("batch,groups,states", [(1, 1, 5000), (1, 3, 1201), (5, 2, 700), (40, 1, 257), (75, 2, 64), (150, 1, 130)])
-def test_sequences_of_every_split(cuda_device, batch, groups, states):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_sequences_of_every_split(cuda_device, batch, groups, states, kernel):
     """From one sequence that many CTAs share to more sequences than the GPU holds CTAs; ragged lengths, some of none."""
     keys, values, table = _filled(batch, groups, states, 64, 16, BF16, 30)
     g = torch.Generator().manual_seed(31)
@@ -165,60 +168,69 @@ def test_sequences_of_every_split(cuda_device, batch, groups, states):
     start[0] = states - 1
     if batch > 2:
         start[1], start[2] = -1, 0
-    _check(cuda_device, _rand((batch, 2 * groups, 1, 64), BF16, 32), keys, values, table, start, scale=0.125)
+    _check(cuda_device, _rand((batch, 2 * groups, 1, 64), BF16, 32), keys, values, table, start, kernel=kernel, scale=0.125)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("heads,groups,queries", [(4, 4, 2), (4, 2, 5), (8, 1, 3), (1, 1, 40), (12, 4, 17)])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (5, 0), (7, 3), (40, 20), (1000, 4), (16, 100)])
-def test_tokens_see_what_is_before_them(cuda_device, dtype, heads, groups, queries, window, sinks):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_tokens_see_what_is_before_them(cuda_device, dtype, heads, groups, queries, window, sinks, kernel):
+    if kernel == "parts" and queries * heads // groups > 16:
+        kernel = "auto"  # rows that the parts do not take
     states, page_size = 90, 7
     keys, values, table = _filled(3, groups, states, 32, page_size, dtype, 40)
     q = _rand((3, heads, queries, 32), dtype, 41)
-    _check(cuda_device, q, keys, values, table, [states - queries, 0, -2], scale=0.2, window=window, sinks=sinks)
+    _check(cuda_device, q, keys, values, table, [states - queries, 0, -2], kernel=kernel, scale=0.2, window=window,
+           sinks=sinks)
 
 
 @pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (64, 4), (100, 17), (333, 0), (1024, 1), (2000, 0)])
 @pytest.mark.parametrize("batch,groups", [(1, 1), (30, 2)])
-def test_windows_over_long_sequences(cuda_device, window, sinks, batch, groups):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_windows_over_long_sequences(cuda_device, window, sinks, batch, groups, kernel):
     states = 1500
     keys, values, table = _filled(batch, groups, states, 64, 24, BF16, 50)
     start = [(states - 1) * (i + 1) // batch for i in range(batch)]
-    _check(cuda_device, _rand((batch, 4 * groups, 1, 64), BF16, 51), keys, values, table, start, scale=0.125, window=window,
-           sinks=sinks)
+    _check(cuda_device, _rand((batch, 4 * groups, 1, 64), BF16, 51), keys, values, table, start, kernel=kernel, scale=0.125,
+           window=window, sinks=sinks)
 
 
-def test_rows_past_their_count_are_zero(cuda_device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_rows_past_their_count_are_zero(cuda_device, kernel):
     keys, values, table = _filled(4, 2, 50, 64, 16, BF16, 60)
     q = _rand((4, 4, 6, 64), BF16, 61)
-    got = _check(cuda_device, q, keys, values, table, [40, 40, 40, 40], scale=0.125, counts=[0, 3, 6, -5])
+    got = _check(cuda_device, q, keys, values, table, [40, 40, 40, 40], kernel=kernel, scale=0.125, counts=[0, 3, 6, -5])
     assert bool((got[0] == 0).all()) and bool((got[1, :, 3:] == 0).all()) and bool((got[3] == 0).all())
     assert bool((got[2] != 0).all())
 
 
-def test_start_outside_the_table(cuda_device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_start_outside_the_table(cuda_device, kernel):
     """Positions past the table see all of it, far ones too; positions before the sequence see nothing."""
     keys, values, table = _filled(6, 1, 32, 16, 8, F16, 70)
     start = [31, 32, 100, 2**31 - 1, -1, -2**31]
-    got = _attend(cuda_device, _rand((1, 2, 1, 16), F16, 71).expand(6, -1, -1, -1), keys, values, table, start, scale=0.25)
+    got = _attend(cuda_device, _rand((1, 2, 1, 16), F16, 71).expand(6, -1, -1, -1), keys, values, table, start, scale=0.25,
+                  kernel=kernel)
     q = _rand((1, 2, 1, 16), F16, 71).expand(6, -1, -1, -1)
     want, bound = oracle.attend(q, keys, values, page_table=table, start=[31, 31, 31, 31, -1, -1], scale=0.25)
     assert ((got.cpu().double() - want).abs() <= bound).all()
     assert bool((got[4:] == 0).all())
-    got = _attend(cuda_device, q, keys, values, table, start, scale=0.25, window=4, sinks=2)
+    got = _attend(cuda_device, q, keys, values, table, start, scale=0.25, window=4, sinks=2, kernel=kernel)
     want, bound = oracle.attend(q, keys, values, page_table=table, start=[31, 32, 100, 10**6, -1, -1], scale=0.25, window=4,
                                 sinks=2)
     assert ((got.cpu().double() - want).abs() <= bound).all()
 
 
-def test_pages_that_are_none_take_no_part(cuda_device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_pages_that_are_none_take_no_part(cuda_device, kernel):
     keys, values, table = _filled(4, 2, 60, 32, 5, BF16, 80)
     pages = keys.shape[0]
     table[0, 3], table[1, 0], table[2, 11], table[3, :] = -1, pages, 2**31 - 1, -2**31
     q = _rand((4, 4, 3, 32), BF16, 81)
-    got = _check(cuda_device, q, keys, values, table, [57] * 4, scale=0.2)
+    got = _check(cuda_device, q, keys, values, table, [57] * 4, kernel=kernel, scale=0.2)
     assert bool((got[3] == 0).all())
-    _check(cuda_device, q[:, :, :1], keys, values, table, [59] * 4, scale=0.2, window=30, sinks=6)
+    _check(cuda_device, q[:, :, :1], keys, values, table, [59] * 4, kernel=kernel, scale=0.2, window=30, sinks=6)
 
 
 def test_shared_pages_and_a_broadcast_table(cuda_device):
@@ -234,9 +246,12 @@ def test_shared_pages_and_a_broadcast_table(cuda_device):
 @pytest.mark.parametrize("bad", [NAN, INF, -INF])
 @pytest.mark.parametrize("queries,window", [(4, None), (4, 6), (17, None), (17, 3)])
 @pytest.mark.parametrize("heads", [1, 3])
-def test_states_that_a_row_does_not_see_never_show(cuda_device, bad, queries, window, heads):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_states_that_a_row_does_not_see_never_show(cuda_device, bad, queries, window, heads, kernel):
     """A state that later rows of the same tile see, or that left the window of some, holds what is not finite."""
     states = 50
+    if kernel == "parts" and queries * heads > 16:
+        kernel = "auto"
     for at in (states - 1, states - 2, states - queries + 1, states - queries - 2):
         for which in (0, 1):
             keys, values, table = _filled(1, 1, states, 32, 16, BF16, 100)
@@ -245,8 +260,8 @@ def test_states_that_a_row_does_not_see_never_show(cuda_device, bad, queries, wi
             (keys, values)[which][page, 0, row, 5] = bad
             q = _rand((1, heads, queries, 32), BF16, 101)
             start = [states - queries]
-            got = _attend(cuda_device, q, keys, values, table, start, scale=0.2, window=window).cpu()
-            base = _attend(cuda_device, q, *clean, table, start, scale=0.2, window=window).cpu()
+            got = _attend(cuda_device, q, keys, values, table, start, scale=0.2, window=window, kernel=kernel).cpu()
+            base = _attend(cuda_device, q, *clean, table, start, scale=0.2, window=window, kernel=kernel).cpu()
             for m in range(queries):
                 position = start[0] + m
                 sees = at <= position and (window is None or at > position - window)
@@ -259,7 +274,8 @@ def test_states_that_a_row_does_not_see_never_show(cuda_device, bad, queries, wi
                     assert torch.equal(got[:, :, m][..., other], base[:, :, m][..., other])
 
 
-def test_minus_infinite_scores(cuda_device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_minus_infinite_scores(cuda_device, kernel):
     """A row whose every score is -inf gives zeros; a single one takes no weight."""
     keys, values, table = _filled(2, 1, 20, 16, 4, BF16, 110)
     q = torch.ones(2, 1, 1, 16).bfloat16()
@@ -268,26 +284,28 @@ def test_minus_infinite_scores(cuda_device):
         keys[page, 0, row] = -INF
     page, row = oracle.place(table, 4, keys.shape[0], 1, 3)
     keys[page, 0, row] = -INF
-    got = _check(cuda_device, q, keys, values, table, [19, 19], scale=0.25)
+    got = _check(cuda_device, q, keys, values, table, [19, 19], kernel=kernel, scale=0.25)
     assert bool((got[0] == 0).all())
 
 
-def test_plus_infinite_scores_and_nan_spread(cuda_device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_plus_infinite_scores_and_nan_spread(cuda_device, kernel):
     keys, values, table = _filled(2, 1, 200, 16, 16, BF16, 120)
     q = torch.ones(2, 1, 1, 16).bfloat16()
     page, row = oracle.place(table, 16, keys.shape[0], 0, 100)
     keys[page, 0, row] = INF
-    got = _attend(cuda_device, q, keys, values, table, [199, 199], scale=0.25)
+    got = _attend(cuda_device, q, keys, values, table, [199, 199], scale=0.25, kernel=kernel)
     assert bool(torch.isnan(got[0]).all()) and bool(torch.isfinite(got[1]).all())
     q[1, 0, 0, 3] = NAN
-    got = _attend(cuda_device, q, keys, values, table, [99, 199], scale=0.25)
+    got = _attend(cuda_device, q, keys, values, table, [99, 199], scale=0.25, kernel=kernel)
     assert bool(torch.isnan(got[1]).all()) and bool(torch.isfinite(got[0]).all())
 
 
-def test_scores_of_any_size(cuda_device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_scores_of_any_size(cuda_device, kernel):
     keys, values, table = _filled(1, 1, 300, 64, 16, BF16, 130)
-    _check(cuda_device, _rand((1, 1, 1, 64), BF16, 131, 30.0), keys, values, table, [299], scale=1.0)
-    _check(cuda_device, _rand((1, 1, 1, 64), BF16, 132, 1e-20), keys, values, table, [299], scale=1.0)
+    _check(cuda_device, _rand((1, 1, 1, 64), BF16, 131, 30.0), keys, values, table, [299], kernel=kernel, scale=1.0)
+    _check(cuda_device, _rand((1, 1, 1, 64), BF16, 132, 1e-20), keys, values, table, [299], kernel=kernel, scale=1.0)
 
 
 # ------------------------------------------------------------------ as it is used
@@ -365,6 +383,9 @@ def test_other_streams_strides_and_repeats(cuda_device):
     q = _rand((2, 1, 4, 64), BF16, 161).to(cuda_device).transpose(1, 2)           # token-major rows
     start = torch.tensor([399, 123], device=cuda_device)
     first = paged_attention(q, cache, page_table=table, start=start, scale=0.125)
+    for kernel in KERNELS * 2:
+        again = [paged_attention(q, cache, page_table=table, start=start, scale=0.125, kernel=kernel) for _ in range(3)]
+        assert torch.equal(again[0], again[1]) and torch.equal(again[0], again[2])
     for _ in range(3):
         assert torch.equal(first, paged_attention(q, cache, page_table=table, start=start, scale=0.125))
     stream = torch.cuda.Stream(cuda_device)
@@ -397,10 +418,12 @@ def test_long_cache_past_32_bit_offsets(cuda_device):
     outs = []
     for table in (far, near):
         cache.append(k, v, page_table=table, start=start)
-        outs.append(paged_attention(q, cache, page_table=table, start=start + 699, scale=dim ** -0.5))
-    assert torch.equal(*outs) and torch.equal(cache.keys[pages - 1, :, 3], k[0, :, 3])
+        outs += [paged_attention(q, cache, page_table=table, start=start + 699, scale=dim ** -0.5, kernel=kernel)
+                 for kernel in KERNELS]
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]) and torch.equal(cache.keys[pages - 1, :, 3], k[0, :, 3])
     want = cross_attention(q, k, v, scale=dim ** -0.5)
-    assert bool(((outs[0].float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 1e-5).all())
+    for got in outs[:2]:
+        assert bool(((got.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 1e-5).all())
 
 
 def test_refusals(cuda_device):
@@ -418,7 +441,8 @@ def test_refusals(cuda_device):
             ((q, cache), {"start": None}, "start"), ((q, cache), {"start": start[:1]}, "start"), ((q, cache), {"start": start.float()}, "start"),
             ((q, cache), {"counts": start[:1]}, "counts"), ((q, cache), {"scale": 0.0}, "scale"), ((q, cache), {"window": 0}, "window"),
             ((q, cache), {"sinks": -1, "window": 4}, "sinks"), ((q, cache), {"sinks": 2}, "window"),
-            ((q, cache), {"out": q[..., :8]}, "out"), ((q.clone().requires_grad_(), cache), {}, "no backward")):
+            ((q, cache), {"out": q[..., :8]}, "out"), ((q, cache), {"kernel": "tiles"}, "kernel"),
+            ((torch.zeros(2, 20, 2, 16, dtype=BF16, device=cuda_device), cache), {"kernel": "parts"}, "does not take"), ((q.clone().requires_grad_(), cache), {}, "no backward")):
         with pytest.raises(ValueError, match=message):
             paged_attention(*args, **{**good, **over})
     good = dict(page_table=table, start=start)

@@ -416,6 +416,7 @@ INTP_API intp_status state_cache_read(const state_cache_args* a, void* stream);
  * sequence b is row p % page_size of page page_table[b][p / page_size]; the table
  * holds table_width pages a sequence.  A page number outside 0 .. pages - 1 is no
  * page: rows that belong there are not written, and states there take no part.
+ * paged_attention wants keys and values of the same strides that span at most 64 GB each.
  */
 typedef struct rotary_args {
   const void* q; const void* k; const void* v;    /* absent ones null; v only to append */
@@ -463,7 +464,8 @@ typedef struct paged_attention_args {
   int64_t workspace_bytes;
   int64_t batch, heads, groups, queries, head_dim;
   int64_t pages, page_size, table_width;
-  int64_t q_stride[4]; int64_t k_stride[4]; int64_t v_stride[4]; int64_t out_stride[4];
+  int64_t q_stride[4]; int64_t out_stride[4];
+  int64_t cache_stride[4];                        /* keys and values: page, head, state        */
   int64_t table_stride;
   int64_t window, sinks;                          /* window 0: the whole sequence              */
   float   scale;

@@ -262,7 +262,7 @@ class PagedAttentionArgs(ctypes.Structure):
         ("workspace_bytes", _i64),
         ("batch", _i64), ("heads", _i64), ("groups", _i64), ("queries", _i64), ("head_dim", _i64),
         ("pages", _i64), ("page_size", _i64), ("table_width", _i64),
-        ("q_stride", _Stride), ("k_stride", _Stride), ("v_stride", _Stride), ("out_stride", _Stride),
+        ("q_stride", _Stride), ("out_stride", _Stride), ("cache_stride", _Stride),
         ("table_stride", _i64),
         ("window", _i64), ("sinks", _i64),
         ("scale", ctypes.c_float),

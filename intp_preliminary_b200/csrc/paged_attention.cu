@@ -40,8 +40,10 @@ struct PagedParams {
   int32_t window, sinks;                   // window 0: none
   float scale;
   const void* q; int64_t qs[3];            // sequence, head, token
-  const void* k; int64_t ks[3];            // page, head, state
-  const void* v; int64_t vs[3];
+  const void* k; const void* v;            // of the same strides
+  int64_t head_stride;
+  uint32_t page_units, row_units;          // strides of a page and a state in 16-byte units
+  uint32_t page_magic; int32_t page_shift; // p / page_size = umulhi(4 p, magic) >> shift for p < 2^30
   void* out; int64_t os[3];
   const int32_t* table; int64_t table_stride;
   const int32_t* start; const int32_t* counts;
@@ -67,6 +69,13 @@ struct Shape {
   static constexpr int kStages = DP == 128 ? 3 : 6;
   static constexpr int kWarpRing = kStages * 2 * kSliceBytes;
 };
+
+// The dynamic shared memory from its first 256-byte boundary on: slices' rows lie on their own length.
+constexpr int kAlign = 256;
+__device__ __forceinline__ uint8_t* aligned_smem() {
+  extern __shared__ __align__(16) uint8_t raw_smem[];
+  return raw_smem + (kAlign - smem_u32(raw_smem) % kAlign) % kAlign;
+}
 
 // What a tile of rows sees of its sequence.
 struct View {
@@ -97,86 +106,93 @@ __device__ __forceinline__ View tile_view(const PagedParams& p, int32_t b, int32
   return x;
 }
 
-// The slices of one warp, `stride` slices apart within an item, copied into its ring in turn.
-template <int DP>
+// The slices of one warp, copied into its ring in turn.  A lane looks up the place of one key, in
+// 16-byte units (32 bits reach 64 GB), and hands it to the lanes that copy the key's chunks.
+template <int DP, bool FULL>
 struct Feed {
   using L = Shape<DP>;
-  static constexpr int CH = L::kChunks, NS = L::kStages;
+  static constexpr int CH = L::kChunks, NS = L::kStages, kRowsAStep = 32 / CH;
   const PagedParams& p;
-  uint32_t ring;
   uint32_t* seen_s;                         // [NS]: which keys of a ring's slice are read
+  const int32_t* table;                     // of the item's sequence
+  const uint8_t *k, *v;                     // of its key head, at this lane's chunk
+  uint32_t to;                              // this lane's chunk of its first row, in the ring's first slice
   int lane, cr, cc;                         // this lane copies chunk cc of rows cr, cr + 32 / CH, ...
   bool chunk_read, chunk_used;
-  // The item: lanes 0-15 look up a slice's keys for K, 16-31 for V.
-  const int32_t* table;
-  const uint8_t* base;
-  int64_t page_bytes, row_bytes;
-  int32_t next_page, next_row;
-  int32_t issued;
+  int32_t issued, slot;
 
-  __device__ __forceinline__ Feed(const PagedParams& params, uint32_t ring_at, uint32_t* seen) : p(params), ring(ring_at), seen_s(seen) {
+  __device__ __forceinline__ Feed(const PagedParams& params, uint32_t ring, uint32_t* seen) : p(params), seen_s(seen) {
     lane = threadIdx.x & 31;
     cr = lane / CH;
     cc = lane % CH;
-    chunk_read = cc * 8 < p.head_dim;
-    chunk_used = cc * 8 < ((p.head_dim + 15) & ~15);  // columns past D that the products read are zero
-    page_bytes = (lane >= 16 ? p.vs[0] : p.ks[0]) * 2;
-    row_bytes = (lane >= 16 ? p.vs[2] : p.ks[2]) * 2;
-    next_page = -1;
-    next_row = 0;
-    issued = 0;
+    chunk_read = FULL || cc * 8 < p.head_dim;
+    chunk_used = FULL || cc * 8 < ((p.head_dim + 15) & ~15);  // columns past D that the products read are zero
+    to = ring;
+    issued = slot = 0;
   }
   __device__ __forceinline__ void enter(int32_t b, int32_t grp) {
     table = p.table + b * p.table_stride;
-    base = static_cast<const uint8_t*>(lane >= 16 ? p.v : p.k) + grp * (lane >= 16 ? p.vs[1] : p.ks[1]) * 2;
+    const int64_t at = grp * p.head_stride * 2 + cc * 16;
+    k = static_cast<const uint8_t*>(p.k) + at;
+    v = static_cast<const uint8_t*>(p.v) + at;
   }
-  // A slice's pages: used a step later.
-  __device__ __forceinline__ void look_up(const View& view, int32_t slice) {
+  // A slice's pages; what comes of the load is used a step later.
+  __device__ __forceinline__ void look_up(const View& view, int32_t slice, int32_t& page, uint32_t& row) const {
     const int32_t key = view.slice(slice) * kStep + (lane & 15);
-    next_page = -1;
+    page = -1;
     if (key < view.end && (key >= view.low || key < view.sink_end)) {
-      const uint32_t index = static_cast<uint32_t>(key) / static_cast<uint32_t>(p.page_size);
-      next_page = __ldg(table + index);
-      next_row = key - static_cast<int32_t>(index) * p.page_size;
+      const uint32_t index = __umulhi(static_cast<uint32_t>(key) << 2, p.page_magic) >> p.page_shift;
+      page = __ldg(table + index);
+      row = key - index * p.page_size;
     }
   }
-  // The rows that were looked up; returns this lane's row, before the next look-up may change the item.
-  __device__ __forceinline__ uint64_t found(uint32_t& seen) const {
-    const bool there = next_page >= 0 && next_page < p.pages;
-    seen = __ballot_sync(0xffffffffu, there) & 0xffffu;
-    return reinterpret_cast<uint64_t>(base + (there ? next_page * page_bytes + next_row * row_bytes : 0));
-  }
-  __device__ __forceinline__ void copy(uint64_t row, uint32_t seen) {
-    const int slot = issued % NS;
+  __device__ __forceinline__ void copy(int32_t page, uint32_t row, const uint8_t* k_at, const uint8_t* v_at) {
+    const bool there = page >= 0 && page < p.pages;
+    const uint32_t place = there ? page * p.page_units + row * p.row_units : 0u;
+    const uint32_t seen = __ballot_sync(0xffffffffu, there) & 0xffffu;
     if (lane == 0) seen_s[slot] = seen;
-    const uint32_t dst = ring + slot * 2 * L::kSliceBytes;
+    const uint32_t dst = to + slot * 2 * L::kSliceBytes;
+    if (FULL && seen == 0xffffu) {
 #pragma unroll
-    for (int u = 0; u < kStep * CH / 32; ++u) {
-      const int r = cr + u * (32 / CH);
-      const uint64_t ks = __shfl_sync(0xffffffffu, row, r), vs = __shfl_sync(0xffffffffu, row, 16 + r);
-      const bool read = chunk_read && (seen >> r & 1u);
-      const uint32_t to = dst + chunk_offset<CH>(r, cc);
-      if (chunk_used) {
-        const uint8_t* none = static_cast<const uint8_t*>(p.q);
-        cp_async16(to, read ? reinterpret_cast<const uint8_t*>(ks) + cc * 16 : none, read);
-        cp_async16(to + L::kSliceBytes, read ? reinterpret_cast<const uint8_t*>(vs) + cc * 16 : none, read);
+      for (int u = 0; u < kStep / kRowsAStep; ++u) {
+        const int r = cr + u * kRowsAStep;
+        const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, place, r)) * 16;
+        const uint32_t d = dst + chunk_offset<CH>(r, cc);
+        cp_async16(d, k_at + at);
+        cp_async16(d + L::kSliceBytes, v_at + at);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kStep / kRowsAStep; ++u) {
+        const int r = cr + u * kRowsAStep;
+        const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, place, r)) * 16;
+        const bool read = chunk_read && (seen >> r & 1u);
+        const uint32_t d = dst + chunk_offset<CH>(r, cc);
+        if (chunk_used) {
+          const uint8_t* none = static_cast<const uint8_t*>(p.q);
+          cp_async16(d, read ? k_at + at : none, read);
+          cp_async16(d + L::kSliceBytes, read ? v_at + at : none, read);
+        }
       }
     }
   }
   __device__ __forceinline__ void commit() {
     ++issued;
+    slot = slot + 1 == NS ? 0 : slot + 1;
     cp_async_commit();
   }
 };
 
 // What a warp holds of a tile of rows: the queries, and the sums over the slices so far.
-template <int DP, bool BF16, int NT>
+template <int DP, bool FULL, bool BF16, int NT>
 struct Rows {
   static constexpr int CH = Shape<DP>::kChunks;
   uint32_t qb[NT][DP / 16][2];              // rows 8 n + g as columns of q^T
   int32_t pos[NT][2];                       // positions of rows 8 n + 2 t, + 1
   float o[NT][DP / 16][4];
-  float m[NT][2], l[NT][2];                 // rows 8 n + 2 t + h: running reference, this lane's part of the sum
+  // Rows 8 n + 2 t + h: running reference, what a score may reach before it moves, what is taken from a
+  // score (0 for a row without one above -inf), this lane's part of the sum.
+  float m[NT][2], limit[NT][2], ref[NT][2], l[NT][2];
 
   __device__ __forceinline__ void enter(const PagedParams& p, const View& view, int32_t b, int32_t grp, int32_t row0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -198,6 +214,8 @@ struct Rows {
       for (int h = 0; h < 2; ++h) {
         pos[n][h] = view.first_pos + (row0 + 8 * n + 2 * t + h) / p.per_group - row0 / p.per_group;
         m[n][h] = -INFINITY;
+        limit[n][h] = -INFINITY;
+        ref[n][h] = BF16 ? 0.f : -7.f;
         l[n][h] = 0.f;
       }
 #pragma unroll
@@ -209,10 +227,12 @@ struct Rows {
 
   // One slice, keys k0 .. k0 + 15, of which the bits of `seen` are there.
   __device__ __forceinline__ void step(const PagedParams& p, const View& view, uint32_t k_s, int32_t k0, uint32_t seen) {
-    const uint32_t v_s = k_s + Shape<DP>::kSliceBytes;
+    constexpr float kShift = BF16 ? 0.f : 7.f, kTiny = BF16 ? 8.67361738e-19f : 5.96046448e-8f;  // 2^-60, 2^-24
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mi = lane >> 3, mr = lane & 7;
     const int D = p.head_dim;
-    const float score_scale = p.scale * kLog2e;
+    // Matrix addresses of chunk 0 and 1; further chunks differ in the bits that the permutation leaves apart.
+    const uint32_t k_at = k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), mi >> 1);
+    const uint32_t v_at = k_s + Shape<DP>::kSliceBytes + chunk_offset<CH>(mr + ((mi >> 1) << 3), mi & 1);
     float s[NT][4];                         // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -220,34 +240,39 @@ struct Rows {
       for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-      if (kk * 16 >= D) break;
+      if (!FULL && kk * 16 >= D) break;
       uint32_t r[4];                        // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
-      ldmatrix4(k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), 2 * kk + (mi >> 1)), r);
+      ldmatrix4(k_at ^ (kk * 32), r);
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma16816<BF16>(s[n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
     }
     // Whether rows of the tile differ in what they see of the slice.
-    const bool mixed = view.first_pos != view.last_pos && (k0 + kStep - 1 > view.first_pos ||
-                                      (p.window > 0 && k0 <= view.last_pos - p.window && k0 + kStep > p.sinks));
-    bool grow = false;
+    const bool mixed = view.first_pos != view.last_pos &&
+                       (k0 + kStep - 1 > view.first_pos ||
+                        (p.window > 0 && k0 <= view.last_pos - p.window && k0 + kStep > p.sinks));
+    const float score_scale = p.scale * kLog2e;
 #pragma unroll
-    for (int kh = 0; kh < 2; ++kh) {
-      const int32_t key = k0 + kh * 8 + g;
-      const bool there = seen >> (kh * 8 + g) & 1u;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < 4; ++e) s[n][e] *= score_scale;
+    if (mixed || seen != 0xffffu) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float& x = s[n][2 * kh + h];
-          x *= score_scale;
-          bool hidden = !there;
-          if (mixed)
-            hidden = hidden || key > pos[n][h] || (p.window > 0 && key <= pos[n][h] - p.window && key >= p.sinks);
-          if (hidden) x = -INFINITY;
-          // a NaN score counts as growth: it has to reach the reference
-          grow = grow || !(x <= m[n][h] + kRescale);
-        }
+      for (int kh = 0; kh < 2; ++kh) {
+        const int32_t key = k0 + kh * 8 + g;
+        const bool there = seen >> (kh * 8 + g) & 1u;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (!there || (mixed && (key > pos[n][h] || (p.window > 0 && key <= pos[n][h] - p.window && key >= p.sinks))))
+              s[n][2 * kh + h] = -INFINITY;
+      }
     }
+    bool grow = false;                      // a NaN score counts as growth: it has to reach the reference
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) grow = grow || !(s[n][e] <= limit[n][e & 1]);
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -258,6 +283,8 @@ struct Rows {
           fo[h] = top == -INFINITY ? 1.f : fast_exp2(m[n][h] - top);
           l[n][h] *= fo[h];
           m[n][h] = top;
+          limit[n][h] = top + kRescale;
+          ref[n][h] = (top == -INFINITY ? 0.f : top) - kShift;
         }
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
@@ -265,35 +292,35 @@ struct Rows {
           for (int e = 0; e < 4; ++e) o[n][c][e] *= fo[e & 1];
       }
     }
-    uint32_t pb[NT][2], pl[NT][2];          // P^T as the 8-wide operand: keys 2t, 2t+1 of each 8, row g; what 16 bits leave out
+    // P^T as the 8-wide operand (keys 2t, 2t+1 of each 8, row g): the value cut off to 16 bits, and what
+    // that leaves out, which is positive wherever the value is: against an infinite state both parts
+    // give the same infinity.  In f16 P is 2^7 times itself, so that the smallest low part, 2^-24, is 2^-31 of it.
+    uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      // A row without a score above -inf keeps 0 as its reference.
-      const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh) {
         float pr[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          pr[h] = fast_exp2(s[n][2 * kh + h] - ref[h]);
+          pr[h] = fast_exp2(s[n][2 * kh + h] - ref[n][h]);
           l[n][h] += pr[h];
         }
-        const uint32_t high = pack2<BF16>(pr[0], pr[1]);
-        pb[n][kh] = transpose8(high);
+        const uint32_t high = pack2_down<BF16>(pr[0], pr[1]);
         const float2 f = unpack2<BF16>(high);
-        pl[n][kh] = transpose8(pack2<BF16>(pr[0] - f.x, pr[1] - f.y));
+        pb[n][kh] = transpose8(high);
+        pl[n][kh] = transpose8(pack2<BF16>(fmaxf(pr[0] - f.x, fminf(pr[0], kTiny)), fmaxf(pr[1] - f.y, fminf(pr[1], kTiny))));
       }
-    }
     bool apart = false;
     if (mixed) {
       // A state that some rows do not see may hold infinities or NaN, which zero probabilities would
       // let through: such a slice goes token by token.
       bool odd = false;
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        if (c * 8 >= D) break;
+      for (int c = 0; c < DP / 16; ++c) {
+        if (!FULL && c * 16 >= D) break;
         uint32_t r[4];
-        ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), c + (mi & 1)), r);
+        ldmatrix4_trans(v_at ^ (c * 32), r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd = odd || not_finite2<BF16>(r[e]);
       }
@@ -301,50 +328,45 @@ struct Rows {
     }
     if (!apart) {
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        if (c * 8 >= D) break;
-        uint32_t r[4];                      // chunk c and c + 1 of keys 0-7, then of 8-15
-        ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), c + (mi & 1)), r);
+      for (int c = 0; c < DP / 16; ++c) {
+        if (!FULL && c * 16 >= D) break;
+        uint32_t r[4];                      // chunk 2 c and 2 c + 1 of keys 0-7, then of 8-15
+        ldmatrix4_trans(v_at ^ (c * 32), r);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
-        // the low parts may be zero or negative: against an infinite value they would turn the
-        // high parts' infinity into NaN, so they meet finite values
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = finite2<BF16>(r[e]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c / 2], r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c], r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
       }
-    } else {
+      return;
+    }
 #pragma unroll 1
-      for (int32_t at = view.first_pos; at <= view.last_pos; ++at) {
-        uint32_t keep[2];                   // keys 2t, 2t+1 of each 8 that position `at` sees
+    for (int32_t at = view.first_pos; at <= view.last_pos; ++at) {
+      uint32_t keep[2];                     // keys 2t, 2t+1 of each 8 that position `at` sees
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          keep[kh] = 0u;
+      for (int kh = 0; kh < 2; ++kh) {
+        keep[kh] = 0u;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int32_t key = k0 + kh * 8 + 2 * t + e;
-            const bool sees = key <= at && (p.window == 0 || key > at - p.window || key < p.sinks);
-            if (sees) keep[kh] |= 0xffffu << (16 * e);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int32_t key = k0 + kh * 8 + 2 * t + e;
+          const bool sees = key <= at && (p.window == 0 || key > at - p.window || key < p.sinks);
+          if (sees) keep[kh] |= 0xffffu << (16 * e);
         }
+      }
 #pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-          if (c * 8 >= D) break;
-          uint32_t r[4];
-          ldmatrix4_trans(v_s + chunk_offset<CH>(mr + ((mi >> 1) << 3), c + (mi & 1)), r);
+      for (int c = 0; c < DP / 16; ++c) {
+        if (!FULL && c * 16 >= D) break;
+        uint32_t r[4];
+        ldmatrix4_trans(v_at ^ (c * 32), r);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] &= keep[e >> 1];
+        for (int e = 0; e < 4; ++e) r[e] &= keep[e >> 1];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16816<BF16>(x, r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
-            mma16816<BF16>(x, finite2<BF16>(r[0]), finite2<BF16>(r[1]), finite2<BF16>(r[2]), finite2<BF16>(r[3]), pl[n][0],
-                           pl[n][1]);
+        for (int n = 0; n < NT; ++n) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816<BF16>(x, r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+          mma16816<BF16>(x, r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (pos[n][e & 1] == at) o[n][c / 2][e] += x[e];
-          }
+          for (int e = 0; e < 4; ++e)
+            if (pos[n][e & 1] == at) o[n][c][e] += x[e];
         }
       }
     }
@@ -352,7 +374,7 @@ struct Rows {
 };
 
 // NT: tiles of 8 query rows.  kWarps warps a CTA, the CTAs of an item a cluster of any size.
-template <int DP, bool BF16, int NT, int kWarps>
+template <int DP, bool FULL, bool BF16, int NT, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_joined_kernel(const PagedParams p) {
   namespace cg = cooperative_groups;
@@ -360,7 +382,7 @@ paged_joined_kernel(const PagedParams p) {
   constexpr int NS = L::kStages;
   constexpr int kTile = 8 * NT;
   constexpr int kJoinStride = DP + 4;       // floats
-  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* smem = aligned_smem();
   __shared__ float m_s[kWarps][kTile], l_s[kWarps][kTile];
   __shared__ float top_s[kTile], total_s[kTile];
   __shared__ uint32_t seen_s[kWarps][NS];
@@ -379,28 +401,30 @@ paged_joined_kernel(const PagedParams p) {
   const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * (rank + 1) / n_ranks);
   const int32_t mine = s1 > s0 ? (s1 - s0 + kWarps - 1) / kWarps : 0;
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  Feed<DP> feed(p, ring, seen_s[warp]);
+  Feed<DP, FULL> feed(p, ring, seen_s[warp]);
   feed.enter(b, grp);
+  int32_t next_page = -1;
+  uint32_t next_row = 0;
   auto issue = [&]() {
     if (feed.issued < mine) {
-      uint32_t seen;
-      const uint64_t row = feed.found(seen);
-      if (feed.issued + 1 < mine) feed.look_up(view, s0 + (feed.issued + 1) * kWarps);
-      feed.copy(row, seen);
+      const int32_t page = next_page;
+      const uint32_t row = next_row;
+      if (feed.issued + 1 < mine) feed.look_up(view, s0 + (feed.issued + 1) * kWarps, next_page, next_row);
+      feed.copy(page, row, feed.k, feed.v);
     }
     feed.commit();
   };
-  if (mine > 0) feed.look_up(view, s0);
+  if (mine > 0) feed.look_up(view, s0, next_page, next_row);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) issue();
   const int32_t row0 = rt * kTile;
   const int32_t n_rows = min(p.rows - row0, kTile);
-  Rows<DP, BF16, NT> rows;
+  Rows<DP, FULL, BF16, NT> rows;
   rows.enter(p, view, b, grp, row0);
-  for (int32_t i = 0; i < mine; ++i) {
+  for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    rows.step(p, view, ring + (i % NS) * 2 * L::kSliceBytes, view.slice(s0 + i * kWarps) * kStep, seen_s[warp][i % NS]);
+    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(s0 + i * kWarps) * kStep, seen_s[warp][at]);
     __syncwarp();
     issue();
   }
@@ -491,12 +515,12 @@ paged_joined_kernel(const PagedParams p) {
 }
 
 // Every warp on its own: kWarps warps a CTA, one wave of CTAs.
-template <int DP, bool BF16, int NT, int kWarps>
+template <int DP, bool FULL, bool BF16, int NT, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_parts_kernel(const PagedParams p, const Parts parts) {
   using L = Shape<DP>;
   constexpr int NS = L::kStages, kTile = 8 * NT, kThreads = kWarps * 32;
-  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* smem = aligned_smem();
   __shared__ uint32_t seen_s[kWarps][NS];
   __shared__ int32_t sum_s[kWarps];
   int32_t* before = reinterpret_cast<int32_t*>(smem + kWarps * L::kWarpRing);  // [batch + 1]
@@ -567,30 +591,33 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
     return true;
   };
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  Feed<DP> feed(p, ring, seen_s[warp]);
+  Feed<DP, FULL> feed(p, ring, seen_s[warp]);
   feed.enter(in.b, in.grp);
+  int32_t next_page = -1;
+  uint32_t next_row = 0;
   auto issue = [&]() {
     if (feed.issued < mine) {
-      uint32_t seen;
-      const uint64_t row = feed.found(seen);
+      const int32_t page = next_page;
+      const uint32_t row = next_row;
+      const uint8_t *k = feed.k, *v = feed.v;
       if (feed.issued + 1 < mine) {
         if (advance(in, view_in)) feed.enter(in.b, in.grp);
-        feed.look_up(view_in, in.slice);
+        feed.look_up(view_in, in.slice, next_page, next_row);
       }
-      feed.copy(row, seen);
+      feed.copy(page, row, k, v);
     }
     feed.commit();
   };
-  feed.look_up(view_in, in.slice);
+  feed.look_up(view_in, in.slice, next_page, next_row);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) issue();
-  Rows<DP, BF16, NT> rows;
+  Rows<DP, FULL, BF16, NT> rows;
   rows.enter(p, view, out.b, out.grp, 0);
   const int g = lane >> 2, t = lane & 3;
-  for (int32_t i = 0; i < mine; ++i) {
+  for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    rows.step(p, view, ring + (i % NS) * 2 * L::kSliceBytes, view.slice(out.slice) * kStep, seen_s[warp][i % NS]);
+    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * kStep, seen_s[warp][at]);
     __syncwarp();
     issue();
     if (i + 1 < mine && out.slice + 1 < out.n) {
@@ -735,13 +762,13 @@ Plan plan(const paged_attention_args* a) {
   return x;
 }
 
-template <int DP, bool BF16, int NT>
+template <int DP, bool FULL, bool BF16, int NT>
 int32_t launch_joined(PagedParams p, cudaStream_t stream) {
   constexpr int W = 4;
   using L = Shape<DP>;
-  auto kernel = paged_joined_kernel<DP, BF16, NT, W>;
+  auto kernel = paged_joined_kernel<DP, FULL, BF16, NT, W>;
   constexpr int kRing = W * L::kWarpRing, kJoin = W * 8 * NT * (DP + 4) * 4;
-  constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kAlign;
   static_assert(kSmem <= 224 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
   if (!allow_smem(kernel, kSmem, done)) return INTP_ERR_LAUNCH;
@@ -764,16 +791,16 @@ int32_t launch_joined(PagedParams p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? INTP_OK : INTP_ERR_LAUNCH;
 }
 
-template <int DP, bool BF16, int NT>
+template <int DP, bool FULL, bool BF16, int NT>
 int32_t launch_parts(PagedParams p, const Parts& parts, cudaStream_t stream) {
   using L = Shape<DP>;
-  auto kernel = paged_parts_kernel<DP, BF16, NT, kPartsWarps>;
-  constexpr int kRing = kPartsWarps * L::kWarpRing, kMost = kRing + (kPartsBatch + 1) * 4;
+  auto kernel = paged_parts_kernel<DP, FULL, BF16, NT, kPartsWarps>;
+  constexpr int kRing = kPartsWarps * L::kWarpRing, kMost = kRing + kAlign + (kPartsBatch + 1) * 4;
   static_assert(kMost <= 112 * 1024, "two CTAs an SM");
   static std::atomic<uint64_t> done{0};
   if (!allow_smem(kernel, kMost, done)) return INTP_ERR_LAUNCH;
   p.n_rt = 1;
-  if (!launch_kernel(kernel, dim3(kPartsCtas), kPartsWarps * 32, kRing + (p.batch + 1) * 4, stream, false, p, parts))
+  if (!launch_kernel(kernel, dim3(kPartsCtas), kPartsWarps * 32, kRing + kAlign + (p.batch + 1) * 4, stream, false, p, parts))
     return INTP_ERR_LAUNCH;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.queries;
   // Few items have many parts each: a CTA per row, whose four warps share them.
@@ -784,11 +811,19 @@ int32_t launch_parts(PagedParams p, const Parts& parts, cudaStream_t stream) {
                                                                                                         : INTP_ERR_LAUNCH;
 }
 
-template <int DP, bool BF16>
+template <int DP, bool FULL, bool BF16>
 int32_t launch_rows(const PagedParams& p, const Parts* parts, cudaStream_t stream) {
   if (parts != nullptr)
-    return p.rows <= 8 ? launch_parts<DP, BF16, 1>(p, *parts, stream) : launch_parts<DP, BF16, 2>(p, *parts, stream);
-  return p.rows <= 8 ? launch_joined<DP, BF16, 1>(p, stream) : launch_joined<DP, BF16, 2>(p, stream);
+    return p.rows <= 8 ? launch_parts<DP, FULL, BF16, 1>(p, *parts, stream) : launch_parts<DP, FULL, BF16, 2>(p, *parts, stream);
+  return p.rows <= 8 ? launch_joined<DP, FULL, BF16, 1>(p, stream) : launch_joined<DP, FULL, BF16, 2>(p, stream);
+}
+
+// Head dims that fill their slices' rows need no checks of columns.
+template <bool BF16>
+int32_t launch_dim(const PagedParams& p, const Parts* parts, cudaStream_t stream) {
+  if (p.head_dim == 64) return launch_rows<64, true, BF16>(p, parts, stream);
+  if (p.head_dim == 128) return launch_rows<128, true, BF16>(p, parts, stream);
+  return p.head_dim < 64 ? launch_rows<64, false, BF16>(p, parts, stream) : launch_rows<128, false, BF16>(p, parts, stream);
 }
 
 intp_status check_shape(const paged_attention_args* a) {
@@ -815,9 +850,14 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
   if (a->batch == 0 || a->queries == 0) return INTP_OK;
   if (!a->q || !a->k || !a->v || !a->out || !a->page_table || !a->start) return INTP_ERR_ARGUMENT;
   const int64_t eq[3] = {a->batch, a->heads, a->queries}, ek[3] = {a->pages, a->groups, a->page_size};
-  if (!rows_ok(a->q, a->q_stride, eq) || !rows_ok(a->out, a->out_stride, eq) || !rows_ok(a->k, a->k_stride, ek) ||
-      !rows_ok(a->v, a->v_stride, ek))
+  if (!rows_ok(a->q, a->q_stride, eq) || !rows_ok(a->out, a->out_stride, eq) || !rows_ok(a->k, a->cache_stride, ek) ||
+      !rows_ok(a->v, a->cache_stride, ek))
     return INTP_ERR_LAYOUT;
+  int64_t cache[3];
+  take(cache, a->cache_stride, ek);
+  // Places are 32-bit numbers of 16-byte units.
+  if (cache[0] / 8 > UINT32_MAX || cache[2] / 8 > UINT32_MAX ||
+      (a->pages - 1) * (cache[0] / 8) + (a->page_size - 1) * (cache[2] / 8) > UINT32_MAX) return INTP_ERR_LAYOUT;
   const Plan how = plan(a);
   if (how.bytes > 0 &&
       (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < how.bytes))
@@ -843,9 +883,14 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
   p.q = a->q;
   take(p.qs, a->q_stride, eq);
   p.k = a->k;
-  take(p.ks, a->k_stride, ek);
   p.v = a->v;
-  take(p.vs, a->v_stride, ek);
+  p.head_stride = cache[1];
+  p.page_units = static_cast<uint32_t>(cache[0] / 8);
+  p.row_units = static_cast<uint32_t>(cache[2] / 8);
+  // With 2^shift >= page_size, magic = ceil(2^(30 + shift) / page_size) is off by less than
+  // 2^shift / page_size of 2^30: the quotient is exact for every p < 2^30.
+  while ((int64_t(1) << p.page_shift) < a->page_size) ++p.page_shift;
+  p.page_magic = static_cast<uint32_t>(((uint64_t(1) << (30 + p.page_shift)) + a->page_size - 1) / a->page_size);
   p.out = a->out;
   take(p.os, a->out_stride, eq);
   p.table = a->page_table;
@@ -860,8 +905,7 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
     parts.plan = reinterpret_cast<int32_t*>(ws + how.o_bytes + how.ml_bytes);
   }
   const Parts* x = how.parts ? &parts : nullptr;
-  if (a->dtype == INTP_BF16) return p.head_dim <= 64 ? launch_rows<64, true>(p, x, stream) : launch_rows<128, true>(p, x, stream);
-  return p.head_dim <= 64 ? launch_rows<64, false>(p, x, stream) : launch_rows<128, false>(p, x, stream);
+  return a->dtype == INTP_BF16 ? launch_dim<true>(p, x, stream) : launch_dim<false>(p, x, stream);
 }
 
 }  // namespace

@@ -38,6 +38,16 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
+// Cut off instead of rounded.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2_down(float lo, float hi) {
+  uint32_t d;
+  if (BF16)
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));

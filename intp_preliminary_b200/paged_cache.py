@@ -33,6 +33,7 @@ from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _che
 
 _ATTENTION_POINTERS = struct.Struct("9Q")  # paged_attention_args up to the sizes
 _MAX_STATES = 1 << 30
+_MAX_SPAN = 1 << 35  # elements: 2^32 units of 16 bytes
 _KERNELS = {"auto": _lib.PAGED_KERNEL_AUTO, "joined": _lib.PAGED_KERNEL_JOINED, "parts": _lib.PAGED_KERNEL_PARTS}
 
 
@@ -52,19 +53,23 @@ def _check_cache(keys, values) -> None:
         raise ValueError("head_dim must be a multiple of 8 up to 128")
     if not (_ready(keys) and _ready(values)):
         raise ValueError("the cache's tensors need unit stride on head_dim and 16-byte aligned rows")
+    if keys.stride() != values.stride():
+        raise ValueError("keys and values must share their strides")
+    if sum((n - 1) * s for n, s in zip(keys.shape, keys.stride())) >= _MAX_SPAN:
+        raise ValueError("a paged cache's keys may span 64 GB at most, and its values too")
 
 
 class PagedCache:
     """``keys`` and ``values`` ``(pages, G, page_size, D)`` bf16 or f16 of the pool's
     pages, any page size from one up, D a multiple of 8 up to 128.  Outer strides are free
-    (multiples of 16 bytes): a pool laid out ``(pages, page_size, G, D)`` is passed
-    transposed.  The tensors may be written to but not replaced."""
+    (multiples of 16 bytes, the same for both): a pool laid out ``(pages, page_size, G, D)``
+    is passed transposed.  The tensors may be written to but not replaced."""
 
     def __init__(self, keys, values) -> None:
         _check_cache(keys, values)
         self._keys, self._values = keys, values
         # what calls know the pool by
-        self._layout = (keys.shape, keys.stride(), values.stride(), keys.dtype, keys.device)
+        self._layout = (keys.shape, keys.stride(), keys.dtype, keys.device)
 
     # read only: a call takes the layout that was checked above
     keys = property(lambda self: self._keys)
@@ -208,7 +213,7 @@ def _attention_tail(q, cache: PagedCache, page_table, scale, window, sinks, out_
     args.batch, args.heads, args.queries, args.head_dim = q.shape
     args.groups, args.pages, args.page_size = groups, pages, page_size
     args.q_stride, args.out_stride = q.stride(), out_stride
-    args.k_stride, args.v_stride = cache._keys.stride(), cache._values.stride()
+    args.cache_stride = cache._keys.stride()
     args.table_width, args.table_stride = page_table.shape[1], page_table.stride(0)
     args.window, args.sinks = window or 0, sinks
     args.scale = _check_scale(scale)

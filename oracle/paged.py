@@ -8,7 +8,9 @@ Where a kernel may round, with u the unit roundoff of the output type (half its 
         products and a sum: 2 * 2^-24 more.  The result is rounded once: u |y| (f16: at most 2^-25
         below its normal range).
   attention: the bound of a kernel that multiplies each probability as two 16-bit numbers, as
-        oracle.cross_attention's ``two_part`` derives it.
+        oracle.cross_attention's ``two_part`` derives it, but for the two parts: the first is cut off
+        (less than eps = 2 u of the probability is left), the second rounded (u of that): 2 u^2.  Its
+        smallest value is 2^-60 of a probability's unit (f16: 2^-31), which is below what f16 loses.
 """
 
 from __future__ import annotations
@@ -90,7 +92,7 @@ def attend(q, keys, values, *, page_table, start, scale, counts=None, window=Non
                 # a score of -inf is exact: its probability is zero
                 size = torch.where(s == -float("inf"), torch.zeros_like(s), scale * (kk.abs() @ q[b, h, m].abs()))
                 score = 2.0 ** -23 * ((dim + 8) * size + 4 * s[s != -float("inf")].abs().max())
-                rel = u ** 2 + 2.0 ** -22 * (1 + 64 + len(found) / 16)
+                rel = 2 * u ** 2 + 2.0 ** -22 * (1 + 64 + len(found) / 16)
                 w = p * (score + rel)
                 bound[b, h, m] = w @ vv.abs() + w.sum() * (p @ vv.abs()) + u * out[b, h, m].abs()
                 if dtype == torch.float16:

@@ -112,8 +112,9 @@ def test_append_refuses_before_a_launch(over, status):
     ({"page_table": None}, _lib.INTP_ERR_ARGUMENT),
     ({"start": None}, _lib.INTP_ERR_ARGUMENT),
     ({"q": FAKE + 8}, _lib.INTP_ERR_LAYOUT),
-    ({"k_stride": _lib._Stride(2048, 1024, 68, 1)}, _lib.INTP_ERR_LAYOUT),
-    ({"v_stride": _lib._Stride(2048, 0, 64, 1)}, _lib.INTP_ERR_LAYOUT),
+    ({"cache_stride": _lib._Stride(2048, 1024, 68, 1)}, _lib.INTP_ERR_LAYOUT),
+    ({"cache_stride": _lib._Stride(2048, 0, 64, 1)}, _lib.INTP_ERR_LAYOUT),
+    ({"cache_stride": _lib._Stride(1 << 32, 1024, 64, 1)}, _lib.INTP_ERR_LAYOUT),  # places leave 32 bits
     ({"out_stride": _lib._Stride(768, 192, 64, 2)}, _lib.INTP_ERR_LAYOUT),
     ({"kernel": 3}, _lib.INTP_ERR_ARGUMENT),
     ({"kernel": _lib.PAGED_KERNEL_PARTS}, _lib.INTP_ERR_ARGUMENT),              # no workspace
@@ -129,7 +130,7 @@ def test_attention_refuses_before_a_launch(over, status):
     a.scale, a.dtype = 0.125, _lib.INTP_BF16
     a.q = a.k = a.v = a.out = a.page_table = a.start = FAKE
     a.q_stride = a.out_stride = _lib._Stride(768, 192, 64, 1)
-    a.k_stride = a.v_stride = _lib._Stride(2048, 1024, 64, 1)
+    a.cache_stride = _lib._Stride(2048, 1024, 64, 1)
     for key, value in over.items():
         setattr(a, key, value)
     assert _lib.load().paged_attention(ctypes.addressof(a), None) == status
@@ -236,4 +237,5 @@ def test_oracle_attends_like_cross_attention_over_the_gathered_states(page_size)
     got, bound = oracle.attend(q, keys, values, page_table=table, start=[x - 1 for x in lengths], scale=0.3)
     want, _, want_bound = cross_oracle.cross_attention(q, k, v, scale=0.3, lengths=lengths, two_part=True)
     assert (got - want).abs().max() < 1e-14
-    assert (bound / want_bound - 1).abs().max() < 1e-6
+    # one more u^2 of the same sum that the other bound holds one of
+    assert bool((bound >= want_bound).all()) and bool((bound <= 2 * want_bound).all())

@@ -458,7 +458,8 @@ def test_refusals(cuda_device):
     for keys, values, message in ((k, k.half(), "dtype"), (k.float(), k.float(), "bfloat16"), (k[0], k[0], "shape"),
                                   (k[:0], k[:0], "needs a page"), (k[..., :4], k[..., :4], "multiple of 8"),
                                   (k[..., :8].transpose(1, 3), k[..., :8].transpose(1, 3), "multiple of 8"),
-                                  (k.expand(2, 2, 5, 16), k.expand(2, 2, 5, 16), "unit stride")):
+                                  (k.expand(2, 2, 5, 16), k.expand(2, 2, 5, 16), "unit stride"),
+                                  (table.new_zeros(2, 2, 3, 16, dtype=BF16), table.new_zeros(2, 3, 2, 16, dtype=BF16).transpose(1, 2), "share their strides")):
         with pytest.raises(ValueError, match=message):
             PagedCache(keys, values)
     for name in ("keys", "values", "layout"):

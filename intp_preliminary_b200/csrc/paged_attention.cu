@@ -4,7 +4,7 @@
 // Reading the states bounds this: the query heads of a key head (and a sequence's few new tokens)
 // share each state, 16 rows at most to a pass, so a state of 4 D bytes carries at most 64 D
 // multiply-adds.  What counts is bytes in flight on every SM and few instructions a byte.
-// A warp streams slices of 16 keys through its own cp.async ring; every row of a slice is looked
+// A warp streams slices of 16 keys (32 of head_dim 64 or less) through its own cp.async ring; every row of a slice is looked
 // up in the page table by one lane, a step ahead of the copy, so pages may be of any size.  The
 // products are 16 x 8 x 16 matrix instructions with the states as the 16-high operand,
 //   S^T = k q^T (16 keys x 8 rows),   O^T += v^T P^T (16 columns x 8 rows),
@@ -28,7 +28,6 @@
 namespace intp {
 namespace {
 
-constexpr int kStep = 16;                  // keys of a slice
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;            // log2 units a score may pass its reference by
 
@@ -37,6 +36,7 @@ struct PagedParams {
   int32_t pages, page_size;
   int32_t capacity;                        // states that a row of the page table has room for
   int32_t rows, n_rt;                      // rows of a sequence and key head, tiles of them
+  int32_t depth;                           // slices that a warp's ring has room for, in one launch
   int32_t window, sinks;                   // window 0: none
   float scale;
   const void* q; int64_t qs[3];            // sequence, head, token
@@ -65,8 +65,9 @@ constexpr int kPartsLeast = 2;             // slices of a part at least
 template <int DP>
 struct Shape {
   static constexpr int kChunks = DP * 2 / 16;
+  static constexpr int kStep = DP == 128 ? 16 : 32;        // keys of a slice: 8 KB of K and V
   static constexpr int kSliceBytes = kStep * DP * 2;       // K or V of a slice
-  static constexpr int kStages = DP == 128 ? 3 : 6;
+  static constexpr int kStages = 3;
   static constexpr int kWarpRing = kStages * 2 * kSliceBytes;
 };
 
@@ -85,7 +86,7 @@ struct View {
   __device__ __forceinline__ int32_t slice(int32_t i) const { return i < sink_slices ? i : i - sink_slices + low_slice; }
 };
 
-template <int kTile>
+template <int kTile, int kStep>
 __device__ __forceinline__ View tile_view(const PagedParams& p, int32_t b, int32_t rt) {
   View x;
   const int32_t m0 = rt * kTile / p.per_group;
@@ -111,23 +112,28 @@ __device__ __forceinline__ View tile_view(const PagedParams& p, int32_t b, int32
 template <int DP, bool FULL>
 struct Feed {
   using L = Shape<DP>;
-  static constexpr int CH = L::kChunks, NS = L::kStages, kRowsAStep = 32 / CH;
+  static constexpr int CH = L::kChunks, NS = L::kStages, kStep = L::kStep, kRowsAStep = 32 / CH;
+  static constexpr uint32_t kAll = 0xffffffffu >> (32 - kStep);
   const PagedParams& p;
   uint32_t* seen_s;                         // [NS]: which keys of a ring's slice are read
   const int32_t* table;                     // of the item's sequence
   const uint8_t *k, *v;                     // of its key head, at this lane's chunk
   uint32_t to;                              // this lane's chunk of its first row, in the ring's first slice
   int lane, cr, cc;                         // this lane copies chunk cc of rows cr, cr + 32 / CH, ...
-  bool chunk_read, chunk_used;
+  bool chunk_read;
   int32_t issued, slot;
 
-  __device__ __forceinline__ Feed(const PagedParams& params, uint32_t ring, uint32_t* seen) : p(params), seen_s(seen) {
+  __device__ __forceinline__ Feed(const PagedParams& params, uint32_t ring, int32_t depth, uint32_t* seen) : p(params), seen_s(seen) {
     lane = threadIdx.x & 31;
     cr = lane / CH;
     cc = lane % CH;
     chunk_read = FULL || cc * 8 < p.head_dim;
-    chunk_used = FULL || cc * 8 < ((p.head_dim + 15) & ~15);  // columns past D that the products read are zero
     to = ring;
+    // The products read columns up to a multiple of 16; those past D are never copied and stay zero.
+    if (!FULL && p.head_dim % 16 != 0)
+      for (int i = lane; i < depth * 2 * kStep; i += 32)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + (i / kStep) * L::kSliceBytes +
+                                                                    chunk_offset<CH>(i % kStep, p.head_dim / 8)), "r"(0) : "memory");
     issued = slot = 0;
   }
   __device__ __forceinline__ void enter(int32_t b, int32_t grp) {
@@ -136,39 +142,42 @@ struct Feed {
     k = static_cast<const uint8_t*>(p.k) + at;
     v = static_cast<const uint8_t*>(p.v) + at;
   }
+  __device__ __forceinline__ void page_of(int32_t key, int32_t& page, uint32_t& row) const {
+    const uint32_t index = __umulhi(static_cast<uint32_t>(key) << 2, p.page_magic) >> p.page_shift;
+    page = __ldg(table + index);
+    row = key - index * p.page_size;
+  }
   // A slice's pages; what comes of the load is used a step later.
   __device__ __forceinline__ void look_up(const View& view, int32_t slice, int32_t& page, uint32_t& row) const {
-    const int32_t key = view.slice(slice) * kStep + (lane & 15);
+    const int32_t key = view.slice(slice) * kStep + (lane & (kStep - 1));
     page = -1;
-    if (key < view.end && (key >= view.low || key < view.sink_end)) {
-      const uint32_t index = __umulhi(static_cast<uint32_t>(key) << 2, p.page_magic) >> p.page_shift;
-      page = __ldg(table + index);
-      row = key - index * p.page_size;
-    }
+    if (key < view.end && (key >= view.low || key < view.sink_end)) page_of(key, page, row);
   }
   __device__ __forceinline__ void copy(int32_t page, uint32_t row, const uint8_t* k_at, const uint8_t* v_at) {
     const bool there = page >= 0 && page < p.pages;
     const uint32_t place = there ? page * p.page_units + row * p.row_units : 0u;
-    const uint32_t seen = __ballot_sync(0xffffffffu, there) & 0xffffu;
+    const uint32_t seen = __ballot_sync(0xffffffffu, there) & kAll;
     if (lane == 0) seen_s[slot] = seen;
     const uint32_t dst = to + slot * 2 * L::kSliceBytes;
-    if (FULL && seen == 0xffffu) {
+    if (seen == kAll) {
 #pragma unroll
       for (int u = 0; u < kStep / kRowsAStep; ++u) {
         const int r = cr + u * kRowsAStep;
         const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, place, r)) * 16;
         const uint32_t d = dst + chunk_offset<CH>(r, cc);
-        cp_async16(d, k_at + at);
-        cp_async16(d + L::kSliceBytes, v_at + at);
+        if (chunk_read) {
+          cp_async16(d, k_at + at);
+          cp_async16(d + L::kSliceBytes, v_at + at);
+        }
       }
-    } else {
+    } else {                                // rows that are not there are zero
 #pragma unroll
       for (int u = 0; u < kStep / kRowsAStep; ++u) {
         const int r = cr + u * kRowsAStep;
         const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, place, r)) * 16;
-        const bool read = chunk_read && (seen >> r & 1u);
+        const bool read = seen >> r & 1u;
         const uint32_t d = dst + chunk_offset<CH>(r, cc);
-        if (chunk_used) {
+        if (chunk_read) {
           const uint8_t* none = static_cast<const uint8_t*>(p.q);
           cp_async16(d, read ? k_at + at : none, read);
           cp_async16(d + L::kSliceBytes, read ? v_at + at : none, read);
@@ -225,26 +234,35 @@ struct Rows {
     }
   }
 
-  // One slice, keys k0 .. k0 + 15, of which the bits of `seen` are there.
+  // One slice, keys from k0 on, of which the bits of `seen` are there.
   __device__ __forceinline__ void step(const PagedParams& p, const View& view, uint32_t k_s, int32_t k0, uint32_t seen) {
     constexpr float kShift = BF16 ? 0.f : 7.f, kTiny = BF16 ? 8.67361738e-19f : 5.96046448e-8f;  // 2^-60, 2^-24
+    constexpr int kStep = Shape<DP>::kStep, KB = kStep / 16, kBlock = 16 * CH * 16;  // blocks of 16 keys, bytes of one
+    constexpr uint32_t kAll = 0xffffffffu >> (32 - kStep);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mi = lane >> 3, mr = lane & 7;
     const int D = p.head_dim;
+    // Whether 16-column block c has columns below D; DP is the smallest of its kind that holds D.
+    auto inside = [&](int c) { return FULL || (DP == 128 && c < 4) || c * 16 < D; };
     // Matrix addresses of chunk 0 and 1; further chunks differ in the bits that the permutation leaves apart.
     const uint32_t k_at = k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), mi >> 1);
     const uint32_t v_at = k_s + Shape<DP>::kSliceBytes + chunk_offset<CH>(mr + ((mi >> 1) << 3), mi & 1);
-    float s[NT][4];                         // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
+    float s[KB][NT][4];                     // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[k][n][e] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-      if (!FULL && kk * 16 >= D) break;
-      uint32_t r[4];                        // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
-      ldmatrix4(k_at ^ (kk * 32), r);
+      if (!inside(kk)) break;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma16816<BF16>(s[n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
+      for (int k = 0; k < KB; ++k) {
+        uint32_t r[4];                      // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
+        ldmatrix4((k_at + k * kBlock) ^ (kk * 32), r);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(s[k][n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
+      }
     }
     // Whether rows of the tile differ in what they see of the slice.
     const bool mixed = view.first_pos != view.last_pos &&
@@ -252,12 +270,14 @@ struct Rows {
                         (p.window > 0 && k0 <= view.last_pos - p.window && k0 + kStep > p.sinks));
     const float score_scale = p.scale * kLog2e;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] *= score_scale;
-    if (mixed || seen != 0xffffu) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
+        for (int e = 0; e < 4; ++e) s[k][n][e] *= score_scale;
+    if (mixed || seen != kAll) {
+#pragma unroll
+      for (int kh = 0; kh < 2 * KB; ++kh) {
         const int32_t key = k0 + kh * 8 + g;
         const bool there = seen >> (kh * 8 + g) & 1u;
 #pragma unroll
@@ -265,21 +285,26 @@ struct Rows {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             if (!there || (mixed && (key > pos[n][h] || (p.window > 0 && key <= pos[n][h] - p.window && key >= p.sinks))))
-              s[n][2 * kh + h] = -INFINITY;
+              s[kh / 2][n][2 * (kh & 1) + h] = -INFINITY;
       }
     }
     bool grow = false;                      // a NaN score counts as growth: it has to reach the reference
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) grow = grow || !(s[n][e] <= limit[n][e & 1]);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) grow = grow || !(s[k][n][e] <= limit[n][e & 1]);
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float fo[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float top = keys_max(max_nan(m[n][h], max_nan(s[n][h], s[n][2 + h])));
+          float top = m[n][h];
+#pragma unroll
+          for (int k = 0; k < KB; ++k) top = max_nan(top, max_nan(s[k][n][h], s[k][n][2 + h]));
+          top = keys_max(top);
           fo[h] = top == -INFINITY ? 1.f : fast_exp2(m[n][h] - top);
           l[n][h] *= fo[h];
           m[n][h] = top;
@@ -295,15 +320,15 @@ struct Rows {
     // P^T as the 8-wide operand (keys 2t, 2t+1 of each 8, row g): the value cut off to 16 bits, and what
     // that leaves out, which is positive wherever the value is: against an infinite state both parts
     // give the same infinity.  In f16 P is 2^7 times itself, so that the smallest low part, 2^-24, is 2^-31 of it.
-    uint32_t pb[NT][2], pl[NT][2];
+    uint32_t pb[NT][2 * KB], pl[NT][2 * KB];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
+      for (int kh = 0; kh < 2 * KB; ++kh) {
         float pr[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          pr[h] = fast_exp2(s[n][2 * kh + h] - ref[n][h]);
+          pr[h] = fast_exp2(s[kh / 2][n][2 * (kh & 1) + h] - ref[n][h]);
           l[n][h] += pr[h];
         }
         const uint32_t high = pack2_down<BF16>(pr[0], pr[1]);
@@ -318,32 +343,38 @@ struct Rows {
       bool odd = false;
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
-        if (!FULL && c * 16 >= D) break;
-        uint32_t r[4];
-        ldmatrix4_trans(v_at ^ (c * 32), r);
+        if (!inside(c)) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd = odd || not_finite2<BF16>(r[e]);
+        for (int k = 0; k < KB; ++k) {
+          uint32_t r[4];
+          ldmatrix4_trans((v_at + k * kBlock) ^ (c * 32), r);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = odd || not_finite2<BF16>(r[e]);
+        }
       }
       apart = __any_sync(0xffffffffu, odd);
     }
     if (!apart) {
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
-        if (!FULL && c * 16 >= D) break;
-        uint32_t r[4];                      // chunk 2 c and 2 c + 1 of keys 0-7, then of 8-15
-        ldmatrix4_trans(v_at ^ (c * 32), r);
+        if (!inside(c)) break;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+        for (int k = 0; k < KB; ++k) {
+          uint32_t r[4];                    // chunk 2 c and 2 c + 1 of keys 0-7, then of 8-15
+          ldmatrix4_trans((v_at + k * kBlock) ^ (c * 32), r);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c], r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
+          for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c], r[0], r[1], r[2], r[3], pb[n][2 * k], pb[n][2 * k + 1]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<BF16>(o[n][c], r[0], r[1], r[2], r[3], pl[n][2 * k], pl[n][2 * k + 1]);
+        }
       }
       return;
     }
 #pragma unroll 1
     for (int32_t at = view.first_pos; at <= view.last_pos; ++at) {
-      uint32_t keep[2];                     // keys 2t, 2t+1 of each 8 that position `at` sees
+      uint32_t keep[2 * KB];                // keys 2t, 2t+1 of each 8 that position `at` sees
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
+      for (int kh = 0; kh < 2 * KB; ++kh) {
         keep[kh] = 0u;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -354,28 +385,59 @@ struct Rows {
       }
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
-        if (!FULL && c * 16 >= D) break;
-        uint32_t r[4];
-        ldmatrix4_trans(v_at ^ (c * 32), r);
+        if (!inside(c)) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] &= keep[e >> 1];
+        for (int k = 0; k < KB; ++k) {
+          uint32_t r[4];
+          ldmatrix4_trans((v_at + k * kBlock) ^ (c * 32), r);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816<BF16>(x, r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
-          mma16816<BF16>(x, r[0], r[1], r[2], r[3], pl[n][0], pl[n][1]);
+          for (int e = 0; e < 4; ++e) r[e] &= keep[2 * k + (e >> 1)];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (pos[n][e & 1] == at) o[n][c][e] += x[e];
+          for (int n = 0; n < NT; ++n) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816<BF16>(x, r[0], r[1], r[2], r[3], pb[n][2 * k], pb[n][2 * k + 1]);
+            mma16816<BF16>(x, r[0], r[1], r[2], r[3], pl[n][2 * k], pl[n][2 * k + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (pos[n][e & 1] == at) o[n][c][e] += x[e];
+          }
         }
       }
     }
   }
 };
 
-// NT: tiles of 8 query rows.  kWarps warps a CTA, the CTAs of an item a cluster of any size.
-template <int DP, bool FULL, bool BF16, int NT, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32)
+// Sums of a row that are held relative to references of their own (one a lane, -inf where there is
+// none): the largest reference, and this lane's factor and part of the sum relative to it.
+struct Joint {
+  float top, total, factor;
+};
+__device__ __forceinline__ Joint join_references(float ref, float part) {
+  Joint j;
+  j.top = ref;
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1) j.top = max_nan(j.top, __shfl_xor_sync(0xffffffffu, j.top, d));
+  j.top = __shfl_sync(0xffffffffu, j.top, 0);
+  j.factor = ref == -INFINITY ? 0.f : fast_exp2(ref - j.top);
+  j.total = ref == -INFINITY ? 0.f : part * j.factor;
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1) j.total += __shfl_xor_sync(0xffffffffu, j.total, d);
+  j.total = __shfl_sync(0xffffffffu, j.total, 0);
+  return j;
+}
+__device__ __forceinline__ void add_weighted(float4& acc, const float4& v, float f) {
+  acc.x = fmaf(v.x, f, acc.x);
+  acc.y = fmaf(v.y, f, acc.y);
+  acc.z = fmaf(v.z, f, acc.z);
+  acc.w = fmaf(v.w, f, acc.w);
+}
+
+constexpr int kMostWarps = 8, kMostRanks = 8;
+
+// NT: tiles of 8 query rows.  One to eight warps a CTA, one to eight CTAs an item: the item's warps take
+// its slices in turn, so that the first look-up needs no length.
+template <int DP, bool FULL, bool BF16, int NT>
+__global__ void __launch_bounds__(kMostWarps * 32)
 paged_joined_kernel(const PagedParams p) {
   namespace cg = cooperative_groups;
   using L = Shape<DP>;
@@ -383,11 +445,12 @@ paged_joined_kernel(const PagedParams p) {
   constexpr int kTile = 8 * NT;
   constexpr int kJoinStride = DP + 4;       // floats
   uint8_t* smem = aligned_smem();
-  __shared__ float m_s[kWarps][kTile], l_s[kWarps][kTile];
+  __shared__ float m_s[kMostWarps][kTile], l_s[kMostWarps][kTile];
   __shared__ float top_s[kTile], total_s[kTile];
-  __shared__ uint32_t seen_s[kWarps][NS];
+  __shared__ uint32_t seen_s[kMostWarps][NS];
   const cg::cluster_group cluster = cg::this_cluster();
   const int32_t n_ranks = static_cast<int32_t>(cluster.num_blocks()), rank = static_cast<int32_t>(cluster.block_rank());
+  const int32_t n_warps = blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;    // fragment row and column pair
 
@@ -395,26 +458,31 @@ paged_joined_kernel(const PagedParams p) {
   const int32_t bg = item / p.n_rt, rt = item - bg * p.n_rt;
   const int32_t b = bg / p.groups, grp = bg - b * p.groups;
   const int32_t D = p.head_dim;
-  const View view = tile_view<kTile>(p, b, rt);
-  // This CTA's share of the slices; warps take them in turn.
-  const int32_t s0 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * rank / n_ranks) + warp;
-  const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(view.n_slices) * (rank + 1) / n_ranks);
-  const int32_t mine = s1 > s0 ? (s1 - s0 + kWarps - 1) / kWarps : 0;
-  const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  Feed<DP, FULL> feed(p, ring, seen_s[warp]);
+  const int32_t first = rank * n_warps + warp, stride = n_ranks * n_warps;
+  const uint32_t ring = smem_u32(smem) + warp * p.depth * 2 * L::kSliceBytes;
+  Feed<DP, FULL> feed(p, ring, p.depth, seen_s[warp]);
   feed.enter(b, grp);
+  // Without a window the first slice's pages are asked for together with the length.
   int32_t next_page = -1;
   uint32_t next_row = 0;
+  const int32_t first_key = first * L::kStep + (lane & (L::kStep - 1));
+  if (p.window == 0 && first_key < p.capacity) feed.page_of(first_key, next_page, next_row);
+  const View view = tile_view<kTile, L::kStep>(p, b, rt);
+  const int32_t mine = view.n_slices > first ? (view.n_slices - first + stride - 1) / stride : 0;
+  if (p.window == 0) {
+    if (first_key >= view.end) next_page = -1;
+  } else if (mine > 0) {
+    feed.look_up(view, first, next_page, next_row);
+  }
   auto issue = [&]() {
     if (feed.issued < mine) {
       const int32_t page = next_page;
       const uint32_t row = next_row;
-      if (feed.issued + 1 < mine) feed.look_up(view, s0 + (feed.issued + 1) * kWarps, next_page, next_row);
+      if (feed.issued + 1 < mine) feed.look_up(view, first + (feed.issued + 1) * stride, next_page, next_row);
       feed.copy(page, row, feed.k, feed.v);
     }
     feed.commit();
   };
-  if (mine > 0) feed.look_up(view, s0, next_page, next_row);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) issue();
   const int32_t row0 = rt * kTile;
@@ -424,7 +492,7 @@ paged_joined_kernel(const PagedParams p) {
   for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(s0 + i * kWarps) * kStep, seen_s[warp][at]);
+    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(first + i * stride) * L::kStep, seen_s[warp][at]);
     __syncwarp();
     issue();
   }
@@ -453,63 +521,55 @@ paged_joined_kernel(const PagedParams p) {
     }
   __syncthreads();
   const bool alone = n_ranks == 1;
+  const int d = lane * 4;
   auto write = [&](int32_t r, float4 acc, float total) {
     const int32_t row = row0 + r, tok = row / p.per_group, h = grp * p.per_group + (row - tok * p.per_group);
     const bool counts = p.counts == nullptr || tok < p.counts[b];
     const float inv = counts && total != 0.f ? 1.f / total : 0.f;
     if (!counts) acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lane * 4 < D)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + b * p.os[0] + h * p.os[1] + tok * p.os[2] + lane * 4) =
+    if (d < D)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + b * p.os[0] + h * p.os[1] + tok * p.os[2] + d) =
           make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
   };
-  auto add = [](float4& acc, const float4& v, float f) {
-    acc.x = fmaf(v.x, f, acc.x);
-    acc.y = fmaf(v.y, f, acc.y);
-    acc.z = fmaf(v.z, f, acc.z);
-    acc.w = fmaf(v.w, f, acc.w);
-  };
-  // The warps' parts of a row, relative to their largest reference.
-  for (int r = warp; r < n_rows; r += kWarps) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = max_nan(top, m_s[w][r]);
-    float total = 0.f;
+  // The warps' parts of a row.
+  for (int r = warp; r < n_rows; r += n_warps) {
+    const bool has = lane < n_warps;
+    const Joint j = join_references(has ? m_s[lane & 7][r] : -INFINITY, has ? l_s[lane & 7][r] : 0.f);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (m_s[w][r] == -INFINITY) continue;
-      const float f = fast_exp2(m_s[w][r] - top);
-      total = fmaf(l_s[w][r], f, total);
-      if (lane * 4 < D) add(acc, *reinterpret_cast<const float4*>(join + (w * kTile + r) * kJoinStride + lane * 4), f);
+    for (int w = 0; w < kMostWarps; ++w) {
+      const float f = __shfl_sync(0xffffffffu, j.factor, w);
+      if (f != 0.f && d < D) add_weighted(acc, *reinterpret_cast<const float4*>(join + (w * kTile + r) * kJoinStride + d), f);
     }
     if (alone) {
-      write(r, acc, total);
+      write(r, acc, j.total);
     } else {
       __syncwarp();
-      if (lane * 4 < D) *reinterpret_cast<float4*>(join + r * kJoinStride + lane * 4) = acc;  // this row's first part, read above
+      if (d < D) *reinterpret_cast<float4*>(join + r * kJoinStride + d) = acc;  // this row's first part, read above
       if (lane == 0) {
-        top_s[r] = top;
-        total_s[r] = total;
+        top_s[r] = j.top;
+        total_s[r] = j.total;
       }
     }
   }
   if (alone) return;
   // The CTAs' parts: each CTA joins its share of the rows.
   cluster.sync();
-  for (int r = rank * kWarps + warp; r < n_rows; r += n_ranks * kWarps) {
-    float top = -INFINITY;
-    for (int c = 0; c < n_ranks; ++c) top = max_nan(top, *cluster.map_shared_rank(&top_s[r], c));
-    float total = 0.f;
+  for (int r = first; r < n_rows; r += stride) {
+    const bool has = lane < n_ranks;
+    const Joint j = join_references(has ? *cluster.map_shared_rank(&top_s[r], lane) : -INFINITY,
+                                    has ? *cluster.map_shared_rank(&total_s[r], lane) : 0.f);
+    float4 v[kMostRanks];
+#pragma unroll
+    for (int c = 0; c < kMostRanks; ++c)
+      if (c < n_ranks && d < D) v[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(join + r * kJoinStride + d, c));
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < n_ranks; ++c) {
-      const float ref = *cluster.map_shared_rank(&top_s[r], c);
-      if (ref == -INFINITY) continue;
-      const float f = fast_exp2(ref - top);
-      total = fmaf(*cluster.map_shared_rank(&total_s[r], c), f, total);
-      if (lane * 4 < D)
-        add(acc, *reinterpret_cast<const float4*>(cluster.map_shared_rank(join + r * kJoinStride + lane * 4, c)), f);
+#pragma unroll
+    for (int c = 0; c < kMostRanks; ++c) {
+      const float f = __shfl_sync(0xffffffffu, j.factor, c);
+      if (f != 0.f && d < D) add_weighted(acc, v[c], f);
     }
-    write(r, acc, total);
+    write(r, acc, j.total);
   }
   cluster.sync();  // nobody leaves while others read its sums
 }
@@ -531,7 +591,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   int32_t sum = 0;
   for (int32_t b = first; b < min(first + run, p.batch); ++b) {
     before[b] = sum;
-    sum += tile_view<kTile>(p, b, 0).n_slices;
+    sum += tile_view<kTile, L::kStep>(p, b, 0).n_slices;
   }
   int32_t scan = sum;
 #pragma unroll
@@ -575,7 +635,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   out.grp = rest / out.n;
   out.slice = rest - out.grp * out.n;
   Cursor in = out;
-  View view = tile_view<kTile>(p, in.b, 0), view_in = view;
+  View view = tile_view<kTile, L::kStep>(p, in.b, 0), view_in = view;
   // To the next slice; true where that is another item's.
   auto advance = [&](Cursor& c, View& v) {
     if (++c.slice < c.n) return false;
@@ -586,12 +646,12 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
         ++c.b;
         c.n = before[c.b + 1] - before[c.b];
       } while (c.n == 0);
-      v = tile_view<kTile>(p, c.b, 0);
+      v = tile_view<kTile, L::kStep>(p, c.b, 0);
     }
     return true;
   };
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  Feed<DP, FULL> feed(p, ring, seen_s[warp]);
+  Feed<DP, FULL> feed(p, ring, NS, seen_s[warp]);
   feed.enter(in.b, in.grp);
   int32_t next_page = -1;
   uint32_t next_row = 0;
@@ -617,7 +677,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * kStep, seen_s[warp][at]);
+    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * L::kStep, seen_s[warp][at]);
     __syncwarp();
     issue();
     if (i + 1 < mine && out.slice + 1 < out.n) {
@@ -652,7 +712,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
 // warps are joined in order.  Lane l holds the weight of its warp's l-th part, so that the parts'
 // values are loaded without waiting for one another.
 template <bool BF16, int WPR>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(WPR > 4 ? WPR * 32 : 128)
 paged_combine_kernel(const PagedParams p, const Parts parts, int32_t tile) {
   __shared__ float4 acc_s[WPR][32];
   __shared__ float total_s[WPR];
@@ -716,7 +776,6 @@ paged_combine_kernel(const PagedParams p, const Parts parts, int32_t tile) {
         make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
 }
 
-constexpr int64_t kPlanSms = 148;
 constexpr int64_t kMaxSize = int64_t(1) << 30;
 
 // Unit stride along D, 16-byte rows, positive strides that are multiples of 16 bytes below 2^40 bytes.
@@ -740,16 +799,18 @@ struct Plan {
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Largest number of states that a row can see, from what the host knows.
-int64_t most_states(const paged_attention_args* a) {
-  const int64_t capacity = a->table_width * a->page_size;
-  return a->window > 0 ? std::min(capacity, a->window + a->sinks + a->queries) : capacity;
+// Largest number of slices of a tile of `tokens` tokens, from what the host knows.
+int64_t most_slices(const paged_attention_args* a, int64_t tokens) {
+  const int64_t kStep = a->head_dim <= 64 ? Shape<64>::kStep : Shape<128>::kStep;
+  const int64_t all = (a->table_width * a->page_size + kStep - 1) / kStep;
+  // window + tokens - 1 states in a row touch less than two slices more than they fill
+  return a->window > 0 ? std::min(all, (a->sinks + kStep - 1) / kStep + (a->window + tokens) / kStep + 2) : all;
 }
 
 Plan plan(const paged_attention_args* a) {
   Plan x{};
   const int64_t rows = a->heads / a->groups * a->queries, items = a->batch * a->groups;
-  const int64_t slices = most_states(a) / kStep + 3;
+  const int64_t slices = most_slices(a, a->queries);
   // One tile a key head, prefix sums that fit, 32-bit slice numbers.
   const bool able = rows <= 16 && a->batch <= kPartsBatch && items * slices <= INT32_MAX - 2 * kPartsAll;
   x.parts = able && (a->kernel == PAGED_KERNEL_PARTS || (a->kernel == PAGED_KERNEL_AUTO && items * slices >= kPartsAll * 2));
@@ -763,28 +824,31 @@ Plan plan(const paged_attention_args* a) {
 }
 
 template <int DP, bool FULL, bool BF16, int NT>
-int32_t launch_joined(PagedParams p, cudaStream_t stream) {
-  constexpr int W = 4;
+int32_t launch_joined(PagedParams p, int64_t slices, cudaStream_t stream) {
   using L = Shape<DP>;
-  auto kernel = paged_joined_kernel<DP, FULL, BF16, NT, W>;
-  constexpr int kRing = W * L::kWarpRing, kJoin = W * 8 * NT * (DP + 4) * 4;
-  constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kAlign;
-  static_assert(kSmem <= 224 * 1024, "shared memory of a CTA");
+  auto kernel = paged_joined_kernel<DP, FULL, BF16, NT>;
+  constexpr int kSlice = 2 * L::kSliceBytes, kJoin = 8 * NT * (DP + 4) * 4;  // of a warp
+  constexpr int kMost = kMostWarps * std::max(L::kStages * kSlice, kJoin) + kAlign;
+  static_assert(kMost <= 224 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
-  if (!allow_smem(kernel, kSmem, done)) return INTP_ERR_LAUNCH;
+  if (!allow_smem(kernel, kMost, done)) return INTP_ERR_LAUNCH;
   p.n_rt = (p.rows + 8 * NT - 1) / (8 * NT);
   const int64_t items = static_cast<int64_t>(p.n_rt) * p.batch * p.groups;
-  int ranks = 1;
-  while (ranks < 8 && items * ranks * 2 <= 2 * kPlanSms) ranks *= 2;
+  // Eight warps an SM hold the memory: an item gets the power of two of warps that leaves all of them
+  // at work, in CTAs of eight.
+  int warps = 1, ranks = 1;
+  while (warps < kMostWarps && items * warps * 2 <= kPartsAll) warps *= 2;
+  while (warps == kMostWarps && ranks < kMostRanks && items * ranks * 2 <= (ranks == 1 ? 144 : ranks == 2 ? 128 : 112)) ranks *= 2;
   if (items * ranks > INT32_MAX) return INTP_ERR_SHAPE;
+  p.depth = static_cast<int32_t>(std::min<int64_t>(L::kStages, (slices + warps * ranks - 1) / (warps * ranks)));
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = static_cast<unsigned>(ranks);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(W * 32);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.blockDim = dim3(static_cast<unsigned>(warps * 32));
+  cfg.dynamicSmemBytes = static_cast<size_t>(warps * std::max(p.depth * kSlice, kJoin) + kAlign);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -803,27 +867,30 @@ int32_t launch_parts(PagedParams p, const Parts& parts, cudaStream_t stream) {
   if (!launch_kernel(kernel, dim3(kPartsCtas), kPartsWarps * 32, kRing + kAlign + (p.batch + 1) * 4, stream, false, p, parts))
     return INTP_ERR_LAUNCH;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.queries;
-  // Few items have many parts each: a CTA per row, whose four warps share them.
-  const bool many = static_cast<int64_t>(p.batch) * p.groups * 8 <= kPartsAll;
-  auto combine = many ? paged_combine_kernel<BF16, 4> : paged_combine_kernel<BF16, 1>;
-  const int64_t grid = many ? rows : (rows + 3) / 4;
-  return launch_kernel(combine, dim3(static_cast<unsigned>(grid)), 128, 0, stream, true, p, parts, 8 * NT) ? INTP_OK
-                                                                                                        : INTP_ERR_LAUNCH;
+  // Few items have many parts each: a CTA per row, whose warps share them.
+  const int64_t each = kPartsAll / (static_cast<int64_t>(p.batch) * p.groups);
+  const int wide = each >= 64 ? 16 : each >= 16 ? 4 : 1;
+  auto combine = wide == 16 ? paged_combine_kernel<BF16, 16> : wide == 4 ? paged_combine_kernel<BF16, 4> : paged_combine_kernel<BF16, 1>;
+  const int64_t grid = wide > 1 ? rows : (rows + 3) / 4;
+  return launch_kernel(combine, dim3(static_cast<unsigned>(grid)), wide == 16 ? 512 : 128, 0, stream, true, p, parts, 8 * NT)
+             ? INTP_OK
+             : INTP_ERR_LAUNCH;
 }
 
 template <int DP, bool FULL, bool BF16>
-int32_t launch_rows(const PagedParams& p, const Parts* parts, cudaStream_t stream) {
+int32_t launch_rows(const PagedParams& p, const Parts* parts, int64_t slices, cudaStream_t stream) {
   if (parts != nullptr)
     return p.rows <= 8 ? launch_parts<DP, FULL, BF16, 1>(p, *parts, stream) : launch_parts<DP, FULL, BF16, 2>(p, *parts, stream);
-  return p.rows <= 8 ? launch_joined<DP, FULL, BF16, 1>(p, stream) : launch_joined<DP, FULL, BF16, 2>(p, stream);
+  return p.rows <= 8 ? launch_joined<DP, FULL, BF16, 1>(p, slices, stream) : launch_joined<DP, FULL, BF16, 2>(p, slices, stream);
 }
 
 // Head dims that fill their slices' rows need no checks of columns.
 template <bool BF16>
-int32_t launch_dim(const PagedParams& p, const Parts* parts, cudaStream_t stream) {
-  if (p.head_dim == 64) return launch_rows<64, true, BF16>(p, parts, stream);
-  if (p.head_dim == 128) return launch_rows<128, true, BF16>(p, parts, stream);
-  return p.head_dim < 64 ? launch_rows<64, false, BF16>(p, parts, stream) : launch_rows<128, false, BF16>(p, parts, stream);
+int32_t launch_dim(const PagedParams& p, const Parts* parts, int64_t slices, cudaStream_t stream) {
+  if (p.head_dim == 64) return launch_rows<64, true, BF16>(p, parts, slices, stream);
+  if (p.head_dim == 128) return launch_rows<128, true, BF16>(p, parts, slices, stream);
+  return p.head_dim < 64 ? launch_rows<64, false, BF16>(p, parts, slices, stream)
+                         : launch_rows<128, false, BF16>(p, parts, slices, stream);
 }
 
 intp_status check_shape(const paged_attention_args* a) {
@@ -905,7 +972,8 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
     parts.plan = reinterpret_cast<int32_t*>(ws + how.o_bytes + how.ml_bytes);
   }
   const Parts* x = how.parts ? &parts : nullptr;
-  return a->dtype == INTP_BF16 ? launch_dim<true>(p, x, stream) : launch_dim<false>(p, x, stream);
+  const int64_t tokens = std::min<int64_t>(a->queries, 16), slices = most_slices(a, tokens);  // a tile has 16 rows at most
+  return a->dtype == INTP_BF16 ? launch_dim<true>(p, x, slices, stream) : launch_dim<false>(p, x, slices, stream);
 }
 
 }  // namespace

@@ -807,13 +807,37 @@ int64_t most_slices(const paged_attention_args* a, int64_t tokens) {
   return a->window > 0 ? std::min(all, (a->sinks + kStep - 1) / kStep + (a->window + tokens) / kStep + 2) : all;
 }
 
+// Warps and CTAs of an item in one launch.  Eight warps an SM hold the memory: an item gets the power of
+// two of warps that leaves all of them at work, in CTAs of eight.  A cluster of eight (or four, two) CTAs
+// that fill an SM each wants its SMs in one part of the GPU: 14, 32 and 72 of them find their place at
+// once (B2 G8, 16 items: clusters of four 5.3 us, of eight 6.8).
+struct Team {
+  int warps, ranks;
+};
+Team team(int64_t items) {
+  Team t{1, 1};
+  while (t.warps < kMostWarps && items * t.warps * 2 <= kPartsAll) t.warps *= 2;
+  while (t.warps == kMostWarps && t.ranks < kMostRanks &&
+         items * t.ranks * 2 <= (t.ranks == 1 ? 144 : t.ranks == 2 ? 128 : 112))
+    t.ranks *= 2;
+  return t;
+}
+
 Plan plan(const paged_attention_args* a) {
   Plan x{};
   const int64_t rows = a->heads / a->groups * a->queries, items = a->batch * a->groups;
   const int64_t slices = most_slices(a, a->queries);
+  // A second launch costs 3 to 4 us; what it saves are warps that wait for others.  Equal parts are taken
+  // where a warp would have more than 125 slices, or 24 while less than half of the warps are at work.
+  // One launch / parts, D128: B32 G8 of 4000 states (63 slices a warp) 68 / 70 us, of 8000 (125) 130 / 126,
+  // B64 G8 of 8192 (256) 257 / 239; B1 G8 of 16000 (16, 512 warps) 16.1 / 17.5, of 32000 (31) 25.9 / 24.4,
+  // of 131071 118 / 89.
+  const Team t = team(items);
+  const int64_t each = (slices + t.warps * t.ranks - 1) / (t.warps * t.ranks);
+  const bool better = each > 125 || (each >= 24 && items * t.warps * t.ranks * 2 < kPartsAll);
   // One tile a key head, prefix sums that fit, 32-bit slice numbers.
   const bool able = rows <= 16 && a->batch <= kPartsBatch && items * slices <= INT32_MAX - 2 * kPartsAll;
-  x.parts = able && (a->kernel == PAGED_KERNEL_PARTS || (a->kernel == PAGED_KERNEL_AUTO && items * slices >= kPartsAll * 2));
+  x.parts = able && (a->kernel == PAGED_KERNEL_PARTS || (a->kernel == PAGED_KERNEL_AUTO && better));
   if (x.parts) {
     const int64_t slots = (kPartsAll + items) * tile_rows(rows);
     x.o_bytes = align256(slots * a->head_dim * 4);
@@ -834,11 +858,8 @@ int32_t launch_joined(PagedParams p, int64_t slices, cudaStream_t stream) {
   if (!allow_smem(kernel, kMost, done)) return INTP_ERR_LAUNCH;
   p.n_rt = (p.rows + 8 * NT - 1) / (8 * NT);
   const int64_t items = static_cast<int64_t>(p.n_rt) * p.batch * p.groups;
-  // Eight warps an SM hold the memory: an item gets the power of two of warps that leaves all of them
-  // at work, in CTAs of eight.
-  int warps = 1, ranks = 1;
-  while (warps < kMostWarps && items * warps * 2 <= kPartsAll) warps *= 2;
-  while (warps == kMostWarps && ranks < kMostRanks && items * ranks * 2 <= (ranks == 1 ? 144 : ranks == 2 ? 128 : 112)) ranks *= 2;
+  const Team t = team(items);
+  const int warps = t.warps, ranks = t.ranks;
   if (items * ranks > INT32_MAX) return INTP_ERR_SHAPE;
   p.depth = static_cast<int32_t>(std::min<int64_t>(L::kStages, (slices + warps * ranks - 1) / (warps * ranks)));
   cudaLaunchAttribute attr{};

@@ -25,11 +25,10 @@ import struct
 import torch
 
 from . import _lib
-from .cross_attention import (_HALF, _MAX_STRIDE, _call, _check_counts, _check_scale, _keep, _output, _plans, _ready,
-                              _refuse_grad, _scratch_bytes)
+from .cross_attention import (_HALF, _MAX_STRIDE, _call, _check_counts, _check_scale, _keep, _laid_out, _output, _plans,
+                              _ready, _refuse_grad, _scratch_bytes)
 from .look_attention import _DTYPE_CODE
-from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _check_rotary, _rows_laid_out, _rows_ready,
-                     _set_rotary)
+from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _check_rotary, _rows_laid_out, _set_rotary)
 
 _ATTENTION_POINTERS = struct.Struct("9Q")  # paged_attention_args up to the sizes
 _MAX_STATES = 1 << 30
@@ -90,10 +89,26 @@ class PagedCache:
     def shape(self) -> tuple[int, ...]:
         return tuple(self._keys.shape)
 
-    def _append_tail(self, q, k, v, q_out, page_table, rotary, positions) -> bytes:
-        """Checks an append and returns its argument block behind the pointers."""
+    def _append_plan(self, q, k, v, page_table, start, counts, rotary, positions) -> bytes:
+        """Checks an append of laid out tensors; its argument block behind the pointers."""
+        args = _lib.RotaryArgs()
+        args.batch, args.groups, args.rows, args.head_dim = k.shape
+        args.k_stride, args.v_stride = k.stride(), v.stride()
+        args.k_out_stride = args.v_out_stride = self._keys.stride()
+        if q is not None:
+            args.heads = q.shape[1]
+            args.q_stride, args.q_out_stride = q.stride(), torch.empty_like(q, device="meta").stride()
+        args.pages, _, args.page_size, _ = self._keys.shape
+        args.table_width, args.table_stride = page_table.shape[1], page_table.stride(0)
+        args.dtype = _DTYPE_CODE[k.dtype]
+        if rotary is not None:
+            _set_rotary(args, rotary, positions)
+        return bytes(args)[_POINTERS.size:]
+
+    def _append_inputs(self, q, k, v, page_table, start, counts, rotary, positions):
+        """Checks a call and returns its tensors as the kernel takes them."""
         what = "a paged cache"
-        pages, groups, page_size, head_dim = self._keys.shape
+        _, groups, page_size, head_dim = self._keys.shape
         for name, t in (("k", k), ("v", v), ("q", q)):
             if t is None:
                 continue
@@ -102,25 +117,16 @@ class PagedCache:
                 raise ValueError(f"{name} must have the cache's dtype and device")
             if t.shape[0] != k.shape[0] or t.shape[2:] != (k.shape[2], head_dim) or (name != "q" and t.shape[1] != groups):
                 raise ValueError("k and v must have shape (B, G, n, D) and q (B, H, n, D) with the cache's G and D")
-        _check_table(page_table, k.shape[0], page_size, k.device)
-        args = _lib.RotaryArgs()
-        args.batch, args.groups, args.rows, args.head_dim = k.shape
-        args.k_stride, args.v_stride = k.stride(), v.stride()
-        args.k_out_stride, args.v_out_stride = self._keys.stride(), self._values.stride()
-        if q is not None:
-            args.heads = q.shape[1]
-            args.q_stride, args.q_out_stride = q.stride(), q_out.stride()
-        args.pages, args.page_size = pages, page_size
-        args.table_width, args.table_stride = page_table.shape[1], page_table.stride(0)
-        args.dtype = _DTYPE_CODE[k.dtype]
+        batch, device = k.shape[0], k.device
+        page_table = _table(page_table, batch, page_size, device)
         if rotary is not None:
-            _check_rotary(rotary, head_dim, k.device)
+            _check_rotary(rotary, head_dim, device)
             if positions is not None:
-                _check_positions(positions, k.shape[0], k.shape[2], max(rotary.axes) + 1, k.device)
-            _set_rotary(args, rotary, positions)
+                _check_positions(positions, batch, k.shape[2], max(rotary.axes) + 1, device)
         elif q is not None or positions is not None:
             raise ValueError("q and positions are for a rotation: pass rotary too")
-        return bytes(args)[_POINTERS.size:]
+        return (None if q is None else _rows_laid_out(q), _rows_laid_out(k), _rows_laid_out(v), page_table,
+                _check_counts(start, batch, device, "start"), _check_counts(counts, batch, device, "counts"))
 
     def append(self, k, v, *, page_table, start, counts=None, rotary=None, positions=None, q=None):
         """Row i of ``k``, ``v`` ``(B, G, n, D)`` to state ``start[b] + i`` of sequence b for
@@ -132,48 +138,60 @@ class PagedCache:
         the state's number on every axis; ``q`` ``(B, H, n, D)`` is turned likewise, every
         row of it, and returned.  Two rows that go to the same row of the pool leave it
         unspecified."""
-        for t in (k, v) + (() if q is None else (q,)):
-            if not isinstance(t, torch.Tensor):
-                raise ValueError("a paged cache requires CUDA tensors")
+        _check_tensors("a paged cache", k, v, page_table, start, q, counts)
         if rotary is not None and not isinstance(rotary, RotaryAxes):
             raise ValueError("rotary must be a RotaryAxes")
         if positions is not None and not isinstance(positions, torch.Tensor):
             raise ValueError("positions must be a tensor")
         _refuse_grad("a paged cache", k, v, q, positions)
-        page_table = _table(page_table)
-        k, v = _rows_laid_out(k), _rows_laid_out(v)
-        q_out = None
-        if q is not None:
-            q = _rows_laid_out(q)
-            q_out = torch.empty_like(q)
         key = ("append", self._layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
-               page_table.shape, page_table.stride(), page_table.device,
-               None if q is None else (q.shape, q.stride(), q.dtype, q.device),
+               page_table.shape, page_table.stride(), page_table.dtype, page_table.device, start.shape, start.stride(),
+               start.dtype, start.device, None if q is None else (q.shape, q.stride(), q.dtype, q.device),
+               None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.device),
                None if rotary is None else rotary._layout,
                None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device))
         tail = _plans.get(key)
-        if tail is None:
-            tail = self._append_tail(q, k, v, q_out, page_table, rotary, positions)
-            _keep(key, tail)
-        device = self._keys.device
-        start = _check_counts(start, k.shape[0], device, "start")
-        if start is None:
-            raise ValueError("start must be an int32 or int64 tensor of shape (B,)")
-        counts = _check_counts(counts, k.shape[0], device, "counts")
-        block = _POINTERS.pack(0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                               0 if q is None else q_out.data_ptr(), self._keys.data_ptr(), self._values.data_ptr(),
-                               0 if rotary is None else rotary._turns.data_ptr(),
-                               0 if rotary is None else rotary._axis.data_ptr(),
+        k_at, v_at, q_at = k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr()
+        if tail is None or (k_at | v_at | q_at) & 15:
+            given = (q, k, v, page_table, start, counts)
+            taken = self._append_inputs(*given, rotary, positions)
+            if any([a is not b for a, b in zip(given, taken)]):
+                q, k, v, page_table, start, counts = taken
+                return self.append(k, v, page_table=page_table, start=start, counts=counts, rotary=rotary,
+                                   positions=positions, q=q)
+            tail = _keep(key, self._append_plan(*given, rotary, positions))
+        q_out, q_to = None, 0
+        if q is not None:
+            q_out = torch.empty_like(q)
+            q_to = q_out.data_ptr()
+        turns, axis = (0, 0) if rotary is None else rotary._pointers
+        block = _POINTERS.pack(q_at, k_at, v_at, q_to, self._keys.data_ptr(), self._values.data_ptr(), turns, axis,
                                0 if positions is None else positions.data_ptr(), start.data_ptr(),
                                0 if counts is None else counts.data_ptr(), page_table.data_ptr()) + tail
-        _call(_lib.load().paged_cache_append, block, device.index, "paged cache append")
+        _call(_lib.load().paged_cache_append, block, self._keys.device.index, "paged cache append")
         return q_out
 
 
-def _table(page_table) -> torch.Tensor:
+def _check_tensors(what: str, *tensors) -> None:
+    """The first four are tensors, the others may be None."""
+    for i, t in enumerate(tensors):
+        if not (isinstance(t, torch.Tensor) or (i > 3 and t is None)):
+            raise ValueError((f"{what} requires CUDA tensors", f"{what} requires CUDA tensors",
+                              "page_table must be an int32 or int64 tensor of shape (B, width)",
+                              "start must be an int32 or int64 tensor of shape (B,)", f"{what} requires CUDA tensors",
+                              "counts must be an int32 or int64 tensor of shape (B,)")[i])
+
+
+def _table(page_table, batch: int, page_size: int, device) -> torch.Tensor:
     """The page table as the kernels take it: int32, unit stride along a sequence's pages."""
-    if not isinstance(page_table, torch.Tensor) or page_table.ndim != 2 or page_table.dtype not in (torch.int32, torch.int64):
+    if page_table.ndim != 2 or page_table.dtype not in (torch.int32, torch.int64):
         raise ValueError("page_table must be an int32 or int64 tensor of shape (B, width)")
+    if page_table.shape[0] != batch:
+        raise ValueError("page_table must have a row for each sequence")
+    if page_table.shape[1] < 1 or page_table.shape[1] * page_size > _MAX_STATES:
+        raise ValueError("page_table must name at least one page and at most 2^30 states a sequence")
+    if page_table.device != device:
+        raise ValueError("page_table must be on the same CUDA device as q")
     if page_table.dtype == torch.int64:
         page_table = page_table.clamp(-1, 2147483647).to(torch.int32)
     strides = page_table.stride()
@@ -182,46 +200,45 @@ def _table(page_table) -> torch.Tensor:
     return page_table
 
 
-def _check_table(page_table, batch: int, page_size: int, device) -> None:
-    if page_table.shape[0] != batch:
-        raise ValueError("page_table must have a row for each sequence")
-    if page_table.shape[1] < 1 or page_table.shape[1] * page_size > _MAX_STATES:
-        raise ValueError("page_table must name at least one page and at most 2^30 states a sequence")
-    if page_table.device != device:
-        raise ValueError("page_table must be on the same CUDA device as q")
-
-
-def _attention_tail(q, cache: PagedCache, page_table, scale, window, sinks, out_stride, kernel):
-    """Checks a call; its argument block behind the pointers and its scratch bytes."""
+def _attention_inputs(q, cache: PagedCache, page_table, start, counts, out):
+    """Checks a call and returns its tensors as the kernels take them."""
     what = "paged attention"
     _check_heads(q, "q", what, _HALF)
-    pages, groups, page_size, head_dim = cache._keys.shape
+    _, groups, page_size, head_dim = cache._keys.shape
     if q.dtype != cache._keys.dtype or q.device != cache._keys.device:
         raise ValueError("q must have the cache's dtype and device")
     if q.shape[3] != head_dim:
         raise ValueError("q and the cache must share head_dim")
     if q.shape[1] < 1 or q.shape[1] % groups:
         raise ValueError("the query heads must be a multiple of the key heads")
-    _check_table(page_table, q.shape[0], page_size, q.device)
+    if out is not None:
+        _output(q, out)
+    return (_laid_out(q), _table(page_table, q.shape[0], page_size, q.device),
+            _check_counts(start, q.shape[0], q.device, "start"), _check_counts(counts, q.shape[0], q.device, "counts"))
+
+
+def _attention_plan(q, cache: PagedCache, page_table, scale, window, sinks, kernel, out):
+    """Checks the numbers of a call; its argument block behind the pointers, its scratch bytes."""
     if window is not None and not 1 <= window <= _MAX_STATES:
         raise ValueError("window must be at least 1 (None: the whole sequence)")
     if not 0 <= sinks <= _MAX_STATES:
         raise ValueError("sinks must not be negative")
     if sinks and window is None:
         raise ValueError("sinks are the states that stay visible beside a window: pass window too")
+    if kernel not in _KERNELS:
+        raise ValueError(f"kernel must be one of {sorted(_KERNELS)}")
     args = _lib.PagedAttentionArgs()
     args.batch, args.heads, args.queries, args.head_dim = q.shape
-    args.groups, args.pages, args.page_size = groups, pages, page_size
-    args.q_stride, args.out_stride = q.stride(), out_stride
+    args.pages, args.groups, args.page_size, _ = cache._keys.shape
+    args.q_stride = q.stride()
+    args.out_stride = (torch.empty_like(q, device="meta") if out is None else out).stride()
     args.cache_stride = cache._keys.stride()
     args.table_width, args.table_stride = page_table.shape[1], page_table.stride(0)
     args.window, args.sinks = window or 0, sinks
     args.scale = _check_scale(scale)
     args.dtype = _DTYPE_CODE[q.dtype]
-    if kernel not in _KERNELS:
-        raise ValueError(f"kernel must be one of {sorted(_KERNELS)}")
     args.kernel = _KERNELS[kernel]
-    scratch = _scratch_bytes(_lib.load().paged_attention_workspace, args, what)
+    scratch = _scratch_bytes(_lib.load().paged_attention_workspace, args, "paged attention")
     return bytes(args)[_ATTENTION_POINTERS.size:], scratch
 
 
@@ -233,7 +250,8 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
     and with its own; with ``window`` only the last ``window`` of them, and the
     sequence's first ``sinks`` states.  Query head h reads key head ``h // (H / G)``.
     Rows from ``counts[b]`` on (all M count without it) and rows that see nothing give
-    zeros; states that a row does not see take no part whatever they hold.
+    zeros; states that a row does not see take no part whatever they hold.  The result
+    is laid out like ``q`` unless ``out`` is given.
 
     Made for few rows: the states are read once for every 16 rows (tokens times
     ``H / G``) of a key head.  fp32 sums and statistics; the result is rounded once.
@@ -243,25 +261,26 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
     what = "paged attention"
     if not isinstance(cache, PagedCache):
         raise ValueError("cache must be a PagedCache")
-    if not isinstance(q, torch.Tensor):
-        raise ValueError(f"{what} requires CUDA tensors")
+    _check_tensors(what, q, q, page_table, start, None, counts)
     _refuse_grad(what, q)
-    page_table = _table(page_table)
     scale, window, sinks = float(scale), None if window is None else int(window), int(sinks)
-    if not _ready(q):
-        q = q.clone(memory_format=torch.contiguous_format)
-    out = _output(q, out) if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, q.device, page_table.shape, page_table.stride(),
-           page_table.device, scale, window, sinks, out.stride(), kernel)
-    plan = _plans.get(key)
-    if plan is None:
-        plan = _keep(key, _attention_tail(q, cache, page_table, scale, window, sinks, out.stride(), kernel))
-    tail, scratch_bytes = plan
     device = q.device
-    start = _check_counts(start, q.shape[0], device, "start")
-    if start is None:
-        raise ValueError("start must be an int32 or int64 tensor of shape (B,)")
-    counts = _check_counts(counts, q.shape[0], device, "counts")
+    key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, device, page_table.shape, page_table.stride(),
+           page_table.dtype, page_table.device, start.shape, start.stride(), start.dtype, start.device,
+           None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.device), scale, window, sinks,
+           kernel, None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+    plan = _plans.get(key)
+    if plan is None or (q.data_ptr() | (0 if out is None else out.data_ptr())) & 15:
+        given = (q, page_table, start, counts)
+        taken = _attention_inputs(q, cache, page_table, start, counts, out)
+        if any([a is not b for a, b in zip(given, taken)]):
+            q, page_table, start, counts = taken
+            return paged_attention(q, cache, page_table=page_table, start=start, scale=scale, counts=counts, window=window,
+                                   sinks=sinks, kernel=kernel, out=out)
+        plan = _keep(key, _attention_plan(q, cache, page_table, scale, window, sinks, kernel, out))
+    tail, scratch_bytes = plan
+    if out is None:
+        out = torch.empty_like(q)
     space = 0
     if scratch_bytes:
         scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)  # from the current stream's pool

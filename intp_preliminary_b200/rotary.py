@@ -57,6 +57,7 @@ class RotaryAxes:
         self._turns = turns.to(self._device)
         self._axis = torch.tensor(axes, dtype=torch.int32).to(self._device)
         self._device = self._turns.device
+        self._pointers = self._turns.data_ptr(), self._axis.data_ptr()
         self._frequencies, self._axes = tuple(frequencies), tuple(axes)
         self._interleaved = bool(interleaved)
         # what a call's checks and argument block depend on
@@ -152,8 +153,9 @@ def _set_rotary(args, rotary, positions) -> None:
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _tail(q, k, q_out, k_out, rotary, positions, inverse: bool) -> bytes:
-    """Checks a call and returns its argument block behind the pointers."""
+def _turn_plan(q, k, rotary, positions, inverse: bool):
+    """Checks a call and returns its argument block behind the pointers, or None when a tensor has to
+    be laid out first."""
     what = "rotate_positions"
     _check_heads(q, "q", what, _DTYPES)
     if k is not None:
@@ -162,12 +164,14 @@ def _tail(q, k, q_out, k_out, rotary, positions, inverse: bool) -> bytes:
             raise ValueError("q and k must share B, n, D, dtype and device")
     _check_rotary(rotary, q.shape[3], q.device)
     _check_positions(positions, q.shape[0], q.shape[2], max(rotary.axes) + 1, q.device)
+    if not (_rows_ready(q) and (k is None or _rows_ready(k))):
+        return None
     args = _lib.RotaryArgs()
     args.batch, args.heads, args.rows, args.head_dim = q.shape
-    args.q_stride, args.q_out_stride = q.stride(), q_out.stride()
+    args.q_stride, args.q_out_stride = q.stride(), torch.empty_like(q, device="meta").stride()
     if k is not None:
         args.groups = k.shape[1]
-        args.k_stride, args.k_out_stride = k.stride(), k_out.stride()
+        args.k_stride, args.k_out_stride = k.stride(), torch.empty_like(k, device="meta").stride()
     args.dtype = _DTYPE_CODE[q.dtype]
     args.inverse = int(inverse)
     _set_rotary(args, rotary, positions)
@@ -175,29 +179,31 @@ def _tail(q, k, q_out, k_out, rotary, positions, inverse: bool) -> bytes:
 
 
 def _rotate(q, k, rotary, positions, inverse: bool):
-    """q and k (or None) turned: one launch."""
+    """q and k (or None) turned: one launch.  What sizes, strides and types decide is kept by those alone."""
     if not isinstance(q, torch.Tensor) or not (k is None or isinstance(k, torch.Tensor)):
         raise ValueError("rotate_positions requires CUDA tensors")
     if not isinstance(rotary, RotaryAxes):
         raise ValueError("rotary must be a RotaryAxes")
     if not isinstance(positions, torch.Tensor):
         raise ValueError("positions must be a tensor")
-    if not _rows_ready(q):
-        q = _rows_laid_out(q)
-    if k is not None and not _rows_ready(k):
-        k = _rows_laid_out(k)
-    key = ("rotate", rotary._layout, q.shape, q.stride(), q.dtype, q.device, positions.shape, positions.stride(), positions.dtype,
-           positions.device, inverse, None if k is None else (k.shape, k.stride(), k.dtype, k.device))
-    q_out = torch.empty_like(q)
-    k_out = None if k is None else torch.empty_like(k)
+    device = q.device
+    key = ("rotate", rotary._layout, q.shape, q.stride(), q.dtype, device, positions.shape, positions.stride(),
+           positions.dtype, positions.device, inverse,
+           None if k is None else (k.shape, k.stride(), k.dtype, k.device))
     tail = _plans.get(key)
-    if tail is None:
-        tail = _tail(q, k, q_out, k_out, rotary, positions, inverse)
+    q_at, k_at = q.data_ptr(), 0 if k is None else k.data_ptr()
+    if tail is None or (q_at | k_at) & 15:
+        tail = _turn_plan(q, k, rotary, positions, inverse)
+        if tail is None:
+            return _rotate(_rows_laid_out(q), None if k is None else _rows_laid_out(k), rotary, positions, inverse)
         _keep(key, tail)
-    block = _POINTERS.pack(q.data_ptr(), 0 if k is None else k.data_ptr(), 0, q_out.data_ptr(),
-                           0 if k is None else k_out.data_ptr(), 0, rotary._turns.data_ptr(), rotary._axis.data_ptr(),
-                           positions.data_ptr(), 0, 0, 0) + tail
-    _call(_lib.load().rotary_positions, block, q.device.index, "rotate_positions")
+    q_out = torch.empty_like(q)
+    k_out, k_to = None, 0
+    if k is not None:
+        k_out = torch.empty_like(k)
+        k_to = k_out.data_ptr()
+    block = _POINTERS.pack(q_at, k_at, 0, q_out.data_ptr(), k_to, 0, *rotary._pointers, positions.data_ptr(), 0, 0, 0) + tail
+    _call(_lib.load().rotary_positions, block, device.index, "rotate_positions")
     return q_out, k_out
 
 
@@ -213,16 +219,18 @@ class _RotatePositions(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
-        (positions,) = ctx.saved_tensors
-        grads = [g if g is not None and n else None for g, n in zip((grad_q, grad_k), ctx.needs_input_grad)]
-        one, two = grads
-        if one is None and two is None:
-            return None, None, None, None, None
-        if one is None:
-            back, _ = rotate_positions(two, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)
-            return None, back, None, None, None
-        back = rotate_positions(one, two, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)
-        return back[0], back[1], None, None, None
+        positions, = ctx.saved_tensors
+        needs_q, needs_k = ctx.needs_input_grad[:2]
+        if not needs_q:
+            grad_q = None
+        if not needs_k or grad_k is None:
+            if grad_q is None:
+                return None, None, None, None, None
+            return rotate_positions(grad_q, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)[0], None, None, None, None
+        if grad_q is None:
+            return None, rotate_positions(grad_k, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)[0], None, None, None
+        return (*rotate_positions(grad_q, grad_k, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse), None,
+                None, None)
 
 
 def rotate_positions(q, k=None, *, rotary, positions, inverse: bool = False):
@@ -235,8 +243,9 @@ def rotate_positions(q, k=None, *, rotary, positions, inverse: bool = False):
     Inputs whose rows are not 16-byte aligned with unit stride along D are copied
     first; broadcast ones (stride zero) are not."""
     _refuse_transforms("rotate_positions", q, k, positions)
-    if isinstance(positions, torch.Tensor) and positions.requires_grad and torch.is_grad_enabled():
-        raise ValueError("positions have no gradient: detach them")
-    if torch.is_grad_enabled() and any([isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)]):
-        return _RotatePositions.apply(q, k, rotary, positions, bool(inverse))
+    if torch.is_grad_enabled():
+        if isinstance(positions, torch.Tensor) and positions.requires_grad:
+            raise ValueError("positions have no gradient: detach them")
+        if (isinstance(q, torch.Tensor) and q.requires_grad) or (isinstance(k, torch.Tensor) and k.requires_grad):
+            return _RotatePositions.apply(q, k, rotary, positions, bool(inverse))
     return _rotate(q, k, rotary, positions, bool(inverse))

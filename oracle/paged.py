@@ -2,9 +2,11 @@
 cache, attention of new tokens over it, and elementwise error bounds for the kernels.
 
 Where a kernel may round, with u the unit roundoff of the output type (half its eps):
-  turned values: the angle is a 64-bit product (2 roundings of 2^-53 of it, one more here), its
-        reduced part is rounded to 32 bits (2^-24 of pi / 4 at most), sin and cos are within 2 units
-        in the last place (2^-24 each, below 1): 4 * 2^-24 + 3 * 2^-53 |t| of |x1| + |x2|.  Two fp32
+  turned values: the angle is a 64-bit product (2 roundings of 2^-53 of it, one more here); its
+        part within an eighth of a turn, x, is rounded to 32 bits and multiplied by 2 pi (2.7 * 2^-24 of
+        pi / 4 at most: 2.1 * 2^-24), sin x and cos x are sums of a power series whose first term left
+        out is 2e-9 (0.1 * 2^-24) and whose last sum is rounded to half of 2^-24, the terms before it
+        adding 0.7 * 2^-24 at most: below 4 * 2^-24 + 3 * 2^-53 |t| of |x1| + |x2|.  Two fp32
         products and a sum: 2 * 2^-24 more.  The result is rounded once: u |y| (f16: at most 2^-25
         below its normal range).
   attention: the bound of a kernel that multiplies each probability as two 16-bit numbers, as

@@ -65,9 +65,9 @@ constexpr int kPartsLeast = 2;             // slices of a part at least
 template <int DP>
 struct Shape {
   static constexpr int kChunks = DP * 2 / 16;
-  static constexpr int kStep = DP == 128 ? 16 : 32;        // keys of a slice: 8 KB of K and V
+  static constexpr int kStep = DP > 64 ? 16 : 32;          // keys of a slice
   static constexpr int kSliceBytes = kStep * DP * 2;       // K or V of a slice
-  static constexpr int kStages = 3;
+  static constexpr int kStages = DP == 32 ? 6 : 3;         // 24 KB a warp
   static constexpr int kWarpRing = kStages * 2 * kSliceBytes;
 };
 
@@ -235,17 +235,23 @@ struct Rows {
   }
 
   // One slice, keys from k0 on, of which the bits of `seen` are there.
-  __device__ __forceinline__ void step(const PagedParams& p, const View& view, uint32_t k_s, int32_t k0, uint32_t seen) {
+  // `meanwhile` runs while the first products are under way.
+  template <class Meanwhile>
+  __device__ __forceinline__ void step(const PagedParams& p, const View& view, uint32_t k_s, int32_t k0, uint32_t seen,
+                                       Meanwhile&& meanwhile) {
     constexpr float kShift = BF16 ? 0.f : 7.f, kTiny = BF16 ? 8.67361738e-19f : 5.96046448e-8f;  // 2^-60, 2^-24
     constexpr int kStep = Shape<DP>::kStep, KB = kStep / 16, kBlock = 16 * CH * 16;  // blocks of 16 keys, bytes of one
     constexpr uint32_t kAll = 0xffffffffu >> (32 - kStep);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mi = lane >> 3, mr = lane & 7;
     const int D = p.head_dim;
-    // Whether 16-column block c has columns below D; DP is the smallest of its kind that holds D.
-    auto inside = [&](int c) { return FULL || (DP == 128 && c < 4) || c * 16 < D; };
-    // Matrix addresses of chunk 0 and 1; further chunks differ in the bits that the permutation leaves apart.
+    // Whether 16-column block c has columns below D, which is above DP / 2 (DP 32: at least 8).
+    auto inside = [&](int c) { return FULL || c * 16 < DP / 2 || c * 16 < D; };
+    // Matrix addresses of chunk 0 or 1; further chunks differ in the bits that the permutation leaves apart.
     const uint32_t k_at = k_s + chunk_offset<CH>(mr + ((mi & 1) << 3), mi >> 1);
     const uint32_t v_at = k_s + Shape<DP>::kSliceBytes + chunk_offset<CH>(mr + ((mi >> 1) << 3), mi & 1);
+    // Two sums of products in turn where there is one block of keys and rows: a product waits for the one before it.
+    constexpr int KS = KB * NT == 1 ? 2 : 1;
+    float half[4] = {0.f, 0.f, 0.f, 0.f};
     float s[KB][NT][4];                     // rows 2t, 2t+1 (e & 1), keys g, g + 8 (e >> 1)
 #pragma unroll
     for (int k = 0; k < KB; ++k)
@@ -261,9 +267,11 @@ struct Rows {
         uint32_t r[4];                      // keys 0-7 and 8-15 of chunk 2 kk, then of 2 kk + 1
         ldmatrix4((k_at + k * kBlock) ^ (kk * 32), r);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<BF16>(s[k][n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
+        for (int n = 0; n < NT; ++n)
+          mma16816<BF16>(KS == 2 && kk % 2 == 1 ? half : s[k][n], r[0], r[1], r[2], r[3], qb[n][kk][0], qb[n][kk][1]);
       }
     }
+    meanwhile();
     // Whether rows of the tile differ in what they see of the slice.
     const bool mixed = view.first_pos != view.last_pos &&
                        (k0 + kStep - 1 > view.first_pos ||
@@ -274,7 +282,7 @@ struct Rows {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[k][n][e] *= score_scale;
+        for (int e = 0; e < 4; ++e) s[k][n][e] = (KS == 2 ? s[k][n][e] + half[e] : s[k][n][e]) * score_scale;
     if (mixed || seen != kAll) {
 #pragma unroll
       for (int kh = 0; kh < 2 * KB; ++kh) {
@@ -492,9 +500,8 @@ paged_joined_kernel(const PagedParams p) {
   for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(first + i * stride) * L::kStep, seen_s[warp][at]);
-    __syncwarp();
-    issue();
+    // the slice before this one has been read by every lane: its place is filled again
+    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(first + i * stride) * L::kStep, seen_s[warp][at], issue);
   }
   cp_async_wait<0>();
   __syncthreads();  // every ring is at rest: the space takes the warps' sums
@@ -677,9 +684,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * L::kStep, seen_s[warp][at]);
-    __syncwarp();
-    issue();
+    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * L::kStep, seen_s[warp][at], issue);
     if (i + 1 < mine && out.slice + 1 < out.n) {
       ++out.slice;
       continue;
@@ -829,9 +834,9 @@ Plan plan(const paged_attention_args* a) {
   const int64_t slices = most_slices(a, a->queries);
   // A second launch costs 3 to 4 us; what it saves are warps that wait for others.  Equal parts are taken
   // where a warp would have more than 125 slices, or 24 while less than half of the warps are at work.
-  // One launch / parts, D128: B32 G8 of 4000 states (63 slices a warp) 68 / 70 us, of 8000 (125) 130 / 126,
-  // B64 G8 of 8192 (256) 257 / 239; B1 G8 of 16000 (16, 512 warps) 16.1 / 17.5, of 32000 (31) 25.9 / 24.4,
-  // of 131071 118 / 89.
+  // One launch / parts, D128: B32 G8 of 4000 states (63 slices a warp) 66 / 71 us, of 8000 (125) 127 / 131,
+  // B64 G8 of 8192 (256) 251 / 241, of 4096 with D80 (128) 104 / 90; B1 G8 of 16000 (16, 512 warps)
+  // 15.6 / 17.1, of 32000 (31) 24.7 / 24.0, of 131071 109 / 90.
   const Team t = team(items);
   const int64_t each = (slices + t.warps * t.ranks - 1) / (t.warps * t.ranks);
   const bool better = each > 125 || (each >= 24 && items * t.warps * t.ranks * 2 < kPartsAll);
@@ -908,10 +913,13 @@ int32_t launch_rows(const PagedParams& p, const Parts* parts, int64_t slices, cu
 // Head dims that fill their slices' rows need no checks of columns.
 template <bool BF16>
 int32_t launch_dim(const PagedParams& p, const Parts* parts, int64_t slices, cudaStream_t stream) {
-  if (p.head_dim == 64) return launch_rows<64, true, BF16>(p, parts, slices, stream);
-  if (p.head_dim == 128) return launch_rows<128, true, BF16>(p, parts, slices, stream);
-  return p.head_dim < 64 ? launch_rows<64, false, BF16>(p, parts, slices, stream)
-                         : launch_rows<128, false, BF16>(p, parts, slices, stream);
+  const int32_t d = p.head_dim;
+  if (d == 32) return launch_rows<32, true, BF16>(p, parts, slices, stream);
+  if (d == 64) return launch_rows<64, true, BF16>(p, parts, slices, stream);
+  if (d == 128) return launch_rows<128, true, BF16>(p, parts, slices, stream);
+  if (d < 32) return launch_rows<32, false, BF16>(p, parts, slices, stream);
+  if (d < 64) return launch_rows<64, false, BF16>(p, parts, slices, stream);
+  return launch_rows<128, false, BF16>(p, parts, slices, stream);
 }
 
 intp_status check_shape(const paged_attention_args* a) {

@@ -50,6 +50,8 @@ def _check_cache(keys, values) -> None:
         raise ValueError("a paged cache needs a page, a key head and a state")
     if keys.shape[3] % 8 or not 8 <= keys.shape[3] <= 128:
         raise ValueError("head_dim must be a multiple of 8 up to 128")
+    if keys.requires_grad or values.requires_grad:
+        raise ValueError("a paged cache takes no part in autograd: detach its tensors")
     if not (_ready(keys) and _ready(values)):
         raise ValueError("the cache's tensors need unit stride on head_dim and 16-byte aligned rows")
     if keys.stride() != values.stride():
@@ -138,11 +140,10 @@ class PagedCache:
         the state's number on every axis; ``q`` ``(B, H, n, D)`` is turned likewise, every
         row of it, and returned.  Two rows that go to the same row of the pool leave it
         unspecified."""
-        _check_tensors("a paged cache", k, v, page_table, start, q, counts)
         if rotary is not None and not isinstance(rotary, RotaryAxes):
             raise ValueError("rotary must be a RotaryAxes")
-        if positions is not None and not isinstance(positions, torch.Tensor):
-            raise ValueError("positions must be a tensor")
+        if not _all_tensors(k, v, page_table, start, q, counts, positions):
+            _check_tensors("a paged cache", k, v, page_table, start, q, counts, positions)
         _refuse_grad("a paged cache", k, v, q, positions)
         key = ("append", self._layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
                page_table.shape, page_table.stride(), page_table.dtype, page_table.device, start.shape, start.stride(),
@@ -172,14 +173,23 @@ class PagedCache:
         return q_out
 
 
+_Tensor = torch.Tensor
+
+
+def _all_tensors(one, two, three, four, *others) -> bool:
+    return (isinstance(one, _Tensor) and isinstance(two, _Tensor) and isinstance(three, _Tensor)
+            and isinstance(four, _Tensor) and all([t is None or isinstance(t, _Tensor) for t in others]))
+
+
 def _check_tensors(what: str, *tensors) -> None:
-    """The first four are tensors, the others may be None."""
-    for i, t in enumerate(tensors):
-        if not (isinstance(t, torch.Tensor) or (i > 3 and t is None)):
-            raise ValueError((f"{what} requires CUDA tensors", f"{what} requires CUDA tensors",
-                              "page_table must be an int32 or int64 tensor of shape (B, width)",
-                              "start must be an int32 or int64 tensor of shape (B,)", f"{what} requires CUDA tensors",
-                              "counts must be an int32 or int64 tensor of shape (B,)")[i])
+    """Says which of a call's arguments is no tensor; from the fifth on they may be None."""
+    what = f"{what} requires CUDA tensors"
+    messages = (what, what, "page_table must be an int32 or int64 tensor of shape (B, width)",
+                "start must be an int32 or int64 tensor of shape (B,)", what,
+                "counts must be an int32 or int64 tensor of shape (B,)", "positions must be a tensor")
+    for i, (t, message) in enumerate(zip(tensors, messages)):
+        if not (isinstance(t, _Tensor) or (i > 3 and t is None)):
+            raise ValueError(message)
 
 
 def _table(page_table, batch: int, page_size: int, device) -> torch.Tensor:
@@ -261,7 +271,8 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
     what = "paged attention"
     if not isinstance(cache, PagedCache):
         raise ValueError("cache must be a PagedCache")
-    _check_tensors(what, q, q, page_table, start, None, counts)
+    if not _all_tensors(q, q, page_table, start, counts):
+        _check_tensors(what, q, q, page_table, start, None, counts)
     _refuse_grad(what, q)
     scale, window, sinks = float(scale), None if window is None else int(window), int(sinks)
     device = q.device

@@ -149,7 +149,8 @@ def test_append_follows_strides(cuda_device):
 
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("heads,groups,dim", [(1, 1, 8), (3, 3, 64), (8, 2, 64), (8, 1, 128), (9, 1, 40), (32, 2, 72), (6, 2, 128)])
+@pytest.mark.parametrize("heads,groups,dim", [(1, 1, 8), (3, 3, 64), (8, 2, 64), (8, 1, 128), (9, 1, 40), (32, 2, 72), (6, 2, 128),
+                                              (4, 2, 24), (16, 4, 32), (6, 3, 96), (12, 1, 104)])
 @pytest.mark.parametrize("states,page_size", [(1, 1), (15, 16), (16, 3), (17, 16), (100, 5), (333, 32)])
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_token_matches_oracle(cuda_device, dtype, heads, groups, dim, states, page_size, kernel):
@@ -404,6 +405,88 @@ def test_other_streams_strides_and_repeats(cuda_device):
     assert bool((wide[:, :, 0] == 7).all()) and bool((wide[:, :, 2] == 7).all())
 
 
+def test_two_graphs_at_once(cuda_device):
+    """Graphs of the two kernels replayed together on two streams: each has its own scratch."""
+    keys, values, table = _filled(3, 2, 700, 64, 16, BF16, 180)
+    cache, table = PagedCache(keys.to(cuda_device), values.to(cuda_device)), table.to(cuda_device)
+    start = torch.tensor([699, 200, 3], dtype=torch.int32, device=cuda_device)
+    work = []
+    for seed in range(4):
+        q = _rand((3, 4, 1, 64), BF16, 181 + seed).to(cuda_device)
+        more = dict(page_table=table, start=start, scale=0.125, kernel=KERNELS[seed % 2])
+        want = paged_attention(q, cache, **more)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged_attention(q, cache, **more)
+        work.append((q, graph, out, want, torch.cuda.Stream(cuda_device)))  # a graph does not keep its inputs
+    for _ in range(20):
+        for _, graph, out, _, stream in work:
+            stream.wait_stream(torch.cuda.current_stream(cuda_device))
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+        for *_, stream in work:
+            torch.cuda.current_stream(cuda_device).wait_stream(stream)
+        assert all(torch.equal(out, want) for *_, out, want, _ in work)
+
+
+def test_calls_from_two_threads(cuda_device):
+    import threading
+
+    keys, values, table = _filled(2, 2, 300, 64, 16, BF16, 190)
+    cache, table = PagedCache(keys.to(cuda_device), values.to(cuda_device)), table.to(cuda_device)
+    rotary = RotaryAxes.sections([32], device=cuda_device)
+    start = torch.tensor([299, 100], dtype=torch.int32, device=cuda_device)
+    results, wants = [[], []], []
+    for which in range(2):
+        q = _rand((2, 4, 1, 64), BF16, 191 + which).to(cuda_device)
+        turned, _ = rotate_positions(q, rotary=rotary, positions=start[:, None, None])
+        wants.append((q, paged_attention(turned, cache, page_table=table, start=start, scale=0.125, kernel=KERNELS[which])))
+    torch.cuda.synchronize(cuda_device)
+
+    def call(which):
+        stream = torch.cuda.Stream(cuda_device)
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                turned, _ = rotate_positions(wants[which][0], rotary=rotary, positions=start[:, None, None])
+                results[which].append(paged_attention(turned, cache, page_table=table, start=start, scale=0.125,
+                                                      kernel=KERNELS[which]))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for got, (_, want) in zip(results, wants):
+        assert len(got) == 50 and all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_the_result_may_take_the_queries_place(cuda_device, kernel):
+    keys, values, table = _filled(2, 2, 900, 64, 16, BF16, 200)
+    q = _rand((2, 8, 3, 64), BF16, 201).to(cuda_device)
+    cache, table = PagedCache(keys.to(cuda_device), values.to(cuda_device)), table.to(cuda_device)
+    start = torch.tensor([897, 40], dtype=torch.int32, device=cuda_device)
+    more = dict(page_table=table, start=start, scale=0.125, kernel=kernel)
+    want = paged_attention(q, cache, **more)
+    assert paged_attention(q, cache, out=q, **more) is q
+    assert torch.equal(q, want)
+
+
+def test_a_long_row_of_new_tokens(cuda_device):
+    """More rows than a tile holds: a prompt of 300 tokens behind 50 states, every query head group size."""
+    for heads, groups in ((2, 2), (6, 2), (16, 1)):
+        keys, values, table = _filled(2, groups, 350, 32, 16, BF16, 210 + heads)
+        q = _rand((2, heads, 300, 32), BF16, 211 + heads)
+        got = _attend(cuda_device, q, keys, values, table, [50, 0], scale=0.2, counts=[300, 290]).cpu()
+        for rows in (slice(0, 3), slice(150, 153), slice(287, 290), slice(297, 300)):
+            at = rows.start
+            want, bound = oracle.attend(q[:, :, rows], keys, values, page_table=table, start=[50 + at, at], scale=0.2,
+                                        counts=[min(max(c - at, 0), 3) for c in (300, 290)])
+            assert ((got[:, :, rows].double() - want).abs() <= bound).all()
+
+
 def test_long_cache_past_32_bit_offsets(cuda_device):
     """Pages whose elements lie past 2^31, written and read."""
     page_size, dim, groups = 256, 128, 8
@@ -462,6 +545,8 @@ def test_refusals(cuda_device):
                                   (table.new_zeros(2, 2, 3, 16, dtype=BF16), table.new_zeros(2, 3, 2, 16, dtype=BF16).transpose(1, 2), "share their strides")):
         with pytest.raises(ValueError, match=message):
             PagedCache(keys, values)
+    with pytest.raises(ValueError, match="no part in autograd"):
+        PagedCache(k.clone().requires_grad_(), k)
     for name in ("keys", "values", "layout"):
         with pytest.raises(AttributeError):
             setattr(cache, name, None)

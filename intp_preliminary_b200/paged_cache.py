@@ -28,7 +28,8 @@ from . import _lib
 from .cross_attention import (_HALF, _MAX_STRIDE, _call, _check_counts, _check_scale, _keep, _laid_out, _output, _plans,
                               _ready, _refuse_grad, _scratch_bytes)
 from .look_attention import _DTYPE_CODE
-from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _check_rotary, _rows_laid_out, _set_rotary)
+from .rotary import (_POINTERS, RotaryAxes, _check_heads, _check_positions, _check_rotary, _grad_enabled, _rows_laid_out,
+                     _set_rotary, _unusual)
 
 _ATTENTION_POINTERS = struct.Struct("9Q")  # paged_attention_args up to the sizes
 _MAX_STATES = 1 << 30
@@ -142,15 +143,20 @@ class PagedCache:
         unspecified."""
         if rotary is not None and not isinstance(rotary, RotaryAxes):
             raise ValueError("rotary must be a RotaryAxes")
-        if not _all_tensors(k, v, page_table, start, q, counts, positions):
+        try:
+            if _unusual() or (_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)
+                                                   or (positions is not None and positions.requires_grad))):
+                _refuse_grad("a paged cache", k, v, q, positions)
+            key = ("append", self._layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+                   page_table.shape, page_table.stride(), page_table.dtype, page_table.device, start.shape,
+                   start.stride(), start.dtype, start.device,
+                   None if q is None else (q.shape, q.stride(), q.dtype, q.device),
+                   None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.device),
+                   None if rotary is None else rotary._layout,
+                   None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device))
+        except (AttributeError, TypeError):
             _check_tensors("a paged cache", k, v, page_table, start, q, counts, positions)
-        _refuse_grad("a paged cache", k, v, q, positions)
-        key = ("append", self._layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
-               page_table.shape, page_table.stride(), page_table.dtype, page_table.device, start.shape, start.stride(),
-               start.dtype, start.device, None if q is None else (q.shape, q.stride(), q.dtype, q.device),
-               None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.device),
-               None if rotary is None else rotary._layout,
-               None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device))
+            raise
         tail = _plans.get(key)
         k_at, v_at, q_at = k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr()
         if tail is None or (k_at | v_at | q_at) & 15:
@@ -173,14 +179,6 @@ class PagedCache:
         return q_out
 
 
-_Tensor = torch.Tensor
-
-
-def _all_tensors(one, two, three, four, *others) -> bool:
-    return (isinstance(one, _Tensor) and isinstance(two, _Tensor) and isinstance(three, _Tensor)
-            and isinstance(four, _Tensor) and all([t is None or isinstance(t, _Tensor) for t in others]))
-
-
 def _check_tensors(what: str, *tensors) -> None:
     """Says which of a call's arguments is no tensor; from the fifth on they may be None."""
     what = f"{what} requires CUDA tensors"
@@ -188,7 +186,7 @@ def _check_tensors(what: str, *tensors) -> None:
                 "start must be an int32 or int64 tensor of shape (B,)", what,
                 "counts must be an int32 or int64 tensor of shape (B,)", "positions must be a tensor")
     for i, (t, message) in enumerate(zip(tensors, messages)):
-        if not (isinstance(t, _Tensor) or (i > 3 and t is None)):
+        if not (isinstance(t, torch.Tensor) or (i > 3 and t is None)):
             raise ValueError(message)
 
 
@@ -271,15 +269,20 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
     what = "paged attention"
     if not isinstance(cache, PagedCache):
         raise ValueError("cache must be a PagedCache")
-    if not _all_tensors(q, q, page_table, start, counts):
+    try:
+        if _unusual() or (_grad_enabled() and q.requires_grad):
+            _refuse_grad(what, q)
+        device = q.device
+        key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, device, page_table.shape, page_table.stride(),
+               page_table.dtype, page_table.device, start.shape, start.stride(), start.dtype, start.device,
+               None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.device), float(scale),
+               None if window is None else int(window), int(sinks), kernel,
+               None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+    except (AttributeError, TypeError):
         _check_tensors(what, q, q, page_table, start, None, counts)
-    _refuse_grad(what, q)
-    scale, window, sinks = float(scale), None if window is None else int(window), int(sinks)
-    device = q.device
-    key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, device, page_table.shape, page_table.stride(),
-           page_table.dtype, page_table.device, start.shape, start.stride(), start.dtype, start.device,
-           None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.device), scale, window, sinks,
-           kernel, None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+        if out is not None:
+            _output(q, out)
+        raise
     plan = _plans.get(key)
     if plan is None or (q.data_ptr() | (0 if out is None else out.data_ptr())) & 15:
         given = (q, page_table, start, counts)
@@ -288,7 +291,8 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
             q, page_table, start, counts = taken
             return paged_attention(q, cache, page_table=page_table, start=start, scale=scale, counts=counts, window=window,
                                    sinks=sinks, kernel=kernel, out=out)
-        plan = _keep(key, _attention_plan(q, cache, page_table, scale, window, sinks, kernel, out))
+        plan = _keep(key, _attention_plan(q, cache, page_table, float(scale), None if window is None else int(window),
+                                          int(sinks), kernel, out))
     tail, scratch_bytes = plan
     if out is None:
         out = torch.empty_like(q)

@@ -24,6 +24,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .cross_attention import _MAX_STRIDE, _call, _keep, _plans
@@ -32,6 +33,13 @@ from .look_attention import _DTYPE_CODE, _refuse_transforms
 _POINTERS = struct.Struct("12Q")  # rotary_args up to the sizes
 _POSITION_TYPES = {torch.int32: _lib.ROTARY_INT32, torch.int64: _lib.ROTARY_INT64, torch.float32: _lib.ROTARY_FLOAT32}
 _MAX_PAIRS = 64
+_grad_enabled = torch.is_grad_enabled
+_tracing = torch._C._get_tracing_state
+
+
+def _unusual() -> bool:
+    """Whether forward-mode tangents or a trace may be about, which the kernels know nothing of."""
+    return forward_ad._current_level >= 0 or _tracing() is not None
 
 
 class RotaryAxes:
@@ -180,16 +188,19 @@ def _turn_plan(q, k, rotary, positions, inverse: bool):
 
 def _rotate(q, k, rotary, positions, inverse: bool):
     """q and k (or None) turned: one launch.  What sizes, strides and types decide is kept by those alone."""
-    if not isinstance(q, torch.Tensor) or not (k is None or isinstance(k, torch.Tensor)):
-        raise ValueError("rotate_positions requires CUDA tensors")
-    if not isinstance(rotary, RotaryAxes):
-        raise ValueError("rotary must be a RotaryAxes")
-    if not isinstance(positions, torch.Tensor):
-        raise ValueError("positions must be a tensor")
-    device = q.device
-    key = ("rotate", rotary._layout, q.shape, q.stride(), q.dtype, device, positions.shape, positions.stride(),
-           positions.dtype, positions.device, inverse,
-           None if k is None else (k.shape, k.stride(), k.dtype, k.device))
+    try:
+        device = q.device
+        key = ("rotate", rotary._layout, q.shape, q.stride(), q.dtype, device, positions.shape, positions.stride(),
+               positions.dtype, positions.device, inverse,
+               None if k is None else (k.shape, k.stride(), k.dtype, k.device))
+    except (AttributeError, TypeError):
+        if not isinstance(q, torch.Tensor) or not (k is None or isinstance(k, torch.Tensor)):
+            raise ValueError("rotate_positions requires CUDA tensors") from None
+        if not isinstance(rotary, RotaryAxes):
+            raise ValueError("rotary must be a RotaryAxes") from None
+        if not isinstance(positions, torch.Tensor):
+            raise ValueError("positions must be a tensor") from None
+        raise
     tail = _plans.get(key)
     q_at, k_at = q.data_ptr(), 0 if k is None else k.data_ptr()
     if tail is None or (q_at | k_at) & 15:
@@ -223,14 +234,19 @@ class _RotatePositions(torch.autograd.Function):
         needs_q, needs_k = ctx.needs_input_grad[:2]
         if not needs_q:
             grad_q = None
-        if not needs_k or grad_k is None:
-            if grad_q is None:
-                return None, None, None, None, None
-            return rotate_positions(grad_q, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)[0], None, None, None, None
-        if grad_q is None:
-            return None, rotate_positions(grad_k, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)[0], None, None, None
-        return (*rotate_positions(grad_q, grad_k, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse), None,
-                None, None)
+        if not needs_k:
+            grad_k = None
+        if grad_q is not None:
+            grad_q, grad_k = _back(ctx, grad_q, grad_k, positions)
+        elif grad_k is not None:
+            grad_k, _ = _back(ctx, grad_k, None, positions)
+        return grad_q, grad_k, None, None, None
+
+
+def _back(ctx, one, two, positions):
+    if _grad_enabled():  # create_graph: the gradient has one of its own
+        return rotate_positions(one, two, rotary=ctx.rotary, positions=positions, inverse=not ctx.inverse)
+    return _rotate(one, two, ctx.rotary, positions, not ctx.inverse)
 
 
 def rotate_positions(q, k=None, *, rotary, positions, inverse: bool = False):
@@ -242,8 +258,9 @@ def rotate_positions(q, k=None, *, rotary, positions, inverse: bool = False):
     int32, int64 or float32 with any strides.  ``inverse`` turns by the negative angles.
     Inputs whose rows are not 16-byte aligned with unit stride along D are copied
     first; broadcast ones (stride zero) are not."""
-    _refuse_transforms("rotate_positions", q, k, positions)
-    if torch.is_grad_enabled():
+    if _unusual():
+        _refuse_transforms("rotate_positions", q, k, positions)
+    if _grad_enabled():
         if isinstance(positions, torch.Tensor) and positions.requires_grad:
             raise ValueError("positions have no gradient: detach them")
         if (isinstance(q, torch.Tensor) and q.requires_grad) or (isinstance(k, torch.Tensor) and k.requires_grad):

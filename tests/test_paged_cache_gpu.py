@@ -522,6 +522,8 @@ def test_refusals(cuda_device):
             ((q, cache), {"page_table": table.float()}, "page_table"), ((q, cache), {"page_table": table[0]}, "page_table"),
             ((q, cache), {"page_table": table.cpu()}, "same CUDA device"), ((q, cache), {"page_table": table[:, :0]}, "at least one page"),
             ((q, cache), {"start": None}, "start"), ((q, cache), {"start": start[:1]}, "start"), ((q, cache), {"start": start.float()}, "start"),
+            ((q, cache), {"page_table": [[0]]}, "page_table"), ((3, cache), {}, "CUDA"), ((q, cache), {"counts": [1, 1]}, "counts"),
+            ((q, cache), {"out": 3}, "out"), ((q, q), {}, "PagedCache"),
             ((q, cache), {"counts": start[:1]}, "counts"), ((q, cache), {"scale": 0.0}, "scale"), ((q, cache), {"window": 0}, "window"),
             ((q, cache), {"sinks": -1, "window": 4}, "sinks"), ((q, cache), {"sinks": 2}, "window"),
             ((q, cache), {"out": q[..., :8]}, "out"), ((q, cache), {"kernel": "tiles"}, "kernel"),
@@ -535,7 +537,10 @@ def test_refusals(cuda_device):
             ((k, k), {"q": q}, "rotary"), ((k, k), {"positions": start[:1, None]}, "rotary"), ((k, k), {"rotary": 3}, "RotaryAxes"),
             ((k, k), {"rotary": rotary, "q": q[:1]}, "shape"), ((k, k), {"rotary": rotary, "positions": start[:, None]}, "positions"),
             ((k, k), {"rotary": RotaryAxes.sections([12], device=cuda_device)}, "more columns"),
-            ((k, k.clone().requires_grad_()), {}, "no backward"), ((k, k), {"page_table": table[:1]}, "row for each sequence")):
+            ((k, k.clone().requires_grad_()), {}, "no backward"), ((k, k), {"start": [0, 0]}, "start"),
+            ((k, k), {"rotary": rotary, "positions": torch.zeros(1, 1, device=cuda_device, requires_grad=True)}, "no backward"),
+            ((k, k), {"rotary": rotary, "q": q.clone().requires_grad_()}, "no backward"), ((k, 3), {}, "CUDA"),
+            ((k, k), {"rotary": rotary, "positions": [0]}, "positions"), ((k, k), {"page_table": table[:1]}, "row for each sequence")):
         with pytest.raises(ValueError, match=message):
             cache.append(*args, **{**good, **over})
     for keys, values, message in ((k, k.half(), "dtype"), (k.float(), k.float(), "bfloat16"), (k[0], k[0], "shape"),
@@ -550,6 +555,26 @@ def test_refusals(cuda_device):
     for name in ("keys", "values", "layout"):
         with pytest.raises(AttributeError):
             setattr(cache, name, None)
+
+
+def test_tangents_and_traces_are_refused(cuda_device):
+    cache, table = _pool(cuda_device, 2, 2, 32, 16, 8)
+    q = torch.zeros(2, 4, 1, 16, dtype=BF16, device=cuda_device)
+    k = torch.zeros(2, 2, 1, 16, dtype=BF16, device=cuda_device)
+    more = dict(page_table=table, start=torch.zeros(2, dtype=torch.int32, device=cuda_device))
+    paged_attention(q, cache, scale=0.25, **more)                 # a call that is known by its layout is refused too
+    cache.append(k, k, **more)
+    forward_ad = torch.autograd.forward_ad
+    with forward_ad.dual_level():
+        dual_q, dual_k = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (q, k))
+        for call in (lambda: paged_attention(dual_q, cache, scale=0.25, **more), lambda: cache.append(dual_k, k, **more),
+                     lambda: cache.append(k, dual_k, **more)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        paged_attention(q, cache, scale=0.25, **more)             # the primal alone is none of that
+    for call in (lambda: paged_attention(q, cache, scale=0.25, **more), lambda: cache.append(k, k, **more)):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(lambda t: (call(), t)[1], torch.zeros(1, device=cuda_device), check_trace=False)
 
 
 def test_empty_batches_and_rows(cuda_device):

@@ -4,17 +4,30 @@
 // Reading the states bounds this: the query heads of a key head (and a sequence's few new tokens)
 // share each state, 16 rows at most to a pass, so a state of 4 D bytes carries at most 64 D
 // multiply-adds.  What counts is bytes in flight on every SM and few instructions a byte.
-// A warp streams slices of 16 keys (32 of head_dim 64 or less) through its own cp.async ring; every row of a slice is looked
-// up in the page table by one lane, a step ahead of the copy, so pages may be of any size.  The
-// products are 16 x 8 x 16 matrix instructions with the states as the 16-high operand,
+// A warp streams slices of 16 keys (32 of head_dim 64 or less) through its own cp.async ring; every
+// row of a slice is looked up in the page table by one lane, a step ahead of the copy, so pages may be
+// of any size.  The products are 16 x 8 x 16 matrix instructions with the states as the 16-high operand,
 //   S^T = k q^T (16 keys x 8 rows),   O^T += v^T P^T (16 columns x 8 rows),
 // the probabilities two 16-bit numbers each, so that only the result's own rounding remains.
 // The reference of the exponentials moves only when a score passes it by 2^8.
-// The warps of a CTA join through shared memory, the CTAs of a cluster (each with its share of the
-// sequence's actual length) through distributed shared memory, in a fixed order: results repeat.
 //
 // Row r of a sequence and key head is query head r % (H / G) of token r / (H / G), so that the rows
 // of a tile stand at neighbouring positions.
+//
+// Two kernels share that loop.  paged_joined_kernel gives each sequence and key head one to eight CTAs:
+// their warps join through shared memory, the CTAs of a cluster through distributed shared memory, in one
+// launch.  paged_parts_kernel gives every warp of the GPU the same number of slices of the whole batch,
+// and paged_combine_kernel joins the parts.  Both join in a fixed order: results repeat.
+//
+// Measured on one B200 (calls in a CUDA graph, us; floor at the measured copy rate): B64 G8 H32 D128 over
+// 4096 to 8192 states 242 (237); one sequence of 131071 90 (82); a window of 1024 and 4 first states, B48 G4
+// D64 11.1 (7.7); two sequences of 777 4.8 (0.1: latency).  Steps: 327, 346, 24.6, 8 with one cluster kernel
+// and 64-bit places handed round; 274, 111, 23 in parts; 238, 99, 14.6 with places in 16-byte units (718 ->
+// 344 instructions a slice: issue, not memory, had bound it) and P's high part cut off instead of V clamped;
+// 11.5 with 32-key slices at D64; 242, 90, 11.1 with the next slice asked for while the first products run.
+// Not kept: slices' rows an odd number of chunks apart instead of permuted (copies straddle lines: batch 276
+// where this form took 255), 96-column slices (D96 in parts 114 us, in 128 columns 103), two slices a ring
+// and three CTAs an SM (batch 233, B1 G8 of 32000 states 26.4 instead of 23.9, 16 rows 40 instead of 27).
 #include <cooperative_groups.h>
 #include <algorithm>
 #include <cmath>

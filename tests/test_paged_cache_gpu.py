@@ -405,6 +405,34 @@ def test_other_streams_strides_and_repeats(cuda_device):
     assert bool((wide[:, :, 0] == 7).all()) and bool((wide[:, :, 2] == 7).all())
 
 
+def test_a_first_call_may_be_captured(cuda_device):
+    """In a process of its own: nothing of a call has to have run before it is captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from intp_preliminary_b200 import PagedCache, RotaryAxes, paged_attention
+cache = PagedCache.empty(9, 2, 8, 64, device="cuda")
+rotary = RotaryAxes.sections([32], device="cuda")
+table = torch.arange(8, dtype=torch.int32, device="cuda").reshape(2, 4)
+start = torch.zeros(2, dtype=torch.int32, device="cuda")
+q, k = torch.randn(2, 4, 3, 64, device="cuda").bfloat16(), torch.randn(2, 2, 3, 64, device="cuda").bfloat16()
+def step(kernel):
+    turned = cache.append(k, k, page_table=table, start=start, rotary=rotary, q=q)
+    return paged_attention(turned, cache, page_table=table, start=start, scale=0.125, kernel=kernel)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [step("joined"), step("parts")]
+graph.replay()
+wants = [step("joined"), step("parts")]
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(outs, wants)) and bool((outs[0] != 0).any())
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+
+
 def test_two_graphs_at_once(cuda_device):
     """Graphs of the two kernels replayed together on two streams: each has its own scratch."""
     keys, values, table = _filled(3, 2, 700, 64, 16, BF16, 180)

@@ -140,7 +140,7 @@ class PagedCache:
         on the way, by ``positions`` ``(B, n, axes)`` or ``(n, axes)``, or without them by
         the state's number on every axis; ``q`` ``(B, H, n, D)`` is turned likewise, every
         row of it, and returned.  Two rows that go to the same row of the pool leave it
-        unspecified."""
+        unspecified, and so do inputs that overlap the rows they are written to."""
         if rotary is not None and not isinstance(rotary, RotaryAxes):
             raise ValueError("rotary must be a RotaryAxes")
         try:

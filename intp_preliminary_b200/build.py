@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -68,15 +69,20 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     ]
     if verbose:
         common += ["-Xptxas", "-v"]
-    for name in SOURCES:
+
+    def compile_one(name: str):
         obj = LIB_DIR / (Path(name).stem + ".o")
         cmd = [*common, "-c", str(CSRC / name), "-o", str(obj)]
-        result = subprocess.run(cmd, capture_output=True, text=True)
+        return name, str(obj), subprocess.run(cmd, capture_output=True, text=True)
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:  # an nvcc a core
+        results = list(pool.map(compile_one, SOURCES))
+    for name, obj, result in results:
         if verbose or result.returncode != 0:
             sys.stderr.write(result.stdout + result.stderr)
         if result.returncode != 0:
             raise RuntimeError(f"nvcc failed on {name}")
-        objects.append(str(obj))
+        objects.append(obj)
     tmp = LIB_DIR / "libintp_b200.so.tmp"
     cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(tmp), *objects, "-lcudart"]
     result = subprocess.run(cmd, capture_output=True, text=True)

@@ -73,7 +73,6 @@ struct Parts {
 constexpr int kPartsCtas = 296, kPartsWarps = 4;          // two CTAs an SM
 constexpr int kPartsAll = kPartsCtas * kPartsWarps;
 constexpr int kPartsBatch = 1024;          // sequences whose prefix sums fit beside the rings
-constexpr int kPartsLeast = 2;             // slices of a part at least
 
 template <int DP>
 struct Shape {
@@ -631,7 +630,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   if (threadIdx.x == 0) before[p.batch] = all;
   __syncthreads();
   const int32_t total = all * p.groups;
-  const int32_t per = max((total + kPartsAll - 1) / kPartsAll, kPartsLeast);
+  const int32_t per = max((total + kPartsAll - 1) / kPartsAll, 1);  // at least one slice; two: 6 items of 777 states 7.6 us instead of 6.6
   if (blockIdx.x == 0) {
     for (int32_t b = threadIdx.x; b <= p.batch; b += kThreads) parts.plan[b] = before[b];
     if (threadIdx.x == 0) parts.plan[p.batch + 1] = per;
@@ -829,13 +828,15 @@ int64_t most_slices(const paged_attention_args* a, int64_t tokens) {
 // two of warps that leaves all of them at work, in CTAs of eight.  A cluster of eight (or four, two) CTAs
 // that fill an SM each wants its SMs in one part of the GPU: 14, 32 and 72 of them find their place at
 // once (B2 G8, 16 items: clusters of four 5.3 us, of eight 6.8).
+// No more warps than slices: a sequence of up to 100 states 3.6 us instead of 4.8; two or more slices a warp
+// before a cluster grows cost more than its join (500 states of D128, 3 items of 777 of D64: 5.1 -> 5.7, 4.8 -> 5.3).
 struct Team {
   int warps, ranks;
 };
-Team team(int64_t items) {
+Team team(int64_t items, int64_t slices) {
   Team t{1, 1};
-  while (t.warps < kMostWarps && items * t.warps * 2 <= kPartsAll) t.warps *= 2;
-  while (t.warps == kMostWarps && t.ranks < kMostRanks &&
+  while (t.warps < kMostWarps && t.warps < slices && items * t.warps * 2 <= kPartsAll) t.warps *= 2;
+  while (t.warps == kMostWarps && t.ranks < kMostRanks && t.warps * t.ranks < slices &&
          items * t.ranks * 2 <= (t.ranks == 1 ? 144 : t.ranks == 2 ? 128 : 112))
     t.ranks *= 2;
   return t;
@@ -850,7 +851,7 @@ Plan plan(const paged_attention_args* a) {
   // One launch / parts, D128: B32 G8 of 4000 states (63 slices a warp) 66 / 71 us, of 8000 (125) 127 / 131,
   // B64 G8 of 8192 (256) 251 / 241, of 4096 with D80 (128) 104 / 90; B1 G8 of 16000 (16, 512 warps)
   // 15.6 / 17.1, of 32000 (31) 24.7 / 24.0, of 131071 109 / 90.
-  const Team t = team(items);
+  const Team t = team(items, slices);
   const int64_t each = (slices + t.warps * t.ranks - 1) / (t.warps * t.ranks);
   const bool better = each > 125 || (each >= 24 && items * t.warps * t.ranks * 2 < kPartsAll);
   // One tile a key head, prefix sums that fit, 32-bit slice numbers.
@@ -876,7 +877,7 @@ int32_t launch_joined(PagedParams p, int64_t slices, cudaStream_t stream) {
   if (!allow_smem(kernel, kMost, done)) return INTP_ERR_LAUNCH;
   p.n_rt = (p.rows + 8 * NT - 1) / (8 * NT);
   const int64_t items = static_cast<int64_t>(p.n_rt) * p.batch * p.groups;
-  const Team t = team(items);
+  const Team t = team(items, slices);
   const int warps = t.warps, ranks = t.ranks;
   if (items * ranks > INT32_MAX) return INTP_ERR_SHAPE;
   p.depth = static_cast<int32_t>(std::min<int64_t>(L::kStages, (slices + warps * ranks - 1) / (warps * ranks)));

@@ -27,7 +27,8 @@
 // 11.5 with 32-key slices at D64; 242, 90, 11.1 with the next slice asked for while the first products run.
 // Not kept: slices' rows an odd number of chunks apart instead of permuted (copies straddle lines: batch 276
 // where this form took 255), 96-column slices (D96 in parts 114 us, in 128 columns 103), two slices a ring
-// and three CTAs an SM (batch 233, B1 G8 of 32000 states 26.4 instead of 23.9, 16 rows 40 instead of 27).
+// and three CTAs an SM (batch 233, B1 G8 of 32000 states 26.4 instead of 23.9, 16 rows 40 instead of 27),
+// packed fp32 pairs for the scores and P (a tenth fewer of those instructions, 0 to 2 % slower).
 #include <cooperative_groups.h>
 #include <algorithm>
 #include <cmath>
@@ -69,9 +70,11 @@ struct Parts {
   float* o;                                // [slot][tile row][D], not normalised
   float2* ml;                              // [slot][tile row]: reference (log2 units) and sum
   int32_t* plan;                           // [batch + 1] slices of one key head before each sequence; then slices a warp
+  bool three;                              // CTAs an SM: three, or two
 };
-constexpr int kPartsCtas = 296, kPartsWarps = 4;          // two CTAs an SM
-constexpr int kPartsAll = kPartsCtas * kPartsWarps;
+constexpr int kPartsWarps = 4;
+constexpr int kPartsCtas = 296, kPartsAll = kPartsCtas * kPartsWarps;  // two CTAs an SM, rings of kStages slices
+constexpr int kThreeCtas = 444, kThreeStages = 2;         // three, rings of two
 constexpr int kPartsBatch = 1024;          // sequences whose prefix sums fit beside the rings
 
 template <int DP>
@@ -80,7 +83,6 @@ struct Shape {
   static constexpr int kStep = DP > 64 ? 16 : 32;          // keys of a slice
   static constexpr int kSliceBytes = kStep * DP * 2;       // K or V of a slice
   static constexpr int kStages = DP == 32 ? 6 : 3;         // 24 KB a warp
-  static constexpr int kWarpRing = kStages * 2 * kSliceBytes;
 };
 
 // The dynamic shared memory from its first 256-byte boundary on: slices' rows lie on their own length.
@@ -121,10 +123,10 @@ __device__ __forceinline__ View tile_view(const PagedParams& p, int32_t b, int32
 
 // The slices of one warp, copied into its ring in turn.  A lane looks up the place of one key, in
 // 16-byte units (32 bits reach 64 GB), and hands it to the lanes that copy the key's chunks.
-template <int DP, bool FULL>
+template <int DP, bool FULL, int NS = Shape<DP>::kStages>
 struct Feed {
   using L = Shape<DP>;
-  static constexpr int CH = L::kChunks, NS = L::kStages, kStep = L::kStep, kRowsAStep = 32 / CH;
+  static constexpr int CH = L::kChunks, kStep = L::kStep, kRowsAStep = 32 / CH;
   static constexpr uint32_t kAll = 0xffffffffu >> (32 - kStep);
   const PagedParams& p;
   uint32_t* seen_s;                         // [NS]: which keys of a ring's slice are read
@@ -593,16 +595,16 @@ paged_joined_kernel(const PagedParams p) {
   cluster.sync();  // nobody leaves while others read its sums
 }
 
-// Every warp on its own: kWarps warps a CTA, one wave of CTAs.
-template <int DP, bool FULL, bool BF16, int NT, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32)
+// Every warp on its own, one wave of kCtas CTAs with rings of NS slices.
+template <int DP, bool FULL, bool BF16, int NT, int kCtas, int NS>
+__global__ void __launch_bounds__(kPartsWarps * 32, kCtas / 148)
 paged_parts_kernel(const PagedParams p, const Parts parts) {
   using L = Shape<DP>;
-  constexpr int NS = L::kStages, kTile = 8 * NT, kThreads = kWarps * 32;
+  constexpr int kWarps = kPartsWarps, kTile = 8 * NT, kThreads = kWarps * 32, kAll = kCtas * kWarps;
   uint8_t* smem = aligned_smem();
   __shared__ uint32_t seen_s[kWarps][NS];
   __shared__ int32_t sum_s[kWarps];
-  int32_t* before = reinterpret_cast<int32_t*>(smem + kWarps * L::kWarpRing);  // [batch + 1]
+  int32_t* before = reinterpret_cast<int32_t*>(smem + kWarps * NS * 2 * L::kSliceBytes);  // [batch + 1]
   allow_next_kernel();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Prefix sums of the sequences' slices: a run of sequences a thread, the runs' sums across the CTA.
@@ -630,13 +632,13 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   if (threadIdx.x == 0) before[p.batch] = all;
   __syncthreads();
   const int32_t total = all * p.groups;
-  const int32_t per = max((total + kPartsAll - 1) / kPartsAll, 1);  // at least one slice; two: 6 items of 777 states 7.6 us instead of 6.6
+  const int32_t per = max((total + kAll - 1) / kAll, 1);  // at least one slice; two: 6 items of 777 states 7.6 us instead of 6.6
   if (blockIdx.x == 0) {
     for (int32_t b = threadIdx.x; b <= p.batch; b += kThreads) parts.plan[b] = before[b];
     if (threadIdx.x == 0) parts.plan[p.batch + 1] = per;
   }
   // Consecutive warps' parts on different SMs, so that few parts find many.
-  const int32_t me = warp * kPartsCtas + blockIdx.x;
+  const int32_t me = warp * kCtas + blockIdx.x;
   if (static_cast<int64_t>(me) * per >= total) return;
   const int32_t f0 = me * per, mine = min(per, total - f0);
   int32_t lo = 0, hi = p.batch;             // the last sequence that starts at f0 or before
@@ -670,7 +672,7 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
     return true;
   };
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
-  Feed<DP, FULL> feed(p, ring, NS, seen_s[warp]);
+  Feed<DP, FULL, NS> feed(p, ring, NS, seen_s[warp]);
   feed.enter(in.b, in.grp);
   int32_t next_page = -1;
   uint32_t next_row = 0;
@@ -810,7 +812,7 @@ void take(int64_t* dst, const int64_t* src, const int64_t* extent) {
 int tile_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 
 struct Plan {
-  bool parts;
+  bool parts, three;                       // three: CTAs an SM
   int64_t o_bytes, ml_bytes, bytes;        // of the workspace
 };
 
@@ -855,10 +857,14 @@ Plan plan(const paged_attention_args* a) {
   const int64_t each = (slices + t.warps * t.ranks - 1) / (t.warps * t.ranks);
   const bool better = each > 125 || (each >= 24 && items * t.warps * t.ranks * 2 < kPartsAll);
   // One tile a key head, prefix sums that fit, 32-bit slice numbers.
-  const bool able = rows <= 16 && a->batch <= kPartsBatch && items * slices <= INT32_MAX - 2 * kPartsAll;
+  const bool able = rows <= 16 && a->batch <= kPartsBatch && items * slices <= INT32_MAX - 2 * kThreeCtas * kPartsWarps;
   x.parts = able && (a->kernel == PAGED_KERNEL_PARTS || (a->kernel == PAGED_KERNEL_AUTO && better));
   if (x.parts) {
-    const int64_t slots = (kPartsAll + items) * tile_rows(rows);
+    // Three CTAs an SM want a tile of 8 rows (16 do not fit their registers), and pay where the parts are long
+    // and of many items: B64 G8 D128 over 4096 to 8192 states 233 us instead of 243; B1 G8 of 32000 26.4
+    // instead of 23.9; B64 G8 D80 of 4096 90.6 instead of 89.2.
+    x.three = rows <= 8 && a->head_dim == 128 && items >= 128;
+    const int64_t slots = ((x.three ? kThreeCtas * kPartsWarps : kPartsAll) + items) * tile_rows(rows);
     x.o_bytes = align256(slots * a->head_dim * 4);
     x.ml_bytes = align256(slots * 8);
     x.bytes = x.o_bytes + x.ml_bytes + align256((a->batch + 2) * 4);
@@ -895,16 +901,16 @@ int32_t launch_joined(PagedParams p, int64_t slices, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? INTP_OK : INTP_ERR_LAUNCH;
 }
 
-template <int DP, bool FULL, bool BF16, int NT>
+template <int DP, bool FULL, bool BF16, int NT, int kCtas, int NS>
 int32_t launch_parts(PagedParams p, const Parts& parts, cudaStream_t stream) {
   using L = Shape<DP>;
-  auto kernel = paged_parts_kernel<DP, FULL, BF16, NT, kPartsWarps>;
-  constexpr int kRing = kPartsWarps * L::kWarpRing, kMost = kRing + kAlign + (kPartsBatch + 1) * 4;
-  static_assert(kMost <= 112 * 1024, "two CTAs an SM");
+  auto kernel = paged_parts_kernel<DP, FULL, BF16, NT, kCtas, NS>;
+  constexpr int kRing = kPartsWarps * NS * 2 * L::kSliceBytes, kMost = kRing + kAlign + (kPartsBatch + 1) * 4;
+  static_assert((kCtas / 148) * (kMost + 256 + 1024) <= 228 * 1024, "CTAs an SM, 1 KB of each the system's");
   static std::atomic<uint64_t> done{0};
   if (!allow_smem(kernel, kMost, done)) return INTP_ERR_LAUNCH;
   p.n_rt = 1;
-  if (!launch_kernel(kernel, dim3(kPartsCtas), kPartsWarps * 32, kRing + kAlign + (p.batch + 1) * 4, stream, false, p, parts))
+  if (!launch_kernel(kernel, dim3(kCtas), kPartsWarps * 32, kRing + kAlign + (p.batch + 1) * 4, stream, false, p, parts))
     return INTP_ERR_LAUNCH;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.queries;
   // Few items have many parts each: a CTA per row, whose warps share them.  Sixteen warps / four: 37 parts
@@ -920,8 +926,12 @@ int32_t launch_parts(PagedParams p, const Parts& parts, cudaStream_t stream) {
 
 template <int DP, bool FULL, bool BF16>
 int32_t launch_rows(const PagedParams& p, const Parts* parts, int64_t slices, cudaStream_t stream) {
+  constexpr int NS = Shape<DP>::kStages;
+  if constexpr (FULL && DP == 128)
+    if (parts != nullptr && parts->three) return launch_parts<DP, FULL, BF16, 1, kThreeCtas, kThreeStages>(p, *parts, stream);
   if (parts != nullptr)
-    return p.rows <= 8 ? launch_parts<DP, FULL, BF16, 1>(p, *parts, stream) : launch_parts<DP, FULL, BF16, 2>(p, *parts, stream);
+    return p.rows <= 8 ? launch_parts<DP, FULL, BF16, 1, kPartsCtas, NS>(p, *parts, stream)
+                       : launch_parts<DP, FULL, BF16, 2, kPartsCtas, NS>(p, *parts, stream);
   return p.rows <= 8 ? launch_joined<DP, FULL, BF16, 1>(p, slices, stream) : launch_joined<DP, FULL, BF16, 2>(p, slices, stream);
 }
 
@@ -1014,6 +1024,7 @@ intp_status run(const paged_attention_args* a, cudaStream_t stream) {
     parts.o = reinterpret_cast<float*>(ws);
     parts.ml = reinterpret_cast<float2*>(ws + how.o_bytes);
     parts.plan = reinterpret_cast<int32_t*>(ws + how.o_bytes + how.ml_bytes);
+    parts.three = how.three;
   }
   const Parts* x = how.parts ? &parts : nullptr;
   const int64_t tokens = std::min<int64_t>(a->queries, 16), slices = most_slices(a, tokens);  // a tile has 16 rows at most

@@ -172,6 +172,17 @@ def test_sequences_of_every_split(cuda_device, batch, groups, states, kernel):
     _check(cuda_device, _rand((batch, 2 * groups, 1, 64), BF16, 32), keys, values, table, start, kernel=kernel, scale=0.125)
 
 
+@pytest.mark.parametrize("batch,groups,states,queries", [(43, 3, 150, 1), (130, 1, 70, 3), (300, 1, 20, 1)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_parts_of_many_sequences(cuda_device, batch, groups, states, queries, dtype):
+    """Heads of 128 and 128 sequences and key heads or more: three CTAs an SM."""
+    keys, values, table = _filled(batch, groups, states, 128, 8, dtype, 35)
+    start = torch.randint(-queries, states - queries + 1, (batch,), generator=torch.Generator().manual_seed(36)).tolist()
+    q = _rand((batch, 2 * groups, queries, 128), dtype, 37)
+    _check(cuda_device, q, keys, values, table, start, kernel="parts", scale=128 ** -0.5)
+    _check(cuda_device, q, keys, values, table, start, kernel="parts", scale=128 ** -0.5, window=33, sinks=2)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("heads,groups,queries", [(4, 4, 2), (4, 2, 5), (8, 1, 3), (1, 1, 40), (12, 4, 17)])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (5, 0), (7, 3), (40, 20), (1000, 4), (16, 100)])

@@ -20,14 +20,15 @@
 // and paged_combine_kernel joins the parts.  Both join in a fixed order: results repeat.
 //
 // Measured on one B200 (calls in a CUDA graph, us; floor at the measured copy rate): B64 G8 H32 D128 over
-// 4096 to 8192 states 242 (237); one sequence of 131071 90 (82); a window of 1024 and 4 first states, B48 G4
+// 4096 to 8192 states 233 (237); one sequence of 131071 90 (82); a window of 1024 and 4 first states, B48 G4
 // D64 11.1 (7.7); two sequences of 777 4.8 (0.1: latency).  Steps: 327, 346, 24.6, 8 with one cluster kernel
 // and 64-bit places handed round; 274, 111, 23 in parts; 238, 99, 14.6 with places in 16-byte units (718 ->
 // 344 instructions a slice: issue, not memory, had bound it) and P's high part cut off instead of V clamped;
-// 11.5 with 32-key slices at D64; 242, 90, 11.1 with the next slice asked for while the first products run.
+// 11.5 with 32-key slices at D64; 240, 90, 11.1 with the next slice asked for while the first products run;
+// 233 with three CTAs an SM where parts are of many items.
 // Not kept: slices' rows an odd number of chunks apart instead of permuted (copies straddle lines: batch 276
 // where this form took 255), 96-column slices (D96 in parts 114 us, in 128 columns 103), two slices a ring
-// and three CTAs an SM (batch 233, B1 G8 of 32000 states 26.4 instead of 23.9, 16 rows 40 instead of 27),
+// and three CTAs an SM for all parts (B1 G8 of 32000 states 26.4 instead of 23.9, 16 rows 40 instead of 27),
 // packed fp32 pairs for the scores and P (a tenth fewer of those instructions, 0 to 2 % slower).
 #include <cooperative_groups.h>
 #include <algorithm>

@@ -61,11 +61,12 @@ class RotaryAxes:
         self._device = torch.device(device)
         if self._device.type != "cuda":
             raise ValueError("rotary positions require a CUDA device")
-        turns = torch.tensor(frequencies, dtype=torch.float64) / (2 * math.pi)
-        self._turns = turns.to(self._device)
-        self._axis = torch.tensor(axes, dtype=torch.int32).to(self._device)
-        self._device = self._turns.device
-        self._pointers = self._turns.data_ptr(), self._axis.data_ptr()
+        # both tables in one copy: turns (64 bits), then axes (32 bits)
+        pairs = len(axes)
+        tables = bytearray(struct.pack(f"{pairs}d{pairs}i", *(f / (2 * math.pi) for f in frequencies), *axes))
+        self._tables = torch.frombuffer(tables, dtype=torch.uint8).to(self._device)
+        self._device = self._tables.device
+        self._pointers = self._tables.data_ptr(), self._tables.data_ptr() + 8 * pairs
         self._frequencies, self._axes = tuple(frequencies), tuple(axes)
         self._interleaved = bool(interleaved)
         # what a call's checks and argument block depend on

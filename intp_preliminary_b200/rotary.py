@@ -61,16 +61,31 @@ class RotaryAxes:
         self._device = torch.device(device)
         if self._device.type != "cuda":
             raise ValueError("rotary positions require a CUDA device")
-        # both tables in one copy: turns (64 bits), then axes (32 bits)
-        pairs = len(axes)
-        tables = bytearray(struct.pack(f"{pairs}d{pairs}i", *(f / (2 * math.pi) for f in frequencies), *axes))
-        self._tables = torch.frombuffer(tables, dtype=torch.uint8).to(self._device)
-        self._device = self._tables.device
-        self._pointers = self._tables.data_ptr(), self._tables.data_ptr() + 8 * pairs
         self._frequencies, self._axes = tuple(frequencies), tuple(axes)
         self._interleaved = bool(interleaved)
+        self._lay_out()
+
+    def _lay_out(self) -> None:
+        """The tables on the device, in one copy: turns (64 bits), then axes (32 bits)."""
+        pairs = len(self._axes)
+        tables = bytearray(struct.pack(f"{pairs}d{pairs}i", *(f / (2 * math.pi) for f in self._frequencies), *self._axes))
+        self._tables = torch.frombuffer(tables, dtype=torch.uint8).to(self._device)
+        self._device = self._tables.device
         # what a call's checks and argument block depend on
-        self._layout = (len(axes), max(axes) + 1, self._interleaved, self._device)
+        self._layout = (pairs, max(self._axes) + 1, self._interleaved, self._device)
+
+    @property
+    def _pointers(self) -> tuple[int, int]:
+        at = self._tables.data_ptr()
+        return at, at + 8 * len(self._axes)
+
+    # A copy, and what is unpickled, lays out tables of its own from the numbers.
+    def __getstate__(self) -> dict:
+        return {name: value for name, value in self.__dict__.items() if name not in ("_tables", "_layout")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._lay_out()
 
     @classmethod
     def sections(cls, sections, *, base: float = 10000.0, apart: bool = False, interleaved: bool = False,

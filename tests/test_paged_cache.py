@@ -239,3 +239,19 @@ def test_oracle_attends_like_cross_attention_over_the_gathered_states(page_size)
     assert (got - want).abs().max() < 1e-14
     # one more u^2 of the same sum that the other bound holds one of
     assert bool((bound >= want_bound).all()) and bool((bound <= 2 * want_bound).all())
+
+
+def test_a_copied_rotary_points_into_its_own_tables():
+    """Without a GPU, on a stand-in whose tables lie in the host's memory."""
+    import copy
+    import pickle
+
+    rotary = _fake_rotary(axes=2)
+    rotary._lay_out()
+    layer = torch.nn.Module()
+    layer.rotary = rotary
+    for other in (copy.copy(rotary), copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary)), copy.deepcopy(layer).rotary):
+        assert other._pointers == (other._tables.data_ptr(), other._tables.data_ptr() + 8 * 8)
+        assert other._tables.data_ptr() != rotary._tables.data_ptr() and torch.equal(other._tables, rotary._tables)
+        assert (other.frequencies, other.axes, other._layout) == (rotary.frequencies, rotary.axes, rotary._layout)
+    assert b"_tables" not in pickle.dumps(rotary)

@@ -231,3 +231,24 @@ def test_rows_past_32_bit_offsets(cuda_device):
     for where in (slice(0, 3), slice(rows - 7, rows)):
         want, _ = rotate_positions(q[:, :, where].clone(), rotary=rotary, positions=at[where].clone())
         assert torch.equal(got[:, :, where], want)
+
+
+def test_copies_turn_alike_without_the_original(cuda_device):
+    """A deep copy, a pickled object, copies inside a module: the same bits once the original is gone."""
+    import copy
+    import pickle
+
+    q = _rand((1, 2, 9, 32), F32, 30).to(cuda_device)
+    at = _positions(1, 9, 2, torch.int32, 31).to(cuda_device)
+    rotary = _rotary(16, 2, cuda_device)
+    layer = torch.nn.Linear(2, 2)
+    layer.rotary = rotary
+    want, _ = rotate_positions(q, rotary=rotary, positions=at)
+    copies = [copy.copy(rotary), copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary)), copy.deepcopy(layer).rotary,
+              pickle.loads(pickle.dumps(layer)).rotary]
+    assert all(c.device == rotary.device for c in copies)
+    del rotary, layer
+    others = [RotaryAxes([0.0] * 16, [1, 0] * 8, device=cuda_device) for _ in range(8)]  # where the original's tables were
+    for c in copies:
+        assert torch.equal(rotate_positions(q, rotary=c, positions=at)[0], want)
+    assert len(others) == 8

@@ -73,6 +73,10 @@ class PagedCache:
         # what calls know the pool by
         self._layout = (keys.shape, keys.stride(), keys.dtype, keys.device)
 
+    def __reduce__(self):
+        """A copy, and what is loaded from a file, is checked again: its tensors may lie elsewhere."""
+        return type(self), (self._keys, self._values)
+
     # read only: a call takes the layout that was checked above
     keys = property(lambda self: self._keys)
     values = property(lambda self: self._values)

@@ -255,3 +255,23 @@ def test_a_copied_rotary_points_into_its_own_tables():
         assert other._tables.data_ptr() != rotary._tables.data_ptr() and torch.equal(other._tables, rotary._tables)
         assert (other.frequencies, other.axes, other._layout) == (rotary.frequencies, rotary.axes, rotary._layout)
     assert b"_tables" not in pickle.dumps(rotary)
+
+
+def test_a_cache_loaded_onto_the_host_is_refused():
+    """Its calls take the layout and device that were checked when it was made, so loading checks again."""
+    import io
+
+    from intp_preliminary_b200 import StateCache
+
+    half, byte = torch.zeros(2, 1, 4, 16, dtype=torch.bfloat16), torch.zeros(2, 1, 4, dtype=torch.uint8)
+    paged, state = PagedCache.__new__(PagedCache), StateCache.__new__(StateCache)
+    paged._keys = paged._values = half
+    state._keys = state._values = half.to(torch.float8_e4m3fn)
+    state._key_exponents = state._value_exponents = byte
+    paged._layout = state._layout = ("as it was on a GPU",)
+    for cache in (paged, state):
+        file = io.BytesIO()
+        torch.save(cache, file)
+        file.seek(0)
+        with pytest.raises(ValueError, match="CUDA"):
+            torch.load(file, weights_only=False)

@@ -626,3 +626,34 @@ def test_empty_batches_and_rows(cuda_device):
     assert paged_attention(q, cache, page_table=table[:0], start=start[:0], scale=0.25).shape == q.shape
     cache.append(q[:, :2], q[:, :2], page_table=table[:0], start=start[:0])
     assert bool((cache.keys == 0).all())
+
+
+def test_copied_caches_hold_states_of_their_own(cuda_device):
+    import copy
+    import io
+    import pickle
+
+    from intp_preliminary_b200 import StateCache
+
+    keys, values, table = _filled(2, 2, 40, 32, 8, BF16, 220, hole=0.0)
+    pool = torch.stack((keys, values)).transpose(2, 3).contiguous().to(cuda_device).transpose(2, 3)
+    cache = PagedCache(pool[0], pool[1])
+    state = StateCache.empty(2, 2, 16, 32, device=cuda_device)
+    state.write(*(_rand((2, 2, 16, 32), BF16, 221 + i).to(cuda_device) for i in range(2)))
+    q, table = _rand((2, 4, 1, 32), BF16, 223).to(cuda_device), table.to(cuda_device)
+    start = torch.tensor([39, 20], device=cuda_device)
+    want, states = paged_attention(q, cache, page_table=table, start=start, scale=0.2), state.read()
+    file = io.BytesIO()
+    torch.save([cache, state], file)
+    file.seek(0)
+    loaded = torch.load(file, weights_only=False)
+    copies = [copy.deepcopy((cache, state)), (pickle.loads(pickle.dumps(cache)), loaded[1]), loaded]
+    pool.zero_()
+    state.keys.zero_()
+    for paged, other in copies:
+        assert paged.keys.stride() == cache.keys.stride()
+        assert torch.equal(paged_attention(q, paged, page_table=table, start=start, scale=0.2), want)
+        assert all(torch.equal(a, b) for a, b in zip(other.read(), states))
+    file.seek(0)
+    with pytest.raises(ValueError, match="CUDA"):
+        torch.load(file, weights_only=False, map_location="cpu")

@@ -149,8 +149,9 @@ class PagedCache:
             raise ValueError("rotary must be a RotaryAxes")
         try:
             if _unusual() or (_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)
-                                                   or (positions is not None and positions.requires_grad))):
-                _refuse_grad("a paged cache", k, v, q, positions)
+                                                   or (positions is not None and positions.requires_grad)
+                                                   or self._keys.requires_grad or self._values.requires_grad)):
+                _refuse_grad("a paged cache", k, v, q, positions, self._keys, self._values)
             key = ("append", self._layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
                    page_table.shape, page_table.stride(), page_table.dtype, page_table.device, start.shape,
                    start.stride(), start.dtype, start.device,
@@ -274,8 +275,9 @@ def paged_attention(q, cache, *, page_table, start, scale, counts=None, window=N
     if not isinstance(cache, PagedCache):
         raise ValueError("cache must be a PagedCache")
     try:
-        if _unusual() or (_grad_enabled() and q.requires_grad):
-            _refuse_grad(what, q)
+        if _unusual() or (_grad_enabled() and (q.requires_grad or cache._keys.requires_grad or cache._values.requires_grad
+                                               or (out is not None and out.requires_grad))):
+            _refuse_grad(what, q, cache._keys, cache._values, out)
         device = q.device
         key = ("attend", cache._layout, q.shape, q.stride(), q.dtype, device, page_table.shape, page_table.stride(),
                page_table.dtype, page_table.device, start.shape, start.stride(), start.dtype, start.device,

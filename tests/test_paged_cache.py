@@ -275,3 +275,21 @@ def test_a_cache_loaded_onto_the_host_is_refused():
         file.seek(0)
         with pytest.raises(ValueError, match="CUDA"):
             torch.load(file, weights_only=False)
+
+
+@pytest.mark.parametrize("which", ["_keys", "_values"])
+def test_a_pool_that_comes_to_require_a_gradient_is_refused(which):
+    """Not only when the cache is made: a tensor may be marked later."""
+    cache = PagedCache.__new__(PagedCache)
+    cache._keys, cache._values = (torch.zeros(2, 1, 4, 16, dtype=torch.bfloat16) for _ in range(2))
+    cache._layout = ()
+    q, start = torch.zeros(1, 1, 1, 16, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="no backward"):
+        paged_attention(q, cache, page_table=start[None], start=start, scale=0.25, out=q.clone().requires_grad_())
+    getattr(cache, which).requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        paged_attention(q, cache, page_table=start[None], start=start, scale=0.25)
+    with pytest.raises(ValueError, match="no backward"):
+        cache.append(q, q, page_table=start[None], start=start)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        paged_attention(q, cache, page_table=start[None], start=start, scale=0.25)

@@ -242,16 +242,14 @@ class _RotatePositions(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
-        return _rotate(q, k, rotary, positions, inverse)
+        outs = _rotate(q, k, rotary, positions, inverse)
+        # the result of an input that needs no gradient needs none either
+        ctx.mark_non_differentiable(*(y for y, needs in zip(outs, ctx.needs_input_grad) if y is not None and not needs))
+        return outs
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
         positions, = ctx.saved_tensors
-        needs_q, needs_k = ctx.needs_input_grad[:2]
-        if not needs_q:
-            grad_q = None
-        if not needs_k:
-            grad_k = None
         if grad_q is not None:
             grad_q, grad_k = _back(ctx, grad_q, grad_k, positions)
         elif grad_k is not None:

@@ -293,3 +293,26 @@ def test_a_pool_that_comes_to_require_a_gradient_is_refused(which):
         cache.append(q, q, page_table=start[None], start=start)
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
         paged_attention(q, cache, page_table=start[None], start=start, scale=0.25)
+
+
+@pytest.mark.parametrize("needs_q,needs_k", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_only_what_needs_a_gradient_gets_one(monkeypatch, needs_q, needs_k, create_graph):
+    """The autograd node alone, over a stand-in for the kernel that doubles."""
+    import importlib
+
+    module = importlib.import_module("intp_preliminary_b200.rotary")
+    turned = []
+
+    def double(q, k, rotary, positions, inverse):
+        turned.append((q is not None) + (k is not None))
+        return q.detach() * 2, None if k is None else k.detach() * 2
+
+    monkeypatch.setattr(module, "_rotate", double)
+    q, k = (torch.ones(1, 2, 3, 8, requires_grad=needs) for needs in (needs_q, needs_k))
+    outs = rotate_positions(q, k, rotary=_fake_rotary(4), positions=torch.zeros(3, 1))
+    assert [t.requires_grad for t in outs] == [needs_q, needs_k]
+    leaves = [t for t in (q, k) if t.requires_grad]
+    grads = torch.autograd.grad(sum(t.sum() for t in outs), leaves, create_graph=create_graph)
+    assert all(torch.equal(g, torch.full_like(g, 2)) for g in grads)
+    assert turned == [2, len(leaves)]

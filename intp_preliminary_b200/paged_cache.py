@@ -176,7 +176,7 @@ class PagedCache:
         if q is not None:
             q_out = torch.empty_like(q)
             q_to = q_out.data_ptr()
-        turns, axis = (0, 0) if rotary is None else rotary._pointers
+        turns, axis = (0, 0) if rotary is None else rotary._launch_pointers()
         block = _POINTERS.pack(q_at, k_at, v_at, q_to, self._keys.data_ptr(), self._values.data_ptr(), turns, axis,
                                0 if positions is None else positions.data_ptr(), start.data_ptr(),
                                0 if counts is None else counts.data_ptr(), page_table.data_ptr()) + tail

@@ -27,7 +27,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .cross_attention import _MAX_STRIDE, _call, _keep, _plans
+from .cross_attention import _MAX_STRIDE, _call, _current_stream, _keep, _plans
 from .look_attention import _DTYPE_CODE, _refuse_transforms
 
 _POINTERS = struct.Struct("12Q")  # rotary_args up to the sizes
@@ -71,6 +71,8 @@ class RotaryAxes:
         tables = bytearray(struct.pack(f"{pairs}d{pairs}i", *(f / (2 * math.pi) for f in self._frequencies), *self._axes))
         self._tables = torch.frombuffer(tables, dtype=torch.uint8).to(self._device)
         self._device = self._tables.device
+        # streams that the tables' memory is held for: the one it was allocated on
+        self._streams = {_current_stream(self._device.index)} if self._tables.is_cuda else set()
         # what a call's checks and argument block depend on
         self._layout = (pairs, max(self._axes) + 1, self._interleaved, self._device)
 
@@ -79,9 +81,18 @@ class RotaryAxes:
         at = self._tables.data_ptr()
         return at, at + 8 * len(self._axes)
 
+    def _launch_pointers(self) -> tuple[int, int]:
+        """The tables' addresses for a launch on the device's current stream: should the object go while
+        the launch is pending, its memory waits for that stream."""
+        stream = _current_stream(self._device.index)
+        if stream not in self._streams:
+            self._tables.record_stream(torch.cuda.current_stream(self._device))
+            self._streams.add(stream)
+        return self._pointers
+
     # A copy, and what is unpickled, lays out tables of its own from the numbers.
     def __getstate__(self) -> dict:
-        return {name: value for name, value in self.__dict__.items() if name not in ("_tables", "_layout")}
+        return {name: value for name, value in self.__dict__.items() if name not in ("_tables", "_streams", "_layout")}
 
     def __setstate__(self, state: dict) -> None:
         self.__dict__.update(state)
@@ -229,7 +240,7 @@ def _rotate(q, k, rotary, positions, inverse: bool):
     if k is not None:
         k_out = torch.empty_like(k)
         k_to = k_out.data_ptr()
-    block = _POINTERS.pack(q_at, k_at, 0, q_out.data_ptr(), k_to, 0, *rotary._pointers, positions.data_ptr(), 0, 0, 0) + tail
+    block = _POINTERS.pack(q_at, k_at, 0, q_out.data_ptr(), k_to, 0, *rotary._launch_pointers(), positions.data_ptr(), 0, 0, 0) + tail
     _call(_lib.load().rotary_positions, block, device.index, "rotate_positions")
     return q_out, k_out
 

@@ -316,3 +316,27 @@ def test_only_what_needs_a_gradient_gets_one(monkeypatch, needs_q, needs_k, crea
     grads = torch.autograd.grad(sum(t.sum() for t in outs), leaves, create_graph=create_graph)
     assert all(torch.equal(g, torch.full_like(g, 2)) for g in grads)
     assert turned == [2, len(leaves)]
+
+
+def test_tables_are_held_for_every_stream_that_reads_them(monkeypatch):
+    """Without a GPU: the launch's stream and the tables' allocator are stand-ins."""
+    import importlib
+
+    module = importlib.import_module("intp_preliminary_b200.rotary")
+    held, now = [], [7]
+
+    class Tables:
+        def data_ptr(self):
+            return 4096
+
+        def record_stream(self, stream):
+            held.append(stream)
+
+    rotary = _fake_rotary()
+    rotary._lay_out()
+    rotary._tables, rotary._streams = Tables(), {7}
+    monkeypatch.setattr(module, "_current_stream", lambda index: now[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: f"stream {now[0]}")
+    for now[0] in (7, 9, 9, 7, 8, 9):
+        assert rotary._launch_pointers() == (4096, 4096 + 8 * 8)
+    assert held == ["stream 9", "stream 8"]

@@ -252,3 +252,36 @@ def test_copies_turn_alike_without_the_original(cuda_device):
     for c in copies:
         assert torch.equal(rotate_positions(q, rotary=c, positions=at)[0], want)
     assert len(others) == 8
+
+
+def test_a_rotary_dropped_while_another_stream_has_yet_to_read_it(cuda_device):
+    """Its memory is not given to new work before that stream's launches are done."""
+    from intp_preliminary_b200 import PagedCache
+
+    q = _rand((1, 2, 9, 32), F32, 32).to(cuda_device)
+    k = q.bfloat16()
+    at = _positions(1, 9, 2, torch.int32, 33).to(cuda_device)
+    table = torch.arange(2, dtype=torch.int32, device=cuda_device)[None]
+    start = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    kept = _rotary(16, 2, cuda_device)
+    want, _ = rotate_positions(q, rotary=kept, positions=at)
+    pool, other = (PagedCache.empty(2, 2, 16, 32, device=cuda_device) for _ in range(2))
+    pool.append(k, k, page_table=table, start=start, rotary=kept, positions=at)
+    for append in (False, True):
+        rotary = _rotary(16, 2, cuda_device)
+        address = rotary._tables.data_ptr()
+        torch.cuda.synchronize(cuda_device)
+        stream, done = torch.cuda.Stream(cuda_device), torch.cuda.Event()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(400_000_000)  # a fifth of a second
+            if append:
+                other.append(k, k, page_table=table, start=start, rotary=rotary, positions=at)
+            else:
+                got, _ = rotate_positions(q, rotary=rotary, positions=at)
+            done.record()
+        del rotary
+        new = [torch.zeros(192, dtype=torch.uint8, device=cuda_device) for _ in range(20)]
+        assert not done.query()
+        assert address not in [t.data_ptr() for t in new]
+        done.synchronize()
+    assert torch.equal(got, want) and torch.equal(other.keys, pool.keys)

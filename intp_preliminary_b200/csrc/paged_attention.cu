@@ -93,9 +93,13 @@ __device__ __forceinline__ uint8_t* aligned_smem() {
   return raw_smem + (kAlign - smem_u32(raw_smem) % kAlign) % kAlign;
 }
 
+// Positions are held less 2^30: start goes up to 2^31 - 1 and a row's number to 2^30.  Positions below -2^30
+// are before the sequence like -2^30.
+constexpr int32_t kFar = 1 << 30;
+
 // What a tile of rows sees of its sequence.
 struct View {
-  int32_t first_pos, last_pos;             // of the tile's tokens that count
+  int32_t first_pos, last_pos;             // of the tile's tokens that count, less kFar
   int32_t end, low, sink_end;              // states [0, sink_end) and [low, end)
   int32_t sink_slices, low_slice, n_slices;
   __device__ __forceinline__ int32_t slice(int32_t i) const { return i < sink_slices ? i : i - sink_slices + low_slice; }
@@ -109,12 +113,12 @@ __device__ __forceinline__ View tile_view(const PagedParams& p, int32_t b, int32
   int32_t count = p.queries;
   if (p.counts != nullptr) count = min(max(p.counts[b], 0), count);
   m1 = min(m1, count - 1);
-  // Positions past 2^30 are behind every table, those below -2^30 before it for any row.
-  const int32_t start = min(max(p.start[b], -(1 << 30)), 1 << 30);
-  x.first_pos = min(start + m0, 1 << 30);
-  x.last_pos = min(start + m1, 1 << 30);
-  x.end = m1 < m0 ? 0 : min(max(x.last_pos, -1), p.capacity - 1) + 1;
-  x.low = p.window > 0 ? max(x.first_pos - p.window + 1, 0) : 0;
+  const int32_t start = max(p.start[b], -kFar) - kFar;
+  x.first_pos = start + m0;
+  x.last_pos = start + m1;
+  x.end = m1 < m0 ? 0 : min(max(x.last_pos, -1 - kFar), p.capacity - 1 - kFar) + kFar + 1;
+  // from 2^31 - 1 on a row is past every window's reach
+  x.low = p.window > 0 ? max(min(x.first_pos, kFar - 1) + (kFar + 1 - p.window), 0) : 0;
   x.sink_end = p.window > 0 ? min(p.sinks, x.end) : 0;
   x.sink_slices = (x.sink_end + kStep - 1) / kStep;
   x.low_slice = max(x.low / kStep, x.sink_slices);
@@ -288,9 +292,10 @@ struct Rows {
     }
     meanwhile();
     // Whether rows of the tile differ in what they see of the slice.
+    const int32_t from = k0 - kFar;         // held like the positions
     const bool mixed = view.first_pos != view.last_pos &&
-                       (k0 + kStep - 1 > view.first_pos ||
-                        (p.window > 0 && k0 <= view.last_pos - p.window && k0 + kStep > p.sinks));
+                       (from + kStep - 1 > view.first_pos ||
+                        (p.window > 0 && from + p.window <= view.last_pos && k0 + kStep > p.sinks));
     const float score_scale = p.scale * kLog2e;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
@@ -301,13 +306,13 @@ struct Rows {
     if (mixed || seen != kAll) {
 #pragma unroll
       for (int kh = 0; kh < 2 * KB; ++kh) {
-        const int32_t key = k0 + kh * 8 + g;
-        const bool there = seen >> (kh * 8 + g) & 1u;
+        const int32_t key = from + kh * 8 + g;
+        const bool there = seen >> (kh * 8 + g) & 1u, sink = k0 + kh * 8 + g < p.sinks;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            if (!there || (mixed && (key > pos[n][h] || (p.window > 0 && key <= pos[n][h] - p.window && key >= p.sinks))))
+            if (!there || (mixed && (key > pos[n][h] || (p.window > 0 && key + p.window <= pos[n][h] && !sink))))
               s[kh / 2][n][2 * (kh & 1) + h] = -INFINITY;
       }
     }
@@ -401,8 +406,8 @@ struct Rows {
         keep[kh] = 0u;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int32_t key = k0 + kh * 8 + 2 * t + e;
-          const bool sees = key <= at && (p.window == 0 || key > at - p.window || key < p.sinks);
+          const int32_t i = kh * 8 + 2 * t + e;
+          const bool sees = from + i <= at && (p.window == 0 || from + i + p.window > at || k0 + i < p.sinks);
           if (sees) keep[kh] |= 0xffffu << (16 * e);
         }
       }

@@ -657,3 +657,18 @@ def test_copied_caches_hold_states_of_their_own(cuda_device):
     file.seek(0)
     with pytest.raises(ValueError, match="CUDA"):
         torch.load(file, weights_only=False, map_location="cpu")
+
+
+@pytest.mark.parametrize("start", [2**30 + 1000, 2**30 - 3, 2**31 - 1, 2**30 + 2100])
+@pytest.mark.parametrize("queries", [1, 4, 20])
+@pytest.mark.parametrize("sinks", [0, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_a_long_window_of_far_rows(cuda_device, start, queries, sinks, kernel):
+    """The window of a row far behind the table ends inside it, at the row's own place: 2^30 states back."""
+    if kernel == "parts" and queries > 16:
+        kernel = "auto"
+    keys, values, table = _filled(2, 1, 2000, 16, 64, BF16, 230)
+    q = _rand((2, 1, queries, 16), BF16, 231)
+    got = _check(cuda_device, q, keys, values, table, [start, 1990], kernel=kernel, scale=0.25, window=2**30, sinks=sinks)
+    if start > 2**30 + 2000 and sinks == 0:
+        assert bool((got[0] == 0).all())

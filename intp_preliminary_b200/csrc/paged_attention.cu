@@ -8,7 +8,8 @@
 // row of a slice is looked up in the page table by one lane, a step ahead of the copy, so pages may be
 // of any size.  The products are 16 x 8 x 16 matrix instructions with the states as the 16-high operand,
 //   S^T = k q^T (16 keys x 8 rows),   O^T += v^T P^T (16 columns x 8 rows),
-// the probabilities two 16-bit numbers each, so that only the result's own rounding remains.
+// the probabilities two 16-bit numbers each, so that only the result's own rounding remains (in f16 a probability
+// below 2^-32 of its row's reference counts as zero, but for its infinite values).
 // The reference of the exponentials moves only when a score passes it by 2^8.
 //
 // Row r of a sequence and key head is query head r % (H / G) of token r / (H / G), so that the rows
@@ -20,12 +21,13 @@
 // and paged_combine_kernel joins the parts.  Both join in a fixed order: results repeat.
 //
 // Measured on one B200 (calls in a CUDA graph, us; floor at the measured copy rate): B64 G8 H32 D128 over
-// 4096 to 8192 states 233 (237); one sequence of 131071 90 (82); a window of 1024 and 4 first states, B48 G4
-// D64 11.1 (7.7); two sequences of 777 4.8 (0.1: latency).  Steps: 327, 346, 24.6, 8 with one cluster kernel
-// and 64-bit places handed round; 274, 111, 23 in parts; 238, 99, 14.6 with places in 16-byte units (718 ->
-// 344 instructions a slice: issue, not memory, had bound it) and P's high part cut off instead of V clamped;
-// 11.5 with 32-key slices at D64; 240, 90, 11.1 with the next slice asked for while the first products run;
-// 233 with three CTAs an SM where parts are of many items.
+// 4096 to 8192 states 235 (237); one sequence of 131071 90 (82); a window of 1024 and 4 first states, B48 G4
+// D64 10.5 (7.7); five tokens of B17 G4 H12 D80 over 2000 to 4001 states 22.5 (9.6); two sequences of 777 4.6
+// (0.1: latency).  Steps: 327, 346, 24.6, -, 8 with one cluster kernel and 64-bit places handed round; 274, 111, 23 in
+// parts; 238, 99, 14.6 with places in 16-byte units (718 -> 344 instructions a slice: issue, not memory, had bound
+// it) and V not clamped; 11.5 with 32-key slices at D64; 240, 90, 11.1, 29 with the next slice asked for while the first
+// products run; 233 with three CTAs an SM where parts are of many items; 10.5, 27 with values that are not finite
+// left to a second pass over a warp's slices, and 22.5 with all of an SM's registers for a tile of 16 rows.
 // Not kept: slices' rows an odd number of chunks apart instead of permuted (copies straddle lines: batch 276
 // where this form took 255), 96-column slices (D96 in parts 114 us, in 128 columns 103), two slices a ring
 // and three CTAs an SM for all parts (B1 G8 of 32000 states 26.4 instead of 23.9, 16 rows 40 instead of 27),
@@ -35,6 +37,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 #include "../../include/intp_b200.h"
 #include "row_mma.cuh"
 #include "xattn_common.cuh"
@@ -204,6 +207,11 @@ struct Feed {
       }
     }
   }
+  // From the first slice on once more, when every lane has read its last one.
+  __device__ __forceinline__ void restart() {
+    cp_async_wait<0>();
+    issued = slot = 0;
+  }
   __device__ __forceinline__ void commit() {
     ++issued;
     slot = slot + 1 == NS ? 0 : slot + 1;
@@ -253,12 +261,31 @@ struct Rows {
     }
   }
 
+  // Whether a sum of this lane, of a row that counts, is NaN.
+  __device__ __forceinline__ bool any_nan(const View& view) const {
+    bool nan = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float sum = 0.f;                    // of infinities of both signs: NaN too, which costs time alone
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) sum += o[n][c][h] + o[n][c][2 + h];
+        nan = nan || (sum != sum && pos[n][h] <= view.last_pos);
+      }
+    return nan;
+  }
+
   // One slice, keys from k0 on, of which the bits of `seen` are there.
   // `meanwhile` runs while the first products are under way.
-  template <class Meanwhile>
+  // A zero times an infinity is NaN: where a state that holds infinities or NaN is not seen by every row of the
+  // tile, or a part of its probability is zero, a column becomes NaN that may not be.  So whatever of a warp's
+  // slices end in NaN is done again, with CAREFUL: slices are looked through for such values, and those that hold
+  // any go token by token, infinities and NaN against 1 for a probability above zero.
+  template <bool CAREFUL, class Meanwhile>
   __device__ __forceinline__ void step(const PagedParams& p, const View& view, uint32_t k_s, int32_t k0, uint32_t seen,
                                        Meanwhile&& meanwhile) {
-    constexpr float kShift = BF16 ? 0.f : 7.f, kTiny = BF16 ? 8.67361738e-19f : 5.96046448e-8f;  // 2^-60, 2^-24
+    constexpr float kShift = BF16 ? 0.f : 7.f;
     constexpr int kStep = Shape<DP>::kStep, KB = kStep / 16, kBlock = 16 * CH * 16;  // blocks of 16 keys, bytes of one
     constexpr uint32_t kAll = 0xffffffffu >> (32 - kStep);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mi = lane >> 3, mr = lane & 7;
@@ -345,10 +372,10 @@ struct Rows {
           for (int e = 0; e < 4; ++e) o[n][c][e] *= fo[e & 1];
       }
     }
-    // P^T as the 8-wide operand (keys 2t, 2t+1 of each 8, row g): the value cut off to 16 bits, and what
-    // that leaves out, which is positive wherever the value is: against an infinite state both parts
-    // give the same infinity.  In f16 P is 2^7 times itself, so that the smallest low part, 2^-24, is 2^-31 of it.
+    // P^T as the 8-wide operand (keys 2t, 2t+1 of each 8, row g) in two 16-bit parts: cut off, and what that leaves
+    // out, rounded.  In f16 P is 2^7 times itself: the parts are multiples of 2^-24, 2^-31 of P's unit.
     uint32_t pb[NT][2 * KB], pl[NT][2 * KB];
+    uint32_t above = 0u;                    // CAREFUL: which of this lane's P's are not zero
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -358,17 +385,16 @@ struct Rows {
         for (int h = 0; h < 2; ++h) {
           pr[h] = fast_exp2(s[kh / 2][n][2 * (kh & 1) + h] - ref[n][h]);
           l[n][h] += pr[h];
+          if (CAREFUL && pr[h] != 0.f) above |= 1u << ((n * 2 * KB + kh) * 2 + h);
         }
         const uint32_t high = pack2_down<BF16>(pr[0], pr[1]);
         const float2 f = unpack2<BF16>(high);
         pb[n][kh] = transpose8(high);
-        pl[n][kh] = transpose8(pack2<BF16>(fmaxf(pr[0] - f.x, fminf(pr[0], kTiny)), fmaxf(pr[1] - f.y, fminf(pr[1], kTiny))));
+        pl[n][kh] = transpose8(pack2<BF16>(pr[0] - f.x, pr[1] - f.y));
       }
     bool apart = false;
-    if (mixed) {
-      // A state that some rows do not see may hold infinities or NaN, which zero probabilities would
-      // let through: such a slice goes token by token.
-      bool odd = false;
+    if (CAREFUL) {
+      uint32_t odd = 0u;
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         if (!inside(c)) break;
@@ -377,10 +403,10 @@ struct Rows {
           uint32_t r[4];
           ldmatrix4_trans((v_at + k * kBlock) ^ (c * 32), r);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd = odd || not_finite2<BF16>(r[e]);
+          for (int e = 0; e < 4; ++e) odd |= not_finite2<BF16>(r[e]);
         }
       }
-      apart = __any_sync(0xffffffffu, odd);
+      apart = __any_sync(0xffffffffu, odd != 0u);
     }
     if (!apart) {
 #pragma unroll
@@ -398,6 +424,14 @@ struct Rows {
       }
       return;
     }
+    uint32_t one[NT][2 * KB];               // 1 where P is not zero, as the operand
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int kh = 0; kh < 2 * KB; ++kh) {
+        const uint32_t two = above >> ((n * 2 * KB + kh) * 2), kOne = BF16 ? 0x3f80u : 0x3c00u;
+        one[n][kh] = transpose8((two & 1u ? kOne : 0u) | (two & 2u ? kOne << 16 : 0u));
+      }
 #pragma unroll 1
     for (int32_t at = view.first_pos; at <= view.last_pos; ++at) {
       uint32_t keep[2 * KB];                // keys 2t, 2t+1 of each 8 that position `at` sees
@@ -420,11 +454,18 @@ struct Rows {
           ldmatrix4_trans((v_at + k * kBlock) ^ (c * 32), r);
 #pragma unroll
           for (int e = 0; e < 4; ++e) r[e] &= keep[2 * k + (e >> 1)];
+          uint32_t odd[4];                  // what is not finite, taken out of r
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            odd[e] = r[e] & not_finite2<BF16>(r[e]);
+            r[e] ^= odd[e];
+          }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float x[4] = {0.f, 0.f, 0.f, 0.f};
             mma16816<BF16>(x, r[0], r[1], r[2], r[3], pb[n][2 * k], pb[n][2 * k + 1]);
             mma16816<BF16>(x, r[0], r[1], r[2], r[3], pl[n][2 * k], pl[n][2 * k + 1]);
+            mma16816<BF16>(x, odd[0], odd[1], odd[2], odd[3], one[n][2 * k], one[n][2 * k + 1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (pos[n][e & 1] == at) o[n][c][e] += x[e];
@@ -462,10 +503,11 @@ __device__ __forceinline__ void add_weighted(float4& acc, const float4& v, float
 
 constexpr int kMostWarps = 8, kMostRanks = 8;
 
-// NT: tiles of 8 query rows.  One to eight warps a CTA, one to eight CTAs an item: the item's warps take
+// NT: tiles of 8 query rows.  Two CTAs an SM of 8 rows, which short sequences' rings leave room for; with 16 rows
+// their registers would not do.  One to eight warps a CTA, one to eight CTAs an item: the item's warps take
 // its slices in turn, so that the first look-up needs no length.
 template <int DP, bool FULL, bool BF16, int NT>
-__global__ void __launch_bounds__(kMostWarps * 32)
+__global__ void __launch_bounds__(kMostWarps * 32, NT == 1 ? 2 : 1)
 paged_joined_kernel(const PagedParams p) {
   namespace cg = cooperative_groups;
   using L = Shape<DP>;
@@ -516,12 +558,23 @@ paged_joined_kernel(const PagedParams p) {
   const int32_t row0 = rt * kTile;
   const int32_t n_rows = min(p.rows - row0, kTile);
   Rows<DP, FULL, BF16, NT> rows;
-  rows.enter(p, view, b, grp, row0);
-  for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    // the slice before this one has been read by every lane: its place is filled again
-    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(first + i * stride) * L::kStep, seen_s[warp][at], issue);
+  auto slices = [&](auto careful) {
+    rows.enter(p, view, b, grp, row0);
+    for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
+      cp_async_wait<NS - 2>();
+      __syncwarp();
+      // the slice before this one has been read by every lane: its place is filled again
+      rows.template step<careful>(p, view, ring + at * 2 * L::kSliceBytes, view.slice(first + i * stride) * L::kStep,
+                                  seen_s[warp][at], issue);
+    }
+  };
+  slices(std::false_type{});
+  if (__any_sync(0xffffffffu, rows.any_nan(view))) {
+    feed.restart();
+    feed.look_up(view, first, next_page, next_row);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) issue();
+    slices(std::true_type{});
   }
   cp_async_wait<0>();
   __syncthreads();  // every ring is at rest: the space takes the warps' sums
@@ -655,14 +708,12 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   struct Cursor {
     int32_t b, grp, slice, n;
   };
-  Cursor out;
-  out.b = lo;
-  out.n = before[lo + 1] - before[lo];
+  Cursor begin;
+  begin.b = lo;
+  begin.n = before[lo + 1] - before[lo];
   const int32_t rest = f0 - before[lo] * p.groups;
-  out.grp = rest / out.n;
-  out.slice = rest - out.grp * out.n;
-  Cursor in = out;
-  View view = tile_view<kTile, L::kStep>(p, in.b, 0), view_in = view;
+  begin.grp = rest / begin.n;
+  begin.slice = rest - begin.grp * begin.n;
   // To the next slice; true where that is another item's.
   auto advance = [&](Cursor& c, View& v) {
     if (++c.slice < c.n) return false;
@@ -679,56 +730,68 @@ paged_parts_kernel(const PagedParams p, const Parts parts) {
   };
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * L::kSliceBytes;
   Feed<DP, FULL, NS> feed(p, ring, NS, seen_s[warp]);
-  feed.enter(in.b, in.grp);
-  int32_t next_page = -1;
-  uint32_t next_row = 0;
-  auto issue = [&]() {
-    if (feed.issued < mine) {
-      const int32_t page = next_page;
-      const uint32_t row = next_row;
-      const uint8_t *k = feed.k, *v = feed.v;
-      if (feed.issued + 1 < mine) {
-        if (advance(in, view_in)) feed.enter(in.b, in.grp);
-        feed.look_up(view_in, in.slice, next_page, next_row);
-      }
-      feed.copy(page, row, k, v);
-    }
-    feed.commit();
-  };
-  feed.look_up(view_in, in.slice, next_page, next_row);
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i) issue();
-  Rows<DP, FULL, BF16, NT> rows;
-  rows.enter(p, view, out.b, out.grp, 0);
   const int g = lane >> 2, t = lane & 3;
-  for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    rows.step(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * L::kStep, seen_s[warp][at], issue);
-    if (i + 1 < mine && out.slice + 1 < out.n) {
-      ++out.slice;
-      continue;
-    }
-    const int64_t slot = static_cast<int64_t>(me) + out.b * p.groups + out.grp;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 8 * n + 2 * t + h;
-        const float part = keys_sum(rows.l[n][h]);
-        if (r >= p.rows) continue;
-        if (g == 0) parts.ml[slot * kTile + r] = make_float2(rows.m[n][h], part);
-        float* dst = parts.o + (slot * kTile + r) * p.head_dim;
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
-          if (c * 16 + g < p.head_dim) dst[c * 16 + g] = rows.o[n][c][h];
-          if (c * 16 + 8 + g < p.head_dim) dst[c * 16 + 8 + g] = rows.o[n][c][2 + h];
+  auto slices = [&](auto careful) {         // true: there is NaN in a part
+    Cursor out = begin, in = begin;
+    View view = tile_view<kTile, L::kStep>(p, in.b, 0), view_in = view;
+    feed.enter(in.b, in.grp);
+    int32_t next_page = -1;
+    uint32_t next_row = 0;
+    auto issue = [&]() {
+      if (feed.issued < mine) {
+        const int32_t page = next_page;
+        const uint32_t row = next_row;
+        const uint8_t *k = feed.k, *v = feed.v;
+        if (feed.issued + 1 < mine) {
+          if (advance(in, view_in)) feed.enter(in.b, in.grp);
+          feed.look_up(view_in, in.slice, next_page, next_row);
         }
+        feed.copy(page, row, k, v);
       }
-    if (i + 1 < mine) {
-      advance(out, view);
-      rows.enter(p, view, out.b, out.grp, 0);
+      feed.commit();
+    };
+    feed.look_up(view_in, in.slice, next_page, next_row);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) issue();
+    Rows<DP, FULL, BF16, NT> rows;
+    rows.enter(p, view, out.b, out.grp, 0);
+    bool nan = false;
+    for (int32_t i = 0, at = 0; i < mine; ++i, at = at + 1 == NS ? 0 : at + 1) {
+      cp_async_wait<NS - 2>();
+      __syncwarp();
+      rows.template step<careful>(p, view, ring + at * 2 * L::kSliceBytes, view.slice(out.slice) * L::kStep, seen_s[warp][at],
+                                  issue);
+      if (i + 1 < mine && out.slice + 1 < out.n) {
+        ++out.slice;
+        continue;
+      }
+      nan = nan || rows.any_nan(view);
+      const int64_t slot = static_cast<int64_t>(me) + out.b * p.groups + out.grp;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 8 * n + 2 * t + h;
+          const float part = keys_sum(rows.l[n][h]);
+          if (r >= p.rows) continue;
+          if (g == 0) parts.ml[slot * kTile + r] = make_float2(rows.m[n][h], part);
+          float* dst = parts.o + (slot * kTile + r) * p.head_dim;
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            if (c * 16 + g < p.head_dim) dst[c * 16 + g] = rows.o[n][c][h];
+            if (c * 16 + 8 + g < p.head_dim) dst[c * 16 + 8 + g] = rows.o[n][c][2 + h];
+          }
+        }
+      if (i + 1 < mine) {
+        advance(out, view);
+        rows.enter(p, view, out.b, out.grp, 0);
+      }
     }
+    return __any_sync(0xffffffffu, nan);
+  };
+  if (slices(std::false_type{})) {          // all of the warp's parts once more
+    feed.restart();
+    slices(std::true_type{});
   }
   cp_async_wait<0>();
 }

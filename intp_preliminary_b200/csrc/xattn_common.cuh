@@ -69,11 +69,11 @@ __device__ __forceinline__ uint32_t finite2(uint32_t v) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Whether one of the two values is an infinity or NaN.
+// All bits of those of the two values that are infinities or NaN.
 template <bool BF16>
-__device__ __forceinline__ bool not_finite2(uint32_t v) {
+__device__ __forceinline__ uint32_t not_finite2(uint32_t v) {
   constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-  return (v & kExp) == kExp || (v >> 16 & kExp) == kExp;
+  return ((v & kExp) == kExp ? 0xffffu : 0u) | ((v >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
 }
 
 // 32 bytes of one thread, a whole memory sector (dst 32-byte aligned).

@@ -10,9 +10,11 @@ Where a kernel may round, with u the unit roundoff of the output type (half its 
         products and a sum: 2 * 2^-24 more.  The result is rounded once: u |y| (f16: at most 2^-25
         below its normal range).
   attention: the bound of a kernel that multiplies each probability as two 16-bit numbers, as
-        oracle.cross_attention's ``two_part`` derives it, but for the two parts: the first is cut off
-        (less than eps = 2 u of the probability is left), the second rounded (u of that): 2 u^2.  Its
-        smallest value is 2^-60 of a probability's unit (f16: 2^-31), which is below what f16 loses.
+        oracle.cross_attention's ``two_part`` derives it, but for the two parts: the first leaves less than
+        (eps + 2^-22) of the probability, eps = 2 u, the second is that rounded: 2 u^2 (and 2^-22 u, within the
+        sum's other terms).  A probability's unit is that of the row's reference, which is at most the largest.  In
+        f16 the parts are multiples of 2^-31 of it and their sum off by 2^-32 at most, whatever the probability.
+        The result is rounded once (f16: 2^-25 at least).
 """
 
 from __future__ import annotations
@@ -98,5 +100,5 @@ def attend(q, keys, values, *, page_table, start, scale, counts=None, window=Non
                 w = p * (score + rel)
                 bound[b, h, m] = w @ vv.abs() + w.sum() * (p @ vv.abs()) + u * out[b, h, m].abs()
                 if dtype == torch.float16:
-                    bound[b, h, m] += 2.0 ** -25 * (1 + p.max() * vv.abs().sum(0))
+                    bound[b, h, m] += 2.0 ** -25 + 2.0 ** -32 * p.max() * vv.abs().sum(0)
     return out, bound

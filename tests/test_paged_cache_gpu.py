@@ -672,3 +672,53 @@ def test_a_long_window_of_far_rows(cuda_device, start, queries, sinks, kernel):
     got = _check(cuda_device, q, keys, values, table, [start, 1990], kernel=kernel, scale=0.25, window=2**30, sinks=sinks)
     if start > 2**30 + 2000 and sinks == 0:
         assert bool((got[0] == 0).all())
+
+
+# ------------------------------------------------------------------ small probabilities
+def _steps(dtype, dim, states, scores, seed):
+    """One sequence whose state j has the score scores.get(j, 0) for every query, and its queries."""
+    keys, values, table = _filled(1, 1, states, dim, 16, dtype, seed)
+    for j in range(states):
+        page, row = oracle.place(table, 16, keys.shape[0], 0, j)
+        keys[page, 0, row] = 0
+        keys[page, 0, row, 0] = scores.get(j, 0.0)
+    return keys, values, table
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [8, 32, 64, 72, 128])
+@pytest.mark.parametrize("heads,queries", [(1, 1), (2, 3), (5, 3)])
+@pytest.mark.parametrize("gap", [5.0, 18.0, 25.0, 40.0, 60.0, 86.0])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_an_infinite_state_shows_however_small_its_probability(cuda_device, dtype, dim, heads, queries, gap, kernel):
+    """Before and behind the state of the largest score; 86 below it is 2^-124, which 32 bits hold."""
+    states, column = 300, dim - 3
+    q = torch.zeros(1, heads, queries, dim).to(dtype)
+    q[..., 0] = 1
+    for top, at, bad in ((150, 7, INF), (150, 290, -INF), (40, 44, INF), (150, 288, NAN)):
+        keys, values, table = _steps(dtype, dim, states, {top: gap}, 240)
+        page, row = oracle.place(table, 16, keys.shape[0], 0, at)
+        values[page, 0, row, column] = bad
+        got = _check(cuda_device, q, keys, values, table, [states - queries], kernel=kernel, scale=1.0)
+        shown = got[..., column]
+        assert bool((torch.isnan(shown) if bad != bad else shown == bad).all())
+        assert bool(torch.isfinite(got[..., torch.arange(dim) != column]).all())
+
+
+@pytest.mark.parametrize("dtype,gap,size", [(BF16, 30.0, 1.0), (BF16, 45.0, 2.0**60), (BF16, 60.0, 2.0**90), (BF16, 75.0, 2.0**100),
+                                            (F16, 10.0, 1.0), (F16, 14.0, 1000.0), (F16, 15.0, 20000.0), (F16, 16.0, 20000.0),
+                                            (F16, 17.0, 20000.0), (F16, 20.0, 30000.0)])
+@pytest.mark.parametrize("dim", [32, 64, 80, 128])
+@pytest.mark.parametrize("heads,queries", [(1, 1), (3, 4)])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_small_probabilities_count_once(cuda_device, dtype, gap, size, dim, heads, queries, kernel):
+    """One state takes nearly all of the weight and holds zeros: the result is what the others add to it."""
+    states, top = 300, 150
+    q = torch.zeros(1, heads, queries, dim).to(dtype)
+    q[..., 0] = 1
+    keys, values, table = _steps(dtype, dim, states, {top: gap}, 250)
+    values = ((values.float().abs() + 0.5).clamp(max=1.9) * size).to(dtype)  # of one sign: errors of one sign add up
+    page, row = oracle.place(table, 16, keys.shape[0], 0, top)
+    values[page, 0, row] = 0
+    got = _check(cuda_device, q, keys, values, table, [states - queries], kernel=kernel, scale=1.0)
+    assert bool((got > 0).all())

@@ -462,13 +462,13 @@ struct Rows {
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            float x[4] = {o[n][c][0], o[n][c][1], o[n][c][2], o[n][c][3]};  // the sums' order is the first pass's
             mma16816<BF16>(x, r[0], r[1], r[2], r[3], pb[n][2 * k], pb[n][2 * k + 1]);
             mma16816<BF16>(x, r[0], r[1], r[2], r[3], pl[n][2 * k], pl[n][2 * k + 1]);
             mma16816<BF16>(x, odd[0], odd[1], odd[2], odd[3], one[n][2 * k], one[n][2 * k + 1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (pos[n][e & 1] == at) o[n][c][e] += x[e];
+              if (pos[n][e & 1] == at) o[n][c][e] = x[e];
           }
         }
       }

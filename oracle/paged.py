@@ -78,13 +78,14 @@ def attend(q, keys, values, *, page_table, start, scale, counts=None, window=Non
     for b in range(batch):
         for m in range(rows if counts is None else min(max(int(counts[b]), 0), rows)):
             at = int(start[b]) + m
-            last = min(at, page_table.shape[1] * keys.shape[2] - 1)
-            states = [j for j in range(last + 1) if window is None or j > at - window or j < sinks]
-            found = [place(page_table, keys.shape[2], keys.shape[0], b, j) for j in states]
-            found = [f for f in found if f is not None]
-            if not found:
+            states = torch.arange(min(at + 1, page_table.shape[1] * keys.shape[2]) if at >= 0 else 0)
+            if window is not None:
+                states = states[(states > at - window) | (states < sinks)]
+            pages = page_table[b, states // keys.shape[2]].long()
+            there = (pages >= 0) & (pages < keys.shape[0])
+            pages, slots = pages[there], (states % keys.shape[2])[there]
+            if not len(pages):
                 continue
-            pages, slots = (torch.tensor(x) for x in zip(*found))
             for h in range(heads):
                 g = h // (heads // groups)
                 kk, vv = keys[pages, g, slots], values[pages, g, slots]
@@ -96,7 +97,7 @@ def attend(q, keys, values, *, page_table, start, scale, counts=None, window=Non
                 # a score of -inf is exact: its probability is zero
                 size = torch.where(s == -float("inf"), torch.zeros_like(s), scale * (kk.abs() @ q[b, h, m].abs()))
                 score = 2.0 ** -23 * ((dim + 8) * size + 4 * s[s != -float("inf")].abs().max())
-                rel = 2 * u ** 2 + 2.0 ** -22 * (1 + 64 + len(found) / 16)
+                rel = 2 * u ** 2 + 2.0 ** -22 * (1 + 64 + len(pages) / 16)
                 w = p * (score + rel)
                 bound[b, h, m] = w @ vv.abs() + w.sum() * (p @ vv.abs()) + u * out[b, h, m].abs()
                 if dtype == torch.float16:

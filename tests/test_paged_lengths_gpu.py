@@ -53,6 +53,82 @@ def _check(device, q, keys, values, table, start, kernels=KERNELS, **more):
         assert bool((error <= bound).all()), f"{kernel}: {float((error / bound).nan_to_num(INF).max())} times the bound"
 
 
+def _slices(lengths, groups, dim):
+    return groups * sum(-(-n // (32 if dim <= 64 else 16)) for n in lengths)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("batch,groups,per_group,queries,dim,longest", [
+    (32, 4, 2, 1, 128, 2500),      # 128 items of 8 rows at most at head_dim 128
+    (43, 3, 2, 3, 128, 1900),
+    (8, 4, 4, 2, 128, 5800),       # 8 rows, fewer items
+    (8, 4, 4, 4, 128, 5800),       # 16 rows
+    (8, 4, 4, 2, 80, 5800),
+    (8, 4, 3, 5, 80, 5800),
+    (8, 4, 1, 7, 72, 5800),
+    (8, 4, 4, 2, 64, 11600),
+    (15, 4, 4, 4, 64, 7000),       # parts of a row joined by four warps
+    (8, 4, 2, 3, 32, 19000),
+    (8, 4, 8, 2, 24, 19000),
+])
+def test_shares_of_many_slices(cuda_device, dtype, batch, groups, per_group, queries, dim, longest):
+    """Every warp has more slices than its ring holds, and the parts' slices run across items."""
+    g = torch.Generator().manual_seed(300)
+    lengths = (longest - torch.randint(0, longest // 8, (batch,), generator=g)).tolist()
+    lengths[1] = 0
+    depth = 6 if dim <= 32 else 3
+    assert _slices(lengths, groups, dim) >= (depth + 2) * MOST_WARPS
+    warps = min(64, 2 * MOST_WARPS // (batch * groups))            # that an item may get of the other kernel
+    assert min(n for n in lengths if n) // (32 if dim <= 64 else 16) > depth * warps
+    keys, values, table = _dealt(lengths, groups, dim, 24, dtype, 301)
+    q = _rand((batch, groups * per_group, queries, dim), dtype, 304)
+    start = [n - queries for n in lengths]
+    counts = [queries] * batch
+    counts[2] -= 1
+    _check(cuda_device, q, keys, values, table, start, scale=dim ** -0.5, counts=counts)
+    _check(cuda_device, q, keys, values, table, start, scale=dim ** -0.5, window=longest // 2, sinks=5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim,states", [(128, 20000), (64, 40000)])
+def test_a_row_of_more_parts_than_one_pass_joins(cuda_device, dtype, dim, states):
+    assert _slices([states], 1, dim) > 1024                       # two slices a warp: more than 512 parts
+    keys, values, table = _dealt([states], 1, dim, 64, dtype, 310)
+    _check(cuda_device, _rand((1, 4, 1, dim), dtype, 313), keys, values, table, [states - 1], scale=dim ** -0.5)
+
+
+@pytest.mark.parametrize("batch,groups,dim,states,parts", [
+    (1, 1, 128, 20000, False), (1, 1, 128, 30000, True),          # a warp's slices while most warps are idle
+    (100, 6, 72, 1900, False), (100, 6, 72, 2100, True),          # and while all are at work
+])
+def test_the_choice_between_the_kernels(cuda_device, batch, groups, dim, states, parts):
+    g = torch.Generator(device=cuda_device).manual_seed(320)
+    width = -(-states // 16)
+    pages = batch * width
+    table = torch.randperm(pages, generator=g, device=cuda_device).reshape(batch, width).to(torch.int32)
+    cache = PagedCache(*(torch.randn(pages, groups, 16, dim, generator=g, device=cuda_device, dtype=BF16) for _ in range(2)))
+    q = torch.randn(batch, 2 * groups, 1, dim, generator=g, device=cuda_device, dtype=BF16)
+    start = torch.randint(0, states, (batch,), generator=g, device=cuda_device, dtype=torch.int32)
+    assert (_attention_plan(q, cache, table, 0.1, None, 0, "auto", None)[1] > 0) == parts
+    more = dict(page_table=table, start=start, scale=dim ** -0.5)
+    auto, forced = (paged_attention(q, cache, kernel=k, **more) for k in ("auto", KERNELS[parts]))
+    assert torch.equal(auto, forced)
+    other = paged_attention(q, cache, kernel=KERNELS[not parts], **more)
+    # the same 64-bit result, rounded once by each
+    assert bool(((auto.float() - other.float()).abs() <= 2.0 ** -7 * auto.float().abs() + 1e-4).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [56, 64, 80, 104, 128])
+@pytest.mark.parametrize("heads,groups,queries", [(4, 4, 2), (4, 2, 4), (6, 2, 5), (8, 1, 2), (12, 4, 17)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (7, 3), (40, 20), (16, 100)])
+def test_tokens_see_what_is_before_them(cuda_device, dtype, dim, heads, groups, queries, window, sinks):
+    keys, values, table = _dealt([90, queries, 61], groups, dim, 7, dtype, 330)
+    q = _rand((3, heads, queries, dim), dtype, 333)
+    _check(cuda_device, q, keys, values, table, [90 - queries, 0, 61 - queries - 2], scale=dim ** -0.5, window=window,
+           sinks=sinks, kernels=KERNELS if queries * heads // groups <= 16 else ["joined"])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("dim", [24, 64, 72, 80, 128])
 @pytest.mark.parametrize("bad", [NAN, INF, -INF])

@@ -919,9 +919,13 @@ Plan plan(const paged_attention_args* a) {
   const int64_t slices = most_slices(a, a->queries);
   // A second launch costs 3 to 4 us; what it saves are warps that wait for others.  Equal parts are taken
   // where a warp would have more than 125 slices, or 24 while less than half of the warps are at work.
-  // One launch / parts, D128: B32 G8 of 4000 states (63 slices a warp) 66 / 71 us, of 8000 (125) 127 / 131,
-  // B64 G8 of 8192 (256) 251 / 241, of 4096 with D80 (128) 104 / 90; B1 G8 of 16000 (16, 512 warps)
-  // 15.6 / 17.1, of 32000 (31) 24.7 / 24.0, of 131071 109 / 90.
+  // One launch / parts, us, G8, lengths from half of the given one up to it (all of it):
+  //   D128 B32: 6000 states (94 slices a warp) 101 / 102 (115 / 124), 8000 (125) 126 / 126 (151 / 163), 8192 130 / 128,
+  //   10000 (156) 162 / 159, 14000 (219) 220 / 210 (260 / 277); B64 of two warps an item: 4000 (125) 126 / 127, 5000 (156)
+  //   157 / 159, 6000 (188) 193 / 185, 8192 (256) 250 / 239 (309 / 320).  D64 B64: 8000 (125) 124 / 127, 12000 (188) 192 / 188.
+  //   D80 B64, where columns are checked: 3000 (94) 79 / 71 (88 / 89), 6000 (188) 153 / 124 (160 / 163).
+  // Lengths that are equal would do better in one launch by 3 to 8 %, but the host does not know them.
+  // One sequence, D128: 16000 (16, 512 warps) 15.6 / 17.1, 32000 (31) 24.7 / 24.0, 131071 109 / 90.
   const Team t = team(items, slices);
   const int64_t each = (slices + t.warps * t.ranks - 1) / (t.warps * t.ranks);
   const bool better = each > 125 || (each >= 24 && items * t.warps * t.ranks * 2 < kPartsAll);
@@ -930,9 +934,10 @@ Plan plan(const paged_attention_args* a) {
   x.parts = able && (a->kernel == PAGED_KERNEL_PARTS || (a->kernel == PAGED_KERNEL_AUTO && better));
   if (x.parts) {
     // Three CTAs an SM want a tile of 8 rows (16 do not fit their registers), and pay where the parts are long
-    // and of many items: B64 G8 D128 over 4096 to 8192 states 233 us instead of 243; B1 G8 of 32000 26.4
-    // instead of 23.9; B64 G8 D80 of 4096 90.6 instead of 89.2.
-    x.three = rows <= 8 && a->head_dim == 128 && items >= 128;
+    // and of many items.  Two / three, us, D128 and G8: 8 items of 32000 states 30.1 / 32.9, of 131071 89 / 93; 16 of 65000
+    // 84.5 / 84.0; 32 of 32000 68.2 / 67.4; 64 of 32000 123 / 120; 128 of 16000 136 / 132; 512 of 8192 245 / 235.  D80, whose
+    // columns are checked: 512 of 4096 89.2 / 90.6.
+    x.three = rows <= 8 && a->head_dim == 128 && items >= 32;
     const int64_t slots = ((x.three ? kThreeCtas * kPartsWarps : kPartsAll) + items) * tile_rows(rows);
     x.o_bytes = align256(slots * a->head_dim * 4);
     x.ml_bytes = align256(slots * 8);

@@ -59,9 +59,10 @@ def _slices(lengths, groups, dim):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("batch,groups,per_group,queries,dim,longest", [
-    (32, 4, 2, 1, 128, 2500),      # 128 items of 8 rows at most at head_dim 128
+    (32, 4, 2, 1, 128, 2500),      # many items of 8 rows at most at head_dim 128
     (43, 3, 2, 3, 128, 1900),
-    (8, 4, 4, 2, 128, 5800),       # 8 rows, fewer items
+    (8, 4, 4, 2, 128, 5800),
+    (4, 4, 4, 2, 128, 15000),      # few of them
     (8, 4, 4, 4, 128, 5800),       # 16 rows
     (8, 4, 4, 2, 80, 5800),
     (8, 4, 3, 5, 80, 5800),

@@ -71,24 +71,26 @@ class RotaryAxes:
         tables = bytearray(struct.pack(f"{pairs}d{pairs}i", *(f / (2 * math.pi) for f in self._frequencies), *self._axes))
         self._tables = torch.frombuffer(tables, dtype=torch.uint8).to(self._device)
         self._device = self._tables.device
+        self._index, self._turn_bytes = self._device.index, 8 * pairs
         # streams that the tables' memory is held for: the one it was allocated on
-        self._streams = {_current_stream(self._device.index)} if self._tables.is_cuda else set()
+        self._streams = {_current_stream(self._index)} if self._tables.is_cuda else set()
         # what a call's checks and argument block depend on
         self._layout = (pairs, max(self._axes) + 1, self._interleaved, self._device)
 
     @property
     def _pointers(self) -> tuple[int, int]:
         at = self._tables.data_ptr()
-        return at, at + 8 * len(self._axes)
+        return at, at + self._turn_bytes
 
     def _launch_pointers(self) -> tuple[int, int]:
         """The tables' addresses for a launch on the device's current stream: should the object go while
         the launch is pending, its memory waits for that stream."""
-        stream = _current_stream(self._device.index)
+        stream = _current_stream(self._index)
         if stream not in self._streams:
             self._tables.record_stream(torch.cuda.current_stream(self._device))
             self._streams.add(stream)
-        return self._pointers
+        at = self._tables.data_ptr()
+        return at, at + self._turn_bytes
 
     # A copy, and what is unpickled, lays out tables of its own from the numbers.
     def __getstate__(self) -> dict:

@@ -14,8 +14,11 @@ A step appends its keys and values there and attends from there:
     q = cache.append(k, v, page_table=table, start=length, rotary=rotary, q=q)
     out = paged_attention(q, cache, page_table=table, start=length, scale=scale)
 
-The operators take no part in autograd.  Every call runs one CUDA kernel of
-``libintp_b200.so`` on the current stream; CPU tensors raise ``ValueError``.
+The operators take no part in autograd.  An append is one CUDA kernel of
+``libintp_b200.so``, an attention one or two (see ``paged_attention``), on the
+current stream; inputs that are not laid out for them are copied first, and int64
+``start``, ``counts`` and ``page_table`` converted to 32 bits (values past those
+become the nearest) in every call.  CPU tensors raise ``ValueError``.
 """
 
 from __future__ import annotations

@@ -14,8 +14,9 @@ height and width, the coordinates of a patch on the hex lattice.
 The operator is differentiable in q and k, any number of times (a gradient is
 turned back by the same angles); results repeat bit for bit.  Forward-mode
 tangents and ``torch.jit.trace`` are refused.  Every call runs one CUDA kernel of
-``libintp_b200.so`` on the current stream of the inputs' device; there is no CPU
-path, CPU tensors raise ``ValueError``.
+``libintp_b200.so`` on the current stream of the inputs' device, behind a copy of
+each input whose rows are not laid out for it; there is no CPU path, CPU tensors
+raise ``ValueError``.
 """
 
 from __future__ import annotations
@@ -46,7 +47,9 @@ class RotaryAxes:
     """The turning of a head's pairs: ``frequencies[i]`` radians for each step along
     axis ``axes[i]``, of as many pairs as there are entries, a multiple of 4 up to 64.
     The axes are numbered from 0 without gaps; ``interleaved`` pairs neighbouring
-    columns.  The object holds its tables on ``device`` and does not change."""
+    columns.  The object holds its tables on ``device`` and does not change; a copy, or one that
+    is unpickled, has tables of its own.  A CUDA graph that was captured with it reads them:
+    keep it as long."""
 
     def __init__(self, frequencies, axes, *, interleaved: bool = False, device) -> None:
         frequencies, axes = [float(f) for f in frequencies], [int(a) for a in axes]
@@ -248,7 +251,8 @@ def _rotate(q, k, rotary, positions, inverse: bool):
 
 
 class _RotatePositions(torch.autograd.Function):
-    """Linear in q and k: the gradient is turned back by the same angles."""
+    """Linear in q and k: the gradient is turned back by the same angles.  A result whose input
+    needs no gradient needs none."""
 
     @staticmethod
     def forward(ctx, q, k, rotary, positions, inverse):

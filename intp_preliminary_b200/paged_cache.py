@@ -76,9 +76,10 @@ class PagedCache:
         # what calls know the pool by
         self._layout = (keys.shape, keys.stride(), keys.dtype, keys.device)
 
-    def __reduce__(self):
+    def __setstate__(self, state: dict) -> None:
         """A copy, and what is loaded from a file, is checked again: its tensors may lie elsewhere."""
-        return type(self), (self._keys, self._values)
+        self.__dict__.update(state)
+        PagedCache.__init__(self, self._keys, self._values)
 
     # read only: a call takes the layout that was checked above
     keys = property(lambda self: self._keys)

@@ -70,9 +70,10 @@ class StateCache:
         self._keys, self._values = keys, values
         self._key_exponents, self._value_exponents = key_exponents, value_exponents
 
-    def __reduce__(self):
+    def __setstate__(self, state: dict) -> None:
         """A copy, and what is loaded from a file, is checked again: its tensors may lie elsewhere."""
-        return type(self), (self._keys, self._key_exponents, self._values, self._value_exponents)
+        self.__dict__.update(state)
+        StateCache.__init__(self, self._keys, self._key_exponents, self._values, self._value_exponents)
 
     # read only: a call takes the layout that was checked above
     keys = property(lambda self: self._keys)

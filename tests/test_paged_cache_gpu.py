@@ -722,3 +722,19 @@ def test_small_probabilities_count_once(cuda_device, dtype, gap, size, dim, head
     values[page, 0, row] = 0
     got = _check(cuda_device, q, keys, values, table, [states - queries], kernel=kernel, scale=1.0)
     assert bool((got > 0).all())
+
+
+class NamedPool(PagedCache):
+    def __init__(self, name, pages):
+        super().__init__(*(torch.zeros(pages, 1, 8, 16, dtype=BF16, device="cuda") for _ in range(2)))
+        self.name = name
+
+
+def test_copies_of_a_subclass_keep_what_it_holds(cuda_device):
+    import copy
+    import pickle
+
+    pool = NamedPool("first", 3)
+    for other in (copy.copy(pool), copy.deepcopy(pool), pickle.loads(pickle.dumps(pool))):
+        assert type(other) is NamedPool and other.name == "first" and other.layout == pool.layout
+    assert copy.copy(pool).keys is pool.keys and copy.deepcopy(pool).keys is not pool.keys
